@@ -49,7 +49,8 @@ typedef enum {
     MOE_EUNSUPPORTED = -5  /* valid in the reference, not implemented here */
 } moe_status;
 
-typedef enum { MOE_F32 = 0, MOE_BF16 = 1, MOE_FP8_E4M3 = 2 } moe_dtype;
+/* MOE_INT8: codes of moe_int8_matmul_async only, not a layer's weight type. */
+typedef enum { MOE_F32 = 0, MOE_BF16 = 1, MOE_FP8_E4M3 = 2, MOE_INT8 = 3 } moe_dtype;
 
 /* Memory order of a weight matrix as the reference holds it.
  * FLUX_OUT_IN: Flux Dense weight of size (out, in), column-major, i.e. memory
@@ -383,6 +384,110 @@ int moe_router_lse(moe_handle *h, int32_t T, float *lse);
 
 /* Copy the per-expert counts of the last call to host memory (int32 [E]). */
 int moe_read_counts(moe_handle *h, int32_t *counts);
+
+/* ---- operators on the caller's device tensors (enqueue only) --------------
+ *
+ * No counterpart in the reference, which has neither gradients nor integer
+ * weights and leaves the norms around the MoE FFN to its caller
+ * (src/llama2/inference.jl:61): the products of an expert FFN with their
+ * gradients, int8 products, and the norms and residual around a block, on
+ * tensors that the caller holds in device memory.  They need no handle.
+ *
+ * All run on `stream` (hipStream_t; NULL = the null stream) of the current HIP
+ * device, allocate nothing, keep nothing between calls and can be captured
+ * into a HIP graph.  Distinct calls may run at once on distinct streams; a
+ * workspace belongs to one call at a time (two graphs that may run at once
+ * need one each).  Results depend on the inputs alone, bit for bit, for a
+ * given set of sizes, strides and alignments.  Rows are ld* elements apart (at
+ * least their length); buffers need only the alignment of their elements, but
+ * 16-byte aligned rows are read faster.  On failure moe_last_error(NULL) holds
+ * the message.
+ *
+ * Groups: rows [offsets[e], offsets[e + 1]) of the row tensors belong to group
+ * (expert) e, offsets being groups + 1 non-decreasing int32 in device memory,
+ * as the layer's routing counts them (moe_forward_aux.offsets).  Offsets are
+ * held within [0, rows] by the kernels; with offsets that decrease the results
+ * are undefined.  A group may be empty; rows outside every group are neither
+ * read nor written.  offsets may be NULL with groups = 1: all rows.  rows = 0
+ * is no work.
+ *
+ * Matrices: group e's starts w_stride elements after group e - 1's;
+ * MOE_LAYOUT_LLAMA_IN_OUT: memory [out_dim][in_dim], MOE_LAYOUT_FLUX_OUT_IN:
+ * [in_dim][out_dim], rows ldw apart.  dtype: MOE_F32 or MOE_BF16 operands; sums
+ * in fp32; the result in MOE_F32 or (bf16 operands) MOE_BF16, rounded once. */
+
+/* y[r] = W_e x[r] for the rows r of group e.  x [rows][in_dim], y [rows][out_dim]. */
+int moe_grouped_matmul_async(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t w_stride, int32_t layout,
+                             const int32_t *offsets, int32_t groups, int32_t rows, int32_t in_dim, int32_t out_dim,
+                             int32_t dtype, void *y, int64_t ldy, int32_t y_dtype, void *stream);
+/* Its gradient with respect to x: dx[r] = W_e' dy[r]. */
+int moe_grouped_matmul_grad_x_async(const void *dy, int64_t lddy, const void *w, int64_t ldw, int64_t w_stride,
+                                    int32_t layout, const int32_t *offsets, int32_t groups, int32_t rows,
+                                    int32_t in_dim, int32_t out_dim, int32_t dtype, void *dx, int64_t lddx,
+                                    int32_t dx_dtype, void *stream);
+/* Its gradient with respect to W, in W's layout: dW_e = sum over the rows of
+ * group e of dy[r] x[r]', zeros for an empty group.  accumulate != 0 adds to
+ * what dw holds (in fp32, rounded once) instead.  workspace: 16-byte aligned,
+ * the bytes that moe_grouped_matmul_grad_w_workspace gives for these sizes
+ * (may be 0: NULL is fine then). */
+int moe_grouped_matmul_grad_w_workspace(int32_t groups, int32_t rows, int32_t in_dim, int32_t out_dim,
+                                        int64_t *bytes);
+int moe_grouped_matmul_grad_w_async(const void *x, int64_t ldx, const void *dy, int64_t lddy, int32_t layout,
+                                    const int32_t *offsets, int32_t groups, int32_t rows, int32_t in_dim,
+                                    int32_t out_dim, int32_t dtype, void *dw, int64_t lddw, int64_t dw_stride,
+                                    int32_t dw_dtype, int32_t accumulate, void *workspace, int64_t workspace_bytes,
+                                    void *stream);
+
+/* int8 codes with a scale per row: scale[r] = max|x[r]| / 127, q[r][c] = 127
+ * x[r][c] / max|x[r]| rounded to nearest even.  A row of zeros has scale 0 and
+ * codes 0; one that holds an infinity or a NaN has scale NaN and codes 0.
+ * x [rows][cols] MOE_F32 or MOE_BF16.  Of a weight matrix in
+ * MOE_LAYOUT_LLAMA_IN_OUT this gives a scale per output channel. */
+int moe_quantize_int8_async(const void *x, int64_t ldx, int32_t x_dtype, int64_t rows, int32_t cols, void *q,
+                            int64_t ldq, float *scale, void *stream);
+/* y[r][n] = x_scale[r] w_scale[e][n] sum_k q[r][k] w[e][n][k], summed exactly
+ * in int32 (in_dim <= 131071).  x_dtype MOE_INT8: x holds the codes and
+ * x_scale [rows] their scales.  MOE_BF16 or MOE_F32: the rows are quantised as
+ * moe_quantize_int8_async does, into the workspace (16-byte aligned,
+ * moe_int8_matmul_workspace bytes; not needed for codes), and x_scale is not
+ * read.  w: codes [groups][out_dim][in_dim], w_scale [groups][out_dim]; y
+ * MOE_F32 or MOE_BF16. */
+int moe_int8_matmul_workspace(int32_t rows, int32_t in_dim, int64_t *bytes);
+int moe_int8_matmul_async(const void *x, int64_t ldx, int32_t x_dtype, const float *x_scale, const void *w,
+                          int64_t ldw, int64_t w_stride, const float *w_scale, const int32_t *offsets, int32_t groups,
+                          int32_t rows, int32_t in_dim, int32_t out_dim, void *y, int64_t ldy, int32_t y_dtype,
+                          void *workspace, int64_t workspace_bytes, void *stream);
+
+/* The norms before and after a block, its gate and the residual, in one pass:
+ *   z = y .* rstd(y) .* post_weight     (post_weight NULL: z = y)
+ *   r = alpha x + beta gate .* z        (gate NULL: 1; y NULL: r = alpha x)
+ *   h = r .* rstd(r) .* pre_weight      (pre_weight and h NULL: not computed)
+ * per row of D channels, rstd(v) = 1 / sqrt(mean(v^2) + eps) (llama2's
+ * rmsnorm).  x is the residual stream, y the block's output, r the stream
+ * after it and h the next block's input: a first norm is the call with y NULL,
+ * alpha 1.  x, r [T][D] in x_dtype, y in y_dtype, h in h_dtype, the weights [D]
+ * in w_dtype; gate [ceil(T / gate_rows)][D] in gate_dtype, row t taking gate
+ * row t / gate_rows (gate_rows >= T: one gate for all rows; 1: one per row).
+ * h is the norm of r as it is stored, rounded to x_dtype.  r may be NULL or x
+ * itself; stats [T][2] (rstd(y), rstd(r); 1 where there is no norm) may be
+ * NULL.  Rows are dense; 1 <= D <= 16384. */
+int moe_block_norm_async(const void *x, int32_t x_dtype, const void *y, int32_t y_dtype, const void *post_weight,
+                         const void *pre_weight, int32_t w_dtype, const void *gate, int32_t gate_dtype,
+                         int64_t gate_rows, float alpha, float beta, float eps, int64_t T, int32_t D, void *r, void *h,
+                         int32_t h_dtype, float *stats, void *stream);
+/* Its gradients from dr (x_dtype; NULL: 0) and dh (h_dtype; NULL: 0): dx
+ * (x_dtype), dy (y_dtype), and in fp32 dgate [ceil(T / gate_rows)][D], dpost [D]
+ * and dpre [D]; any may be NULL.  r and stats are the forward call's.  T = 0
+ * gives dpost and dpre of zeros.  workspace: 16-byte aligned, the bytes that
+ * moe_block_norm_grad_workspace gives for these sizes (gate_rows 0: no gate);
+ * not needed without dgate, dpost and dpre. */
+int moe_block_norm_grad_workspace(int64_t T, int32_t D, int64_t gate_rows, int64_t *bytes);
+int moe_block_norm_grad_async(const void *dr, const void *dh, const void *r, int32_t x_dtype, const void *y,
+                              int32_t y_dtype, int32_t h_dtype, const float *stats, const void *post_weight,
+                              const void *pre_weight, int32_t w_dtype, const void *gate, int32_t gate_dtype,
+                              int64_t gate_rows, float alpha, float beta, int64_t T, int32_t D, void *dx, void *dy,
+                              float *dgate, float *dpost, float *dpre, void *workspace, int64_t workspace_bytes,
+                              void *stream);
 
 #ifdef __cplusplus
 }

@@ -166,6 +166,27 @@ class DeviceLayer:
         )
         return out, float(np.float32(loss.value)), self._aux_result(res, keep)
 
+    def forward_device(self, x, training=False, decode=False):
+        """moe_forward_async (or, with ``decode``, moe_decode_async) on a torch
+        tensor x (T, D) in GPU memory, float32 or bfloat16 (decode: float32), on
+        torch's current stream: (out (T, D_out) float32, loss (1,) float32)."""
+        import torch
+
+        T = x.shape[0]
+        out = torch.empty((T, self.output_dim), dtype=torch.float32, device=x.device)
+        loss = torch.zeros(1, dtype=torch.float32, device=x.device)
+        if T == 0:
+            return out, loss
+        L, stream = _lib.lib(), torch.cuda.current_stream(x.device).cuda_stream
+        if decode:
+            st = L.moe_decode_async(self.h, x.data_ptr(), T, out.data_ptr(), stream)
+        else:
+            code = _lib.MOE_BF16 if x.dtype == torch.bfloat16 else _lib.MOE_F32
+            st = L.moe_forward_async(self.h, x.data_ptr(), code, T, int(bool(training)), out.data_ptr(),
+                                     loss.data_ptr(), stream)
+        _lib.check(st, self.h)
+        return out, loss
+
     def _aux(self, T, slots, want_aux):
         aux = _lib.MoeForwardAux()
         res = {}

@@ -2073,3 +2073,5 @@ int moe_read_counts(moe_handle *h, int32_t *counts) {
 }
 
 }  // extern "C"
+
+#include "moe_api_ops.h"

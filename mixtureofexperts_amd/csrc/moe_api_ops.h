@@ -1,0 +1,299 @@
+// moe_api_ops.h -- the C entry points of the operators on a caller's own
+// device tensors: argument checks, then one launcher call.  Included by
+// moe_api.hip only (it uses that file's fail()).
+#pragma once
+#include <mutex>
+
+#include "moe_ops.h"
+
+namespace {
+// compute units of the current device (looked up once per device)
+int op_cus() {
+    static std::mutex mu;
+    static int cus[64] = {};
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+    std::lock_guard<std::mutex> lk(mu);
+    if (!cus[dev]) {
+        int n = 0;
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1) n = 256;
+        cus[dev] = n;
+    }
+    return cus[dev];
+}
+
+int op_fail(const char *fn, const std::string &why) { return fail(nullptr, MOE_EINVAL, std::string(fn) + ": " + why); }
+int op_done(const char *fn, hipError_t e) {
+    if (e == hipSuccess) return MOE_OK;
+    if (e == hipErrorInvalidValue) return op_fail(fn, "too many tiles for one launch");
+    return fail(nullptr, MOE_EHIP, std::string(fn) + ": " + hipGetErrorString(e));
+}
+
+// What the grouped products share: groups, sizes, types, the rows' strides.
+int op_check_groups(const char *fn, const int32_t *offsets, int32_t groups, int32_t rows, int32_t in_dim,
+                    int32_t out_dim) {
+    if (groups < 1) return op_fail(fn, "groups must be positive");
+    if (rows < 0) return op_fail(fn, "rows must not be negative");
+    if (in_dim < 1 || out_dim < 1) return op_fail(fn, "dimensions must be positive");
+    if (!offsets && groups != 1) return op_fail(fn, "offsets are needed for more than one group");
+    return MOE_OK;
+}
+int op_check_dtypes(const char *fn, int32_t dtype, int32_t out_dtype) {
+    if (dtype != MOE_F32 && dtype != MOE_BF16) return op_fail(fn, "dtype must be MOE_F32 or MOE_BF16");
+    if (out_dtype != MOE_F32 && out_dtype != MOE_BF16) return op_fail(fn, "the result must be MOE_F32 or MOE_BF16");
+    if (dtype == MOE_F32 && out_dtype != MOE_F32) return op_fail(fn, "fp32 operands have an fp32 result");
+    return MOE_OK;
+}
+bool op_misaligned(const void *p, int32_t dtype) { return ((uintptr_t)p & (dtype == MOE_F32 ? 3 : 1)) != 0; }
+
+// y[r] = W_e x[r] (grad: dx[r] = W_e^T dy[r]) on rows of k elements -> n
+int op_rows_product(const char *fn, bool grad, const void *x, int64_t ldx, const void *w, int64_t ldw,
+                    int64_t w_stride, int32_t layout, const int32_t *offsets, int32_t groups, int32_t rows,
+                    int32_t in_dim, int32_t out_dim, int32_t dtype, void *y, int64_t ldy, int32_t y_dtype,
+                    void *stream) {
+    int r = op_check_groups(fn, offsets, groups, rows, in_dim, out_dim);
+    if (r == MOE_OK) r = op_check_dtypes(fn, dtype, y_dtype);
+    if (r != MOE_OK) return r;
+    if (layout != MOE_LAYOUT_FLUX_OUT_IN && layout != MOE_LAYOUT_LLAMA_IN_OUT) return op_fail(fn, "unknown layout");
+    const int k = grad ? out_dim : in_dim, n = grad ? in_dim : out_dim;
+    const bool flux = layout == MOE_LAYOUT_FLUX_OUT_IN;
+    const int wcols = flux ? out_dim : in_dim, wrows = flux ? in_dim : out_dim;
+    if (ldx < k || ldy < n || ldw < wcols) return op_fail(fn, "a row stride is smaller than its row");
+    if (groups > 1 && w_stride < (wrows - 1) * ldw + wcols) return op_fail(fn, "w_stride is smaller than a matrix");
+    if (rows == 0) return MOE_OK;
+    if (!x || !w || !y) return op_fail(fn, "null buffer");
+    if (op_misaligned(x, dtype) || op_misaligned(w, dtype) || op_misaligned(y, y_dtype))
+        return op_fail(fn, "a buffer is not aligned to its elements");
+    OpGemmArgs g{};
+    g.A = x, g.B = w, g.C = y;
+    g.lda = ldx, g.ldb = ldw, g.ldc = ldy;
+    g.b_stride = groups > 1 ? w_stride : 0;
+    g.offsets = offsets, g.E = groups, g.rows = rows;
+    g.N = n, g.K = k, g.c_f32 = y_dtype == MOE_F32, g.splits = 1;
+    // the weight is a "row" operand where its contiguous axis is the product's k
+    const bool b_col = flux != grad;
+    return op_done(fn, dtype == MOE_F32 ? launch_op_gemm_f32(false, b_col, false, g, op_cus(), (hipStream_t)stream)
+                                        : launch_op_gemm_bf16(false, b_col, false, g, op_cus(), (hipStream_t)stream));
+}
+
+// Ranges a group's rows are split into for the weight gradient (1: none).
+int op_wgrad_splits(int32_t, int32_t, int32_t, int32_t) { return 1; }
+}  // namespace
+
+extern "C" {
+
+int moe_grouped_matmul_async(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t w_stride, int32_t layout,
+                             const int32_t *offsets, int32_t groups, int32_t rows, int32_t in_dim, int32_t out_dim,
+                             int32_t dtype, void *y, int64_t ldy, int32_t y_dtype, void *stream) {
+    return op_rows_product("moe_grouped_matmul_async", false, x, ldx, w, ldw, w_stride, layout, offsets, groups, rows,
+                           in_dim, out_dim, dtype, y, ldy, y_dtype, stream);
+}
+
+int moe_grouped_matmul_grad_x_async(const void *dy, int64_t lddy, const void *w, int64_t ldw, int64_t w_stride,
+                                    int32_t layout, const int32_t *offsets, int32_t groups, int32_t rows,
+                                    int32_t in_dim, int32_t out_dim, int32_t dtype, void *dx, int64_t lddx,
+                                    int32_t dx_dtype, void *stream) {
+    return op_rows_product("moe_grouped_matmul_grad_x_async", true, dy, lddy, w, ldw, w_stride, layout, offsets,
+                           groups, rows, in_dim, out_dim, dtype, dx, lddx, dx_dtype, stream);
+}
+
+int moe_grouped_matmul_grad_w_workspace(int32_t groups, int32_t rows, int32_t in_dim, int32_t out_dim,
+                                        int64_t *bytes) {
+    const char *fn = "moe_grouped_matmul_grad_w_workspace";
+    if (!bytes) return op_fail(fn, "null bytes");
+    int r = op_check_groups(fn, (const int32_t *)bytes, groups, rows, in_dim, out_dim);
+    if (r != MOE_OK) return r;
+    const int splits = op_wgrad_splits(groups, rows, in_dim, out_dim);
+    *bytes = splits > 1 ? (int64_t)4 * splits * groups * in_dim * out_dim : 0;
+    return MOE_OK;
+}
+
+int moe_grouped_matmul_grad_w_async(const void *x, int64_t ldx, const void *dy, int64_t lddy, int32_t layout,
+                                    const int32_t *offsets, int32_t groups, int32_t rows, int32_t in_dim,
+                                    int32_t out_dim, int32_t dtype, void *dw, int64_t lddw, int64_t dw_stride,
+                                    int32_t dw_dtype, int32_t accumulate, void *workspace, int64_t workspace_bytes,
+                                    void *stream) {
+    const char *fn = "moe_grouped_matmul_grad_w_async";
+    int r = op_check_groups(fn, offsets, groups, rows, in_dim, out_dim);
+    if (r == MOE_OK) r = op_check_dtypes(fn, dtype, dw_dtype);
+    if (r != MOE_OK) return r;
+    if (layout != MOE_LAYOUT_FLUX_OUT_IN && layout != MOE_LAYOUT_LLAMA_IN_OUT) return op_fail(fn, "unknown layout");
+    const bool flux = layout == MOE_LAYOUT_FLUX_OUT_IN;
+    const int m = flux ? in_dim : out_dim, n = flux ? out_dim : in_dim;
+    if (ldx < in_dim || lddy < out_dim || lddw < n) return op_fail(fn, "a row stride is smaller than its row");
+    if (groups > 1 && dw_stride < (m - 1) * lddw + n) return op_fail(fn, "dw_stride is smaller than a matrix");
+    if (!dw || (rows > 0 && (!x || !dy))) return op_fail(fn, "null buffer");
+    if (op_misaligned(x, dtype) || op_misaligned(dy, dtype) || op_misaligned(dw, dw_dtype))
+        return op_fail(fn, "a buffer is not aligned to its elements");
+    if (rows == 0 && accumulate) return MOE_OK;
+    int64_t need = 0;
+    r = moe_grouped_matmul_grad_w_workspace(groups, rows, in_dim, out_dim, &need);
+    if (r != MOE_OK) return r;
+    if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
+        return op_fail(fn, "the workspace must be 16-byte aligned and hold " + std::to_string(need) + " bytes");
+    OpGemmArgs g{};
+    g.A = flux ? x : dy, g.B = flux ? dy : x, g.C = dw;
+    g.lda = flux ? ldx : lddy, g.ldb = flux ? lddy : ldx, g.ldc = lddw;
+    g.c_stride = groups > 1 ? dw_stride : 0;
+    g.offsets = offsets, g.E = groups, g.rows = rows;
+    g.M = m, g.N = n, g.c_f32 = dw_dtype == MOE_F32, g.accumulate = accumulate != 0;
+    g.splits = op_wgrad_splits(groups, rows, in_dim, out_dim);
+    g.ws = (float *)workspace;
+    return op_done(fn, dtype == MOE_F32 ? launch_op_gemm_f32(true, true, true, g, op_cus(), (hipStream_t)stream)
+                                        : launch_op_gemm_bf16(true, true, true, g, op_cus(), (hipStream_t)stream));
+}
+
+int moe_quantize_int8_async(const void *x, int64_t ldx, int32_t x_dtype, int64_t rows, int32_t cols, void *q,
+                            int64_t ldq, float *scale, void *stream) {
+    const char *fn = "moe_quantize_int8_async";
+    if (x_dtype != MOE_F32 && x_dtype != MOE_BF16) return op_fail(fn, "x_dtype must be MOE_F32 or MOE_BF16");
+    if (rows < 0 || cols < 1) return op_fail(fn, "rows must not be negative and cols positive");
+    if (ldx < cols || ldq < cols) return op_fail(fn, "a row stride is smaller than its row");
+    if (rows == 0) return MOE_OK;
+    if (!x || !q || !scale) return op_fail(fn, "null buffer");
+    if (op_misaligned(x, x_dtype) || op_misaligned(scale, MOE_F32))
+        return op_fail(fn, "a buffer is not aligned to its elements");
+    if (rows > INT_MAX / 256) return op_fail(fn, "too many rows");
+    return op_done(fn, launch_quantize_i8(x, ldx, x_dtype == MOE_BF16, rows, cols, (int8_t *)q, ldq, cols, scale,
+                                          (hipStream_t)stream));
+}
+
+int moe_int8_matmul_workspace(int32_t rows, int32_t in_dim, int64_t *bytes) {
+    const char *fn = "moe_int8_matmul_workspace";
+    if (!bytes) return op_fail(fn, "null bytes");
+    if (rows < 0 || in_dim < 1) return op_fail(fn, "rows must not be negative and in_dim positive");
+    // scales, then the codes, rows padded to 16 bytes
+    *bytes = round_up((int64_t)rows * 4, 16) + (int64_t)rows * round_up(in_dim, 16);
+    return MOE_OK;
+}
+
+int moe_int8_matmul_async(const void *x, int64_t ldx, int32_t x_dtype, const float *x_scale, const void *w,
+                          int64_t ldw, int64_t w_stride, const float *w_scale, const int32_t *offsets, int32_t groups,
+                          int32_t rows, int32_t in_dim, int32_t out_dim, void *y, int64_t ldy, int32_t y_dtype,
+                          void *workspace, int64_t workspace_bytes, void *stream) {
+    const char *fn = "moe_int8_matmul_async";
+    int r = op_check_groups(fn, offsets, groups, rows, in_dim, out_dim);
+    if (r != MOE_OK) return r;
+    const bool codes = x_dtype == MOE_INT8;
+    if (!codes && x_dtype != MOE_F32 && x_dtype != MOE_BF16)
+        return op_fail(fn, "x_dtype must be MOE_INT8, MOE_BF16 or MOE_F32");
+    if (y_dtype != MOE_F32 && y_dtype != MOE_BF16) return op_fail(fn, "the result must be MOE_F32 or MOE_BF16");
+    if (in_dim > 131071) return op_fail(fn, "in_dim above 131071 (the int32 sums could overflow)");
+    if (ldx < in_dim || ldy < out_dim || ldw < in_dim) return op_fail(fn, "a row stride is smaller than its row");
+    if (groups > 1 && w_stride < (out_dim - 1) * ldw + in_dim) return op_fail(fn, "w_stride is smaller than a matrix");
+    if (rows == 0) return MOE_OK;
+    if (!x || !w || !w_scale || !y) return op_fail(fn, "null buffer");
+    if (codes && !x_scale) return op_fail(fn, "int8 rows need x_scale");
+    if ((!codes && op_misaligned(x, x_dtype)) || op_misaligned(y, y_dtype) || op_misaligned(w_scale, MOE_F32) ||
+        (codes && op_misaligned(x_scale, MOE_F32)))
+        return op_fail(fn, "a buffer is not aligned to its elements");
+    if (rows > INT_MAX / 256) return op_fail(fn, "too many rows");
+    if (!codes) {
+        int64_t need = 0;
+        r = moe_int8_matmul_workspace(rows, in_dim, &need);
+        if (r != MOE_OK) return r;
+        if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))
+            return op_fail(fn, "the workspace must be 16-byte aligned and hold " + std::to_string(need) + " bytes");
+        float *sx = (float *)workspace;
+        int8_t *q = (int8_t *)workspace + round_up((int64_t)rows * 4, 16);
+        const int64_t ldq = round_up(in_dim, 16);
+        r = op_done(fn, launch_quantize_i8(x, ldx, x_dtype == MOE_BF16, rows, in_dim, q, ldq, (int)ldq, sx,
+                                           (hipStream_t)stream));
+        if (r != MOE_OK) return r;
+        x = q, ldx = ldq, x_scale = sx;
+    }
+    OpGemmArgs g{};
+    g.A = x, g.B = w, g.C = y;
+    g.lda = ldx, g.ldb = ldw, g.ldc = ldy;
+    g.b_stride = groups > 1 ? w_stride : 0;
+    g.offsets = offsets, g.E = groups, g.rows = rows;
+    g.N = out_dim, g.K = in_dim, g.c_f32 = y_dtype == MOE_F32, g.splits = 1;
+    g.sa = x_scale, g.sb = w_scale;
+    return op_done(fn, launch_op_gemm_i8(g, op_cus(), (hipStream_t)stream));
+}
+
+static int op_check_norm(const char *fn, int64_t T, int32_t D, int32_t x_dtype, int32_t y_dtype, int32_t h_dtype,
+                         int32_t w_dtype, int32_t gate_dtype, const void *gate, int64_t gate_rows) {
+    for (const int32_t t : {x_dtype, y_dtype, h_dtype, w_dtype, gate_dtype})
+        if (t != MOE_F32 && t != MOE_BF16) return op_fail(fn, "dtypes must be MOE_F32 or MOE_BF16");
+    if (T < 0) return op_fail(fn, "T must not be negative");
+    if (D < 1 || D > kMaxNormDim) return op_fail(fn, "D must be 1 to " + std::to_string(kMaxNormDim));
+    if (T > INT_MAX / 1024) return op_fail(fn, "too many rows");
+    if (gate && gate_rows < 1) return op_fail(fn, "gate_rows must be positive");
+    return MOE_OK;
+}
+
+int moe_block_norm_async(const void *x, int32_t x_dtype, const void *y, int32_t y_dtype, const void *post_weight,
+                         const void *pre_weight, int32_t w_dtype, const void *gate, int32_t gate_dtype,
+                         int64_t gate_rows, float alpha, float beta, float eps, int64_t T, int32_t D, void *r, void *h,
+                         int32_t h_dtype, float *stats, void *stream) {
+    const char *fn = "moe_block_norm_async";
+    int rc = op_check_norm(fn, T, D, x_dtype, y_dtype, h_dtype, w_dtype, gate_dtype, gate, gate_rows);
+    if (rc != MOE_OK) return rc;
+    if (!(eps >= 0.0f)) return op_fail(fn, "eps must not be negative");
+    if (T == 0) return MOE_OK;
+    if ((h != nullptr) != (pre_weight != nullptr)) return op_fail(fn, "h and pre_weight come together");
+    if (!y && (post_weight || gate)) return op_fail(fn, "post_weight and gate need y");
+    if (!x || (!r && !h)) return op_fail(fn, "null buffer");
+    if (op_misaligned(x, x_dtype) || op_misaligned(r, x_dtype) || op_misaligned(y, y_dtype) ||
+        op_misaligned(h, h_dtype) || op_misaligned(pre_weight, w_dtype) || op_misaligned(post_weight, w_dtype) ||
+        op_misaligned(gate, gate_dtype) || op_misaligned(stats, MOE_F32))
+        return op_fail(fn, "a buffer is not aligned to its elements");
+    NormArgs a{};
+    a.x = x, a.y = y, a.x_bf16 = x_dtype == MOE_BF16, a.y_bf16 = y_dtype == MOE_BF16, a.h_bf16 = h_dtype == MOE_BF16;
+    a.pre = pre_weight, a.post = post_weight, a.w_bf16 = w_dtype == MOE_BF16;
+    a.gate = gate, a.gate_bf16 = gate_dtype == MOE_BF16, a.gate_rows = gate_rows;
+    a.alpha = alpha, a.beta = beta, a.eps = eps, a.T = T, a.D = D;
+    a.r = r, a.h = h, a.stats = stats;
+    return op_done(fn, launch_block_norm(a, (hipStream_t)stream));
+}
+
+int moe_block_norm_grad_workspace(int64_t T, int32_t D, int64_t gate_rows, int64_t *bytes) {
+    const char *fn = "moe_block_norm_grad_workspace";
+    if (!bytes) return op_fail(fn, "null bytes");
+    if (T < 0 || T > INT_MAX / 1024 || D < 1 || D > kMaxNormDim || gate_rows < 0) return op_fail(fn, "bad sizes");
+    *bytes = T == 0 ? 0 : 4 * (int64_t)norm_workspace_floats(T, D, gate_rows);
+    return MOE_OK;
+}
+
+int moe_block_norm_grad_async(const void *dr, const void *dh, const void *r, int32_t x_dtype, const void *y,
+                              int32_t y_dtype, int32_t h_dtype, const float *stats, const void *post_weight,
+                              const void *pre_weight, int32_t w_dtype, const void *gate, int32_t gate_dtype,
+                              int64_t gate_rows, float alpha, float beta, int64_t T, int32_t D, void *dx, void *dy,
+                              float *dgate, float *dpost, float *dpre, void *workspace, int64_t workspace_bytes,
+                              void *stream) {
+    const char *fn = "moe_block_norm_grad_async";
+    int rc = op_check_norm(fn, T, D, x_dtype, y_dtype, h_dtype, w_dtype, gate_dtype, gate, gate_rows);
+    if (rc != MOE_OK) return rc;
+    if (T > 0) {
+        if (!y && (post_weight || gate || dy)) return op_fail(fn, "post_weight, gate and dy need y");
+        if (dgate && !gate) return op_fail(fn, "dgate needs gate");
+        if (dpost && !post_weight) return op_fail(fn, "dpost needs post_weight");
+        if (dh && !pre_weight) return op_fail(fn, "dh needs pre_weight");
+        if (dpre && !dh) return op_fail(fn, "dpre needs dh");
+        if (!dr && !dh) return op_fail(fn, "dr or dh is needed");
+        if ((dh && !r) || ((dh || post_weight) && !stats)) return op_fail(fn, "null buffer");
+    }
+    if (op_misaligned(dr, x_dtype) || op_misaligned(r, x_dtype) || op_misaligned(dx, x_dtype) ||
+        op_misaligned(y, y_dtype) || op_misaligned(dy, y_dtype) || op_misaligned(dh, h_dtype) ||
+        op_misaligned(pre_weight, w_dtype) || op_misaligned(post_weight, w_dtype) || op_misaligned(gate, gate_dtype) ||
+        op_misaligned(stats, MOE_F32) || op_misaligned(dgate, MOE_F32) || op_misaligned(dpost, MOE_F32) ||
+        op_misaligned(dpre, MOE_F32))
+        return op_fail(fn, "a buffer is not aligned to its elements");
+    int64_t need = 0;
+    rc = moe_block_norm_grad_workspace(T, D, gate ? gate_rows : 0, &need);
+    if (rc != MOE_OK) return rc;
+    if ((dgate || dpost || dpre) && need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
+        return op_fail(fn, "the workspace must be 16-byte aligned and hold " + std::to_string(need) + " bytes");
+    NormArgs a{};
+    a.y = y, a.x_bf16 = x_dtype == MOE_BF16, a.y_bf16 = y_dtype == MOE_BF16, a.h_bf16 = h_dtype == MOE_BF16;
+    a.pre = pre_weight, a.post = post_weight, a.w_bf16 = w_dtype == MOE_BF16;
+    a.gate = gate, a.gate_bf16 = gate_dtype == MOE_BF16, a.gate_rows = gate_rows;
+    a.alpha = alpha, a.beta = beta, a.T = T, a.D = D;
+    a.r = (void *)r, a.stats = (float *)stats;
+    a.dr = dr, a.dh = dh, a.dx = dx, a.dy = dy, a.dgate = dgate, a.dpost = dpost, a.dpre = dpre;
+    a.ws = (float *)workspace;
+    return op_done(fn, launch_block_norm_grad(a, (hipStream_t)stream));
+}
+
+}  // extern "C"

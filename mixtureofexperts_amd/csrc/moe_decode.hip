@@ -26,6 +26,7 @@
 #include "moe_decode.h"
 #include "moe_decode_batch.h"
 #include "moe_internal.h"
+#include "moe_ops_stream.h"
 
 namespace moe {
 
@@ -563,6 +564,29 @@ hipError_t launch_decode_ffn(const DecodeArgs &a, int ncu, hipStream_t s, hipEve
     case WT_BF16: return launch_decode_wt<WT_BF16>(a, ncu, s, done);
     default: return launch_decode_wt<WT_FP8>(a, ncu, s, done);
     }
+}
+
+// ---- products of few rows per group, row quantisation (moe_ops_stream.h) ------------
+// Up to 16 rows per group on average.
+bool op_stream_fits(int, const OpGemmArgs &g) { return (long long)g.rows <= 16ll * g.E; }
+
+hipError_t launch_op_stream(int ot, const OpGemmArgs &g0, hipStream_t s) {
+    OpGemmArgs g = g0;
+    g.nt = (g.N + 15) / 16;
+    const long long grid = (long long)g.E * g.nt;
+    if (grid > 0x7fffffffll / (ops::kStreamWaves * 64)) return hipErrorInvalidValue;
+    const dim3 b(ops::kStreamWaves * 64);
+    if (ot == OT_F32) ops::op_stream_kernel<OT_F32><<<(unsigned)grid, b, 0, s>>>(g);
+    else if (ot == OT_BF16) ops::op_stream_kernel<OT_BF16><<<(unsigned)grid, b, 0, s>>>(g);
+    else ops::op_stream_kernel<OT_I8><<<(unsigned)grid, b, 0, s>>>(g);
+    return hipGetLastError();
+}
+
+hipError_t launch_quantize_i8(const void *x, long long ldx, int x_bf16, long long rows, int cols, int8_t *q,
+                              long long ldq, int pad_to, float *scale, hipStream_t s) {
+    if (x_bf16) ops::quantize_i8_kernel<1><<<(unsigned)rows, 256, 0, s>>>(x, ldx, cols, q, ldq, pad_to, scale);
+    else ops::quantize_i8_kernel<0><<<(unsigned)rows, 256, 0, s>>>(x, ldx, cols, q, ldq, pad_to, scale);
+    return hipGetLastError();
 }
 
 }  // namespace moe

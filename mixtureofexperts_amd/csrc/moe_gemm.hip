@@ -32,6 +32,7 @@
 
 #include "moe_gemm.h"
 #include "moe_internal.h"
+#include "moe_ops_gemm.h"
 
 namespace moe {
 
@@ -379,6 +380,18 @@ hipError_t launch_grouped_gemm_f32(int mode, const GemmArgs &g0, hipStream_t s) 
     if (mode == MODE_STD_UP) return launch_one<MODE_STD_UP>(g, s);
     if (mode == MODE_DOWN) return launch_one<MODE_DOWN>(g, s);
     return hipErrorInvalidValue;
+}
+
+hipError_t launch_op_gemm_f32(bool, bool b_col, bool ragged_k, OpGemmArgs g, int ncu, hipStream_t s) {
+    if (ragged_k) return ops::op_gemm_plan<OT_F32, true, true, true>(g, ncu, s);
+    if (b_col) return ops::op_gemm_plan<OT_F32, false, true, false>(g, ncu, s);
+    if (op_stream_fits(OT_F32, g)) return launch_op_stream(OT_F32, g, s);
+    return ops::op_gemm_plan<OT_F32, false, false, false>(g, ncu, s);
+}
+
+hipError_t launch_op_gemm_i8(OpGemmArgs g, int ncu, hipStream_t s) {
+    if (op_stream_fits(OT_I8, g)) return launch_op_stream(OT_I8, g, s);
+    return ops::op_gemm_plan<OT_I8, false, false, false>(g, ncu, s);
 }
 
 }  // namespace moe

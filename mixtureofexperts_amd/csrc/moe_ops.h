@@ -1,0 +1,93 @@
+// moe_ops.h -- argument blocks and launchers of the operators on a caller's
+// own device tensors (grouped products and their gradients, int8 products,
+// block norms), shared by the translation units that hold their kernels.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace moe {
+
+enum OpType { OT_F32 = 0, OT_BF16 = 1, OT_I8 = 2 };
+__host__ __device__ constexpr int op_size(int ot) { return ot == OT_F32 ? 4 : (ot == OT_BF16 ? 2 : 1); }
+
+// C[m][n] = sum_k A(m, k) B(n, k) per group.  An operand is held with k
+// contiguous ("row": address m ld + k) or with m (n) contiguous ("col":
+// address k ld + m).
+//
+// Ragged rows (ragged_k = 0): group e's rows [offsets[e], offsets[e + 1]) of A
+// and C against its own B (b_stride elements apart): the forward product and
+// the gradient of the rows.
+// Ragged k (ragged_k = 1): A and B are both "col" over the group's rows and C
+// is the group's own matrix (c_stride elements apart): the weight gradient.
+struct OpGemmArgs {
+    const void *A, *B;
+    void *C;
+    long long lda, ldb, ldc;       // elements
+    long long b_stride, c_stride;  // elements per group
+    const int *offsets;            // [E + 1] or null: one group of all rows
+    int E, rows;                   // groups, rows of the ragged tensors
+    int M, N, K;                   // sizes that are not ragged
+    int c_f32;                     // C in fp32, else bf16
+    int accumulate;                // ragged k: C += (fp32 sums, one rounding)
+    const float *sa;               // int8: scale per row of A
+    const float *sb;               // int8: scale per group and column [E][N]
+    float *ws;                     // ragged k: partial sums of split groups
+    int splits;                    // ragged k: ranges a group's rows are split into (1: none)
+    int nt, mt;                    // tiles along N, and (ragged k) along M
+};
+
+// The rows of group e, held within [0, rows] whatever the offsets say.
+__device__ __forceinline__ void op_group(const int *offsets, int e, int rows, int &lo, int &hi) {
+    lo = 0;
+    hi = rows;
+    if (offsets) {
+        lo = min(max(offsets[e], 0), rows);
+        hi = min(max(offsets[e + 1], lo), rows);
+    }
+}
+
+// a_col / b_col as above; the launchers pick tile and load form (op_gemm_plan)
+hipError_t launch_op_gemm_f32(bool a_col, bool b_col, bool ragged_k, OpGemmArgs g, int ncu, hipStream_t s);
+hipError_t launch_op_gemm_bf16(bool a_col, bool b_col, bool ragged_k, OpGemmArgs g, int ncu, hipStream_t s);
+hipError_t launch_op_gemm_i8(OpGemmArgs g, int ncu, hipStream_t s);
+// few rows per group, both operands "row": the weights streamed once
+hipError_t launch_op_stream(int ot, const OpGemmArgs &g, hipStream_t s);
+bool op_stream_fits(int ot, const OpGemmArgs &g);
+
+// q[r][k] = rne(127 x[r][k] / max|x[r]|) as int8, scale[r] = max|x[r]| / 127;
+// columns [cols, ldq) are not written past pad_to (zeros up to it)
+hipError_t launch_quantize_i8(const void *x, long long ldx, int x_bf16, long long rows, int cols, int8_t *q,
+                              long long ldq, int pad_to, float *scale, hipStream_t s);
+
+// ---- norms around a block ----------------------------------------------------------
+// z = y (post: y rstd(y) post), r = alpha x + beta gate z (rounded to x's
+// type), h = r rstd(r) pre; rstd(v) = 1 / sqrt(mean(v^2) + eps) over a row.
+struct NormArgs {
+    const void *x, *y;           // [T][D]; y may be null (r = alpha x)
+    int x_bf16, y_bf16, h_bf16;
+    const void *pre, *post;      // [D] or null
+    int w_bf16;
+    const void *gate;            // [ceil(T / gate_rows)][D] or null
+    int gate_bf16;
+    long long gate_rows;         // rows that share a gate row
+    float alpha, beta, eps;
+    long long T;
+    int D;
+    void *r, *h;                 // [T][D] or null
+    float *stats;                // [T][2] rstd(y), rstd(r), or null
+    // gradients
+    const void *dr, *dh;         // [T][D] or null
+    void *dx, *dy;               // [T][D] or null
+    float *dgate, *dpost, *dpre; // [gates][D], [D], [D] or null
+    float *ws;                   // partial sums, 3 x [chunks][D]
+    // chunks of rows (norm_chunks): rows per chunk; cpg > 0: cpg chunks per
+    // gate row, none crossing its rows, their gate sums partial; cpg = 0: a
+    // chunk holds whole gate rows
+    long long chunk_rows, cpg, chunks;
+};
+constexpr int kMaxNormDim = 16384;
+long long norm_workspace_floats(long long T, int D, long long gate_rows);
+hipError_t launch_block_norm(const NormArgs &a, hipStream_t s);
+hipError_t launch_block_norm_grad(NormArgs a, hipStream_t s);
+
+}  // namespace moe

@@ -1,0 +1,645 @@
+// moe_ops_gemm.h -- grouped products on a caller's own row-major tensors: no
+// packing, any strides, groups of any length whose bounds stay on the device.
+//
+// Per group C = A B^T with fp32 (int8: int32) sums.  The three products of a
+// linear layer are one kernel with three operand orders (OpGemmArgs):
+//   forward / row gradient: A "row", B "row" or "col" by the weight's layout;
+//   weight gradient: A and B "col", k running over the group's rows.
+//
+// LDS.  A stage is 128 bytes of k per "row" operand row (64 bf16, 32 fp32,
+// 128 int8) and the same number of k rows of a "col" operand.  A lane's
+// fragment is 16 bytes of consecutive k of one row for every type, so one
+// loop serves bf16 (one MFMA per fragment pair), int8 (one) and fp32 (four,
+// element j of each lane's four: the k order inside a fragment is free as
+// long as both operands use the same).
+//   row operand: row r's 16-byte chunk c at slot c ^ ((r >> 1) & 7);
+//   col operand: k row kr, its 16-element unit u at unit u ^ col_swz(kr).
+//     bf16 fragments come through ds_read_b64_tr_b16 (16 lanes read 4 k rows
+//     x 16 columns and each receives one column), fp32 ones through four
+//     ds_read_b32.
+#pragma once
+#include <type_traits>
+
+#include "moe_internal.h"
+#include "moe_ops.h"
+
+namespace moe {
+namespace ops {
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+
+template <int N>
+using num = std::integral_constant<int, N>;
+
+template <int OT>
+using acc_t = std::conditional_t<OT == OT_I8, i32x4, f32x4>;
+
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// One 16-byte fragment pair into the 16 x 16 block: rows of `b` become the
+// block's rows (4 (lane / 16) + c), rows of `a` its columns (lane % 16).
+template <int OT>
+__device__ __forceinline__ acc_t<OT> fma16(const u32x4 &b, const u32x4 &a, acc_t<OT> c) {
+    if constexpr (OT == OT_BF16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, b),
+                                                       __builtin_bit_cast(bf16x8_t, a), c, 0, 0, 0);
+    } else if constexpr (OT == OT_I8) {
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, b), __builtin_bit_cast(i32x4, a), c, 0,
+                                                     0, 0);
+    } else {
+        const f32x4 fb = __builtin_bit_cast(f32x4, b), fa = __builtin_bit_cast(f32x4, a);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[j], fa[j], c, 0, 0, 0);
+        return c;
+    }
+}
+
+// 16 bytes at p of which the first n elements exist (the others read as 0).
+// p need only have the element's alignment.
+template <int ES>
+__device__ __forceinline__ u32x4 load_chunk(const uint8_t *p, int n) {
+    constexpr int CE = 16 / ES;
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (n >= CE) {
+        __builtin_memcpy(&v, p, 16);
+    } else if (n > 0) {
+        // element by element into a 128-bit value (no indexed register array)
+        unsigned long long lo = 0, hi = 0;
+#pragma unroll
+        for (int i = 0; i < CE; ++i) {
+            unsigned long long x = 0;
+            if (i < n) {
+                if constexpr (ES == 4) x = *(const uint32_t *)(p + 4 * i);
+                else if constexpr (ES == 2) x = *(const uint16_t *)(p + 2 * i);
+                else x = p[i];
+            }
+            if (i * ES < 8) lo |= x << (8 * (i * ES)); else hi |= x << (8 * (i * ES - 8));
+        }
+        v = u32x4{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)};
+    }
+    return v;
+}
+
+// Unit swizzle of a "col" operand's k row: the fragment reads of half a wave
+// (8 k rows x 32 bytes, bf16; 4 k rows x 64 bytes per instruction, fp32) fall
+// into different banks.  NU: 16-element units per k row.
+template <int ES, int NU>
+__device__ __forceinline__ int col_swz(int kr) {
+    if constexpr (ES == 2) {
+        if constexpr (NU >= 8) return (kr & 3) | (((kr >> 3) & 1) << 2);
+        else if constexpr (NU == 4) return ((kr >> 1) & 1) | (((kr >> 3) & 1) << 1);
+        else return (kr >> 3) & 1;
+    } else {
+        return (kr >> 2) & (NU >= 4 ? 3 : NU - 1);
+    }
+}
+
+constexpr unsigned kOutOfRange = 0x80000000u;  // past every buffer's num_records: reads as 0
+
+// One operand's tile of ROWS rows: its LDS stage image and how NT threads fill
+// it.  DIRECT: by buffer loads straight into LDS (16-byte aligned rows and
+// whole chunks; a lane whose chunk lies outside reads zeros by the buffer's
+// own range check).  Otherwise through registers, any alignment.
+template <int ES, int ROWS, bool COL, int NT, bool DIRECT>
+struct Tile {
+    static constexpr int CE = 16 / ES;           // elements per chunk
+    static constexpr int KE = 128 / ES;          // k per stage
+    static constexpr int NC = ROWS * 8 / NT;     // chunks per thread
+    static constexpr int ROWB = COL ? ROWS * ES : 128;
+    static constexpr int CPR = ROWB / 16;        // chunks per LDS row
+    static constexpr int NU = ROWS / 16;         // 16-element units per k row (COL)
+    static constexpr int UC = ES;                // chunks per unit
+    static constexpr int BYTES = ROWS * 128;
+    static_assert(NC >= 1 && ROWS * 8 % NT == 0, "threads cover the tile");
+
+    const uint8_t *base;  // element (row 0, first k) of the tile
+    long long ldb;        // bytes between rows (COL: between k)
+    int lim;              // valid rows (COL: valid elements of a k row)
+    int klen;             // k range
+    unsigned voff[DIRECT ? NC : 1];
+    u32x4 reg[DIRECT ? 1 : NC];
+
+    // chunk i of the image -> its LDS row and source chunk within the row
+    static __device__ __forceinline__ void place(int i, int &row, int &chunk) {
+        row = i / CPR;
+        const int q = i % CPR;
+        if constexpr (COL) chunk = (((q / UC) ^ col_swz<ES, NU>(row)) * UC) + q % UC;
+        else chunk = q ^ ((row >> 1) & 7);
+    }
+    // DIRECT: wave w's load j fills the 1 KB from chunk (j NW + w) 64
+    static __device__ __forceinline__ int chunk_of(int j) { return j * NT + (int)threadIdx.x; }
+
+    __device__ __forceinline__ void init(const uint8_t *b, long long ld_bytes, int limit, int k) {
+        base = b;
+        ldb = ld_bytes;
+        lim = limit;
+        klen = k;
+        if constexpr (DIRECT) {
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+                int row, chunk;
+                place(chunk_of(j), row, chunk);
+                const bool ok = COL ? chunk * CE < lim : row < lim;
+                voff[j] = ok ? (unsigned)(row * (int)ldb + chunk * 16) : kOutOfRange;
+            }
+        }
+    }
+    // stage s straight into the LDS image at byte offset lds (DIRECT)
+    __device__ __forceinline__ void load_lds(int s, unsigned lds, int w) const {
+        const int k0 = s * KE;
+        const uint8_t *p = base + (COL ? (long long)k0 * ldb : (long long)k0 * ES);
+        const unsigned long long a = (unsigned long long)p;
+        u32x4 rs;
+        rs[0] = __builtin_amdgcn_readfirstlane((unsigned)a);
+        rs[1] = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32) & 0xffffu);
+        rs[2] = 0x7fffffffu;
+        rs[3] = 0x00027000u;
+        const int krem = klen - k0;
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+            unsigned v = voff[j];
+            if (krem < KE) {  // the last stage: chunks past the k range read as 0
+                int row, chunk;
+                place(chunk_of(j), row, chunk);
+                if (COL ? row >= krem : chunk * CE >= krem) v = kOutOfRange;
+            }
+            const unsigned m0 = __builtin_amdgcn_readfirstlane(lds + (j * NT + w * 64) * 16);
+            asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(v), "s"(rs), "{m0}"(m0));
+        }
+    }
+    __device__ __forceinline__ void load_regs(int s) {
+        const int k0 = s * KE, krem = klen - k0;
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+            int row, chunk;
+            place(chunk_of(j), row, chunk);
+            int n;
+            const uint8_t *p;
+            if constexpr (COL) {
+                n = row < krem ? lim - chunk * CE : 0;
+                p = base + (long long)(k0 + row) * ldb + chunk * 16;
+            } else {
+                n = row < lim ? krem - chunk * CE : 0;
+                p = base + (long long)row * ldb + (long long)k0 * ES + chunk * 16;
+            }
+            reg[j] = load_chunk<ES>(p, n);
+        }
+    }
+    __device__ __forceinline__ void store_regs(lds_u8 *lds) const {
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+            *(__attribute__((address_space(3))) u32x4 *)(lds + chunk_of(j) * 16) = reg[j];
+    }
+
+    // fragment of rows [row0 + 16 i, +16) (row0 a multiple of 16), half ks of
+    // the stage
+    static __device__ __forceinline__ u32x4 frag(const lds_u8 *lds, int row0, int i, int ks, int lane) {
+        const int r16 = lane & 15, q4 = lane >> 4;
+        if constexpr (!COL) {
+            const lds_u8 *p = lds + (row0 + i * 16 + r16) * 128 + (((ks * 4 + q4) ^ ((r16 >> 1) & 7)) << 4);
+            return *(const __attribute__((address_space(3))) u32x4 *)p;
+        } else if constexpr (ES == 2) {
+            union { s16x4 h[2]; u32x4 v; } f;
+            const int kr = ks * 32 + q4 * 8 + (r16 >> 2);
+            const lds_u8 *p = lds + kr * ROWB + (((row0 >> 4) + i) ^ col_swz<ES, NU>(kr)) * 32 + (r16 & 3) * 8;
+            const lds_u8 *p1 = p + 4 * ROWB;  // k rows kr + 4: bit 2 of kr is clear and not part of the swizzle
+            f.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
+            f.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p1);
+            return f.v;
+        } else {
+            u32x4 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int kr = ks * 16 + q4 * 4 + j;
+                const lds_u8 *p = lds + kr * ROWB + (((row0 >> 4) + i) ^ col_swz<ES, NU>(kr)) * 64 + r16 * 4;
+                v[j] = *(const __attribute__((address_space(3))) unsigned *)p;
+            }
+            return v;
+        }
+    }
+};
+
+// ---- work list -------------------------------------------------------------------
+struct OpJob {
+    int e;         // group
+    int m0, n0;    // tile origin (ragged rows: m0 counted from the group's first row)
+    int lo, len;   // the group's first row and rows
+    int ks, nks;   // ragged k: range of the group's rows
+};
+
+// M tiles per block of the order (block, n tile, M tile): a group of many M
+// tiles re-reads neither its rows for every n tile nor its matrix for every M tile.
+constexpr int kOpMBlock = 8;
+
+// Item `item` of the tiles of all groups, group-major; false past the last.
+// Every wave scans the groups' lengths, 64 groups at a time.
+template <int BM>
+__device__ __forceinline__ bool ragged_job(const OpGemmArgs &g, OpJob &jb, int BN) {
+    const int lane = threadIdx.x & 63, NT = g.nt;
+    // tiles of the group of this lane, summed over the lanes up to it
+    auto scan = [&](int base, int &lo, int &len) {
+        lo = 0;
+        len = 0;
+        if (base + lane < g.E) {
+            int hi;
+            op_group(g.offsets, base + lane, g.rows, lo, hi);
+            len = hi - lo;
+        }
+        int t = (len + BM - 1) / BM;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int u = __shfl_up(t, d);
+            if (lane >= d) t += u;
+        }
+        return t;
+    };
+    int lo, len, W = 0, t = 0;
+    for (int base = 0; base < g.E; base += 64) {
+        t = scan(base, lo, len);
+        W += __shfl(t, 63);
+    }
+    W *= NT;
+    // contiguous per-XCD ranges (block L runs on XCD L mod 8)
+    const int per = (W + 7) >> 3, slot = blockIdx.x >> 3;
+    int item = (blockIdx.x & 7) * per + slot;
+    if (slot >= per || item >= W) return false;
+    for (int base = 0; base < g.E; base += 64) {
+        if (g.E > 64) t = scan(base, lo, len);
+        const unsigned long long past = __ballot(t * NT > item);
+        if (past) {
+            const int src = __ffsll((long long)past) - 1;
+            const int before = src > 0 ? __shfl(t, src - 1) : 0;
+            const int nte = __shfl(t, src) - before;
+            jb.e = base + src;
+            jb.lo = __shfl(lo, src);
+            jb.len = __shfl(len, src);
+            item -= before * NT;
+            int m, n;
+            const int nfb = nte / kOpMBlock, infull = nfb * kOpMBlock * NT;
+            if (item < infull) {
+                const int b = item / (kOpMBlock * NT), q = item - b * (kOpMBlock * NT);
+                n = q / kOpMBlock;
+                m = b * kOpMBlock + (q - n * kOpMBlock);
+            } else {
+                const int ml = nte - nfb * kOpMBlock, q = item - infull;
+                n = q / ml;
+                m = nfb * kOpMBlock + (q - n * ml);
+            }
+            jb.m0 = __builtin_amdgcn_readfirstlane(m * BM);
+            jb.n0 = __builtin_amdgcn_readfirstlane(n * BN);
+            jb.e = __builtin_amdgcn_readfirstlane(jb.e);
+            jb.lo = __builtin_amdgcn_readfirstlane(jb.lo);
+            jb.len = __builtin_amdgcn_readfirstlane(jb.len);
+            jb.ks = 0;
+            jb.nks = 1;
+            return true;
+        }
+        item -= __shfl(t, 63) * NT;
+    }
+    return false;
+}
+
+// Weight gradient: tiles of every group's matrix, group-major, then blocks of
+// kOpMBlock M tiles, n tile, M tile, and the ranges of a split group.
+__device__ __forceinline__ bool matrix_job(const OpGemmArgs &g, OpJob &jb, int BM, int BN, int KE) {
+    const int per_group = g.mt * g.nt * g.splits;
+    const int W = g.E * per_group;
+    const int per = (W + 7) >> 3, slot = blockIdx.x >> 3;
+    int item = (blockIdx.x & 7) * per + slot;
+    if (slot >= per || item >= W) return false;
+    jb.e = item / per_group;
+    item -= jb.e * per_group;
+    jb.ks = item / (g.mt * g.nt);
+    item -= jb.ks * (g.mt * g.nt);
+    jb.nks = g.splits;
+    const int nfb = g.mt / kOpMBlock, infull = nfb * kOpMBlock * g.nt;
+    int m, n;
+    if (item < infull) {
+        const int b = item / (kOpMBlock * g.nt), q = item - b * (kOpMBlock * g.nt);
+        n = q / kOpMBlock;
+        m = b * kOpMBlock + (q - n * kOpMBlock);
+    } else {
+        const int ml = g.mt - nfb * kOpMBlock, q = item - infull;
+        n = q / ml;
+        m = nfb * kOpMBlock + (q - n * ml);
+    }
+    jb.m0 = m * BM;
+    jb.n0 = n * BN;
+    int lo, hi;
+    op_group(g.offsets, jb.e, g.rows, lo, hi);
+    if (jb.nks > 1) {  // equal ranges of whole stages
+        const int chunk = ((hi - lo + jb.nks - 1) / jb.nks + KE - 1) / KE * KE;
+        const int b = min(lo + jb.ks * chunk, hi);
+        hi = min(b + chunk, hi);
+        lo = b;
+    }
+    jb.lo = __builtin_amdgcn_readfirstlane(lo);
+    jb.len = __builtin_amdgcn_readfirstlane(hi - lo);
+    return true;
+}
+
+// ---- results ---------------------------------------------------------------------
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 v = {(__bf16)a, (__bf16)b};
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+// four results at columns n .. n + 3 of a row of C (element index at), N the
+// row's columns; vec: a whole aligned store is possible
+__device__ __forceinline__ void put4(const OpGemmArgs &g, long long at, int n, float v0, float v1, float v2, float v3,
+                                     bool vec) {
+    float v[4] = {v0, v1, v2, v3};
+    if (g.c_f32) {
+        float *c = (float *)g.C + at;
+        if (vec && n + 3 < g.N) {
+            float4 o = make_float4(v0, v1, v2, v3);
+            if (g.accumulate) {
+                const float4 p = *(const float4 *)c;
+                o = make_float4(p.x + v0, p.y + v1, p.z + v2, p.w + v3);
+            }
+            *(float4 *)c = o;
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (n + q < g.N) c[q] = g.accumulate ? c[q] + v[q] : v[q];
+        }
+    } else {
+        uint16_t *c = (uint16_t *)g.C + at;
+        if (vec && n + 3 < g.N) {
+            if (g.accumulate) {
+                const uint2 p = *(const uint2 *)c;
+                v[0] += bf16_to_f32((uint16_t)p.x), v[1] += bf16_to_f32((uint16_t)(p.x >> 16));
+                v[2] += bf16_to_f32((uint16_t)p.y), v[3] += bf16_to_f32((uint16_t)(p.y >> 16));
+            }
+            *(uint2 *)c = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (n + q < g.N) c[q] = f32_to_bf16(g.accumulate ? bf16_to_f32(c[q]) + v[q] : v[q]);
+        }
+    }
+}
+
+__device__ __forceinline__ bool vec_ok(const OpGemmArgs &g) {
+    const int es = g.c_f32 ? 4 : 2;
+    return (((uintptr_t)g.C | (uintptr_t)(g.ldc * es) | (uintptr_t)(g.c_stride * es)) & (4 * es - 1)) == 0;
+}
+
+// ---- the kernel --------------------------------------------------------------------
+// WM x WN waves; each owns (BM / WM) x (BN / WN) outputs.
+template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, bool DIRECT>
+__device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_) {
+    constexpr int ES = op_size(OT), NT = WM * WN * 64, KE = 128 / ES;
+    constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;
+    using TA = Tile<ES, BM, ACOL, NT, DIRECT>;
+    using TB = Tile<ES, BN, BCOL, NT, DIRECT>;
+
+    OpJob jb;
+    if constexpr (RAGK) {
+        if (!matrix_job(g, jb, BM, BN, KE)) return;
+    } else {
+        if (!ragged_job<BM>(g, jb, BN)) return;
+    }
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = w % WM, wn = w / WM;
+
+    TA ta;
+    TB tb;
+    int klen;
+    {
+        const uint8_t *A = (const uint8_t *)g.A, *B = (const uint8_t *)g.B;
+        if constexpr (RAGK) {
+            klen = jb.len;
+            ta.init(A + ((long long)jb.lo * g.lda + jb.m0) * ES, g.lda * ES, g.M - jb.m0, klen);
+            tb.init(B + ((long long)jb.lo * g.ldb + jb.n0) * ES, g.ldb * ES, g.N - jb.n0, klen);
+        } else {
+            klen = g.K;
+            static_assert(!ACOL || RAGK, "ragged rows: A is a row operand");
+            ta.init(A + ((long long)(jb.lo + jb.m0) * g.lda) * ES, g.lda * ES, jb.len - jb.m0, klen);
+            B += (long long)jb.e * g.b_stride * ES;
+            tb.init(B + (BCOL ? (long long)jb.n0 : (long long)jb.n0 * g.ldb) * ES, g.ldb * ES, g.N - jb.n0, klen);
+        }
+    }
+    acc_t<OT> acc[MI][NJ];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = acc_t<OT>{0, 0, 0, 0};
+
+    lds_u8 *ring = (lds_u8 *)ring_;
+    // both slots of A, then both of B: the slots of an operand are within a DS
+    // instruction's 16-bit offset of each other
+    auto a_slot = [](auto SLOT) { return decltype(SLOT)::value * TA::BYTES; };
+    auto b_slot = [](auto SLOT) { return 2 * TA::BYTES + decltype(SLOT)::value * TB::BYTES; };
+    const int S = (klen + KE - 1) / KE;
+    auto compute = [&](auto SLOT) {
+        const lds_u8 *la = ring + a_slot(SLOT), *lb = ring + b_slot(SLOT);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            // the wave's columns in parts of up to four blocks, which bounds the live fragments
+            constexpr int JP = NJ < 4 ? NJ : 4;
+            u32x4 fa[MI], fb[JP];
+#pragma unroll
+            for (int i = 0; i < MI; ++i) fa[i] = TA::frag(la, wm * (BM / WM), i, ks, lane);
+#pragma unroll
+            for (int j0 = 0; j0 < NJ; j0 += JP) {
+#pragma unroll
+                for (int j = 0; j < JP; ++j) fb[j] = TB::frag(lb, wn * (BN / WN), j0 + j, ks, lane);
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < JP; ++j) acc[i][j0 + j] = fma16<OT>(fb[j], fa[i], acc[i][j0 + j]);
+            }
+        }
+    };
+    if (S > 0) {
+        if constexpr (DIRECT) {
+            const unsigned l0 = (unsigned)(uintptr_t)ring;
+            auto load = [&](auto SLOT, int s) {
+                ta.load_lds(s, l0 + a_slot(SLOT), w);
+                tb.load_lds(s, l0 + b_slot(SLOT), w);
+            };
+            auto step = [&](auto SLOT, int s) {
+                wait_loads<0>();
+                lds_barrier();  // stage s landed in every wave; the other slot's reads are done
+                if (s + 1 < S) load(num<1 - decltype(SLOT)::value>{}, s + 1);
+                compute(SLOT);
+            };
+            load(num<0>{}, 0);
+            int s = 0;
+            for (; s + 2 <= S; s += 2) {
+                step(num<0>{}, s);
+                step(num<1>{}, s + 1);
+            }
+            if (s < S) step(num<0>{}, s);
+        } else {
+            auto store = [&](auto SLOT) {
+                ta.store_regs(ring + a_slot(SLOT));
+                tb.store_regs(ring + b_slot(SLOT));
+            };
+            auto step = [&](auto SLOT, int s) {
+                lds_barrier();
+                if (s + 1 < S) {
+                    ta.load_regs(s + 1);
+                    tb.load_regs(s + 1);
+                }
+                compute(SLOT);
+                if (s + 1 < S) store(num<1 - decltype(SLOT)::value>{});
+            };
+            ta.load_regs(0);
+            tb.load_regs(0);
+            store(num<0>{});
+            int s = 0;
+            for (; s + 2 <= S; s += 2) {
+                step(num<0>{}, s);
+                step(num<1>{}, s + 1);
+            }
+            if (s < S) step(num<0>{}, s);
+        }
+    }
+
+    const int r16 = lane & 15, q4 = lane >> 4;
+    if constexpr (RAGK) {
+        if (g.splits > 1) {  // a range's sums: [e][range][M][N] fp32, folded by op_fold_kernel
+            float *ws = g.ws + ((long long)(jb.e * g.splits + jb.ks) * g.M) * g.N;
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                const int m = jb.m0 + wm * (BM / WM) + i * 16 + r16;
+                if (m >= g.M) continue;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    const int n = jb.n0 + wn * (BN / WN) + j * 16 + 4 * q4;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (n + c < g.N) ws[(long long)m * g.N + n + c] = acc[i][j][c];
+                }
+            }
+            return;
+        }
+    }
+    const bool vec = vec_ok(g);
+    const int mrows = RAGK ? g.M - jb.m0 : jb.len - jb.m0;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+        const int ml = wm * (BM / WM) + i * 16 + r16;
+        if (ml >= mrows) continue;
+        const long long row = RAGK ? (long long)jb.e * g.c_stride + (long long)(jb.m0 + ml) * g.ldc
+                                   : (long long)(jb.lo + jb.m0 + ml) * g.ldc;
+        float sa = 0.0f;
+        if constexpr (OT == OT_I8) sa = g.sa[jb.lo + jb.m0 + ml];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int n = jb.n0 + wn * (BN / WN) + j * 16 + 4 * q4;
+            float v[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                v[c] = (float)acc[i][j][c];
+                if constexpr (OT == OT_I8)
+                    v[c] = v[c] * sa * (n + c < g.N ? g.sb[(long long)jb.e * g.N + n + c] : 0.0f);
+            }
+            put4(g, row + n, n, v[0], v[1], v[2], v[3], vec);
+        }
+    }
+}
+
+template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, bool DIRECT, int WPE>
+__global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void op_gemm_kernel(
+    OpGemmArgs g) {
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[2 * (BM + BN) * 128];
+    op_gemm_tile<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, DIRECT>(g, ring);
+}
+
+// C of a split group: its ranges' sums in range order, one element per thread.
+template <int DUMMY>
+__global__ __launch_bounds__(256) void op_fold_kernel(OpGemmArgs g) {
+    const long long per = (long long)g.M * g.N, total = per * g.E;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long e = i / per, r = i - e * per;
+        const float *ws = g.ws + e * g.splits * per + r;
+        float v = 0.0f;
+        for (int s = 0; s < g.splits; ++s) v += ws[s * per];
+        const long long m = r / g.N, n = r - m * g.N;
+        const long long at = e * g.c_stride + m * g.ldc + n;
+        if (g.c_f32) {
+            float *c = (float *)g.C + at;
+            *c = g.accumulate ? *c + v : v;
+        } else {
+            uint16_t *c = (uint16_t *)g.C + at;
+            *c = f32_to_bf16(g.accumulate ? bf16_to_f32(*c) + v : v);
+        }
+    }
+}
+
+// Rows that can be loaded straight into LDS: 16-byte aligned, whole chunks
+// along the contiguous axis, and a tile's byte offsets within 31 bits.
+inline bool direct_ok(const void *p, long long ld, long long stride, int contiguous, int es) {
+    return (((uintptr_t)p | (uintptr_t)(ld * es) | (uintptr_t)(stride * es)) & 15) == 0 &&
+           (long long)contiguous * es % 16 == 0 && ld * es < (1ll << 22);
+}
+
+template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int WPE>
+hipError_t launch_tiles(OpGemmArgs g, bool direct, hipStream_t s) {
+    g.nt = (g.N + BN - 1) / BN;
+    g.mt = RAGK ? (g.M + BM - 1) / BM : 0;
+    // ragged rows: sum of ceil(rows_e / BM) <= rows / BM + the groups that can hold a row
+    const long long mtiles = RAGK ? (long long)g.E * g.mt * g.splits
+                                  : (long long)(g.rows / BM) + (g.E < g.rows ? g.E : g.rows);
+    const long long grid = (mtiles * g.nt + 7) / 8 * 8;
+    if (grid > 0x7fffffffll / (WM * WN * 64)) return hipErrorInvalidValue;
+    const dim3 b(WM * WN * 64);
+    if constexpr (BM == 256) {  // (staging through registers leaves too few for these tiles)
+        if (!direct) return hipErrorInvalidValue;
+        op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, true, WPE><<<(unsigned)grid, b, 0, s>>>(g);
+    } else {
+        if (direct) op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, true, WPE><<<(unsigned)grid, b, 0, s>>>(g);
+        else op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, false, WPE><<<(unsigned)grid, b, 0, s>>>(g);
+    }
+    hipError_t e = hipGetLastError();
+    if constexpr (RAGK) {
+        if (e == hipSuccess && g.splits > 1) {
+            const long long n = ((long long)g.E * g.M * g.N + 255) / 256;
+            op_fold_kernel<0><<<(unsigned)(n < 8192 ? n : 8192), 256, 0, s>>>(g);
+            e = hipGetLastError();
+        }
+    }
+    return e;
+}
+
+// Tile and load form of a call.  Ragged rows: 256 x 256 tiles where groups
+// average enough rows to fill them and there are two rounds of them, else
+// 128 x 128, and 64 x 64 for short groups or few tiles.  Ragged k: by the
+// tiles of all groups; where even 64 x 64 tiles are few, a group's rows are
+// split into ranges (op_wgrad_splits).
+template <int OT, bool ACOL, bool BCOL, bool RAGK>
+hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
+    constexpr int ES = op_size(OT);
+    const bool direct =
+        direct_ok(g.A, g.lda, 0, ACOL ? g.M : g.K, ES) && direct_ok(g.B, g.ldb, g.b_stride, BCOL ? g.N : g.K, ES);
+    auto tiles = [&](int b) -> long long {
+        const long long nt = (g.N + b - 1) / b;
+        if (RAGK) return nt * ((g.M + b - 1) / b) * g.E;
+        const long long few = (long long)g.rows / b > g.E ? (long long)g.rows / b : (g.E < g.rows ? g.E : g.rows);
+        return nt * few;
+    };
+    const long long avg = RAGK ? g.M : (long long)g.rows / g.E;
+    if constexpr (OT != OT_F32) {
+        if (direct && avg >= 192 && g.N >= 192 && tiles(256) >= 2 * ncu)
+            return launch_tiles<OT, ACOL, BCOL, RAGK, 256, 256, 4, 2, 2>(g, direct, s);
+    }
+    if (avg >= 64 && g.N >= 64 && tiles(128) >= ncu)
+        return launch_tiles<OT, ACOL, BCOL, RAGK, 128, 128, 2, 2, 2>(g, direct, s);
+    return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, 3>(g, direct, s);
+}
+
+}  // namespace ops
+}  // namespace moe

@@ -1,0 +1,509 @@
+// moe_ops_norm.h -- the norms before and after a block with its gate and
+// residual scale, and their gradients: one pass over the data, a row held in
+// registers by TPR threads (8 consecutive channels per thread and vector).
+#pragma once
+#include "moe_internal.h"
+#include "moe_ops.h"
+
+namespace moe {
+namespace ops {
+
+// Eight channels of a row.
+struct Row8 {
+    float v[8];
+};
+// The same as they are loaded: fp32, or bf16 pairs in the first four words.  A
+// load and its widening are apart so that loads of several tensors are in
+// flight together, whatever their types (the branches are uniform).  Without
+// VEC (odd D or unaligned rows) the elements are widened as they are read.
+struct Raw8 {
+    unsigned u[8];
+};
+// channels from c of a row; those past D read as 0
+template <bool VEC>
+__device__ __forceinline__ Raw8 load_raw(const void *p, int bf16, long long row, int c, int D) {
+    Raw8 o{};
+    if (bf16) {
+        const uint16_t *q = (const uint16_t *)p + row * D + c;
+        if constexpr (VEC) {
+            if (c < D) {
+                const uint4 w = *(const uint4 *)q;
+                o.u[0] = w.x, o.u[1] = w.y, o.u[2] = w.z, o.u[3] = w.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o.u[i] = c + i < D ? (unsigned)q[i] << 16 : 0u;
+        }
+    } else {
+        const unsigned *q = (const unsigned *)p + row * D + c;
+        if constexpr (VEC) {
+            if (c < D) {
+                const uint4 w = *(const uint4 *)q, x = *(const uint4 *)(q + 4);
+                o.u[0] = w.x, o.u[1] = w.y, o.u[2] = w.z, o.u[3] = w.w;
+                o.u[4] = x.x, o.u[5] = x.y, o.u[6] = x.z, o.u[7] = x.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o.u[i] = c + i < D ? q[i] : 0u;
+        }
+    }
+    return o;
+}
+template <bool VEC>
+__device__ __forceinline__ Row8 widen(const Raw8 &r, int bf16) {
+    Row8 o;
+    if (VEC && bf16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            o.v[2 * i] = __uint_as_float(r.u[i] << 16);
+            o.v[2 * i + 1] = __uint_as_float(r.u[i] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o.v[i] = __uint_as_float(r.u[i]);
+    }
+    return o;
+}
+template <bool VEC>
+__device__ __forceinline__ Row8 load8(const void *p, int bf16, long long row, int c, int D) {
+    return widen<VEC>(load_raw<VEC>(p, bf16, row, c, D), bf16);
+}
+template <bool VEC>
+__device__ __forceinline__ void store8(void *p, int bf16, long long row, int c, int D, const Row8 &o) {
+    if (c >= D) return;
+    if (bf16) {
+        uint16_t *q = (uint16_t *)p + row * D + c;
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        unsigned w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bf16x2 b = {(__bf16)o.v[2 * i], (__bf16)o.v[2 * i + 1]};
+            w[i] = __builtin_bit_cast(unsigned, b);
+        }
+        if constexpr (VEC) {
+            *(uint4 *)q = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < D) q[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+        }
+    } else {
+        float *q = (float *)p + row * D + c;
+        if constexpr (VEC) {
+            *(float4 *)q = make_float4(o.v[0], o.v[1], o.v[2], o.v[3]);
+            *(float4 *)(q + 4) = make_float4(o.v[4], o.v[5], o.v[6], o.v[7]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < D) q[i] = o.v[i];
+        }
+    }
+}
+
+// Sum over the TPR threads of a row, the same bits in each of them.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float *part) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+    if constexpr (TPR > 64) {
+        constexpr int NW = TPR / 64;
+        __syncthreads();  // the previous sum has been read
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = part[0];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) v += part[w];
+    }
+    return v;
+}
+
+__device__ __forceinline__ float round_to(float v, int bf16) { return bf16 ? bf16_to_f32(f32_to_bf16(v)) : v; }
+
+template <int TPR, int NV, bool VEC>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(NormArgs a) {
+    constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
+    __shared__ float part[16];
+    const long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
+    if (RPB > 1 && row >= a.T) return;  // whole waves; no barrier below when RPB > 1
+    const int tid = threadIdx.x % TPR, D = a.D;
+    Row8 r[NV], y[NV];
+    {
+        Raw8 rx[NV], ry[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (tid + i * TPR) * 8;
+            rx[i] = load_raw<VEC>(a.x, a.x_bf16, row, c, D);
+            ry[i] = a.y ? load_raw<VEC>(a.y, a.y_bf16, row, c, D) : Raw8{};
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            r[i] = widen<VEC>(rx[i], a.x_bf16);
+            y[i] = widen<VEC>(ry[i], a.y_bf16);
+        }
+    }
+    float iy = 1.0f;
+    if (a.y && a.post) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int q = 0; q < 8; ++q) s += y[i].v[q] * y[i].v[q];
+        iy = 1.0f / sqrtf(row_sum<TPR>(s, part) / (float)D + a.eps);
+    }
+    const long long grow = a.gate ? row / a.gate_rows : 0;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (tid + i * TPR) * 8;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) r[i].v[q] *= a.alpha;
+        if (a.y) {
+            Row8 z = y[i];
+            if (a.post) {
+                const Row8 p = load8<VEC>(a.post, a.w_bf16, 0, c, D);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) z.v[q] = z.v[q] * iy * p.v[q];
+            }
+            if (a.gate) {
+                const Row8 p = load8<VEC>(a.gate, a.gate_bf16, grow, c, D);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) z.v[q] *= p.v[q];
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) r[i].v[q] += a.beta * z.v[q];
+        }
+        // the norm is taken of the residual stream as it is stored, which is what
+        // the next block and the gradient read
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            r[i].v[q] = round_to(r[i].v[q], a.x_bf16);
+            s += r[i].v[q] * r[i].v[q];
+        }
+        if (a.r) store8<VEC>(a.r, a.x_bf16, row, c, D, r[i]);
+    }
+    float ir = 1.0f;
+    if (a.h) {
+        ir = 1.0f / sqrtf(row_sum<TPR>(s, part) / (float)D + a.eps);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (tid + i * TPR) * 8;
+            const Row8 p = load8<VEC>(a.pre, a.w_bf16, 0, c, D);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) r[i].v[q] = r[i].v[q] * ir * p.v[q];
+            store8<VEC>(a.h, a.h_bf16, row, c, D, r[i]);
+        }
+    }
+    if (a.stats && tid == 0) {
+        a.stats[2 * row] = iy;
+        a.stats[2 * row + 1] = ir;
+    }
+}
+
+// With rhat = r rstd(r), a = dh pre, b = dz post, yhat = y rstd(y) (y without
+// the post norm):
+//   G = dr + rstd(r) (a - rhat mean(a rhat)),   dpre = sum_t dh rhat
+//   dx = alpha G,  dgate = sum beta G yhat post,  dz = beta G gate
+//   dy = rstd(y) (b - yhat mean(b yhat)),       dpost = sum_t dz yhat
+// A workgroup takes a chunk of rows and keeps its columns' sums in registers;
+// norm_fold_kernel adds the chunks' in order.
+template <int TPR, int NV, bool VEC>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_grad_kernel(NormArgs a) {
+    constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
+    __shared__ float part[16];
+    // two vectors of 1024 threads leave too few registers for every sum: the
+    // weights' go to LDS, each slot its own thread's
+    constexpr bool SL = TPR == 1024 && NV == 2;
+    __shared__ float4 lsum[SL ? 4 * NV * TPR : 1];
+    const long long chunk = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
+    if (RPB > 1 && chunk >= a.chunks) return;  // whole waves when TPR = 64 (no barrier then)
+    const int tid = threadIdx.x % TPR, D = a.D;
+    long long row, end;
+    if (a.cpg > 0) {
+        const long long grp = chunk / a.cpg, first = grp * a.gate_rows;
+        row = first + (chunk - grp * a.cpg) * a.chunk_rows;
+        end = min(min(row + a.chunk_rows, first + a.gate_rows), a.T);
+    } else {
+        row = chunk * a.chunk_rows;
+        end = min(row + a.chunk_rows, a.T);
+    }
+    Row8 spre[SL ? 1 : NV], spost[SL ? 1 : NV], sgate[NV];
+    // sums += t * u, which = 0: pre, 1: post
+    auto slot = [&](int which, int i, int half) -> float4 & { return lsum[((which * NV + i) * 2 + half) * TPR + tid]; };
+    auto add = [&](Row8 *reg, int which, int i, const Row8 &t, const Row8 &u) {
+        if constexpr (SL) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                float4 f = slot(which, i, half);
+                f.x += t.v[4 * half] * u.v[4 * half], f.y += t.v[4 * half + 1] * u.v[4 * half + 1];
+                f.z += t.v[4 * half + 2] * u.v[4 * half + 2], f.w += t.v[4 * half + 3] * u.v[4 * half + 3];
+                slot(which, i, half) = f;
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) reg[i].v[q] += t.v[q] * u.v[q];
+        }
+    };
+    auto total = [&](const Row8 *reg, int which, int i) -> Row8 {
+        if constexpr (SL) {
+            const float4 f = slot(which, i, 0), h = slot(which, i, 1);
+            return Row8{{f.x, f.y, f.z, f.w, h.x, h.y, h.z, h.w}};
+        } else {
+            return reg[i];
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        sgate[i] = Row8{};
+        if constexpr (SL) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) slot(j >> 1, i, j & 1) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        } else {
+            spre[i] = spost[i] = Row8{};
+        }
+    }
+    for (; row < end; ++row) {
+        int wrow = 0;  // the weights' row; opaque where keeping them in registers over the rows would spill
+        if constexpr (SL) asm volatile("" : "+s"(wrow));
+        const float iy = a.post ? a.stats[2 * row] : 1.0f;
+        Row8 g[NV], y[NV];
+        Raw8 wg[NV], wy[NV], wr[NV], wh[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (tid + i * TPR) * 8;
+            wr[i] = a.dh ? load_raw<VEC>(a.r, a.x_bf16, row, c, D) : Raw8{};
+            wh[i] = a.dh ? load_raw<VEC>(a.dh, a.h_bf16, row, c, D) : Raw8{};
+            if (!SL) {
+                wg[i] = a.dr ? load_raw<VEC>(a.dr, a.x_bf16, row, c, D) : Raw8{};
+                wy[i] = a.y ? load_raw<VEC>(a.y, a.y_bf16, row, c, D) : Raw8{};
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) g[i] = Row8{};
+        if (a.dh) {
+            const float ir = a.stats[2 * row + 1];
+            Row8 rh[NV], t[NV];
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (tid + i * TPR) * 8;
+                rh[i] = widen<VEC>(wr[i], a.x_bf16);
+                t[i] = widen<VEC>(wh[i], a.h_bf16);
+                const Row8 p = load8<VEC>(a.pre, a.w_bf16, wrow, c, D);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) rh[i].v[q] *= ir;
+                add(spre, 0, i, t[i], rh[i]);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    t[i].v[q] *= p.v[q];
+                    s += t[i].v[q] * rh[i].v[q];
+                }
+            }
+            s = row_sum<TPR>(s, part) / (float)D;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int q = 0; q < 8; ++q) g[i].v[q] += ir * (t[i].v[q] - rh[i].v[q] * s);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (tid + i * TPR) * 8;
+            if (SL) {  // (loaded here: fewer registers live above)
+                wg[i] = a.dr ? load_raw<VEC>(a.dr, a.x_bf16, row, c, D) : Raw8{};
+                wy[i] = a.y ? load_raw<VEC>(a.y, a.y_bf16, row, c, D) : Raw8{};
+            }
+            const Row8 o = widen<VEC>(wg[i], a.x_bf16);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) g[i].v[q] += o.v[q];
+            y[i] = widen<VEC>(wy[i], a.y_bf16);
+        }
+        const long long grow = a.gate ? row / a.gate_rows : 0;
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (tid + i * TPR) * 8;
+            if (a.dx) {
+                Row8 o;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) o.v[q] = a.alpha * g[i].v[q];
+                store8<VEC>(a.dx, a.x_bf16, row, c, D, o);
+            }
+            if (a.y) {
+                Row8 po;
+                if (a.post) {
+                    po = load8<VEC>(a.post, a.w_bf16, wrow, c, D);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) y[i].v[q] *= iy;  // yhat
+                }
+#pragma unroll
+                for (int q = 0; q < 8; ++q) g[i].v[q] *= a.beta;
+                if (a.gate) {
+                    const Row8 gt = load8<VEC>(a.gate, a.gate_bf16, grow, c, D);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        sgate[i].v[q] += g[i].v[q] * (a.post ? y[i].v[q] * po.v[q] : y[i].v[q]);
+                        g[i].v[q] *= gt.v[q];
+                    }
+                }
+                if (a.post) {
+                    add(spost, 1, i, g[i], y[i]);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        g[i].v[q] *= po.v[q];
+                        s += g[i].v[q] * y[i].v[q];
+                    }
+                }
+            }
+        }
+        if (a.y && a.post) {
+            s = row_sum<TPR>(s, part) / (float)D;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int q = 0; q < 8; ++q) g[i].v[q] = iy * (g[i].v[q] - y[i].v[q] * s);
+        }
+        if (a.y && a.dy) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) store8<VEC>(a.dy, a.y_bf16, row, (tid + i * TPR) * 8, D, g[i]);
+        }
+        // a gate row that ends inside the chunk is complete
+        if (a.dgate && a.cpg == 0 && (row + 1 == a.T || (row + 1) % a.gate_rows == 0)) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                store8<VEC>(a.dgate, 0, grow, (tid + i * TPR) * 8, D, sgate[i]);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) sgate[i].v[q] = 0.0f;
+            }
+        }
+    }
+    // partial sums: [pre | post | gate][chunk][D]
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (tid + i * TPR) * 8;
+        if (a.dpre) store8<VEC>(a.ws, 0, chunk, c, D, total(spre, 0, i));
+        if (a.dpost) store8<VEC>(a.ws, 0, a.chunks + chunk, c, D, total(spost, 1, i));
+        if (a.dgate && a.cpg > 0) store8<VEC>(a.ws, 0, 2 * a.chunks + chunk, c, D, sgate[i]);
+    }
+}
+
+// Adds the chunks' sums in a fixed order: 64 columns per workgroup, 16 slices
+// of the chunks.  blockIdx.y: 0 dpre, 1 dpost, 2 + g gate row g.
+template <int DUMMY>
+__global__ __launch_bounds__(1024) void norm_fold_kernel(NormArgs a) {
+    __shared__ float part[16][64];
+    const int what = blockIdx.y;
+    float *out = what == 0 ? a.dpre : (what == 1 ? a.dpost : a.dgate + (long long)(what - 2) * a.D);
+    if ((what == 0 && !a.dpre) || (what == 1 && !a.dpost)) return;
+    const long long first = what < 2 ? what * a.chunks : 2 * a.chunks + (what - 2) * a.cpg;
+    const long long n = what < 2 ? a.chunks : a.cpg;
+    const int col = blockIdx.x * 64 + (threadIdx.x & 63), sl = threadIdx.x >> 6;
+    float v = 0.0f;
+    if (col < a.D) {
+        const float *p = a.ws + first * a.D + col;
+        for (long long i = sl; i < n; i += 16) v += p[i * a.D];
+    }
+    part[sl][threadIdx.x & 63] = v;
+    __syncthreads();
+    if (sl == 0 && col < a.D) {
+#pragma unroll
+        for (int i = 1; i < 16; ++i) v += part[i][threadIdx.x];
+        out[col] = v;
+    }
+}
+
+}  // namespace ops
+
+// Waves per row of the gradient kernel for D channels.
+static int norm_grad_threads(int D) {
+    return D <= 512 ? 64 : (D <= 2048 ? 256 : (D <= 4096 ? 512 : 1024));
+}
+
+// Chunks of the gradient's rows: about sixteen waves per CU, at least four
+// rows each (their sums are written once per chunk).
+static void norm_chunks(long long T, int D, long long gate_rows, long long &chunk_rows, long long &cpg,
+                        long long &chunks) {
+    const long long target = 4096 / (norm_grad_threads(D) / 64);
+    long long R = (T + target - 1) / target;
+    if (R < 4) R = 4;
+    cpg = 0;
+    if (gate_rows > 0 && gate_rows <= R) {
+        chunk_rows = R / gate_rows * gate_rows;  // whole gate rows
+        chunks = (T + chunk_rows - 1) / chunk_rows;
+    } else {
+        const long long per = gate_rows > 0 ? gate_rows : T, groups = (T + per - 1) / per;
+        chunk_rows = R < per ? R : per;
+        cpg = (per + chunk_rows - 1) / chunk_rows;
+        chunks = groups * cpg;
+    }
+}
+
+long long norm_workspace_floats(long long T, int D, long long gate_rows) {
+    long long r, c, n;
+    if (gate_rows > T) gate_rows = T;
+    norm_chunks(T, D, gate_rows, r, c, n);
+    return 3 * n * D;
+}
+
+template <bool VEC>
+static hipError_t norm_launch(const NormArgs &a, bool grad, hipStream_t s) {
+    using namespace ops;
+#define MOE_NORM(K, TPR, NV, N)                                                          \
+    {                                                                                    \
+        const long long rpb = TPR < 256 ? 256 / TPR : 1, blocks = ((N) + rpb - 1) / rpb; \
+        if (blocks > 0x7fffffffll / 1024) return hipErrorInvalidValue;                   \
+        K<TPR, NV, VEC><<<(unsigned)blocks, TPR < 256 ? 256 : TPR, 0, s>>>(a);           \
+    }
+    if (!grad) {
+        if (a.D <= 512) MOE_NORM(block_norm_kernel, 64, 1, a.T)
+        else if (a.D <= 2048) MOE_NORM(block_norm_kernel, 256, 1, a.T)
+        else if (a.D <= 4096) MOE_NORM(block_norm_kernel, 256, 2, a.T)
+        else if (a.D <= 8192) MOE_NORM(block_norm_kernel, 1024, 1, a.T)
+        else MOE_NORM(block_norm_kernel, 1024, 2, a.T)
+    } else {
+        if (a.D <= 512) MOE_NORM(block_norm_grad_kernel, 64, 1, a.chunks)
+        else if (a.D <= 2048) MOE_NORM(block_norm_grad_kernel, 256, 1, a.chunks)
+        else if (a.D <= 4096) MOE_NORM(block_norm_grad_kernel, 512, 1, a.chunks)
+        else if (a.D <= 8192) MOE_NORM(block_norm_grad_kernel, 1024, 1, a.chunks)
+        else MOE_NORM(block_norm_grad_kernel, 1024, 2, a.chunks)
+    }
+#undef MOE_NORM
+    return hipGetLastError();
+}
+
+// whole 16-byte vectors in every tensor of the call
+static bool norm_vec(const NormArgs &a) {
+    if (a.D & 7) return false;
+    for (const void *p : {a.x, a.y, a.pre, a.post, a.gate, (const void *)a.r, (const void *)a.h, a.dr, a.dh,
+                          (const void *)a.dx, (const void *)a.dy, (const void *)a.dgate, (const void *)a.ws})
+        if ((uintptr_t)p & 15) return false;
+    return true;
+}
+static hipError_t norm_run(const NormArgs &a, bool grad, hipStream_t s) {
+    return norm_vec(a) ? norm_launch<true>(a, grad, s) : norm_launch<false>(a, grad, s);
+}
+
+hipError_t launch_block_norm(const NormArgs &a, hipStream_t s) {
+    if (a.T <= 0) return hipSuccess;
+    if (a.D < 1 || a.D > kMaxNormDim) return hipErrorInvalidValue;
+    return norm_run(a, false, s);
+}
+
+hipError_t launch_block_norm_grad(NormArgs a, hipStream_t s) {
+    if (a.D < 1 || a.D > kMaxNormDim) return hipErrorInvalidValue;
+    if (a.gate && a.gate_rows > a.T) a.gate_rows = a.T;
+    long long gr = a.gate ? a.gate_rows : 0;
+    if (a.T > 0) {
+        norm_chunks(a.T, a.D, gr, a.chunk_rows, a.cpg, a.chunks);
+        if (gr == 0) a.gate_rows = a.T;  // the chunks' one group
+        hipError_t e = norm_run(a, true, s);
+        if (e != hipSuccess) return e;
+    } else {
+        a.chunks = a.cpg = 0;  // no rows: the weights' gradients are zeros
+    }
+    const long long gates = a.dgate && a.cpg > 0 ? (a.T + a.gate_rows - 1) / a.gate_rows : 0;
+    if (!a.dpre && !a.dpost && gates == 0) return hipSuccess;
+    if (gates > 65000) return hipErrorInvalidValue;
+    ops::norm_fold_kernel<0><<<dim3((a.D + 63) / 64, (unsigned)(2 + gates)), 1024, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace moe

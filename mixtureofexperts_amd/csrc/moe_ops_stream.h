@@ -1,0 +1,144 @@
+// moe_ops_stream.h -- products of a few rows per group (a decode step): the
+// weights are the traffic, so they go from global memory straight into MFMA
+// fragments, each read once per 16 MT rows of a group.
+//
+// A workgroup owns 16 columns of one group; its eight waves take interleaved
+// 128-byte pieces of k, U of them in flight, and their partial 16 x 16 blocks
+// are added in wave order through LDS.
+#pragma once
+#include "moe_ops_gemm.h"
+
+namespace moe {
+namespace ops {
+
+constexpr int kStreamWaves = 8;
+
+template <int OT, int MT>
+__device__ __forceinline__ void stream_rows(const OpGemmArgs &g, int e, int n0, int lo, int rows, lds_u8 *red) {
+    constexpr int ES = op_size(OT), KE = 128 / ES, CE = 16 / ES;
+    constexpr int U = MT == 1 ? 4 : 2;
+    const int lane = threadIdx.x & 63, r16 = lane & 15, q4 = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // rows past the last one repeat it (their results are not stored)
+    const uint8_t *b = (const uint8_t *)g.B + ((long long)e * g.b_stride + (long long)min(n0 + r16, g.N - 1) * g.ldb) * ES;
+    const uint8_t *a[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+        a[m] = (const uint8_t *)g.A + (long long)(lo + min(m * 16 + r16, rows - 1)) * g.lda * ES;
+    acc_t<OT> acc[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m] = acc_t<OT>{0, 0, 0, 0};
+    const int pieces = (g.K + KE - 1) / KE;
+    const int whole = g.K / KE;
+    int p = w;
+    for (; p + (U - 1) * kStreamWaves < whole; p += U * kStreamWaves) {
+        u32x4 fb[U][2], fa[MT][U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const long long o = (long long)(p + u * kStreamWaves) * 128 + h * 64 + q4 * 16;
+                __builtin_memcpy(&fb[u][h], b + o, 16);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) __builtin_memcpy(&fa[m][u][h], a[m] + o, 16);
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) acc[m] = fma16<OT>(fb[u][h], fa[m][u][h], acc[m]);
+    }
+    for (; p < pieces; p += kStreamWaves) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = p * KE + (h * 4 + q4) * CE;
+            const u32x4 fb = load_chunk<ES>(b + (long long)k * ES, g.K - k);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+                acc[m] = fma16<OT>(fb, load_chunk<ES>(a[m] + (long long)k * ES, g.K - k), acc[m]);
+        }
+    }
+    // red: [wave][MT][64 lanes] 16 bytes
+    typedef __attribute__((address_space(3))) acc_t<OT> lds_acc;
+    lds_acc *ra = (lds_acc *)red;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) ra[(w * MT + m) * 64 + lane] = acc[m];
+    __syncthreads();
+    if (w < MT) {
+        acc_t<OT> v = ra[w * 64 + lane];
+        for (int x = 1; x < kStreamWaves; ++x) v += ra[(x * MT + w) * 64 + lane];
+        const int ml = w * 16 + r16, n = n0 + 4 * q4;
+        if (ml < rows) {
+            float o[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                o[c] = (float)v[c];
+                if constexpr (OT == OT_I8)
+                    o[c] = o[c] * g.sa[lo + ml] * (n + c < g.N ? g.sb[(long long)e * g.N + n + c] : 0.0f);
+            }
+            put4(g, (long long)(lo + ml) * g.ldc + n, n, o[0], o[1], o[2], o[3], vec_ok(g));
+        }
+    }
+    __syncthreads();
+}
+
+template <int OT>
+__global__ __launch_bounds__(kStreamWaves * 64) void op_stream_kernel(OpGemmArgs g) {
+    __shared__ __attribute__((aligned(16))) uint8_t red_[kStreamWaves * 4 * 64 * 16];
+    lds_u8 *red = (lds_u8 *)red_;
+    const int e = blockIdx.x / g.nt, n0 = (blockIdx.x - e * g.nt) * 16;
+    int lo, hi;
+    op_group(g.offsets, e, g.rows, lo, hi);
+    while (lo < hi) {
+        const int rows = min(hi - lo, 64);
+        if (rows <= 16) stream_rows<OT, 1>(g, e, n0, lo, rows, red);
+        else if (rows <= 32) stream_rows<OT, 2>(g, e, n0, lo, rows, red);
+        else stream_rows<OT, 4>(g, e, n0, lo, rows, red);
+        lo += rows;
+    }
+}
+
+// One row's codes: the largest magnitude, then rne(127 x / max).  127 x is
+// formed first so that a code's border, an odd multiple of max / 254, divides
+// exactly; x and max are scaled by 2^-64 where 127 x could overflow.  A row
+// of zeros has scale 0 and codes 0; a row that holds an infinity or a NaN has
+// scale NaN (and codes 0), so that its products are NaN.
+template <int XB>
+__global__ __launch_bounds__(256) void quantize_i8_kernel(const void *x_, long long ldx, int cols, int8_t *q_,
+                                                          long long ldq, int pad_to, float *scale) {
+    __shared__ float part[4];
+    const long long r = blockIdx.x;
+    int8_t *q = q_ + r * ldq;
+    auto at = [&](int c) -> float {
+        if constexpr (XB) return bf16_to_f32(((const uint16_t *)x_)[r * ldx + c]);
+        else return ((const float *)x_)[r * ldx + c];
+    };
+    float m = 0.0f;
+    bool bad = false;
+    for (int c = threadIdx.x; c < cols; c += 256) {
+        const float v = fabsf(at(c));
+        bad |= !(v <= 3.402823466e38f);
+        m = fmaxf(m, v);
+    }
+    if (bad) m = __builtin_nanf("");
+    // NaN has to survive the maximum
+    auto larger = [](float a, float b) { return (a != a || b != b) ? __builtin_nanf("") : fmaxf(a, b); };
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = larger(m, __shfl_xor(m, d));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = larger(larger(part[0], part[1]), larger(part[2], part[3]));
+    if (threadIdx.x == 0) scale[r] = m / 127.0f;
+    const float down = m > 1.0e36f ? 5.421010862427522e-20f : 1.0f;  // 2^-64: exact
+    const float ms = m * down;
+    const bool live = m > 0.0f;  // false for 0 and NaN
+    for (int c = threadIdx.x; c < pad_to; c += 256) {
+        float v = 0.0f;
+        if (live && c < cols) v = rintf(at(c) * down * 127.0f / ms);
+        q[c] = (int8_t)(int)v;
+    }
+}
+
+}  // namespace ops
+}  // namespace moe

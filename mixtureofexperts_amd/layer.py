@@ -18,6 +18,7 @@ from .balancing import (AuxiliaryFreeLoss, LoadBalancingLoss, NoBalancingLoss, S
                         update_bias)
 from .experts import GatedExpert, StandardExpert
 from .gating import HOST_ROUTED_GATES, GatingMechanism, TopKGating, gate_spec
+from .ops import block_norm
 
 _DTYPES = {"f32": _lib.MOE_F32, "fp32": _lib.MOE_F32, "bf16": _lib.MOE_BF16, "fp8": _lib.MOE_FP8_E4M3,
            "fp8_e4m3": _lib.MOE_FP8_E4M3}
@@ -291,6 +292,49 @@ def moe_ffn_forward(moe, xb):
     if vec:
         return out[0], idx[0].astype(np.int64), gates[0]
     return out.T, idx.T.astype(np.int64), gates.T
+
+
+def moe_block_forward(moe, x, *, pre_weight, post_weight=None, gate=None, next_weight=None, alpha=1.0, beta=1.0,
+                      eps=1e-5, training=False, decode=False):
+    """A transformer block's FFN half on torch tensors in GPU memory: rmsnorm!
+    of the residual stream, the layer, and the residual -- moe_ffn_forward!
+    with its rmsnorm and the caller's ``x .+= xb2`` (src/llama2/inference.jl:
+    31-41, 58-61), and the parts that models have put around it since:
+
+        h = x * rstd(x) * pre_weight
+        y = MoE(h)
+        r = alpha x + beta gate * (y, or y * rstd(y) * post_weight)
+        n = r * rstd(r) * next_weight     (the next block's input)
+
+    x (T, input_dim) float32 or bfloat16, rows are tokens; weights, gate, alpha
+    and beta as block_norm takes them (ops.py).  ``decode`` runs the layer as its
+    decode caller does (moe_decode_async: each token on its own, h in float32),
+    else as a forward pass with ``training``.  Returns (r, n or None, balance
+    loss as a (1,) tensor).  Nothing waits for the GPU, and the layer's
+    training_stats are not updated.  Layers whose gate or balance loss keeps
+    state on the host (HashGating, RandomGating, AuxiliaryFreeLoss) have no such
+    path."""
+    c = moe.config
+    if isinstance(moe.router.gate_type, HOST_ROUTED_GATES) or isinstance(moe.balance_loss, AuxiliaryFreeLoss):
+        raise _lib.MoeError(_lib.MOE_EUNSUPPORTED, "moe_block_forward: the gate or loss keeps state on the host")
+    if c.input_dim != c.output_dim:
+        raise _lib.MoeError(_lib.MOE_EINVAL, "a residual needs input_dim == output_dim")
+    if getattr(x, "ndim", 0) != 2 or x.shape[1] != c.input_dim:
+        raise _lib.MoeError(_lib.MOE_EINVAL, f"x must be (T, {c.input_dim})")
+    if pre_weight is None:
+        raise _lib.MoeError(_lib.MOE_EINVAL, "pre_weight is needed")
+    import torch
+
+    # bf16 activations are the bf16 and fp8 layers' own input
+    half = x.dtype == torch.bfloat16 and not decode and c.weight_dtype not in ("f32", "fp32")
+    _, h, _ = block_norm(x, pre_weight=pre_weight, eps=eps, h_dtype=torch.bfloat16 if half else torch.float32)
+    dev = moe._dev if moe._dev is not None else moe.sync_weights()
+    if training and moe._noise_error is not None:
+        raise moe._noise_error
+    y, loss = dev.forward_device(h, training, decode)
+    r, n, _ = block_norm(x, y, pre_weight=next_weight, post_weight=post_weight, gate=gate, alpha=alpha, beta=beta,
+                         eps=eps)
+    return r, n, loss
 
 
 def reset_stats(moe):

@@ -1,0 +1,384 @@
+"""Operators on torch tensors in GPU memory: the grouped products of expert
+FFNs with their gradients, int8 products, and the norms, gate and residual
+around a block.  No counterpart in the reference (it has neither gradients nor
+integer weights, and its caller does the norms, src/llama2/inference.jl:61).
+
+Every function runs on torch's current stream of the tensors' device, allocates
+through torch (workspaces included), does not wait for the GPU and can be
+captured into a graph.  Tensors of one call are on one device.  A wrong
+argument raises MoeError.
+
+Groups: ``offsets`` is an int32 tensor of E + 1 non-decreasing row numbers on
+the device; rows [offsets[e], offsets[e + 1]) belong to expert e, and rows
+outside every group are neither read nor written.  ``None``: one expert, all
+rows.  Weights are (E, out, in) with ``layout=MOE_LAYOUT_LLAMA_IN_OUT`` (the
+default) and (E, in, out) with ``MOE_LAYOUT_FLUX_OUT_IN``; one expert's may be
+2-D.  Rows may be strided (contiguous within a row); 16-byte aligned rows are
+read faster.  A result must not overlap an operand.
+"""
+import ctypes
+
+from . import _lib
+from ._lib import MOE_EINVAL, MOE_LAYOUT_FLUX_OUT_IN, MOE_LAYOUT_LLAMA_IN_OUT
+
+_torch = None
+_codes = {}
+
+
+def _t():
+    """torch, imported at first use (the host API needs only numpy)."""
+    global _torch
+    if _torch is None:
+        import torch
+
+        _torch = torch
+        _codes.update({torch.float32: _lib.MOE_F32, torch.bfloat16: _lib.MOE_BF16, torch.int8: _lib.MOE_INT8})
+    return _torch
+
+
+def _bad(msg):
+    raise _lib.MoeError(MOE_EINVAL, msg)
+
+
+def _tensor(t, name, dtypes, dims):
+    torch = _t()
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _bad(f"{name} must be a tensor in GPU memory")
+    if t.dtype not in dtypes:
+        _bad(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if t.dim() not in dims:
+        _bad(f"{name} must have {' or '.join(str(d) for d in dims)} dimensions, got {t.dim()}")
+    return t
+
+
+def _row_stride(t, name):
+    """Elements between the rows of t's last two dimensions."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        _bad(f"{name}: a row's elements must be contiguous")
+    ld = t.stride(-2)
+    if t.shape[-2] <= 1:
+        ld = max(ld, t.shape[-1])
+    if ld < t.shape[-1]:
+        _bad(f"{name}: rows must not overlap")
+    return ld
+
+
+def _rows(t, name, dtypes):
+    """A 2-D tensor of rows: (pointer, row stride)."""
+    _tensor(t, name, dtypes, (2,))
+    if t.shape[0] > 2**31 - 1 or t.shape[1] > 2**31 - 1:
+        _bad(f"{name}: sizes must fit 32 bits")
+    return t.data_ptr(), _row_stride(t, name)
+
+
+def _matrices(t, name, dtypes):
+    """(E, a, b) or (a, b): (E, a, b, row stride, matrix stride)."""
+    _tensor(t, name, dtypes, (2, 3))
+    E = t.shape[0] if t.dim() == 3 else 1
+    a, b = t.shape[-2], t.shape[-1]
+    ld = _row_stride(t, name)
+    stride = t.stride(0) if t.dim() == 3 and E > 1 else 0
+    if E > 1 and stride < (a - 1) * ld + b:
+        _bad(f"{name}: matrices must not overlap")
+    return E, a, b, ld, stride
+
+
+def _offsets(offsets, E):
+    if offsets is None:
+        if E != 1:
+            _bad("offsets are needed for more than one expert")
+        return None
+    torch = _t()
+    _tensor(offsets, "offsets", (torch.int32,), (1,))
+    if offsets.shape[0] != E + 1 or not offsets.is_contiguous():
+        _bad(f"offsets must be {E + 1} contiguous int32")
+    return offsets.data_ptr()
+
+
+def _same_device(*tensors):
+    first = None
+    for t in tensors:
+        if t is None:
+            continue
+        if first is None:
+            first = t.device
+        elif t.device != first:
+            _bad("tensors must be on one device")
+    return first
+
+
+def _call(fn, device, *args):
+    """The library call on `device`'s current stream (its last argument)."""
+    torch = _t()
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _call(fn, device, *args)
+    _lib.check(fn(*args, torch.cuda.current_stream().cuda_stream))
+
+
+def _layout(layout):
+    if layout not in (MOE_LAYOUT_LLAMA_IN_OUT, MOE_LAYOUT_FLUX_OUT_IN):
+        _bad("unknown layout")
+    return layout == MOE_LAYOUT_FLUX_OUT_IN
+
+
+def _result(out, shape, dtype, dtypes, like, clear):
+    """The caller's `out`, checked, or a new tensor (zeros where a call may
+    leave elements unwritten)."""
+    torch = _t()
+    if out is None:
+        if dtype not in dtypes:
+            _bad(f"the result must be {' or '.join(str(d) for d in dtypes)}, got {dtype}")
+        return (torch.zeros if clear else torch.empty)(shape, dtype=dtype, device=like.device)
+    _tensor(out, "out", dtypes, (len(shape),))
+    if tuple(out.shape) != tuple(shape):
+        _bad(f"out must be {tuple(shape)}, got {tuple(out.shape)}")
+    if dtype is not None and out.dtype != dtype:
+        _bad("out and out_dtype differ")
+    return out
+
+
+def _float_types(dtype):
+    torch = _t()
+    return (torch.float32,) if dtype == torch.float32 else (torch.bfloat16, torch.float32)
+
+
+def _rows_product(fn, x, name, w, offsets, layout, out, out_dtype, grad):
+    torch = _t()
+    xp, ldx = _rows(x, name, (torch.float32, torch.bfloat16))
+    E, a, b, ldw, stride = _matrices(w, "w", (x.dtype,))
+    in_dim, out_dim = (a, b) if _layout(layout) else (b, a)
+    k, n = (out_dim, in_dim) if grad else (in_dim, out_dim)
+    if x.shape[1] != k:
+        _bad(f"{name} has {x.shape[1]} columns, the weights take {k}")
+    if out is None and out_dtype is None:
+        out_dtype = x.dtype
+    out = _result(out, (x.shape[0], n), out_dtype, _float_types(x.dtype), x, offsets is not None)
+    device = _same_device(x, w, offsets, out)
+    _call(fn, device, xp, ldx, w.data_ptr(), ldw, stride, layout, _offsets(offsets, E), E, x.shape[0], in_dim, out_dim,
+          _codes[x.dtype], out.data_ptr(), _row_stride(out, "out"), _codes[out.dtype])
+    return out
+
+
+def grouped_matmul(x, w, offsets=None, *, layout=MOE_LAYOUT_LLAMA_IN_OUT, out=None, out_dtype=None):
+    """y[r] = W_e x[r] for the rows r of expert e: x (M, in) float32 or
+    bfloat16, w of the same type; sums in float32, the result in x's type or,
+    for bfloat16, ``out_dtype=torch.float32``.  Without ``out`` rows outside
+    every group are zeros."""
+    return _rows_product(_lib.lib().moe_grouped_matmul_async, x, "x", w, offsets, layout, out, out_dtype, False)
+
+
+def grouped_matmul_grad_x(dy, w, offsets=None, *, layout=MOE_LAYOUT_LLAMA_IN_OUT, out=None, out_dtype=None):
+    """The gradient of grouped_matmul with respect to x: dx[r] = W_e' dy[r]."""
+    return _rows_product(_lib.lib().moe_grouped_matmul_grad_x_async, dy, "dy", w, offsets, layout, out, out_dtype,
+                         True)
+
+
+def grouped_matmul_grad_w(x, dy, offsets=None, *, layout=MOE_LAYOUT_LLAMA_IN_OUT, out=None, out_dtype=None,
+                          accumulate=False):
+    """The gradient of grouped_matmul with respect to w, in ``layout``: for each
+    expert the sum over its rows of dy[r] x[r]'; zeros for an expert without
+    rows.  ``accumulate`` adds to what ``out`` holds (in float32, rounded
+    once)."""
+    torch = _t()
+    L = _lib.lib()
+    xp, ldx = _rows(x, "x", (torch.float32, torch.bfloat16))
+    dp, lddy = _rows(dy, "dy", (x.dtype,))
+    if x.shape[0] != dy.shape[0]:
+        _bad("x and dy must have the same rows")
+    if accumulate and out is None:
+        _bad("accumulate needs out")
+    E = 1 if offsets is None else _tensor(offsets, "offsets", (torch.int32,), (1,)).shape[0] - 1
+    if E < 1:
+        _bad("offsets must hold at least two row numbers")
+    a, b = (x.shape[1], dy.shape[1]) if _layout(layout) else (dy.shape[1], x.shape[1])
+    if out is None and out_dtype is None:
+        out_dtype = x.dtype
+    shape = (a, b) if (out.dim() == 2 if out is not None else offsets is None) and E == 1 else (E, a, b)
+    out = _result(out, shape, out_dtype, _float_types(x.dtype), x, False)
+    _, _, _, ldw, stride = _matrices(out, "out", _float_types(x.dtype))
+    device = _same_device(x, dy, offsets, out)
+    need = ctypes.c_int64(0)
+    _lib.check(L.moe_grouped_matmul_grad_w_workspace(E, x.shape[0], x.shape[1], dy.shape[1], ctypes.byref(need)))
+    ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    _call(L.moe_grouped_matmul_grad_w_async, device, xp, ldx, dp, lddy, layout, _offsets(offsets, E), E, x.shape[0],
+          x.shape[1], dy.shape[1], _codes[x.dtype], out.data_ptr(), ldw, stride, _codes[out.dtype], int(accumulate),
+          ws.data_ptr() if ws is not None else None, need.value)
+    return out
+
+
+def quantize_int8(x):
+    """int8 codes with a scale per row: x (..., cols) float32 or bfloat16 ->
+    (codes int8 of x's shape, scales float32 (...)).  scale = max|row| / 127,
+    code = 127 x / max|row| rounded to nearest even; a row of zeros has scale 0,
+    one that holds an infinity or a NaN scale NaN.  Of a weight (E, out, in)
+    this gives the codes and scales that int8_matmul takes."""
+    torch = _t()
+    _tensor(x, "x", (torch.float32, torch.bfloat16), range(1, 9))
+    x2 = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
+    if x2.shape[1] < 1:
+        _bad("x has no columns")
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    _call(_lib.lib().moe_quantize_int8_async, x.device, x2.data_ptr(), _row_stride(x2, "x"), _codes[x.dtype],
+          x2.shape[0], x2.shape[1], q.data_ptr(), x2.shape[1], scale.data_ptr())
+    return q, scale
+
+
+def int8_matmul(x, w, w_scale, offsets=None, *, x_scale=None, out=None, out_dtype=None):
+    """y[r][n] = x_scale[r] w_scale[e][n] sum_k q[r][k] w[e][n][k], the sum exact
+    in int32.  x (M, in): int8 codes with ``x_scale`` (M,), or float32 /
+    bfloat16 rows, which are quantised as quantize_int8 does; w (E, out, in) int8
+    and w_scale (E, out) float32 from quantize_int8.  The result is bfloat16 or,
+    with ``out_dtype``, float32; without ``out`` rows outside every group are
+    zeros."""
+    torch = _t()
+    L = _lib.lib()
+    xp, ldx = _rows(x, "x", (torch.float32, torch.bfloat16, torch.int8))
+    E, n, k, ldw, stride = _matrices(w, "w", (torch.int8,))
+    if x.shape[1] != k:
+        _bad(f"x has {x.shape[1]} columns, the weights take {k}")
+    _tensor(w_scale, "w_scale", (torch.float32,), (w.dim() - 1,))
+    if tuple(w_scale.shape) != tuple(w.shape[:-1]) or not w_scale.is_contiguous():
+        _bad(f"w_scale must be contiguous {tuple(w.shape[:-1])}")
+    codes = x.dtype == torch.int8
+    if codes != (x_scale is not None):
+        _bad("x_scale belongs to int8 rows")
+    if codes:
+        _tensor(x_scale, "x_scale", (torch.float32,), (1,))
+        if x_scale.shape[0] != x.shape[0] or not x_scale.is_contiguous():
+            _bad("x_scale must be contiguous with one scale per row")
+    if out is None and out_dtype is None:
+        out_dtype = torch.bfloat16
+    out = _result(out, (x.shape[0], n), out_dtype, (torch.bfloat16, torch.float32), x, offsets is not None)
+    device = _same_device(x, w, w_scale, x_scale, offsets, out)
+    need, ws = ctypes.c_int64(0), None
+    if not codes:
+        _lib.check(L.moe_int8_matmul_workspace(x.shape[0], k, ctypes.byref(need)))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=device)
+    _call(L.moe_int8_matmul_async, device, xp, ldx, _codes[x.dtype], x_scale.data_ptr() if codes else None,
+          w.data_ptr(), ldw, stride, w_scale.data_ptr(), _offsets(offsets, E), E, x.shape[0], k, n, out.data_ptr(),
+          _row_stride(out, "out"), _codes[out.dtype], ws.data_ptr() if ws is not None else None, need.value)
+    return out
+
+
+def _dense(t, name, dtypes, shape):
+    """A contiguous tensor of the given shape, or None."""
+    if t is None:
+        return None
+    _tensor(t, name, dtypes, range(1, 9))
+    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        _bad(f"{name} must be contiguous {tuple(shape)}, got {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _norm_params(D, T, pre_weight, post_weight, gate):
+    """Checks shared by block_norm and its gradient: (weights' type code, gate's
+    type code, rows per gate row)."""
+    torch = _t()
+    floats = (torch.float32, torch.bfloat16)
+    for w, name in ((pre_weight, "pre_weight"), (post_weight, "post_weight")):
+        _dense(w, name, floats, (D,))
+    given = [w for w in (pre_weight, post_weight) if w is not None]
+    if len(given) == 2 and given[0].dtype != given[1].dtype:
+        _bad("pre_weight and post_weight must have one type")
+    rows = 0
+    if gate is not None:
+        _tensor(gate, "gate", floats, (1, 2))
+        gates = gate.shape[0] if gate.dim() == 2 else 1
+        if gate.shape[-1] != D or not gate.is_contiguous():
+            _bad(f"gate must be contiguous (gates, {D}) or ({D},)")
+        if gates < 1 or T % gates:
+            _bad(f"{T} rows do not divide among {gates} gate rows")
+        rows = max(1, T // gates)
+    return _codes[given[0].dtype] if given else _lib.MOE_F32, _codes[gate.dtype] if gate is not None else 0, rows
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def block_norm(x, y=None, *, pre_weight=None, post_weight=None, gate=None, alpha=1.0, beta=1.0, eps=1e-5,
+               h_dtype=None):
+    """The norms before and after a block with its gate and the residual:
+
+        z = y * rstd(y) * post_weight     (without post_weight: y)
+        r = alpha x + beta gate * z       (without gate: 1; without y: alpha x)
+        h = r * rstd(r) * pre_weight      (without pre_weight: no h)
+
+    over the last dimension D (at most 16384), rstd(v) = 1 / sqrt(mean(v^2) +
+    eps).  x (..., D) is the residual stream, y the block's output, r the stream
+    after it and h what the next block reads, in ``h_dtype`` (x's type if not
+    given); float32 or bfloat16 each.  gate (D,), or (G, D) with each of its
+    rows for the next T / G of the T rows.  Returns (r, h, stats); stats (T, 2)
+    is what block_norm_grad needs.  Without y and with alpha 1 r is x."""
+    torch = _t()
+    floats = (torch.float32, torch.bfloat16)
+    _tensor(x, "x", floats, range(1, 9))
+    D = x.shape[-1]
+    if D < 1:
+        _bad("x has no channels")
+    T = x.numel() // D
+    xp = _dense(x, "x", floats, x.shape)
+    yp = _dense(y, "y", floats, x.shape)
+    if y is None and (post_weight is not None or gate is not None):
+        _bad("post_weight and gate need y")
+    if y is None and pre_weight is None:
+        _bad("nothing to compute: give y or pre_weight")
+    wt, gt, gate_rows = _norm_params(D, T, pre_weight, post_weight, gate)
+    h_dtype = x.dtype if h_dtype is None else h_dtype
+    if h_dtype not in floats:
+        _bad("h_dtype must be float32 or bfloat16")
+    device = _same_device(x, y, pre_weight, post_weight, gate)
+    r = x if y is None and alpha == 1.0 else torch.empty_like(x)
+    h = torch.empty(x.shape, dtype=h_dtype, device=device) if pre_weight is not None else None
+    stats = torch.empty((T, 2), dtype=torch.float32, device=device)
+    _call(_lib.lib().moe_block_norm_async, device, xp, _codes[x.dtype], yp, _codes[y.dtype] if y is not None else 0,
+          _ptr(post_weight), _ptr(pre_weight), wt, _ptr(gate), gt, gate_rows, alpha, beta, eps, T, D,
+          None if r is x else r.data_ptr(), _ptr(h), _codes[h_dtype], stats.data_ptr())
+    return r, h, stats
+
+
+def block_norm_grad(dr, dh, r, y=None, stats=None, *, pre_weight=None, post_weight=None, gate=None, alpha=1.0,
+                    beta=1.0):
+    """Gradients of block_norm from dr and dh (None: 0), with its r and stats:
+    (dx, dy, dgate, dpost, dpre), None for what the call does not have; dx in
+    r's type, dy in y's, the others float32."""
+    torch = _t()
+    L = _lib.lib()
+    floats = (torch.float32, torch.bfloat16)
+    _tensor(r, "r", floats, range(1, 9))
+    D = r.shape[-1]
+    if D < 1:
+        _bad("r has no channels")
+    T = r.numel() // D
+    rp = _dense(r, "r", floats, r.shape)
+    drp = _dense(dr, "dr", (r.dtype,), r.shape)
+    dhp = _dense(dh, "dh", floats, r.shape)
+    yp = _dense(y, "y", floats, r.shape)
+    sp = _dense(stats, "stats", (torch.float32,), (T, 2))
+    if dr is None and dh is None:
+        _bad("dr or dh is needed")
+    if (dh is not None) != (pre_weight is not None):
+        _bad("dh and pre_weight come together")
+    if y is None and (post_weight is not None or gate is not None):
+        _bad("post_weight and gate need y")
+    if stats is None and (pre_weight is not None or post_weight is not None):
+        _bad("stats are needed")
+    wt, gt, gate_rows = _norm_params(D, T, pre_weight, post_weight, gate)
+    device = _same_device(dr, dh, r, y, stats, pre_weight, post_weight, gate)
+    new = lambda shape: torch.empty(shape, dtype=torch.float32, device=device)
+    dx = torch.empty_like(r)
+    dy = torch.empty_like(y) if y is not None else None
+    dgate = new(gate.shape) if gate is not None else None
+    dpost = new(D) if post_weight is not None else None
+    dpre = new(D) if pre_weight is not None else None
+    need, ws = ctypes.c_int64(0), None
+    _lib.check(L.moe_block_norm_grad_workspace(T, D, gate_rows, ctypes.byref(need)))
+    if need.value and (dgate is not None or dpost is not None or dpre is not None):
+        ws = torch.empty(need.value, dtype=torch.uint8, device=device)
+    _call(L.moe_block_norm_grad_async, device, drp, dhp, rp, _codes[r.dtype], yp, _codes[y.dtype] if y is not None else 0,
+          _codes[dh.dtype] if dh is not None else 0, sp, _ptr(post_weight), _ptr(pre_weight), wt, _ptr(gate), gt,
+          gate_rows, alpha, beta, T, D, dx.data_ptr(), _ptr(dy), _ptr(dgate), _ptr(dpost), _ptr(dpre), _ptr(ws),
+          need.value)
+    return dx, dy, dgate, dpost, dpre

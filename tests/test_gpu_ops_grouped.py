@@ -1,0 +1,226 @@
+"""The grouped products and their gradients (grouped_matmul*, ops.py) against
+float64 products of the same inputs.
+
+Tolerance per element: K products summed in fp32 are off by at most K * 2^-23
+of the sum of their magnitudes (every addition rounds by at most one fp32 step,
+whatever the order or the rounding mode of the matrix unit), then one rounding
+to the result's type, at most half a step (2^-8 of a bf16 value, 2^-24 of an
+fp32 one)."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+FLUX, LLAMA = 0, 1
+SENTINEL = 776.0  # exact in bf16 and fp32
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def _rows(rng, rows, cols, dtype, pad, tail=0):
+    """rows + tail rows of a wider tensor; the padding columns and the rows
+    past the groups hold NaN."""
+    t = torch.full((rows + tail, cols + pad), float("nan"), dtype=DT[dtype])
+    t[:rows, :cols] = torch.from_numpy(rng.standard_normal((rows, cols))).to(DT[dtype])
+    return t.cuda()[:, :cols]
+
+
+def _mats(rng, E, a, b, dtype, pad):
+    t = torch.full((E, a, b + pad), float("nan"), dtype=DT[dtype])
+    t[:, :, :b] = torch.from_numpy(rng.standard_normal((E, a, b))).to(DT[dtype])
+    return t.cuda()[:, :, :b]
+
+
+def _f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def _close(got, ref, mag, K, dtype):
+    tol = K * 2.0**-23 * mag + np.abs(ref) * {"bf16": 2.0**-8, "f32": 2.0**-24}[dtype] + 1e-35
+    bad = ~(np.abs(got - ref) <= tol)
+    assert not bad.any(), (int(bad.sum()), float(np.abs(got - ref).max()))
+
+
+def _offsets(lens, start=0):
+    return torch.tensor(np.concatenate([[start], start + np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+
+
+# group lengths, K, N: no rows, one row, odd sizes below, at and past the tiles' edges
+SHAPES = [
+    ([1], 1, 1),
+    ([0, 3, 0], 7, 5),
+    ([17, 0, 1, 64], 64, 96),
+    ([33, 130, 5, 0, 300], 200, 136),
+    ([16, 16, 31, 2], 129, 257),
+    ([70, 90, 65], 333, 72),
+    ([0, 0], 40, 24),
+    ([5] * 70, 96, 48),            # more groups than a wave has lanes
+    ([700, 0, 900, 500], 72, 2048),  # 128 x 128 tiles
+]
+
+
+@pytest.mark.parametrize("pad", [0, 8, 3])
+@pytest.mark.parametrize("layout", [LLAMA, FLUX])
+@pytest.mark.parametrize("dtype,odt", [("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32")])
+def test_rows_products(moe, dtype, odt, layout, pad):
+    for lens, K, N in SHAPES:
+        print(f"grouped rows {dtype}->{odt} layout={layout} pad={pad} lens={lens[:6]} K={K} N={N}", flush=True)
+        rng = np.random.default_rng([K, N, layout, pad])
+        M, E, tail = sum(lens), len(lens), 5
+        off = _offsets(lens)
+        shape = (N, K) if layout == LLAMA else (K, N)
+        w = _mats(rng, E, *shape, dtype, pad)
+        W = _f64(w) if layout == LLAMA else _f64(w).transpose(0, 2, 1)
+        for grad in (False, True):
+            src = _rows(rng, M, N if grad else K, dtype, pad, tail)
+            out = torch.full((M + tail, (K if grad else N) + pad), SENTINEL, dtype=DT[odt], device="cuda")
+            view = out[:, :K if grad else N]
+            fn = moe.grouped_matmul_grad_x if grad else moe.grouped_matmul
+            assert fn(src, w, off, layout=layout, out=view) is view
+            got, s, at = _f64(view), _f64(src), 0
+            for e, n in enumerate(lens):
+                m = W[e] if grad else W[e].T
+                a = s[at:at + n]
+                _close(got[at:at + n], a @ m, np.abs(a) @ np.abs(m), N if grad else K, odt)
+                at += n
+            # rows past the groups and columns past the rows stay as they were
+            assert (got[M:] == SENTINEL).all() and (_f64(out)[:, view.shape[1]:] == SENTINEL).all()
+
+
+@pytest.mark.parametrize("layout", [LLAMA, FLUX])
+def test_large_tiles(moe, layout):
+    # 256 x 256 tiles (both operand orders), ragged last tiles, K with a part stage
+    rng = np.random.default_rng(5)
+    lens, K, N = [2100, 1, 3000, 3400], 136, 4040
+    print(f"grouped 256-row tiles layout={layout}", flush=True)
+    shape = (N, K) if layout == LLAMA else (K, N)
+    w, x = _mats(rng, 4, *shape, "bf16", 0), _rows(rng, sum(lens), K, "bf16", 0)
+    y = moe.grouped_matmul(x, w, _offsets(lens), layout=layout)
+    dy = _rows(rng, sum(lens), N, "bf16", 0)
+    dx = moe.grouped_matmul_grad_x(dy, w, _offsets(lens), layout=layout)
+    W, X, D, at = _f64(w), _f64(x), _f64(dy), 0
+    for e, n in enumerate(lens):
+        m = W[e].T if layout == LLAMA else W[e]  # (K, N)
+        s = slice(at, at + n)
+        _close(_f64(y[s]), X[s] @ m, np.abs(X[s]) @ np.abs(m), K, "bf16")
+        _close(_f64(dx[s]), D[s] @ m.T, np.abs(D[s]) @ np.abs(m.T), N, "bf16")
+        at += n
+
+
+WSHAPES = [
+    ([1], 1, 1),
+    ([0, 3, 0], 7, 5),
+    ([17, 0, 1, 64], 64, 96),
+    ([33, 130, 5, 0, 300], 200, 136),
+    ([129, 65, 0], 333, 71),
+    ([100, 40, 0, 64], 1024, 1024),           # 128 x 128 tiles
+    ([70, 0, 64, 1, 200, 66, 2, 30], 2048, 2040),  # 256 x 256 tiles
+    ([3000], 96, 40),                          # a long sum for few tiles
+    ([2500, 0, 4000], 64, 64),
+]
+
+
+@pytest.mark.parametrize("pad", [0, 8, 3])
+@pytest.mark.parametrize("layout", [LLAMA, FLUX])
+@pytest.mark.parametrize("dtype,odt", [("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32")])
+def test_weight_gradient(moe, dtype, odt, layout, pad):
+    for lens, K, N in WSHAPES:
+        print(f"grad_w {dtype}->{odt} layout={layout} pad={pad} lens={lens} K={K} N={N}", flush=True)
+        rng = np.random.default_rng([K, N, layout, pad, 1])
+        M, E, tail = sum(lens), len(lens), 3
+        x, dy = _rows(rng, M, K, dtype, pad, tail), _rows(rng, M, N, dtype, pad, tail)
+        off = _offsets(lens)
+        shape = (N, K) if layout == LLAMA else (K, N)
+        buf = torch.full((E, shape[0], shape[1] + pad), SENTINEL, dtype=DT[odt], device="cuda")
+        out = buf[:, :, :shape[1]]
+        moe.grouped_matmul_grad_w(x, dy, off, layout=layout, out=out)
+        a, b = (_f64(dy), _f64(x)) if layout == LLAMA else (_f64(x), _f64(dy))
+        got, at = _f64(out), 0
+        refs = []
+        for e, n in enumerate(lens):
+            s = slice(at, at + n)
+            ref, mag = a[s].T @ b[s], np.abs(a[s]).T @ np.abs(b[s])
+            refs.append((ref, mag))
+            _close(got[e], ref, mag, max(n, 1), odt)
+            at += n
+        assert (_f64(buf)[:, :, shape[1]:] == SENTINEL).all()
+        # accumulate: what out held, plus the sums (one more fp32 addition)
+        base = torch.from_numpy(rng.standard_normal((E, *shape))).to(DT[odt]).cuda()
+        acc = base.clone()
+        moe.grouped_matmul_grad_w(x, dy, off, layout=layout, out=acc, accumulate=True)
+        for e, (ref, mag) in enumerate(refs):
+            p = _f64(base)[e]
+            _close(_f64(acc)[e], ref + p, mag + np.abs(p), max(lens[e], 1) + 1, odt)
+
+
+def test_one_expert_and_defaults(moe):
+    rng = np.random.default_rng(8)
+    x, w, dy = _rows(rng, 50, 24, "bf16", 0), _mats(rng, 1, 40, 24, "bf16", 0), _rows(rng, 50, 40, "bf16", 0)
+    y = moe.grouped_matmul(x, w[0], out_dtype=torch.float32)
+    assert y.dtype == torch.float32 and y.shape == (50, 40)
+    X, W, D = _f64(x), _f64(w[0]), _f64(dy)
+    _close(_f64(y), X @ W.T, np.abs(X) @ np.abs(W.T), 24, "f32")
+    dw = moe.grouped_matmul_grad_w(x, dy)
+    assert dw.shape == (40, 24) and dw.dtype == torch.bfloat16
+    _close(_f64(dw), D.T @ X, np.abs(D.T) @ np.abs(X), 50, "bf16")
+    # rows outside every group, when the call makes the result: zeros
+    off = torch.tensor([10, 30], dtype=torch.int32, device="cuda")
+    y = moe.grouped_matmul(x, w, off)
+    assert (y[:10] == 0).all() and (y[30:] == 0).all() and (y[10:30] != 0).any()
+    # no rows at all
+    assert moe.grouped_matmul(x[:0], w, _offsets([0])).shape == (0, 40)
+    assert (moe.grouped_matmul_grad_w(x[:0], dy[:0], _offsets([0, 0])) == 0).all()
+
+
+def test_infinities_stay_in_their_rows(moe):
+    rng = np.random.default_rng(9)
+    x, w = _rows(rng, 200, 72, "bf16", 0), _mats(rng, 2, 72, 72, "bf16", 0)
+    x[5, 3], x[150, 71] = float("inf"), float("nan")
+    y = moe.grouped_matmul(x, w, _offsets([100, 100]))
+    fin = torch.isfinite(y).all(dim=1).cpu()
+    assert not fin[5] and not fin[150] and fin.sum() == 198
+
+
+def test_offsets_out_of_range_stay_in_bounds(moe):
+    # offsets past the rows are held within them: group 1 gets the rest, group 2 nothing
+    rng = np.random.default_rng(10)
+    x, w = _rows(rng, 40, 64, "bf16", 0), _mats(rng, 3, 64, 64, "bf16", 0)
+    good = moe.grouped_matmul(x, w, _offsets([16, 24, 0]))
+    off = torch.tensor([-5, 16, 1000, 2000], dtype=torch.int32, device="cuda")
+    assert torch.equal(moe.grouped_matmul(x, w, off), good)
+    dy = _rows(rng, 40, 64, "bf16", 0)
+    assert torch.equal(moe.grouped_matmul_grad_w(x, dy, off), moe.grouped_matmul_grad_w(x, dy, _offsets([16, 24, 0])))
+
+
+def test_streams_and_graph_replay(moe):
+    # the same bits on another stream and in every replay of a captured graph,
+    # with new inputs copied in between
+    rng = np.random.default_rng(11)
+    lens = [40, 0, 100, 77]
+    off = _offsets(lens)
+    xs = [_rows(rng, 217, 264, "bf16", 0) for _ in range(3)]
+    dys = [_rows(rng, 217, 136, "bf16", 0) for _ in range(3)]
+    w = _mats(rng, 4, 136, 264, "bf16", 0)
+
+    def step(x, dy):
+        return (moe.grouped_matmul(x, w, off), moe.grouped_matmul_grad_x(dy, w, off),
+                moe.grouped_matmul_grad_w(x, dy, off, out_dtype=torch.float32))
+
+    want = [step(x, dy) for x, dy in zip(xs, dys)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = step(xs[0], dys[0])
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+    x, dy = xs[0].clone(), dys[0].clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x, dy)
+    for i in (0, 1, 2, 1):
+        x.copy_(xs[i])
+        dy.copy_(dys[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[i])), i

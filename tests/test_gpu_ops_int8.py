@@ -1,0 +1,151 @@
+"""quantize_int8 and int8_matmul (ops.py) against their definition in float64.
+
+Codes: rne(127 x / max) in float64; for bf16 rows they have to be equal (a
+quotient is either a border, met exactly, or at least 2^-9 away from one), for
+fp32 rows within 2^-20 of a border either neighbour is right.  Products: the
+int32 sum is exact; its conversion to fp32 and the two scales round by at most
+2^-24 each (1e-6 relative bounds the four with room for the scale's own
+rounding), then one rounding to bf16 (2^-8)."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def _define(x):
+    """(codes before rounding, scale) in float64."""
+    a = np.abs(x).max(axis=-1, keepdims=True)
+    with np.errstate(all="ignore"):
+        v = np.where(a > 0, 127.0 * x / a, 0.0)
+    return v, a[..., 0] / 127.0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,cols,pad", [(1, 1, 0), (3, 7, 0), (5, 64, 8), (2, 255, 3), (9, 1000, 0), (4, 14336, 0),
+                                           (2, 20001, 0)])
+def test_quantize(moe, dtype, rows, cols, pad):
+    print(f"quantize {dtype} {rows}x{cols}+{pad}", flush=True)
+    rng = np.random.default_rng([rows, cols])
+    t = torch.full((rows, cols + pad), float("nan"), dtype=DT[dtype])
+    t[:, :cols] = torch.from_numpy(rng.standard_normal((rows, cols)) * 10.0 ** rng.integers(-3, 4, (rows, 1))).to(DT[dtype])
+    x = t.cuda()[:, :cols]
+    q, s = moe.quantize_int8(x)
+    v, sc = _define(t[:, :cols].double().numpy())
+    got = q.cpu().numpy().astype(np.float64)
+    if dtype == "bf16":
+        assert np.array_equal(got, np.round(v))
+    else:
+        assert (np.abs(got - v) <= 0.5 + 2.0**-20).all()
+    assert np.allclose(s.cpu().numpy(), sc, rtol=2.0**-23, atol=0)
+
+
+def test_quantize_borders_and_special_rows(moe):
+    # odd multiples of max / 254 are borders: half to even
+    n = np.arange(-254, 255, dtype=np.float32)
+    x = torch.from_numpy(np.stack([n, n * 2.0**100, n * 2.0**-100])).cuda()
+    q, _ = moe.quantize_int8(x)
+    assert all(np.array_equal(r, np.round(n / 2)) for r in q.cpu().numpy())
+    q, _ = moe.quantize_int8(x.to(torch.bfloat16))
+    assert np.array_equal(q.cpu().numpy()[0], np.round(n / 2))
+    x = torch.zeros(8, 300)
+    x[1, 7], x[2, 299] = float("inf"), float("nan")
+    x[3, :] = 3e38
+    x[4, 5] = 1e-45
+    x[5, 0], x[5, 1] = -1e-38, 1e-45
+    x[6] = torch.linspace(-3.4e38, 3.4e38, 300)
+    q, s = (t.cpu().numpy() for t in moe.quantize_int8(x.cuda()))
+    assert s[0] == 0 and (q[0] == 0).all()
+    assert np.isnan(s[1]) and np.isnan(s[2]) and (q[1] == 0).all() and (q[2] == 0).all()
+    assert (q[3] == 127).all() and q[4, 5] == 127 and q[5, 0] == -127 and q[5, 1] == 0
+    # linspace forms end - start = 6.8e38, past fp32: row 6 holds values that are not finite
+    assert not torch.isfinite(x[6]).all() and np.isnan(s[6]) and (q[6] == 0).all()
+    v = torch.linspace(-1, 1, 300) * 3.4e38  # 127 v overflows, v does not
+    q, s = (t.cpu().numpy() for t in moe.quantize_int8(v[None].cuda()))
+    ref = np.round(127.0 * v.double().numpy() / v.abs().max().double().item())
+    assert np.isfinite(s).all() and np.abs(q[0] - ref).max() <= 1 and q[0, 0] == -127 and q[0, -1] == 127
+    w = torch.randn(4, 6, 50, device="cuda")
+    q, s = moe.quantize_int8(w)  # a weight: a scale per output channel
+    q2, s2 = moe.quantize_int8(w.reshape(24, 50))
+    assert q.shape == w.shape and s.shape == (4, 6) and torch.equal(q.reshape(24, 50), q2) and torch.equal(s.reshape(-1), s2)
+
+
+# group lengths, K, N: streamed and tiled forms, odd sizes, long sums
+SHAPES = [
+    ([1], 1, 1),
+    ([0, 3, 0], 7, 5),
+    ([2], 4096, 130),
+    ([17, 0, 1, 64], 128, 96),
+    ([33, 130, 5, 0, 300], 208, 136),
+    ([16, 16, 40, 2], 129, 257),
+    ([100, 90, 65], 333, 72),
+    ([700, 0, 900, 500], 144, 2048),
+    ([3000, 5500], 160, 4112),
+    ([40, 30], 20000, 33),
+]
+
+
+@pytest.mark.parametrize("wpad", [0, 5])
+@pytest.mark.parametrize("xt,odt", [("bf16", "bf16"), ("f32", "f32"), ("codes", "f32")])
+def test_int8_matmul(moe, xt, odt, wpad):
+    for lens, K, N in SHAPES:
+        print(f"int8 {xt}->{odt} wpad={wpad} lens={lens} K={K} N={N}", flush=True)
+        rng = np.random.default_rng([K, N, wpad])
+        M, E, tail = sum(lens), len(lens), 2
+        off = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+        wb = torch.full((E, N, K + wpad), 99, dtype=torch.int8)
+        wb[:, :, :K] = torch.from_numpy(rng.integers(-127, 128, (E, N, K)).astype(np.int8))
+        w = wb.cuda()[:, :, :K]
+        ws = torch.from_numpy(rng.uniform(0.001, 0.02, (E, N)).astype(np.float32)).cuda()
+        if xt == "codes":
+            q = rng.integers(-128, 128, (M + tail, K)).astype(np.int8)
+            s = rng.uniform(0.001, 0.02, M + tail).astype(np.float32)
+            kw = dict(x_scale=torch.from_numpy(s).cuda())
+            x = torch.from_numpy(q).cuda()
+        else:
+            x = torch.from_numpy(rng.standard_normal((M + tail, K))).to(DT[xt]).cuda()
+            tq, ts = moe.quantize_int8(x)
+            q, s, kw = tq.cpu().numpy(), ts.cpu().numpy(), {}
+        out = torch.full((M + tail, N), 776.0, dtype=DT[odt], device="cuda")
+        moe.int8_matmul(x, w, ws, off, out=out, **kw)
+        got, W, at = out.cpu().double().numpy(), wb[:, :, :K].numpy().astype(np.float64), 0
+        for e, n in enumerate(lens):
+            r = slice(at, at + n)
+            ref = (q[r].astype(np.float64) @ W[e].T) * s[r, None].astype(np.float64) * ws[e].cpu().double().numpy()
+            tol = np.abs(ref) * (1e-6 + (2.0**-8 if odt == "bf16" else 0.0)) + 1e-37
+            assert (np.abs(got[r] - ref) <= tol).all(), float(np.abs(got[r] - ref).max())
+            at += n
+        assert (got[M:] == 776.0).all()
+
+
+def test_extreme_sums_are_exact(moe):
+    # the largest int32 sum the entry allows, of one sign
+    K = 131071
+    for rows in (1, 40):
+        x = torch.full((rows, K), -128, dtype=torch.int8, device="cuda")
+        w = torch.full((17, K), -128, dtype=torch.int8, device="cuda")
+        one = torch.ones(rows, device="cuda")
+        y = moe.int8_matmul(x, w, torch.ones(17, device="cuda"), x_scale=one, out_dtype=torch.float32)
+        assert (y == float(128 * 128 * K)).all()
+
+
+def test_nan_rows_and_graph(moe):
+    rng = np.random.default_rng(3)
+    x = torch.from_numpy(rng.standard_normal((70, 256))).to(torch.bfloat16).cuda()
+    w, ws = moe.quantize_int8(torch.from_numpy(rng.standard_normal((2, 80, 256)).astype(np.float32)).cuda())
+    off = torch.tensor([0, 30, 70], dtype=torch.int32, device="cuda")
+    want = [moe.int8_matmul(x * f, w, ws, off) for f in (1, 3, -2)]
+    buf = x.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = moe.int8_matmul(buf, w, ws, off)
+    for i, f in enumerate((1, 3, -2)):
+        buf.copy_(x * f)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[i])
+    x[4, 9], x[50, 1] = float("nan"), float("-inf")
+    fin = torch.isfinite(moe.int8_matmul(x, w, ws, off)).all(dim=1)
+    assert not fin[4] and not fin[50] and fin.sum() == 68

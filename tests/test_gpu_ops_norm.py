@@ -1,0 +1,268 @@
+"""block_norm and block_norm_grad (ops.py) against their formulas in float64,
+and the gradients against differences.
+
+Tolerances.  A sum over D channels in fp32 rounds by at most D 2^-24 of the sum
+of magnitudes, in a tree of at most 16 + log2 steps here: rstd, from a sum of
+squares of one sign, is good to 64 * 2^-24 =: E.  A forward value is a handful
+of products of such factors: E of each term's magnitude, then half a step of
+its type.  The reference takes the stored r (rounded to its type) as the kernel
+gave it, so that a rounding tie decided the other way is not counted twice."""
+import itertools
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+HALF = {"f32": 2.0**-24, "bf16": 2.0**-8}
+E = 64 * 2.0**-24
+ALPHA, BETA, EPS = 0.75, -1.5, 1e-5
+
+
+def _f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def _make(rng, shape, dt):
+    return torch.from_numpy(rng.standard_normal(shape)).to(DT[dt]).cuda()
+
+
+def _inputs(rng, T, D, xt, yt, wt, gates, pre, post, y=True):
+    w = lambda on: _make(rng, D, wt) if on else None
+    gate = None
+    if gates:
+        gate = _make(rng, (gates, D), xt)
+    return dict(x=_make(rng, (T, D), xt), y=_make(rng, (T, D), yt) if y else None, pre_weight=w(pre),
+                post_weight=w(post), gate=gate)
+
+
+def _rstd(v, on):
+    return (1.0 / np.sqrt((v * v).mean(axis=1, keepdims=True) + EPS)) if on else np.ones((v.shape[0], 1))
+
+
+def _terms(a):
+    """alpha x, beta gate z in float64."""
+    x = ALPHA * _f64(a["x"])
+    if a["y"] is None:
+        return x, np.zeros_like(x)
+    y = _f64(a["y"])
+    z = y * _rstd(y, a["post_weight"] is not None)
+    if a["post_weight"] is not None:
+        z = z * _f64(a["post_weight"])
+    if a["gate"] is not None:
+        z = z * np.repeat(_f64(a["gate"]), x.shape[0] // a["gate"].shape[0], axis=0)
+    return x, BETA * z
+
+
+def _check_forward(moe, a, xt, ht):
+    r, h, stats = moe.block_norm(a["x"], a["y"], pre_weight=a["pre_weight"], post_weight=a["post_weight"],
+                                 gate=a["gate"], alpha=ALPHA, beta=BETA, eps=EPS, h_dtype=DT[ht])
+    x, z = _terms(a)
+    tol = E * (np.abs(x) + np.abs(z)) + HALF[xt] * np.abs(x + z) + 1e-37
+    assert (np.abs(_f64(r) - (x + z)) <= tol).all()
+    if a["pre_weight"] is not None:
+        R = _f64(r)
+        ref = R * _rstd(R, True) * _f64(a["pre_weight"])
+        assert h.dtype == DT[ht]
+        assert (np.abs(_f64(h) - ref) <= (E + HALF[ht]) * np.abs(ref) + 1e-37).all()
+        assert np.allclose(_f64(stats)[:, 1:], _rstd(R, True), rtol=E, atol=0)
+    else:
+        assert h is None
+    if a["post_weight"] is not None:
+        assert np.allclose(_f64(stats)[:, :1], _rstd(_f64(a["y"]), True), rtol=E, atol=0)
+    return r, h, stats
+
+
+def _formula(a, dr, dh, r):
+    """(dx, dy, dgate, dpost, dpre), and the magnitudes that each one's terms have."""
+    T, D = r.shape
+    R, dr = _f64(r), _f64(dr) if dr is not None else np.zeros((T, D))
+    G, mG, dpre, mpre = dr, np.abs(dr), None, None
+    if a["pre_weight"] is not None:
+        w, ir = _f64(a["pre_weight"]), _rstd(R, True)
+        rh, t = R * ir, _f64(dh) * w
+        dpre, mpre = (_f64(dh) * rh).sum(0), np.abs(_f64(dh) * rh).sum(0)
+        G = dr + ir * (t - rh * (t * rh).mean(1, keepdims=True))
+        mG = np.abs(dr) + ir * (np.abs(t) + np.abs(rh) * np.abs(t * rh).mean(1, keepdims=True))
+    dx, mx = ALPHA * G, abs(ALPHA) * mG
+    if a["y"] is None:
+        return (dx, None, None, None, dpre), (mx, None, None, None, mpre)
+    post = a["post_weight"] is not None
+    y = _f64(a["y"])
+    iy = _rstd(y, post)
+    yh, wp = y * iy, _f64(a["post_weight"]) if post else np.ones(D)
+    u, mu = BETA * G, abs(BETA) * mG
+    dgate = mgate = None
+    dz, mz = u, mu
+    if a["gate"] is not None:
+        n = a["gate"].shape[0]
+        g = np.repeat(_f64(a["gate"]), T // n, axis=0)
+        dgate, mgate = (u * yh * wp).reshape(n, T // n, D).sum(1), (mu * np.abs(yh * wp)).reshape(n, T // n, D).sum(1)
+        dz, mz = u * g, mu * np.abs(g)
+    dpost = mpost = None
+    dy, my = dz, mz
+    if post:
+        dpost, mpost = (dz * yh).sum(0), (mz * np.abs(yh)).sum(0)
+        b, mb = dz * wp, mz * np.abs(wp)
+        dy = iy * (b - yh * (b * yh).mean(1, keepdims=True))
+        my = iy * (mb + np.abs(yh) * (mb * np.abs(yh)).mean(1, keepdims=True))
+    return (dx, dy, dgate, dpost, dpre), (mx, my, mgate, mpost, mpre)
+
+
+def _check_grad(moe, a, r, stats, dr, dh, xt, yt):
+    got = moe.block_norm_grad(dr, dh, r, a["y"], stats, pre_weight=a["pre_weight"], post_weight=a["post_weight"],
+                              gate=a["gate"], alpha=ALPHA, beta=BETA)
+    ref, mag = _formula(a, dr, dh, r)
+    # dx, dy: a few factors of E each, sums over D; the column sums over T rows
+    # add a rounding per row (at most T of them, in chunks)
+    T = r.shape[0]
+    for name, g, f, m, half in zip(("dx", "dy", "dgate", "dpost", "dpre"), got, ref, mag,
+                                   (HALF[xt], HALF[yt], 2.0**-24, 2.0**-24, 2.0**-24)):
+        if f is None:
+            assert g is None, name
+            continue
+        tol = (4 * E + (T * 2.0**-24 if name[1:] not in ("x", "y") else 0.0)) * m + half * np.abs(f) + 1e-37
+        bad = ~(np.abs(_f64(g).reshape(f.shape) - f) <= tol)
+        assert not bad.any(), (name, int(bad.sum()))
+    return got
+
+
+SIZES = [(1, 1), (3, 7), (1, 512), (5, 520), (4, 1000), (66, 96), (2, 2048), (3, 2056), (4, 4096), (2, 5000), (3, 8192),
+         (2, 9001), (6, 16384), (700, 64), (130, 1024)]
+
+
+@pytest.mark.parametrize("xt,yt,ht,wt", [("f32", "f32", "f32", "f32"), ("bf16", "f32", "bf16", "f32"),
+                                         ("bf16", "bf16", "bf16", "bf16"), ("f32", "bf16", "bf16", "f32"),
+                                         ("bf16", "bf16", "f32", "f32")])
+def test_sizes(moe, xt, yt, ht, wt):
+    for T, D in SIZES:
+        for gates in (0, 1, T):
+            print(f"norm {xt}/{yt}/{ht}/{wt} T={T} D={D} gates={gates}", flush=True)
+            rng = np.random.default_rng([T, D, gates])
+            a = _inputs(rng, T, D, xt, yt, wt, gates, True, True)
+            r, h, stats = _check_forward(moe, a, xt, ht)
+            _check_grad(moe, a, r, stats, _make(rng, (T, D), xt), _make(rng, (T, D), ht), xt, yt)
+
+
+def test_parts(moe):
+    # every combination of the optional parts, gates shared by 1, 2, 7 and 35 rows
+    T, D = 70, 72
+    for pre, post, gates, y, hasdr in itertools.product((True, False), (True, False), (0, 1, 2, 10, 35, 70), (True, False),
+                                                        (True, False)):
+        if not y and (post or gates or not pre) or not (hasdr or pre) or not (pre or y):
+            continue
+        print(f"norm parts pre={pre} post={post} gates={gates} y={y} dr={hasdr}", flush=True)
+        rng = np.random.default_rng(gates)
+        a = _inputs(rng, T, D, "bf16", "f32", "f32", gates, pre, post, y)
+        r, h, stats = _check_forward(moe, a, "bf16", "bf16")
+        dr = _make(rng, (T, D), "bf16") if hasdr else None
+        _check_grad(moe, a, r, stats, dr, _make(rng, (T, D), "bf16") if pre else None, "bf16", "f32")
+
+
+def test_long_gate_groups(moe):
+    # gate rows of many chunks each, a long sum over rows
+    for T, D, gates in ((20000, 64, 2), (9000, 512, 3), (4099, 136, 1), (6000, 32, 3000)):
+        print(f"norm long T={T} D={D} gates={gates}", flush=True)
+        rng = np.random.default_rng(T)
+        a = _inputs(rng, T, D, "f32", "f32", "f32", gates, True, True)
+        r, h, stats = _check_forward(moe, a, "f32", "f32")
+        _check_grad(moe, a, r, stats, _make(rng, (T, D), "f32"), _make(rng, (T, D), "f32"), "f32", "f32")
+
+
+def test_against_differences(moe):
+    # directional derivatives of a scalar of (r, h) in float64
+    rng = np.random.default_rng(4)
+    T, D = 6, 40
+    a = _inputs(rng, T, D, "f32", "f32", "f32", 2, True, True)
+    dr, dh = _make(rng, (T, D), "f32"), _make(rng, (T, D), "f32")
+    r, h, stats = _check_forward(moe, a, "f32", "f32")
+    grads = _check_grad(moe, a, r, stats, dr, dh, "f32", "f32")
+
+    def value(v):
+        y = v["y"] * _rstd(v["y"], True) * v["post_weight"] * np.repeat(v["gate"], 3, axis=0)
+        R = ALPHA * v["x"] + BETA * y
+        return (R * _f64(dr)).sum() + (R * _rstd(R, True) * v["pre_weight"] * _f64(dh)).sum()
+
+    base = {k: _f64(t) for k, t in a.items()}
+    for name, g in zip(("x", "y", "gate", "post_weight", "pre_weight"), grads):
+        for _ in range(3):
+            d = rng.standard_normal(base[name].shape)
+            step = 1e-5
+            up, down = ({**base, name: base[name] + s * step * d} for s in (1, -1))
+            slope = (value(up) - value(down)) / (2 * step)
+            scale = np.abs(_f64(g) * d).sum()
+            # differences: step^2 of the third derivative and 2^-52 / step of the value;
+            # the fp32 gradient: 4 E
+            assert abs((_f64(g) * d).sum() - slope) <= (4 * E + 1e-7) * scale + 1e-7, name
+
+
+def test_special_values_and_in_place(moe):
+    rng = np.random.default_rng(6)
+    a = _inputs(rng, 8, 64, "f32", "f32", "f32", 0, True, True)
+    a["y"][1], a["x"][2] = 0, 0
+    a["y"][2] = 0
+    a["y"][3, 5] = float("inf")
+    a["x"][4, 0] = float("nan")
+    r, h, _ = moe.block_norm(a["x"], a["y"], pre_weight=a["pre_weight"], post_weight=a["post_weight"])
+    fin = torch.isfinite(r).all(dim=1).cpu().numpy()
+    assert fin[[0, 1, 2, 5, 6, 7]].all() and not fin[3] and not fin[4]
+    assert torch.equal(r[1], a["x"][1]) and (h[2] == 0).all()  # a zero row stays zero
+    # r in the memory of x
+    from mixtureofexperts_amd import _lib
+
+    x = a["x"].clone()
+    hh = torch.empty_like(x)
+    _lib.check(_lib.lib().moe_block_norm_async(
+        x.data_ptr(), 0, a["y"].data_ptr(), 0, a["post_weight"].data_ptr(), a["pre_weight"].data_ptr(), 0, None, 0, 0, 1.0,
+        1.0, 1e-5, 8, 64, x.data_ptr(), hh.data_ptr(), 0, None, torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(x[[0, 1, 2, 5]], r[[0, 1, 2, 5]]) and torch.equal(hh[[0, 1, 2, 5]], h[[0, 1, 2, 5]])
+    # a first norm: r is x
+    r, h, _ = moe.block_norm(a["x"], pre_weight=a["pre_weight"])
+    assert r is a["x"] and torch.isfinite(h[0]).all()
+
+
+def test_no_rows(moe):
+    w = torch.ones(32, device="cuda")
+    x = torch.empty(0, 32, device="cuda")
+    r, h, stats = moe.block_norm(x, x, pre_weight=w, post_weight=w)
+    assert r.shape == h.shape == (0, 32) and stats.shape == (0, 2)
+    dx, dy, dgate, dpost, dpre = moe.block_norm_grad(x, x, r, x, stats, pre_weight=w, post_weight=w)
+    assert dx.shape == dy.shape == (0, 32) and dgate is None and (dpost == 0).all() and (dpre == 0).all()
+
+
+def test_unaligned_rows(moe):
+    # a view two elements into its buffer: 16-byte vectors do not fit
+    rng = np.random.default_rng(12)
+    a = _inputs(rng, 9, 128, "bf16", "bf16", "f32", 1, True, True)
+    want = moe.block_norm(a["x"], a["y"], pre_weight=a["pre_weight"], post_weight=a["post_weight"], gate=a["gate"])
+    flat = torch.empty(9 * 128 + 2, dtype=torch.bfloat16, device="cuda")
+    flat[2:] = a["x"].reshape(-1)
+    got = moe.block_norm(flat[2:].view(9, 128), a["y"], pre_weight=a["pre_weight"], post_weight=a["post_weight"],
+                         gate=a["gate"])
+    assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+
+def test_graph_replay(moe):
+    rng = np.random.default_rng(13)
+    T, D = 300, 512
+    sets = [_inputs(rng, T, D, "bf16", "f32", "f32", 3, True, True) for _ in range(3)]
+    dr, dh = _make(rng, (T, D), "bf16"), _make(rng, (T, D), "bf16")
+
+    def step(a):
+        kw = dict(pre_weight=a["pre_weight"], post_weight=a["post_weight"], gate=a["gate"], alpha=ALPHA, beta=BETA)
+        r, h, stats = moe.block_norm(a["x"], a["y"], **kw)
+        return (r, h) + moe.block_norm_grad(dr, dh, r, a["y"], stats, **kw)
+
+    want = [step(a) for a in sets]
+    buf = {k: v.clone() for k, v in sets[0].items()}
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(buf)
+    for i in (0, 2, 1, 2):
+        for k, v in sets[i].items():
+            buf[k].copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(u, v) for u, v in zip(out, want[i])), i

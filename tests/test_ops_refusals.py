@@ -1,0 +1,196 @@
+"""What the operators on device tensors refuse, at the C entry points and in
+the Python functions.  Every call here is refused on the host: the pointers
+are never read."""
+import ctypes
+
+import pytest
+
+P = 0x10000  # an aligned address that no refused call reads
+F32, BF16, FP8, INT8 = 0, 1, 2, 3
+FLUX, LLAMA = 0, 1
+
+ROWS = dict(x=P, ldx=64, w=P, ldw=64, w_stride=64 * 32, layout=LLAMA, offsets=P, groups=4, rows=10, in_dim=64, out_dim=32,
+            dtype=BF16, y=P, ldy=32, y_dtype=BF16, stream=None)
+
+
+def _refused(moe, fn, args, msg):
+    from mixtureofexperts_amd import _lib
+
+    rc = getattr(_lib.lib(), fn)(*args.values())
+    text = _lib.lib().moe_last_error(None).decode()
+    assert rc == _lib.MOE_EINVAL, (rc, args)
+    assert fn in text and msg in text, text
+
+
+@pytest.mark.parametrize("bad,msg", [
+    (dict(groups=0), "groups"), (dict(rows=-1), "rows"), (dict(in_dim=0), "dimensions"), (dict(out_dim=-3), "dimensions"),
+    (dict(offsets=None), "offsets"), (dict(dtype=FP8), "dtype"), (dict(dtype=7), "dtype"), (dict(y_dtype=FP8), "result"),
+    (dict(dtype=F32, y_dtype=BF16), "fp32"), (dict(layout=2), "layout"), (dict(ldx=63), "row stride"),
+    (dict(ldy=31), "row stride"), (dict(ldw=63), "row stride"), (dict(w_stride=64 * 31), "w_stride"),
+    (dict(x=None), "null"), (dict(w=None), "null"), (dict(y=None), "null"), (dict(x=P + 1), "aligned"),
+    (dict(w=P + 1), "aligned"), (dict(y=P + 1), "aligned"), (dict(y=P + 2, y_dtype=F32), "aligned"),
+])
+def test_grouped_matmul_refuses(moe, bad, msg):
+    _refused(moe, "moe_grouped_matmul_async", {**ROWS, **bad}, msg)
+
+
+@pytest.mark.parametrize("bad,msg", [(dict(ldx=31), "row stride"), (dict(ldy=63), "row stride"), (dict(dtype=FP8), "dtype"),
+                                     (dict(y=None), "null"), (dict(offsets=None), "offsets")])
+def test_grouped_matmul_grad_x_refuses(moe, bad, msg):
+    _refused(moe, "moe_grouped_matmul_grad_x_async", {**ROWS, "ldx": 32, "ldy": 64, **bad}, msg)
+
+
+GRADW = dict(x=P, ldx=64, dy=P, lddy=32, layout=LLAMA, offsets=P, groups=4, rows=10, in_dim=64, out_dim=32, dtype=BF16,
+             dw=P, lddw=64, dw_stride=64 * 32, dw_dtype=F32, accumulate=0, workspace=None, workspace_bytes=0, stream=None)
+
+
+@pytest.mark.parametrize("bad,msg", [
+    (dict(groups=0), "groups"), (dict(rows=-1), "rows"), (dict(offsets=None), "offsets"), (dict(dtype=INT8), "dtype"),
+    (dict(dtype=F32, dw_dtype=BF16), "fp32"), (dict(layout=-1), "layout"), (dict(ldx=63), "row stride"),
+    (dict(lddy=31), "row stride"), (dict(lddw=63), "row stride"), (dict(dw_stride=64 * 31), "dw_stride"),
+    (dict(x=None), "null"), (dict(dw=None), "null"), (dict(dw=P + 2), "aligned"), (dict(dy=P + 1), "aligned"),
+])
+def test_grouped_matmul_grad_w_refuses(moe, bad, msg):
+    _refused(moe, "moe_grouped_matmul_grad_w_async", {**GRADW, **bad}, msg)
+
+
+def test_grad_w_refuses_a_small_workspace(moe):
+    from mixtureofexperts_amd import _lib
+
+    L, n = _lib.lib(), ctypes.c_int64(-1)
+    # one group of many rows and a small matrix: its rows may be split over workgroups
+    assert L.moe_grouped_matmul_grad_w_workspace(1, 100000, 64, 64, ctypes.byref(n)) == 0 and n.value >= 0
+    if n.value:
+        args = {**GRADW, "groups": 1, "rows": 100000, "out_dim": 64, "lddy": 64, "lddw": 64}
+        for ws, size in ((None, n.value), (P, n.value - 1), (P + 8, n.value)):
+            _refused(moe, "moe_grouped_matmul_grad_w_async", {**args, "workspace": ws, "workspace_bytes": size},
+                     "workspace")
+    assert L.moe_grouped_matmul_grad_w_workspace(0, 1, 1, 1, ctypes.byref(n)) == _lib.MOE_EINVAL
+    assert L.moe_grouped_matmul_grad_w_workspace(1, 1, 1, 1, None) == _lib.MOE_EINVAL
+
+
+QUANT = dict(x=P, ldx=64, x_dtype=BF16, rows=4, cols=64, q=P, ldq=64, scale=P, stream=None)
+
+
+@pytest.mark.parametrize("bad,msg", [
+    (dict(x_dtype=INT8), "x_dtype"), (dict(rows=-1), "rows"), (dict(cols=0), "cols"), (dict(ldx=63), "row stride"),
+    (dict(ldq=63), "row stride"), (dict(x=None), "null"), (dict(q=None), "null"), (dict(scale=None), "null"),
+    (dict(x=P + 1), "aligned"), (dict(scale=P + 2), "aligned"), (dict(rows=2**31), "too many"),
+])
+def test_quantize_refuses(moe, bad, msg):
+    _refused(moe, "moe_quantize_int8_async", {**QUANT, **bad}, msg)
+
+
+INT8MM = dict(x=P, ldx=64, x_dtype=BF16, x_scale=None, w=P, ldw=64, w_stride=64 * 32, w_scale=P, offsets=P, groups=4,
+              rows=10, in_dim=64, out_dim=32, y=P, ldy=32, y_dtype=BF16, workspace=P, workspace_bytes=48 + 640, stream=None)
+
+
+@pytest.mark.parametrize("bad,msg", [
+    (dict(groups=0), "groups"), (dict(offsets=None), "offsets"), (dict(x_dtype=FP8), "x_dtype"), (dict(y_dtype=INT8), "result"),
+    (dict(in_dim=131072, ldx=131072, ldw=131072), "131071"), (dict(ldx=63), "row stride"), (dict(ldw=63), "row stride"),
+    (dict(ldy=31), "row stride"), (dict(w_stride=64 * 31), "w_stride"), (dict(w_scale=None), "null"),
+    (dict(x_dtype=INT8), "x_scale"), (dict(workspace=None), "workspace"), (dict(workspace=P + 8), "workspace"),
+    (dict(workspace_bytes=48 + 639), "workspace"), (dict(x=P + 1), "aligned"), (dict(w_scale=P + 2), "aligned"),
+])
+def test_int8_matmul_refuses(moe, bad, msg):
+    _refused(moe, "moe_int8_matmul_async", {**INT8MM, **bad}, msg)
+
+
+NORM = dict(x=P, x_dtype=BF16, y=P, y_dtype=F32, post=P, pre=P, w_dtype=F32, gate=P, gate_dtype=BF16, gate_rows=4,
+            alpha=1.0, beta=1.0, eps=1e-5, T=8, D=64, r=P, h=P, h_dtype=BF16, stats=P, stream=None)
+
+
+@pytest.mark.parametrize("bad,msg", [
+    (dict(x_dtype=FP8), "dtypes"), (dict(h_dtype=9), "dtypes"), (dict(T=-1), "T must"), (dict(D=0), "D must"),
+    (dict(D=16385), "D must"), (dict(gate_rows=0), "gate_rows"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"),
+    (dict(h=None), "come together"), (dict(pre=None), "come together"), (dict(y=None), "need y"), (dict(x=None), "null"),
+    (dict(r=None, h=None, pre=None), "null"), (dict(x=P + 1), "aligned"), (dict(stats=P + 2), "aligned"),
+    (dict(T=2**31), "too many"),
+])
+def test_block_norm_refuses(moe, bad, msg):
+    _refused(moe, "moe_block_norm_async", {**NORM, **bad}, msg)
+
+
+NORMG = dict(dr=P, dh=P, r=P, x_dtype=BF16, y=P, y_dtype=F32, h_dtype=BF16, stats=P, post=P, pre=P, w_dtype=F32, gate=P,
+             gate_dtype=BF16, gate_rows=8, alpha=1.0, beta=1.0, T=8, D=64, dx=P, dy=P, dgate=P, dpost=P, dpre=P,
+             workspace=P, workspace_bytes=2**30, stream=None)
+
+
+@pytest.mark.parametrize("bad,msg", [
+    (dict(x_dtype=INT8), "dtypes"), (dict(D=16385), "D must"), (dict(y=None), "need y"), (dict(gate=None), "dgate needs"),
+    (dict(post=None), "dpost needs"), (dict(pre=None), "dh needs"), (dict(dh=None), "dpre needs"),
+    (dict(dr=None, dh=None, dpre=None), "dr or dh"), (dict(r=None), "null"), (dict(stats=None), "null"),
+    (dict(workspace=None), "workspace"), (dict(workspace_bytes=16), "workspace"), (dict(workspace=P + 4), "workspace"),
+    (dict(dpost=P + 2), "aligned"), (dict(gate_rows=-1), "gate_rows"),
+])
+def test_block_norm_grad_refuses(moe, bad, msg):
+    _refused(moe, "moe_block_norm_grad_async", {**NORMG, **bad}, msg)
+
+
+def test_empty_calls_are_no_work(moe):
+    from mixtureofexperts_amd import _lib
+
+    L = _lib.lib()
+    assert L.moe_grouped_matmul_async(*{**ROWS, "rows": 0, "x": None, "y": None}.values()) == 0
+    assert L.moe_grouped_matmul_grad_x_async(*{**ROWS, "ldx": 32, "ldy": 64, "rows": 0, "x": None}.values()) == 0
+    assert L.moe_quantize_int8_async(*{**QUANT, "rows": 0, "x": None}.values()) == 0
+    assert L.moe_int8_matmul_async(*{**INT8MM, "rows": 0, "workspace": None}.values()) == 0
+    assert L.moe_block_norm_async(*{**NORM, "T": 0, "x": None}.values()) == 0
+    assert L.moe_grouped_matmul_grad_w_async(*{**GRADW, "rows": 0, "accumulate": 1}.values()) == 0
+
+
+def test_python_refuses_host_tensors(moe):
+    torch = pytest.importorskip("torch")
+    x, w = torch.zeros(4, 8), torch.zeros(2, 6, 8)
+    off = torch.zeros(3, dtype=torch.int32)
+    for call in (lambda: moe.grouped_matmul(x, w, off), lambda: moe.grouped_matmul_grad_x(x[:, :6], w, off),
+                 lambda: moe.grouped_matmul_grad_w(x, x, off), lambda: moe.quantize_int8(x),
+                 lambda: moe.int8_matmul(x, w.to(torch.int8), torch.zeros(2, 6), off),
+                 lambda: moe.block_norm(x, pre_weight=torch.ones(8)), lambda: moe.block_norm_grad(x, None, x)):
+        with pytest.raises(moe.MoeError, match="GPU memory"):
+            call()
+
+
+@pytest.mark.gpu
+def test_python_refuses(moe):
+    torch = pytest.importorskip("torch")
+    z = lambda *s, t=torch.bfloat16: torch.zeros(*s, dtype=t, device="cuda")
+    x, w, off = z(4, 8), z(2, 6, 8), z(3, t=torch.int32)
+    f32, i8, one = torch.float32, torch.int8, torch.ones(8, device="cuda")
+    calls = [
+        (lambda: moe.grouped_matmul(x.half(), w, off), "must be"),
+        (lambda: moe.grouped_matmul(x, w.float(), off), "must be"),
+        (lambda: moe.grouped_matmul(x, w), "offsets are needed"),
+        (lambda: moe.grouped_matmul(x, w, off.long()), "must be"),
+        (lambda: moe.grouped_matmul(x, w, off[:2]), "contiguous int32"),
+        (lambda: moe.grouped_matmul(x[:, :7], w, off), "columns"),
+        (lambda: moe.grouped_matmul(x.t(), w, off), "contiguous"),
+        (lambda: moe.grouped_matmul(z(1, 8).expand(4, 8), w, off), "overlap"),
+        (lambda: moe.grouped_matmul(x, z(1, 6, 8).expand(2, 6, 8), off), "overlap"),
+        (lambda: moe.grouped_matmul(x, w, off, layout=3), "layout"),
+        (lambda: moe.grouped_matmul(x, w, off, out=z(4, 7)), "out must be"),
+        (lambda: moe.grouped_matmul(x, w, off, out_dtype=i8), "result must be"),
+        (lambda: moe.grouped_matmul(x.float(), w.float(), off, out_dtype=torch.bfloat16), "result must be"),
+        (lambda: moe.grouped_matmul(x, w, off.cpu()), "one device"),
+        (lambda: moe.grouped_matmul_grad_w(x, z(5, 6), off), "same rows"),
+        (lambda: moe.grouped_matmul_grad_w(x, z(4, 6), off, accumulate=True), "needs out"),
+        (lambda: moe.grouped_matmul_grad_w(x, z(4, 6), off[:1]), "two row numbers"),
+        (lambda: moe.quantize_int8(z(4, 8, t=i8)), "must be"),
+        (lambda: moe.int8_matmul(x, z(2, 6, 8, t=i8), z(2, 5, t=f32), off), "w_scale"),
+        (lambda: moe.int8_matmul(z(4, 8, t=i8), z(2, 6, 8, t=i8), z(2, 6, t=f32), off), "x_scale"),
+        (lambda: moe.int8_matmul(x, z(2, 6, 8, t=i8), z(2, 6, t=f32), off, x_scale=z(4, t=f32)), "x_scale"),
+        (lambda: moe.block_norm(x), "nothing to compute"),
+        (lambda: moe.block_norm(x, post_weight=one), "need y"),
+        (lambda: moe.block_norm(x, x[:3], post_weight=one), "contiguous"),
+        (lambda: moe.block_norm(x, x, pre_weight=one, post_weight=one.bfloat16()), "one type"),
+        (lambda: moe.block_norm(x, x, gate=z(3, 8)), "do not divide"),
+        (lambda: moe.block_norm(x, x, gate=z(2, 7)), "gate must be"),
+        (lambda: moe.block_norm(z(2, 16392), pre_weight=z(16392, t=f32)), "16384"),
+        (lambda: moe.block_norm_grad(None, None, x), "dr or dh"),
+        (lambda: moe.block_norm_grad(x, x, x), "come together"),
+        (lambda: moe.block_norm_grad(x, x, x, pre_weight=one), "stats"),
+    ]
+    for i, (call, msg) in enumerate(calls):
+        with pytest.raises(moe.MoeError, match=msg):
+            call()
+            print("not refused:", i, flush=True)
