@@ -23,6 +23,7 @@ from ._lib import MOE_EINVAL, MOE_LAYOUT_FLUX_OUT_IN, MOE_LAYOUT_LLAMA_IN_OUT
 
 _torch = None
 _codes = {}
+_floats = []  # the types of float operands
 
 
 def _t():
@@ -32,6 +33,7 @@ def _t():
         import torch
 
         _torch = torch
+        _floats.extend((torch.float32, torch.bfloat16))
         _codes.update({torch.float32: _lib.MOE_F32, torch.bfloat16: _lib.MOE_BF16, torch.int8: _lib.MOE_INT8})
     return _torch
 
@@ -41,8 +43,7 @@ def _bad(msg):
 
 
 def _tensor(t, name, dtypes, dims):
-    torch = _t()
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    if not isinstance(t, _t().Tensor) or not t.is_cuda:
         _bad(f"{name} must be a tensor in GPU memory")
     if t.dtype not in dtypes:
         _bad(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
@@ -53,20 +54,21 @@ def _tensor(t, name, dtypes, dims):
 
 def _row_stride(t, name):
     """Elements between the rows of t's last two dimensions."""
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        _bad(f"{name}: a row's elements must be contiguous")
+    rows, cols = t.shape[-2:]
     ld = t.stride(-2)
-    if t.shape[-2] <= 1:
-        ld = max(ld, t.shape[-1])
-    if ld < t.shape[-1]:
-        _bad(f"{name}: rows must not overlap")
+    if cols > 1 and t.stride(-1) != 1:
+        _bad(f"{name}: a row's elements must be contiguous")
+    if ld < cols:
+        if rows > 1:
+            _bad(f"{name}: rows must not overlap")
+        ld = cols
     return ld
 
 
 def _rows(t, name, dtypes):
     """A 2-D tensor of rows: (pointer, row stride)."""
     _tensor(t, name, dtypes, (2,))
-    if t.shape[0] > 2**31 - 1 or t.shape[1] > 2**31 - 1:
+    if max(t.shape) > 2**31 - 1:
         _bad(f"{name}: sizes must fit 32 bits")
     return t.data_ptr(), _row_stride(t, name)
 
@@ -74,10 +76,12 @@ def _rows(t, name, dtypes):
 def _matrices(t, name, dtypes):
     """(E, a, b) or (a, b): (E, a, b, row stride, matrix stride)."""
     _tensor(t, name, dtypes, (2, 3))
-    E = t.shape[0] if t.dim() == 3 else 1
-    a, b = t.shape[-2], t.shape[-1]
+    a, b = t.shape[-2:]
     ld = _row_stride(t, name)
-    stride = t.stride(0) if t.dim() == 3 and E > 1 else 0
+    if t.dim() == 2:
+        return 1, a, b, ld, 0
+    E = t.shape[0]
+    stride = t.stride(0) if E > 1 else 0
     if E > 1 and stride < (a - 1) * ld + b:
         _bad(f"{name}: matrices must not overlap")
     return E, a, b, ld, stride
@@ -109,11 +113,14 @@ def _same_device(*tensors):
 
 def _call(fn, device, *args):
     """The library call on `device`'s current stream (its last argument)."""
-    torch = _t()
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
+    # torch's own binding: building a torch.cuda.Stream costs 3 us, as much as the launch
+    index, cuda = device.index, _torch._C
+    if index != cuda._cuda_getDevice():
+        with _torch.cuda.device(device):
             return _call(fn, device, *args)
-    _lib.check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    status = fn(*args, cuda._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status)
 
 
 def _layout(layout):
@@ -125,13 +132,13 @@ def _layout(layout):
 def _result(out, shape, dtype, dtypes, like, clear):
     """The caller's `out`, checked, or a new tensor (zeros where a call may
     leave elements unwritten)."""
-    torch = _t()
+    torch = _torch
     if out is None:
         if dtype not in dtypes:
             _bad(f"the result must be {' or '.join(str(d) for d in dtypes)}, got {dtype}")
         return (torch.zeros if clear else torch.empty)(shape, dtype=dtype, device=like.device)
     _tensor(out, "out", dtypes, (len(shape),))
-    if tuple(out.shape) != tuple(shape):
+    if out.shape != shape:
         _bad(f"out must be {tuple(shape)}, got {tuple(out.shape)}")
     if dtype is not None and out.dtype != dtype:
         _bad("out and out_dtype differ")
@@ -139,13 +146,13 @@ def _result(out, shape, dtype, dtypes, like, clear):
 
 
 def _float_types(dtype):
-    torch = _t()
-    return (torch.float32,) if dtype == torch.float32 else (torch.bfloat16, torch.float32)
+    """The results that operands of dtype may have."""
+    return (dtype,) if dtype == _torch.float32 else _floats
 
 
 def _rows_product(fn, x, name, w, offsets, layout, out, out_dtype, grad):
-    torch = _t()
-    xp, ldx = _rows(x, name, (torch.float32, torch.bfloat16))
+    _t()
+    xp, ldx = _rows(x, name, _floats)
     E, a, b, ldw, stride = _matrices(w, "w", (x.dtype,))
     in_dim, out_dim = (a, b) if _layout(layout) else (b, a)
     k, n = (out_dim, in_dim) if grad else (in_dim, out_dim)
@@ -182,7 +189,7 @@ def grouped_matmul_grad_w(x, dy, offsets=None, *, layout=MOE_LAYOUT_LLAMA_IN_OUT
     once)."""
     torch = _t()
     L = _lib.lib()
-    xp, ldx = _rows(x, "x", (torch.float32, torch.bfloat16))
+    xp, ldx = _rows(x, "x", _floats)
     dp, lddy = _rows(dy, "dy", (x.dtype,))
     if x.shape[0] != dy.shape[0]:
         _bad("x and dy must have the same rows")
@@ -214,7 +221,7 @@ def quantize_int8(x):
     one that holds an infinity or a NaN scale NaN.  Of a weight (E, out, in)
     this gives the codes and scales that int8_matmul takes."""
     torch = _t()
-    _tensor(x, "x", (torch.float32, torch.bfloat16), range(1, 9))
+    _tensor(x, "x", _floats, range(1, 9))
     x2 = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
     if x2.shape[1] < 1:
         _bad("x has no columns")
@@ -239,7 +246,7 @@ def int8_matmul(x, w, w_scale, offsets=None, *, x_scale=None, out=None, out_dtyp
     if x.shape[1] != k:
         _bad(f"x has {x.shape[1]} columns, the weights take {k}")
     _tensor(w_scale, "w_scale", (torch.float32,), (w.dim() - 1,))
-    if tuple(w_scale.shape) != tuple(w.shape[:-1]) or not w_scale.is_contiguous():
+    if w_scale.shape != w.shape[:-1] or not w_scale.is_contiguous():
         _bad(f"w_scale must be contiguous {tuple(w.shape[:-1])}")
     codes = x.dtype == torch.int8
     if codes != (x_scale is not None):
@@ -263,35 +270,34 @@ def int8_matmul(x, w, w_scale, offsets=None, *, x_scale=None, out=None, out_dtyp
 
 
 def _dense(t, name, dtypes, shape):
-    """A contiguous tensor of the given shape, or None."""
+    """The address of a contiguous tensor of the given shape (None of None)."""
     if t is None:
         return None
-    _tensor(t, name, dtypes, range(1, 9))
-    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if not (isinstance(t, _torch.Tensor) and t.is_cuda and t.dtype in dtypes and t.shape == shape and t.is_contiguous()):
+        _tensor(t, name, dtypes, range(1, 9))
         _bad(f"{name} must be contiguous {tuple(shape)}, got {tuple(t.shape)}")
     return t.data_ptr()
 
 
 def _norm_params(D, T, pre_weight, post_weight, gate):
-    """Checks shared by block_norm and its gradient: (weights' type code, gate's
-    type code, rows per gate row)."""
-    torch = _t()
-    floats = (torch.float32, torch.bfloat16)
-    for w, name in ((pre_weight, "pre_weight"), (post_weight, "post_weight")):
-        _dense(w, name, floats, (D,))
-    given = [w for w in (pre_weight, post_weight) if w is not None]
-    if len(given) == 2 and given[0].dtype != given[1].dtype:
-        _bad("pre_weight and post_weight must have one type")
-    rows = 0
-    if gate is not None:
-        _tensor(gate, "gate", floats, (1, 2))
-        gates = gate.shape[0] if gate.dim() == 2 else 1
-        if gate.shape[-1] != D or not gate.is_contiguous():
-            _bad(f"gate must be contiguous (gates, {D}) or ({D},)")
-        if gates < 1 or T % gates:
-            _bad(f"{T} rows do not divide among {gates} gate rows")
-        rows = max(1, T // gates)
-    return _codes[given[0].dtype] if given else _lib.MOE_F32, _codes[gate.dtype] if gate is not None else 0, rows
+    """Checks shared by block_norm and its gradient: the weights' addresses and
+    type code, the gate's address, type code and rows per gate row."""
+    shape = (D,)
+    pre, post = _dense(pre_weight, "pre_weight", _floats, shape), _dense(post_weight, "post_weight", _floats, shape)
+    wt = _lib.MOE_F32
+    if pre_weight is not None or post_weight is not None:
+        wt = _codes[(pre_weight if pre_weight is not None else post_weight).dtype]
+        if pre_weight is not None and post_weight is not None and pre_weight.dtype != post_weight.dtype:
+            _bad("pre_weight and post_weight must have one type")
+    if gate is None:
+        return pre, post, wt, None, 0, 0
+    _tensor(gate, "gate", _floats, (1, 2))
+    gates = gate.shape[0] if gate.dim() == 2 else 1
+    if gate.shape[-1] != D or not gate.is_contiguous():
+        _bad(f"gate must be contiguous (gates, {D}) or ({D},)")
+    if gates < 1 or T % gates:
+        _bad(f"{T} rows do not divide among {gates} gate rows")
+    return pre, post, wt, gate.data_ptr(), _codes[gate.dtype], max(1, T // gates)
 
 
 def _ptr(t):
@@ -313,29 +319,32 @@ def block_norm(x, y=None, *, pre_weight=None, post_weight=None, gate=None, alpha
     rows for the next T / G of the T rows.  Returns (r, h, stats); stats (T, 2)
     is what block_norm_grad needs.  Without y and with alpha 1 r is x."""
     torch = _t()
-    floats = (torch.float32, torch.bfloat16)
-    _tensor(x, "x", floats, range(1, 9))
-    D = x.shape[-1]
+    _tensor(x, "x", _floats, range(1, 9))
+    shape = x.shape
+    D = shape[-1]
     if D < 1:
         _bad("x has no channels")
     T = x.numel() // D
-    xp = _dense(x, "x", floats, x.shape)
-    yp = _dense(y, "y", floats, x.shape)
-    if y is None and (post_weight is not None or gate is not None):
-        _bad("post_weight and gate need y")
-    if y is None and pre_weight is None:
-        _bad("nothing to compute: give y or pre_weight")
-    wt, gt, gate_rows = _norm_params(D, T, pre_weight, post_weight, gate)
-    h_dtype = x.dtype if h_dtype is None else h_dtype
-    if h_dtype not in floats:
+    xp, yp = _dense(x, "x", _floats, shape), _dense(y, "y", _floats, shape)
+    if y is None:
+        if post_weight is not None or gate is not None:
+            _bad("post_weight and gate need y")
+        if pre_weight is None:
+            _bad("nothing to compute: give y or pre_weight")
+    pre, post, wt, gp, gt, gate_rows = _norm_params(D, T, pre_weight, post_weight, gate)
+    xt = x.dtype
+    h_dtype = xt if h_dtype is None else h_dtype
+    if h_dtype not in _floats:
         _bad("h_dtype must be float32 or bfloat16")
     device = _same_device(x, y, pre_weight, post_weight, gate)
     r = x if y is None and alpha == 1.0 else torch.empty_like(x)
-    h = torch.empty(x.shape, dtype=h_dtype, device=device) if pre_weight is not None else None
+    h = None
+    if pre is not None:
+        h = torch.empty_like(x) if h_dtype == xt else torch.empty(shape, dtype=h_dtype, device=device)
     stats = torch.empty((T, 2), dtype=torch.float32, device=device)
-    _call(_lib.lib().moe_block_norm_async, device, xp, _codes[x.dtype], yp, _codes[y.dtype] if y is not None else 0,
-          _ptr(post_weight), _ptr(pre_weight), wt, _ptr(gate), gt, gate_rows, alpha, beta, eps, T, D,
-          None if r is x else r.data_ptr(), _ptr(h), _codes[h_dtype], stats.data_ptr())
+    _call(_lib.lib().moe_block_norm_async, device, xp, _codes[xt], yp, _codes[y.dtype] if y is not None else 0, post, pre,
+          wt, gp, gt, gate_rows, alpha, beta, eps, T, D, None if r is x else r.data_ptr(), _ptr(h), _codes[h_dtype],
+          stats.data_ptr())
     return r, h, stats
 
 
@@ -346,16 +355,14 @@ def block_norm_grad(dr, dh, r, y=None, stats=None, *, pre_weight=None, post_weig
     r's type, dy in y's, the others float32."""
     torch = _t()
     L = _lib.lib()
-    floats = (torch.float32, torch.bfloat16)
-    _tensor(r, "r", floats, range(1, 9))
-    D = r.shape[-1]
+    _tensor(r, "r", _floats, range(1, 9))
+    shape = r.shape
+    D = shape[-1]
     if D < 1:
         _bad("r has no channels")
     T = r.numel() // D
-    rp = _dense(r, "r", floats, r.shape)
-    drp = _dense(dr, "dr", (r.dtype,), r.shape)
-    dhp = _dense(dh, "dh", floats, r.shape)
-    yp = _dense(y, "y", floats, r.shape)
+    rp, drp = _dense(r, "r", _floats, shape), _dense(dr, "dr", (r.dtype,), shape)
+    dhp, yp = _dense(dh, "dh", _floats, shape), _dense(y, "y", _floats, shape)
     sp = _dense(stats, "stats", (torch.float32,), (T, 2))
     if dr is None and dh is None:
         _bad("dr or dh is needed")
@@ -365,20 +372,20 @@ def block_norm_grad(dr, dh, r, y=None, stats=None, *, pre_weight=None, post_weig
         _bad("post_weight and gate need y")
     if stats is None and (pre_weight is not None or post_weight is not None):
         _bad("stats are needed")
-    wt, gt, gate_rows = _norm_params(D, T, pre_weight, post_weight, gate)
+    pre, post, wt, gp, gt, gate_rows = _norm_params(D, T, pre_weight, post_weight, gate)
     device = _same_device(dr, dh, r, y, stats, pre_weight, post_weight, gate)
-    new = lambda shape: torch.empty(shape, dtype=torch.float32, device=device)
     dx = torch.empty_like(r)
     dy = torch.empty_like(y) if y is not None else None
+    new = lambda size: torch.empty(size, dtype=torch.float32, device=device)
     dgate = new(gate.shape) if gate is not None else None
-    dpost = new(D) if post_weight is not None else None
-    dpre = new(D) if pre_weight is not None else None
+    dpost = new(D) if post is not None else None
+    dpre = new(D) if pre is not None else None
     need, ws = ctypes.c_int64(0), None
-    _lib.check(L.moe_block_norm_grad_workspace(T, D, gate_rows, ctypes.byref(need)))
-    if need.value and (dgate is not None or dpost is not None or dpre is not None):
-        ws = torch.empty(need.value, dtype=torch.uint8, device=device)
+    if dgate is not None or dpost is not None or dpre is not None:
+        _lib.check(L.moe_block_norm_grad_workspace(T, D, gate_rows, ctypes.byref(need)))
+        if need.value:
+            ws = torch.empty(need.value, dtype=torch.uint8, device=device)
     _call(L.moe_block_norm_grad_async, device, drp, dhp, rp, _codes[r.dtype], yp, _codes[y.dtype] if y is not None else 0,
-          _codes[dh.dtype] if dh is not None else 0, sp, _ptr(post_weight), _ptr(pre_weight), wt, _ptr(gate), gt,
-          gate_rows, alpha, beta, T, D, dx.data_ptr(), _ptr(dy), _ptr(dgate), _ptr(dpost), _ptr(dpre), _ptr(ws),
-          need.value)
+          _codes[dh.dtype] if dh is not None else 0, sp, post, pre, wt, gp, gt, gate_rows, alpha, beta, T, D,
+          dx.data_ptr(), _ptr(dy), _ptr(dgate), _ptr(dpost), _ptr(dpre), _ptr(ws), need.value)
     return dx, dy, dgate, dpost, dpre
