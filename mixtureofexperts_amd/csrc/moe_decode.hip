@@ -26,6 +26,7 @@
 #include "moe_decode.h"
 #include "moe_decode_batch.h"
 #include "moe_internal.h"
+#include "moe_ops_norm.h"
 #include "moe_ops_stream.h"
 
 namespace moe {

@@ -48,7 +48,6 @@
 #include <type_traits>
 
 #include "moe_internal.h"
-#include "moe_ops_gemm.h"
 
 namespace moe {
 
@@ -1208,13 +1207,6 @@ hipError_t launch_grouped_gemm_bf16(int mode, int bm, int wfp8, const GemmArgs &
     MOE_BF16_CASE(MODE_DOWN, 128, 1)
 #undef MOE_BF16_CASE
     return hipErrorInvalidValue;
-}
-
-hipError_t launch_op_gemm_bf16(bool, bool b_col, bool ragged_k, OpGemmArgs g, int ncu, hipStream_t s) {
-    if (ragged_k) return ops::op_gemm_plan<OT_BF16, true, true, true>(g, ncu, s);
-    if (b_col) return ops::op_gemm_plan<OT_BF16, false, true, false>(g, ncu, s);
-    if (op_stream_fits(OT_BF16, g)) return launch_op_stream(OT_BF16, g, s);
-    return ops::op_gemm_plan<OT_BF16, false, false, false>(g, ncu, s);
 }
 
 }  // namespace moe

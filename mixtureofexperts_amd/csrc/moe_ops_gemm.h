@@ -307,16 +307,64 @@ __device__ __forceinline__ bool ragged_job(const OpGemmArgs &g, OpJob &jb, int B
     return false;
 }
 
-// Weight gradient: tiles of every group's matrix, group-major, then blocks of
-// kOpMBlock M tiles, n tile, M tile, and the ranges of a split group.
+// The group of the r-th longest length (ties by index), with its rows.  Up to
+// 512 groups, held eight to a lane: the length is found by bisection over the
+// count of groups at least that long; more groups are taken in their order.
+__device__ __forceinline__ int longest_group(const OpGemmArgs &g, int r, int &lo, int &hi) {
+    int e = r;
+    if (g.E > 1 && g.E <= 512) {
+        const int lane = threadIdx.x & 63, n = (g.E + 63) >> 6;
+        int len[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            len[q] = -1;
+            if (q < n && q * 64 + lane < g.E) {
+                int a, b;
+                op_group(g.offsets, q * 64 + lane, g.rows, a, b);
+                len[q] = b - a;
+            }
+        }
+        auto count = [&](int t) {  // groups of at least t rows
+            int c = 0;
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (q < n) c += __popcll(__ballot(len[q] >= t));
+            return c;
+        };
+        int t = 0;
+        for (int bit = 1 << (31 - __clz(g.rows | 1)); bit > 0; bit >>= 1)
+            if (count(t | bit) > r) t |= bit;
+        int skip = r - count(t + 1);  // among the groups of exactly t rows
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            if (q >= n) break;
+            unsigned long long m = __ballot(len[q] == t);
+            const int c = __popcll(m);
+            if (skip >= 0 && skip < c) {
+                for (int k = 0; k < skip; ++k) m &= m - 1;
+                e = q * 64 + __ffsll((long long)m) - 1;
+            }
+            skip -= c;
+        }
+    }
+    op_group(g.offsets, e, g.rows, lo, hi);
+    return e;
+}
+
+// Weight gradient: tiles of the groups' matrices, the longest group first (a
+// tile's time is its group's rows).  A group's tiles are dealt to the 8 XCDs
+// in contiguous parts, so that every XCD has its share of every group: with
+// whole groups per XCD one long group kept one XCD busy while the others were
+// done (64 groups of 2048 x 1408 over 49152 rows, Zipf lengths: 1000 us).
+// Within a group: ranges of its rows, blocks of kOpMBlock M tiles, n tile, M tile.
 __device__ __forceinline__ bool matrix_job(const OpGemmArgs &g, OpJob &jb, int BM, int BN, int KE) {
-    const int per_group = g.mt * g.nt * g.splits;
-    const int W = g.E * per_group;
-    const int per = (W + 7) >> 3, slot = blockIdx.x >> 3;
-    int item = (blockIdx.x & 7) * per + slot;
-    if (slot >= per || item >= W) return false;
-    jb.e = item / per_group;
-    item -= jb.e * per_group;
+    const int T = g.mt * g.nt * g.splits, part = (T + 7) >> 3;
+    const int slot = blockIdx.x >> 3, r = slot / part;
+    if (r >= g.E) return false;
+    int item = (((int)blockIdx.x + r) & 7) * part + slot - r * part;
+    if (item >= T) return false;
+    int lo, hi;
+    jb.e = __builtin_amdgcn_readfirstlane(longest_group(g, r, lo, hi));
     jb.ks = item / (g.mt * g.nt);
     item -= jb.ks * (g.mt * g.nt);
     jb.nks = g.splits;
@@ -333,8 +381,6 @@ __device__ __forceinline__ bool matrix_job(const OpGemmArgs &g, OpJob &jb, int B
     }
     jb.m0 = m * BM;
     jb.n0 = n * BN;
-    int lo, hi;
-    op_group(g.offsets, jb.e, g.rows, lo, hi);
     if (jb.nks > 1) {  // equal ranges of whole stages
         const int chunk = ((hi - lo + jb.nks - 1) / jb.nks + KE - 1) / KE * KE;
         const int b = min(lo + jb.ks * chunk, hi);
@@ -592,9 +638,9 @@ hipError_t launch_tiles(OpGemmArgs g, bool direct, hipStream_t s) {
     g.nt = (g.N + BN - 1) / BN;
     g.mt = RAGK ? (g.M + BM - 1) / BM : 0;
     // ragged rows: sum of ceil(rows_e / BM) <= rows / BM + the groups that can hold a row
-    const long long mtiles = RAGK ? (long long)g.E * g.mt * g.splits
-                                  : (long long)(g.rows / BM) + (g.E < g.rows ? g.E : g.rows);
-    const long long grid = (mtiles * g.nt + 7) / 8 * 8;
+    // ragged k: every XCD's part of every group
+    const long long mtiles = (long long)(g.rows / BM) + (g.E < g.rows ? g.E : g.rows);
+    const long long grid = RAGK ? ((long long)g.mt * g.nt * g.splits + 7) / 8 * 8 * g.E : (mtiles * g.nt + 7) / 8 * 8;
     if (grid > 0x7fffffffll / (WM * WN * 64)) return hipErrorInvalidValue;
     const dim3 b(WM * WN * 64);
     if constexpr (BM == 256) {  // (staging through registers leaves too few for these tiles)
@@ -633,7 +679,9 @@ hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
     };
     const long long avg = RAGK ? g.M : (long long)g.rows / g.E;
     if constexpr (OT != OT_F32) {
-        if (direct && avg >= 192 && g.N >= 192 && tiles(256) >= 2 * ncu)
+        // ragged k: a group that holds most rows has to fill the GPU by itself
+        const bool large = RAGK ? tiles(256) >= g.E * (long long)(ncu / 2) : avg >= 192 && g.N >= 192 && tiles(256) >= 2 * ncu;
+        if (direct && large)
             return launch_tiles<OT, ACOL, BCOL, RAGK, 256, 256, 4, 2, 2>(g, direct, s);
     }
     if (avg >= 64 && g.N >= 64 && tiles(128) >= ncu)

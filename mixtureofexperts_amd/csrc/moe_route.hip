@@ -18,7 +18,6 @@
 #include <type_traits>
 
 #include "moe_internal.h"
-#include "moe_ops_norm.h"
 
 namespace moe {
 
