@@ -6,13 +6,15 @@
 //   forward / row gradient: A "row", B "row" or "col" by the weight's layout;
 //   weight gradient: A and B "col", k running over the group's rows.
 //
-// LDS.  A stage is 128 bytes of k per "row" operand row (64 bf16, 32 fp32,
-// 128 int8) and the same number of k rows of a "col" operand.  A lane's
-// fragment is 16 bytes of consecutive k of one row for every type, so one
-// loop serves bf16 (one MFMA per fragment pair), int8 (one) and fp32 (four,
-// element j of each lane's four: the k order inside a fragment is free as
-// long as both operands use the same).
-//   row operand: row r's 16-byte chunk c at slot c ^ ((r >> 1) & 7);
+// LDS.  A stage is 64 bytes of k per "row" operand row (32 bf16, 16 fp32, 64
+// int8) and the same number of k rows of a "col" operand.  A lane's fragment
+// is 16 bytes of consecutive k of one row for every type, so one loop serves
+// bf16 (one MFMA per fragment pair), int8 (one) and fp32 (four, element j of
+// each lane's four: the k order inside a fragment is free as long as both
+// operands use the same).
+//   row operand: row r's 16-byte chunk c at slot c ^ (-(r >> 2) & 3): the
+//     sixteen lanes that a ds_read_b128 serves at a time (rows 0-3 and 12-15 of
+//     one k group, 4-7 and 8-11 of the next) lie in all 64 banks once;
 //   col operand: k row kr, its 16-element unit u at unit u ^ col_swz(kr).
 //     bf16 fragments come through ds_read_b64_tr_b16 (16 lanes read 4 k rows
 //     x 16 columns and each receives one column), fp32 ones through four
@@ -111,19 +113,20 @@ constexpr unsigned kOutOfRange = 0x80000000u;  // past every buffer's num_record
 template <int ES, int ROWS, bool COL, int NT, bool DIRECT>
 struct Tile {
     static constexpr int CE = 16 / ES;           // elements per chunk
-    static constexpr int KE = 128 / ES;          // k per stage
-    static constexpr int NC = ROWS * 8 / NT;     // chunks per thread
-    static constexpr int ROWB = COL ? ROWS * ES : 128;
+    static constexpr int KE = 64 / ES;            // k per stage
+    static constexpr int NC = ROWS * 4 / NT;     // chunks per thread
+    static constexpr int ROWB = COL ? ROWS * ES : 64;
     static constexpr int CPR = ROWB / 16;        // chunks per LDS row
     static constexpr int NU = ROWS / 16;         // 16-element units per k row (COL)
     static constexpr int UC = ES;                // chunks per unit
-    static constexpr int BYTES = ROWS * 128;
-    static_assert(NC >= 1 && ROWS * 8 % NT == 0, "threads cover the tile");
+    static constexpr int BYTES = ROWS * 64;
+    static_assert(NC >= 1 && ROWS * 4 % NT == 0, "threads cover the tile");
 
     const uint8_t *base;  // element (row 0, first k) of the tile
     long long ldb;        // bytes between rows (COL: between k)
     int lim;              // valid rows (COL: valid elements of a k row)
     int klen;             // k range
+    unsigned base_lo, base_hi;  // DIRECT: base, in scalar registers
     unsigned voff[DIRECT ? NC : 1];
     u32x4 reg[DIRECT ? 1 : NC];
 
@@ -132,7 +135,7 @@ struct Tile {
         row = i / CPR;
         const int q = i % CPR;
         if constexpr (COL) chunk = (((q / UC) ^ col_swz<ES, NU>(row)) * UC) + q % UC;
-        else chunk = q ^ ((row >> 1) & 7);
+        else chunk = q ^ (-(row >> 2) & 3);
     }
     // DIRECT: wave w's load j fills the 1 KB from chunk (j NW + w) 64
     static __device__ __forceinline__ int chunk_of(int j) { return j * NT + (int)threadIdx.x; }
@@ -143,6 +146,8 @@ struct Tile {
         lim = limit;
         klen = k;
         if constexpr (DIRECT) {
+            base_lo = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long long)b);
+            base_hi = __builtin_amdgcn_readfirstlane((unsigned)((unsigned long long)b >> 32));
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
                 int row, chunk;
@@ -152,28 +157,55 @@ struct Tile {
             }
         }
     }
-    // stage s straight into the LDS image at byte offset lds (DIRECT)
+    // Stage s straight into the LDS image at byte offset lds (DIRECT).  Inline
+    // assembly that the compiler does not see as a memory access: its wait
+    // insertion would otherwise make every later LDS read wait for all loads in
+    // flight.  Order is kept by the kernel's own waits and barriers.  The
+    // compiler's hazard handling does not look inside either: a VMEM
+    // instruction needs five wait states after a VALU instruction
+    // (v_readfirstlane) wrote a scalar register that it reads, one after a
+    // scalar write of M0.
     __device__ __forceinline__ void load_lds(int s, unsigned lds, int w) const {
         const int k0 = s * KE;
-        const uint8_t *p = base + (COL ? (long long)k0 * ldb : (long long)k0 * ES);
-        const unsigned long long a = (unsigned long long)p;
+        const unsigned long long a =
+            ((unsigned long long)base_hi << 32 | base_lo) + (COL ? (long long)k0 * ldb : (long long)k0 * ES);
         u32x4 rs;
-        rs[0] = __builtin_amdgcn_readfirstlane((unsigned)a);
-        rs[1] = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32) & 0xffffu);
+        rs[0] = (unsigned)a;
+        rs[1] = (unsigned)(a >> 32) & 0xffffu;
         rs[2] = 0x7fffffffu;
         rs[3] = 0x00027000u;
         const int krem = klen - k0;
+        unsigned v[NC];
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
-            unsigned v = voff[j];
+            v[j] = voff[j];
             if (krem < KE) {  // the last stage: chunks past the k range read as 0
                 int row, chunk;
                 place(chunk_of(j), row, chunk);
-                if (COL ? row >= krem : chunk * CE >= krem) v = kOutOfRange;
+                if (COL ? row >= krem : chunk * CE >= krem) v[j] = kOutOfRange;
             }
-            const unsigned m0 = __builtin_amdgcn_readfirstlane(lds + (j * NT + w * 64) * 16);
-            asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(v), "s"(rs), "{m0}"(m0));
         }
+        const unsigned m0 = __builtin_amdgcn_readfirstlane(lds + w * 1024);
+        constexpr int STEP = NT * 16;  // LDS bytes between a thread's chunks
+        static_assert(NC == 1 || NC == 2 || NC == 4, "chunks per thread");
+        if constexpr (NC == 1)
+            asm volatile("s_nop 4\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(v[0]),
+                         "s"(rs), "s"(m0)
+                         : "m0");
+        else if constexpr (NC == 2)
+            asm volatile(
+                "s_nop 4\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds\n\t"
+                "s_add_u32 m0, m0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"v"(v[0]),
+                "v"(v[1]), "s"(rs), "s"(m0), "n"(STEP)
+                : "m0", "scc");
+        else
+            asm volatile(
+                "s_nop 4\n\ts_mov_b32 m0, %5\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %4, 0 offen lds\n\t"
+                "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %4, 0 offen lds\n\t"
+                "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %4, 0 offen lds\n\t"
+                "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %4, 0 offen lds" ::"v"(v[0]),
+                "v"(v[1]), "v"(v[NC > 2 ? 2 : 0]), "v"(v[NC > 3 ? 3 : 0]), "s"(rs), "s"(m0), "n"(STEP)
+                : "m0", "scc");
     }
     __device__ __forceinline__ void load_regs(int s) {
         const int k0 = s * KE, krem = klen - k0;
@@ -199,17 +231,16 @@ struct Tile {
             *(__attribute__((address_space(3))) u32x4 *)(lds + chunk_of(j) * 16) = reg[j];
     }
 
-    // fragment of rows [row0 + 16 i, +16) (row0 a multiple of 16), half ks of
-    // the stage
-    static __device__ __forceinline__ u32x4 frag(const lds_u8 *lds, int row0, int i, int ks, int lane) {
+    // fragment of the 16 rows from 16 * blk
+    static __device__ __forceinline__ u32x4 frag(const lds_u8 *lds, int blk, int lane) {
         const int r16 = lane & 15, q4 = lane >> 4;
         if constexpr (!COL) {
-            const lds_u8 *p = lds + (row0 + i * 16 + r16) * 128 + (((ks * 4 + q4) ^ ((r16 >> 1) & 7)) << 4);
+            const lds_u8 *p = lds + (blk * 16 + r16) * 64 + ((q4 ^ (-(r16 >> 2) & 3)) << 4);
             return *(const __attribute__((address_space(3))) u32x4 *)p;
         } else if constexpr (ES == 2) {
             union { s16x4 h[2]; u32x4 v; } f;
-            const int kr = ks * 32 + q4 * 8 + (r16 >> 2);
-            const lds_u8 *p = lds + kr * ROWB + (((row0 >> 4) + i) ^ col_swz<ES, NU>(kr)) * 32 + (r16 & 3) * 8;
+            const int kr = q4 * 8 + (r16 >> 2);
+            const lds_u8 *p = lds + kr * ROWB + (blk ^ col_swz<ES, NU>(kr)) * 32 + (r16 & 3) * 8;
             const lds_u8 *p1 = p + 4 * ROWB;  // k rows kr + 4: bit 2 of kr is clear and not part of the swizzle
             f.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
             f.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p1);
@@ -218,13 +249,14 @@ struct Tile {
             u32x4 v;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int kr = ks * 16 + q4 * 4 + j;
-                const lds_u8 *p = lds + kr * ROWB + (((row0 >> 4) + i) ^ col_swz<ES, NU>(kr)) * 64 + r16 * 4;
+                const int kr = q4 * 4 + j;
+                const lds_u8 *p = lds + kr * ROWB + (blk ^ col_swz<ES, NU>(kr)) * 64 + r16 * 4;
                 v[j] = *(const __attribute__((address_space(3))) unsigned *)p;
             }
             return v;
         }
     }
+    static constexpr int READS = !COL ? 1 : (ES == 2 ? 2 : 4);  // LDS reads per fragment
 };
 
 // ---- work list -------------------------------------------------------------------
@@ -441,11 +473,22 @@ __device__ __forceinline__ bool vec_ok(const OpGemmArgs &g) {
 }
 
 // ---- the kernel --------------------------------------------------------------------
-// WM x WN waves; each owns (BM / WM) x (BN / WN) outputs.
-template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, bool DIRECT>
+// WM x WN waves; wave (wm, wn) owns the 16-row blocks wm, wm + WM, ... (so that
+// the blocks of a part-filled tile are spread over the SIMDs, and a wave skips
+// those past the last row) and BN / WN adjacent columns.
+//
+// DIRECT: a ring of NS stages in LDS.  The wave's columns are taken in two
+// halves.  Stage s:
+//   half 0: MFMAs of the first columns | reads of the stage's second columns
+//   wait until stage s + 1 landed; barrier (nothing of slot s is read any more)
+//   half 1: MFMAs of the second columns | reads of stage s + 1's rows and first
+//           columns | loads of stage s + NS into slot s
+// Loads past the last stage read zeros without touching memory, which keeps
+// the count of loads in flight exact.
+template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int NS, bool DIRECT>
 __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_) {
-    constexpr int ES = op_size(OT), NT = WM * WN * 64, KE = 128 / ES;
-    constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;
+    constexpr int ES = op_size(OT), NT = WM * WN * 64, KE = 64 / ES;
+    constexpr int MI = BM / WM / 16, NJ = BN / WN / 16, JH = NJ / 2;
     using TA = Tile<ES, BM, ACOL, NT, DIRECT>;
     using TB = Tile<ES, BN, BCOL, NT, DIRECT>;
 
@@ -483,68 +526,111 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
         for (int j = 0; j < NJ; ++j) acc[i][j] = acc_t<OT>{0, 0, 0, 0};
 
     lds_u8 *ring = (lds_u8 *)ring_;
-    // both slots of A, then both of B: the slots of an operand are within a DS
+    // all slots of A, then all of B: the slots of an operand are within a DS
     // instruction's 16-bit offset of each other
     auto a_slot = [](auto SLOT) { return decltype(SLOT)::value * TA::BYTES; };
-    auto b_slot = [](auto SLOT) { return 2 * TA::BYTES + decltype(SLOT)::value * TB::BYTES; };
+    auto b_slot = [](auto SLOT) { return NS * TA::BYTES + decltype(SLOT)::value * TB::BYTES; };
     const int S = (klen + KE - 1) / KE;
-    auto compute = [&](auto SLOT) {
-        const lds_u8 *la = ring + a_slot(SLOT), *lb = ring + b_slot(SLOT);
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            // the wave's columns in parts of up to four blocks, which bounds the live fragments
-            constexpr int JP = NJ < 4 ? NJ : 4;
-            u32x4 fa[MI], fb[JP];
-#pragma unroll
-            for (int i = 0; i < MI; ++i) fa[i] = TA::frag(la, wm * (BM / WM), i, ks, lane);
-#pragma unroll
-            for (int j0 = 0; j0 < NJ; j0 += JP) {
-#pragma unroll
-                for (int j = 0; j < JP; ++j) fb[j] = TB::frag(lb, wn * (BN / WN), j0 + j, ks, lane);
-#pragma unroll
-                for (int i = 0; i < MI; ++i)
-#pragma unroll
-                    for (int j = 0; j < JP; ++j) acc[i][j0 + j] = fma16<OT>(fb[j], fa[i], acc[i][j0 + j]);
-            }
-        }
-    };
+    const int mrows = RAGK ? g.M - jb.m0 : jb.len - jb.m0;
+    auto read_a = [&](auto SLOT, int i) { return TA::frag(ring + a_slot(SLOT), i * WM + wm, lane); };
+    auto read_b = [&](auto SLOT, int j) { return TB::frag(ring + b_slot(SLOT), wn * NJ + j, lane); };
     if (S > 0) {
         if constexpr (DIRECT) {
+            constexpr int NL = TA::NC + TB::NC;
             const unsigned l0 = (unsigned)(uintptr_t)ring;
             auto load = [&](auto SLOT, int s) {
                 ta.load_lds(s, l0 + a_slot(SLOT), w);
                 tb.load_lds(s, l0 + b_slot(SLOT), w);
             };
-            auto step = [&](auto SLOT, int s) {
-                wait_loads<0>();
-                lds_barrier();  // stage s landed in every wave; the other slot's reads are done
-                if (s + 1 < S) load(num<1 - decltype(SLOT)::value>{}, s + 1);
-                compute(SLOT);
-            };
             load(num<0>{}, 0);
-            int s = 0;
-            for (; s + 2 <= S; s += 2) {
-                step(num<0>{}, s);
-                step(num<1>{}, s + 1);
-            }
-            if (s < S) step(num<0>{}, s);
-        } else {
-            auto store = [&](auto SLOT) {
-                ta.store_regs(ring + a_slot(SLOT));
-                tb.store_regs(ring + b_slot(SLOT));
+            load(num<1>{}, 1);
+            if constexpr (NS > 2) load(num<2 % NS>{}, 2);
+            if constexpr (NS > 3) load(num<3 % NS>{}, 3);
+            wait_loads<(NS - 1) * NL>();
+            lds_barrier();
+            // NI: the wave's row blocks that hold rows
+            auto run = [&](auto NI_) {
+                constexpr int NI = decltype(NI_)::value;
+                u32x4 fa[MI], fb[2][JH];
+#pragma unroll
+                for (int i = 0; i < NI; ++i) fa[i] = read_a(num<0>{}, i);
+                if constexpr (NI > 0) {
+#pragma unroll
+                    for (int j = 0; j < JH; ++j) fb[0][j] = read_b(num<0>{}, j);
+                }
+                auto stage = [&](auto SLOT, int s) {
+                    using Next = num<(decltype(SLOT)::value + 1) % NS>;
+                    if constexpr (NI > 0) {
+#pragma unroll
+                        for (int j = 0; j < JH; ++j) fb[1][j] = read_b(SLOT, JH + j);
+#pragma unroll
+                        for (int i = 0; i < NI; ++i)
+#pragma unroll
+                            for (int j = 0; j < JH; ++j) acc[i][j] = fma16<OT>(fb[0][j], fa[i], acc[i][j]);
+                    }
+                    wait_loads<(NS - 2) * NL>();
+                    lds_barrier();
+                    if constexpr (NI > 0) {
+#pragma unroll
+                        for (int j = 0; j < JH; ++j) fb[0][j] = read_b(Next{}, j);
+                    }
+                    load(SLOT, s + NS);
+#pragma unroll
+                    for (int i = 0; i < NI; ++i) {
+#pragma unroll
+                        for (int j = 0; j < JH; ++j) acc[i][JH + j] = fma16<OT>(fb[1][j], fa[i], acc[i][JH + j]);
+                        fa[i] = read_a(Next{}, i);
+                    }
+                };
+                int s = 0;
+                for (; s + NS <= S; s += NS) {
+                    stage(num<0>{}, s);
+                    stage(num<1>{}, s + 1);
+                    if constexpr (NS > 2) stage(num<2 % NS>{}, s + 2);
+                    if constexpr (NS > 3) stage(num<3 % NS>{}, s + 3);
+                }
+                if (s < S) stage(num<0>{}, s);
+                if (s + 1 < S) stage(num<1>{}, s + 1);
+                if constexpr (NS > 3)
+                    if (s + 2 < S) stage(num<2 % NS>{}, s + 2);
             };
+            if constexpr (RAGK || MI < 4) {
+                run(num<MI>{});
+            } else {
+                const int ni = (mrows - wm * 16 + WM * 16 - 1) / (WM * 16);
+                if (ni >= MI) run(num<MI>{});
+                else if (ni == 3) run(num<3>{});
+                else if (ni == 2) run(num<2>{});
+                else if (ni == 1) run(num<1>{});
+                else run(num<0>{});
+            }
+            wait_loads<0>();  // no load may still be writing LDS when the workgroup ends
+        } else {
             auto step = [&](auto SLOT, int s) {
                 lds_barrier();
                 if (s + 1 < S) {
                     ta.load_regs(s + 1);
                     tb.load_regs(s + 1);
                 }
-                compute(SLOT);
-                if (s + 1 < S) store(num<1 - decltype(SLOT)::value>{});
+                u32x4 fa[MI], fb[NJ];
+#pragma unroll
+                for (int i = 0; i < MI; ++i) fa[i] = read_a(SLOT, i);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) fb[j] = read_b(SLOT, j);
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) acc[i][j] = fma16<OT>(fb[j], fa[i], acc[i][j]);
+                if (s + 1 < S) {
+                    using Other = num<1 - decltype(SLOT)::value>;
+                    ta.store_regs(ring + a_slot(Other{}));
+                    tb.store_regs(ring + b_slot(Other{}));
+                }
             };
             ta.load_regs(0);
             tb.load_regs(0);
-            store(num<0>{});
+            ta.store_regs(ring + a_slot(num<0>{}));
+            tb.store_regs(ring + b_slot(num<0>{}));
             int s = 0;
             for (; s + 2 <= S; s += 2) {
                 step(num<0>{}, s);
@@ -560,7 +646,7 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
             float *ws = g.ws + ((long long)(jb.e * g.splits + jb.ks) * g.M) * g.N;
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
-                const int m = jb.m0 + wm * (BM / WM) + i * 16 + r16;
+                const int m = jb.m0 + (i * WM + wm) * 16 + r16;
                 if (m >= g.M) continue;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
@@ -574,10 +660,9 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
         }
     }
     const bool vec = vec_ok(g);
-    const int mrows = RAGK ? g.M - jb.m0 : jb.len - jb.m0;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-        const int ml = wm * (BM / WM) + i * 16 + r16;
+        const int ml = (i * WM + wm) * 16 + r16;
         if (ml >= mrows) continue;
         const long long row = RAGK ? (long long)jb.e * g.c_stride + (long long)(jb.m0 + ml) * g.ldc
                                    : (long long)(jb.lo + jb.m0 + ml) * g.ldc;
@@ -598,11 +683,11 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
     }
 }
 
-template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, bool DIRECT, int WPE>
+template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int NS, int WPE, bool DIRECT>
 __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void op_gemm_kernel(
     OpGemmArgs g) {
-    __shared__ __attribute__((aligned(1024))) uint8_t ring[2 * (BM + BN) * 128];
-    op_gemm_tile<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, DIRECT>(g, ring);
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * (BM + BN) * 64];
+    op_gemm_tile<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, NS, DIRECT>(g, ring);
 }
 
 // C of a split group: its ranges' sums in range order, one element per thread.
@@ -633,7 +718,7 @@ inline bool direct_ok(const void *p, long long ld, long long stride, int contigu
            (long long)contiguous * es % 16 == 0 && ld * es < (1ll << 22);
 }
 
-template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int WPE>
+template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int NS, int WPE>
 hipError_t launch_tiles(OpGemmArgs g, bool direct, hipStream_t s) {
     g.nt = (g.N + BN - 1) / BN;
     g.mt = RAGK ? (g.M + BM - 1) / BM : 0;
@@ -643,12 +728,12 @@ hipError_t launch_tiles(OpGemmArgs g, bool direct, hipStream_t s) {
     const long long grid = RAGK ? ((long long)g.mt * g.nt * g.splits + 7) / 8 * 8 * g.E : (mtiles * g.nt + 7) / 8 * 8;
     if (grid > 0x7fffffffll / (WM * WN * 64)) return hipErrorInvalidValue;
     const dim3 b(WM * WN * 64);
-    if constexpr (BM == 256) {  // (staging through registers leaves too few for these tiles)
+    if constexpr (BN == 256) {  // (staging through registers leaves too few for these tiles)
         if (!direct) return hipErrorInvalidValue;
-        op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, true, WPE><<<(unsigned)grid, b, 0, s>>>(g);
+        op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, NS, WPE, true><<<(unsigned)grid, b, 0, s>>>(g);
     } else {
-        if (direct) op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, true, WPE><<<(unsigned)grid, b, 0, s>>>(g);
-        else op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, false, WPE><<<(unsigned)grid, b, 0, s>>>(g);
+        if (direct) op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, NS, WPE, true><<<(unsigned)grid, b, 0, s>>>(g);
+        else op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, 2, WPE, false><<<(unsigned)grid, b, 0, s>>>(g);
     }
     hipError_t e = hipGetLastError();
     if constexpr (RAGK) {
@@ -682,11 +767,11 @@ hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
         // ragged k: a group that holds most rows has to fill the GPU by itself
         const bool large = RAGK ? tiles(256) >= g.E * (long long)(ncu / 2) : avg >= 192 && g.N >= 192 && tiles(256) >= 2 * ncu;
         if (direct && large)
-            return launch_tiles<OT, ACOL, BCOL, RAGK, 256, 256, 4, 2, 2>(g, direct, s);
+            return launch_tiles<OT, ACOL, BCOL, RAGK, 256, 256, 4, 2, 4, 2>(g, direct, s);
     }
     if (avg >= 64 && g.N >= 64 && tiles(128) >= ncu)
-        return launch_tiles<OT, ACOL, BCOL, RAGK, 128, 128, 2, 2, 2>(g, direct, s);
-    return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, 3>(g, direct, s);
+        return launch_tiles<OT, ACOL, BCOL, RAGK, 128, 128, 2, 2, 4, 2>(g, direct, s);
+    return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, 4, 3>(g, direct, s);
 }
 
 }  // namespace ops
