@@ -110,17 +110,17 @@ constexpr unsigned kOutOfRange = 0x80000000u;  // past every buffer's num_record
 // it.  DIRECT: by buffer loads straight into LDS (16-byte aligned rows and
 // whole chunks; a lane whose chunk lies outside reads zeros by the buffer's
 // own range check).  Otherwise through registers, any alignment.
-template <int ES, int ROWS, bool COL, int NT, bool DIRECT>
+template <int ES, int ROWS, bool COL, int NT, int KSUB, bool DIRECT>
 struct Tile {
     static constexpr int CE = 16 / ES;           // elements per chunk
-    static constexpr int KE = 64 / ES;            // k per stage
-    static constexpr int NC = ROWS * 4 / NT;     // chunks per thread
-    static constexpr int ROWB = COL ? ROWS * ES : 64;
+    static constexpr int KE = KSUB * 64 / ES;     // k per stage
+    static constexpr int NC = KSUB * ROWS * 4 / NT;  // chunks per thread
+    static constexpr int ROWB = COL ? ROWS * ES : 64 * KSUB;
     static constexpr int CPR = ROWB / 16;        // chunks per LDS row
     static constexpr int NU = ROWS / 16;         // 16-element units per k row (COL)
     static constexpr int UC = ES;                // chunks per unit
-    static constexpr int BYTES = ROWS * 64;
-    static_assert(NC >= 1 && ROWS * 4 % NT == 0, "threads cover the tile");
+    static constexpr int BYTES = ROWS * 64 * KSUB;
+    static_assert(NC >= 1 && KSUB * ROWS * 4 % NT == 0, "threads cover the tile");
 
     const uint8_t *base;  // element (row 0, first k) of the tile
     long long ldb;        // bytes between rows (COL: between k)
@@ -130,12 +130,15 @@ struct Tile {
     unsigned voff[DIRECT ? NC : 1];
     u32x4 reg[DIRECT ? 1 : NC];
 
+    static __device__ __forceinline__ int row_swz(int row) {
+        return KSUB == 2 ? (row >> 1) & 7 : -(row >> 2) & 3;
+    }
     // chunk i of the image -> its LDS row and source chunk within the row
     static __device__ __forceinline__ void place(int i, int &row, int &chunk) {
         row = i / CPR;
         const int q = i % CPR;
         if constexpr (COL) chunk = (((q / UC) ^ col_swz<ES, NU>(row)) * UC) + q % UC;
-        else chunk = q ^ (-(row >> 2) & 3);
+        else chunk = q ^ row_swz(row);
     }
     // DIRECT: wave w's load j fills the 1 KB from chunk (j NW + w) 64
     static __device__ __forceinline__ int chunk_of(int j) { return j * NT + (int)threadIdx.x; }
@@ -231,15 +234,15 @@ struct Tile {
             *(__attribute__((address_space(3))) u32x4 *)(lds + chunk_of(j) * 16) = reg[j];
     }
 
-    // fragment of the 16 rows from 16 * blk
-    static __device__ __forceinline__ u32x4 frag(const lds_u8 *lds, int blk, int lane) {
+    // fragment of the 16 rows from 16 * blk, 64-byte piece ks of the stage
+    static __device__ __forceinline__ u32x4 frag(const lds_u8 *lds, int blk, int ks, int lane) {
         const int r16 = lane & 15, q4 = lane >> 4;
         if constexpr (!COL) {
-            const lds_u8 *p = lds + (blk * 16 + r16) * 64 + ((q4 ^ (-(r16 >> 2) & 3)) << 4);
+            const lds_u8 *p = lds + (blk * 16 + r16) * ROWB + (((ks * 4 + q4) ^ row_swz(r16)) << 4);
             return *(const __attribute__((address_space(3))) u32x4 *)p;
         } else if constexpr (ES == 2) {
             union { s16x4 h[2]; u32x4 v; } f;
-            const int kr = q4 * 8 + (r16 >> 2);
+            const int kr = ks * 32 + q4 * 8 + (r16 >> 2);
             const lds_u8 *p = lds + kr * ROWB + (blk ^ col_swz<ES, NU>(kr)) * 32 + (r16 & 3) * 8;
             const lds_u8 *p1 = p + 4 * ROWB;  // k rows kr + 4: bit 2 of kr is clear and not part of the swizzle
             f.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
@@ -249,7 +252,7 @@ struct Tile {
             u32x4 v;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int kr = q4 * 4 + j;
+                const int kr = ks * 16 + q4 * 4 + j;
                 const lds_u8 *p = lds + kr * ROWB + (blk ^ col_swz<ES, NU>(kr)) * 64 + r16 * 4;
                 v[j] = *(const __attribute__((address_space(3))) unsigned *)p;
             }
@@ -485,12 +488,12 @@ __device__ __forceinline__ bool vec_ok(const OpGemmArgs &g) {
 //           columns | loads of stage s + NS into slot s
 // Loads past the last stage read zeros without touching memory, which keeps
 // the count of loads in flight exact.
-template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int NS, bool DIRECT>
+template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int KSUB, int NS, bool DIRECT>
 __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_) {
-    constexpr int ES = op_size(OT), NT = WM * WN * 64, KE = 64 / ES;
+    constexpr int ES = op_size(OT), NT = WM * WN * 64, KE = KSUB * 64 / ES;
     constexpr int MI = BM / WM / 16, NJ = BN / WN / 16, JH = NJ / 2;
-    using TA = Tile<ES, BM, ACOL, NT, DIRECT>;
-    using TB = Tile<ES, BN, BCOL, NT, DIRECT>;
+    using TA = Tile<ES, BM, ACOL, NT, KSUB, DIRECT>;
+    using TB = Tile<ES, BN, BCOL, NT, KSUB, DIRECT>;
 
     OpJob jb;
     if constexpr (RAGK) {
@@ -532,8 +535,8 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
     auto b_slot = [](auto SLOT) { return NS * TA::BYTES + decltype(SLOT)::value * TB::BYTES; };
     const int S = (klen + KE - 1) / KE;
     const int mrows = RAGK ? g.M - jb.m0 : jb.len - jb.m0;
-    auto read_a = [&](auto SLOT, int i) { return TA::frag(ring + a_slot(SLOT), i * WM + wm, lane); };
-    auto read_b = [&](auto SLOT, int j) { return TB::frag(ring + b_slot(SLOT), wn * NJ + j, lane); };
+    auto read_a = [&](auto SLOT, int i, int ks) { return TA::frag(ring + a_slot(SLOT), i * WM + wm, ks, lane); };
+    auto read_b = [&](auto SLOT, int j, int ks) { return TB::frag(ring + b_slot(SLOT), wn * NJ + j, ks, lane); };
     if (S > 0) {
         if constexpr (DIRECT) {
             constexpr int NL = TA::NC + TB::NC;
@@ -553,33 +556,40 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
                 constexpr int NI = decltype(NI_)::value;
                 u32x4 fa[MI], fb[2][JH];
 #pragma unroll
-                for (int i = 0; i < NI; ++i) fa[i] = read_a(num<0>{}, i);
+                for (int i = 0; i < NI; ++i) fa[i] = read_a(num<0>{}, i, 0);
                 if constexpr (NI > 0) {
 #pragma unroll
-                    for (int j = 0; j < JH; ++j) fb[0][j] = read_b(num<0>{}, j);
+                    for (int j = 0; j < JH; ++j) fb[0][j] = read_b(num<0>{}, j, 0);
                 }
                 auto stage = [&](auto SLOT, int s) {
                     using Next = num<(decltype(SLOT)::value + 1) % NS>;
-                    if constexpr (NI > 0) {
 #pragma unroll
-                        for (int j = 0; j < JH; ++j) fb[1][j] = read_b(SLOT, JH + j);
+                    for (int ks = 0; ks < KSUB; ++ks) {
+                        if constexpr (NI > 0) {
 #pragma unroll
-                        for (int i = 0; i < NI; ++i)
+                            for (int j = 0; j < JH; ++j) fb[1][j] = read_b(SLOT, JH + j, ks);
 #pragma unroll
-                            for (int j = 0; j < JH; ++j) acc[i][j] = fma16<OT>(fb[0][j], fa[i], acc[i][j]);
-                    }
-                    wait_loads<(NS - 2) * NL>();
-                    lds_barrier();
-                    if constexpr (NI > 0) {
+                            for (int i = 0; i < NI; ++i)
 #pragma unroll
-                        for (int j = 0; j < JH; ++j) fb[0][j] = read_b(Next{}, j);
-                    }
-                    load(SLOT, s + NS);
+                                for (int j = 0; j < JH; ++j) acc[i][j] = fma16<OT>(fb[0][j], fa[i], acc[i][j]);
+                        }
+                        const bool last = ks == KSUB - 1;
+                        if (last) {
+                            wait_loads<(NS - 2) * NL>();
+                            lds_barrier();
+                        }
+                        if constexpr (NI > 0) {
 #pragma unroll
-                    for (int i = 0; i < NI; ++i) {
+                            for (int j = 0; j < JH; ++j)
+                                fb[0][j] = last ? read_b(Next{}, j, 0) : read_b(SLOT, j, ks + 1);
+                        }
+                        if (last) load(SLOT, s + NS);
 #pragma unroll
-                        for (int j = 0; j < JH; ++j) acc[i][JH + j] = fma16<OT>(fb[1][j], fa[i], acc[i][JH + j]);
-                        fa[i] = read_a(Next{}, i);
+                        for (int i = 0; i < NI; ++i) {
+#pragma unroll
+                            for (int j = 0; j < JH; ++j) acc[i][JH + j] = fma16<OT>(fb[1][j], fa[i], acc[i][JH + j]);
+                            fa[i] = last ? read_a(Next{}, i, 0) : read_a(SLOT, i, ks + 1);
+                        }
                     }
                 };
                 int s = 0;
@@ -612,15 +622,18 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
                     ta.load_regs(s + 1);
                     tb.load_regs(s + 1);
                 }
-                u32x4 fa[MI], fb[NJ];
 #pragma unroll
-                for (int i = 0; i < MI; ++i) fa[i] = read_a(SLOT, i);
+                for (int ks = 0; ks < KSUB; ++ks) {
+                    u32x4 fa[MI], fb[NJ];
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) fb[j] = read_b(SLOT, j);
+                    for (int i = 0; i < MI; ++i) fa[i] = read_a(SLOT, i, ks);
 #pragma unroll
-                for (int i = 0; i < MI; ++i)
+                    for (int j = 0; j < NJ; ++j) fb[j] = read_b(SLOT, j, ks);
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) acc[i][j] = fma16<OT>(fb[j], fa[i], acc[i][j]);
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j) acc[i][j] = fma16<OT>(fb[j], fa[i], acc[i][j]);
+                }
                 if (s + 1 < S) {
                     using Other = num<1 - decltype(SLOT)::value>;
                     ta.store_regs(ring + a_slot(Other{}));
@@ -683,11 +696,11 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
     }
 }
 
-template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int NS, int WPE, bool DIRECT>
+template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int KSUB, int NS, int WPE, bool DIRECT>
 __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void op_gemm_kernel(
     OpGemmArgs g) {
-    __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * (BM + BN) * 64];
-    op_gemm_tile<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, NS, DIRECT>(g, ring);
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * (BM + BN) * 64 * KSUB];
+    op_gemm_tile<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, KSUB, NS, DIRECT>(g, ring);
 }
 
 // C of a split group: its ranges' sums in range order, one element per thread.
@@ -718,7 +731,7 @@ inline bool direct_ok(const void *p, long long ld, long long stride, int contigu
            (long long)contiguous * es % 16 == 0 && ld * es < (1ll << 22);
 }
 
-template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int NS, int WPE>
+template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int KSUB, int NS, int WPE>
 hipError_t launch_tiles(OpGemmArgs g, bool direct, hipStream_t s) {
     g.nt = (g.N + BN - 1) / BN;
     g.mt = RAGK ? (g.M + BM - 1) / BM : 0;
@@ -730,10 +743,10 @@ hipError_t launch_tiles(OpGemmArgs g, bool direct, hipStream_t s) {
     const dim3 b(WM * WN * 64);
     if constexpr (BN == 256) {  // (staging through registers leaves too few for these tiles)
         if (!direct) return hipErrorInvalidValue;
-        op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, NS, WPE, true><<<(unsigned)grid, b, 0, s>>>(g);
+        op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, KSUB, NS, WPE, true><<<(unsigned)grid, b, 0, s>>>(g);
     } else {
-        if (direct) op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, NS, WPE, true><<<(unsigned)grid, b, 0, s>>>(g);
-        else op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, 2, WPE, false><<<(unsigned)grid, b, 0, s>>>(g);
+        if (direct) op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, KSUB, NS, WPE, true><<<(unsigned)grid, b, 0, s>>>(g);
+        else op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, 1, 2, WPE, false><<<(unsigned)grid, b, 0, s>>>(g);
     }
     hipError_t e = hipGetLastError();
     if constexpr (RAGK) {
@@ -754,6 +767,8 @@ hipError_t launch_tiles(OpGemmArgs g, bool direct, hipStream_t s) {
 template <int OT, bool ACOL, bool BCOL, bool RAGK>
 hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
     constexpr int ES = op_size(OT);
+    // row operands are loaded in whole 128-byte lines
+    constexpr int KSUB = ACOL && BCOL ? 1 : 2;
     const bool direct =
         direct_ok(g.A, g.lda, 0, ACOL ? g.M : g.K, ES) && direct_ok(g.B, g.ldb, g.b_stride, BCOL ? g.N : g.K, ES);
     auto tiles = [&](int b) -> long long {
@@ -767,11 +782,11 @@ hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
         // ragged k: a group that holds most rows has to fill the GPU by itself
         const bool large = RAGK ? tiles(256) >= g.E * (long long)(ncu / 2) : avg >= 192 && g.N >= 192 && tiles(256) >= 2 * ncu;
         if (direct && large)
-            return launch_tiles<OT, ACOL, BCOL, RAGK, 256, 256, 4, 2, 4, 2>(g, direct, s);
+            return launch_tiles<OT, ACOL, BCOL, RAGK, 256, 256, 4, 2, KSUB, 4 / KSUB, 2>(g, direct, s);
     }
     if (avg >= 64 && g.N >= 64 && tiles(128) >= ncu)
-        return launch_tiles<OT, ACOL, BCOL, RAGK, 128, 128, 2, 2, 4, 2>(g, direct, s);
-    return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, 4, 3>(g, direct, s);
+        return launch_tiles<OT, ACOL, BCOL, RAGK, 128, 128, 2, 2, KSUB, 4 / KSUB, 2>(g, direct, s);
+    return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, KSUB, 4 / KSUB, 3>(g, direct, s);
 }
 
 }  // namespace ops
