@@ -470,9 +470,86 @@ __device__ __forceinline__ void put4(const OpGemmArgs &g, long long at, int n, f
     }
 }
 
+// Rows of C that take whole 16-byte chunks, as store_tile_rows writes them (a
+// bf16 sum that is added to stays in fp32 until its one rounding: put4).
+__device__ __forceinline__ bool rows16(const OpGemmArgs &g) {
+    const int es = g.c_f32 ? 4 : 2;
+    return (((uintptr_t)g.C | (uintptr_t)(g.ldc * es) | (uintptr_t)(g.c_stride * es)) & 15) == 0 &&
+           (g.c_f32 || !g.accumulate);
+}
 __device__ __forceinline__ bool vec_ok(const OpGemmArgs &g) {
     const int es = g.c_f32 ? 4 : 2;
     return (((uintptr_t)g.C | (uintptr_t)(g.ldc * es) | (uintptr_t)(g.c_stride * es)) & (4 * es - 1)) == 0;
+}
+
+// A tile's results through LDS, so that whole rows are stored: a wave's own
+// stores are 16 rows x 32 (fp32: 64) bytes each.  Row r's 16-byte chunk c is
+// kept at chunk c ^ (r mod CH): the column-wise writes and the row-wise reads
+// both spread over the banks.  EO: bytes of a result; PR rows at a time.  val(i,
+// j, c): the lane's result in row block i, column block j, column 4 (lane / 16) + c.
+template <int EO, int BM, int BN, int WM, int WN, int RING, typename Val>
+__device__ __forceinline__ void store_tile_rows(const OpGemmArgs &g, lds_u8 *ring, long long at0, int mrows, int n0,
+                                                int wm, int wn, int lane, Val val) {
+    constexpr int NT = WM * WN * 64, MI = BM / WM / 16, NJ = BN / WN / 16;
+    constexpr int CW = BN * EO, CH = CW / 16, CE = 16 / EO;
+    constexpr int FIT = RING / CW, PR = FIT < BM ? FIT : BM;  // rows per pass
+    static_assert(PR % (WM * 16) == 0 && BM % PR == 0 && NT % CH == 0 && PR % (NT / CH) == 0, "passes");
+    constexpr int IP = PR / (WM * 16);  // row blocks of a wave per pass
+    const int r16 = lane & 15, q4 = lane >> 4;
+#pragma unroll
+    for (int p = 0; p < BM / PR; ++p) {
+        if (p * PR >= mrows) break;
+        __syncthreads();  // the ring (the previous pass) is no longer read
+#pragma unroll
+        for (int ii = 0; ii < IP; ++ii) {
+            const int i = p * IP + ii, r = (ii * WM + wm) * 16 + r16;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int b = ((wn * NJ + j) * 16 + 4 * q4) * EO, c = b / 16;
+                lds_u8 *q = ring + r * CW + ((c ^ (r & (CH - 1))) << 4) + (b & 15);
+                if constexpr (EO == 4) {
+                    typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+                    *(lds_f32x4 *)q = f32x4{val(i, j, 0), val(i, j, 1), val(i, j, 2), val(i, j, 3)};
+                } else {
+                    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+                    *(__attribute__((address_space(3))) u32x2 *)q =
+                        u32x2{pack2(val(i, j, 0), val(i, j, 1)), pack2(val(i, j, 2), val(i, j, 3))};
+                }
+            }
+        }
+        __syncthreads();
+        const int ch = (int)threadIdx.x % CH, n = n0 + ch * CE;
+        const int rows = min(PR, mrows - p * PR);
+        if (n < g.N) {
+            for (int r = (int)threadIdx.x / CH; r < rows; r += NT / CH) {
+                u32x4 v = *(const __attribute__((address_space(3))) u32x4 *)(ring + r * CW + ((ch ^ (r & (CH - 1))) << 4));
+                uint8_t *dst = (uint8_t *)g.C + (at0 + (long long)(p * PR + r) * g.ldc + n) * EO;
+                if (n + CE <= g.N) {
+                    if (g.accumulate) {
+                        const u32x4 o = *(const u32x4 *)dst;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            if constexpr (EO == 4)
+                                v[q] = __float_as_uint(__uint_as_float(o[q]) + __uint_as_float(v[q]));
+                        }
+                    }
+                    *(u32x4 *)dst = v;
+                } else {
+#pragma unroll
+                    for (int q = 0; q < CE; ++q) {
+                        if (n + q >= g.N) continue;
+                        if constexpr (EO == 4) {
+                            float *d = (float *)dst + q;
+                            const float x = __uint_as_float(v[q]);
+                            *d = g.accumulate ? *d + x : x;
+                        } else {
+                            ((uint16_t *)dst)[q] = (uint16_t)(v[q / 2] >> (16 * (q & 1)));
+                        }
+                    }
+                }
+            }
+        }
+    }
 }
 
 // ---- the kernel --------------------------------------------------------------------
@@ -672,26 +749,43 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
             return;
         }
     }
+    const long long at0 = RAGK ? (long long)jb.e * g.c_stride + (long long)jb.m0 * g.ldc
+                               : (long long)(jb.lo + jb.m0) * g.ldc;  // the tile's first row in C
+    // int8: the lane's scales, of its row blocks and its columns
+    float sa[MI], sb[NJ][4];
+    if constexpr (OT == OT_I8) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int ml = (i * WM + wm) * 16 + r16;
+            sa[i] = ml < mrows ? g.sa[jb.lo + jb.m0 + ml] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int n = jb.n0 + (wn * NJ + j) * 16 + 4 * q4 + c;
+                sb[j][c] = n < g.N ? g.sb[(long long)jb.e * g.N + n] : 0.0f;
+            }
+    }
+    auto val = [&](int i, int j, int c) -> float {
+        if constexpr (OT == OT_I8) return (float)acc[i][j][c] * sa[i] * sb[j][c];
+        else return acc[i][j][c];
+    };
+    constexpr int RING = NS * (TA::BYTES + TB::BYTES);
+    if (DIRECT && rows16(g)) {
+        if (g.c_f32) store_tile_rows<4, BM, BN, WM, WN, RING>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
+        else store_tile_rows<2, BM, BN, WM, WN, RING>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
+        return;
+    }
     const bool vec = vec_ok(g);
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
         const int ml = (i * WM + wm) * 16 + r16;
         if (ml >= mrows) continue;
-        const long long row = RAGK ? (long long)jb.e * g.c_stride + (long long)(jb.m0 + ml) * g.ldc
-                                   : (long long)(jb.lo + jb.m0 + ml) * g.ldc;
-        float sa = 0.0f;
-        if constexpr (OT == OT_I8) sa = g.sa[jb.lo + jb.m0 + ml];
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            const int n = jb.n0 + wn * (BN / WN) + j * 16 + 4 * q4;
-            float v[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                v[c] = (float)acc[i][j][c];
-                if constexpr (OT == OT_I8)
-                    v[c] = v[c] * sa * (n + c < g.N ? g.sb[(long long)jb.e * g.N + n + c] : 0.0f);
-            }
-            put4(g, row + n, n, v[0], v[1], v[2], v[3], vec);
+            const int n = jb.n0 + (wn * NJ + j) * 16 + 4 * q4;
+            put4(g, at0 + (long long)ml * g.ldc + n, n, val(i, j, 0), val(i, j, 1), val(i, j, 2), val(i, j, 3), vec);
         }
     }
 }
