@@ -107,20 +107,24 @@ __device__ __forceinline__ int col_swz(int kr) {
 constexpr unsigned kOutOfRange = 0x80000000u;  // past every buffer's num_records: reads as 0
 
 // One operand's tile of ROWS rows: its LDS stage image and how NT threads fill
-// it.  DIRECT: by buffer loads straight into LDS (16-byte aligned rows and
-// whole chunks; a lane whose chunk lies outside reads zeros by the buffer's
-// own range check).  Otherwise through registers, any alignment.
-template <int ES, int ROWS, bool COL, int NT, int KSUB, bool DIRECT>
+// it.  VB 16 or 4: by buffer loads of VB bytes a lane straight into LDS (16:
+// 16-byte aligned rows of whole chunks; 4: fp32 of any stride and length); a
+// lane whose bytes lie outside reads zeros by the buffer's own range check.
+// VB 0: through registers, any alignment.
+template <int ES, int ROWS, bool COL, int NT, int KSUB, int VB>
 struct Tile {
+    static constexpr bool DIRECT = VB > 0;
+    static_assert(VB == 0 || VB == 16 || (VB == 4 && ES == 4), "bytes per lane");
     static constexpr int CE = 16 / ES;           // elements per chunk
     static constexpr int KE = KSUB * 64 / ES;     // k per stage
-    static constexpr int NC = KSUB * ROWS * 4 / NT;  // chunks per thread
+    static constexpr int PER = VB == 4 ? 4 : 1;  // loads per chunk
+    static constexpr int NC = PER * KSUB * ROWS * 4 / NT;  // loads per thread
     static constexpr int ROWB = COL ? ROWS * ES : 64 * KSUB;
     static constexpr int CPR = ROWB / 16;        // chunks per LDS row
     static constexpr int NU = ROWS / 16;         // 16-element units per k row (COL)
     static constexpr int UC = ES;                // chunks per unit
     static constexpr int BYTES = ROWS * 64 * KSUB;
-    static_assert(NC >= 1 && KSUB * ROWS * 4 % NT == 0, "threads cover the tile");
+    static_assert(NC >= 1 && PER * KSUB * ROWS * 4 % NT == 0, "threads cover the tile");
 
     const uint8_t *base;  // element (row 0, first k) of the tile
     long long ldb;        // bytes between rows (COL: between k)
@@ -143,6 +147,14 @@ struct Tile {
     // DIRECT: wave w's load j fills the 1 KB from chunk (j NW + w) 64
     static __device__ __forceinline__ int chunk_of(int j) { return j * NT + (int)threadIdx.x; }
 
+    // load j of this thread: its LDS row and its first element within the row
+    static __device__ __forceinline__ void place_load(int j, int &row, int &elem) {
+        const int i = chunk_of(j);
+        int chunk;
+        place(i / PER, row, chunk);
+        elem = chunk * CE + i % PER;
+    }
+
     __device__ __forceinline__ void init(const uint8_t *b, long long ld_bytes, int limit, int k) {
         base = b;
         ldb = ld_bytes;
@@ -153,10 +165,10 @@ struct Tile {
             base_hi = __builtin_amdgcn_readfirstlane((unsigned)((unsigned long long)b >> 32));
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
-                int row, chunk;
-                place(chunk_of(j), row, chunk);
-                const bool ok = COL ? chunk * CE < lim : row < lim;
-                voff[j] = ok ? (unsigned)(row * (int)ldb + chunk * 16) : kOutOfRange;
+                int row, elem;
+                place_load(j, row, elem);
+                const bool ok = COL ? elem < lim : row < lim;
+                voff[j] = ok ? (unsigned)(row * (int)ldb + elem * ES) : kOutOfRange;
             }
         }
     }
@@ -182,26 +194,39 @@ struct Tile {
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             v[j] = voff[j];
-            if (krem < KE) {  // the last stage: chunks past the k range read as 0
-                int row, chunk;
-                place(chunk_of(j), row, chunk);
-                if (COL ? row >= krem : chunk * CE >= krem) v[j] = kOutOfRange;
+            if (krem < KE) {  // the last stage: what lies past the k range reads as 0
+                int row, elem;
+                place_load(j, row, elem);
+                if (COL ? row >= krem : elem >= krem) v[j] = kOutOfRange;
             }
         }
-        const unsigned m0 = __builtin_amdgcn_readfirstlane(lds + w * 1024);
-        constexpr int STEP = NT * 16;  // LDS bytes between a thread's chunks
-        static_assert(NC == 1 || NC == 2 || NC == 4, "chunks per thread");
-        if constexpr (NC == 1)
+        constexpr int VL = VB == 4 ? 4 : 16;
+        const unsigned m0 = __builtin_amdgcn_readfirstlane(lds + w * (64 * VL));
+        constexpr int STEP = NT * VL;  // LDS bytes between a thread's loads
+        if constexpr (VB == 4) {
+            static_assert(NC % 4 == 0, "loads per thread");
+#pragma unroll
+            for (int j = 0; j < NC; j += 4)
+                asm volatile(
+                    "s_nop 4\n\ts_mov_b32 m0, %5\n\ts_nop 0\n\tbuffer_load_dword %0, %4, 0 offen lds\n\t"
+                    "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dword %1, %4, 0 offen lds\n\t"
+                    "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dword %2, %4, 0 offen lds\n\t"
+                    "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dword %3, %4, 0 offen lds" ::"v"(v[j]),
+                    "v"(v[j + 1 < NC ? j + 1 : 0]), "v"(v[j + 2 < NC ? j + 2 : 0]), "v"(v[j + 3 < NC ? j + 3 : 0]),
+                    "s"(rs), "s"(m0 + j * STEP), "n"(STEP)
+                    : "m0", "scc");
+        } else if constexpr (NC == 1) {
             asm volatile("s_nop 4\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(v[0]),
                          "s"(rs), "s"(m0)
                          : "m0");
-        else if constexpr (NC == 2)
+        } else if constexpr (NC == 2) {
             asm volatile(
                 "s_nop 4\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds\n\t"
                 "s_add_u32 m0, m0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"v"(v[0]),
                 "v"(v[1]), "s"(rs), "s"(m0), "n"(STEP)
                 : "m0", "scc");
-        else
+        } else {
+            static_assert(NC <= 4 && NC != 3, "loads per thread");
             asm volatile(
                 "s_nop 4\n\ts_mov_b32 m0, %5\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %4, 0 offen lds\n\t"
                 "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %4, 0 offen lds\n\t"
@@ -209,23 +234,27 @@ struct Tile {
                 "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %4, 0 offen lds" ::"v"(v[0]),
                 "v"(v[1]), "v"(v[NC > 2 ? 2 : 0]), "v"(v[NC > 3 ? 3 : 0]), "s"(rs), "s"(m0), "n"(STEP)
                 : "m0", "scc");
+        }
     }
+    // Stage s into registers.  Whole chunks are loaded without a branch, so that
+    // they are in flight together: rows past the last one repeat it (their
+    // products are not stored); chunks that cross an edge element by element.
     __device__ __forceinline__ void load_regs(int s) {
         const int k0 = s * KE, krem = klen - k0;
+        const bool whole = krem >= KE && (!COL || lim >= ROWS);
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             int row, chunk;
             place(chunk_of(j), row, chunk);
-            int n;
-            const uint8_t *p;
-            if constexpr (COL) {
-                n = row < krem ? lim - chunk * CE : 0;
-                p = base + (long long)(k0 + row) * ldb + chunk * 16;
+            if (!COL) row = min(row, lim - 1);
+            const uint8_t *p = COL ? base + (long long)(k0 + row) * ldb + chunk * 16
+                                   : base + (long long)row * ldb + (long long)k0 * ES + chunk * 16;
+            if (whole) {
+                __builtin_memcpy(&reg[j], p, 16);
             } else {
-                n = row < lim ? krem - chunk * CE : 0;
-                p = base + (long long)row * ldb + (long long)k0 * ES + chunk * 16;
+                const int n = COL ? (row < krem ? lim - chunk * CE : 0) : krem - chunk * CE;
+                reg[j] = load_chunk<ES>(p, n);
             }
-            reg[j] = load_chunk<ES>(p, n);
         }
     }
     __device__ __forceinline__ void store_regs(lds_u8 *lds) const {
@@ -565,12 +594,13 @@ __device__ __forceinline__ void store_tile_rows(const OpGemmArgs &g, lds_u8 *rin
 //           columns | loads of stage s + NS into slot s
 // Loads past the last stage read zeros without touching memory, which keeps
 // the count of loads in flight exact.
-template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int KSUB, int NS, bool DIRECT>
+template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int KSUB, int NS, int VB>
 __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_) {
     constexpr int ES = op_size(OT), NT = WM * WN * 64, KE = KSUB * 64 / ES;
     constexpr int MI = BM / WM / 16, NJ = BN / WN / 16, JH = NJ / 2;
-    using TA = Tile<ES, BM, ACOL, NT, KSUB, DIRECT>;
-    using TB = Tile<ES, BN, BCOL, NT, KSUB, DIRECT>;
+    constexpr bool DIRECT = VB > 0;
+    using TA = Tile<ES, BM, ACOL, NT, KSUB, VB>;
+    using TB = Tile<ES, BN, BCOL, NT, KSUB, VB>;
 
     OpJob jb;
     if constexpr (RAGK) {
@@ -790,11 +820,11 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
     }
 }
 
-template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int KSUB, int NS, int WPE, bool DIRECT>
+template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int KSUB, int NS, int WPE, int VB>
 __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void op_gemm_kernel(
     OpGemmArgs g) {
     __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * (BM + BN) * 64 * KSUB];
-    op_gemm_tile<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, KSUB, NS, DIRECT>(g, ring);
+    op_gemm_tile<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, KSUB, NS, VB>(g, ring);
 }
 
 // C of a split group: its ranges' sums in range order, one element per thread.
@@ -818,15 +848,16 @@ __global__ __launch_bounds__(256) void op_fold_kernel(OpGemmArgs g) {
     }
 }
 
-// Rows that can be loaded straight into LDS: 16-byte aligned, whole chunks
-// along the contiguous axis, and a tile's byte offsets within 31 bits.
-inline bool direct_ok(const void *p, long long ld, long long stride, int contiguous, int es) {
+// Rows of whole 16-byte chunks.
+inline bool whole_chunks(const void *p, long long ld, long long stride, int contiguous, int es) {
     return (((uintptr_t)p | (uintptr_t)(ld * es) | (uintptr_t)(stride * es)) & 15) == 0 &&
-           (long long)contiguous * es % 16 == 0 && ld * es < (1ll << 22);
+           (long long)contiguous * es % 16 == 0;
 }
+// A tile's byte offsets (up to 255 rows) within 31 bits.
+inline bool tile_offsets_ok(long long ld, int es) { return ld * es < (1ll << 22); }
 
 template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int KSUB, int NS, int WPE>
-hipError_t launch_tiles(OpGemmArgs g, bool direct, hipStream_t s) {
+hipError_t launch_tiles(OpGemmArgs g, int vb, hipStream_t s) {
     g.nt = (g.N + BN - 1) / BN;
     g.mt = RAGK ? (g.M + BM - 1) / BM : 0;
     // ragged rows: sum of ceil(rows_e / BM) <= rows / BM + the groups that can hold a row
@@ -835,13 +866,24 @@ hipError_t launch_tiles(OpGemmArgs g, bool direct, hipStream_t s) {
     const long long grid = RAGK ? ((long long)g.mt * g.nt * g.splits + 7) / 8 * 8 * g.E : (mtiles * g.nt + 7) / 8 * 8;
     if (grid > 0x7fffffffll / (WM * WN * 64)) return hipErrorInvalidValue;
     const dim3 b(WM * WN * 64);
-    if constexpr (BN == 256) {  // (staging through registers leaves too few for these tiles)
-        if (!direct) return hipErrorInvalidValue;
-        op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, KSUB, NS, WPE, true><<<(unsigned)grid, b, 0, s>>>(g);
+#define MOE_OP_TILES(KS_, NS_, VB_) \
+    op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, KS_, NS_, WPE, VB_><<<(unsigned)grid, b, 0, s>>>(g)
+    if (vb == 16) {
+        MOE_OP_TILES(KSUB, NS, 16);
+    } else if constexpr (BN == 256) {
+        return hipErrorInvalidValue;  // (staging through registers leaves too few for these tiles)
+    } else if constexpr (OT == OT_F32) {
+        if (vb == 4) {
+            MOE_OP_TILES(1, 4, 4);
+        } else if constexpr (BM == 64) {
+            MOE_OP_TILES(1, 2, 0);  // row strides of 4 MB and more
+        } else {
+            return hipErrorInvalidValue;
+        }
     } else {
-        if (direct) op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, KSUB, NS, WPE, true><<<(unsigned)grid, b, 0, s>>>(g);
-        else op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, 1, 2, WPE, false><<<(unsigned)grid, b, 0, s>>>(g);
+        MOE_OP_TILES(1, 2, 0);
     }
+#undef MOE_OP_TILES
     hipError_t e = hipGetLastError();
     if constexpr (RAGK) {
         if (e == hipSuccess && g.splits > 1) {
@@ -863,8 +905,14 @@ hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
     constexpr int ES = op_size(OT);
     // row operands are loaded in whole 128-byte lines
     constexpr int KSUB = ACOL && BCOL ? 1 : 2;
-    const bool direct =
-        direct_ok(g.A, g.lda, 0, ACOL ? g.M : g.K, ES) && direct_ok(g.B, g.ldb, g.b_stride, BCOL ? g.N : g.K, ES);
+    // bytes a lane loads straight into LDS; 0: through registers
+    int vb = 0;
+    if (tile_offsets_ok(g.lda, ES) && tile_offsets_ok(g.ldb, ES)) {
+        if (whole_chunks(g.A, g.lda, 0, ACOL ? g.M : g.K, ES) && whole_chunks(g.B, g.ldb, g.b_stride, BCOL ? g.N : g.K, ES))
+            vb = 16;
+        else if (OT == OT_F32)
+            vb = 4;
+    }
     auto tiles = [&](int b) -> long long {
         const long long nt = (g.N + b - 1) / b;
         if (RAGK) return nt * ((g.M + b - 1) / b) * g.E;
@@ -875,12 +923,12 @@ hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
     if constexpr (OT != OT_F32) {
         // ragged k: a group that holds most rows has to fill the GPU by itself
         const bool large = RAGK ? tiles(256) >= g.E * (long long)(ncu / 2) : avg >= 192 && g.N >= 192 && tiles(256) >= 2 * ncu;
-        if (direct && large)
-            return launch_tiles<OT, ACOL, BCOL, RAGK, 256, 256, 4, 2, KSUB, 4 / KSUB, 2>(g, direct, s);
+        if (vb == 16 && large)
+            return launch_tiles<OT, ACOL, BCOL, RAGK, 256, 256, 4, 2, KSUB, 4 / KSUB, 2>(g, vb, s);
     }
-    if (avg >= 64 && g.N >= 64 && tiles(128) >= ncu)
-        return launch_tiles<OT, ACOL, BCOL, RAGK, 128, 128, 2, 2, KSUB, 4 / KSUB, 2>(g, direct, s);
-    return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, KSUB, 4 / KSUB, 3>(g, direct, s);
+    if (!(OT == OT_F32 && vb == 0) && avg >= 64 && g.N >= 64 && tiles(128) >= ncu)
+        return launch_tiles<OT, ACOL, BCOL, RAGK, 128, 128, 2, 2, KSUB, 4 / KSUB, 2>(g, vb, s);
+    return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, KSUB, 4 / KSUB, 3>(g, vb, s);
 }
 
 }  // namespace ops
