@@ -881,7 +881,7 @@ hipError_t launch_tiles(OpGemmArgs g, int vb, hipStream_t s) {
             return hipErrorInvalidValue;
         }
     } else {
-        MOE_OP_TILES(1, 2, 0);
+        MOE_OP_TILES(2, 2, 0);
     }
 #undef MOE_OP_TILES
     hipError_t e = hipGetLastError();
