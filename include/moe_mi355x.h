@@ -416,15 +416,22 @@ int moe_read_counts(moe_handle *h, int32_t *counts);
  * [in_dim][out_dim], rows ldw apart.  dtype: MOE_F32 or MOE_BF16 operands; sums
  * in fp32; the result in MOE_F32 or (bf16 operands) MOE_BF16, rounded once. */
 
-/* y[r] = W_e x[r] for the rows r of group e.  x [rows][in_dim], y [rows][out_dim]. */
+/* y[r] = W_e x[r] for the rows r of group e.  x [rows][in_dim], y [rows][out_dim].
+ * workspace: 16-byte aligned, the bytes that moe_grouped_matmul_workspace gives
+ * for these sizes (few rows and columns of a long sum are split over
+ * workgroups; 0 otherwise: NULL is fine then), for either layout and for
+ * moe_grouped_matmul_grad_x_async too. */
+int moe_grouped_matmul_workspace(int32_t groups, int32_t rows, int32_t in_dim, int32_t out_dim, int32_t dtype,
+                                 int64_t *bytes);
 int moe_grouped_matmul_async(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t w_stride, int32_t layout,
                              const int32_t *offsets, int32_t groups, int32_t rows, int32_t in_dim, int32_t out_dim,
-                             int32_t dtype, void *y, int64_t ldy, int32_t y_dtype, void *stream);
+                             int32_t dtype, void *y, int64_t ldy, int32_t y_dtype, void *workspace,
+                             int64_t workspace_bytes, void *stream);
 /* Its gradient with respect to x: dx[r] = W_e' dy[r]. */
 int moe_grouped_matmul_grad_x_async(const void *dy, int64_t lddy, const void *w, int64_t ldw, int64_t w_stride,
                                     int32_t layout, const int32_t *offsets, int32_t groups, int32_t rows,
                                     int32_t in_dim, int32_t out_dim, int32_t dtype, void *dx, int64_t lddx,
-                                    int32_t dx_dtype, void *stream);
+                                    int32_t dx_dtype, void *workspace, int64_t workspace_bytes, void *stream);
 /* Its gradient with respect to W, in W's layout: dW_e = sum over the rows of
  * group e of dy[r] x[r]', zeros for an empty group.  accumulate != 0 adds to
  * what dw holds (in fp32, rounded once) instead.  workspace: 16-byte aligned,
@@ -448,11 +455,12 @@ int moe_quantize_int8_async(const void *x, int64_t ldx, int32_t x_dtype, int64_t
 /* y[r][n] = x_scale[r] w_scale[e][n] sum_k q[r][k] w[e][n][k], summed exactly
  * in int32 (in_dim <= 131071).  x_dtype MOE_INT8: x holds the codes and
  * x_scale [rows] their scales.  MOE_BF16 or MOE_F32: the rows are quantised as
- * moe_quantize_int8_async does, into the workspace (16-byte aligned,
- * moe_int8_matmul_workspace bytes; not needed for codes), and x_scale is not
- * read.  w: codes [groups][out_dim][in_dim], w_scale [groups][out_dim]; y
+ * moe_quantize_int8_async does, into the workspace, and x_scale is not read.
+ * workspace: 16-byte aligned, the bytes that moe_int8_matmul_workspace gives
+ * for these sizes (0 for codes, unless a long sum is split over workgroups).  w: codes [groups][out_dim][in_dim], w_scale [groups][out_dim]; y
  * MOE_F32 or MOE_BF16. */
-int moe_int8_matmul_workspace(int32_t rows, int32_t in_dim, int64_t *bytes);
+int moe_int8_matmul_workspace(int32_t groups, int32_t rows, int32_t in_dim, int32_t out_dim, int32_t x_dtype,
+                              int64_t *bytes);
 int moe_int8_matmul_async(const void *x, int64_t ldx, int32_t x_dtype, const float *x_scale, const void *w,
                           int64_t ldw, int64_t w_stride, const float *w_scale, const int32_t *offsets, int32_t groups,
                           int32_t rows, int32_t in_dim, int32_t out_dim, void *y, int64_t ldy, int32_t y_dtype,

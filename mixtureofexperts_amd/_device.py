@@ -45,6 +45,7 @@ class DeviceLayer:
         self.num_experts = num_experts
         self.output_dim = output_dim
         self.input_dim = input_dim
+        self._side = None  # forward_device's stream beside torch's default one
         h = ctypes.c_void_p()
         _lib.check(_lib.lib().moe_create(ctypes.byref(c), ctypes.byref(h)), None)
         self.h = h
@@ -177,13 +178,27 @@ class DeviceLayer:
         loss = torch.zeros(1, dtype=torch.float32, device=x.device)
         if T == 0:
             return out, loss
-        L, stream = _lib.lib(), torch.cuda.current_stream(x.device).cuda_stream
+        current = torch.cuda.current_stream(x.device)
+        stream = current
+        if current.cuda_stream == 0:
+            # torch's default stream is the null stream, which these calls take to
+            # mean the handle's own: run on a stream that waits for it, and make
+            # it wait in turn
+            if self._side is None:
+                self._side = torch.cuda.Stream(x.device)
+            stream = self._side
+            stream.wait_stream(current)
+        L = _lib.lib()
         if decode:
-            st = L.moe_decode_async(self.h, x.data_ptr(), T, out.data_ptr(), stream)
+            st = L.moe_decode_async(self.h, x.data_ptr(), T, out.data_ptr(), stream.cuda_stream)
         else:
             code = _lib.MOE_BF16 if x.dtype == torch.bfloat16 else _lib.MOE_F32
             st = L.moe_forward_async(self.h, x.data_ptr(), code, T, int(bool(training)), out.data_ptr(),
-                                     loss.data_ptr(), stream)
+                                     loss.data_ptr(), stream.cuda_stream)
+        if stream is not current:
+            # after this wait the current stream owns the tensors again, so their
+            # memory may be reused in its order
+            current.wait_stream(stream)
         _lib.check(st, self.h)
         return out, loss
 

@@ -42,7 +42,7 @@ EXPORTED_SYMBOLS = [
     "moe_read_counts", "moe_switch_loss", "moe_z_loss", "moe_decode", "moe_decode_async",
     "moe_set_aux_free", "moe_get_aux_free", "moe_aux_free_update_bias", "moe_forward_routed",
     "moe_init_experts_from_dense", "moe_get_expert", "moe_switch_loss_noalloc",
-    "moe_grouped_matmul_async", "moe_grouped_matmul_grad_x_async", "moe_grouped_matmul_grad_w_async",
+    "moe_grouped_matmul_async", "moe_grouped_matmul_workspace", "moe_grouped_matmul_grad_x_async", "moe_grouped_matmul_grad_w_async",
     "moe_grouped_matmul_grad_w_workspace", "moe_quantize_int8_async", "moe_int8_matmul_async",
     "moe_int8_matmul_workspace", "moe_block_norm_async", "moe_block_norm_grad_async", "moe_block_norm_grad_workspace",
 ]
@@ -153,14 +153,15 @@ def lib():
     L.moe_init_experts_from_dense.argtypes = [vp, i32, i32, vp, vp, vp, vp, vp, vp, i32, f32, ctypes.c_uint64]
     L.moe_get_expert.argtypes = [vp, i32, i32, vp, vp, vp, vp, vp, vp]
     i64p = ctypes.POINTER(i64)
-    rows = [vp, i64, vp, i64, i64, i32, vp, i32, i32, i32, i32, i32, vp, i64, i32, vp]
+    rows = [vp, i64, vp, i64, i64, i32, vp, i32, i32, i32, i32, i32, vp, i64, i32, vp, i64, vp]
+    L.moe_grouped_matmul_workspace.argtypes = [i32, i32, i32, i32, i32, i64p]
     L.moe_grouped_matmul_async.argtypes = rows
     L.moe_grouped_matmul_grad_x_async.argtypes = rows
     L.moe_grouped_matmul_grad_w_workspace.argtypes = [i32, i32, i32, i32, i64p]
     L.moe_grouped_matmul_grad_w_async.argtypes = [vp, i64, vp, i64, i32, vp, i32, i32, i32, i32, i32, vp, i64, i64, i32,
                                                   i32, vp, i64, vp]
     L.moe_quantize_int8_async.argtypes = [vp, i64, i32, i64, i32, vp, i64, vp, vp]
-    L.moe_int8_matmul_workspace.argtypes = [i32, i32, i64p]
+    L.moe_int8_matmul_workspace.argtypes = [i32, i32, i32, i32, i32, i64p]
     L.moe_int8_matmul_async.argtypes = [vp, i64, i32, vp, vp, i64, i64, vp, vp, i32, i32, i32, i32, vp, i64, i32, vp,
                                         i64, vp]
     L.moe_block_norm_async.argtypes = [vp, i32, vp, i32, vp, vp, i32, vp, i32, i64, f32, f32, f32, i64, i32, vp, vp,

@@ -44,13 +44,18 @@ int op_check_dtypes(const char *fn, int32_t dtype, int32_t out_dtype) {
     if (dtype == MOE_F32 && out_dtype != MOE_F32) return op_fail(fn, "fp32 operands have an fp32 result");
     return MOE_OK;
 }
+int op_check_workspace(const char *fn, int64_t need, const void *workspace, int64_t bytes) {
+    if (need > 0 && (!workspace || bytes < need || ((uintptr_t)workspace & 15)))
+        return op_fail(fn, "the workspace must be 16-byte aligned and hold " + std::to_string(need) + " bytes");
+    return MOE_OK;
+}
 bool op_misaligned(const void *p, int32_t dtype) { return ((uintptr_t)p & (dtype == MOE_F32 ? 3 : 1)) != 0; }
 
 // y[r] = W_e x[r] (grad: dx[r] = W_e^T dy[r]) on rows of k elements -> n
 int op_rows_product(const char *fn, bool grad, const void *x, int64_t ldx, const void *w, int64_t ldw,
                     int64_t w_stride, int32_t layout, const int32_t *offsets, int32_t groups, int32_t rows,
                     int32_t in_dim, int32_t out_dim, int32_t dtype, void *y, int64_t ldy, int32_t y_dtype,
-                    void *stream) {
+                    void *workspace, int64_t workspace_bytes, void *stream) {
     int r = op_check_groups(fn, offsets, groups, rows, in_dim, out_dim);
     if (r == MOE_OK) r = op_check_dtypes(fn, dtype, y_dtype);
     if (r != MOE_OK) return r;
@@ -69,32 +74,34 @@ int op_rows_product(const char *fn, bool grad, const void *x, int64_t ldx, const
     g.lda = ldx, g.ldb = ldw, g.ldc = ldy;
     g.b_stride = groups > 1 ? w_stride : 0;
     g.offsets = offsets, g.E = groups, g.rows = rows;
-    g.N = n, g.K = k, g.c_f32 = y_dtype == MOE_F32, g.splits = 1;
+    g.N = n, g.K = k, g.c_f32 = y_dtype == MOE_F32;
     // the weight is a "row" operand where its contiguous axis is the product's k
     const bool b_col = flux != grad;
+    g.splits = op_rows_splits(dtype == MOE_F32 ? OT_F32 : OT_BF16, b_col, rows, groups, n, k, op_cus());
+    g.ws = (float *)workspace;
+    r = op_check_workspace(fn, g.splits > 1 ? (int64_t)4 * g.splits * rows * n : 0, workspace, workspace_bytes);
+    if (r != MOE_OK) return r;
     return op_done(fn, dtype == MOE_F32 ? launch_op_gemm_f32(false, b_col, false, g, op_cus(), (hipStream_t)stream)
                                         : launch_op_gemm_bf16(false, b_col, false, g, op_cus(), (hipStream_t)stream));
 }
-
-// Ranges a group's rows are split into for the weight gradient (1: none).
-int op_wgrad_splits(int32_t, int32_t, int32_t, int32_t) { return 1; }
 }  // namespace
 
 extern "C" {
 
 int moe_grouped_matmul_async(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t w_stride, int32_t layout,
                              const int32_t *offsets, int32_t groups, int32_t rows, int32_t in_dim, int32_t out_dim,
-                             int32_t dtype, void *y, int64_t ldy, int32_t y_dtype, void *stream) {
+                             int32_t dtype, void *y, int64_t ldy, int32_t y_dtype, void *workspace,
+                             int64_t workspace_bytes, void *stream) {
     return op_rows_product("moe_grouped_matmul_async", false, x, ldx, w, ldw, w_stride, layout, offsets, groups, rows,
-                           in_dim, out_dim, dtype, y, ldy, y_dtype, stream);
+                           in_dim, out_dim, dtype, y, ldy, y_dtype, workspace, workspace_bytes, stream);
 }
 
 int moe_grouped_matmul_grad_x_async(const void *dy, int64_t lddy, const void *w, int64_t ldw, int64_t w_stride,
                                     int32_t layout, const int32_t *offsets, int32_t groups, int32_t rows,
                                     int32_t in_dim, int32_t out_dim, int32_t dtype, void *dx, int64_t lddx,
-                                    int32_t dx_dtype, void *stream) {
+                                    int32_t dx_dtype, void *workspace, int64_t workspace_bytes, void *stream) {
     return op_rows_product("moe_grouped_matmul_grad_x_async", true, dy, lddy, w, ldw, w_stride, layout, offsets,
-                           groups, rows, in_dim, out_dim, dtype, dx, lddx, dx_dtype, stream);
+                           groups, rows, in_dim, out_dim, dtype, dx, lddx, dx_dtype, workspace, workspace_bytes, stream);
 }
 
 int moe_grouped_matmul_grad_w_workspace(int32_t groups, int32_t rows, int32_t in_dim, int32_t out_dim,
@@ -103,8 +110,28 @@ int moe_grouped_matmul_grad_w_workspace(int32_t groups, int32_t rows, int32_t in
     if (!bytes) return op_fail(fn, "null bytes");
     int r = op_check_groups(fn, (const int32_t *)bytes, groups, rows, in_dim, out_dim);
     if (r != MOE_OK) return r;
-    const int splits = op_wgrad_splits(groups, rows, in_dim, out_dim);
+    const int splits = op_matrix_splits(rows, groups, in_dim, out_dim, op_cus());
     *bytes = splits > 1 ? (int64_t)4 * splits * groups * in_dim * out_dim : 0;
+    return MOE_OK;
+}
+
+int moe_grouped_matmul_workspace(int32_t groups, int32_t rows, int32_t in_dim, int32_t out_dim, int32_t dtype,
+                                 int64_t *bytes) {
+    const char *fn = "moe_grouped_matmul_workspace";
+    if (!bytes) return op_fail(fn, "null bytes");
+    int r = op_check_groups(fn, (const int32_t *)bytes, groups, rows, in_dim, out_dim);
+    if (r == MOE_OK) r = op_check_dtypes(fn, dtype, MOE_F32);
+    if (r != MOE_OK) return r;
+    *bytes = 0;
+    if (rows == 0) return MOE_OK;
+    // enough for either layout, forward or row gradient
+    const int ot = dtype == MOE_F32 ? OT_F32 : OT_BF16;
+    for (const bool col : {false, true}) {
+        const int s = op_rows_splits(ot, col, rows, groups, out_dim, in_dim, op_cus());
+        const int t = op_rows_splits(ot, col, rows, groups, in_dim, out_dim, op_cus());
+        if (s > 1) *bytes = std::max(*bytes, (int64_t)4 * s * rows * out_dim);
+        if (t > 1) *bytes = std::max(*bytes, (int64_t)4 * t * rows * in_dim);
+    }
     return MOE_OK;
 }
 
@@ -129,15 +156,15 @@ int moe_grouped_matmul_grad_w_async(const void *x, int64_t ldx, const void *dy, 
     int64_t need = 0;
     r = moe_grouped_matmul_grad_w_workspace(groups, rows, in_dim, out_dim, &need);
     if (r != MOE_OK) return r;
-    if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
-        return op_fail(fn, "the workspace must be 16-byte aligned and hold " + std::to_string(need) + " bytes");
+    r = op_check_workspace(fn, need, workspace, workspace_bytes);
+    if (r != MOE_OK) return r;
     OpGemmArgs g{};
     g.A = flux ? x : dy, g.B = flux ? dy : x, g.C = dw;
     g.lda = flux ? ldx : lddy, g.ldb = flux ? lddy : ldx, g.ldc = lddw;
     g.c_stride = groups > 1 ? dw_stride : 0;
     g.offsets = offsets, g.E = groups, g.rows = rows;
     g.M = m, g.N = n, g.c_f32 = dw_dtype == MOE_F32, g.accumulate = accumulate != 0;
-    g.splits = op_wgrad_splits(groups, rows, in_dim, out_dim);
+    g.splits = op_matrix_splits(rows, groups, m, n, op_cus());
     g.ws = (float *)workspace;
     return op_done(fn, dtype == MOE_F32 ? launch_op_gemm_f32(true, true, true, g, op_cus(), (hipStream_t)stream)
                                         : launch_op_gemm_bf16(true, true, true, g, op_cus(), (hipStream_t)stream));
@@ -158,12 +185,21 @@ int moe_quantize_int8_async(const void *x, int64_t ldx, int32_t x_dtype, int64_t
                                           (hipStream_t)stream));
 }
 
-int moe_int8_matmul_workspace(int32_t rows, int32_t in_dim, int64_t *bytes) {
+// Workspace of the int8 product: partial sums, then the rows' scales and codes
+// (padded to 16 bytes) where the call quantises them.
+static int64_t int8_partial_bytes(int32_t groups, int32_t rows, int32_t in_dim, int32_t out_dim) {
+    const int s = op_rows_splits(OT_I8, false, rows, groups, out_dim, in_dim, op_cus());
+    return s > 1 ? round_up((int64_t)4 * s * rows * out_dim, 16) : 0;
+}
+
+int moe_int8_matmul_workspace(int32_t groups, int32_t rows, int32_t in_dim, int32_t out_dim, int32_t x_dtype,
+                              int64_t *bytes) {
     const char *fn = "moe_int8_matmul_workspace";
     if (!bytes) return op_fail(fn, "null bytes");
-    if (rows < 0 || in_dim < 1) return op_fail(fn, "rows must not be negative and in_dim positive");
-    // scales, then the codes, rows padded to 16 bytes
-    *bytes = round_up((int64_t)rows * 4, 16) + (int64_t)rows * round_up(in_dim, 16);
+    const int r = op_check_groups(fn, (const int32_t *)bytes, groups, rows, in_dim, out_dim);
+    if (r != MOE_OK) return r;
+    *bytes = rows > 0 ? int8_partial_bytes(groups, rows, in_dim, out_dim) : 0;
+    if (x_dtype != MOE_INT8) *bytes += round_up((int64_t)rows * 4, 16) + (int64_t)rows * round_up(in_dim, 16);
     return MOE_OK;
 }
 
@@ -188,14 +224,13 @@ int moe_int8_matmul_async(const void *x, int64_t ldx, int32_t x_dtype, const flo
         (codes && op_misaligned(x_scale, MOE_F32)))
         return op_fail(fn, "a buffer is not aligned to its elements");
     if (rows > INT_MAX / 256) return op_fail(fn, "too many rows");
+    int64_t need = 0;
+    r = moe_int8_matmul_workspace(groups, rows, in_dim, out_dim, x_dtype, &need);
+    if (r == MOE_OK) r = op_check_workspace(fn, need, workspace, workspace_bytes);
+    if (r != MOE_OK) return r;
     if (!codes) {
-        int64_t need = 0;
-        r = moe_int8_matmul_workspace(rows, in_dim, &need);
-        if (r != MOE_OK) return r;
-        if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))
-            return op_fail(fn, "the workspace must be 16-byte aligned and hold " + std::to_string(need) + " bytes");
-        float *sx = (float *)workspace;
-        int8_t *q = (int8_t *)workspace + round_up((int64_t)rows * 4, 16);
+        float *sx = (float *)((uint8_t *)workspace + int8_partial_bytes(groups, rows, in_dim, out_dim));
+        int8_t *q = (int8_t *)sx + round_up((int64_t)rows * 4, 16);
         const int64_t ldq = round_up(in_dim, 16);
         r = op_done(fn, launch_quantize_i8(x, ldx, x_dtype == MOE_BF16, rows, in_dim, q, ldq, (int)ldq, sx,
                                            (hipStream_t)stream));
@@ -207,7 +242,9 @@ int moe_int8_matmul_async(const void *x, int64_t ldx, int32_t x_dtype, const flo
     g.lda = ldx, g.ldb = ldw, g.ldc = ldy;
     g.b_stride = groups > 1 ? w_stride : 0;
     g.offsets = offsets, g.E = groups, g.rows = rows;
-    g.N = out_dim, g.K = in_dim, g.c_f32 = y_dtype == MOE_F32, g.splits = 1;
+    g.N = out_dim, g.K = in_dim, g.c_f32 = y_dtype == MOE_F32;
+    g.splits = op_rows_splits(OT_I8, false, rows, groups, out_dim, in_dim, op_cus());
+    g.ws = (float *)workspace;
     g.sa = x_scale, g.sb = w_scale;
     return op_done(fn, launch_op_gemm_i8(g, op_cus(), (hipStream_t)stream));
 }

@@ -567,19 +567,27 @@ hipError_t launch_decode_ffn(const DecodeArgs &a, int ncu, hipStream_t s, hipEve
     }
 }
 
-// ---- products of few rows per group, row quantisation (moe_ops_stream.h) ------------
-// Up to 16 rows per group on average.
-bool op_stream_fits(int, const OpGemmArgs &g) { return (long long)g.rows <= 16ll * g.E; }
-
+// ---- products of few rows per group, folds, row quantisation (moe_ops_stream.h) ----
 hipError_t launch_op_stream(int ot, const OpGemmArgs &g0, hipStream_t s) {
     OpGemmArgs g = g0;
     g.nt = (g.N + 15) / 16;
     const long long grid = (long long)g.E * g.nt;
-    if (grid > 0x7fffffffll / (ops::kStreamWaves * 64)) return hipErrorInvalidValue;
-    const dim3 b(ops::kStreamWaves * 64);
-    if (ot == OT_F32) ops::op_stream_kernel<OT_F32><<<(unsigned)grid, b, 0, s>>>(g);
-    else if (ot == OT_BF16) ops::op_stream_kernel<OT_BF16><<<(unsigned)grid, b, 0, s>>>(g);
-    else ops::op_stream_kernel<OT_I8><<<(unsigned)grid, b, 0, s>>>(g);
+    if (grid * g.splits > 0x7fffffffll / (ops::kStreamWaves * 64)) return hipErrorInvalidValue;
+    const dim3 gr((unsigned)grid, g.splits), b(ops::kStreamWaves * 64);
+    if (ot == OT_F32) ops::op_stream_kernel<OT_F32><<<gr, b, 0, s>>>(g);
+    else if (ot == OT_BF16) ops::op_stream_kernel<OT_BF16><<<gr, b, 0, s>>>(g);
+    else ops::op_stream_kernel<OT_I8><<<gr, b, 0, s>>>(g);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess && g.splits > 1 ? launch_op_fold(ot, false, g, s) : e;
+}
+
+hipError_t launch_op_fold(int ot, bool ragged_k, const OpGemmArgs &g, hipStream_t s) {
+    const long long n = ragged_k ? (long long)g.E * g.M * g.N : (long long)g.rows * g.N;
+    const long long blocks = (n + 255) / 256;
+    if (blocks > 0x7fffffffll / 256) return hipErrorInvalidValue;
+    if (ot == OT_I8) ops::op_fold_kernel<OT_I8, false><<<(unsigned)blocks, 256, 0, s>>>(g);
+    else if (ragged_k) ops::op_fold_kernel<OT_BF16, true><<<(unsigned)blocks, 256, 0, s>>>(g);
+    else ops::op_fold_kernel<OT_BF16, false><<<(unsigned)blocks, 256, 0, s>>>(g);
     return hipGetLastError();
 }
 

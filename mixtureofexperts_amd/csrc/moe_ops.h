@@ -31,8 +31,8 @@ struct OpGemmArgs {
     int accumulate;                // ragged k: C += (fp32 sums, one rounding)
     const float *sa;               // int8: scale per row of A
     const float *sb;               // int8: scale per group and column [E][N]
-    float *ws;                     // ragged k: partial sums of split groups
-    int splits;                    // ragged k: ranges a group's rows are split into (1: none)
+    float *ws;                     // partial sums (splits > 1), [range][rows][N] or [group][range][M][N]
+    int splits;                    // ranges that k is split into over workgroups (1: none)
     int nt, mt;                    // tiles along N, and (ragged k) along M
 };
 
@@ -46,13 +46,39 @@ __device__ __forceinline__ void op_group(const int *offsets, int e, int rows, in
     }
 }
 
+// Few rows per group and the weights as rows: streamed (moe_ops_stream.h).
+inline bool op_streamed(bool b_col, long long rows, long long E) { return !b_col && rows <= 16 * E; }
+
+constexpr int kOpMaxSplits = 16;
+// Ranges of k for `tiles` workgroups of a call, so that the GPU is filled:
+// none where half its CUs have one, no range shorter than `least`.
+inline int op_splits(long long tiles, long long k, long long least, int ncu) {
+    if (tiles < 1 || 2 * tiles > ncu) return 1;
+    long long s = (ncu + tiles - 1) / tiles;
+    if (s > k / least) s = k / least;
+    if (s > kOpMaxSplits) s = kOpMaxSplits;
+    return s > 1 ? (int)s : 1;
+}
+// Ragged rows: by 64 x 64 tiles, or the streamed products' 16 columns.
+inline int op_rows_splits(int ot, bool b_col, long long rows, long long E, long long N, long long K, int ncu) {
+    const long long held = E < rows ? E : rows;  // groups that may hold rows
+    if (op_streamed(b_col, rows, E)) return op_splits(held * ((N + 15) / 16), K * op_size(ot), 2048, ncu);
+    const long long mt = (rows + 63) / 64;
+    return op_splits((mt > held ? mt : held) * ((N + 63) / 64), K, 256, ncu);
+}
+// Ragged k: the rows of each group.
+inline int op_matrix_splits(long long rows, long long E, long long M, long long N, int ncu) {
+    return op_splits(E * ((M + 63) / 64) * ((N + 63) / 64), rows / E, 256, ncu);
+}
+
 // a_col / b_col as above; the launchers pick tile and load form (op_gemm_plan)
 hipError_t launch_op_gemm_f32(bool a_col, bool b_col, bool ragged_k, OpGemmArgs g, int ncu, hipStream_t s);
 hipError_t launch_op_gemm_bf16(bool a_col, bool b_col, bool ragged_k, OpGemmArgs g, int ncu, hipStream_t s);
 hipError_t launch_op_gemm_i8(OpGemmArgs g, int ncu, hipStream_t s);
 // few rows per group, both operands "row": the weights streamed once
 hipError_t launch_op_stream(int ot, const OpGemmArgs &g, hipStream_t s);
-bool op_stream_fits(int ot, const OpGemmArgs &g);
+// C of a call whose k was split: its ranges' sums, in range order
+hipError_t launch_op_fold(int ot, bool ragged_k, const OpGemmArgs &g, hipStream_t s);
 
 // q[r][k] = rne(127 x[r][k] / max|x[r]|) as int8, scale[r] = max|x[r]| / 127;
 // columns [cols, ldq) are not written past pad_to (zeros up to it)

@@ -40,6 +40,9 @@ using num = std::integral_constant<int, N>;
 template <int OT>
 using acc_t = std::conditional_t<OT == OT_I8, i32x4, f32x4>;
 
+template <int OT>
+using acc_elem = std::conditional_t<OT == OT_I8, int, float>;
+
 template <int N>
 __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -185,8 +188,8 @@ struct Tile {
         const unsigned long long a =
             ((unsigned long long)base_hi << 32 | base_lo) + (COL ? (long long)k0 * ldb : (long long)k0 * ES);
         u32x4 rs;
-        rs[0] = (unsigned)a;
-        rs[1] = (unsigned)(a >> 32) & 0xffffu;
+        rs[0] = __builtin_amdgcn_readfirstlane((unsigned)a);
+        rs[1] = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32) & 0xffffu);
         rs[2] = 0x7fffffffu;
         rs[3] = 0x00027000u;
         const int krem = klen - k0;
@@ -296,7 +299,7 @@ struct OpJob {
     int e;         // group
     int m0, n0;    // tile origin (ragged rows: m0 counted from the group's first row)
     int lo, len;   // the group's first row and rows
-    int ks, nks;   // ragged k: range of the group's rows
+    int ks;        // range of k (of g.splits)
 };
 
 // M tiles per block of the order (block, n tile, M tile): a group of many M
@@ -330,11 +333,13 @@ __device__ __forceinline__ bool ragged_job(const OpGemmArgs &g, OpJob &jb, int B
         t = scan(base, lo, len);
         W += __shfl(t, 63);
     }
-    W *= NT;
+    W *= NT * g.splits;
     // contiguous per-XCD ranges (block L runs on XCD L mod 8)
     const int per = (W + 7) >> 3, slot = blockIdx.x >> 3;
     int item = (blockIdx.x & 7) * per + slot;
     if (slot >= per || item >= W) return false;
+    jb.ks = __builtin_amdgcn_readfirstlane(item % g.splits);
+    item = __builtin_amdgcn_readfirstlane(item / g.splits);
     for (int base = 0; base < g.E; base += 64) {
         if (g.E > 64) t = scan(base, lo, len);
         const unsigned long long past = __ballot(t * NT > item);
@@ -362,8 +367,6 @@ __device__ __forceinline__ bool ragged_job(const OpGemmArgs &g, OpJob &jb, int B
             jb.e = __builtin_amdgcn_readfirstlane(jb.e);
             jb.lo = __builtin_amdgcn_readfirstlane(jb.lo);
             jb.len = __builtin_amdgcn_readfirstlane(jb.len);
-            jb.ks = 0;
-            jb.nks = 1;
             return true;
         }
         item -= __shfl(t, 63) * NT;
@@ -431,7 +434,6 @@ __device__ __forceinline__ bool matrix_job(const OpGemmArgs &g, OpJob &jb, int B
     jb.e = __builtin_amdgcn_readfirstlane(longest_group(g, r, lo, hi));
     jb.ks = item / (g.mt * g.nt);
     item -= jb.ks * (g.mt * g.nt);
-    jb.nks = g.splits;
     const int nfb = g.mt / kOpMBlock, infull = nfb * kOpMBlock * g.nt;
     int m, n;
     if (item < infull) {
@@ -445,8 +447,8 @@ __device__ __forceinline__ bool matrix_job(const OpGemmArgs &g, OpJob &jb, int B
     }
     jb.m0 = m * BM;
     jb.n0 = n * BN;
-    if (jb.nks > 1) {  // equal ranges of whole stages
-        const int chunk = ((hi - lo + jb.nks - 1) / jb.nks + KE - 1) / KE * KE;
+    if (g.splits > 1) {  // equal ranges of whole stages
+        const int chunk = ((hi - lo + g.splits - 1) / g.splits + KE - 1) / KE * KE;
         const int b = min(lo + jb.ks * chunk, hi);
         hi = min(b + chunk, hi);
         lo = b;
@@ -454,6 +456,17 @@ __device__ __forceinline__ bool matrix_job(const OpGemmArgs &g, OpJob &jb, int B
     jb.lo = __builtin_amdgcn_readfirstlane(lo);
     jb.len = __builtin_amdgcn_readfirstlane(hi - lo);
     return true;
+}
+
+// Range ks of k, in whole stages of KE (the last ones may be empty).
+__device__ __forceinline__ void k_range(const OpGemmArgs &g, int ks, int KE, int &k0, int &klen) {
+    k0 = 0;
+    klen = g.K;
+    if (g.splits > 1) {
+        const int chunk = ((g.K + g.splits - 1) / g.splits + KE - 1) / KE * KE;
+        k0 = __builtin_amdgcn_readfirstlane(min(ks * chunk, g.K));
+        klen = __builtin_amdgcn_readfirstlane(min(chunk, g.K - k0));
+    }
 }
 
 // ---- results ---------------------------------------------------------------------
@@ -519,7 +532,7 @@ __device__ __forceinline__ bool vec_ok(const OpGemmArgs &g) {
 template <int EO, int BM, int BN, int WM, int WN, int RING, typename Val>
 __device__ __forceinline__ void store_tile_rows(const OpGemmArgs &g, lds_u8 *ring, long long at0, int mrows, int n0,
                                                 int wm, int wn, int lane, Val val) {
-    constexpr int NT = WM * WN * 64, MI = BM / WM / 16, NJ = BN / WN / 16;
+    constexpr int NT = WM * WN * 64, NJ = BN / WN / 16;
     constexpr int CW = BN * EO, CH = CW / 16, CE = 16 / EO;
     constexpr int FIT = RING / CW, PR = FIT < BM ? FIT : BM;  // rows per pass
     static_assert(PR % (WM * 16) == 0 && BM % PR == 0 && NT % CH == 0 && PR % (NT / CH) == 0, "passes");
@@ -622,11 +635,13 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
             ta.init(A + ((long long)jb.lo * g.lda + jb.m0) * ES, g.lda * ES, g.M - jb.m0, klen);
             tb.init(B + ((long long)jb.lo * g.ldb + jb.n0) * ES, g.ldb * ES, g.N - jb.n0, klen);
         } else {
-            klen = g.K;
             static_assert(!ACOL || RAGK, "ragged rows: A is a row operand");
-            ta.init(A + ((long long)(jb.lo + jb.m0) * g.lda) * ES, g.lda * ES, jb.len - jb.m0, klen);
+            int k0;
+            k_range(g, jb.ks, KE, k0, klen);
+            ta.init(A + ((long long)(jb.lo + jb.m0) * g.lda + k0) * ES, g.lda * ES, jb.len - jb.m0, klen);
             B += (long long)jb.e * g.b_stride * ES;
-            tb.init(B + (BCOL ? (long long)jb.n0 : (long long)jb.n0 * g.ldb) * ES, g.ldb * ES, g.N - jb.n0, klen);
+            tb.init(B + (BCOL ? (long long)k0 * g.ldb + jb.n0 : (long long)jb.n0 * g.ldb + k0) * ES, g.ldb * ES,
+                    g.N - jb.n0, klen);
         }
     }
     acc_t<OT> acc[MI][NJ];
@@ -761,19 +776,21 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
     }
 
     const int r16 = lane & 15, q4 = lane >> 4;
-    if constexpr (RAGK) {
-        if (g.splits > 1) {  // a range's sums: [e][range][M][N] fp32, folded by op_fold_kernel
-            float *ws = g.ws + ((long long)(jb.e * g.splits + jb.ks) * g.M) * g.N;
+    if constexpr (BM <= 64) {  // (split calls run the smallest tiles)
+        if (g.splits > 1) {    // a range's sums, folded by op_fold_kernel
+            const long long first = RAGK ? (long long)(jb.e * g.splits + jb.ks) * g.M + jb.m0
+                                         : (long long)jb.ks * g.rows + jb.lo + jb.m0;
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
-                const int m = jb.m0 + (i * WM + wm) * 16 + r16;
-                if (m >= g.M) continue;
+                const int ml = (i * WM + wm) * 16 + r16;
+                if (ml >= mrows) continue;
+                acc_elem<OT> *ws = (acc_elem<OT> *)g.ws + (first + ml) * g.N;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
-                    const int n = jb.n0 + wn * (BN / WN) + j * 16 + 4 * q4;
+                    const int n = jb.n0 + (wn * NJ + j) * 16 + 4 * q4;
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
-                        if (n + c < g.N) ws[(long long)m * g.N + n + c] = acc[i][j][c];
+                        if (n + c < g.N) ws[n + c] = acc[i][j][c];
                 }
             }
             return;
@@ -827,27 +844,6 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WP
     op_gemm_tile<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, KSUB, NS, VB>(g, ring);
 }
 
-// C of a split group: its ranges' sums in range order, one element per thread.
-template <int DUMMY>
-__global__ __launch_bounds__(256) void op_fold_kernel(OpGemmArgs g) {
-    const long long per = (long long)g.M * g.N, total = per * g.E;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const long long e = i / per, r = i - e * per;
-        const float *ws = g.ws + e * g.splits * per + r;
-        float v = 0.0f;
-        for (int s = 0; s < g.splits; ++s) v += ws[s * per];
-        const long long m = r / g.N, n = r - m * g.N;
-        const long long at = e * g.c_stride + m * g.ldc + n;
-        if (g.c_f32) {
-            float *c = (float *)g.C + at;
-            *c = g.accumulate ? *c + v : v;
-        } else {
-            uint16_t *c = (uint16_t *)g.C + at;
-            *c = f32_to_bf16(g.accumulate ? bf16_to_f32(*c) + v : v);
-        }
-    }
-}
-
 // Rows of whole 16-byte chunks.
 inline bool whole_chunks(const void *p, long long ld, long long stride, int contiguous, int es) {
     return (((uintptr_t)p | (uintptr_t)(ld * es) | (uintptr_t)(stride * es)) & 15) == 0 &&
@@ -863,7 +859,8 @@ hipError_t launch_tiles(OpGemmArgs g, int vb, hipStream_t s) {
     // ragged rows: sum of ceil(rows_e / BM) <= rows / BM + the groups that can hold a row
     // ragged k: every XCD's part of every group
     const long long mtiles = (long long)(g.rows / BM) + (g.E < g.rows ? g.E : g.rows);
-    const long long grid = RAGK ? ((long long)g.mt * g.nt * g.splits + 7) / 8 * 8 * g.E : (mtiles * g.nt + 7) / 8 * 8;
+    const long long grid =
+        RAGK ? ((long long)g.mt * g.nt * g.splits + 7) / 8 * 8 * g.E : (mtiles * g.nt * g.splits + 7) / 8 * 8;
     if (grid > 0x7fffffffll / (WM * WN * 64)) return hipErrorInvalidValue;
     const dim3 b(WM * WN * 64);
 #define MOE_OP_TILES(KS_, NS_, VB_) \
@@ -884,22 +881,15 @@ hipError_t launch_tiles(OpGemmArgs g, int vb, hipStream_t s) {
         MOE_OP_TILES(2, 2, 0);
     }
 #undef MOE_OP_TILES
-    hipError_t e = hipGetLastError();
-    if constexpr (RAGK) {
-        if (e == hipSuccess && g.splits > 1) {
-            const long long n = ((long long)g.E * g.M * g.N + 255) / 256;
-            op_fold_kernel<0><<<(unsigned)(n < 8192 ? n : 8192), 256, 0, s>>>(g);
-            e = hipGetLastError();
-        }
-    }
-    return e;
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess && g.splits > 1 ? launch_op_fold(OT, RAGK, g, s) : e;
 }
 
 // Tile and load form of a call.  Ragged rows: 256 x 256 tiles where groups
 // average enough rows to fill them and there are two rounds of them, else
 // 128 x 128, and 64 x 64 for short groups or few tiles.  Ragged k: by the
-// tiles of all groups; where even 64 x 64 tiles are few, a group's rows are
-// split into ranges (op_wgrad_splits).
+// tiles of all groups.  Where even 64 x 64 tiles are few, k is split into
+// ranges (op_rows_splits, op_matrix_splits).
 template <int OT, bool ACOL, bool BCOL, bool RAGK>
 hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
     constexpr int ES = op_size(OT);
@@ -920,6 +910,7 @@ hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
         return nt * few;
     };
     const long long avg = RAGK ? g.M : (long long)g.rows / g.E;
+    if (g.splits > 1) return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, KSUB, 4 / KSUB, 3>(g, vb, s);
     if constexpr (OT != OT_F32) {
         // ragged k: a group that holds most rows has to fill the GPU by itself
         const bool large = RAGK ? tiles(256) >= g.E * (long long)(ncu / 2) : avg >= 192 && g.N >= 192 && tiles(256) >= 2 * ncu;

@@ -14,22 +14,25 @@ namespace ops {
 constexpr int kStreamWaves = 8;
 
 template <int OT, int MT>
-__device__ __forceinline__ void stream_rows(const OpGemmArgs &g, int e, int n0, int lo, int rows, lds_u8 *red) {
+__device__ __forceinline__ void stream_rows(const OpGemmArgs &g, int e, int n0, int lo, int rows, int ks, lds_u8 *red) {
     constexpr int ES = op_size(OT), KE = 128 / ES, CE = 16 / ES;
     constexpr int U = MT == 1 ? 4 : 2;
     const int lane = threadIdx.x & 63, r16 = lane & 15, q4 = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int k0, klen;
+    k_range(g, ks, KE, k0, klen);
     // rows past the last one repeat it (their results are not stored)
-    const uint8_t *b = (const uint8_t *)g.B + ((long long)e * g.b_stride + (long long)min(n0 + r16, g.N - 1) * g.ldb) * ES;
+    const uint8_t *b =
+        (const uint8_t *)g.B + ((long long)e * g.b_stride + (long long)min(n0 + r16, g.N - 1) * g.ldb + k0) * ES;
     const uint8_t *a[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
-        a[m] = (const uint8_t *)g.A + (long long)(lo + min(m * 16 + r16, rows - 1)) * g.lda * ES;
+        a[m] = (const uint8_t *)g.A + ((long long)(lo + min(m * 16 + r16, rows - 1)) * g.lda + k0) * ES;
     acc_t<OT> acc[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[m] = acc_t<OT>{0, 0, 0, 0};
-    const int pieces = (g.K + KE - 1) / KE;
-    const int whole = g.K / KE;
+    const int pieces = (klen + KE - 1) / KE;
+    const int whole = klen / KE;
     int p = w;
     for (; p + (U - 1) * kStreamWaves < whole; p += U * kStreamWaves) {
         u32x4 fb[U][2], fa[MT][U][2];
@@ -53,10 +56,10 @@ __device__ __forceinline__ void stream_rows(const OpGemmArgs &g, int e, int n0, 
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int k = p * KE + (h * 4 + q4) * CE;
-            const u32x4 fb = load_chunk<ES>(b + (long long)k * ES, g.K - k);
+            const u32x4 fb = load_chunk<ES>(b + (long long)k * ES, klen - k);
 #pragma unroll
             for (int m = 0; m < MT; ++m)
-                acc[m] = fma16<OT>(fb, load_chunk<ES>(a[m] + (long long)k * ES, g.K - k), acc[m]);
+                acc[m] = fma16<OT>(fb, load_chunk<ES>(a[m] + (long long)k * ES, klen - k), acc[m]);
         }
     }
     // red: [wave][MT][64 lanes] 16 bytes
@@ -69,7 +72,12 @@ __device__ __forceinline__ void stream_rows(const OpGemmArgs &g, int e, int n0, 
         acc_t<OT> v = ra[w * 64 + lane];
         for (int x = 1; x < kStreamWaves; ++x) v += ra[(x * MT + w) * 64 + lane];
         const int ml = w * 16 + r16, n = n0 + 4 * q4;
-        if (ml < rows) {
+        if (ml < rows && g.splits > 1) {  // a range's sums, folded by op_fold_kernel
+            acc_elem<OT> *ws = (acc_elem<OT> *)g.ws + ((long long)ks * g.rows + lo + ml) * g.N;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (n + c < g.N) ws[n + c] = v[c];
+        } else if (ml < rows) {
             float o[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -92,10 +100,61 @@ __global__ __launch_bounds__(kStreamWaves * 64) void op_stream_kernel(OpGemmArgs
     op_group(g.offsets, e, g.rows, lo, hi);
     while (lo < hi) {
         const int rows = min(hi - lo, 64);
-        if (rows <= 16) stream_rows<OT, 1>(g, e, n0, lo, rows, red);
-        else if (rows <= 32) stream_rows<OT, 2>(g, e, n0, lo, rows, red);
-        else stream_rows<OT, 4>(g, e, n0, lo, rows, red);
+        if (rows <= 16) stream_rows<OT, 1>(g, e, n0, lo, rows, blockIdx.y, red);
+        else if (rows <= 32) stream_rows<OT, 2>(g, e, n0, lo, rows, blockIdx.y, red);
+        else stream_rows<OT, 4>(g, e, n0, lo, rows, blockIdx.y, red);
         lo += rows;
+    }
+}
+
+// Results of a call whose k was split: the ranges' sums in range order.  One
+// element per thread.  Ragged rows: ws [range][rows][N], rows of the groups
+// only; ragged k: ws [group][range][M][N].
+template <int OT, bool RAGK>
+__global__ __launch_bounds__(256) void op_fold_kernel(OpGemmArgs g) {
+    const acc_elem<OT> *ws = (const acc_elem<OT> *)g.ws;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long per = RAGK ? (long long)g.M * g.N : (long long)g.rows * g.N;
+    long long e = 0, at = i, row = 0, n;
+    if constexpr (RAGK) {
+        e = i / per;
+        if (e >= g.E) return;
+        at = i - e * per;
+        ws += e * g.splits * per;
+        row = at / g.N;
+        n = at - row * g.N;
+    } else {
+        if (i >= per) return;
+        row = i / g.N;
+        n = i - row * g.N;
+        if (g.offsets) {
+            int lo, hi, unused;
+            op_group(g.offsets, 0, g.rows, lo, unused);
+            op_group(g.offsets, g.E - 1, g.rows, unused, hi);
+            if (row < lo || row >= hi) return;
+        }
+    }
+    acc_elem<OT> sum = 0;
+    for (int s = 0; s < g.splits; ++s) sum += ws[s * per + at];
+    float v = (float)sum;
+    if constexpr (OT == OT_I8) {
+        int a = 0;
+        if (g.offsets) {  // the last group that starts at or before the row
+            int b = g.E - 1;
+            while (a < b) {
+                const int mid = (a + b + 1) >> 1;
+                if (g.offsets[mid] <= row) a = mid; else b = mid - 1;
+            }
+        }
+        v = v * g.sa[row] * g.sb[(long long)a * g.N + n];
+    }
+    const long long c = e * g.c_stride + row * g.ldc + n;
+    if (g.c_f32) {
+        float *d = (float *)g.C + c;
+        *d = RAGK && g.accumulate ? *d + v : v;
+    } else {
+        uint16_t *d = (uint16_t *)g.C + c;
+        *d = f32_to_bf16(RAGK && g.accumulate ? bf16_to_f32(*d) + v : v);
     }
 }
 

@@ -123,6 +123,26 @@ def _call(fn, device, *args):
         _lib.check(status)
 
 
+_workspace_bytes = {}  # (query, device, sizes) -> bytes: a function of the sizes and the GPU's CUs
+
+
+def _workspace(fn, device, *sizes):
+    """(tensor or None, its address, its bytes) as the library's query asks."""
+    key = (fn.__name__, device.index, sizes)
+    n = _workspace_bytes.get(key)
+    if n is None:
+        need = ctypes.c_int64(0)
+        with _torch.cuda.device(device):
+            _lib.check(fn(*sizes, ctypes.byref(need)))
+        if len(_workspace_bytes) >= 4096:
+            _workspace_bytes.clear()
+        n = _workspace_bytes[key] = need.value
+    if n == 0:
+        return None, None, 0
+    ws = _torch.empty(n, dtype=_torch.uint8, device=device)
+    return ws, ws.data_ptr(), n
+
+
 def _layout(layout):
     if layout not in (MOE_LAYOUT_LLAMA_IN_OUT, MOE_LAYOUT_FLUX_OUT_IN):
         _bad("unknown layout")
@@ -161,9 +181,10 @@ def _rows_product(fn, x, name, w, offsets, layout, out, out_dtype, grad):
     if out is None and out_dtype is None:
         out_dtype = x.dtype
     out = _result(out, (x.shape[0], n), out_dtype, _float_types(x.dtype), x, offsets is not None)
-    device = _same_device(x, w, offsets, out)
-    _call(fn, device, xp, ldx, w.data_ptr(), ldw, stride, layout, _offsets(offsets, E), E, x.shape[0], in_dim, out_dim,
-          _codes[x.dtype], out.data_ptr(), _row_stride(out, "out"), _codes[out.dtype])
+    device, M, dt = _same_device(x, w, offsets, out), x.shape[0], _codes[x.dtype]
+    ws, wsp, wsn = _workspace(_lib.lib().moe_grouped_matmul_workspace, device, E, M, in_dim, out_dim, dt)
+    _call(fn, device, xp, ldx, w.data_ptr(), ldw, stride, layout, _offsets(offsets, E), E, M, in_dim, out_dim, dt,
+          out.data_ptr(), _row_stride(out, "out"), _codes[out.dtype], wsp, wsn)
     return out
 
 
@@ -205,12 +226,10 @@ def grouped_matmul_grad_w(x, dy, offsets=None, *, layout=MOE_LAYOUT_LLAMA_IN_OUT
     out = _result(out, shape, out_dtype, _float_types(x.dtype), x, False)
     _, _, _, ldw, stride = _matrices(out, "out", _float_types(x.dtype))
     device = _same_device(x, dy, offsets, out)
-    need = ctypes.c_int64(0)
-    _lib.check(L.moe_grouped_matmul_grad_w_workspace(E, x.shape[0], x.shape[1], dy.shape[1], ctypes.byref(need)))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    ws, wsp, wsn = _workspace(L.moe_grouped_matmul_grad_w_workspace, device, E, x.shape[0], x.shape[1], dy.shape[1])
     _call(L.moe_grouped_matmul_grad_w_async, device, xp, ldx, dp, lddy, layout, _offsets(offsets, E), E, x.shape[0],
           x.shape[1], dy.shape[1], _codes[x.dtype], out.data_ptr(), ldw, stride, _codes[out.dtype], int(accumulate),
-          ws.data_ptr() if ws is not None else None, need.value)
+          wsp, wsn)
     return out
 
 
@@ -259,13 +278,10 @@ def int8_matmul(x, w, w_scale, offsets=None, *, x_scale=None, out=None, out_dtyp
         out_dtype = torch.bfloat16
     out = _result(out, (x.shape[0], n), out_dtype, (torch.bfloat16, torch.float32), x, offsets is not None)
     device = _same_device(x, w, w_scale, x_scale, offsets, out)
-    need, ws = ctypes.c_int64(0), None
-    if not codes:
-        _lib.check(L.moe_int8_matmul_workspace(x.shape[0], k, ctypes.byref(need)))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=device)
+    ws, wsp, wsn = _workspace(L.moe_int8_matmul_workspace, device, E, x.shape[0], k, n, _codes[x.dtype])
     _call(L.moe_int8_matmul_async, device, xp, ldx, _codes[x.dtype], x_scale.data_ptr() if codes else None,
           w.data_ptr(), ldw, stride, w_scale.data_ptr(), _offsets(offsets, E), E, x.shape[0], k, n, out.data_ptr(),
-          _row_stride(out, "out"), _codes[out.dtype], ws.data_ptr() if ws is not None else None, need.value)
+          _row_stride(out, "out"), _codes[out.dtype], wsp, wsn)
     return out
 
 
@@ -380,12 +396,10 @@ def block_norm_grad(dr, dh, r, y=None, stats=None, *, pre_weight=None, post_weig
     dgate = new(gate.shape) if gate is not None else None
     dpost = new(D) if post is not None else None
     dpre = new(D) if pre is not None else None
-    need, ws = ctypes.c_int64(0), None
+    ws, wsp, wsn = None, None, 0
     if dgate is not None or dpost is not None or dpre is not None:
-        _lib.check(L.moe_block_norm_grad_workspace(T, D, gate_rows, ctypes.byref(need)))
-        if need.value:
-            ws = torch.empty(need.value, dtype=torch.uint8, device=device)
+        ws, wsp, wsn = _workspace(L.moe_block_norm_grad_workspace, device, T, D, gate_rows)
     _call(L.moe_block_norm_grad_async, device, drp, dhp, rp, _codes[r.dtype], yp, _codes[y.dtype] if y is not None else 0,
           _codes[dh.dtype] if dh is not None else 0, sp, post, pre, wt, gp, gt, gate_rows, alpha, beta, T, D,
-          dx.data_ptr(), _ptr(dy), _ptr(dgate), _ptr(dpost), _ptr(dpre), _ptr(ws), need.value)
+          dx.data_ptr(), _ptr(dy), _ptr(dgate), _ptr(dpost), _ptr(dpre), wsp, wsn)
     return dx, dy, dgate, dpost, dpre

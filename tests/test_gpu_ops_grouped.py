@@ -107,6 +107,43 @@ def test_large_tiles(moe, layout):
         at += n
 
 
+# long sums for few rows and columns: k split over workgroups, streamed and
+# tiled, whole and odd lengths
+LONG = [([1], 8192, 16), ([3, 0, 2], 4001, 125), ([71], 5440, 64), ([200, 0, 150], 3456, 131), ([40, 3], 2999, 64)]
+
+
+@pytest.mark.parametrize("layout", [LLAMA, FLUX])
+@pytest.mark.parametrize("dtype,odt", [("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32")])
+def test_long_sums(moe, dtype, odt, layout):
+    for lens, K, N in LONG:
+        print(f"grouped long sum {dtype}->{odt} layout={layout} lens={lens} K={K} N={N}", flush=True)
+        rng = np.random.default_rng([K, N, layout, 2])
+        M, E, start = sum(lens), len(lens), 2
+        x = _rows(rng, M + start, K, dtype, 0, 4)
+        w = _mats(rng, E, *((N, K) if layout == LLAMA else (K, N)), dtype, 0)
+        W, X = (_f64(w) if layout == LLAMA else _f64(w).transpose(0, 2, 1)), _f64(x)
+        out = torch.full((M + start + 4, N + 3), SENTINEL, dtype=DT[odt], device="cuda")
+        y = moe.grouped_matmul(x, w, _offsets(lens, start), layout=layout, out=out[:, :N])
+        got, at = _f64(y), start
+        for e, n in enumerate(lens):
+            a = X[at:at + n]
+            _close(got[at:at + n], a @ W[e].T, np.abs(a) @ np.abs(W[e].T), K, odt)
+            at += n
+        assert (got[:start] == SENTINEL).all() and (got[at:] == SENTINEL).all() and (_f64(out)[:, N:] == SENTINEL).all()
+
+
+@pytest.mark.parametrize("layout", [LLAMA, FLUX])
+def test_large_weight_gradient_tiles(moe, layout):
+    # 256 x 256 tiles: groups whose matrices fill the GPU by themselves
+    rng = np.random.default_rng(6)
+    lens, K, N = [70, 0, 133], 4096, 2040
+    x, dy = _rows(rng, 203, K, "bf16", 0), _rows(rng, 203, N, "bf16", 0)
+    dw = moe.grouped_matmul_grad_w(x, dy, _offsets(lens), layout=layout, out_dtype=torch.float32)
+    a, b = (_f64(dy), _f64(x)) if layout == LLAMA else (_f64(x), _f64(dy))
+    for e, s in enumerate((slice(0, 70), slice(70, 70), slice(70, 203))):
+        _close(_f64(dw[e]), a[s].T @ b[s], np.abs(a[s]).T @ np.abs(b[s]), max(lens[e], 1), "f32")
+
+
 WSHAPES = [
     ([1], 1, 1),
     ([0, 3, 0], 7, 5),

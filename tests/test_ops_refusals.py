@@ -10,7 +10,7 @@ F32, BF16, FP8, INT8 = 0, 1, 2, 3
 FLUX, LLAMA = 0, 1
 
 ROWS = dict(x=P, ldx=64, w=P, ldw=64, w_stride=64 * 32, layout=LLAMA, offsets=P, groups=4, rows=10, in_dim=64, out_dim=32,
-            dtype=BF16, y=P, ldy=32, y_dtype=BF16, stream=None)
+            dtype=BF16, y=P, ldy=32, y_dtype=BF16, workspace=None, workspace_bytes=0, stream=None)
 
 
 def _refused(moe, fn, args, msg):
@@ -67,6 +67,22 @@ def test_grad_w_refuses_a_small_workspace(moe):
                      "workspace")
     assert L.moe_grouped_matmul_grad_w_workspace(0, 1, 1, 1, ctypes.byref(n)) == _lib.MOE_EINVAL
     assert L.moe_grouped_matmul_grad_w_workspace(1, 1, 1, 1, None) == _lib.MOE_EINVAL
+
+
+def test_matmul_refuses_a_small_workspace(moe):
+    from mixtureofexperts_amd import _lib
+
+    L, n = _lib.lib(), ctypes.c_int64(-1)
+    # three rows against a narrow matrix: the long sum is split over workgroups
+    assert L.moe_grouped_matmul_workspace(1, 3, 100000, 48, BF16, ctypes.byref(n)) == 0 and n.value > 0
+    args = {**ROWS, "groups": 1, "rows": 3, "in_dim": 100000, "out_dim": 48, "ldx": 100000, "ldw": 100000, "ldy": 48}
+    for ws, size in ((None, n.value), (P + 8, n.value), (P, 16)):
+        _refused(moe, "moe_grouped_matmul_async", {**args, "workspace": ws, "workspace_bytes": size}, "workspace")
+    assert L.moe_grouped_matmul_workspace(8, 8192, 4096, 14336, BF16, ctypes.byref(n)) == 0 and n.value == 0
+    assert L.moe_grouped_matmul_workspace(1, 3, 8, 8, FP8, ctypes.byref(n)) == _lib.MOE_EINVAL
+    assert L.moe_grouped_matmul_workspace(1, 3, 8, 8, BF16, None) == _lib.MOE_EINVAL
+    assert L.moe_int8_matmul_workspace(1, 3, 100000, 48, INT8, ctypes.byref(n)) == 0 and n.value > 0
+    assert L.moe_int8_matmul_workspace(0, 3, 8, 8, INT8, ctypes.byref(n)) == _lib.MOE_EINVAL
 
 
 QUANT = dict(x=P, ldx=64, x_dtype=BF16, rows=4, cols=64, q=P, ldq=64, scale=P, stream=None)
