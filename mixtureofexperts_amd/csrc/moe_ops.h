@@ -51,7 +51,9 @@ inline bool op_streamed(bool b_col, long long rows, long long E) { return !b_col
 
 constexpr int kOpMaxSplits = 16;
 // Ranges of k for `tiles` workgroups of a call, so that the GPU is filled:
-// none where half its CUs have one, no range shorter than `least`.
+// none where half its CUs have one, no range shorter than `least` (folding the
+// ranges is a launch of its own, about 4 us: a 64 x 64 tile runs 2 KB of k per
+// row in about 16 us, the streamed form 8 KB in about 10).
 inline int op_splits(long long tiles, long long k, long long least, int ncu) {
     if (tiles < 1 || 2 * tiles > ncu) return 1;
     long long s = (ncu + tiles - 1) / tiles;
@@ -62,13 +64,13 @@ inline int op_splits(long long tiles, long long k, long long least, int ncu) {
 // Ragged rows: by 64 x 64 tiles, or the streamed products' 16 columns.
 inline int op_rows_splits(int ot, bool b_col, long long rows, long long E, long long N, long long K, int ncu) {
     const long long held = E < rows ? E : rows;  // groups that may hold rows
-    if (op_streamed(b_col, rows, E)) return op_splits(held * ((N + 15) / 16), K * op_size(ot), 2048, ncu);
+    if (op_streamed(b_col, rows, E)) return op_splits(held * ((N + 15) / 16), K * op_size(ot), 8192, ncu);
     const long long mt = (rows + 63) / 64;
-    return op_splits((mt > held ? mt : held) * ((N + 63) / 64), K, 256, ncu);
+    return op_splits((mt > held ? mt : held) * ((N + 63) / 64), K * op_size(ot), 2048, ncu);
 }
 // Ragged k: the rows of each group.
 inline int op_matrix_splits(long long rows, long long E, long long M, long long N, int ncu) {
-    return op_splits(E * ((M + 63) / 64) * ((N + 63) / 64), rows / E, 256, ncu);
+    return op_splits(E * ((M + 63) / 64) * ((N + 63) / 64), rows / E, 512, ncu);
 }
 
 // a_col / b_col as above; the launchers pick tile and load form (op_gemm_plan)

@@ -109,7 +109,7 @@ def test_large_tiles(moe, layout):
 
 # long sums for few rows and columns: k split over workgroups, streamed and
 # tiled, whole and odd lengths
-LONG = [([1], 8192, 16), ([3, 0, 2], 4001, 125), ([71], 5440, 64), ([200, 0, 150], 3456, 131), ([40, 3], 2999, 64)]
+LONG = [([1], 8192, 16), ([3, 0, 2], 4001, 125), ([3, 0, 2], 16401, 125), ([71], 5440, 64), ([200, 0, 150], 3456, 131), ([40, 3], 2999, 64)]
 
 
 @pytest.mark.parametrize("layout", [LLAMA, FLUX])
