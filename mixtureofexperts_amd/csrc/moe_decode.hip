@@ -571,7 +571,7 @@ hipError_t launch_decode_ffn(const DecodeArgs &a, int ncu, hipStream_t s, hipEve
 hipError_t launch_op_stream(int ot, const OpGemmArgs &g0, hipStream_t s) {
     OpGemmArgs g = g0;
     g.nt = (g.N + 15) / 16;
-    const long long grid = (long long)g.E * g.nt;
+    const long long grid = (long long)(g.E < g.rows ? g.E : g.rows) * g.nt;  // the groups that can hold rows
     if (grid * g.splits > 0x7fffffffll / (ops::kStreamWaves * 64)) return hipErrorInvalidValue;
     const dim3 gr((unsigned)grid, g.splits), b(ops::kStreamWaves * 64);
     if (ot == OT_F32) ops::op_stream_kernel<OT_F32><<<gr, b, 0, s>>>(g);
@@ -591,10 +591,26 @@ hipError_t launch_op_fold(int ot, bool ragged_k, const OpGemmArgs &g, hipStream_
     return hipGetLastError();
 }
 
+template <int XB, bool VEC>
+static void quantize_rows(const void *x, long long ldx, long long rows, int cols, int8_t *q, long long ldq, int pad_to,
+                          float *scale, hipStream_t s) {
+    const dim3 g((unsigned)rows), b(256);
+    if (pad_to <= 2048) ops::quantize_i8_kernel<XB, 1, VEC><<<g, b, 0, s>>>(x, ldx, cols, q, ldq, pad_to, scale);
+    else if (pad_to <= 4096) ops::quantize_i8_kernel<XB, 2, VEC><<<g, b, 0, s>>>(x, ldx, cols, q, ldq, pad_to, scale);
+    else if (pad_to <= 8192) ops::quantize_i8_kernel<XB, 4, VEC><<<g, b, 0, s>>>(x, ldx, cols, q, ldq, pad_to, scale);
+    else if (pad_to <= 16384) ops::quantize_i8_kernel<XB, 8, VEC><<<g, b, 0, s>>>(x, ldx, cols, q, ldq, pad_to, scale);
+    else ops::quantize_i8_long_kernel<XB><<<g, b, 0, s>>>(x, ldx, cols, q, ldq, pad_to, scale);
+}
+
 hipError_t launch_quantize_i8(const void *x, long long ldx, int x_bf16, long long rows, int cols, int8_t *q,
                               long long ldq, int pad_to, float *scale, hipStream_t s) {
-    if (x_bf16) ops::quantize_i8_kernel<1><<<(unsigned)rows, 256, 0, s>>>(x, ldx, cols, q, ldq, pad_to, scale);
-    else ops::quantize_i8_kernel<0><<<(unsigned)rows, 256, 0, s>>>(x, ldx, cols, q, ldq, pad_to, scale);
+    const int es = x_bf16 ? 2 : 4;
+    const bool vec = (((uintptr_t)x | (uintptr_t)(ldx * es)) & 15) == 0 && (((uintptr_t)q | (uintptr_t)ldq) & 7) == 0 &&
+                     (cols & 7) == 0 && (pad_to & 7) == 0;
+    if (x_bf16 && vec) quantize_rows<1, true>(x, ldx, rows, cols, q, ldq, pad_to, scale, s);
+    else if (x_bf16) quantize_rows<1, false>(x, ldx, rows, cols, q, ldq, pad_to, scale, s);
+    else if (vec) quantize_rows<0, true>(x, ldx, rows, cols, q, ldq, pad_to, scale, s);
+    else quantize_rows<0, false>(x, ldx, rows, cols, q, ldq, pad_to, scale, s);
     return hipGetLastError();
 }
 

@@ -2,7 +2,7 @@
 // weights are the traffic, so they go from global memory straight into MFMA
 // fragments, each read once per 16 MT rows of a group.
 //
-// A workgroup owns 16 columns of one group; its eight waves take interleaved
+// A workgroup owns 16 columns of one group; its four waves take interleaved
 // 128-byte pieces of k, U of them in flight, and their partial 16 x 16 blocks
 // are added in wave order through LDS.
 #pragma once
@@ -11,7 +11,7 @@
 namespace moe {
 namespace ops {
 
-constexpr int kStreamWaves = 8;
+constexpr int kStreamWaves = 4;
 
 template <int OT, int MT>
 __device__ __forceinline__ void stream_rows(const OpGemmArgs &g, int e, int n0, int lo, int rows, int ks, lds_u8 *red) {
@@ -52,7 +52,21 @@ __device__ __forceinline__ void stream_rows(const OpGemmArgs &g, int e, int n0, 
 #pragma unroll
                 for (int m = 0; m < MT; ++m) acc[m] = fma16<OT>(fb[u][h], fa[m][u][h], acc[m]);
     }
-    for (; p < pieces; p += kStreamWaves) {
+    for (; p < whole; p += kStreamWaves) {
+        u32x4 fb[2], fa[MT][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const long long o = (long long)p * 128 + h * 64 + q4 * 16;
+            __builtin_memcpy(&fb[h], b + o, 16);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) __builtin_memcpy(&fa[m][h], a[m] + o, 16);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[m] = fma16<OT>(fb[h], fa[m][h], acc[m]);
+    }
+    for (; p < pieces; p += kStreamWaves) {  // the last, part piece
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int k = p * KE + (h * 4 + q4) * CE;
@@ -95,9 +109,28 @@ template <int OT>
 __global__ __launch_bounds__(kStreamWaves * 64) void op_stream_kernel(OpGemmArgs g) {
     __shared__ __attribute__((aligned(16))) uint8_t red_[kStreamWaves * 4 * 64 * 16];
     lds_u8 *red = (lds_u8 *)red_;
-    const int e = blockIdx.x / g.nt, n0 = (blockIdx.x - e * g.nt) * 16;
-    int lo, hi;
-    op_group(g.offsets, e, g.rows, lo, hi);
+    // workgroup (r, n): the r-th group that holds rows, 16 columns
+    int r = blockIdx.x / g.nt;
+    const int n0 = (blockIdx.x - r * g.nt) * 16, lane = threadIdx.x & 63;
+    int e = -1, lo = 0, hi = 0;
+    for (int base = 0; base < g.E && e < 0; base += 64) {
+        int a = 0, b = 0;
+        if (base + lane < g.E) op_group(g.offsets, base + lane, g.rows, a, b);
+        unsigned long long held = __ballot(a < b);
+        const int n = __popcll(held);
+        if (r < n) {
+            for (int i = 0; i < r; ++i) held &= held - 1;
+            const int src = __ffsll((long long)held) - 1;
+            e = base + src;
+            lo = __shfl(a, src);
+            hi = __shfl(b, src);
+        }
+        r -= n;
+    }
+    e = __builtin_amdgcn_readfirstlane(e);
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    if (e < 0) return;
     while (lo < hi) {
         const int rows = min(hi - lo, 64);
         if (rows <= 16) stream_rows<OT, 1>(g, e, n0, lo, rows, blockIdx.y, red);
@@ -158,14 +191,115 @@ __global__ __launch_bounds__(256) void op_fold_kernel(OpGemmArgs g) {
     }
 }
 
-// One row's codes: the largest magnitude, then rne(127 x / max).  127 x is
-// formed first so that a code's border, an odd multiple of max / 254, divides
-// exactly; x and max are scaled by 2^-64 where 127 x could overflow.  A row
-// of zeros has scale 0 and codes 0; a row that holds an infinity or a NaN has
-// scale NaN (and codes 0), so that its products are NaN.
-template <int XB>
+// One row's codes: the largest magnitude, then rne(127 x / max).  A code's
+// border is an odd multiple of max / 254: 127 x is formed before the division,
+// so that a border divides exactly.  x and max are scaled by 2^-64 where 127 x
+// could overflow.  A row of zeros has scale 0 and codes 0; a row that holds an
+// infinity or a NaN has scale NaN (and codes 0), so that its products are NaN.
+struct RowMax {
+    float m = 0.0f;
+    bool bad = false;
+    __device__ __forceinline__ void take(float x) {
+        const float v = fabsf(x);
+        bad |= !(v <= 3.402823466e38f);
+        m = fmaxf(m, v);
+    }
+    // over the 256 threads of a workgroup; NaN has to survive the maximum
+    __device__ __forceinline__ float all(float *part) {
+        auto larger = [](float a, float b) { return (a != a || b != b) ? __builtin_nanf("") : fmaxf(a, b); };
+        float v = bad ? __builtin_nanf("") : m;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) v = larger(v, __shfl_xor(v, d));
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+        __syncthreads();
+        return larger(larger(part[0], part[1]), larger(part[2], part[3]));
+    }
+};
+struct RowCode {
+    float down, ms, inv;
+    bool live;
+    __device__ __forceinline__ explicit RowCode(float m)
+        : down(m > 1.0e36f ? 5.421010862427522e-20f : 1.0f), ms(m * down), inv(127.0f / ms),
+          live(m > 0.0f) {}  // (false for 0 and NaN)
+    // The product with 127 / max is off by less than 127 * 2^-22: the division
+    // itself runs only where that could cross a border, or max is so small that
+    // 127 / max overflows.
+    __device__ __forceinline__ int operator()(float x) const {
+        const float y = x * down;
+        float r = y * inv;
+        const float t = fabsf(r) - floorf(fabsf(r));
+        if (!(fabsf(t - 0.5f) > 1.0e-4f) || !(inv < 1.0e38f)) r = y * 127.0f / ms;
+        return live ? (int)rintf(r) : 0;
+    }
+};
+
+// Rows of up to 2048 NV columns, in registers: 256 threads with NV groups of 8
+// columns each (VEC: 16-byte loads of x, 8-byte stores of the codes).
+template <int XB, int NV, bool VEC>
 __global__ __launch_bounds__(256) void quantize_i8_kernel(const void *x_, long long ldx, int cols, int8_t *q_,
                                                           long long ldq, int pad_to, float *scale) {
+    __shared__ float part[4];
+    const long long r = blockIdx.x;
+    int8_t *q = q_ + r * ldq;
+    float v[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = VEC ? ((int)threadIdx.x + i * 256) * 8 : (int)threadIdx.x + i * 2048;
+        if constexpr (VEC && XB) {
+            uint4 u = make_uint4(0u, 0u, 0u, 0u);
+            if (c < cols) u = *(const uint4 *)((const uint16_t *)x_ + r * ldx + c);
+            const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v[i][2 * k] = __uint_as_float(w[k] << 16);
+                v[i][2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+            }
+        } else if constexpr (VEC) {
+            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = a;
+            if (c < cols) {
+                a = *(const float4 *)((const float *)x_ + r * ldx + c);
+                b = *(const float4 *)((const float *)x_ + r * ldx + c + 4);
+            }
+            v[i][0] = a.x, v[i][1] = a.y, v[i][2] = a.z, v[i][3] = a.w;
+            v[i][4] = b.x, v[i][5] = b.y, v[i][6] = b.z, v[i][7] = b.w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int ck = c + k * 256;
+                v[i][k] = 0.0f;
+                if (ck < cols)
+                    v[i][k] = XB ? bf16_to_f32(((const uint16_t *)x_)[r * ldx + ck]) : ((const float *)x_)[r * ldx + ck];
+            }
+        }
+    }
+    RowMax mx;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mx.take(v[i][k]);
+    const float m = mx.all(part);
+    if (threadIdx.x == 0) scale[r] = m / 127.0f;
+    const RowCode code(m);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = VEC ? ((int)threadIdx.x + i * 256) * 8 : (int)threadIdx.x + i * 2048;
+        if constexpr (VEC) {
+            if (c >= pad_to) continue;
+            unsigned w[2] = {0u, 0u};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k >> 2] |= (unsigned)(code(v[i][k]) & 255) << (8 * (k & 3));
+            *(uint2 *)(q + c) = make_uint2(w[0], w[1]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (c + k * 256 < pad_to) q[c + k * 256] = (int8_t)code(v[i][k]);
+        }
+    }
+}
+// Longer rows, read twice.
+template <int XB>
+__global__ __launch_bounds__(256) void quantize_i8_long_kernel(const void *x_, long long ldx, int cols, int8_t *q_,
+                                                               long long ldq, int pad_to, float *scale) {
     __shared__ float part[4];
     const long long r = blockIdx.x;
     int8_t *q = q_ + r * ldq;
@@ -173,30 +307,12 @@ __global__ __launch_bounds__(256) void quantize_i8_kernel(const void *x_, long l
         if constexpr (XB) return bf16_to_f32(((const uint16_t *)x_)[r * ldx + c]);
         else return ((const float *)x_)[r * ldx + c];
     };
-    float m = 0.0f;
-    bool bad = false;
-    for (int c = threadIdx.x; c < cols; c += 256) {
-        const float v = fabsf(at(c));
-        bad |= !(v <= 3.402823466e38f);
-        m = fmaxf(m, v);
-    }
-    if (bad) m = __builtin_nanf("");
-    // NaN has to survive the maximum
-    auto larger = [](float a, float b) { return (a != a || b != b) ? __builtin_nanf("") : fmaxf(a, b); };
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) m = larger(m, __shfl_xor(m, d));
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = larger(larger(part[0], part[1]), larger(part[2], part[3]));
+    RowMax mx;
+    for (int c = threadIdx.x; c < cols; c += 256) mx.take(at(c));
+    const float m = mx.all(part);
     if (threadIdx.x == 0) scale[r] = m / 127.0f;
-    const float down = m > 1.0e36f ? 5.421010862427522e-20f : 1.0f;  // 2^-64: exact
-    const float ms = m * down;
-    const bool live = m > 0.0f;  // false for 0 and NaN
-    for (int c = threadIdx.x; c < pad_to; c += 256) {
-        float v = 0.0f;
-        if (live && c < cols) v = rintf(at(c) * down * 127.0f / ms);
-        q[c] = (int8_t)(int)v;
-    }
+    const RowCode code(m);
+    for (int c = threadIdx.x; c < pad_to; c += 256) q[c] = (int8_t)(c < cols ? code(at(c)) : 0);
 }
 
 }  // namespace ops
