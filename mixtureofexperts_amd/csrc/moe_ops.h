@@ -50,13 +50,13 @@ __device__ __forceinline__ void op_group(const int *offsets, int e, int rows, in
 inline bool op_streamed(bool b_col, long long rows, long long E) { return !b_col && rows <= 16 * E; }
 
 constexpr int kOpMaxSplits = 16;
-// Ranges of k for `tiles` workgroups of a call, so that the GPU is filled:
-// none where half its CUs have one, no range shorter than `least` (folding the
+// Ranges of k for `tiles` workgroups of a call that could run in `slots`: none
+// where half of those have one, no range shorter than `least` (folding the
 // ranges is a launch of its own, about 4 us: a 64 x 64 tile runs 2 KB of k per
 // row in about 16 us, the streamed form 8 KB in about 10).
-inline int op_splits(long long tiles, long long k, long long least, int ncu) {
-    if (tiles < 1 || 2 * tiles > ncu) return 1;
-    long long s = (ncu + tiles - 1) / tiles;
+inline int op_splits(long long tiles, long long k, long long least, int slots) {
+    if (tiles < 1 || 2 * tiles > slots) return 1;
+    long long s = (slots + tiles - 1) / tiles;
     if (s > k / least) s = k / least;
     if (s > kOpMaxSplits) s = kOpMaxSplits;
     return s > 1 ? (int)s : 1;
@@ -66,7 +66,10 @@ inline int op_rows_splits(int ot, bool b_col, long long rows, long long E, long 
     const long long held = E < rows ? E : rows;  // groups that may hold rows
     if (op_streamed(b_col, rows, E)) return op_splits(held * ((N + 15) / 16), K * op_size(ot), 8192, ncu);
     const long long mt = (rows + 63) / 64;
-    return op_splits((mt > held ? mt : held) * ((N + 63) / 64), K * op_size(ot), 2048, ncu);
+    // a few rows per group read the weights as fast as loads are in flight: four
+    // 64 x 64 tiles per CU (4 rows of 3991 on 4 experts of 4970 columns, fp32: 114 us at one)
+    const int slots = rows <= 16 * E ? 4 * ncu : ncu;
+    return op_splits((mt > held ? mt : held) * ((N + 63) / 64), K * op_size(ot), 2048, slots);
 }
 // Ragged k: the rows of each group.
 inline int op_matrix_splits(long long rows, long long E, long long M, long long N, int ncu) {

@@ -512,12 +512,10 @@ __device__ __forceinline__ void put4(const OpGemmArgs &g, long long at, int n, f
     }
 }
 
-// Rows of C that take whole 16-byte chunks, as store_tile_rows writes them (a
-// bf16 sum that is added to stays in fp32 until its one rounding: put4).
+// Rows of C that start on 16 bytes.
 __device__ __forceinline__ bool rows16(const OpGemmArgs &g) {
     const int es = g.c_f32 ? 4 : 2;
-    return (((uintptr_t)g.C | (uintptr_t)(g.ldc * es) | (uintptr_t)(g.c_stride * es)) & 15) == 0 &&
-           (g.c_f32 || !g.accumulate);
+    return (((uintptr_t)g.C | (uintptr_t)(g.ldc * es) | (uintptr_t)(g.c_stride * es)) & 15) == 0;
 }
 __device__ __forceinline__ bool vec_ok(const OpGemmArgs &g) {
     const int es = g.c_f32 ? 4 : 2;
@@ -531,11 +529,11 @@ __device__ __forceinline__ bool vec_ok(const OpGemmArgs &g) {
 // j, c): the lane's result in row block i, column block j, column 4 (lane / 16) + c.
 template <int EO, int BM, int BN, int WM, int WN, int RING, typename Val>
 __device__ __forceinline__ void store_tile_rows(const OpGemmArgs &g, lds_u8 *ring, long long at0, int mrows, int n0,
-                                                int wm, int wn, int lane, Val val) {
+                                                int wm, int wn, int lane, bool chunks, Val val) {
     constexpr int NT = WM * WN * 64, NJ = BN / WN / 16;
     constexpr int CW = BN * EO, CH = CW / 16, CE = 16 / EO;
     constexpr int FIT = RING / CW, PR = FIT < BM ? FIT : BM;  // rows per pass
-    static_assert(PR % (WM * 16) == 0 && BM % PR == 0 && NT % CH == 0 && PR % (NT / CH) == 0, "passes");
+    static_assert(PR % (WM * 16) == 0 && BM % PR == 0 && NT % CH == 0 && PR % (NT / CH) == 0 && NT % BN == 0, "passes");
     constexpr int IP = PR / (WM * 16);  // row blocks of a wave per pass
     const int r16 = lane & 15, q4 = lane >> 4;
 #pragma unroll
@@ -562,7 +560,23 @@ __device__ __forceinline__ void store_tile_rows(const OpGemmArgs &g, lds_u8 *rin
         __syncthreads();
         const int ch = (int)threadIdx.x % CH, n = n0 + ch * CE;
         const int rows = min(PR, mrows - p * PR);
-        if (n < g.N) {
+        if (!chunks) {
+            // rows that do not start on 16 bytes: consecutive lanes, consecutive elements
+            const int col = (int)threadIdx.x % BN, b = col * EO;
+            if (n0 + col < g.N) {
+                for (int r = (int)threadIdx.x / BN; r < rows; r += NT / BN) {
+                    const lds_u8 *q = ring + r * CW + (((b / 16) ^ (r & (CH - 1))) << 4) + (b & 15);
+                    const long long at = at0 + (long long)(p * PR + r) * g.ldc + n0 + col;
+                    if constexpr (EO == 4) {
+                        const float x = *(const __attribute__((address_space(3))) float *)q;
+                        float *d = (float *)g.C + at;
+                        *d = g.accumulate ? *d + x : x;
+                    } else {
+                        ((uint16_t *)g.C)[at] = *(const __attribute__((address_space(3))) uint16_t *)q;
+                    }
+                }
+            }
+        } else if (n < g.N) {
             for (int r = (int)threadIdx.x / CH; r < rows; r += NT / CH) {
                 u32x4 v = *(const __attribute__((address_space(3))) u32x4 *)(ring + r * CW + ((ch ^ (r & (CH - 1))) << 4));
                 uint8_t *dst = (uint8_t *)g.C + (at0 + (long long)(p * PR + r) * g.ldc + n) * EO;
@@ -819,11 +833,13 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
         else return acc[i][j][c];
     };
     constexpr int RING = NS * (TA::BYTES + TB::BYTES);
-    if (DIRECT && rows16(g)) {
-        if (g.c_f32) store_tile_rows<4, BM, BN, WM, WN, RING>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
-        else store_tile_rows<2, BM, BN, WM, WN, RING>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
+    if (g.c_f32 || !g.accumulate) {
+        const bool chunks = rows16(g);
+        if (g.c_f32) store_tile_rows<4, BM, BN, WM, WN, RING>(g, ring, at0, mrows, jb.n0, wm, wn, lane, chunks, val);
+        else store_tile_rows<2, BM, BN, WM, WN, RING>(g, ring, at0, mrows, jb.n0, wm, wn, lane, chunks, val);
         return;
     }
+    // a bf16 sum that is added to stays in fp32 until its one rounding
     const bool vec = vec_ok(g);
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
