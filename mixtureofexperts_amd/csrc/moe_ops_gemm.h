@@ -532,7 +532,8 @@ __device__ __forceinline__ void store_tile_rows(const OpGemmArgs &g, lds_u8 *rin
                                                 int wm, int wn, int lane, bool chunks, Val val) {
     constexpr int NT = WM * WN * 64, NJ = BN / WN / 16;
     constexpr int CW = BN * EO, CH = CW / 16, CE = 16 / EO;
-    constexpr int FIT = RING / CW, PR = FIT < BM ? FIT : BM;  // rows per pass
+    constexpr int FIT = RING / CW;
+    constexpr int PR = FIT >= BM ? BM : (FIT >= BM / 2 ? BM / 2 : BM / 4);  // rows per pass
     static_assert(PR % (WM * 16) == 0 && BM % PR == 0 && NT % CH == 0 && PR % (NT / CH) == 0 && NT % BN == 0, "passes");
     constexpr int IP = PR / (WM * 16);  // row blocks of a wave per pass
     const int r16 = lane & 15, q4 = lane >> 4;
@@ -901,10 +902,13 @@ hipError_t launch_tiles(OpGemmArgs g, int vb, hipStream_t s) {
     return e == hipSuccess && g.splits > 1 ? launch_op_fold(OT, RAGK, g, s) : e;
 }
 
-// Tile and load form of a call.  Ragged rows: 256 x 256 tiles where groups
-// average enough rows to fill them and there are two rounds of them, else
-// 128 x 128, and 64 x 64 for short groups or few tiles.  Ragged k: by the
-// tiles of all groups.  Where even 64 x 64 tiles are few, k is split into
+// Tile and load form of a call.  256 x 256 tiles where there are two rounds of
+// them (ragged rows: and groups average enough rows to fill them), else 128 x
+// 128, and 64 x 64 for short groups or few tiles.  Measured on 8192 rows, 8 bf16
+// experts of 4096 / 14336, 256 x 256 against 128 x 256 with two workgroups per
+// CU: forward 874 / 1055 us, row gradient 852 / 926, int8 563 / 627; the weight
+// gradient of 64 Zipf groups of 2048 / 1408, 256 x 256 against 128 x 128 with three
+// workgroups per CU: 454 / 485 us.  Where even 64 x 64 tiles are few, k is split into
 // ranges (op_rows_splits, op_matrix_splits).
 template <int OT, bool ACOL, bool BCOL, bool RAGK>
 hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
@@ -928,13 +932,12 @@ hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
     const long long avg = RAGK ? g.M : (long long)g.rows / g.E;
     if (g.splits > 1) return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, KSUB, 4 / KSUB, 3>(g, vb, s);
     if constexpr (OT != OT_F32) {
-        // ragged k: a group that holds most rows has to fill the GPU by itself
-        const bool large = RAGK ? tiles(256) >= g.E * (long long)(ncu / 2) : avg >= 192 && g.N >= 192 && tiles(256) >= 2 * ncu;
+        const bool large = RAGK ? tiles(256) >= 2 * ncu : avg >= 192 && g.N >= 192 && tiles(256) >= 2 * ncu;
         if (vb == 16 && large)
             return launch_tiles<OT, ACOL, BCOL, RAGK, 256, 256, 4, 2, KSUB, 4 / KSUB, 2>(g, vb, s);
     }
     if (!(OT == OT_F32 && vb == 0) && avg >= 64 && g.N >= 64 && tiles(128) >= ncu)
-        return launch_tiles<OT, ACOL, BCOL, RAGK, 128, 128, 2, 2, KSUB, 4 / KSUB, 2>(g, vb, s);
+        return launch_tiles<OT, ACOL, BCOL, RAGK, 128, 128, 2, 2, KSUB, RAGK ? 3 : 4 / KSUB, RAGK ? 3 : 2>(g, vb, s);
     return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, KSUB, 4 / KSUB, 3>(g, vb, s);
 }
 
