@@ -936,7 +936,11 @@ hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
         if (vb == 16 && large)
             return launch_tiles<OT, ACOL, BCOL, RAGK, 256, 256, 4, 2, KSUB, 4 / KSUB, 2>(g, vb, s);
     }
-    if (!(OT == OT_F32 && vb == 0) && avg >= 64 && g.N >= 64 && tiles(128) >= ncu)
+    // fp32 is bound by its matrix rate alone, so the rows that a group's last tile
+    // lacks cost more than 64 x 64 tiles' loads: one group of 469 rows, 3008 -> 11648,
+    // 358 us at 128 against 283 at 64; 4096 rows, 4096 -> 4096, 985 against 1010
+    const long long least = OT == OT_F32 && !RAGK ? 512 : 64;
+    if (!(OT == OT_F32 && vb == 0) && avg >= least && g.N >= 64 && tiles(128) >= ncu)
         return launch_tiles<OT, ACOL, BCOL, RAGK, 128, 128, 2, 2, KSUB, RAGK ? 3 : 4 / KSUB, RAGK ? 3 : 2>(g, vb, s);
     return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, KSUB, 4 / KSUB, 3>(g, vb, s);
 }
