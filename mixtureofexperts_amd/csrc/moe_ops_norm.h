@@ -100,9 +100,10 @@ __device__ __forceinline__ void store8(void *p, int bf16, long long row, int c, 
     }
 }
 
-// Sum over the TPR threads of a row, the same bits in each of them.  Sums that
-// follow each other use different `part`s: the barrier of one sum then also
-// separates the reads of the sum before from the writes of the one after.
+// Sum over the TPR threads of a row, the same bits in each of them.  Every sum
+// of a workgroup uses another `part` than the one before it: the barrier of a
+// sum then also separates the reads of the sum before from the writes of the
+// one after.
 // A wave's part runs on DPP (four steps inside rows of 16 lanes, then the four
 // rows' sums by lane reads): no LDS round trips.
 template <int CTRL>
@@ -304,6 +305,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_grad_kernel(
         if (a.dh) kpre = load8<VEC>(a.pre, a.w_bf16, 0, tid * 8, D);
         if (a.post) kpost = load8<VEC>(a.post, a.w_bf16, 0, tid * 8, D);
     }
+    int turn = 0;  // the part of the next sum
     auto work = [&](RowData &d) {
         const float iy = d.iy, ir = d.ir;
         int wrow = 0;  // the weights' row; opaque where keeping them in registers over the rows would spill
@@ -333,7 +335,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_grad_kernel(
                     s += t[i].v[q] * rh[i].v[q];
                 }
             }
-            s = row_sum<TPR>(s, part[0]) / (float)D;
+            s = row_sum<TPR>(s, part[turn]) / (float)D;
+            turn ^= 1;
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -398,7 +401,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_grad_kernel(
             }
         }
         if (a.y && a.post) {
-            s = row_sum<TPR>(s, part[1]) / (float)D;
+            s = row_sum<TPR>(s, part[turn]) / (float)D;
+            turn ^= 1;
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll

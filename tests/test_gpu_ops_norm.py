@@ -160,6 +160,22 @@ def test_parts(moe):
         _check_grad(moe, a, r, stats, dr, _make(rng, (T, D), "bf16") if pre else None, "bf16", "f32")
 
 
+@pytest.mark.parametrize("D", [1000, 2056, 6000, 16384])
+@pytest.mark.parametrize("post", [False, True])
+def test_many_rows_of_one_sum(moe, D, post):
+    # only one of the two norms: the waves of a workgroup meet once per row, and
+    # each workgroup takes several rows in turn
+    T = 600
+    print(f"norm one sum per row D={D} post={post}", flush=True)
+    rng = np.random.default_rng([D, post])
+    a = _inputs(rng, T, D, "bf16", "f32", "f32", 0, not post, post, y=post)
+    r, h, stats = moe.block_norm(a["x"], a["y"], pre_weight=a["pre_weight"], post_weight=a["post_weight"], alpha=ALPHA,
+                                 beta=BETA, eps=EPS)
+    dr = _make(rng, (T, D), "bf16") if post else None
+    dh = None if post else _make(rng, (T, D), "bf16")
+    _check_grad(moe, a, r, stats, dr, dh, "bf16", "f32")
+
+
 def test_long_gate_groups(moe):
     # gate rows of many chunks each, a long sum over rows
     for T, D, gates in ((20000, 64, 2), (9000, 512, 3), (4099, 136, 1), (6000, 32, 3000)):
