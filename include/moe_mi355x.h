@@ -407,9 +407,10 @@ int moe_read_counts(moe_handle *h, int32_t *counts);
  * (expert) e, offsets being groups + 1 non-decreasing int32 in device memory,
  * as the layer's routing counts them (moe_forward_aux.offsets).  Offsets are
  * held within [0, rows] by the kernels; with offsets that decrease the results
- * are undefined.  A group may be empty; rows outside every group are neither
- * read nor written.  offsets may be NULL with groups = 1: all rows.  rows = 0
- * is no work.
+ * are undefined.  A group may be empty; rows outside every group are not
+ * written and their values have no effect.  offsets may be NULL with groups =
+ * 1: all rows.  rows = 0 is no work.  Sizes up to 2^30; a result must not
+ * overlap an operand.
  *
  * Matrices: group e's starts w_stride elements after group e - 1's;
  * MOE_LAYOUT_LLAMA_IN_OUT: memory [out_dim][in_dim], MOE_LAYOUT_FLUX_OUT_IN:

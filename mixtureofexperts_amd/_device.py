@@ -49,6 +49,9 @@ class DeviceLayer:
         h = ctypes.c_void_p()
         _lib.check(_lib.lib().moe_create(ctypes.byref(c), ctypes.byref(h)), None)
         self.h = h
+        # the device the library took (the current one): torch's, if torch has set it up
+        torch = sys.modules.get("torch")
+        self.device = torch.cuda.current_device() if torch is not None and torch.cuda.is_initialized() else 0
         self.router_outputs = _lib.lib().moe_router_outputs(h)
         self.slots = _lib.lib().moe_slots_per_token(h)
         # AuxiliaryFreeLoss bias length: the router outputs, or all experts
@@ -173,6 +176,8 @@ class DeviceLayer:
         torch's current stream: (out (T, D_out) float32, loss (1,) float32)."""
         import torch
 
+        if x.device.index != self.device:
+            raise _lib.MoeError(_lib.MOE_EINVAL, f"the layer is on device {self.device}, x on {x.device}")
         T = x.shape[0]
         out = torch.empty((T, self.output_dim), dtype=torch.float32, device=x.device)
         loss = torch.zeros(1, dtype=torch.float32, device=x.device)

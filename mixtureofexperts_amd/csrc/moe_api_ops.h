@@ -29,12 +29,18 @@ int op_done(const char *fn, hipError_t e) {
     return fail(nullptr, MOE_EHIP, std::string(fn) + ": " + hipGetErrorString(e));
 }
 
+// tile counts and byte offsets of a row are formed in 32 bits, with room for a
+// part tile past the last element
+constexpr int kOpMaxSize = 1 << 30;
+
 // What the grouped products share: groups, sizes, types, the rows' strides.
 int op_check_groups(const char *fn, const int32_t *offsets, int32_t groups, int32_t rows, int32_t in_dim,
                     int32_t out_dim) {
     if (groups < 1) return op_fail(fn, "groups must be positive");
     if (rows < 0) return op_fail(fn, "rows must not be negative");
     if (in_dim < 1 || out_dim < 1) return op_fail(fn, "dimensions must be positive");
+    if (groups > kOpMaxSize || rows > kOpMaxSize || in_dim > kOpMaxSize || out_dim > kOpMaxSize)
+        return op_fail(fn, "sizes above 2^30");
     if (!offsets && groups != 1) return op_fail(fn, "offsets are needed for more than one group");
     return MOE_OK;
 }
@@ -81,6 +87,7 @@ int op_rows_product(const char *fn, bool grad, const void *x, int64_t ldx, const
     g.ws = (float *)workspace;
     r = op_check_workspace(fn, g.splits > 1 ? (int64_t)4 * g.splits * rows * n : 0, workspace, workspace_bytes);
     if (r != MOE_OK) return r;
+    if (y == x || y == w) return op_fail(fn, "the result must not overlap an operand");
     return op_done(fn, dtype == MOE_F32 ? launch_op_gemm_f32(false, b_col, false, g, op_cus(), (hipStream_t)stream)
                                         : launch_op_gemm_bf16(false, b_col, false, g, op_cus(), (hipStream_t)stream));
 }
@@ -158,6 +165,7 @@ int moe_grouped_matmul_grad_w_async(const void *x, int64_t ldx, const void *dy, 
     if (r != MOE_OK) return r;
     r = op_check_workspace(fn, need, workspace, workspace_bytes);
     if (r != MOE_OK) return r;
+    if (dw == x || dw == dy) return op_fail(fn, "the result must not overlap an operand");
     OpGemmArgs g{};
     g.A = flux ? x : dy, g.B = flux ? dy : x, g.C = dw;
     g.lda = flux ? ldx : lddy, g.ldb = flux ? lddy : ldx, g.ldc = lddw;
@@ -175,6 +183,7 @@ int moe_quantize_int8_async(const void *x, int64_t ldx, int32_t x_dtype, int64_t
     const char *fn = "moe_quantize_int8_async";
     if (x_dtype != MOE_F32 && x_dtype != MOE_BF16) return op_fail(fn, "x_dtype must be MOE_F32 or MOE_BF16");
     if (rows < 0 || cols < 1) return op_fail(fn, "rows must not be negative and cols positive");
+    if (cols > kOpMaxSize) return op_fail(fn, "sizes above 2^30");
     if (ldx < cols || ldq < cols) return op_fail(fn, "a row stride is smaller than its row");
     if (rows == 0) return MOE_OK;
     if (!x || !q || !scale) return op_fail(fn, "null buffer");
@@ -228,6 +237,7 @@ int moe_int8_matmul_async(const void *x, int64_t ldx, int32_t x_dtype, const flo
     r = moe_int8_matmul_workspace(groups, rows, in_dim, out_dim, x_dtype, &need);
     if (r == MOE_OK) r = op_check_workspace(fn, need, workspace, workspace_bytes);
     if (r != MOE_OK) return r;
+    if (y == x || y == w) return op_fail(fn, "the result must not overlap an operand");
     if (!codes) {
         float *sx = (float *)((uint8_t *)workspace + int8_partial_bytes(groups, rows, in_dim, out_dim));
         int8_t *q = (int8_t *)sx + round_up((int64_t)rows * 4, 16);

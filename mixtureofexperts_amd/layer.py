@@ -313,7 +313,7 @@ def moe_block_forward(moe, x, *, pre_weight, post_weight=None, gate=None, next_w
     loss as a (1,) tensor).  Nothing waits for the GPU, and the layer's
     training_stats are not updated.  Layers whose gate or balance loss keeps
     state on the host (HashGating, RandomGating, AuxiliaryFreeLoss) have no such
-    path."""
+    path, and the call cannot be captured into a graph (block_norm can)."""
     c = moe.config
     if isinstance(moe.router.gate_type, HOST_ROUTED_GATES) or isinstance(moe.balance_loss, AuxiliaryFreeLoss):
         raise _lib.MoeError(_lib.MOE_EUNSUPPORTED, "moe_block_forward: the gate or loss keeps state on the host")
@@ -325,6 +325,9 @@ def moe_block_forward(moe, x, *, pre_weight, post_weight=None, gate=None, next_w
         raise _lib.MoeError(_lib.MOE_EINVAL, "pre_weight is needed")
     import torch
 
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        # the handle orders its calls across streams by events of its own
+        raise _lib.MoeError(_lib.MOE_EUNSUPPORTED, "moe_block_forward: a layer's calls cannot be captured into a graph")
     # bf16 activations are the bf16 and fp8 layers' own input
     half = x.dtype == torch.bfloat16 and not decode and c.weight_dtype not in ("f32", "fp32")
     _, h, _ = block_norm(x, pre_weight=pre_weight, eps=eps, h_dtype=torch.bfloat16 if half else torch.float32)

@@ -10,7 +10,7 @@ argument raises MoeError.
 
 Groups: ``offsets`` is an int32 tensor of E + 1 non-decreasing row numbers on
 the device; rows [offsets[e], offsets[e + 1]) belong to expert e, and rows
-outside every group are neither read nor written.  ``None``: one expert, all
+outside every group are not written and have no effect.  ``None``: one expert, all
 rows.  Weights are (E, out, in) with ``layout=MOE_LAYOUT_LLAMA_IN_OUT`` (the
 default) and (E, in, out) with ``MOE_LAYOUT_FLUX_OUT_IN``; one expert's may be
 2-D.  Rows may be strided (contiguous within a row); 16-byte aligned rows are
@@ -76,6 +76,8 @@ def _rows(t, name, dtypes):
 def _matrices(t, name, dtypes):
     """(E, a, b) or (a, b): (E, a, b, row stride, matrix stride)."""
     _tensor(t, name, dtypes, (2, 3))
+    if max(t.shape) > 2**31 - 1:
+        _bad(f"{name}: sizes must fit 32 bits")
     a, b = t.shape[-2:]
     ld = _row_stride(t, name)
     if t.dim() == 2:
@@ -241,9 +243,9 @@ def quantize_int8(x):
     this gives the codes and scales that int8_matmul takes."""
     torch = _t()
     _tensor(x, "x", _floats, range(1, 9))
+    if not 1 <= x.shape[-1] < 2**31:
+        _bad("x must have 1 to 2^31 - 1 columns")
     x2 = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
-    if x2.shape[1] < 1:
-        _bad("x has no columns")
     q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     _call(_lib.lib().moe_quantize_int8_async, x.device, x2.data_ptr(), _row_stride(x2, "x"), _codes[x.dtype],

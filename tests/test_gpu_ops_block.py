@@ -196,3 +196,56 @@ def test_block_forward_refuses_host_gates(moe):
                         activation=moe.silu, gate_type=moe.RandomGating(2), max_tokens=8)
     with pytest.raises(moe.MoeError, match="host"):
         moe.moe_block_forward(moe.MoELayer(cfg), torch.zeros(2, 32, device="cuda"), pre_weight=torch.ones(32, device="cuda"))
+
+
+@pytest.mark.parametrize("decode", [False, True])
+def test_block_forward_on_streams(moe, decode):
+    # the same bits on torch's null stream and on another one, in turn on one layer;
+    # a capture is refused (the layer's calls order themselves by events)
+    rng = np.random.default_rng(16)
+    cfg = moe.MoEConfig(num_experts=8, expert_type="gated", input_dim=128, hidden_dim=256, output_dim=128,
+                        activation=moe.silu, gate_type=moe.TopKGating(2), weight_dtype="bf16", max_tokens=64)
+    layer = moe.MoELayer(cfg, rng=rng)
+    T = 3 if decode else 50
+    xs = [torch.from_numpy(rng.standard_normal((T, 128)).astype(np.float32)).cuda() for _ in range(3)]
+    pre, post = (torch.ones(128, device="cuda") for _ in range(2))
+    step = lambda x: moe.moe_block_forward(layer, x, pre_weight=pre, post_weight=post, next_weight=pre, decode=decode)[:2]
+    want = []
+    for x in xs:
+        want.append(step(x))
+        torch.cuda.synchronize()
+    side, got = torch.cuda.Stream(), []
+    for turn in range(4):
+        for i, x in enumerate(xs):
+            if (turn + i) % 2:
+                with torch.cuda.stream(side):
+                    got.append((i, step(x)))
+            else:
+                got.append((i, step(x)))
+    torch.cuda.synchronize()
+    for i, res in got:
+        assert all(torch.equal(a, b) for a, b in zip(res, want[i])), i
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(moe.MoeError, match="captured"):
+            step(xs[0])
+        y = xs[0] + 1
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, xs[0] + 1)
+    layer.close()
+
+
+def test_block_forward_refuses_too_many_tokens(moe):
+    cfg = moe.MoEConfig(num_experts=4, expert_type="gated", input_dim=32, hidden_dim=64, output_dim=32,
+                        activation=moe.silu, gate_type=moe.TopKGating(2), max_tokens=8)
+    layer = moe.MoELayer(cfg)
+    pre = torch.ones(32, device="cuda")
+    for decode in (False, True):
+        with pytest.raises(moe.MoeError):
+            moe.moe_block_forward(layer, torch.zeros(4096, 32, device="cuda"), pre_weight=pre, decode=decode)
+    r, _, _ = moe.moe_block_forward(layer, torch.ones(8, 32, device="cuda"), pre_weight=pre)
+    assert torch.isfinite(r).all()
+    with pytest.raises(moe.MoeError, match="GPU memory"):
+        moe.moe_block_forward(layer, torch.ones(8, 32), pre_weight=pre)
+    layer.close()

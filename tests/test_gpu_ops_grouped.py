@@ -261,3 +261,134 @@ def test_streams_and_graph_replay(moe):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want[i])), i
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_wide_strides(moe, dtype):
+    # rows 4 MB and more apart: a tile's byte offsets no longer fit the loads'
+    # 32 bits, and elements lie past 2^31 from the tensor's start
+    print(f"grouped wide strides {dtype}", flush=True)
+    rng = np.random.default_rng(12)
+    lens, K, N, ld = [150, 0, 100, 170], 136, 72, 2**23 + 8
+    M = sum(lens)
+    big = torch.empty(M * ld, dtype=DT[dtype], device="cuda")
+    assert M * ld > 2**31
+    wide = lambda cols: big.as_strided((M, cols), (ld, 1))
+    off = _offsets(lens)
+    x = _rows(rng, M, K, dtype, 0)
+    dy = _rows(rng, M, N, dtype, 0)
+    w = {LLAMA: _mats(rng, 4, N, K, dtype, 0)}
+    w[FLUX] = w[LLAMA].transpose(1, 2).contiguous()
+    for layout in (LLAMA, FLUX):
+        y, dx = moe.grouped_matmul(x, w[layout], off, layout=layout), moe.grouped_matmul_grad_x(dy, w[layout], off, layout=layout)
+        dw = moe.grouped_matmul_grad_w(x, dy, off, layout=layout, out_dtype=torch.float32)
+        X, D = _f64(x), _f64(dy)
+        W = _f64(w[LLAMA])
+        # operands, then results, in the wide tensor
+        xw = wide(K)
+        xw.copy_(x)
+        got = [moe.grouped_matmul(xw, w[layout], off, layout=layout),
+               moe.grouped_matmul_grad_w(xw, dy, off, layout=layout, out_dtype=torch.float32)]
+        yw = wide(N)
+        moe.grouped_matmul(x, w[layout], off, layout=layout, out=yw)
+        got.append(yw.clone())
+        yw.copy_(dy)
+        got.append(moe.grouped_matmul_grad_x(yw, w[layout], off, layout=layout))
+        at = 0
+        for e, n in enumerate(lens):
+            s = slice(at, at + n)
+            for r in (y, got[0], got[2]):
+                _close(_f64(r[s]), X[s] @ W[e].T, np.abs(X[s]) @ np.abs(W[e].T), K, dtype)
+            for r in (dx, got[3]):
+                _close(_f64(r[s]), D[s] @ W[e], np.abs(D[s]) @ np.abs(W[e]), N, dtype)
+            g = (D[s].T @ X[s], np.abs(D[s]).T @ np.abs(X[s]))
+            if layout == FLUX:
+                g = tuple(m.T for m in g)
+            for r in (dw, got[1]):
+                _close(_f64(r[e]), *g, max(n, 1), "f32")
+            at += n
+
+
+def test_wide_strides_many_tiles(moe):
+    # as many tiles as the larger tile sizes take
+    print("grouped wide strides, many tiles", flush=True)
+    rng = np.random.default_rng(17)
+    E, K, N, ld = 64, 200, 200, 2**20 + 8
+    M = 3 * E
+    off = _offsets([3] * E)
+    buf = torch.empty(M * ld, dtype=torch.float32, device="cuda")
+    xw = buf.as_strided((M, K), (ld, 1))
+    x, dy = _rows(rng, M, K, "f32", 0), _rows(rng, M, N, "f32", 0)
+    xw.copy_(x)
+    dw, X, D = _f64(moe.grouped_matmul_grad_w(xw, dy, off)), _f64(x), _f64(dy)
+    for e in range(E):
+        s = slice(3 * e, 3 * e + 3)
+        _close(dw[e], D[s].T @ X[s], np.abs(D[s]).T @ np.abs(X[s]), 3, "f32")
+
+
+def test_weight_matrices_past_2_31_elements(moe):
+    print("grouped matrices past 2^31 elements", flush=True)
+    rng = np.random.default_rng(13)
+    E, N, K = 3, 40, 64
+    stride = 2**30 + 64  # elements between the matrices: the last one starts past 2^31
+    buf = torch.empty(2 * stride + N * K, dtype=torch.bfloat16, device="cuda")
+    w = buf.as_strided((E, N, K), (stride, K, 1))
+    w.copy_(_mats(rng, E, N, K, "bf16", 0))
+    lens = [20, 70, 33]
+    x, dy, off = _rows(rng, 123, K, "bf16", 0), _rows(rng, 123, N, "bf16", 0), _offsets(lens)
+    W, dense = _f64(w), w.contiguous()
+    assert torch.equal(moe.grouped_matmul(x, w, off), moe.grouped_matmul(x, dense, off))
+    assert torch.equal(moe.grouped_matmul_grad_x(dy, w, off), moe.grouped_matmul_grad_x(dy, dense, off))
+    dw = moe.grouped_matmul_grad_w(x, dy, off)
+    X, D, at = _f64(x), _f64(dy), 0
+    for e, n in enumerate(lens):
+        _close(_f64(dw[e]), D[at:at + n].T @ X[at:at + n], np.abs(D[at:at + n]).T @ np.abs(X[at:at + n]), n, "bf16")
+        at += n
+    moe.grouped_matmul_grad_w(x, dy, off, out=w)
+    assert torch.equal(w, dw)
+
+
+@pytest.mark.parametrize("E", [500, 513, 1300])
+def test_many_groups(moe, E):
+    # the weight gradient's work list, longest group first, up to 512 groups and
+    # past them; the row products' one, 64 groups at a time
+    print(f"grouped many groups E={E}", flush=True)
+    rng = np.random.default_rng(E)
+    lens = [int(n) for n in rng.integers(0, 9, E)]
+    lens[7], lens[E - 1] = 150, 0
+    K, N, M = 40, 24, sum(lens)
+    x, dy, w, off = _rows(rng, M, K, "bf16", 0), _rows(rng, M, N, "bf16", 0), _mats(rng, E, N, K, "bf16", 0), _offsets(lens)
+    y, dx, dw = moe.grouped_matmul(x, w, off), moe.grouped_matmul_grad_x(dy, w, off), moe.grouped_matmul_grad_w(x, dy, off)
+    X, D, W, Y, DX, DW, at = _f64(x), _f64(dy), _f64(w), _f64(y), _f64(dx), _f64(dw), 0
+    for e, n in enumerate(lens):
+        s = slice(at, at + n)
+        _close(Y[s], X[s] @ W[e].T, np.abs(X[s]) @ np.abs(W[e].T), K, "bf16")
+        _close(DX[s], D[s] @ W[e], np.abs(D[s]) @ np.abs(W[e]), N, "bf16")
+        _close(DW[e], D[s].T @ X[s], np.abs(D[s]).T @ np.abs(X[s]), max(n, 1), "bf16")
+        at += n
+
+
+def test_two_streams_at_once(moe):
+    # calls that run side by side on two streams, split ones (each with its own
+    # workspace) among them: the bits of the calls alone
+    rng = np.random.default_rng(14)
+    jobs = []
+    for lens, K, N in (([71], 5440, 64), ([3, 0, 2], 16401, 125), ([3000], 96, 40), ([33, 130, 5, 0, 300], 200, 136)):
+        x, dy = _rows(rng, sum(lens), K, "bf16", 0), _rows(rng, sum(lens), N, "bf16", 0)
+        w, off = _mats(rng, len(lens), N, K, "bf16", 0), _offsets(lens)
+        jobs.append((x, dy, w, off))
+
+    def run(i):
+        x, dy, w, off = jobs[i]
+        return (moe.grouped_matmul(x, w, off), moe.grouped_matmul_grad_x(dy, w, off), moe.grouped_matmul_grad_w(x, dy, off))
+
+    want = [run(i) for i in range(len(jobs))]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for turn in range(6):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append(((turn + k) % len(jobs), run((turn + k) % len(jobs))))
+    torch.cuda.synchronize()
+    for i, res in got:
+        assert all(torch.equal(a, b) for a, b in zip(res, want[i])), i

@@ -149,3 +149,27 @@ def test_nan_rows_and_graph(moe):
     x[4, 9], x[50, 1] = float("nan"), float("-inf")
     fin = torch.isfinite(moe.int8_matmul(x, w, ws, off)).all(dim=1)
     assert not fin[4] and not fin[50] and fin.sum() == 68
+
+
+def test_split_sums_with_empty_groups(moe):
+    # long sums of few rows: k split over workgroups, the fold finds each row's
+    # group among empty ones (first, middle, last) and groups outside the rows
+    rng = np.random.default_rng(15)
+    for lens, start, K, N in (([0, 0, 2, 0, 1, 0, 0], 0, 20000, 17), ([0, 40, 0, 0, 31, 0], 3, 9000, 64)):
+        print(f"int8 split lens={lens} K={K} N={N}", flush=True)
+        E, M = len(lens), sum(lens)
+        q = torch.from_numpy(rng.integers(-127, 128, (M + start + 2, K)).astype(np.int8)).cuda()
+        w = torch.from_numpy(rng.integers(-127, 128, (E, N, K)).astype(np.int8)).cuda()
+        xs, ws = (torch.from_numpy(rng.uniform(0.5, 2, s).astype(np.float32)).cuda() for s in ((M + start + 2,), (E, N)))
+        off = torch.tensor(np.concatenate([[start], start + np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+        y = moe.int8_matmul(q, w, ws, off, x_scale=xs, out_dtype=torch.float32).cpu().double().numpy()
+        Q, W = q.cpu().numpy().astype(np.int64), w.cpu().numpy().astype(np.int64)
+        XS, WS = xs.cpu().double().numpy(), ws.cpu().double().numpy()
+        at = start
+        for e, n in enumerate(lens):
+            s = slice(at, at + n)
+            ref = (Q[s] @ W[e].T) * XS[s, None] * WS[e]
+            # the exact sum to fp32 and two products: three roundings
+            assert (np.abs(y[s] - ref) <= 3.01 * 2.0**-24 * np.abs(ref)).all(), e
+            at += n
+        assert (y[:start] == 0).all() and (y[at:] == 0).all()

@@ -143,6 +143,33 @@ def test_block_norm_grad_refuses(moe, bad, msg):
     _refused(moe, "moe_block_norm_grad_async", {**NORMG, **bad}, msg)
 
 
+def test_sizes_past_the_32_bit_arithmetic_are_refused(moe):
+    from mixtureofexperts_amd import _lib
+
+    big, n = 2**30 + 1, ctypes.c_int64(-1)
+    for bad in (dict(rows=big), dict(in_dim=big, ldx=big, ldw=big), dict(out_dim=big, ldy=big, w_stride=64 * big),
+                dict(groups=big)):
+        _refused(moe, "moe_grouped_matmul_async", {**ROWS, **bad}, "2^30")
+    _refused(moe, "moe_grouped_matmul_grad_w_async", {**GRADW, "rows": big}, "2^30")
+    _refused(moe, "moe_int8_matmul_async", {**INT8MM, "rows": big}, "2^30")
+    _refused(moe, "moe_quantize_int8_async", {**QUANT, "cols": big, "ldx": big, "ldq": big}, "2^30")
+    assert _lib.lib().moe_grouped_matmul_workspace(1, big, 8, 8, BF16, ctypes.byref(n)) == _lib.MOE_EINVAL
+
+
+def test_a_result_on_its_operand_is_refused(moe):
+    # square products, so that the sizes alone would allow it
+    q = 2 * P
+    rows = dict(in_dim=64, out_dim=64, ldy=64, w_stride=64 * 64, dtype=F32, y_dtype=F32)
+    for place in (dict(x=P, w=q, y=P), dict(x=P, w=q, y=q)):
+        for fn in ("moe_grouped_matmul_async", "moe_grouped_matmul_grad_x_async"):
+            _refused(moe, fn, {**ROWS, **rows, **place, "workspace": 4 * P, "workspace_bytes": 2**30}, "overlap")
+        args = {**INT8MM, "x": place["x"], "w": place["w"], "y": place["y"], "workspace": 4 * P, "workspace_bytes": 2**30}
+        _refused(moe, "moe_int8_matmul_async", args, "overlap")
+    for place in (dict(x=P, dy=q, dw=P), dict(x=P, dy=q, dw=q)):
+        _refused(moe, "moe_grouped_matmul_grad_w_async", {**GRADW, **place, "workspace": 4 * P, "workspace_bytes": 2**30},
+                 "overlap")
+
+
 def test_empty_calls_are_no_work(moe):
     from mixtureofexperts_amd import _lib
 
@@ -210,3 +237,14 @@ def test_python_refuses(moe):
         with pytest.raises(moe.MoeError, match=msg):
             call()
             print("not refused:", i, flush=True)
+
+
+@pytest.mark.gpu
+def test_python_refuses_no_columns_and_results_in_place(moe):
+    torch = pytest.importorskip("torch")
+    with pytest.raises(moe.MoeError, match="columns"):
+        moe.quantize_int8(torch.zeros(3, 2, 0, device="cuda"))
+    x, w = torch.zeros(8, 8, device="cuda"), torch.zeros(8, 8, device="cuda")
+    for out in (x, w):
+        with pytest.raises(moe.MoeError, match="overlap"):
+            moe.grouped_matmul(x, w, out=out)
