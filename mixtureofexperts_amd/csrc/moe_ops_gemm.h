@@ -110,24 +110,27 @@ __device__ __forceinline__ int col_swz(int kr) {
 constexpr unsigned kOutOfRange = 0x80000000u;  // past every buffer's num_records: reads as 0
 
 // One operand's tile of ROWS rows: its LDS stage image and how NT threads fill
-// it.  VB 16 or 4: by buffer loads of VB bytes a lane straight into LDS (16:
-// 16-byte aligned rows of whole chunks; 4: fp32 of any stride and length); a
-// lane whose bytes lie outside reads zeros by the buffer's own range check.
-// VB 0: through registers, any alignment.
+// it.  VB 16 or 4: by buffer loads of 16 bytes a lane straight into LDS, a lane
+// whose bytes lie outside reads zeros by the buffer's own range check.  16: rows
+// of whole, aligned chunks.  4: fp32 rows of any stride (from 4) and length, whose
+// last chunk may hold elements of the next row: of a "col" operand they only
+// reach results that are not stored, and the next row is there except in the
+// last stage; of a "row" operand they would be summed.  Such a last stage is
+// loaded by dwords (weight gradient, 12 groups of 259 rows of 1001 / 2731: 169 us,
+// by dwords alone 210).  VB 0: through registers, any alignment.
 template <int ES, int ROWS, bool COL, int NT, int KSUB, int VB>
 struct Tile {
     static constexpr bool DIRECT = VB > 0;
     static_assert(VB == 0 || VB == 16 || (VB == 4 && ES == 4), "bytes per lane");
     static constexpr int CE = 16 / ES;           // elements per chunk
     static constexpr int KE = KSUB * 64 / ES;     // k per stage
-    static constexpr int PER = VB == 4 ? 4 : 1;  // loads per chunk
-    static constexpr int NC = PER * KSUB * ROWS * 4 / NT;  // loads per thread
+    static constexpr int NC = KSUB * ROWS * 4 / NT;  // chunks per thread
     static constexpr int ROWB = COL ? ROWS * ES : 64 * KSUB;
     static constexpr int CPR = ROWB / 16;        // chunks per LDS row
     static constexpr int NU = ROWS / 16;         // 16-element units per k row (COL)
     static constexpr int UC = ES;                // chunks per unit
     static constexpr int BYTES = ROWS * 64 * KSUB;
-    static_assert(NC >= 1 && PER * KSUB * ROWS * 4 % NT == 0, "threads cover the tile");
+    static_assert(NC >= 1 && KSUB * ROWS * 4 % NT == 0, "threads cover the tile");
 
     const uint8_t *base;  // element (row 0, first k) of the tile
     long long ldb;        // bytes between rows (COL: between k)
@@ -152,10 +155,40 @@ struct Tile {
 
     // load j of this thread: its LDS row and its first element within the row
     static __device__ __forceinline__ void place_load(int j, int &row, int &elem) {
-        const int i = chunk_of(j);
         int chunk;
-        place(i / PER, row, chunk);
-        elem = chunk * CE + i % PER;
+        place(chunk_of(j), row, chunk);
+        elem = chunk * CE;
+    }
+    // a stage whose last chunks may not be read whole (krem: what is left of k)
+    __device__ __forceinline__ bool part_chunks(int krem) const {
+        if constexpr (COL) return krem > 0 && krem <= KE && lim < ROWS && lim % CE != 0;
+        else return krem > 0 && krem < KE && krem % CE != 0;
+    }
+    // such a stage, by dwords
+    __device__ __forceinline__ void load_dwords(const u32x4 &rs, int krem, unsigned lds, int w) const {
+        static_assert(ES == 4, "a dword per element");
+        constexpr int STEP = NT * 4;
+        const unsigned m0 = __builtin_amdgcn_readfirstlane(lds + w * 256);
+#pragma unroll
+        for (int j = 0; j < 4 * NC; j += 4) {
+            unsigned v[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int i = (j + q) * NT + (int)threadIdx.x;
+                int row, chunk;
+                place(i / 4, row, chunk);
+                const int elem = chunk * CE + i % 4;
+                const bool ok = COL ? elem < lim && row < krem : row < lim && elem < krem;
+                v[q] = ok ? (unsigned)(row * (int)ldb + elem * ES) : kOutOfRange;
+            }
+            asm volatile(
+                "s_nop 4\n\ts_mov_b32 m0, %5\n\ts_nop 0\n\tbuffer_load_dword %0, %4, 0 offen lds\n\t"
+                "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dword %1, %4, 0 offen lds\n\t"
+                "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dword %2, %4, 0 offen lds\n\t"
+                "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dword %3, %4, 0 offen lds" ::"v"(v[0]),
+                "v"(v[1]), "v"(v[2]), "v"(v[3]), "s"(rs), "s"(m0 + j * STEP), "n"(STEP)
+                : "m0", "scc");
+        }
     }
 
     __device__ __forceinline__ void init(const uint8_t *b, long long ld_bytes, int limit, int k) {
@@ -193,6 +226,12 @@ struct Tile {
         rs[2] = 0x7fffffffu;
         rs[3] = 0x00027000u;
         const int krem = klen - k0;
+        if constexpr (VB == 4) {
+            if (part_chunks(krem)) {
+                load_dwords(rs, krem, lds, w);
+                return;
+            }
+        }
         unsigned v[NC];
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
@@ -203,22 +242,9 @@ struct Tile {
                 if (COL ? row >= krem : elem >= krem) v[j] = kOutOfRange;
             }
         }
-        constexpr int VL = VB == 4 ? 4 : 16;
-        const unsigned m0 = __builtin_amdgcn_readfirstlane(lds + w * (64 * VL));
-        constexpr int STEP = NT * VL;  // LDS bytes between a thread's loads
-        if constexpr (VB == 4) {
-            static_assert(NC % 4 == 0, "loads per thread");
-#pragma unroll
-            for (int j = 0; j < NC; j += 4)
-                asm volatile(
-                    "s_nop 4\n\ts_mov_b32 m0, %5\n\ts_nop 0\n\tbuffer_load_dword %0, %4, 0 offen lds\n\t"
-                    "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dword %1, %4, 0 offen lds\n\t"
-                    "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dword %2, %4, 0 offen lds\n\t"
-                    "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dword %3, %4, 0 offen lds" ::"v"(v[j]),
-                    "v"(v[j + 1 < NC ? j + 1 : 0]), "v"(v[j + 2 < NC ? j + 2 : 0]), "v"(v[j + 3 < NC ? j + 3 : 0]),
-                    "s"(rs), "s"(m0 + j * STEP), "n"(STEP)
-                    : "m0", "scc");
-        } else if constexpr (NC == 1) {
+        const unsigned m0 = __builtin_amdgcn_readfirstlane(lds + w * 1024);
+        constexpr int STEP = NT * 16;  // LDS bytes between a thread's loads
+        if constexpr (NC == 1) {
             asm volatile("s_nop 4\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(v[0]),
                          "s"(rs), "s"(m0)
                          : "m0");
@@ -512,11 +538,6 @@ __device__ __forceinline__ void put4(const OpGemmArgs &g, long long at, int n, f
     }
 }
 
-// Rows of C that start on 16 bytes.
-__device__ __forceinline__ bool rows16(const OpGemmArgs &g) {
-    const int es = g.c_f32 ? 4 : 2;
-    return (((uintptr_t)g.C | (uintptr_t)(g.ldc * es) | (uintptr_t)(g.c_stride * es)) & 15) == 0;
-}
 __device__ __forceinline__ bool vec_ok(const OpGemmArgs &g) {
     const int es = g.c_f32 ? 4 : 2;
     return (((uintptr_t)g.C | (uintptr_t)(g.ldc * es) | (uintptr_t)(g.c_stride * es)) & (4 * es - 1)) == 0;
@@ -525,16 +546,18 @@ __device__ __forceinline__ bool vec_ok(const OpGemmArgs &g) {
 // A tile's results through LDS, so that whole rows are stored: a wave's own
 // stores are 16 rows x 32 (fp32: 64) bytes each.  Row r's 16-byte chunk c is
 // kept at chunk c ^ (r mod CH): the column-wise writes and the row-wise reads
-// both spread over the banks.  EO: bytes of a result; PR rows at a time.  val(i,
+// both spread over the banks.  The chunks are stored whole at whatever alignment
+// their rows have (12 groups of 259 rows of 1001 / 2731, weight gradient: 169 us, by
+// elements 175; bf16 69, by elements 75).  EO: bytes of a result; PR rows at a time.  val(i,
 // j, c): the lane's result in row block i, column block j, column 4 (lane / 16) + c.
 template <int EO, int BM, int BN, int WM, int WN, int RING, typename Val>
 __device__ __forceinline__ void store_tile_rows(const OpGemmArgs &g, lds_u8 *ring, long long at0, int mrows, int n0,
-                                                int wm, int wn, int lane, bool chunks, Val val) {
+                                                int wm, int wn, int lane, Val val) {
     constexpr int NT = WM * WN * 64, NJ = BN / WN / 16;
     constexpr int CW = BN * EO, CH = CW / 16, CE = 16 / EO;
     constexpr int FIT = RING / CW;
     constexpr int PR = FIT >= BM ? BM : (FIT >= BM / 2 ? BM / 2 : BM / 4);  // rows per pass
-    static_assert(PR % (WM * 16) == 0 && BM % PR == 0 && NT % CH == 0 && PR % (NT / CH) == 0 && NT % BN == 0, "passes");
+    static_assert(PR % (WM * 16) == 0 && BM % PR == 0 && NT % CH == 0 && PR % (NT / CH) == 0, "passes");
     constexpr int IP = PR / (WM * 16);  // row blocks of a wave per pass
     const int r16 = lane & 15, q4 = lane >> 4;
 #pragma unroll
@@ -561,36 +584,21 @@ __device__ __forceinline__ void store_tile_rows(const OpGemmArgs &g, lds_u8 *rin
         __syncthreads();
         const int ch = (int)threadIdx.x % CH, n = n0 + ch * CE;
         const int rows = min(PR, mrows - p * PR);
-        if (!chunks) {
-            // rows that do not start on 16 bytes: consecutive lanes, consecutive elements
-            const int col = (int)threadIdx.x % BN, b = col * EO;
-            if (n0 + col < g.N) {
-                for (int r = (int)threadIdx.x / BN; r < rows; r += NT / BN) {
-                    const lds_u8 *q = ring + r * CW + (((b / 16) ^ (r & (CH - 1))) << 4) + (b & 15);
-                    const long long at = at0 + (long long)(p * PR + r) * g.ldc + n0 + col;
-                    if constexpr (EO == 4) {
-                        const float x = *(const __attribute__((address_space(3))) float *)q;
-                        float *d = (float *)g.C + at;
-                        *d = g.accumulate ? *d + x : x;
-                    } else {
-                        ((uint16_t *)g.C)[at] = *(const __attribute__((address_space(3))) uint16_t *)q;
-                    }
-                }
-            }
-        } else if (n < g.N) {
+        if (n < g.N) {
             for (int r = (int)threadIdx.x / CH; r < rows; r += NT / CH) {
                 u32x4 v = *(const __attribute__((address_space(3))) u32x4 *)(ring + r * CW + ((ch ^ (r & (CH - 1))) << 4));
                 uint8_t *dst = (uint8_t *)g.C + (at0 + (long long)(p * PR + r) * g.ldc + n) * EO;
                 if (n + CE <= g.N) {
                     if (g.accumulate) {
-                        const u32x4 o = *(const u32x4 *)dst;
+                        u32x4 o;
+                        __builtin_memcpy(&o, dst, 16);
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
                             if constexpr (EO == 4)
                                 v[q] = __float_as_uint(__uint_as_float(o[q]) + __uint_as_float(v[q]));
                         }
                     }
-                    *(u32x4 *)dst = v;
+                    __builtin_memcpy(dst, &v, 16);
                 } else {
 #pragma unroll
                     for (int q = 0; q < CE; ++q) {
@@ -621,7 +629,8 @@ __device__ __forceinline__ void store_tile_rows(const OpGemmArgs &g, lds_u8 *rin
 //   half 1: MFMAs of the second columns | reads of stage s + 1's rows and first
 //           columns | loads of stage s + NS into slot s
 // Loads past the last stage read zeros without touching memory, which keeps
-// the count of loads in flight exact.
+// the count of loads in flight exact (a stage loaded by dwords counts for more
+// and is waited for earlier).
 template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int KSUB, int NS, int VB>
 __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_) {
     constexpr int ES = op_size(OT), NT = WM * WN * 64, KE = KSUB * 64 / ES;
@@ -835,9 +844,8 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
     };
     constexpr int RING = NS * (TA::BYTES + TB::BYTES);
     if (g.c_f32 || !g.accumulate) {
-        const bool chunks = rows16(g);
-        if (g.c_f32) store_tile_rows<4, BM, BN, WM, WN, RING>(g, ring, at0, mrows, jb.n0, wm, wn, lane, chunks, val);
-        else store_tile_rows<2, BM, BN, WM, WN, RING>(g, ring, at0, mrows, jb.n0, wm, wn, lane, chunks, val);
+        if (g.c_f32) store_tile_rows<4, BM, BN, WM, WN, RING>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
+        else store_tile_rows<2, BM, BN, WM, WN, RING>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
         return;
     }
     // a bf16 sum that is added to stays in fp32 until its one rounding
@@ -888,7 +896,7 @@ hipError_t launch_tiles(OpGemmArgs g, int vb, hipStream_t s) {
         return hipErrorInvalidValue;  // (staging through registers leaves too few for these tiles)
     } else if constexpr (OT == OT_F32) {
         if (vb == 4) {
-            MOE_OP_TILES(1, 4, 4);
+            MOE_OP_TILES(KSUB, NS, 4);
         } else if constexpr (BM == 64) {
             MOE_OP_TILES(1, 2, 0);  // row strides of 4 MB and more
         } else {
@@ -920,7 +928,7 @@ hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
     if (tile_offsets_ok(g.lda, ES) && tile_offsets_ok(g.ldb, ES)) {
         if (whole_chunks(g.A, g.lda, 0, ACOL ? g.M : g.K, ES) && whole_chunks(g.B, g.ldb, g.b_stride, BCOL ? g.N : g.K, ES))
             vb = 16;
-        else if (OT == OT_F32)
+        else if (OT == OT_F32 && g.lda >= 4 && g.ldb >= 4)
             vb = 4;
     }
     auto tiles = [&](int b) -> long long {
