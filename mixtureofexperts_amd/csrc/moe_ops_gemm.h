@@ -548,9 +548,11 @@ __device__ __forceinline__ bool vec_ok(const OpGemmArgs &g) {
 // kept at chunk c ^ (r mod CH): the column-wise writes and the row-wise reads
 // both spread over the banks.  The chunks are stored whole at whatever alignment
 // their rows have (12 groups of 259 rows of 1001 / 2731, weight gradient: 169 us, by
-// elements 175; bf16 69, by elements 75).  EO: bytes of a result; PR rows at a time.  val(i,
+// elements 175; bf16 69, by elements 75).  PAST: around the caches (weight gradients,
+// which the optimizer reads when all of them are done: 64 Zipf groups of 2048 / 1408
+// 383 us, 404 through the caches; results of row products gain nothing).  EO: bytes of a result; PR rows at a time.  val(i,
 // j, c): the lane's result in row block i, column block j, column 4 (lane / 16) + c.
-template <int EO, int BM, int BN, int WM, int WN, int RING, typename Val>
+template <int EO, int BM, int BN, int WM, int WN, int RING, bool PAST, typename Val>
 __device__ __forceinline__ void store_tile_rows(const OpGemmArgs &g, lds_u8 *ring, long long at0, int mrows, int n0,
                                                 int wm, int wn, int lane, Val val) {
     constexpr int NT = WM * WN * 64, NJ = BN / WN / 16;
@@ -598,7 +600,9 @@ __device__ __forceinline__ void store_tile_rows(const OpGemmArgs &g, lds_u8 *rin
                                 v[q] = __float_as_uint(__uint_as_float(o[q]) + __uint_as_float(v[q]));
                         }
                     }
-                    __builtin_memcpy(dst, &v, 16);
+                    typedef u32x4 __attribute__((aligned(2))) u32x4_u;
+                    if constexpr (PAST) __builtin_nontemporal_store(v, (u32x4_u *)dst);
+                    else *(u32x4_u *)dst = v;
                 } else {
 #pragma unroll
                     for (int q = 0; q < CE; ++q) {
@@ -844,8 +848,8 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
     };
     constexpr int RING = NS * (TA::BYTES + TB::BYTES);
     if (g.c_f32 || !g.accumulate) {
-        if (g.c_f32) store_tile_rows<4, BM, BN, WM, WN, RING>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
-        else store_tile_rows<2, BM, BN, WM, WN, RING>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
+        if (g.c_f32) store_tile_rows<4, BM, BN, WM, WN, RING, RAGK>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
+        else store_tile_rows<2, BM, BN, WM, WN, RING, RAGK>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
         return;
     }
     // a bf16 sum that is added to stays in fp32 until its one rounding
