@@ -112,16 +112,16 @@ constexpr unsigned kOutOfRange = 0x80000000u;  // past every buffer's num_record
 // One operand's tile of ROWS rows: its LDS stage image and how NT threads fill
 // it.  VB 16 or 4: by buffer loads of 16 bytes a lane straight into LDS, a lane
 // whose bytes lie outside reads zeros by the buffer's own range check.  16: rows
-// of whole, aligned chunks.  4: fp32 rows of any stride (from 4) and length, whose
-// last chunk may hold elements of the next row: of a "col" operand they only
+// of whole, aligned chunks.  4: rows of whole, aligned dwords (fp32: any; at least
+// a chunk apart), whose last chunk may hold elements of the next row: of a "col" operand they only
 // reach results that are not stored, and the next row is there except in the
 // last stage; of a "row" operand they would be summed.  Such a last stage is
-// loaded by dwords (weight gradient, 12 groups of 259 rows of 1001 / 2731: 169 us,
-// by dwords alone 210).  VB 0: through registers, any alignment.
+// loaded by dwords (weight gradient, 12 groups of 259 rows: fp32, 1001 / 2731, 169 us,
+// by dwords alone 210; bf16, 1002 / 2730, 47 us, through registers 75).  VB 0: through registers, any alignment.
 template <int ES, int ROWS, bool COL, int NT, int KSUB, int VB>
 struct Tile {
     static constexpr bool DIRECT = VB > 0;
-    static_assert(VB == 0 || VB == 16 || (VB == 4 && ES == 4), "bytes per lane");
+    static_assert(VB == 0 || VB == 16 || VB == 4, "alignment of the rows");
     static constexpr int CE = 16 / ES;           // elements per chunk
     static constexpr int KE = KSUB * 64 / ES;     // k per stage
     static constexpr int NC = KSUB * ROWS * 4 / NT;  // chunks per thread
@@ -166,8 +166,7 @@ struct Tile {
     }
     // such a stage, by dwords
     __device__ __forceinline__ void load_dwords(const u32x4 &rs, int krem, unsigned lds, int w) const {
-        static_assert(ES == 4, "a dword per element");
-        constexpr int STEP = NT * 4;
+        constexpr int STEP = NT * 4, DE = 4 / ES;  // elements per dword
         const unsigned m0 = __builtin_amdgcn_readfirstlane(lds + w * 256);
 #pragma unroll
         for (int j = 0; j < 4 * NC; j += 4) {
@@ -177,7 +176,7 @@ struct Tile {
                 const int i = (j + q) * NT + (int)threadIdx.x;
                 int row, chunk;
                 place(i / 4, row, chunk);
-                const int elem = chunk * CE + i % 4;
+                const int elem = chunk * CE + i % 4 * DE;
                 const bool ok = COL ? elem < lim && row < krem : row < lim && elem < krem;
                 v[q] = ok ? (unsigned)(row * (int)ldb + elem * ES) : kOutOfRange;
             }
@@ -873,10 +872,10 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WP
     op_gemm_tile<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, KSUB, NS, VB>(g, ring);
 }
 
-// Rows of whole 16-byte chunks.
-inline bool whole_chunks(const void *p, long long ld, long long stride, int contiguous, int es) {
-    return (((uintptr_t)p | (uintptr_t)(ld * es) | (uintptr_t)(stride * es)) & 15) == 0 &&
-           (long long)contiguous * es % 16 == 0;
+// Rows of whole, aligned pieces of `bytes`.
+inline bool whole_pieces(const void *p, long long ld, long long stride, int contiguous, int es, int bytes) {
+    return (((uintptr_t)p | (uintptr_t)(ld * es) | (uintptr_t)(stride * es)) & (bytes - 1)) == 0 &&
+           (long long)contiguous * es % bytes == 0;
 }
 // A tile's byte offsets (up to 255 rows) within 31 bits.
 inline bool tile_offsets_ok(long long ld, int es) { return ld * es < (1ll << 22); }
@@ -892,16 +891,19 @@ hipError_t launch_tiles(OpGemmArgs g, int vb, hipStream_t s) {
         RAGK ? ((long long)g.mt * g.nt * g.splits + 7) / 8 * 8 * g.E : (mtiles * g.nt * g.splits + 7) / 8 * 8;
     if (grid > 0x7fffffffll / (WM * WN * 64)) return hipErrorInvalidValue;
     const dim3 b(WM * WN * 64);
-#define MOE_OP_TILES(KS_, NS_, VB_) \
-    op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, KS_, NS_, WPE, VB_><<<(unsigned)grid, b, 0, s>>>(g)
+    // (bf16 pairs by dwords: the registers of three waves per SIMD are too few)
+    constexpr int W4 = WPE == 3 && BM == 128 && OT == OT_BF16 ? 2 : WPE;
+#define MOE_OP_TILES(KS_, NS_, VB_)                                                                       \
+    op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, KS_, NS_, VB_ == 4 ? W4 : WPE, VB_><<<(unsigned)grid, b, 0, \
+                                                                                              s>>>(g)
     if (vb == 16) {
         MOE_OP_TILES(KSUB, NS, 16);
     } else if constexpr (BN == 256) {
         return hipErrorInvalidValue;  // (staging through registers leaves too few for these tiles)
+    } else if (vb == 4) {
+        MOE_OP_TILES(KSUB, NS, 4);
     } else if constexpr (OT == OT_F32) {
-        if (vb == 4) {
-            MOE_OP_TILES(KSUB, NS, 4);
-        } else if constexpr (BM == 64) {
+        if constexpr (BM == 64) {
             MOE_OP_TILES(1, 2, 0);  // row strides of 4 MB and more
         } else {
             return hipErrorInvalidValue;
@@ -927,13 +929,15 @@ hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
     constexpr int ES = op_size(OT);
     // row operands are loaded in whole 128-byte lines
     constexpr int KSUB = ACOL && BCOL ? 1 : 2;
-    // bytes a lane loads straight into LDS; 0: through registers
+    // alignment of the rows that are loaded straight into LDS; 0: through registers
     int vb = 0;
     if (tile_offsets_ok(g.lda, ES) && tile_offsets_ok(g.ldb, ES)) {
-        if (whole_chunks(g.A, g.lda, 0, ACOL ? g.M : g.K, ES) && whole_chunks(g.B, g.ldb, g.b_stride, BCOL ? g.N : g.K, ES))
-            vb = 16;
-        else if (OT == OT_F32 && g.lda >= 4 && g.ldb >= 4)
-            vb = 4;
+        auto pieces = [&](int bytes) {
+            return whole_pieces(g.A, g.lda, 0, ACOL ? g.M : g.K, ES, bytes) &&
+                   whole_pieces(g.B, g.ldb, g.b_stride, BCOL ? g.N : g.K, ES, bytes);
+        };
+        if (pieces(16)) vb = 16;
+        else if (g.lda >= 16 / ES && g.ldb >= 16 / ES && pieces(4)) vb = 4;
     }
     auto tiles = [&](int b) -> long long {
         const long long nt = (g.N + b - 1) / b;

@@ -309,6 +309,31 @@ def test_wide_strides(moe, dtype):
             at += n
 
 
+@pytest.mark.parametrize("pad", [0, 2, 6])
+@pytest.mark.parametrize("layout", [LLAMA, FLUX])
+def test_rows_of_whole_dwords(moe, layout, pad):
+    # bf16 rows of an even length that do not start on 16 bytes: loaded by chunks
+    # whose last one may reach into the next row (or its padding, NaN here)
+    for lens, K, N in (([1, 0, 30], 2, 6), ([3, 40], 18, 22), ([33, 130, 5, 0, 300], 202, 134), ([700, 0, 900, 500], 70, 2046),
+                       ([100, 40, 0, 64], 1022, 1026), ([71], 5442, 62)):
+        print(f"grouped dword rows layout={layout} pad={pad} lens={lens} K={K} N={N}", flush=True)
+        rng = np.random.default_rng([K, N, layout, pad, 4])
+        M, E = sum(lens), len(lens)
+        w = _mats(rng, E, *((N, K) if layout == LLAMA else (K, N)), "bf16", pad)
+        x, dy, off = _rows(rng, M, K, "bf16", pad), _rows(rng, M, N, "bf16", pad), _offsets(lens)
+        y, dx = moe.grouped_matmul(x, w, off, layout=layout), moe.grouped_matmul_grad_x(dy, w, off, layout=layout)
+        dw = _f64(moe.grouped_matmul_grad_w(x, dy, off, layout=layout, out_dtype=torch.float32))
+        W = _f64(w) if layout == LLAMA else _f64(w).transpose(0, 2, 1)
+        X, D, Y, DX, at = _f64(x), _f64(dy), _f64(y), _f64(dx), 0
+        for e, n in enumerate(lens):
+            s = slice(at, at + n)
+            _close(Y[s], X[s] @ W[e].T, np.abs(X[s]) @ np.abs(W[e].T), K, "bf16")
+            _close(DX[s], D[s] @ W[e], np.abs(D[s]) @ np.abs(W[e]), N, "bf16")
+            g = dw[e] if layout == LLAMA else dw[e].T
+            _close(g, D[s].T @ X[s], np.abs(D[s]).T @ np.abs(X[s]), max(n, 1), "f32")
+            at += n
+
+
 def test_wide_strides_many_tiles(moe):
     # as many tiles as the larger tile sizes take
     print("grouped wide strides, many tiles", flush=True)

@@ -173,3 +173,23 @@ def test_split_sums_with_empty_groups(moe):
             assert (np.abs(y[s] - ref) <= 3.01 * 2.0**-24 * np.abs(ref)).all(), e
             at += n
         assert (y[:start] == 0).all() and (y[at:] == 0).all()
+
+
+@pytest.mark.parametrize("pad", [0, 4])
+def test_codes_of_whole_dwords(moe, pad):
+    # code rows of a multiple of four that do not start on 16 bytes; the padding
+    # holds codes that must not be summed
+    rng = np.random.default_rng(18)
+    for lens, K, N in (([20, 0, 45], 4, 30), ([33, 130, 0, 300], 204, 134), ([700, 0, 900], 68, 2046), ([90], 5444, 62)):
+        print(f"int8 dword rows pad={pad} lens={lens} K={K} N={N}", flush=True)
+        E, M = len(lens), sum(lens)
+        q = torch.from_numpy(rng.integers(-127, 128, (M, K + pad)).astype(np.int8)).cuda()[:, :K]
+        w = torch.from_numpy(rng.integers(-127, 128, (E, N, K + pad)).astype(np.int8)).cuda()[:, :, :K]
+        xs, ws = torch.ones(M, device="cuda"), torch.ones(E, N, device="cuda")
+        off = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+        y = moe.int8_matmul(q, w, ws, off, x_scale=xs, out_dtype=torch.float32).cpu().double().numpy()
+        Q, W, at = q.cpu().numpy().astype(np.int64), w.cpu().numpy().astype(np.int64), 0
+        for e, n in enumerate(lens):
+            ref = Q[at:at + n] @ W[e].T
+            assert (np.abs(y[at:at + n] - ref) <= 2.0**-24 * np.abs(ref)).all(), e
+            at += n
