@@ -6,15 +6,18 @@
 //   forward / row gradient: A "row", B "row" or "col" by the weight's layout;
 //   weight gradient: A and B "col", k running over the group's rows.
 //
-// LDS.  A stage is 64 bytes of k per "row" operand row (32 bf16, 16 fp32, 64
-// int8) and the same number of k rows of a "col" operand.  A lane's fragment
+// LDS.  A stage is KSUB pieces of 64 bytes of k per "row" operand row (32 bf16,
+// 16 fp32, 64 int8) and the same number of k rows of a "col" operand.  KSUB is 2
+// where an operand is "row", so that whole 128-byte lines are read (8192 rows,
+// 8 bf16 experts of 4096 / 14336: 902 us, 954 at 1), else 1.  A lane's fragment
 // is 16 bytes of consecutive k of one row for every type, so one loop serves
 // bf16 (one MFMA per fragment pair), int8 (one) and fp32 (four, element j of
 // each lane's four: the k order inside a fragment is free as long as both
 // operands use the same).
-//   row operand: row r's 16-byte chunk c at slot c ^ (-(r >> 2) & 3): the
-//     sixteen lanes that a ds_read_b128 serves at a time (rows 0-3 and 12-15 of
-//     one k group, 4-7 and 8-11 of the next) lie in all 64 banks once;
+//   row operand: row r's 16-byte chunk c at slot c ^ (-(r >> 2) & 3), KSUB 2: c ^
+//     ((r >> 1) & 7): the sixteen lanes that a ds_read_b128 serves at a time
+//     (rows 0-3 and 12-15 of one k group, 4-7 and 8-11 of the next) lie in all 64
+//     banks once;
 //   col operand: k row kr, its 16-element unit u at unit u ^ col_swz(kr).
 //     bf16 fragments come through ds_read_b64_tr_b16 (16 lanes read 4 k rows
 //     x 16 columns and each receives one column), fp32 ones through four
@@ -549,8 +552,9 @@ __device__ __forceinline__ bool vec_ok(const OpGemmArgs &g) {
 // their rows have (12 groups of 259 rows of 1001 / 2731, weight gradient: 169 us, by
 // elements 175; bf16 69, by elements 75).  PAST: around the caches (weight gradients,
 // which the optimizer reads when all of them are done: 64 Zipf groups of 2048 / 1408
-// 383 us, 404 through the caches; results of row products gain nothing).  EO: bytes of a result; PR rows at a time.  val(i,
-// j, c): the lane's result in row block i, column block j, column 4 (lane / 16) + c.
+// 383 us, 404 through the caches; results of row products gain nothing).  EO:
+// bytes of a result; PR rows at a time.  val(i, j, c): the lane's result in row
+// block i, column block j, column 4 (lane / 16) + c.
 template <int EO, int BM, int BN, int WM, int WN, int RING, bool PAST, typename Val>
 __device__ __forceinline__ void store_tile_rows(const OpGemmArgs &g, lds_u8 *ring, long long at0, int mrows, int n0,
                                                 int wm, int wn, int lane, Val val) {
@@ -621,6 +625,12 @@ __device__ __forceinline__ void store_tile_rows(const OpGemmArgs &g, lds_u8 *rin
 }
 
 // ---- the kernel --------------------------------------------------------------------
+// Bound by the matrix units at the clock that their load leaves: 8192 rows, 8
+// bf16 experts of 4096 / 14336 in 843 us (1140 TFLOP/s, units 56 % busy; one 8192
+// cubed product 1325), their row gradient 844, int8 475 (2020 TOP/s); fp32, 4096
+// cubed, 142 TFLOP/s of 154.  The weight gradient of 64 groups of 2048 / 1408 over
+// 49152 rows (383 us) is bound by its 738 MB result, stored after each tile.
+//
 // WM x WN waves; wave (wm, wn) owns the 16-row blocks wm, wm + WM, ... (so that
 // the blocks of a part-filled tile are spread over the SIMDs, and a wave skips
 // those past the last row) and BN / WN adjacent columns.
@@ -922,7 +932,7 @@ hipError_t launch_tiles(OpGemmArgs g, int vb, hipStream_t s) {
 // experts of 4096 / 14336, 256 x 256 against 128 x 256 with two workgroups per
 // CU: forward 874 / 1055 us, row gradient 852 / 926, int8 563 / 627; the weight
 // gradient of 64 Zipf groups of 2048 / 1408, 256 x 256 against 128 x 128 with three
-// workgroups per CU: 454 / 485 us.  Where even 64 x 64 tiles are few, k is split into
+// workgroups per CU: 411 / 453 us.  Where even 64 x 64 tiles are few, k is split into
 // ranges (op_rows_splits, op_matrix_splits).
 template <int OT, bool ACOL, bool BCOL, bool RAGK>
 hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {

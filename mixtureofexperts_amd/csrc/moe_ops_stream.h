@@ -4,7 +4,10 @@
 //
 // A workgroup owns 16 columns of one group; its four waves take interleaved
 // 128-byte pieces of k, U of them in flight, and their partial 16 x 16 blocks
-// are added in wave order through LDS.
+// are added in wave order through LDS.  Bound by HBM reads: 256 rows on 8 bf16
+// experts of 4096 / 14336 161 us (5.8 TB/s), two int8 rows on two of them 26 us
+// (4.4 TB/s).  32 fp32 rows on 8 experts of 512 / 2048 10 us (3.4 TB/s, one round of
+// workgroups).
 #pragma once
 #include "moe_ops_gemm.h"
 
@@ -233,6 +236,7 @@ struct RowCode {
     }
 };
 
+// Bound by HBM: 8192 x 4096 bf16 rows 24 us (100 MB, 4.2 TB/s).
 // Rows of up to 2048 NV columns, in registers: 256 threads with NV groups of 8
 // columns each (VEC: 16-byte loads of x, 8-byte stores of the codes).
 template <int XB, int NV, bool VEC>
