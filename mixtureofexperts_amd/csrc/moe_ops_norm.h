@@ -156,12 +156,35 @@ __device__ __forceinline__ float row_sum(float v, float *part) {
     return v;
 }
 
+// The same with its last steps in fp64: those of the few largest partial sums,
+// whose roundings would be the sum's (the others' average out).
+template <int TPR>
+__device__ __forceinline__ double row_sum_wide(float v, double *part) {
+    v = add_dpp<0x140>(add_dpp<0x141>(add_dpp<0x4E>(add_dpp<0xB1>(v))));
+    auto row = [&](int l) {
+        return (double)__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+    };
+    double d = (row(0) + row(16)) + (row(32) + row(48));
+    if constexpr (TPR > 64) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = d;
+        __syncthreads();
+        d = part[0];
+#pragma unroll
+        for (int w = 1; w < TPR / 64; ++w) d += part[w];
+    }
+    return d;
+}
 __device__ __forceinline__ float round_to(float v, int bf16) { return bf16 ? bf16_to_f32(f32_to_bf16(v)) : v; }
 
-template <int TPR, int NV, bool VEC>
+// WIDE: a bf16 stream whose norm is wanted in fp32.  An r that a few fp32 roundings
+// put on the other side of a bf16 border (one in 30000) would be 2^-8 off in h, far
+// more than all else there, so r is formed in fp64 and rounded by way of fp32 (one
+// in 290000 then, 2000 x 4096; h off by 2e-6 of its norm, 1.3e-5 before).
+template <int TPR, int NV, bool VEC, bool WIDE>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(NormArgs a) {
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
     __shared__ float part[2][16];
+    __shared__ double wpart[WIDE ? 16 : 1];
     const long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
     if (RPB > 1 && row >= a.T) return;  // whole waves; no barrier below when RPB > 1
     const int tid = threadIdx.x % TPR, D = a.D;
@@ -181,22 +204,45 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(NormA
         }
     }
     float iy = 1.0f;
+    double iyw = 1.0;
     if (a.y && a.post) {
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int q = 0; q < 8; ++q) s += y[i].v[q] * y[i].v[q];
-        iy = 1.0f / sqrtf(row_sum<TPR>(s, part[0]) / (float)D + a.eps);
+        if constexpr (WIDE) {
+            iyw = 1.0 / sqrt(row_sum_wide<TPR>(s, wpart) / (double)D + (double)a.eps);
+            iy = (float)iyw;
+        } else {
+            iy = 1.0f / sqrtf(row_sum<TPR>(s, part[0]) / (float)D + a.eps);
+        }
     }
     const long long grow = a.gate ? row / a.gate_rows : 0;
     float s = 0.0f;
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (tid + i * TPR) * 8;
+            const Row8 p = a.post ? load8<VEC>(a.post, a.w_bf16, 0, c, D) : Row8{};
+            const Row8 t = a.gate ? load8<VEC>(a.gate, a.gate_bf16, grow, c, D) : Row8{};
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                double z = (double)y[i].v[q];
+                if (a.post) z = z * iyw * (double)p.v[q];
+                if (a.gate) z *= (double)t.v[q];
+                r[i].v[q] = (float)((double)a.alpha * (double)r[i].v[q] + (double)a.beta * z);
+            }
+        }
+    }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (tid + i * TPR) * 8;
+        if constexpr (!WIDE) {
 #pragma unroll
-        for (int q = 0; q < 8; ++q) r[i].v[q] *= a.alpha;
-        if (a.y) {
+            for (int q = 0; q < 8; ++q) r[i].v[q] *= a.alpha;
+        }
+        if (!WIDE && a.y) {
             Row8 z = y[i];
             if (a.post) {
                 const Row8 p = load8<VEC>(a.post, a.w_bf16, 0, c, D);
@@ -551,14 +597,14 @@ long long norm_workspace_floats(long long T, int D, long long gate_rows) {
         if (blocks > 0x7fffffffll / 1024) return hipErrorInvalidValue;                   \
         __VA_ARGS__<<<(unsigned)blocks, TPR < 256 ? 256 : TPR, 0, s>>>(a);               \
     }
-template <bool VEC>
+template <bool VEC, bool WIDE>
 static hipError_t norm_launch(const NormArgs &a, hipStream_t s) {
     using namespace ops;
-    if (a.D <= 512) MOE_NORM(a.T, 64, block_norm_kernel<64, 1, VEC>)
-    else if (a.D <= 2048) MOE_NORM(a.T, 256, block_norm_kernel<256, 1, VEC>)
-    else if (a.D <= 4096) MOE_NORM(a.T, 256, block_norm_kernel<256, 2, VEC>)
-    else if (a.D <= 8192) MOE_NORM(a.T, 1024, block_norm_kernel<1024, 1, VEC>)
-    else MOE_NORM(a.T, 1024, block_norm_kernel<1024, 2, VEC>)
+    if (a.D <= 512) MOE_NORM(a.T, 64, block_norm_kernel<64, 1, VEC, WIDE>)
+    else if (a.D <= 2048) MOE_NORM(a.T, 256, block_norm_kernel<256, 1, VEC, WIDE>)
+    else if (a.D <= 4096) MOE_NORM(a.T, 256, block_norm_kernel<256, 2, VEC, WIDE>)
+    else if (a.D <= 8192) MOE_NORM(a.T, 1024, block_norm_kernel<1024, 1, VEC, WIDE>)
+    else MOE_NORM(a.T, 1024, block_norm_kernel<1024, 2, VEC, WIDE>)
     return hipGetLastError();
 }
 template <bool VEC, int XB, int YB, int HB>
@@ -582,7 +628,11 @@ static bool norm_vec(const NormArgs &a) {
     return true;
 }
 static hipError_t norm_run(const NormArgs &a, bool grad, hipStream_t s) {
-    if (!grad) return norm_vec(a) ? norm_launch<true>(a, s) : norm_launch<false>(a, s);
+    if (!grad) {
+        const bool wide = a.x_bf16 && a.h && !a.h_bf16 && a.y && (a.post || a.gate);
+        if (wide) return norm_vec(a) ? norm_launch<true, true>(a, s) : norm_launch<false, true>(a, s);
+        return norm_vec(a) ? norm_launch<true, false>(a, s) : norm_launch<false, false>(a, s);
+    }
     if (!norm_vec(a)) return norm_grad_launch<false, 2, 2, 2>(a, s);
     // the gradient is bound by its instructions as much as by its bytes: types
     // known at compile time, and the weights and the next row held in registers

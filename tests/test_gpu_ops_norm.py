@@ -176,6 +176,24 @@ def test_many_rows_of_one_sum(moe, D, post):
     _check_grad(moe, a, r, stats, dr, dh, "bf16", "f32")
 
 
+@pytest.mark.parametrize("T,D,yt,gates", [(300, 1000, "f32", 300), (200, 4096, "bf16", 0), (60, 12000, "f32", 60), (900, 328, "f32", 1)])
+def test_bf16_stream_with_an_fp32_norm(moe, T, D, yt, gates):
+    # r is the float64 formula's value rounded by way of fp32, but for values whose
+    # sum of squares decides the border: per thread at most 32 squares are added in
+    # fp32, so rstd is off by at most 16 * 2^-24, which moves a bf16 border (2^-8
+    # apart, on either side) for at most 2 * 16 * 2^-24 / 2^-9 = 2^-10 of the elements;
+    # the terms' magnitudes may be up to 4 times r: 2^-8
+    rng = np.random.default_rng([T, D])
+    a = _inputs(rng, T, D, "bf16", yt, "f32", gates, True, True)
+    r, h, _ = _check_forward(moe, a, "bf16", "f32")
+    x, z = _terms(a)
+    want = torch.from_numpy((x + z).astype(np.float32)).to(torch.bfloat16)
+    assert (r.cpu() != want).double().mean() <= 2.0**-8
+    R = _f64(r)
+    ref = R * _rstd(R, True) * _f64(a["pre_weight"])
+    assert (np.abs(_f64(h) - ref) <= (E + 2.0**-24) * np.abs(ref) + 1e-37).all()
+
+
 def test_long_gate_groups(moe):
     # gate rows of many chunks each, a long sum over rows
     for T, D, gates in ((20000, 64, 2), (9000, 512, 3), (4099, 136, 1), (6000, 32, 3000)):
