@@ -394,7 +394,8 @@ def block_norm_grad(dr, dh, r, y=None, stats=None, *, pre_weight=None, post_weig
     device = _same_device(dr, dh, r, y, stats, pre_weight, post_weight, gate)
     dx = torch.empty_like(r)
     dy = torch.empty_like(y) if y is not None else None
-    new = lambda size: torch.empty(size, dtype=torch.float32, device=device)
+    # (a sum over no rows is zero; the call writes a gate row's sum with its rows)
+    new = lambda size: (torch.empty if T else torch.zeros)(size, dtype=torch.float32, device=device)
     dgate = new(gate.shape) if gate is not None else None
     dpost = new(D) if post is not None else None
     dpre = new(D) if pre is not None else None

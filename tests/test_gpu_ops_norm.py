@@ -300,3 +300,20 @@ def test_graph_replay(moe):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(u, v) for u, v in zip(out, want[i])), i
+
+
+@pytest.mark.parametrize("shape", [(32,), (1, 32), (3, 32)])
+def test_no_rows_with_a_gate(moe, shape):
+    # the sum over no rows is zero, also where the allocator's free blocks hold NaN
+    print(f"norm no rows, gate {shape}", flush=True)
+    w, gate = torch.ones(32, device="cuda"), torch.ones(shape, device="cuda")
+    x = torch.empty(0, 32, device="cuda")
+    _, _, stats = moe.block_norm(x, x, pre_weight=w, post_weight=w, gate=gate)
+    for pre, post in itertools.product((w, None), (w, None)):
+        dirt = [torch.full(s, float("nan"), device="cuda") for s in ((32,), (3, 32)) for _ in range(64)]
+        del dirt
+        dx, dy, dgate, dpost, dpre = moe.block_norm_grad(x, x if pre is not None else None, x, x, stats, pre_weight=pre,
+                                                         post_weight=post, gate=gate)
+        assert dx.shape == dy.shape == (0, 32) and dgate.shape == gate.shape
+        for g in (dgate, dpost, dpre):
+            assert g is None or (g == 0).all()
