@@ -498,6 +498,24 @@ __device__ __forceinline__ void k_range(const OpGemmArgs &g, int ks, int KE, int
 }
 
 // ---- results ---------------------------------------------------------------------
+// int8: a row's scale, applied before its channel's.  A sum, up to 2^31, times a
+// scale past 2^96 or a subnormal one would overflow or lose bits where the
+// channel's scale brings the result back, so such a scale is moved by 2^64 and
+// the result moved back; a factor of 1 leaves every other result as it is.
+struct RowScale {
+    float s = 0.0f, back = 1.0f;
+    __device__ __forceinline__ RowScale() {}
+    __device__ __forceinline__ explicit RowScale(float x) {
+        const float m = fabsf(x);
+        const bool big = m > 0x1p96f, tiny = m < 0x1p-126f && m > 0.0f;
+        s = x * (big ? 0x1p-64f : (tiny ? 0x1p64f : 1.0f));
+        back = big ? 0x1p64f : (tiny ? 0x1p-64f : 1.0f);
+    }
+    __device__ __forceinline__ float operator()(int sum, float channel) const {
+        return (float)sum * s * channel * back;
+    }
+};
+
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
     const bf16x2 v = {(__bf16)a, (__bf16)b};
@@ -837,6 +855,7 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
                                : (long long)(jb.lo + jb.m0) * g.ldc;  // the tile's first row in C
     // int8: the lane's scales, of its row blocks and its columns
     float sa[MI], sb[NJ][4];
+    bool far = false;
     if constexpr (OT == OT_I8) {
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
@@ -850,15 +869,29 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
                 const int n = jb.n0 + (wn * NJ + j) * 16 + 4 * q4 + c;
                 sb[j][c] = n < g.N ? g.sb[(long long)jb.e * g.N + n] : 0.0f;
             }
+        // every wave looks at all rows of the tile: the answer is the workgroup's
+        for (int r = lane; r < min(mrows, BM); r += 64) far |= RowScale(g.sa[jb.lo + jb.m0 + r]).back != 1.0f;
+        far = __any(far);
     }
+    constexpr int RING = NS * (TA::BYTES + TB::BYTES);
+    auto store = [&](auto val) {
+        if (g.c_f32) store_tile_rows<4, BM, BN, WM, WN, RING, RAGK>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
+        else store_tile_rows<2, BM, BN, WM, WN, RING, RAGK>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
+    };
     auto val = [&](int i, int j, int c) -> float {
         if constexpr (OT == OT_I8) return (float)acc[i][j][c] * sa[i] * sb[j][c];
         else return acc[i][j][c];
     };
-    constexpr int RING = NS * (TA::BYTES + TB::BYTES);
+    if constexpr (OT == OT_I8) {
+        // (the factor that moves a result back on every one: 8192 rows on 8 experts of
+        // 4096 / 14336 2 % longer)
+        if (far) {
+            store([&](int i, int j, int c) -> float { return RowScale(sa[i])(acc[i][j][c], sb[j][c]); });
+            return;
+        }
+    }
     if (g.c_f32 || !g.accumulate) {
-        if (g.c_f32) store_tile_rows<4, BM, BN, WM, WN, RING, RAGK>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
-        else store_tile_rows<2, BM, BN, WM, WN, RING, RAGK>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
+        store(val);
         return;
     }
     // a bf16 sum that is added to stays in fp32 until its one rounding

@@ -96,11 +96,12 @@ __device__ __forceinline__ void stream_rows(const OpGemmArgs &g, int e, int n0, 
                 if (n + c < g.N) ws[n + c] = v[c];
         } else if (ml < rows) {
             float o[4];
+            RowScale sa;
+            if constexpr (OT == OT_I8) sa = RowScale(g.sa[lo + ml]);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                o[c] = (float)v[c];
-                if constexpr (OT == OT_I8)
-                    o[c] = o[c] * g.sa[lo + ml] * (n + c < g.N ? g.sb[(long long)e * g.N + n + c] : 0.0f);
+                if constexpr (OT == OT_I8) o[c] = sa(v[c], n + c < g.N ? g.sb[(long long)e * g.N + n + c] : 0.0f);
+                else o[c] = v[c];
             }
             put4(g, (long long)(lo + ml) * g.ldc + n, n, o[0], o[1], o[2], o[3], vec_ok(g));
         }
@@ -172,7 +173,7 @@ __global__ __launch_bounds__(256) void op_fold_kernel(OpGemmArgs g) {
     }
     acc_elem<OT> sum = 0;
     for (int s = 0; s < g.splits; ++s) sum += ws[s * per + at];
-    float v = (float)sum;
+    float v;
     if constexpr (OT == OT_I8) {
         int a = 0;
         if (g.offsets) {  // the last group that starts at or before the row
@@ -182,7 +183,9 @@ __global__ __launch_bounds__(256) void op_fold_kernel(OpGemmArgs g) {
                 if (g.offsets[mid] <= row) a = mid; else b = mid - 1;
             }
         }
-        v = v * g.sa[row] * g.sb[(long long)a * g.N + n];
+        v = RowScale(g.sa[row])(sum, g.sb[(long long)a * g.N + n]);
+    } else {
+        v = sum;
     }
     const long long c = e * g.c_stride + row * g.ldc + n;
     if (g.c_f32) {

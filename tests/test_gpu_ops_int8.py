@@ -193,3 +193,113 @@ def test_codes_of_whole_dwords(moe, pad):
             ref = Q[at:at + n] @ W[e].T
             assert (np.abs(y[at:at + n] - ref) <= 2.0**-24 * np.abs(ref)).all(), e
             at += n
+
+
+# streamed, tiled, k split (streamed and tiled): each has its own last step
+SCALED = [([3, 0, 2], 64, 40), ([40, 30, 0, 90], 96, 72), ([3, 0, 2], 20000, 17), ([40, 30], 20000, 33)]
+
+
+@pytest.mark.parametrize("odt", ["f32", "bf16"])
+def test_scales_far_from_one(moe, odt):
+    # rows and channels whose scales nearly cancel: no step on the way may leave
+    # fp32's range or lose bits to its subnormals where the result does not
+    for lens, K, N in SCALED:
+        print(f"int8 far scales ->{odt} lens={lens} K={K} N={N}", flush=True)
+        rng = np.random.default_rng([K, N, 21])
+        E, M = len(lens), sum(lens)
+        q = torch.from_numpy(rng.integers(64, 128, (M, K)).astype(np.int8)).cuda()
+        w = torch.from_numpy(rng.integers(64, 128, (E, N, K)).astype(np.int8)).cuda()
+        off = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+        Q, W = q.cpu().numpy().astype(np.int64), w.cpu().numpy().astype(np.int64)
+        for xs, ws in ((1e33, 1e-33), (3e38, 1e-40), (1e-37, 1e30), (1e-43, 1e36), (-2e35, 1e-36), (1.0, 1.0), (0.0, 2.0)):
+            sx = torch.full((M,), xs, device="cuda") * torch.linspace(0.5, 1.0, M, device="cuda")
+            sw = torch.full((E, N), ws, device="cuda")
+            y = moe.int8_matmul(q, w, sw, off, x_scale=sx, out_dtype=DT[odt]).cpu().double().numpy()
+            SX, SW, at = sx.cpu().double().numpy(), sw.cpu().double().numpy(), 0
+            for e, n in enumerate(lens):
+                s = slice(at, at + n)
+                ref = (Q[s] @ W[e].T) * SX[s, None] * SW[e]
+                # the exact sum to fp32 and two products, then the result's type
+                tol = (3.01 * 2.0**-24 + (2.0**-8 if odt == "bf16" else 0.0)) * np.abs(ref)
+                assert np.isfinite(ref).all() and (np.abs(y[s] - ref) <= tol).all(), (xs, ws, e)
+                at += n
+
+
+@pytest.mark.parametrize("xt", ["bf16", "f32"])
+def test_rows_far_from_one(moe, xt):
+    # the same through the call's own quantiser
+    rng = np.random.default_rng(22)
+    x = torch.from_numpy(rng.standard_normal((6, 300)).astype(np.float32))
+    x = (x * torch.tensor([1e33, 1e-34, 1.0, 1e35, 1e-30, 1e37])[:, None]).to(DT[xt]).cuda()
+    w = torch.from_numpy(rng.integers(-127, 128, (33, 300)).astype(np.int8)).cuda()
+    q, s = moe.quantize_int8(x)
+    for ws in (1e-6, 1e-2, 1.0):
+        y = moe.int8_matmul(x, w, torch.full((33,), ws, device="cuda"), out_dtype=torch.float32).cpu().double().numpy()
+        sw = float(np.float32(ws))
+        ref = (q.cpu().numpy().astype(np.int64) @ w.cpu().numpy().astype(np.int64).T) * s.cpu().double().numpy()[:, None] * sw
+        big = np.abs(ref) > 3.4e38
+        assert (np.abs(y - ref) <= 3.01 * 2.0**-24 * np.abs(ref) + 2.0**-149)[~big].all() and np.isinf(y[big]).all()
+
+
+def test_scales_that_are_not_finite(moe):
+    # a NaN scale gives NaN, an infinite one an infinity, in their rows and columns only
+    rng = np.random.default_rng(23)
+    for M, K, N in ((4, 64, 20), (90, 64, 70), (3, 20000, 17)):
+        q = torch.from_numpy(rng.integers(1, 128, (M, K)).astype(np.int8)).cuda()
+        w = torch.from_numpy(rng.integers(1, 128, (N, K)).astype(np.int8)).cuda()
+        xs, ws = torch.ones(M, device="cuda"), torch.ones(N, device="cuda")
+        xs[1], xs[2], ws[3], ws[5] = float("nan"), float("inf"), float("nan"), float("-inf")
+        y = moe.int8_matmul(q, w, ws, x_scale=xs, out_dtype=torch.float32).cpu().numpy()
+        assert np.isnan(y[1]).all() and np.isnan(y[:, 3]).all()
+        rest = np.delete(np.arange(N), [3, 5])
+        assert np.isposinf(y[2, rest]).all() and np.isneginf(np.delete(y[:, 5], 1)).all()
+        assert np.isfinite(y[np.ix_([0, M - 1], rest)] if M > 3 else y[0, rest]).all()
+
+
+@pytest.mark.parametrize("odt", ["f32", "bf16"])
+def test_scales_far_from_one(moe, odt):
+    # rows and channels whose scales nearly cancel: no step on the way may leave
+    # fp32's range or lose bits to its subnormals where the result does not
+    for lens, K, N in SCALED:
+        print(f"int8 far scales ->{odt} lens={lens} K={K} N={N}", flush=True)
+        rng = np.random.default_rng([K, N, 21])
+        E, M = len(lens), sum(lens)
+        q = torch.from_numpy(rng.integers(64, 128, (M, K)).astype(np.int8)).cuda()
+        w = torch.from_numpy(rng.integers(64, 128, (E, N, K)).astype(np.int8)).cuda()
+        off = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+        Q, W = q.cpu().numpy().astype(np.int64), w.cpu().numpy().astype(np.int64)
+        for xs, ws in ((1e33, 1e-33), (3e38, 1e-40), (1e-37, 1e30), (1e-43, 1e36), (-2e35, 1e-36), (1.0, 1.0), (0.0, 2.0)):
+            sx = torch.full((M,), xs, device="cuda") * torch.linspace(0.5, 1.0, M, device="cuda")
+            sw = torch.full((E, N), ws, device="cuda")
+            y = moe.int8_matmul(q, w, sw, off, x_scale=sx, out_dtype=DT[odt]).cpu().double().numpy()
+            SX, SW, at = sx.cpu().double().numpy(), sw.cpu().double().numpy(), 0
+            for e, n in enumerate(lens):
+                s = slice(at, at + n)
+                ref = (Q[s] @ W[e].T) * SX[s, None] * SW[e]
+                # the exact sum to fp32 and two products, then the result's type
+                tol = (3.01 * 2.0**-24 + (2.0**-8 if odt == "bf16" else 0.0)) * np.abs(ref)
+                assert np.isfinite(ref).all() and (np.abs(y[s] - ref) <= tol).all(), (xs, ws, e)
+                at += n
+
+@pytest.mark.parametrize("lens,K,N", [([700, 0, 900, 500], 144, 2048), ([3000, 5500], 160, 4112)])
+def test_far_scales_in_large_tiles(moe, lens, K, N):
+    # 128 x 128 and 256 x 256 tiles that hold one row of a far scale, many, or none
+    print(f"int8 far scales in large tiles lens={lens}", flush=True)
+    rng = np.random.default_rng([K, N, 24])
+    E, M = len(lens), sum(lens)
+    q = torch.from_numpy(rng.integers(64, 128, (M, K)).astype(np.int8)).cuda()
+    w = torch.from_numpy(rng.integers(64, 128, (E, N, K)).astype(np.int8)).cuda()
+    sx, sw = torch.ones(M, device="cuda"), torch.full((E, N), 1e-3, device="cuda")
+    sx[5], sx[300:310], sx[600], sx[M - 1], sx[M - 2] = 1e35, 1e-42, 0.0, 3e38, -1e-40
+    sw[:, 3::7] = 1e-36
+    off = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+    y = moe.int8_matmul(q, w, sw, off, x_scale=sx, out_dtype=torch.float32).double()
+    at = 0
+    for e, n in enumerate(lens):
+        s = slice(at, at + n)
+        ref = (q[s].double() @ w[e].double().t().contiguous()) * sx[s, None].double() * sw[e].double()
+        # three roundings, the last one possibly to a subnormal; past fp32's largest: infinity
+        big = ref.abs() > 3.4028236e38
+        assert ((y[s] - ref).abs() <= 3.01 * 2.0**-24 * ref.abs() + 2.0**-149)[~big].all(), e
+        assert torch.isinf(y[s])[big].all() and (big.any() or e != E - 1)
+        at += n
