@@ -18,7 +18,7 @@ from .balancing import (AuxiliaryFreeLoss, LoadBalancingLoss, NoBalancingLoss, S
                         update_bias)
 from .experts import GatedExpert, StandardExpert
 from .gating import HOST_ROUTED_GATES, GatingMechanism, TopKGating, gate_spec
-from .ops import block_norm
+from .ops import _plain, block_norm
 
 _DTYPES = {"f32": _lib.MOE_F32, "fp32": _lib.MOE_F32, "bf16": _lib.MOE_BF16, "fp8": _lib.MOE_FP8_E4M3,
            "fp8_e4m3": _lib.MOE_FP8_E4M3}
@@ -313,7 +313,8 @@ def moe_block_forward(moe, x, *, pre_weight, post_weight=None, gate=None, next_w
     loss as a (1,) tensor).  Nothing waits for the GPU, and the layer's
     training_stats are not updated.  Layers whose gate or balance loss keeps
     state on the host (HashGating, RandomGating, AuxiliaryFreeLoss) have no such
-    path, and the call cannot be captured into a graph (block_norm can)."""
+    path, and the call cannot be captured into a graph (block_norm can).  Nothing
+    is recorded for autograd; tensors that it would differentiate are refused."""
     c = moe.config
     if isinstance(moe.router.gate_type, HOST_ROUTED_GATES) or isinstance(moe.balance_loss, AuxiliaryFreeLoss):
         raise _lib.MoeError(_lib.MOE_EUNSUPPORTED, "moe_block_forward: the gate or loss keeps state on the host")
@@ -323,6 +324,7 @@ def moe_block_forward(moe, x, *, pre_weight, post_weight=None, gate=None, next_w
         raise _lib.MoeError(_lib.MOE_EINVAL, f"x must be (T, {c.input_dim})")
     if pre_weight is None:
         raise _lib.MoeError(_lib.MOE_EINVAL, "pre_weight is needed")
+    _plain("x pre_weight post_weight gate next_weight", x, pre_weight, post_weight, gate, next_weight)
     import torch
 
     if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():

@@ -8,6 +8,12 @@ through torch (workspaces included), does not wait for the GPU and can be
 captured into a graph.  Tensors of one call are on one device.  A wrong
 argument raises MoeError.
 
+Nothing is recorded for autograd: the gradients are calls of their own, for an
+autograd.Function or a training loop that makes them itself.  A tensor that
+torch would differentiate (requires_grad while gradients are recorded, or a
+forward-mode tangent) is refused, so that no graph is cut unseen: call under
+torch.no_grad(), inside a Function, or with detached tensors.
+
 Groups: ``offsets`` is an int32 tensor of E + 1 non-decreasing row numbers on
 the device; rows [offsets[e], offsets[e + 1]) belong to expert e, and rows
 outside every group are not written and have no effect.  ``None``: one expert, all
@@ -21,18 +27,19 @@ import ctypes
 from . import _lib
 from ._lib import MOE_EINVAL, MOE_LAYOUT_FLUX_OUT_IN, MOE_LAYOUT_LLAMA_IN_OUT
 
-_torch = None
+_torch = _forward_ad = _written = None
 _codes = {}
 _floats = []  # the types of float operands
 
 
 def _t():
     """torch, imported at first use (the host API needs only numpy)."""
-    global _torch
+    global _torch, _forward_ad, _written
     if _torch is None:
         import torch
+        import torch.autograd.forward_ad as forward_ad
 
-        _torch = torch
+        _torch, _forward_ad, _written = torch, forward_ad, torch.autograd.graph.increment_version
         _floats.extend((torch.float32, torch.bfloat16))
         _codes.update({torch.float32: _lib.MOE_F32, torch.bfloat16: _lib.MOE_BF16, torch.int8: _lib.MOE_INT8})
     return _torch
@@ -40,6 +47,21 @@ def _t():
 
 def _bad(msg):
     raise _lib.MoeError(MOE_EINVAL, msg)
+
+
+def _plain(names, *tensors):
+    """Refuses what autograd would have to record (see above); names: the
+    arguments', as one string."""
+    torch = _torch or _t()
+    if torch.is_grad_enabled():
+        for i, t in enumerate(tensors):
+            if t is not None and getattr(t, "requires_grad", False):
+                _bad(f"{names.split()[i]} requires a gradient, which this call does not record: use torch.no_grad() or "
+                     "detach it")
+    if _forward_ad._current_level >= 0:  # within a forward_ad.dual_level()
+        for i, t in enumerate(tensors):
+            if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+                _bad(f"{names.split()[i]} carries a tangent, which this call does not propagate")
 
 
 def _tensor(t, name, dtypes, dims):
@@ -173,7 +195,7 @@ def _float_types(dtype):
 
 
 def _rows_product(fn, x, name, w, offsets, layout, out, out_dtype, grad):
-    _t()
+    _plain(name + " w out", x, w, out)
     xp, ldx = _rows(x, name, _floats)
     E, a, b, ldw, stride = _matrices(w, "w", (x.dtype,))
     in_dim, out_dim = (a, b) if _layout(layout) else (b, a)
@@ -182,11 +204,14 @@ def _rows_product(fn, x, name, w, offsets, layout, out, out_dtype, grad):
         _bad(f"{name} has {x.shape[1]} columns, the weights take {k}")
     if out is None and out_dtype is None:
         out_dtype = x.dtype
+    given = out
     out = _result(out, (x.shape[0], n), out_dtype, _float_types(x.dtype), x, offsets is not None)
     device, M, dt = _same_device(x, w, offsets, out), x.shape[0], _codes[x.dtype]
     ws, wsp, wsn = _workspace(_lib.lib().moe_grouped_matmul_workspace, device, E, M, in_dim, out_dim, dt)
     _call(fn, device, xp, ldx, w.data_ptr(), ldw, stride, layout, _offsets(offsets, E), E, M, in_dim, out_dim, dt,
           out.data_ptr(), _row_stride(out, "out"), _codes[out.dtype], wsp, wsn)
+    if given is not None:
+        _written(out)  # autograd sees the caller's tensor change
     return out
 
 
@@ -211,6 +236,7 @@ def grouped_matmul_grad_w(x, dy, offsets=None, *, layout=MOE_LAYOUT_LLAMA_IN_OUT
     rows.  ``accumulate`` adds to what ``out`` holds (in float32, rounded
     once)."""
     torch = _t()
+    _plain("x dy out", x, dy, out)
     L = _lib.lib()
     xp, ldx = _rows(x, "x", _floats)
     dp, lddy = _rows(dy, "dy", (x.dtype,))
@@ -225,6 +251,7 @@ def grouped_matmul_grad_w(x, dy, offsets=None, *, layout=MOE_LAYOUT_LLAMA_IN_OUT
     if out is None and out_dtype is None:
         out_dtype = x.dtype
     shape = (a, b) if (out.dim() == 2 if out is not None else offsets is None) and E == 1 else (E, a, b)
+    given = out
     out = _result(out, shape, out_dtype, _float_types(x.dtype), x, False)
     _, _, _, ldw, stride = _matrices(out, "out", _float_types(x.dtype))
     device = _same_device(x, dy, offsets, out)
@@ -232,6 +259,8 @@ def grouped_matmul_grad_w(x, dy, offsets=None, *, layout=MOE_LAYOUT_LLAMA_IN_OUT
     _call(L.moe_grouped_matmul_grad_w_async, device, xp, ldx, dp, lddy, layout, _offsets(offsets, E), E, x.shape[0],
           x.shape[1], dy.shape[1], _codes[x.dtype], out.data_ptr(), ldw, stride, _codes[out.dtype], int(accumulate),
           wsp, wsn)
+    if given is not None:
+        _written(out)  # autograd sees the caller's tensor change
     return out
 
 
@@ -242,6 +271,7 @@ def quantize_int8(x):
     one that holds an infinity or a NaN scale NaN.  Of a weight (E, out, in)
     this gives the codes and scales that int8_matmul takes."""
     torch = _t()
+    _plain("x", x)
     _tensor(x, "x", _floats, range(1, 9))
     if not 1 <= x.shape[-1] < 2**31:
         _bad("x must have 1 to 2^31 - 1 columns")
@@ -261,6 +291,7 @@ def int8_matmul(x, w, w_scale, offsets=None, *, x_scale=None, out=None, out_dtyp
     with ``out_dtype``, float32; without ``out`` rows outside every group are
     zeros."""
     torch = _t()
+    _plain("x w_scale x_scale out", x, w_scale, x_scale, out)
     L = _lib.lib()
     xp, ldx = _rows(x, "x", (torch.float32, torch.bfloat16, torch.int8))
     E, n, k, ldw, stride = _matrices(w, "w", (torch.int8,))
@@ -278,12 +309,15 @@ def int8_matmul(x, w, w_scale, offsets=None, *, x_scale=None, out=None, out_dtyp
             _bad("x_scale must be contiguous with one scale per row")
     if out is None and out_dtype is None:
         out_dtype = torch.bfloat16
+    given = out
     out = _result(out, (x.shape[0], n), out_dtype, (torch.bfloat16, torch.float32), x, offsets is not None)
     device = _same_device(x, w, w_scale, x_scale, offsets, out)
     ws, wsp, wsn = _workspace(L.moe_int8_matmul_workspace, device, E, x.shape[0], k, n, _codes[x.dtype])
     _call(L.moe_int8_matmul_async, device, xp, ldx, _codes[x.dtype], x_scale.data_ptr() if codes else None,
           w.data_ptr(), ldw, stride, w_scale.data_ptr(), _offsets(offsets, E), E, x.shape[0], k, n, out.data_ptr(),
           _row_stride(out, "out"), _codes[out.dtype], wsp, wsn)
+    if given is not None:
+        _written(out)  # autograd sees the caller's tensor change
     return out
 
 
@@ -337,6 +371,7 @@ def block_norm(x, y=None, *, pre_weight=None, post_weight=None, gate=None, alpha
     rows for the next T / G of the T rows.  Returns (r, h, stats); stats (T, 2)
     is what block_norm_grad needs.  Without y and with alpha 1 r is x."""
     torch = _t()
+    _plain("x y pre_weight post_weight gate", x, y, pre_weight, post_weight, gate)
     _tensor(x, "x", _floats, range(1, 9))
     shape = x.shape
     D = shape[-1]
@@ -372,6 +407,7 @@ def block_norm_grad(dr, dh, r, y=None, stats=None, *, pre_weight=None, post_weig
     (dx, dy, dgate, dpost, dpre), None for what the call does not have; dx in
     r's type, dy in y's, the others float32."""
     torch = _t()
+    _plain("dr dh r y stats pre_weight post_weight gate", dr, dh, r, y, stats, pre_weight, post_weight, gate)
     L = _lib.lib()
     _tensor(r, "r", _floats, range(1, 9))
     shape = r.shape
