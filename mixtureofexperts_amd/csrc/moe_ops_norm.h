@@ -176,10 +176,16 @@ __device__ __forceinline__ double row_sum_wide(float v, double *part) {
 }
 __device__ __forceinline__ float round_to(float v, int bf16) { return bf16 ? bf16_to_f32(f32_to_bf16(v)) : v; }
 
-// WIDE: a bf16 stream whose norm is wanted in fp32.  An r that a few fp32 roundings
-// put on the other side of a bf16 border (one in 30000) would be 2^-8 off in h, far
-// more than all else there, so r is formed in fp64 and rounded by way of fp32 (one
-// in 290000 then, 2000 x 4096; h off by 2e-6 of its norm, 1.3e-5 before).
+// WIDE: a bf16 stream that a gate or a post norm is added to.  An r that a few fp32
+// roundings put on the other side of a bf16 border (one in 30000) would be 2^-8 off
+// in an fp32 h, far more than all else there, and whether h is wanted, and in which
+// type, may not decide r.  So r is always the fp64 formula's value rounded by way of
+// fp32 (one in 290000 on the other side then; 2000 x 4096: an fp32 h off by 2e-6 of its
+// norm, 1.3e-5 by fp32 steps): it is formed in fp32, and again in fp64 where a border
+// lies within what the fp32 steps may be off (about an element in 4000).  They round by
+// 2^-24 of the terms' magnitudes each: rstd and its two products, the gate, beta (or
+// alpha), the sum, and the way by fp32: seven.  8192 x 4096, fp32 y, both norms, a gate:
+// 69 us, 67 all in fp32, 81 all in fp64 (117 registers instead of 70).
 template <int TPR, int NV, bool VEC, bool WIDE>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(NormArgs a) {
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
@@ -189,17 +195,18 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(NormA
     if (RPB > 1 && row >= a.T) return;  // whole waves; no barrier below when RPB > 1
     const int tid = threadIdx.x % TPR, D = a.D;
     Row8 r[NV], y[NV];
+    Raw8 rx[NV];
     {
-        Raw8 rx[NV], ry[NV];
+        Raw8 ry[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (tid + i * TPR) * 8;
-            rx[i] = load_raw<VEC>(a.x, a.x_bf16, row, c, D);
+            rx[i] = load_raw<VEC>(a.x, WIDE ? 1 : a.x_bf16, row, c, D);
             ry[i] = a.y ? load_raw<VEC>(a.y, a.y_bf16, row, c, D) : Raw8{};
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            r[i] = widen<VEC>(rx[i], a.x_bf16);
+            if constexpr (!WIDE) r[i] = widen<VEC>(rx[i], a.x_bf16);
             y[i] = widen<VEC>(ry[i], a.y_bf16);
         }
     }
@@ -212,7 +219,13 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(NormA
 #pragma unroll
             for (int q = 0; q < 8; ++q) s += y[i].v[q] * y[i].v[q];
         if constexpr (WIDE) {
-            iyw = 1.0 / sqrt(row_sum_wide<TPR>(s, wpart) / (double)D + (double)a.eps);
+            const double m = row_sum_wide<TPR>(s, wpart) / (double)D + (double)a.eps;
+            if (m > 1e-30 && m < 1e30) {  // a Newton step of 1 / sqrt(m) from its fp32 value
+                const double v = 1.0f / sqrtf((float)m);
+                iyw = v * (1.5 - 0.5 * m * v * v);
+            } else {
+                iyw = 1.0 / sqrt(m);
+            }
             iy = (float)iyw;
         } else {
             iy = 1.0f / sqrtf(row_sum<TPR>(s, part[0]) / (float)D + a.eps);
@@ -226,12 +239,22 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(NormA
             const int c = (tid + i * TPR) * 8;
             const Row8 p = a.post ? load8<VEC>(a.post, a.w_bf16, 0, c, D) : Row8{};
             const Row8 t = a.gate ? load8<VEC>(a.gate, a.gate_bf16, grow, c, D) : Row8{};
+            r[i] = widen<VEC>(rx[i], 1);
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
-                double z = (double)y[i].v[q];
-                if (a.post) z = z * iyw * (double)p.v[q];
-                if (a.gate) z *= (double)t.v[q];
-                r[i].v[q] = (float)((double)a.alpha * (double)r[i].v[q] + (double)a.beta * z);
+                float z = y[i].v[q];
+                if (a.post) z = z * iy * p.v[q];
+                if (a.gate) z *= t.v[q];
+                const float ax = a.alpha * r[i].v[q], bz = a.beta * z;
+                float v = ax + bz;
+                const float border = __uint_as_float((__float_as_uint(v) & 0xffff0000u) | 0x8000u);
+                if (!(fabsf(v - border) > (fabsf(ax) + fabsf(bz)) * 0x1.c8p-22f)) {
+                    double w = (double)y[i].v[q];
+                    if (a.post) w = w * iyw * (double)p.v[q];
+                    if (a.gate) w *= (double)t.v[q];
+                    v = (float)((double)a.alpha * (double)r[i].v[q] + (double)a.beta * w);
+                }
+                r[i].v[q] = v;
             }
         }
     }
@@ -629,7 +652,7 @@ static bool norm_vec(const NormArgs &a) {
 }
 static hipError_t norm_run(const NormArgs &a, bool grad, hipStream_t s) {
     if (!grad) {
-        const bool wide = a.x_bf16 && a.h && !a.h_bf16 && a.y && (a.post || a.gate);
+        const bool wide = a.x_bf16 && a.y && (a.post || a.gate);
         if (wide) return norm_vec(a) ? norm_launch<true, true>(a, s) : norm_launch<false, true>(a, s);
         return norm_vec(a) ? norm_launch<true, false>(a, s) : norm_launch<false, false>(a, s);
     }

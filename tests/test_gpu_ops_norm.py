@@ -317,3 +317,52 @@ def test_no_rows_with_a_gate(moe, shape):
         assert dx.shape == dy.shape == (0, 32) and dgate.shape == gate.shape
         for g in (dgate, dpost, dpre):
             assert g is None or (g == 0).all()
+
+
+@pytest.mark.parametrize("T,D,yt,post,gates", [(2000, 4096, "f32", True, 2000), (3000, 328, "f32", False, 3), (700, 12000, "bf16", True, 0),
+                                               (2500, 2050, "bf16", True, 1)])
+def test_the_stream_does_not_depend_on_what_else_is_asked_for(moe, T, D, yt, post, gates):
+    # r and rstd(y) with h in fp32, h in bf16 and no h, in the memory of x and not:
+    # a forward pass computed again for its backward has to give the same bits.
+    # (r formed once in fp64 and once in fp32 differs at one element in about 30000:
+    # none in 980000 or more would be an accident of probability e^-30.)
+    print(f"norm stream T={T} D={D} {yt} post={post} gates={gates}", flush=True)
+    rng = np.random.default_rng([T, D, 3])
+    a = _inputs(rng, T, D, "bf16", yt, "f32", gates, True, post)
+    x, y, pre = a.pop("x"), a.pop("y"), a.pop("pre_weight")
+    a.update(alpha=ALPHA, beta=BETA, eps=EPS)
+    r, h32, stats = moe.block_norm(x, y, pre_weight=pre, h_dtype=torch.float32, **a)
+    r16, h16, stats16 = moe.block_norm(x, y, pre_weight=pre, **a)
+    r0, none, stats0 = moe.block_norm(x, y, **a)
+    assert none is None and torch.equal(r, r16) and torch.equal(r, r0)
+    assert torch.equal(stats, stats16) and torch.equal(stats[:, 0], stats0[:, 0])
+    assert torch.equal(h16, h32.to(torch.bfloat16))
+
+
+def test_bf16_stream_is_formed_closer_than_in_fp32(moe):
+    # against the float64 formula's r, rounded by way of fp32 as torch does: r formed
+    # in fp32 by plain operations lands on the other bf16 neighbour at about one
+    # element in 30000 (250 of these), at most a third as often may the call; every
+    # such r is one bf16 step off, so h's distance from the norm of the right r is
+    # at most sqrt(1/3) of theirs, 0.7 with room for the sizes of the values hit
+    T, D = 2000, 4096
+    print("norm bf16 stream, fp64 against fp32", flush=True)
+    rng = np.random.default_rng(77)
+    a = _inputs(rng, T, D, "bf16", "f32", "f32", T, True, True)
+    x, z = _terms(a)
+    want = torch.from_numpy((x + z).astype(np.float32)).to(torch.bfloat16)
+    r, h, _ = moe.block_norm(a["x"], a["y"], pre_weight=a["pre_weight"], post_weight=a["post_weight"], gate=a["gate"],
+                             alpha=ALPHA, beta=BETA, eps=EPS, h_dtype=torch.float32)
+    f = lambda t: t.float().cpu()
+    y = f(a["y"])
+    zf = y * torch.rsqrt((y * y).mean(1, keepdim=True) + EPS) * f(a["post_weight"]) * f(a["gate"])
+    plain = (ALPHA * f(a["x"]) + BETA * zf).to(torch.bfloat16)
+    flips, fp32 = int((r.cpu() != want).sum()), int((plain != want).sum())
+    print("other neighbour:", flips, "in fp32:", fp32, flush=True)
+    assert fp32 >= 100 and 3 * flips <= fp32
+    W = _f64(want)
+    ref = W * _rstd(W, True) * _f64(a["pre_weight"])
+    P = _f64(plain)
+    off = np.linalg.norm(_f64(h) - ref) / np.linalg.norm(ref)
+    off32 = np.linalg.norm(P * _rstd(P, True) * _f64(a["pre_weight"]) - ref) / np.linalg.norm(ref)
+    assert off <= 0.7 * off32, (off, off32)
