@@ -409,8 +409,12 @@ int moe_read_counts(moe_handle *h, int32_t *counts);
  * held within [0, rows] by the kernels; with offsets that decrease the results
  * are undefined.  A group may be empty; rows outside every group are not
  * written and their values have no effect.  offsets may be NULL with groups =
- * 1: all rows.  rows = 0 is no work.  Sizes up to 2^30; a result must not
- * overlap an operand.
+ * 1: all rows.  rows = 0 is no work.  A result must not overlap an operand.
+ *
+ * Sizes and numbers of rows, of the norms and the quantiser too, go up to 2^30.
+ * A product runs in one launch of at most 8 million workgroups (2^31 threads),
+ * each with 256 x 256, 128 x 128 or 64 x 64 results by the call's sizes, or 16
+ * columns of a group of few rows; a call that needs more is refused.
  *
  * Matrices: group e's starts w_stride elements after group e - 1's;
  * MOE_LAYOUT_LLAMA_IN_OUT: memory [out_dim][in_dim], MOE_LAYOUT_FLUX_OUT_IN:

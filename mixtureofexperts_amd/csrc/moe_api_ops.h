@@ -184,12 +184,12 @@ int moe_quantize_int8_async(const void *x, int64_t ldx, int32_t x_dtype, int64_t
     if (x_dtype != MOE_F32 && x_dtype != MOE_BF16) return op_fail(fn, "x_dtype must be MOE_F32 or MOE_BF16");
     if (rows < 0 || cols < 1) return op_fail(fn, "rows must not be negative and cols positive");
     if (cols > kOpMaxSize) return op_fail(fn, "sizes above 2^30");
+    if (rows > kOpMaxSize) return op_fail(fn, "too many rows (above 2^30)");
     if (ldx < cols || ldq < cols) return op_fail(fn, "a row stride is smaller than its row");
     if (rows == 0) return MOE_OK;
     if (!x || !q || !scale) return op_fail(fn, "null buffer");
     if (op_misaligned(x, x_dtype) || op_misaligned(scale, MOE_F32))
         return op_fail(fn, "a buffer is not aligned to its elements");
-    if (rows > INT_MAX / 256) return op_fail(fn, "too many rows");
     return op_done(fn, launch_quantize_i8(x, ldx, x_dtype == MOE_BF16, rows, cols, (int8_t *)q, ldq, cols, scale,
                                           (hipStream_t)stream));
 }
@@ -232,7 +232,6 @@ int moe_int8_matmul_async(const void *x, int64_t ldx, int32_t x_dtype, const flo
     if ((!codes && op_misaligned(x, x_dtype)) || op_misaligned(y, y_dtype) || op_misaligned(w_scale, MOE_F32) ||
         (codes && op_misaligned(x_scale, MOE_F32)))
         return op_fail(fn, "a buffer is not aligned to its elements");
-    if (rows > INT_MAX / 256) return op_fail(fn, "too many rows");
     int64_t need = 0;
     r = moe_int8_matmul_workspace(groups, rows, in_dim, out_dim, x_dtype, &need);
     if (r == MOE_OK) r = op_check_workspace(fn, need, workspace, workspace_bytes);
@@ -265,7 +264,7 @@ static int op_check_norm(const char *fn, int64_t T, int32_t D, int32_t x_dtype, 
         if (t != MOE_F32 && t != MOE_BF16) return op_fail(fn, "dtypes must be MOE_F32 or MOE_BF16");
     if (T < 0) return op_fail(fn, "T must not be negative");
     if (D < 1 || D > kMaxNormDim) return op_fail(fn, "D must be 1 to " + std::to_string(kMaxNormDim));
-    if (T > INT_MAX / 1024) return op_fail(fn, "too many rows");
+    if (T > kOpMaxSize) return op_fail(fn, "too many rows (above 2^30)");
     if (gate && gate_rows < 1) return op_fail(fn, "gate_rows must be positive");
     return MOE_OK;
 }
@@ -298,7 +297,7 @@ int moe_block_norm_async(const void *x, int32_t x_dtype, const void *y, int32_t 
 int moe_block_norm_grad_workspace(int64_t T, int32_t D, int64_t gate_rows, int64_t *bytes) {
     const char *fn = "moe_block_norm_grad_workspace";
     if (!bytes) return op_fail(fn, "null bytes");
-    if (T < 0 || T > INT_MAX / 1024 || D < 1 || D > kMaxNormDim || gate_rows < 0) return op_fail(fn, "bad sizes");
+    if (T < 0 || T > kOpMaxSize || D < 1 || D > kMaxNormDim || gate_rows < 0) return op_fail(fn, "bad sizes");
     *bytes = T == 0 ? 0 : 4 * (int64_t)norm_workspace_floats(T, D, gate_rows);
     return MOE_OK;
 }

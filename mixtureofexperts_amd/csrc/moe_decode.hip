@@ -594,12 +594,12 @@ hipError_t launch_op_fold(int ot, bool ragged_k, const OpGemmArgs &g, hipStream_
 template <int XB, bool VEC>
 static void quantize_rows(const void *x, long long ldx, long long rows, int cols, int8_t *q, long long ldq, int pad_to,
                           float *scale, hipStream_t s) {
-    const dim3 g((unsigned)rows), b(256);
-    if (pad_to <= 2048) ops::quantize_i8_kernel<XB, 1, VEC><<<g, b, 0, s>>>(x, ldx, cols, q, ldq, pad_to, scale);
-    else if (pad_to <= 4096) ops::quantize_i8_kernel<XB, 2, VEC><<<g, b, 0, s>>>(x, ldx, cols, q, ldq, pad_to, scale);
-    else if (pad_to <= 8192) ops::quantize_i8_kernel<XB, 4, VEC><<<g, b, 0, s>>>(x, ldx, cols, q, ldq, pad_to, scale);
-    else if (pad_to <= 16384) ops::quantize_i8_kernel<XB, 8, VEC><<<g, b, 0, s>>>(x, ldx, cols, q, ldq, pad_to, scale);
-    else ops::quantize_i8_long_kernel<XB><<<g, b, 0, s>>>(x, ldx, cols, q, ldq, pad_to, scale);
+    const dim3 g = op_row_grid(rows), b(256);
+    if (pad_to <= 2048) ops::quantize_i8_kernel<XB, 1, VEC><<<g, b, 0, s>>>(x, ldx, rows, cols, q, ldq, pad_to, scale);
+    else if (pad_to <= 4096) ops::quantize_i8_kernel<XB, 2, VEC><<<g, b, 0, s>>>(x, ldx, rows, cols, q, ldq, pad_to, scale);
+    else if (pad_to <= 8192) ops::quantize_i8_kernel<XB, 4, VEC><<<g, b, 0, s>>>(x, ldx, rows, cols, q, ldq, pad_to, scale);
+    else if (pad_to <= 16384) ops::quantize_i8_kernel<XB, 8, VEC><<<g, b, 0, s>>>(x, ldx, rows, cols, q, ldq, pad_to, scale);
+    else ops::quantize_i8_long_kernel<XB><<<g, b, 0, s>>>(x, ldx, rows, cols, q, ldq, pad_to, scale);
 }
 
 hipError_t launch_quantize_i8(const void *x, long long ldx, int x_bf16, long long rows, int cols, int8_t *q,

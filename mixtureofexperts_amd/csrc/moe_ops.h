@@ -46,6 +46,14 @@ __device__ __forceinline__ void op_group(const int *offsets, int e, int rows, in
     }
 }
 
+// Grid of kernels with a row (or a few) per workgroup: 2^20 workgroups along x, since
+// a dimension's threads have to fit 32 bits, and the workgroup's number in it.
+inline dim3 op_row_grid(long long blocks) {
+    constexpr long long X = 1 << 20;
+    return blocks <= X ? dim3((unsigned)blocks) : dim3((unsigned)X, (unsigned)((blocks + X - 1) / X));
+}
+__device__ __forceinline__ long long op_row_block() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // Few rows per group and the weights as rows: streamed (moe_ops_stream.h).
 inline bool op_streamed(bool b_col, long long rows, long long E) { return !b_col && rows <= 16 * E; }
 

@@ -191,8 +191,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(NormA
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
     __shared__ float part[2][16];
     __shared__ double wpart[WIDE ? 16 : 1];
-    const long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
-    if (RPB > 1 && row >= a.T) return;  // whole waves; no barrier below when RPB > 1
+    const long long row = op_row_block() * RPB + threadIdx.x / TPR;
+    if (row >= a.T) return;  // whole waves; no barrier below when RPB > 1, the whole workgroup otherwise
     const int tid = threadIdx.x % TPR, D = a.D;
     Row8 r[NV], y[NV];
     Raw8 rx[NV];
@@ -589,7 +589,7 @@ static int norm_grad_threads(int D) {
 }
 
 // Chunks of the gradient's rows: about eight waves per CU, at least four rows
-// each (their sums are written once per chunk).
+// each (their sums are written once per chunk); a few thousand at most, whatever T.
 static void norm_chunks(long long T, int D, long long gate_rows, long long &chunk_rows, long long &cpg,
                         long long &chunks) {
     const long long target = 2048 / (norm_grad_threads(D) / 64);
@@ -617,8 +617,7 @@ long long norm_workspace_floats(long long T, int D, long long gate_rows) {
 #define MOE_NORM(N, TPR, ...)                                                            \
     {                                                                                    \
         const long long rpb = TPR < 256 ? 256 / TPR : 1, blocks = ((N) + rpb - 1) / rpb; \
-        if (blocks > 0x7fffffffll / 1024) return hipErrorInvalidValue;                   \
-        __VA_ARGS__<<<(unsigned)blocks, TPR < 256 ? 256 : TPR, 0, s>>>(a);               \
+        __VA_ARGS__<<<op_row_grid(blocks), TPR < 256 ? 256 : TPR, 0, s>>>(a);            \
     }
 template <bool VEC, bool WIDE>
 static hipError_t norm_launch(const NormArgs &a, hipStream_t s) {

@@ -243,10 +243,11 @@ struct RowCode {
 // Rows of up to 2048 NV columns, in registers: 256 threads with NV groups of 8
 // columns each (VEC: 16-byte loads of x, 8-byte stores of the codes).
 template <int XB, int NV, bool VEC>
-__global__ __launch_bounds__(256) void quantize_i8_kernel(const void *x_, long long ldx, int cols, int8_t *q_,
-                                                          long long ldq, int pad_to, float *scale) {
+__global__ __launch_bounds__(256) void quantize_i8_kernel(const void *x_, long long ldx, long long rows, int cols,
+                                                          int8_t *q_, long long ldq, int pad_to, float *scale) {
     __shared__ float part[4];
-    const long long r = blockIdx.x;
+    const long long r = op_row_block();
+    if (r >= rows) return;
     int8_t *q = q_ + r * ldq;
     float v[NV][8];
 #pragma unroll
@@ -305,10 +306,11 @@ __global__ __launch_bounds__(256) void quantize_i8_kernel(const void *x_, long l
 }
 // Longer rows, read twice.
 template <int XB>
-__global__ __launch_bounds__(256) void quantize_i8_long_kernel(const void *x_, long long ldx, int cols, int8_t *q_,
-                                                               long long ldq, int pad_to, float *scale) {
+__global__ __launch_bounds__(256) void quantize_i8_long_kernel(const void *x_, long long ldx, long long rows, int cols,
+                                                               int8_t *q_, long long ldq, int pad_to, float *scale) {
     __shared__ float part[4];
-    const long long r = blockIdx.x;
+    const long long r = op_row_block();
+    if (r >= rows) return;
     int8_t *q = q_ + r * ldq;
     auto at = [&](int c) -> float {
         if constexpr (XB) return bf16_to_f32(((const uint16_t *)x_)[r * ldx + c]);

@@ -21,6 +21,10 @@ rows.  Weights are (E, out, in) with ``layout=MOE_LAYOUT_LLAMA_IN_OUT`` (the
 default) and (E, in, out) with ``MOE_LAYOUT_FLUX_OUT_IN``; one expert's may be
 2-D.  Rows may be strided (contiguous within a row); 16-byte aligned rows are
 read faster.  A result must not overlap an operand.
+
+Sizes and rows go up to 2^30.  A product is one launch of at most 8 million
+workgroups, each with 64 x 64 results or more (few rows per group: 16 columns
+of one); what needs more is refused.
 """
 import ctypes
 

@@ -303,3 +303,22 @@ def test_far_scales_in_large_tiles(moe, lens, K, N):
         assert ((y[s] - ref).abs() <= 3.01 * 2.0**-24 * ref.abs() + 2.0**-149)[~big].all(), e
         assert torch.isinf(y[s])[big].all() and (big.any() or e != E - 1)
         at += n
+
+
+@pytest.mark.parametrize("rows", [2**20 + 9, 2**23 + 5])
+def test_millions_of_rows(moe, rows):
+    # more rows than one dimension of a launch takes, through the quantiser and the product
+    print(f"int8 rows {rows}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn(rows, 16, generator=g, device="cuda").to(torch.bfloat16)
+    q, s = moe.quantize_int8(x)
+    most = x.abs().amax(1, keepdim=True).double()
+    assert torch.equal(q.double(), torch.round(127 * x.double() / most))
+    assert torch.equal(s, (most[:, 0] / 127).float())
+    w, ws = moe.quantize_int8(torch.randn(24, 16, generator=g, device="cuda"))
+    y = moe.int8_matmul(x, w, ws, out_dtype=torch.float32)
+    part = slice(rows - 70, rows)
+    ref = (q[part].double() @ w.double().t()) * s[part, None].double() * ws.double()
+    assert ((y[part].double() - ref).abs() <= 3.01 * 2.0**-24 * ref.abs()).all()
+    head = (q[:70].double() @ w.double().t()) * s[:70, None].double() * ws.double()
+    assert ((y[:70].double() - head).abs() <= 3.01 * 2.0**-24 * head.abs()).all()

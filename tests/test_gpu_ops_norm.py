@@ -366,3 +366,32 @@ def test_bf16_stream_is_formed_closer_than_in_fp32(moe):
     off = np.linalg.norm(_f64(h) - ref) / np.linalg.norm(ref)
     off32 = np.linalg.norm(P * _rstd(P, True) * _f64(a["pre_weight"]) - ref) / np.linalg.norm(ref)
     assert off <= 0.7 * off32, (off, off32)
+
+
+@pytest.mark.parametrize("T,D", [(2**21 + 5, 8), (2**22 + 2**20 + 3, 16), (2**20 + 7, 520)])
+def test_millions_of_rows(moe, T, D):
+    # more rows than one dimension of a launch takes; compared with the same rows in
+    # parts, a part at the end in float64
+    print(f"norm rows T={T} D={D}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(T)
+    new = lambda r: torch.randn(r, D, generator=g, device="cuda").to(torch.bfloat16)
+    x, y, gate, pre = new(T), new(T), new(1), new(1)[0].float()
+    kw = dict(pre_weight=pre, post_weight=pre, gate=gate, alpha=ALPHA, beta=BETA, eps=EPS)
+    r, h, stats = moe.block_norm(x, y, **kw)
+    cut = T // 2 // 4 * 4
+    for s in (slice(0, cut), slice(cut, T)):
+        for got, part in zip((r, h, stats), moe.block_norm(x[s], y[s], **kw)):
+            assert torch.equal(got[s], part)
+    tail = slice(T - 999, T)
+    _check_forward(moe, dict(x=x[tail], y=y[tail], pre_weight=pre, post_weight=pre, gate=gate), "bf16", "bf16")
+    dr, dh = new(T), new(T)
+    dx, dy, dgate, dpost, dpre = moe.block_norm_grad(dr, dh, r, y, stats, **{k: v for k, v in kw.items() if k != "eps"})
+    a = dict(x=x[tail], y=y[tail], pre_weight=pre, post_weight=pre, gate=gate)
+    (wx, wy, *_), (mx, my, *_) = _formula(a, dr[tail], dh[tail], r[tail])
+    for got, ref, mag in ((dx, wx, mx), (dy, wy, my)):
+        assert (np.abs(_f64(got[tail]) - ref) <= 4 * E * mag + HALF["bf16"] * np.abs(ref) + 1e-37).all()
+    # the column sums, in float64 on the GPU: a rounding of fp32 per addition, in
+    # chunks of T / 512 rows at most, whose sums are added in turn
+    rh = r.double() * stats[:, 1:].double()
+    ref, mag = (dh.double() * rh).sum(0), (dh.double() * rh).abs().sum(0)
+    assert ((dpre.double() - ref).abs() <= (T / 512 + 2048) * 2.0**-24 * mag).all()

@@ -248,3 +248,23 @@ def test_python_refuses_no_columns_and_results_in_place(moe):
     for out in (x, w):
         with pytest.raises(moe.MoeError, match="overlap"):
             moe.grouped_matmul(x, w, out=out)
+
+
+def test_rows_up_to_2_30(moe):
+    # the limit is the documented one: sizes are checked before the pointers, so the
+    # largest calls get as far as those (null, or one byte off)
+    from mixtureofexperts_amd import _lib
+
+    most, n = 2**30, ctypes.c_int64(-1)
+    _refused(moe, "moe_block_norm_async", {**NORM, "T": most, "x": None}, "null")
+    _refused(moe, "moe_block_norm_async", {**NORM, "T": most + 1, "x": None}, "2^30")
+    _refused(moe, "moe_block_norm_grad_async", {**NORMG, "T": most, "dpost": P + 2}, "aligned")
+    _refused(moe, "moe_block_norm_grad_async", {**NORMG, "T": most + 1, "dpost": P + 2}, "2^30")
+    _refused(moe, "moe_quantize_int8_async", {**QUANT, "rows": most, "x": None}, "null")
+    _refused(moe, "moe_quantize_int8_async", {**QUANT, "rows": most + 1, "x": None}, "2^30")
+    _refused(moe, "moe_int8_matmul_async", {**INT8MM, "rows": most, "x": P + 1}, "aligned")
+    L = _lib.lib()
+    assert L.moe_block_norm_grad_workspace(most, 64, 1, ctypes.byref(n)) == 0 and 0 < n.value < 2**32
+    assert L.moe_block_norm_grad_workspace(most + 1, 64, 1, ctypes.byref(n)) == _lib.MOE_EINVAL
+    assert L.moe_int8_matmul_workspace(8, most, 64, 32, BF16, ctypes.byref(n)) == 0
+    assert n.value >= 4 * most + 64 * most  # scales and codes, past 32 bits
