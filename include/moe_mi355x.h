@@ -409,7 +409,9 @@ int moe_read_counts(moe_handle *h, int32_t *counts);
  * held within [0, rows] by the kernels; with offsets that decrease the results
  * are undefined.  A group may be empty; rows outside every group are not
  * written and their values have no effect.  offsets may be NULL with groups =
- * 1: all rows.  rows = 0 is no work.  A result must not overlap an operand.
+ * 1: all rows.  rows = 0 is no work.  A result must not overlap an
+ * operand, which the products and the quantiser refuse; both may be columns of
+ * one buffer.
  *
  * Sizes and numbers of rows, of the norms and the quantiser too, go up to 2^30.
  * A product runs in one launch of at most 8 million workgroups (2^31 threads),

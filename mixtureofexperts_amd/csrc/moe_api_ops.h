@@ -2,6 +2,7 @@
 // device tensors: argument checks, then one launcher call.  Included by
 // moe_api.hip only (it uses that file's fail()).
 #pragma once
+#include <initializer_list>
 #include <mutex>
 
 #include "moe_ops.h"
@@ -55,6 +56,56 @@ int op_check_workspace(const char *fn, int64_t need, const void *workspace, int6
         return op_fail(fn, "the workspace must be 16-byte aligned and hold " + std::to_string(need) + " bytes");
     return MOE_OK;
 }
+// The bytes that a tensor of `mats` matrices covers: rows of `width` bytes, ld apart.
+struct OpRegion {
+    int64_t at, width, ld, rows, stride, mats;
+    OpRegion(const void *p, int64_t cols, int64_t ld_, int64_t rows_, int64_t stride_, int64_t mats_, int64_t es)
+        : at((int64_t)(uintptr_t)p), width(cols * es), ld(ld_ * es), rows(rows_), stride(stride_ * es), mats(mats_) {
+        if (rows == 1 || ld == width) width += (rows - 1) * ld, rows = 1, ld = width;  // one piece
+        if (rows == 1 && (mats == 1 || stride == width)) width += (mats - 1) * stride, ld = width, mats = 1;
+        if (!p) mats = 0;
+    }
+    OpRegion(const void *p, int64_t bytes) : OpRegion(p, bytes, bytes, 1, 0, 1, 1) {}
+    int64_t end() const { return at + (mats - 1) * stride + (rows - 1) * ld + width; }
+};
+// Whether two matrices (a's ma-th, b's mb-th) share a byte.
+bool op_matrices_meet(const OpRegion &a, int64_t ma, const OpRegion &b, int64_t mb) {
+    const int64_t pa = a.at + ma * a.stride, pb = b.at + mb * b.stride;
+    auto below = [](int64_t x, int64_t d) { return x >= 0 ? x / d : -((-x + d - 1) / d); };  // floor
+    if (a.rows == 1 || b.rows == 1 || a.ld == b.ld) {
+        // row i of a and row j of b meet where pb - a.width < pa + (i - j) ld < pb + b.width
+        const int64_t ld = a.rows > 1 ? a.ld : b.ld;
+        const int64_t lo = std::max(below(pb - a.width - pa, ld) + 1, -(b.rows - 1));
+        const int64_t hi = std::min(below(pb + b.width - pa - 1, ld), a.rows - 1);
+        return lo <= hi;
+    }
+    // rows of different strides: from one to the next that ends past the other's
+    // start.  (So many of them that are interleaved are taken as apart.)
+    auto next = [&](int64_t p, const OpRegion &r, int64_t x) { return std::max<int64_t>(0, below(x - p - r.width, r.ld) + 1); };
+    int64_t i = 0, j = 0;
+    for (int step = 0; step < 1 << 16; ++step) {
+        i = next(pa, a, pb + j * b.ld);
+        if (i >= a.rows) return false;
+        if (pa + i * a.ld < pb + j * b.ld + b.width) return true;
+        j = next(pb, b, pa + i * a.ld);
+        if (j >= b.rows) return false;
+        if (pb + j * b.ld < pa + i * a.ld + a.width) return true;
+    }
+    return false;
+}
+bool op_overlap(const OpRegion &a, const OpRegion &b) {
+    if (a.mats < 1 || b.mats < 1 || a.end() <= b.at || b.end() <= a.at) return false;
+    for (int64_t i = 0; i < a.mats; ++i)
+        for (int64_t j = 0; j < b.mats; ++j)
+            if (op_matrices_meet(a, i, b, j)) return true;
+    return false;
+}
+int op_check_overlap(const char *fn, const OpRegion &result, std::initializer_list<OpRegion> operands) {
+    for (const OpRegion &o : operands)
+        if (op_overlap(result, o)) return op_fail(fn, "the result must not overlap an operand");
+    return MOE_OK;
+}
+constexpr int64_t op_bytes(int32_t dtype) { return dtype == MOE_F32 ? 4 : (dtype == MOE_BF16 ? 2 : 1); }
 bool op_misaligned(const void *p, int32_t dtype) { return ((uintptr_t)p & (dtype == MOE_F32 ? 3 : 1)) != 0; }
 
 // y[r] = W_e x[r] (grad: dx[r] = W_e^T dy[r]) on rows of k elements -> n
@@ -87,7 +138,11 @@ int op_rows_product(const char *fn, bool grad, const void *x, int64_t ldx, const
     g.ws = (float *)workspace;
     r = op_check_workspace(fn, g.splits > 1 ? (int64_t)4 * g.splits * rows * n : 0, workspace, workspace_bytes);
     if (r != MOE_OK) return r;
-    if (y == x || y == w) return op_fail(fn, "the result must not overlap an operand");
+    const int64_t es = op_bytes(dtype);
+    r = op_check_overlap(fn, OpRegion(y, n, ldy, rows, 0, 1, op_bytes(y_dtype)),
+                         {OpRegion(x, k, ldx, rows, 0, 1, es), OpRegion(w, wcols, ldw, wrows, w_stride, groups, es),
+                          OpRegion(offsets, 4 * ((int64_t)groups + 1))});
+    if (r != MOE_OK) return r;
     return op_done(fn, dtype == MOE_F32 ? launch_op_gemm_f32(false, b_col, false, g, op_cus(), (hipStream_t)stream)
                                         : launch_op_gemm_bf16(false, b_col, false, g, op_cus(), (hipStream_t)stream));
 }
@@ -165,7 +220,13 @@ int moe_grouped_matmul_grad_w_async(const void *x, int64_t ldx, const void *dy, 
     if (r != MOE_OK) return r;
     r = op_check_workspace(fn, need, workspace, workspace_bytes);
     if (r != MOE_OK) return r;
-    if (dw == x || dw == dy) return op_fail(fn, "the result must not overlap an operand");
+    if (rows > 0) {
+        const int64_t es = op_bytes(dtype);
+        r = op_check_overlap(fn, OpRegion(dw, n, lddw, m, dw_stride, groups, op_bytes(dw_dtype)),
+                             {OpRegion(x, in_dim, ldx, rows, 0, 1, es), OpRegion(dy, out_dim, lddy, rows, 0, 1, es),
+                              OpRegion(offsets, 4 * ((int64_t)groups + 1))});
+        if (r != MOE_OK) return r;
+    }
     OpGemmArgs g{};
     g.A = flux ? x : dy, g.B = flux ? dy : x, g.C = dw;
     g.lda = flux ? ldx : lddy, g.ldb = flux ? lddy : ldx, g.ldc = lddw;
@@ -190,6 +251,10 @@ int moe_quantize_int8_async(const void *x, int64_t ldx, int32_t x_dtype, int64_t
     if (!x || !q || !scale) return op_fail(fn, "null buffer");
     if (op_misaligned(x, x_dtype) || op_misaligned(scale, MOE_F32))
         return op_fail(fn, "a buffer is not aligned to its elements");
+    const OpRegion from(x, cols, ldx, rows, 0, 1, op_bytes(x_dtype)), codes(q, cols, ldq, rows, 0, 1, 1), scales(scale, 4 * rows);
+    int r = op_check_overlap(fn, codes, {from, scales});
+    if (r == MOE_OK) r = op_check_overlap(fn, scales, {from});
+    if (r != MOE_OK) return r;
     return op_done(fn, launch_quantize_i8(x, ldx, x_dtype == MOE_BF16, rows, cols, (int8_t *)q, ldq, cols, scale,
                                           (hipStream_t)stream));
 }
@@ -236,7 +301,11 @@ int moe_int8_matmul_async(const void *x, int64_t ldx, int32_t x_dtype, const flo
     r = moe_int8_matmul_workspace(groups, rows, in_dim, out_dim, x_dtype, &need);
     if (r == MOE_OK) r = op_check_workspace(fn, need, workspace, workspace_bytes);
     if (r != MOE_OK) return r;
-    if (y == x || y == w) return op_fail(fn, "the result must not overlap an operand");
+    r = op_check_overlap(fn, OpRegion(y, out_dim, ldy, rows, 0, 1, op_bytes(y_dtype)),
+                         {OpRegion(x, in_dim, ldx, rows, 0, 1, op_bytes(x_dtype)),
+                          OpRegion(w, in_dim, ldw, out_dim, w_stride, groups, 1), OpRegion(codes ? x_scale : nullptr, 4 * (int64_t)rows),
+                          OpRegion(w_scale, 4 * (int64_t)groups * out_dim), OpRegion(offsets, 4 * ((int64_t)groups + 1))});
+    if (r != MOE_OK) return r;
     if (!codes) {
         float *sx = (float *)((uint8_t *)workspace + int8_partial_bytes(groups, rows, in_dim, out_dim));
         int8_t *q = (int8_t *)sx + round_up((int64_t)rows * 4, 16);

@@ -20,7 +20,8 @@ outside every group are not written and have no effect.  ``None``: one expert, a
 rows.  Weights are (E, out, in) with ``layout=MOE_LAYOUT_LLAMA_IN_OUT`` (the
 default) and (E, in, out) with ``MOE_LAYOUT_FLUX_OUT_IN``; one expert's may be
 2-D.  Rows may be strided (contiguous within a row); 16-byte aligned rows are
-read faster.  A result must not overlap an operand.
+read faster.  A result that shares an element with an operand is refused; both
+may be columns of one buffer.
 
 Sizes and rows go up to 2^30.  A product is one launch of at most 8 million
 workgroups, each with 64 x 64 results or more (few rows per group: 16 columns

@@ -268,3 +268,65 @@ def test_rows_up_to_2_30(moe):
     assert L.moe_block_norm_grad_workspace(most + 1, 64, 1, ctypes.byref(n)) == _lib.MOE_EINVAL
     assert L.moe_int8_matmul_workspace(8, most, 64, 32, BF16, ctypes.byref(n)) == 0
     assert n.value >= 4 * most + 64 * most  # scales and codes, past 32 bits
+
+
+def test_a_result_that_reaches_into_an_operand_is_refused(moe):
+    # sizes in elements: x 10 rows of 64, w 4 matrices of 32 x 64, y 10 rows of 32
+    ws = dict(workspace=64 * P, workspace_bytes=2**30)
+    at = dict(x=P, w=4 * P, offsets=16 * P)
+    bf16 = 2
+    inside = [P + 64 * bf16, P + 9 * 64 * bf16, P - 32 * bf16 * 10 + bf16,      # within x, its last row, its first element
+              4 * P + 3 * 64 * 32 * bf16 + 62, 4 * P - bf16 * 320 + bf16,        # w's last matrix, its first element
+              16 * P + 16, 16 * P - 2 * 320 + 2]                                 # the offsets
+    for y in inside:
+        _refused(moe, "moe_grouped_matmul_async", {**ROWS, **at, **ws, "y": y}, "overlap")
+        _refused(moe, "moe_int8_matmul_async",
+                 {**INT8MM, **at, **ws, "x_dtype": INT8, "x_scale": 20 * P, "w_scale": 24 * P, "ldx": 128, "ldw": 128,
+                  "in_dim": 128, "w_stride": 128 * 32, "y": y}, "overlap")
+    for y in (20 * P + 4 * 9, 24 * P + 4 * 127, 24 * P - 320 * bf16 + 2):        # the scales
+        _refused(moe, "moe_int8_matmul_async",
+                 {**INT8MM, **at, **ws, "x_dtype": INT8, "x_scale": 20 * P, "w_scale": 24 * P, "y": y}, "overlap")
+    # columns of one buffer of 96: y's last element is x's first, or x's last y's first
+    one = dict(ldx=96, ldy=96)
+    for x, y in ((P + 31 * bf16, P), (P, P + 63 * bf16), (P, P + 95 * bf16)):  # (the last wraps into the next row)
+        _refused(moe, "moe_grouped_matmul_async", {**ROWS, **at, **ws, **one, "x": x, "y": y}, "overlap")
+    # rows of different strides: the fourth of y meets the second of x
+    _refused(moe, "moe_grouped_matmul_async", {**ROWS, **at, **ws, "ldx": 1000, "ldy": 300, "y": P + 70 * bf16}, "overlap")
+    grad = dict(x=P, dy=4 * P, offsets=16 * P)
+    for dw in (P + 4, 4 * P + 10 * 32 * bf16 - 4, 16 * P + 16, P - 4 * 64 * 32 * 4 + 4):
+        _refused(moe, "moe_grouped_matmul_grad_w_async", {**GRADW, **grad, **ws, "dw": dw}, "overlap")
+    quant = dict(x=P, q=4 * P, scale=8 * P)
+    for bad in (dict(q=P + 511), dict(q=P - 255), dict(scale=P + 508), dict(scale=4 * P + 252), dict(scale=4 * P - 12)):
+        _refused(moe, "moe_quantize_int8_async", {**QUANT, **quant, **bad}, "overlap")
+
+
+@pytest.mark.gpu
+def test_columns_of_one_buffer_are_taken(moe):
+    torch = pytest.importorskip("torch")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    off = torch.tensor([0, 40, 40, 100], dtype=torch.int32, device="cuda")
+    w = torch.randn(3, 32, 64, generator=g, device="cuda")
+    buf = torch.randn(100, 64 + 32 + 3, generator=g, device="cuda")
+    for x, y in ((buf[:, :64], buf[:, 64:96]), (buf[:, 35:], buf[:, 2:34])):
+        want = moe.grouped_matmul(x.contiguous(), w, off)
+        keep = x.clone()
+        assert torch.equal(moe.grouped_matmul(x, w, off, out=y), want) and torch.equal(x, keep)
+    # the weights' gradient beside the weights, the rows in every other row of a buffer
+    both = torch.randn(3, 32, 128, generator=g, device="cuda")
+    x, dy = torch.randn(200, 64, generator=g, device="cuda"), torch.randn(100, 32, generator=g, device="cuda")
+    want = moe.grouped_matmul_grad_w(x[::2].contiguous(), dy, off)
+    keep = both[:, :, :64].clone()
+    assert torch.equal(moe.grouped_matmul_grad_w(x[::2], dy, off, out=both[:, :, 64:]), want)
+    assert torch.equal(both[:, :, :64], keep)
+    want = moe.grouped_matmul_grad_x(dy, both[:, :, :64], off)
+    assert torch.equal(moe.grouped_matmul_grad_x(dy, both[:, :, :64], off, out=x[1::2]), want)
+    # rows of different strides that pass each other
+    flat = torch.zeros(100 * 200 + 64, device="cuda")
+    x = flat.as_strided((50, 64), (400, 1))
+    x.copy_(torch.randn(50, 64, generator=g, device="cuda"))
+    y = flat.as_strided((50, 32), (200, 1), 64)
+    want = moe.grouped_matmul(x.contiguous(), w[0])
+    assert torch.equal(moe.grouped_matmul(x, w[0], out=y), want)
+    for x, y in ((x, flat.as_strided((50, 32), (200, 1), 63)), (buf[:50, :64], buf[:50, 63:95])):
+        with pytest.raises(moe.MoeError, match="overlap"):
+            moe.grouped_matmul(x, w[0], out=y)
