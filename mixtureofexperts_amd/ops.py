@@ -59,14 +59,14 @@ def _plain(names, *tensors):
     arguments', as one string."""
     torch = _torch or _t()
     if torch.is_grad_enabled():
-        for i, t in enumerate(tensors):
+        for t in tensors:
             if t is not None and getattr(t, "requires_grad", False):
-                _bad(f"{names.split()[i]} requires a gradient, which this call does not record: use torch.no_grad() or "
-                     "detach it")
+                name = names.split()[[t is u for u in tensors].index(True)]
+                _bad(f"{name} requires a gradient, which this call does not record: use torch.no_grad() or detach it")
     if _forward_ad._current_level >= 0:  # within a forward_ad.dual_level()
-        for i, t in enumerate(tensors):
+        for name, t in zip(names.split(), tensors):
             if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
-                _bad(f"{names.split()[i]} carries a tangent, which this call does not propagate")
+                _bad(f"{name} carries a tangent, which this call does not propagate")
 
 
 def _tensor(t, name, dtypes, dims):
@@ -82,8 +82,8 @@ def _tensor(t, name, dtypes, dims):
 def _row_stride(t, name):
     """Elements between the rows of t's last two dimensions."""
     rows, cols = t.shape[-2:]
-    ld = t.stride(-2)
-    if cols > 1 and t.stride(-1) != 1:
+    ld, one = t.stride()[-2:]
+    if one != 1 and cols > 1:
         _bad(f"{name}: a row's elements must be contiguous")
     if ld < cols:
         if rows > 1:
@@ -199,8 +199,8 @@ def _float_types(dtype):
     return (dtype,) if dtype == _torch.float32 else _floats
 
 
-def _rows_product(fn, x, name, w, offsets, layout, out, out_dtype, grad):
-    _plain(name + " w out", x, w, out)
+def _rows_product(fn, x, name, names, w, offsets, layout, out, out_dtype, grad):
+    _plain(names, x, w, out)
     xp, ldx = _rows(x, name, _floats)
     E, a, b, ldw, stride = _matrices(w, "w", (x.dtype,))
     in_dim, out_dim = (a, b) if _layout(layout) else (b, a)
@@ -225,13 +225,14 @@ def grouped_matmul(x, w, offsets=None, *, layout=MOE_LAYOUT_LLAMA_IN_OUT, out=No
     bfloat16, w of the same type; sums in float32, the result in x's type or,
     for bfloat16, ``out_dtype=torch.float32``.  Without ``out`` rows outside
     every group are zeros."""
-    return _rows_product(_lib.lib().moe_grouped_matmul_async, x, "x", w, offsets, layout, out, out_dtype, False)
+    return _rows_product(_lib.lib().moe_grouped_matmul_async, x, "x", "x w out", w, offsets, layout, out, out_dtype,
+                         False)
 
 
 def grouped_matmul_grad_x(dy, w, offsets=None, *, layout=MOE_LAYOUT_LLAMA_IN_OUT, out=None, out_dtype=None):
     """The gradient of grouped_matmul with respect to x: dx[r] = W_e' dy[r]."""
-    return _rows_product(_lib.lib().moe_grouped_matmul_grad_x_async, dy, "dy", w, offsets, layout, out, out_dtype,
-                         True)
+    return _rows_product(_lib.lib().moe_grouped_matmul_grad_x_async, dy, "dy", "dy w out", w, offsets, layout, out,
+                         out_dtype, True)
 
 
 def grouped_matmul_grad_w(x, dy, offsets=None, *, layout=MOE_LAYOUT_LLAMA_IN_OUT, out=None, out_dtype=None,
