@@ -26,7 +26,7 @@ int op_cus() {
 int op_fail(const char *fn, const std::string &why) { return fail(nullptr, MOE_EINVAL, std::string(fn) + ": " + why); }
 int op_done(const char *fn, hipError_t e) {
     if (e == hipSuccess) return MOE_OK;
-    if (e == hipErrorInvalidValue) return op_fail(fn, "too many tiles for one launch");
+    if (e == kOpTooLarge) return op_fail(fn, "too many tiles for one launch");
     return fail(nullptr, MOE_EHIP, std::string(fn) + ": " + hipGetErrorString(e));
 }
 
@@ -143,8 +143,8 @@ int op_rows_product(const char *fn, bool grad, const void *x, int64_t ldx, const
                          {OpRegion(x, k, ldx, rows, 0, 1, es), OpRegion(w, wcols, ldw, wrows, w_stride, groups, es),
                           OpRegion(offsets, 4 * ((int64_t)groups + 1))});
     if (r != MOE_OK) return r;
-    return op_done(fn, dtype == MOE_F32 ? launch_op_gemm_f32(false, b_col, false, g, op_cus(), (hipStream_t)stream)
-                                        : launch_op_gemm_bf16(false, b_col, false, g, op_cus(), (hipStream_t)stream));
+    return op_done(fn, dtype == MOE_F32 ? launch_op_gemm_f32(b_col, false, g, op_cus(), (hipStream_t)stream)
+                                        : launch_op_gemm_bf16(b_col, false, g, op_cus(), (hipStream_t)stream));
 }
 }  // namespace
 
@@ -235,8 +235,8 @@ int moe_grouped_matmul_grad_w_async(const void *x, int64_t ldx, const void *dy, 
     g.M = m, g.N = n, g.c_f32 = dw_dtype == MOE_F32, g.accumulate = accumulate != 0;
     g.splits = op_matrix_splits(rows, groups, m, n, op_cus());
     g.ws = (float *)workspace;
-    return op_done(fn, dtype == MOE_F32 ? launch_op_gemm_f32(true, true, true, g, op_cus(), (hipStream_t)stream)
-                                        : launch_op_gemm_bf16(true, true, true, g, op_cus(), (hipStream_t)stream));
+    return op_done(fn, dtype == MOE_F32 ? launch_op_gemm_f32(true, true, g, op_cus(), (hipStream_t)stream)
+                                        : launch_op_gemm_bf16(true, true, g, op_cus(), (hipStream_t)stream));
 }
 
 int moe_quantize_int8_async(const void *x, int64_t ldx, int32_t x_dtype, int64_t rows, int32_t cols, void *q,

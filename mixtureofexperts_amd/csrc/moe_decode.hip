@@ -572,7 +572,7 @@ hipError_t launch_op_stream(int ot, const OpGemmArgs &g0, hipStream_t s) {
     OpGemmArgs g = g0;
     g.nt = (g.N + 15) / 16;
     const long long grid = (long long)(g.E < g.rows ? g.E : g.rows) * g.nt;  // the groups that can hold rows
-    if (grid * g.splits > 0x7fffffffll / (ops::kStreamWaves * 64)) return hipErrorInvalidValue;
+    if (grid * g.splits > 0x7fffffffll / (ops::kStreamWaves * 64)) return kOpTooLarge;
     const dim3 gr((unsigned)grid, g.splits), b(ops::kStreamWaves * 64);
     if (ot == OT_F32) ops::op_stream_kernel<OT_F32><<<gr, b, 0, s>>>(g);
     else if (ot == OT_BF16) ops::op_stream_kernel<OT_BF16><<<gr, b, 0, s>>>(g);
@@ -584,7 +584,7 @@ hipError_t launch_op_stream(int ot, const OpGemmArgs &g0, hipStream_t s) {
 hipError_t launch_op_fold(int ot, bool ragged_k, const OpGemmArgs &g, hipStream_t s) {
     const long long n = ragged_k ? (long long)g.E * g.M * g.N : (long long)g.rows * g.N;
     const long long blocks = (n + 255) / 256;
-    if (blocks > 0x7fffffffll / 256) return hipErrorInvalidValue;
+    if (blocks > 0x7fffffffll / 256) return kOpTooLarge;
     if (ot == OT_I8) ops::op_fold_kernel<OT_I8, false><<<(unsigned)blocks, 256, 0, s>>>(g);
     else if (ragged_k) ops::op_fold_kernel<OT_BF16, true><<<(unsigned)blocks, 256, 0, s>>>(g);
     else ops::op_fold_kernel<OT_BF16, false><<<(unsigned)blocks, 256, 0, s>>>(g);

@@ -84,9 +84,13 @@ inline int op_matrix_splits(long long rows, long long E, long long M, long long 
     return op_splits(E * ((M + 63) / 64) * ((N + 63) / 64), rows / E, 512, ncu);
 }
 
-// a_col / b_col as above; the launchers pick tile and load form (op_gemm_plan)
-hipError_t launch_op_gemm_f32(bool a_col, bool b_col, bool ragged_k, OpGemmArgs g, int ncu, hipStream_t s);
-hipError_t launch_op_gemm_bf16(bool a_col, bool b_col, bool ragged_k, OpGemmArgs g, int ncu, hipStream_t s);
+// What a launcher answers to a call of more workgroups than one launch takes.
+constexpr hipError_t kOpTooLarge = hipErrorNotSupported;
+
+// b_col as above (ragged k: both operands are); the launchers pick tile and load
+// form (op_gemm_plan)
+hipError_t launch_op_gemm_f32(bool b_col, bool ragged_k, OpGemmArgs g, int ncu, hipStream_t s);
+hipError_t launch_op_gemm_bf16(bool b_col, bool ragged_k, OpGemmArgs g, int ncu, hipStream_t s);
 hipError_t launch_op_gemm_i8(OpGemmArgs g, int ncu, hipStream_t s);
 // few rows per group, both operands "row": the weights streamed once
 hipError_t launch_op_stream(int ot, const OpGemmArgs &g, hipStream_t s);

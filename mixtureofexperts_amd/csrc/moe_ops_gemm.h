@@ -932,7 +932,7 @@ hipError_t launch_tiles(OpGemmArgs g, int vb, hipStream_t s) {
     const long long mtiles = (long long)(g.rows / BM) + (g.E < g.rows ? g.E : g.rows);
     const long long grid =
         RAGK ? ((long long)g.mt * g.nt * g.splits + 7) / 8 * 8 * g.E : (mtiles * g.nt * g.splits + 7) / 8 * 8;
-    if (grid > 0x7fffffffll / (WM * WN * 64)) return hipErrorInvalidValue;
+    if (grid > 0x7fffffffll / (WM * WN * 64)) return kOpTooLarge;
     const dim3 b(WM * WN * 64);
     // (bf16 pairs by dwords: the registers of three waves per SIMD are too few)
     constexpr int W4 = WPE == 3 && BM == 128 && OT == OT_BF16 ? 2 : WPE;

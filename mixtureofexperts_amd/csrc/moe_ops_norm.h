@@ -550,7 +550,6 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_grad_kernel(
 
 // Adds the chunks' sums in a fixed order: 64 columns per workgroup, 16 slices
 // of the chunks.  blockIdx.y: 0 dpre, 1 dpost, 2 + g gate row g.
-template <int DUMMY>
 __global__ __launch_bounds__(1024) void norm_fold_kernel(NormArgs a) {
     __shared__ float part[16][64];
     const int what = blockIdx.y;
@@ -691,8 +690,8 @@ hipError_t launch_block_norm_grad(NormArgs a, hipStream_t s) {
     }
     const long long gates = a.dgate && a.cpg > 0 ? (a.T + a.gate_rows - 1) / a.gate_rows : 0;
     if (!a.dpre && !a.dpost && gates == 0) return hipSuccess;
-    if (gates > 65000) return hipErrorInvalidValue;
-    ops::norm_fold_kernel<0><<<dim3((a.D + 63) / 64, (unsigned)(2 + gates)), 1024, 0, s>>>(a);
+    if (gates > 65000) return kOpTooLarge;  // (a few thousand at most: norm_chunks)
+    ops::norm_fold_kernel<<<dim3((a.D + 63) / 64, (unsigned)(2 + gates)), 1024, 0, s>>>(a);
     return hipGetLastError();
 }
 

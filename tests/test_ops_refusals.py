@@ -330,3 +330,14 @@ def test_columns_of_one_buffer_are_taken(moe):
     for x, y in ((x, flat.as_strided((50, 32), (200, 1), 63)), (buf[:50, :64], buf[:50, 63:95])):
         with pytest.raises(moe.MoeError, match="overlap"):
             moe.grouped_matmul(x, w[0], out=y)
+
+
+def test_more_tiles_than_a_launch_are_refused(moe):
+    # the documented limit: no more than 8 million workgroups
+    far = dict(x=2**44, w=2**45, offsets=2**46, y=2**56)
+    many = dict(rows=2**30, out_dim=2**20, ldy=2**20, w_stride=2**26)
+    _refused(moe, "moe_grouped_matmul_async", {**ROWS, **far, **many}, "too many tiles")
+    _refused(moe, "moe_grouped_matmul_grad_w_async",
+             {**GRADW, "x": 2**44, "dy": 2**45, "offsets": 2**46, "dw": 2**56, "groups": 2**24, "rows": 2**24}, "too many tiles")
+    _refused(moe, "moe_int8_matmul_async",
+             {**INT8MM, **far, **many, "x_dtype": INT8, "x_scale": 2**43, "w_scale": 2**42, "w_stride": 2**26}, "too many tiles")
