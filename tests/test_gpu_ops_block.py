@@ -249,3 +249,36 @@ def test_block_forward_refuses_too_many_tokens(moe):
     with pytest.raises(moe.MoeError, match="GPU memory"):
         moe.moe_block_forward(layer, torch.ones(8, 32), pre_weight=pre)
     layer.close()
+
+
+@pytest.mark.parametrize("T", [1, 7, 150])
+def test_int8_serving_to_the_end(moe, T):
+    # the same block's last steps: the experts' rows gathered by token, the norm of
+    # their sum with the residual, and the norm of the stream
+    print(f"block int8 serving to the end T={T}", flush=True)
+    p = _problem(torch.bfloat16, 3, T=150)
+    keep = p["token"] < T
+    off = p["offsets"].tolist()
+    offsets = np.concatenate([[0], np.cumsum([int(keep[off[e]:off[e + 1]].sum()) for e in range(6)])]).tolist()
+    token, weight = p["token"][keep], p["weight"][keep]
+    d = {n: t.cuda() for n, t in p.items()}
+    x = d["x"][:T].contiguous()
+    w2, s2 = moe.quantize_int8(d["w2"])
+    rng = np.random.default_rng(T)
+    act = torch.from_numpy(rng.standard_normal((len(token), 256))).to(torch.bfloat16).cuda()
+    yr = moe.int8_matmul(act, w2, s2, torch.tensor(offsets, dtype=torch.int32, device="cuda"), out_dtype=torch.float32)
+    y = torch.zeros(T, yr.shape[1], device="cuda").index_add(0, token.cuda(), yr * weight.cuda()[:, None])
+    r, n, _ = moe.block_norm(x, y, pre_weight=d["nxt"], post_weight=d["post"])
+    # float64 on the CPU, from the codes' values
+    q, s = (t.cpu().double() for t in moe.quantize_int8(act))
+    wq, ws = w2.cpu().double(), s2.cpu().double()
+    o = offsets
+    rows = torch.cat([(q[o[e]:o[e + 1]] @ wq[e].t()) * s[o[e]:o[e + 1], None] * ws[e] for e in range(6)])
+    Y = torch.zeros(T, rows.shape[1], dtype=torch.float64).index_add(0, token, rows * weight.double()[:, None])
+    rms = lambda v: v * torch.rsqrt((v * v).mean(1, keepdim=True) + 1e-5)
+    X, Z = p["x"][:T].double(), rms(Y) * p["post"].double()
+    # r: fp32 steps (1e-5 of the terms, which may cancel), then one rounding to bf16;
+    # n: the norm of r as it is stored, the same
+    assert ((r.cpu().double() - (X + Z)).abs() <= 2.0**-8 * (X + Z).abs() + 1e-5 * (X.abs() + Z.abs())).all()
+    N = rms(r.cpu().double()) * p["nxt"].double()
+    assert ((n.cpu().double() - N).abs() <= (2.0**-8 + 1e-5) * N.abs()).all()

@@ -417,3 +417,15 @@ def test_two_streams_at_once(moe):
     torch.cuda.synchronize()
     for i, res in got:
         assert all(torch.equal(a, b) for a, b in zip(res, want[i])), i
+
+
+@pytest.mark.parametrize("layout", [LLAMA, FLUX])
+def test_weight_gradient_of_two_rounds_of_large_tiles(moe, layout):
+    # four groups of 8 x 16 tiles of 256 x 256: as many as take that size
+    rng = np.random.default_rng(19)
+    lens, K, N = [70, 0, 133, 9], 4096, 2040
+    x, dy = _rows(rng, 212, K, "bf16", 0), _rows(rng, 212, N, "bf16", 0)
+    dw = moe.grouped_matmul_grad_w(x, dy, _offsets(lens), layout=layout, out_dtype=torch.float32)
+    a, b = (_f64(dy), _f64(x)) if layout == LLAMA else (_f64(x), _f64(dy))
+    for e, s in enumerate((slice(0, 70), slice(70, 70), slice(70, 203), slice(203, 212))):
+        _close(_f64(dw[e]), a[s].T @ b[s], np.abs(a[s]).T @ np.abs(b[s]), max(lens[e], 1), "f32")
