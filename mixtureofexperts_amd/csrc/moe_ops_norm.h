@@ -23,8 +23,10 @@ struct Row8 {
 struct Raw8 {
     unsigned u[8];
 };
-// channels from c of a row; those past D read as 0
-template <bool VEC>
+// channels from c of a row; those past D read as 0.  ANY (without VEC): whole vectors
+// by loads that need not be aligned, all but a row's last (8190 x 4092, bf16: the norm
+// 77 us, by elements 262; the gradient's largest form has no registers left for it).
+template <bool VEC, bool ANY = false>
 __device__ __forceinline__ Raw8 load_raw(const void *p, int bf16, long long row, int c, int D) {
     Raw8 o{};
     if (bf16) {
@@ -34,6 +36,11 @@ __device__ __forceinline__ Raw8 load_raw(const void *p, int bf16, long long row,
                 const uint4 w = *(const uint4 *)q;
                 o.u[0] = w.x, o.u[1] = w.y, o.u[2] = w.z, o.u[3] = w.w;
             }
+        } else if (ANY && c + 8 <= D) {
+            unsigned w[4];
+            __builtin_memcpy(w, q, 16);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o.u[i] = i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16;
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) o.u[i] = c + i < D ? (unsigned)q[i] << 16 : 0u;
@@ -46,6 +53,8 @@ __device__ __forceinline__ Raw8 load_raw(const void *p, int bf16, long long row,
                 o.u[0] = w.x, o.u[1] = w.y, o.u[2] = w.z, o.u[3] = w.w;
                 o.u[4] = x.x, o.u[5] = x.y, o.u[6] = x.z, o.u[7] = x.w;
             }
+        } else if (ANY && c + 8 <= D) {
+            __builtin_memcpy(o.u, q, 32);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) o.u[i] = c + i < D ? q[i] : 0u;
@@ -68,24 +77,27 @@ __device__ __forceinline__ Row8 widen(const Raw8 &r, int bf16) {
     }
     return o;
 }
-template <bool VEC>
+template <bool VEC, bool ANY = false>
 __device__ __forceinline__ Row8 load8(const void *p, int bf16, long long row, int c, int D) {
-    return widen<VEC>(load_raw<VEC>(p, bf16, row, c, D), bf16);
+    return widen<VEC>(load_raw<VEC, ANY>(p, bf16, row, c, D), bf16);
 }
-template <bool VEC>
+__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 v = {(__bf16)a, (__bf16)b};
+    return __builtin_bit_cast(unsigned, v);
+}
+template <bool VEC, bool ANY = false>
 __device__ __forceinline__ void store8(void *p, int bf16, long long row, int c, int D, const Row8 &o) {
     if (c >= D) return;
     if (bf16) {
         uint16_t *q = (uint16_t *)p + row * D + c;
-        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
         unsigned w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bf16x2 b = {(__bf16)o.v[2 * i], (__bf16)o.v[2 * i + 1]};
-            w[i] = __builtin_bit_cast(unsigned, b);
-        }
+        for (int i = 0; i < 4; ++i) w[i] = pack_bf16(o.v[2 * i], o.v[2 * i + 1]);
         if constexpr (VEC) {
             *(uint4 *)q = make_uint4(w[0], w[1], w[2], w[3]);
+        } else if (ANY && c + 8 <= D) {
+            __builtin_memcpy(q, w, 16);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -96,6 +108,8 @@ __device__ __forceinline__ void store8(void *p, int bf16, long long row, int c, 
         if constexpr (VEC) {
             *(float4 *)q = make_float4(o.v[0], o.v[1], o.v[2], o.v[3]);
             *(float4 *)(q + 4) = make_float4(o.v[4], o.v[5], o.v[6], o.v[7]);
+        } else if (ANY && c + 8 <= D) {
+            __builtin_memcpy(q, o.v, 32);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -174,7 +188,6 @@ __device__ __forceinline__ double row_sum_wide(float v, double *part) {
     }
     return d;
 }
-__device__ __forceinline__ float round_to(float v, int bf16) { return bf16 ? bf16_to_f32(f32_to_bf16(v)) : v; }
 
 // WIDE: a bf16 stream that a gate or a post norm is added to.  An r that a few fp32
 // roundings put on the other side of a bf16 border (one in 30000) would be 2^-8 off
@@ -182,10 +195,10 @@ __device__ __forceinline__ float round_to(float v, int bf16) { return bf16 ? bf1
 // type, may not decide r.  So r is always the fp64 formula's value rounded by way of
 // fp32 (one in 290000 on the other side then; 2000 x 4096: an fp32 h off by 2e-6 of its
 // norm, 1.3e-5 by fp32 steps): it is formed in fp32, and again in fp64 where a border
-// lies within what the fp32 steps may be off (about an element in 4000).  They round by
-// 2^-24 of the terms' magnitudes each: rstd and its two products, the gate, beta (or
-// alpha), the sum, and the way by fp32: seven.  8192 x 4096, fp32 y, both norms, a gate:
-// 69 us, 67 all in fp32, 81 all in fp64 (117 registers instead of 70).
+// lies within what the fp32 steps may be off (about an element in 8000).  Each rounds
+// by 2^-24 of its value: y's term at rstd beta, its product with y, the weight and the
+// gate, the sum at the addition and on the way by fp32.  8192 x 4096, fp32 y, both
+// norms, a gate: 67 to 68 us, 67 all in fp32, 81 all in fp64 (117 registers instead of 68).
 template <int TPR, int NV, bool VEC, bool WIDE>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(NormArgs a) {
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
@@ -201,8 +214,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(NormA
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (tid + i * TPR) * 8;
-            rx[i] = load_raw<VEC>(a.x, WIDE ? 1 : a.x_bf16, row, c, D);
-            ry[i] = a.y ? load_raw<VEC>(a.y, a.y_bf16, row, c, D) : Raw8{};
+            rx[i] = load_raw<VEC, true>(a.x, WIDE ? 1 : a.x_bf16, row, c, D);
+            ry[i] = a.y ? load_raw<VEC, true>(a.y, a.y_bf16, row, c, D) : Raw8{};
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -234,25 +247,25 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(NormA
     const long long grow = a.gate ? row / a.gate_rows : 0;
     float s = 0.0f;
     if constexpr (WIDE) {
+        const float f = (float)((double)a.beta * iyw);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (tid + i * TPR) * 8;
-            const Row8 p = a.post ? load8<VEC>(a.post, a.w_bf16, 0, c, D) : Row8{};
-            const Row8 t = a.gate ? load8<VEC>(a.gate, a.gate_bf16, grow, c, D) : Row8{};
+            const Row8 p = a.post ? load8<VEC, true>(a.post, a.w_bf16, 0, c, D) : Row8{};
+            const Row8 t = a.gate ? load8<VEC, true>(a.gate, a.gate_bf16, grow, c, D) : Row8{};
             r[i] = widen<VEC>(rx[i], 1);
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
-                float z = y[i].v[q];
-                if (a.post) z = z * iy * p.v[q];
+                float z = y[i].v[q] * f;
+                if (a.post) z *= p.v[q];
                 if (a.gate) z *= t.v[q];
-                const float ax = a.alpha * r[i].v[q], bz = a.beta * z;
-                float v = ax + bz;
+                float v = __builtin_fmaf(a.alpha, r[i].v[q], z);
                 const float border = __uint_as_float((__float_as_uint(v) & 0xffff0000u) | 0x8000u);
-                if (!(fabsf(v - border) > (fabsf(ax) + fabsf(bz)) * 0x1.c8p-22f)) {
-                    double w = (double)y[i].v[q];
-                    if (a.post) w = w * iyw * (double)p.v[q];
+                if (!(fabsf(v - border) > __builtin_fmaf(fabsf(z), 4.1f * 0x1p-24f, fabsf(v) * (2.1f * 0x1p-24f)))) {
+                    double w = (double)a.beta * iyw * (double)y[i].v[q];
+                    if (a.post) w *= (double)p.v[q];
                     if (a.gate) w *= (double)t.v[q];
-                    v = (float)((double)a.alpha * (double)r[i].v[q] + (double)a.beta * w);
+                    v = (float)((double)a.alpha * (double)r[i].v[q] + w);
                 }
                 r[i].v[q] = v;
             }
@@ -268,12 +281,12 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(NormA
         if (!WIDE && a.y) {
             Row8 z = y[i];
             if (a.post) {
-                const Row8 p = load8<VEC>(a.post, a.w_bf16, 0, c, D);
+                const Row8 p = load8<VEC, true>(a.post, a.w_bf16, 0, c, D);
 #pragma unroll
                 for (int q = 0; q < 8; ++q) z.v[q] = z.v[q] * iy * p.v[q];
             }
             if (a.gate) {
-                const Row8 p = load8<VEC>(a.gate, a.gate_bf16, grow, c, D);
+                const Row8 p = load8<VEC, true>(a.gate, a.gate_bf16, grow, c, D);
 #pragma unroll
                 for (int q = 0; q < 8; ++q) z.v[q] *= p.v[q];
             }
@@ -282,18 +295,22 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(NormA
         }
         // the norm is taken of the residual stream as it is stored, which is what
         // the next block and the gradient read
+        if (WIDE || a.x_bf16) {
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            r[i].v[q] = round_to(r[i].v[q], a.x_bf16);
-            s += r[i].v[q] * r[i].v[q];
+            for (int q = 0; q < 8; q += 2) {
+                const unsigned w = pack_bf16(r[i].v[q], r[i].v[q + 1]);
+                r[i].v[q] = __uint_as_float(w << 16), r[i].v[q + 1] = __uint_as_float(w & 0xffff0000u);
+            }
         }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s += r[i].v[q] * r[i].v[q];
         // h is what the next block reads at once, r waits until that block is done:
         // it leaves the caches to h and to the inputs (8192 x 4096, a bf16 stream and
         // fp32 y: 63 -> 51 us alone; y written, this, h read, y written and the norm of
         // r and y: 245 -> 232; only where r is read at once does it cost: five norms in
         // a row 233 -> 250)
         if (VEC && a.r && a.h) store8_past(a.r, a.x_bf16, row, c, D, r[i]);
-        else if (a.r) store8<VEC>(a.r, a.x_bf16, row, c, D, r[i]);
+        else if (a.r) store8<VEC, true>(a.r, a.x_bf16, row, c, D, r[i]);
     }
     float ir = 1.0f;
     if (a.h) {
@@ -301,10 +318,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(NormA
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (tid + i * TPR) * 8;
-            const Row8 p = load8<VEC>(a.pre, a.w_bf16, 0, c, D);
+            const Row8 p = load8<VEC, true>(a.pre, a.w_bf16, 0, c, D);
 #pragma unroll
             for (int q = 0; q < 8; ++q) r[i].v[q] = r[i].v[q] * ir * p.v[q];
-            store8<VEC>(a.h, a.h_bf16, row, c, D, r[i]);
+            store8<VEC, true>(a.h, a.h_bf16, row, c, D, r[i]);
         }
     }
     if (a.stats && tid == 0) {
