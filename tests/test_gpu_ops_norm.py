@@ -395,3 +395,26 @@ def test_millions_of_rows(moe, T, D):
     rh = r.double() * stats[:, 1:].double()
     ref, mag = (dh.double() * rh).sum(0), (dh.double() * rh).abs().sum(0)
     assert ((dpre.double() - ref).abs() <= (T / 512 + 2048) * 2.0**-24 * mag).all()
+
+
+@pytest.mark.parametrize("T,D", [(800, 1024), (300, 4100), (60, 16384), (900, 331)])
+def test_gated_bf16_stream_to_the_bit(moe, T, D):
+    # without a post norm the formula's fp64 value is exact (bf16 factors), so r has one
+    # right answer, by way of fp32, also where the two terms cancel; and rows of zeros,
+    # infinities, NaN and products past fp32's range on the way
+    print(f"norm gated stream T={T} D={D}", flush=True)
+    rng = np.random.default_rng([T, D, 5])
+    y, gate = _make(rng, (T, D), "bf16"), _make(rng, (T, D), "bf16")
+    z = -(BETA * y.double() * gate.double()) / ALPHA
+    x = torch.where(torch.rand(T, D, device="cuda") < 0.5, z, torch.randn(T, D, device="cuda").double()).to(torch.bfloat16)
+    x[3], y[3], gate[4] = 0, 0, 0
+    x[5, 7], y[6, D - 1], gate[7, 0], y[8, 1] = float("nan"), float("inf"), float("-inf"), float("nan")
+    x[9, 2], y[9, 2] = float("inf"), float("inf")
+    y[10], gate[10] = 2.0**120, 2.0**-120
+    y[11], gate[11] = -(2.0**-130), 2.0**100
+    want = (ALPHA * x.double() + BETA * (y.double() * gate.double())).float().to(torch.bfloat16)
+    for pre, ht in ((None, None), (torch.ones(D, device="cuda"), torch.bfloat16), (torch.ones(D, device="cuda"), torch.float32)):
+        r, h, stats = moe.block_norm(x, y, gate=gate, pre_weight=pre, alpha=ALPHA, beta=BETA, h_dtype=ht)
+        bad = ~((r == want) | (torch.isnan(r) & torch.isnan(want)))
+        assert not bad.any(), bad.nonzero()[:5]
+    assert torch.isnan(want[5, 7]) and torch.isinf(want[6, D - 1]) and torch.isnan(want[9, 2]) == torch.isnan(r[9, 2])
