@@ -172,7 +172,9 @@ int moe_grouped_matmul_grad_w_workspace(int32_t groups, int32_t rows, int32_t in
     if (!bytes) return op_fail(fn, "null bytes");
     int r = op_check_groups(fn, (const int32_t *)bytes, groups, rows, in_dim, out_dim);
     if (r != MOE_OK) return r;
-    const int splits = op_matrix_splits(rows, groups, in_dim, out_dim, op_cus());
+    // enough for either type
+    const int splits = std::max(op_matrix_splits(OT_F32, rows, groups, in_dim, out_dim, op_cus()),
+                                op_matrix_splits(OT_BF16, rows, groups, in_dim, out_dim, op_cus()));
     *bytes = splits > 1 ? (int64_t)4 * splits * groups * in_dim * out_dim : 0;
     return MOE_OK;
 }
@@ -233,7 +235,7 @@ int moe_grouped_matmul_grad_w_async(const void *x, int64_t ldx, const void *dy, 
     g.c_stride = groups > 1 ? dw_stride : 0;
     g.offsets = offsets, g.E = groups, g.rows = rows;
     g.M = m, g.N = n, g.c_f32 = dw_dtype == MOE_F32, g.accumulate = accumulate != 0;
-    g.splits = op_matrix_splits(rows, groups, m, n, op_cus());
+    g.splits = op_matrix_splits(dtype == MOE_F32 ? OT_F32 : OT_BF16, rows, groups, m, n, op_cus());
     g.ws = (float *)workspace;
     return op_done(fn, dtype == MOE_F32 ? launch_op_gemm_f32(true, true, g, op_cus(), (hipStream_t)stream)
                                         : launch_op_gemm_bf16(true, true, g, op_cus(), (hipStream_t)stream));

@@ -54,14 +54,22 @@ inline dim3 op_row_grid(long long blocks) {
 }
 __device__ __forceinline__ long long op_row_block() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }
 
-// Few rows per group and the weights as rows: streamed (moe_ops_stream.h).
-inline bool op_streamed(bool b_col, long long rows, long long E) { return !b_col && rows <= 16 * E; }
+// Few rows per group and the weights as rows: streamed (moe_ops_stream.h), against 64 x
+// 64 tiles of the same product, us.  fp32: up to 16 rows (8 experts of 4096 / 4096, 16
+// rows each: 145 / 178, 24: 168 / 162).  bf16 and int8: up to 8 rows, of weights with 4 KB
+// and more per row (bf16, 4096 / 14336: 1 row 164 / 183, 4 170 / 204, 8 193 / 191, 16 241 /
+// 201; int8 104 / 105, 106 / 122, 109 / 119, 124 / 126; 64 experts of 1408 / 2048, bf16: 1
+// row 53 / 51, 8 89 / 77, int8 36 / 30, 57 / 45; 8 of 2048 / 4096: bf16, 8 rows, 37 / 39, int8 17 / 14).
+inline bool op_streamed(int ot, bool b_col, long long rows, long long E, long long K) {
+    if (b_col) return false;
+    return ot == OT_F32 ? rows <= 16 * E : rows <= 8 * E && K * op_size(ot) >= 4096;
+}
 
 constexpr int kOpMaxSplits = 16;
 // Ranges of k for `tiles` workgroups of a call that could run in `slots`: none
 // where half of those have one, no range shorter than `least` (folding the
-// ranges is a launch of its own, about 4 us: a 64 x 64 tile runs 2 KB of k per
-// row in about 16 us, the streamed form 8 KB in about 10).
+// ranges is a launch of its own, about 4 us: the streamed form runs 8 KB of k in
+// about 10).
 inline int op_splits(long long tiles, long long k, long long least, int slots) {
     if (tiles < 1 || 2 * tiles > slots) return 1;
     long long s = (slots + tiles - 1) / tiles;
@@ -69,19 +77,37 @@ inline int op_splits(long long tiles, long long k, long long least, int slots) {
     if (s > kOpMaxSplits) s = kOpMaxSplits;
     return s > 1 ? (int)s : 1;
 }
-// Ragged rows: by 64 x 64 tiles, or the streamed products' 16 columns.
-inline int op_rows_splits(int ot, bool b_col, long long rows, long long E, long long N, long long K, int ncu) {
-    const long long held = E < rows ? E : rows;  // groups that may hold rows
-    if (op_streamed(b_col, rows, E)) return op_splits(held * ((N + 15) / 16), K * op_size(ot), 8192, ncu);
-    const long long mt = (rows + 63) / 64;
-    // a few rows per group read the weights as fast as loads are in flight: four
-    // 64 x 64 tiles per CU (4 rows of 3991 on 4 experts of 4970 columns, fp32: 114 us at one)
-    const int slots = rows <= 16 * E ? 4 * ncu : ncu;
-    return op_splits((mt > held ? mt : held) * ((N + 63) / 64), K * op_size(ot), 2048, slots);
+// 64 x 64 tiles, three workgroups per CU: as many ranges as have room in one round.
+// More than half a tile per CU: the fold writes and reads more than a short k takes, so k
+// has to be `lengthy`.
+inline int op_tile_splits(long long tiles, long long k, long long least, long long lengthy, int ncu) {
+    if (tiles < 1 || (2 * tiles > ncu && k < lengthy)) return 1;
+    long long s = 3ll * ncu / tiles;
+    if (s > k / least) s = k / least;
+    if (s > kOpMaxSplits) s = kOpMaxSplits;
+    return s > 1 ? (int)s : 1;
 }
-// Ragged k: the rows of each group.
-inline int op_matrix_splits(long long rows, long long E, long long M, long long N, int ncu) {
-    return op_splits(E * ((M + 63) / 64) * ((N + 63) / 64), rows / E, 512, ncu);
+// Ragged rows: by 64 x 64 tiles, or the streamed products' 16 columns.  On 256 CUs, one
+// range / this many, us: bf16, rows of 16 KB: 64 tiles 61 / 21, 128 56 / 28, 256 61 / 39, 384
+// 63 / 51, of 8 KB: 33 / 16, 33 / 20, 33 / 28, 33 / 33; of 4 KB (256 tiles: none) 18 / 22.
+// int8 within 1 us of those.  fp32: 16 KB 85 / 29, 83 / 47, 83 / 77, 135 / 111; 8 KB 45 / 20, 45
+// / 28, (none) 45 / 47, 70 / 63.
+inline int op_rows_splits(int ot, bool b_col, long long rows, long long E, long long N, long long K, int ncu) {
+    const long long held = E < rows ? E : rows, bytes = K * op_size(ot);  // groups that may hold rows
+    if (op_streamed(ot, b_col, rows, E, K)) return op_splits(held * ((N + 15) / 16), bytes, 8192, ncu);
+    const long long mt = (rows + 63) / 64, tiles = (mt > held ? mt : held) * ((N + 63) / 64);
+    // a few rows per group read the weights as fast as loads are in flight: four
+    // 64 x 64 tiles per CU (4 rows of 3991 on 8 experts of 4970 columns, fp32: 114 us at one)
+    if (rows <= 16 * E) return op_splits(tiles, bytes, 2048, 4 * ncu);
+    return op_tile_splits(tiles, bytes, 2048, ot == OT_F32 ? 12288 : 8192, ncu);
+}
+// Ragged k: the rows of each group.  fp32, bound by its products: 8000 rows, 512 / 1024 (128
+// tiles) 165 / 77 us, 1000 / 1000 (256) 166 / 141, 4000 rows of 1536 / 1024 (384) 136 / 111, 1900
+// of 1000 / 1000 43 / 46 (none).  bf16, bound by its reads: 8000 rows of 512 / 1024 in two
+// ranges 41 / 28, but 1000 / 1000 43 / 47: only where half the CUs have no tile.
+inline int op_matrix_splits(int ot, long long rows, long long E, long long M, long long N, int ncu) {
+    const long long tiles = E * ((M + 63) / 64) * ((N + 63) / 64);
+    return ot == OT_F32 ? op_tile_splits(tiles, rows / E, 800, 4000, ncu) : op_splits(tiles, rows / E, 512, ncu);
 }
 
 // What a launcher answers to a call of more workgroups than one launch takes.

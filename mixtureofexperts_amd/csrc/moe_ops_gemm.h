@@ -995,11 +995,26 @@ hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
         if (vb == 16 && large)
             return launch_tiles<OT, ACOL, BCOL, RAGK, 256, 256, 4, 2, KSUB, 4 / KSUB, 2>(g, vb, s);
     }
-    // fp32 is bound by its matrix rate alone, so the rows that a group's last tile
-    // lacks cost more than 64 x 64 tiles' loads: one group of 469 rows, 3008 -> 11648,
-    // 358 us at 128 against 283 at 64; 4096 rows, 4096 -> 4096, 985 against 1010
-    const long long least = OT == OT_F32 && !RAGK ? 512 : 64;
-    if (!(OT == OT_F32 && vb == 0) && avg >= least && g.N >= 64 && tiles(128) >= ncu)
+    bool medium = avg >= 64 && g.N >= 64 && tiles(128) >= ncu;
+    if constexpr (OT == OT_F32) {
+        // fp32 is bound by its matrix rate: the CU with the most tiles decides, a 128 x 128
+        // tile taking as long as 3.8 of 64 x 64 (weight gradient, whose stores it spares:
+        // 3.4).  A group's last tile is half empty on average.  us, 128 / 64: row products
+        // of 4096 cubed 964 / 1000, 3000 cubed 536 / 424, 8 groups of 1024 rows 2048 / 2048 605 /
+        // 545, 44114 rows 2240 / 192 409 / 326; weight gradients of 4096 cubed 957 / 1009, 12 groups
+        // of 259 rows 1001 / 2731 164 / 194, 3 of 1325 rows 12810 / 69 176 / 135.
+        auto per_cu = [&](int b) -> long long {
+            const long long nt = (g.N + b - 1) / b;
+            const long long mt = RAGK ? (g.M + b - 1) / b * (long long)g.E
+                                      : (g.E > 1 ? g.rows / b + (g.E < g.rows ? g.E : g.rows) / 2 + 1 : (g.rows + b - 1) / b);
+            return (nt * mt + ncu - 1) / ncu;
+        };
+        // (a weight gradient of fewer rows than 64 is bound by its stores: 71 groups of one
+        // row at most, 6193 / 257, 158 / 181)
+        if (vb == 0) medium = false;
+        else if (!RAGK || g.rows >= 64ll * g.E) medium = (RAGK ? 34 : 38) * per_cu(128) < 10 * per_cu(64);
+    }
+    if (medium)
         return launch_tiles<OT, ACOL, BCOL, RAGK, 128, 128, 2, 2, KSUB, RAGK ? 3 : 4 / KSUB, RAGK ? 3 : 2>(g, vb, s);
     return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, KSUB, 4 / KSUB, 3>(g, vb, s);
 }

@@ -32,19 +32,20 @@ import ctypes
 from . import _lib
 from ._lib import MOE_EINVAL, MOE_LAYOUT_FLUX_OUT_IN, MOE_LAYOUT_LLAMA_IN_OUT
 
-_torch = _forward_ad = _written = None
+_torch = _forward_ad = _grad_enabled = _written = None
 _codes = {}
 _floats = []  # the types of float operands
 
 
 def _t():
     """torch, imported at first use (the host API needs only numpy)."""
-    global _torch, _forward_ad, _written
+    global _torch, _forward_ad, _grad_enabled, _written
     if _torch is None:
         import torch
         import torch.autograd.forward_ad as forward_ad
 
-        _torch, _forward_ad, _written = torch, forward_ad, torch.autograd.graph.increment_version
+        _torch, _forward_ad, _grad_enabled = torch, forward_ad, torch.is_grad_enabled
+        _written = torch.autograd.graph.increment_version
         _floats.extend((torch.float32, torch.bfloat16))
         _codes.update({torch.float32: _lib.MOE_F32, torch.bfloat16: _lib.MOE_BF16, torch.int8: _lib.MOE_INT8})
     return _torch
@@ -57,15 +58,19 @@ def _bad(msg):
 def _plain(names, *tensors):
     """Refuses what autograd would have to record (see above); names: the
     arguments', as one string."""
-    torch = _torch or _t()
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and getattr(t, "requires_grad", False):
-                name = names.split()[[t is u for u in tensors].index(True)]
-                _bad(f"{name} requires a gradient, which this call does not record: use torch.no_grad() or detach it")
+    if _torch is None:
+        _t()
+    if _grad_enabled():
+        try:
+            for t in tensors:
+                if t is not None and t.requires_grad:
+                    name = names.split()[[t is u for u in tensors].index(True)]
+                    _bad(f"{name} requires a gradient, which this call does not record: use torch.no_grad() or detach it")
+        except AttributeError:
+            pass  # not a tensor, which is refused for that
     if _forward_ad._current_level >= 0:  # within a forward_ad.dual_level()
         for name, t in zip(names.split(), tensors):
-            if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+            if isinstance(t, _torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
                 _bad(f"{name} carries a tangent, which this call does not propagate")
 
 
@@ -100,11 +105,13 @@ def _rows(t, name, dtypes):
     return t.data_ptr(), _row_stride(t, name)
 
 
-def _matrices(t, name, dtypes):
-    """(E, a, b) or (a, b): (E, a, b, row stride, matrix stride)."""
-    _tensor(t, name, dtypes, (2, 3))
-    if max(t.shape) > 2**31 - 1:
-        _bad(f"{name}: sizes must fit 32 bits")
+def _matrices(t, name, dtypes=None):
+    """(E, a, b) or (a, b): (E, a, b, row stride, matrix stride); without dtypes
+    of a tensor that is checked already."""
+    if dtypes is not None:
+        _tensor(t, name, dtypes, (2, 3))
+        if max(t.shape) > 2**31 - 1:
+            _bad(f"{name}: sizes must fit 32 bits")
     a, b = t.shape[-2:]
     ld = _row_stride(t, name)
     if t.dim() == 2:
@@ -128,16 +135,13 @@ def _offsets(offsets, E):
     return offsets.data_ptr()
 
 
-def _same_device(*tensors):
-    first = None
+def _same_device(first, *tensors):
+    """The device of all tensors (None: left out), `first` among them."""
+    device = first.device
     for t in tensors:
-        if t is None:
-            continue
-        if first is None:
-            first = t.device
-        elif t.device != first:
+        if t is not None and t.device != device:
             _bad("tensors must be on one device")
-    return first
+    return device
 
 
 def _call(fn, device, *args):
@@ -259,7 +263,7 @@ def grouped_matmul_grad_w(x, dy, offsets=None, *, layout=MOE_LAYOUT_LLAMA_IN_OUT
     shape = (a, b) if (out.dim() == 2 if out is not None else offsets is None) and E == 1 else (E, a, b)
     given = out
     out = _result(out, shape, out_dtype, _float_types(x.dtype), x, False)
-    _, _, _, ldw, stride = _matrices(out, "out", _float_types(x.dtype))
+    _, _, _, ldw, stride = _matrices(out, "out")
     device = _same_device(x, dy, offsets, out)
     ws, wsp, wsn = _workspace(L.moe_grouped_matmul_grad_w_workspace, device, E, x.shape[0], x.shape[1], dy.shape[1])
     _call(L.moe_grouped_matmul_grad_w_async, device, xp, ldx, dp, lddy, layout, _offsets(offsets, E), E, x.shape[0],
@@ -384,7 +388,9 @@ def block_norm(x, y=None, *, pre_weight=None, post_weight=None, gate=None, alpha
     if D < 1:
         _bad("x has no channels")
     T = x.numel() // D
-    xp, yp = _dense(x, "x", _floats, shape), _dense(y, "y", _floats, shape)
+    if not x.is_contiguous():
+        _bad(f"x must be contiguous {tuple(shape)}")
+    xp, yp = x.data_ptr(), _dense(y, "y", _floats, shape)
     if y is None:
         if post_weight is not None or gate is not None:
             _bad("post_weight and gate need y")
@@ -421,7 +427,9 @@ def block_norm_grad(dr, dh, r, y=None, stats=None, *, pre_weight=None, post_weig
     if D < 1:
         _bad("r has no channels")
     T = r.numel() // D
-    rp, drp = _dense(r, "r", _floats, shape), _dense(dr, "dr", (r.dtype,), shape)
+    if not r.is_contiguous():
+        _bad(f"r must be contiguous {tuple(shape)}")
+    rp, drp = r.data_ptr(), _dense(dr, "dr", (r.dtype,), shape)
     dhp, yp = _dense(dh, "dh", _floats, shape), _dense(y, "y", _floats, shape)
     sp = _dense(stats, "stats", (torch.float32,), (T, 2))
     if dr is None and dh is None:
@@ -433,7 +441,7 @@ def block_norm_grad(dr, dh, r, y=None, stats=None, *, pre_weight=None, post_weig
     if stats is None and (pre_weight is not None or post_weight is not None):
         _bad("stats are needed")
     pre, post, wt, gp, gt, gate_rows = _norm_params(D, T, pre_weight, post_weight, gate)
-    device = _same_device(dr, dh, r, y, stats, pre_weight, post_weight, gate)
+    device = _same_device(r, dr, dh, y, stats, pre_weight, post_weight, gate)
     dx = torch.empty_like(r)
     dy = torch.empty_like(y) if y is not None else None
     # (a sum over no rows is zero; the call writes a gate row's sum with its rows)
