@@ -55,7 +55,12 @@ def test_rows_products(moe, layout):
         ([71], 5440, 64, "f32", 64, True),
         ([1], 8192, 16, "f32", 64 if col else 0, True),
         ([3, 0, 2], 16401, 125, "f32", 64 if col else 0, True),
-        ([3, 0, 2], 64, 96, "bf16", 64 if col else 0, False),
+        ([3, 0, 2], 64, 96, "bf16", 64, False),
+        ([3, 0, 2], 64, 96, "f32", 64 if col else 0, False),
+        ([8, 3, 13], 2048, 96, "bf16", 64 if col else 0, True if col else False),
+        ([8, 3, 14], 2048, 96, "bf16", 64, True),
+        ([3000], 96, 3000, "f32", 64, False),
+        ([2048], 96, 4096, "f32", 128, False),
         ([17, 0, 1, 64], 64, 96, "f32", 64, False),
     ):
         x, dy, w, off = _operands(lens, K, N, dtype, layout)
@@ -83,6 +88,9 @@ def test_weight_gradients(moe, layout):
         ([33, 130, 5, 0, 300], 200, 136, "bf16", 64, False),
         ([3000], 96, 40, "bf16", 64, True),
         ([2500, 0, 4000], 64, 64, "f32", 64, True),
+        ([4000], 2048, 640, "f32", 64, True),
+        ([4096], 1024, 1024, "f32", 64, True),
+        ([300, 900], 2048, 2048, "f32", 128, False),
     ):
         x, dy, w, off = _operands(lens, K, N, dtype, layout)
         got = _kernels(lambda: moe.grouped_matmul_grad_w(x, dy, off, layout=layout, out_dtype=torch.float32))
@@ -102,7 +110,7 @@ def test_loads_by_alignment(moe):
 def test_int8_products(moe):
     for lens, K, N, tile, split in (([3000, 5500], 160, 4112, 256, False), ([700, 0, 900, 500], 144, 2048, 128, False),
                                     ([33, 130, 5, 0, 300], 208, 136, 64, False), ([40, 30], 20000, 33, 64, True),
-                                    ([0, 3, 0], 7, 5, 0, False), ([0, 0, 2, 0, 1, 0, 0], 20000, 17, 0, True)):
+                                    ([0, 3, 0], 7, 5, 64, False), ([0, 3, 0], 4096, 50, 0, False), ([0, 0, 2, 0, 1, 0, 0], 20000, 17, 0, True)):
         x, _, w, off = _operands(lens, K, N, "bf16", LLAMA)
         ws = torch.ones(w.shape[:2], device="cuda")
         w = w.to(torch.int8)

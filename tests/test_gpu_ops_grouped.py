@@ -429,3 +429,41 @@ def test_weight_gradient_of_two_rounds_of_large_tiles(moe, layout):
     a, b = (_f64(dy), _f64(x)) if layout == LLAMA else (_f64(x), _f64(dy))
     for e, s in enumerate((slice(0, 70), slice(70, 70), slice(70, 203), slice(203, 212))):
         _close(_f64(dw[e]), a[s].T @ b[s], np.abs(a[s]).T @ np.abs(b[s]), max(lens[e], 1), "f32")
+
+
+@pytest.mark.parametrize("layout", [LLAMA, FLUX])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_long_sums_of_more_than_half_a_tile_per_cu(moe, dtype, layout):
+    # k split over workgroups where 64 x 64 tiles alone fill more than half of the GPU
+    K = {"f32": 3101, "bf16": 5440}[dtype]
+    for lens, N in (([200], 2500), ([150, 0, 77, 1], 1800), ([130], 8200)):
+        print(f"grouped split of many tiles {dtype} layout={layout} lens={lens} K={K} N={N}", flush=True)
+        rng = np.random.default_rng([K, N, layout, 6])
+        M, E, start = sum(lens), len(lens), 1
+        x = _rows(rng, M + start, K, dtype, 0, 2)
+        w = _mats(rng, E, *((N, K) if layout == LLAMA else (K, N)), dtype, 0)
+        W, X = (_f64(w) if layout == LLAMA else _f64(w).transpose(0, 2, 1)), _f64(x)
+        out = torch.full((M + start + 2, N + 2), SENTINEL, dtype=DT[dtype], device="cuda")
+        got, at = _f64(moe.grouped_matmul(x, w, _offsets(lens, start), layout=layout, out=out[:, :N])), start
+        for e, n in enumerate(lens):
+            a = X[at:at + n]
+            _close(got[at:at + n], a @ W[e].T, np.abs(a) @ np.abs(W[e].T), K, dtype)
+            at += n
+        assert (got[:start] == SENTINEL).all() and (got[at:] == SENTINEL).all() and (_f64(out)[:, N:] == SENTINEL).all()
+
+
+@pytest.mark.parametrize("layout", [LLAMA, FLUX])
+def test_long_weight_gradients_of_more_than_half_a_tile_per_cu(moe, layout):
+    for lens, K, N in (([4100], 1030, 1000), ([6000, 0, 7001], 330, 700)):
+        print(f"grad_w split of many tiles layout={layout} lens={lens} K={K} N={N}", flush=True)
+        rng = np.random.default_rng([K, N, layout, 7])
+        M = sum(lens)
+        x, dy, off = _rows(rng, M, K, "f32", 0), _rows(rng, M, N, "f32", 0), _offsets(lens)
+        a, b = (_f64(dy), _f64(x)) if layout == LLAMA else (_f64(x), _f64(dy))
+        out = torch.ones(len(lens), a.shape[1], b.shape[1], device="cuda")
+        moe.grouped_matmul_grad_w(x, dy, off, layout=layout, out=out, accumulate=True)
+        got, at = _f64(out), 0
+        for e, n in enumerate(lens):
+            s = slice(at, at + n)
+            _close(got[e], 1 + a[s].T @ b[s], 1 + np.abs(a[s]).T @ np.abs(b[s]), max(n, 1) + 1, "f32")
+            at += n
