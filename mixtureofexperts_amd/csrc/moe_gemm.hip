@@ -385,19 +385,19 @@ hipError_t launch_grouped_gemm_f32(int mode, const GemmArgs &g0, hipStream_t s) 
 hipError_t launch_op_gemm_f32(bool b_col, bool ragged_k, OpGemmArgs g, int ncu, hipStream_t s) {
     if (ragged_k) return ops::op_gemm_plan<OT_F32, true, true, true>(g, ncu, s);
     if (b_col) return ops::op_gemm_plan<OT_F32, false, true, false>(g, ncu, s);
-    if (op_streamed(OT_F32, b_col, g.rows, g.E, g.K)) return launch_op_stream(OT_F32, g, s);
+    if (op_streamed(OT_F32, b_col, g.rows, g.E, g.N, g.K, ncu)) return launch_op_stream(OT_F32, g, s);
     return ops::op_gemm_plan<OT_F32, false, false, false>(g, ncu, s);
 }
 
 hipError_t launch_op_gemm_bf16(bool b_col, bool ragged_k, OpGemmArgs g, int ncu, hipStream_t s) {
     if (ragged_k) return ops::op_gemm_plan<OT_BF16, true, true, true>(g, ncu, s);
     if (b_col) return ops::op_gemm_plan<OT_BF16, false, true, false>(g, ncu, s);
-    if (op_streamed(OT_BF16, b_col, g.rows, g.E, g.K)) return launch_op_stream(OT_BF16, g, s);
+    if (op_streamed(OT_BF16, b_col, g.rows, g.E, g.N, g.K, ncu)) return launch_op_stream(OT_BF16, g, s);
     return ops::op_gemm_plan<OT_BF16, false, false, false>(g, ncu, s);
 }
 
 hipError_t launch_op_gemm_i8(OpGemmArgs g, int ncu, hipStream_t s) {
-    if (op_streamed(OT_I8, false, g.rows, g.E, g.K)) return launch_op_stream(OT_I8, g, s);
+    if (op_streamed(OT_I8, false, g.rows, g.E, g.N, g.K, ncu)) return launch_op_stream(OT_I8, g, s);
     return ops::op_gemm_plan<OT_I8, false, false, false>(g, ncu, s);
 }
 

@@ -59,10 +59,17 @@ __device__ __forceinline__ long long op_row_block() { return (long long)blockIdx
 // rows each: 145 / 178, 24: 168 / 162).  bf16 and int8: up to 8 rows, of weights with 4 KB
 // and more per row (bf16, 4096 / 14336: 1 row 164 / 183, 4 170 / 204, 8 193 / 191, 16 241 /
 // 201; int8 104 / 105, 106 / 122, 109 / 119, 124 / 126; 64 experts of 1408 / 2048, bf16: 1
-// row 53 / 51, 8 89 / 77, int8 36 / 30, 57 / 45; 8 of 2048 / 4096: bf16, 8 rows, 37 / 39, int8 17 / 14).
-inline bool op_streamed(int ot, bool b_col, long long rows, long long E, long long K) {
+// row 53 / 51, 8 89 / 77, int8 36 / 30, 57 / 45; 8 of 2048 / 4096: bf16, 8 rows, 37 / 39, int8 17
+// / 14) or, shorter, fewer tiles than CUs (2048 / 4096: 12.5 / 15).  Rows that do not end
+// on 4 bytes, whose elements' loads bound both: only such few tiles, and of a k too short
+// to split or about one row per group (4 rows on each of 3 experts of 1665 / 3000 25 / 26,
+// of 16 86 / 52; of 3001 / 3000, 3 experts, 35 / 27, one row 20 / 23).
+inline bool op_streamed(int ot, bool b_col, long long rows, long long E, long long N, long long K, int ncu) {
     if (b_col) return false;
-    return ot == OT_F32 ? rows <= 16 * E : rows <= 8 * E && K * op_size(ot) >= 4096;
+    if (ot == OT_F32) return rows <= 16 * E;
+    const long long bytes = K * op_size(ot);
+    const bool few = (E < rows ? E : rows) * ((N + 63) / 64) < ncu, lengthy = bytes >= 4096;
+    return rows <= 8 * E && (bytes % 4 ? few && (!lengthy || rows <= E) : few || lengthy);
 }
 
 constexpr int kOpMaxSplits = 16;
@@ -94,7 +101,7 @@ inline int op_tile_splits(long long tiles, long long k, long long least, long lo
 // / 28, (none) 45 / 47, 70 / 63.
 inline int op_rows_splits(int ot, bool b_col, long long rows, long long E, long long N, long long K, int ncu) {
     const long long held = E < rows ? E : rows, bytes = K * op_size(ot);  // groups that may hold rows
-    if (op_streamed(ot, b_col, rows, E, K)) return op_splits(held * ((N + 15) / 16), bytes, 8192, ncu);
+    if (op_streamed(ot, b_col, rows, E, N, K, ncu)) return op_splits(held * ((N + 15) / 16), bytes, 8192, ncu);
     const long long mt = (rows + 63) / 64, tiles = (mt > held ? mt : held) * ((N + 63) / 64);
     // a few rows per group read the weights as fast as loads are in flight: four
     // 64 x 64 tiles per CU (4 rows of 3991 on 8 experts of 4970 columns, fp32: 114 us at one)

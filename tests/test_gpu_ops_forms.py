@@ -55,7 +55,8 @@ def test_rows_products(moe, layout):
         ([71], 5440, 64, "f32", 64, True),
         ([1], 8192, 16, "f32", 64 if col else 0, True),
         ([3, 0, 2], 16401, 125, "f32", 64 if col else 0, True),
-        ([3, 0, 2], 64, 96, "bf16", 64, False),
+        ([3, 0, 2], 64, 96, "bf16", 64 if col else 0, False),
+        ([3, 0, 2], 64, 8200, "bf16", 64, False),
         ([3, 0, 2], 64, 96, "f32", 64 if col else 0, False),
         ([8, 3, 13], 2048, 96, "bf16", 64 if col else 0, True if col else False),
         ([8, 3, 14], 2048, 96, "bf16", 64, True),
@@ -110,7 +111,8 @@ def test_loads_by_alignment(moe):
 def test_int8_products(moe):
     for lens, K, N, tile, split in (([3000, 5500], 160, 4112, 256, False), ([700, 0, 900, 500], 144, 2048, 128, False),
                                     ([33, 130, 5, 0, 300], 208, 136, 64, False), ([40, 30], 20000, 33, 64, True),
-                                    ([0, 3, 0], 7, 5, 64, False), ([0, 3, 0], 4096, 50, 0, False), ([0, 0, 2, 0, 1, 0, 0], 20000, 17, 0, True)):
+                                    ([0, 3, 0], 7, 5, 0, False), ([0, 9, 0], 4096, 8200, 0, False), ([0, 9, 0], 2048, 8200, 64, False),
+                                    ([0, 9, 0], 5001, 50, 64, True), ([0, 0, 2, 0, 1, 0, 0], 20000, 17, 0, True)):
         x, _, w, off = _operands(lens, K, N, "bf16", LLAMA)
         ws = torch.ones(w.shape[:2], device="cuda")
         w = w.to(torch.int8)
