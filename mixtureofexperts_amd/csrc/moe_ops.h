@@ -104,7 +104,8 @@ inline int op_rows_splits(int ot, bool b_col, long long rows, long long E, long 
     if (op_streamed(ot, b_col, rows, E, N, K, ncu)) return op_splits(held * ((N + 15) / 16), bytes, 8192, ncu);
     const long long mt = (rows + 63) / 64, tiles = (mt > held ? mt : held) * ((N + 63) / 64);
     // a few rows per group read the weights as fast as loads are in flight: four
-    // 64 x 64 tiles per CU (4 rows of 3991 on 8 experts of 4970 columns, fp32: 114 us at one)
+    // 64 x 64 tiles per CU (4 rows of 3991 on 4 experts of 4970 columns, fp32: 112 us in one
+    // range, 86 so)
     if (rows <= 16 * E) return op_splits(tiles, bytes, 2048, 4 * ncu);
     return op_tile_splits(tiles, bytes, 2048, ot == OT_F32 ? 12288 : 8192, ncu);
 }

@@ -644,8 +644,8 @@ __device__ __forceinline__ void store_tile_rows(const OpGemmArgs &g, lds_u8 *rin
 
 // ---- the kernel --------------------------------------------------------------------
 // Bound by the matrix units at the clock that their load leaves: 8192 rows, 8
-// bf16 experts of 4096 / 14336 in 843 us (1140 TFLOP/s, units 56 % busy; one 8192
-// cubed product 1325), their row gradient 844, int8 475 (2020 TOP/s); fp32, 4096
+// bf16 experts of 4096 / 14336 in 835 to 862 us (1140 TFLOP/s, units 56 % busy; one 8192
+// cubed product 1325), their row gradient the same, int8 485 (2000 TOP/s); fp32, 4096
 // cubed, 142 TFLOP/s of 154.  The weight gradient of 64 groups of 2048 / 1408 over
 // 49152 rows (383 us) is bound by its 738 MB result, stored after each tile.
 //

@@ -198,7 +198,7 @@ __device__ __forceinline__ double row_sum_wide(float v, double *part) {
 // lies within what the fp32 steps may be off (about an element in 8000).  Each rounds
 // by 2^-24 of its value: y's term at rstd beta, its product with y, the weight and the
 // gate, the sum at the addition and on the way by fp32.  8192 x 4096, fp32 y, both
-// norms, a gate: 67 to 68 us, 67 all in fp32, 81 all in fp64 (117 registers instead of 68).
+// norms, a gate: 67 to 68 us, 67 all in fp32, 81 all in fp64 (117 registers instead of 66).
 template <int TPR, int NV, bool VEC, bool WIDE>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void block_norm_kernel(NormArgs a) {
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;

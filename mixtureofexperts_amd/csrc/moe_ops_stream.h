@@ -4,10 +4,11 @@
 //
 // A workgroup owns 16 columns of one group; its four waves take interleaved
 // 128-byte pieces of k, U of them in flight, and their partial 16 x 16 blocks
-// are added in wave order through LDS.  Bound by HBM reads: 256 rows on 8 bf16
-// experts of 4096 / 14336 161 us (5.8 TB/s), two int8 rows on two of them 26 us
-// (4.4 TB/s).  32 fp32 rows on 8 experts of 512 / 2048 10 us (3.4 TB/s, one round of
-// workgroups).
+// are added in wave order through LDS.  Bound by HBM reads: 32 rows on 8 bf16
+// experts of 4096 / 14336 154 to 166 us (5.6 to 6 TB/s), two int8 rows on two of them
+// 26 us (4.4 TB/s).  64 fp32 rows on 8 experts of 512 / 2048 10 us (3.4 TB/s, one round of
+// workgroups).  Up to 8 or 16 rows per group on average (op_streamed): a group of more
+// than 64 is walked 64 rows at a time, its weights read again each time.
 #pragma once
 #include "moe_ops_gemm.h"
 
