@@ -467,3 +467,42 @@ def test_long_weight_gradients_of_more_than_half_a_tile_per_cu(moe, layout):
             s = slice(at, at + n)
             _close(got[e], 1 + a[s].T @ b[s], 1 + np.abs(a[s]).T @ np.abs(b[s]), max(n, 1) + 1, "f32")
             at += n
+
+
+def test_two_graphs_of_split_sums(moe):
+    # calls with workspaces in two captured graphs, replayed in turn and side by side
+    # with eager calls of the same between them
+    rng = np.random.default_rng(20)
+    jobs = []
+    for dtype, lens, K, N in (("f32", [150, 0, 77], 3101, 1800), ("bf16", [200], 5440, 2500), ("f32", [3000, 1], 96, 40)):
+        x, dy = _rows(rng, sum(lens), K, dtype, 0), _rows(rng, sum(lens), N, dtype, 0)
+        jobs.append((x, dy, _mats(rng, len(lens), N, K, dtype, 0), _offsets(lens)))
+
+    def run(xs):
+        return [f for x, (_, dy, w, off) in zip(xs, jobs)
+                for f in (moe.grouped_matmul(x, w, off), moe.grouped_matmul_grad_w(x, dy, off))]
+
+    first = [j[0] for j in jobs]
+    sets = [first, [x * 2 for x in first], [x * -0.5 for x in first]]
+    want = [run(s) for s in sets]
+    bufs = [[x.clone() for x in first] for _ in range(2)]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for b in bufs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(run(b))
+        graphs.append(g)
+    side = torch.cuda.Stream()
+    for i, k in ((0, 1), (1, 2), (2, 0), (1, 1)):
+        for b, n in zip(bufs, (i, k)):
+            for x, v in zip(b, sets[n]):
+                x.copy_(v)
+        side.wait_stream(torch.cuda.current_stream())
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        eager = run(sets[k])
+        torch.cuda.synchronize()
+        for got, n in ((outs[0], i), (outs[1], k), (eager, k)):
+            assert all(torch.equal(a, b) for a, b in zip(got, want[n])), (i, k)
