@@ -452,6 +452,47 @@ int moe_grouped_matmul_grad_w_async(const void *x, int64_t ldx, const void *dy, 
                                     int32_t dw_dtype, int32_t accumulate, void *workspace, int64_t workspace_bytes,
                                     void *stream);
 
+/* The two projections of a gated feed-forward block, its activation and the
+ * product in one pass, for the rows r of group e:
+ *   a[r] = W1_e x[r], b[r] = W3_e x[r], h[r] = act(a[r]) .* b[r]
+ * x [rows][in_dim], h, a, b [rows][hidden_dim]; W1 and W3 are matrices of in_dim
+ * to hidden_dim in one layout, each with its own strides.  activation:
+ * moe_activation.  The sums stay in fp32 until h is formed; h in h_dtype, a and b
+ * (what a backward pass needs; both NULL: not stored) in dtype.  No result may
+ * overlap another.  workspace: as moe_grouped_matmul_async's, from
+ * moe_gated_matmul_workspace. */
+int moe_gated_matmul_workspace(int32_t groups, int32_t rows, int32_t in_dim, int32_t hidden_dim, int32_t dtype,
+                               int64_t *bytes);
+int moe_gated_matmul_async(const void *x, int64_t ldx, const void *w1, int64_t ldw1, int64_t w1_stride, const void *w3,
+                           int64_t ldw3, int64_t w3_stride, int32_t layout, int32_t activation, const int32_t *offsets,
+                           int32_t groups, int32_t rows, int32_t in_dim, int32_t hidden_dim, int32_t dtype, void *h,
+                           int64_t ldh, int32_t h_dtype, void *a, int64_t lda, void *b, int64_t ldb, void *workspace,
+                           int64_t workspace_bytes, void *stream);
+/* Its gradients with respect to a and b, from that of the block's output
+ * y[r] = W2_e h[r]:
+ *   dh = W2_e' dy, da = dh .* b .* act'(a), db = dh .* act(a), h = act(a) .* b
+ * dh is not stored and not rounded; h is formed again from a and b as they are
+ * stored, for the gradient of W2.  w2: matrices of hidden_dim to out_dim; NULL:
+ * dy is dh itself, out_dim = hidden_dim, no workspace.  All in dtype.  No result
+ * may overlap another or an operand.  The gradients of the weights are
+ * moe_grouped_matmul_grad_w_async's (x with da and db, h with dy). */
+int moe_gated_matmul_grad_workspace(int32_t groups, int32_t rows, int32_t hidden_dim, int32_t out_dim, int32_t dtype,
+                                    int64_t *bytes);
+int moe_gated_matmul_grad_async(const void *dy, int64_t lddy, const void *w2, int64_t ldw2, int64_t w2_stride,
+                                int32_t layout, int32_t activation, const void *a, int64_t lda, const void *b, int64_t ldb,
+                                const int32_t *offsets, int32_t groups, int32_t rows, int32_t hidden_dim, int32_t out_dim,
+                                int32_t dtype, void *da, int64_t ldda, void *db, int64_t lddb, void *h, int64_t ldh,
+                                void *workspace, int64_t workspace_bytes, void *stream);
+/* And with respect to x, both projections in one sum: dx[r] = W1_e' da[r] +
+ * W3_e' db[r]. */
+int moe_gated_matmul_grad_x_workspace(int32_t groups, int32_t rows, int32_t in_dim, int32_t hidden_dim, int32_t dtype,
+                                      int64_t *bytes);
+int moe_gated_matmul_grad_x_async(const void *da, int64_t ldda, const void *db, int64_t lddb, const void *w1,
+                                  int64_t ldw1, int64_t w1_stride, const void *w3, int64_t ldw3, int64_t w3_stride,
+                                  int32_t layout, const int32_t *offsets, int32_t groups, int32_t rows, int32_t in_dim,
+                                  int32_t hidden_dim, int32_t dtype, void *dx, int64_t lddx, int32_t dx_dtype,
+                                  void *workspace, int64_t workspace_bytes, void *stream);
+
 /* int8 codes with a scale per row: scale[r] = max|x[r]| / 127, q[r][c] = 127
  * x[r][c] / max|x[r]| rounded to nearest even.  A row of zeros has scale 0 and
  * codes 0; one that holds an infinity or a NaN has scale NaN and codes 0.

@@ -43,7 +43,9 @@ EXPORTED_SYMBOLS = [
     "moe_set_aux_free", "moe_get_aux_free", "moe_aux_free_update_bias", "moe_forward_routed",
     "moe_init_experts_from_dense", "moe_get_expert", "moe_switch_loss_noalloc",
     "moe_grouped_matmul_async", "moe_grouped_matmul_workspace", "moe_grouped_matmul_grad_x_async", "moe_grouped_matmul_grad_w_async",
-    "moe_grouped_matmul_grad_w_workspace", "moe_quantize_int8_async", "moe_int8_matmul_async",
+    "moe_grouped_matmul_grad_w_workspace", "moe_gated_matmul_workspace", "moe_gated_matmul_async",
+    "moe_gated_matmul_grad_workspace", "moe_gated_matmul_grad_async", "moe_gated_matmul_grad_x_workspace",
+    "moe_gated_matmul_grad_x_async", "moe_quantize_int8_async", "moe_int8_matmul_async",
     "moe_int8_matmul_workspace", "moe_block_norm_async", "moe_block_norm_grad_async", "moe_block_norm_grad_workspace",
 ]
 
@@ -160,6 +162,17 @@ def lib():
     L.moe_grouped_matmul_grad_w_workspace.argtypes = [i32, i32, i32, i32, i64p]
     L.moe_grouped_matmul_grad_w_async.argtypes = [vp, i64, vp, i64, i32, vp, i32, i32, i32, i32, i32, vp, i64, i64, i32,
                                                   i32, vp, i64, vp]
+    sizes = [i32, i32, i32, i32, i32, i64p]
+    w = [vp, i64, i64]
+    L.moe_gated_matmul_workspace.argtypes = sizes
+    L.moe_gated_matmul_async.argtypes = [vp, i64, *w, *w, i32, i32, vp, i32, i32, i32, i32, i32, vp, i64, i32, vp, i64, vp,
+                                         i64, vp, i64, vp]
+    L.moe_gated_matmul_grad_workspace.argtypes = sizes
+    L.moe_gated_matmul_grad_async.argtypes = [vp, i64, *w, i32, i32, vp, i64, vp, i64, vp, i32, i32, i32, i32, i32, vp, i64,
+                                              vp, i64, vp, i64, vp, i64, vp]
+    L.moe_gated_matmul_grad_x_workspace.argtypes = sizes
+    L.moe_gated_matmul_grad_x_async.argtypes = [vp, i64, vp, i64, *w, *w, i32, vp, i32, i32, i32, i32, i32, vp, i64, i32, vp,
+                                                i64, vp]
     L.moe_quantize_int8_async.argtypes = [vp, i64, i32, i64, i32, vp, i64, vp, vp]
     L.moe_int8_matmul_workspace.argtypes = [i32, i32, i32, i32, i32, i64p]
     L.moe_int8_matmul_async.argtypes = [vp, i64, i32, vp, vp, i64, i64, vp, vp, i32, i32, i32, i32, vp, i64, i32, vp,

@@ -6,6 +6,7 @@
 #include <mutex>
 
 #include "moe_ops.h"
+#include "moe_ops_gated.h"
 
 namespace {
 // compute units of the current device (looked up once per device)
@@ -239,6 +240,191 @@ int moe_grouped_matmul_grad_w_async(const void *x, int64_t ldx, const void *dy, 
     g.ws = (float *)workspace;
     return op_done(fn, dtype == MOE_F32 ? launch_op_gemm_f32(true, true, g, op_cus(), (hipStream_t)stream)
                                         : launch_op_gemm_bf16(true, true, g, op_cus(), (hipStream_t)stream));
+}
+
+// ---- gated blocks --------------------------------------------------------------------
+static int op_check_gated(const char *fn, const int32_t *offsets, int32_t groups, int32_t rows, int32_t in_dim,
+                          int32_t out_dim, int32_t dtype, int32_t out_dtype, int32_t layout, int32_t activation) {
+    int r = op_check_groups(fn, offsets, groups, rows, in_dim, out_dim);
+    if (r == MOE_OK) r = op_check_dtypes(fn, dtype, out_dtype);
+    if (r != MOE_OK) return r;
+    if (layout != MOE_LAYOUT_FLUX_OUT_IN && layout != MOE_LAYOUT_LLAMA_IN_OUT) return op_fail(fn, "unknown layout");
+    if (activation < MOE_ACT_GELU || activation > MOE_ACT_IDENTITY) return op_fail(fn, "unknown activation");
+    return MOE_OK;
+}
+static int64_t gated_workspace(OpMode mode, int32_t groups, int32_t rows, int32_t n, int32_t k, int32_t dtype) {
+    int64_t bytes = 0;
+    if (rows == 0) return 0;
+    for (const bool col : {false, true}) {  // enough for either layout
+        const int s = op_gated_splits(mode, dtype == MOE_F32 ? OT_F32 : OT_BF16, col, rows, groups, n, k, op_cus());
+        if (s > 1) bytes = std::max(bytes, (int64_t)4 * (mode == OM_GATED ? 2 : 1) * s * rows * n);
+    }
+    return bytes;
+}
+static int gated_workspace_of(const char *fn, OpMode mode, int32_t groups, int32_t rows, int32_t n, int32_t k,
+                              int32_t dtype, int64_t *bytes) {
+    if (!bytes) return op_fail(fn, "null bytes");
+    int r = op_check_groups(fn, (const int32_t *)bytes, groups, rows, n, k);
+    if (r == MOE_OK) r = op_check_dtypes(fn, dtype, MOE_F32);
+    if (r != MOE_OK) return r;
+    *bytes = gated_workspace(mode, groups, rows, n, k, dtype);
+    return MOE_OK;
+}
+// No result may share a byte with an operand or with another result.
+static int op_check_results(const char *fn, std::initializer_list<OpRegion> results,
+                            std::initializer_list<OpRegion> operands) {
+    for (const OpRegion *a = results.begin(); a != results.end(); ++a) {
+        const int r = op_check_overlap(fn, *a, operands);
+        if (r != MOE_OK) return r;
+        for (const OpRegion *b = results.begin(); b != a; ++b)
+            if (op_overlap(*a, *b)) return op_fail(fn, "results must not overlap each other");
+    }
+    return MOE_OK;
+}
+static bool op_any_misaligned(int32_t dtype, std::initializer_list<const void *> ps) {
+    for (const void *p : ps)
+        if (op_misaligned(p, dtype)) return true;
+    return false;
+}
+
+int moe_gated_matmul_workspace(int32_t groups, int32_t rows, int32_t in_dim, int32_t hidden_dim, int32_t dtype,
+                               int64_t *bytes) {
+    return gated_workspace_of("moe_gated_matmul_workspace", OM_GATED, groups, rows, hidden_dim, in_dim, dtype, bytes);
+}
+
+int moe_gated_matmul_async(const void *x, int64_t ldx, const void *w1, int64_t ldw1, int64_t w1_stride, const void *w3,
+                           int64_t ldw3, int64_t w3_stride, int32_t layout, int32_t activation, const int32_t *offsets,
+                           int32_t groups, int32_t rows, int32_t in_dim, int32_t hidden_dim, int32_t dtype, void *h,
+                           int64_t ldh, int32_t h_dtype, void *a, int64_t lda, void *b, int64_t ldb, void *workspace,
+                           int64_t workspace_bytes, void *stream) {
+    const char *fn = "moe_gated_matmul_async";
+    int r = op_check_gated(fn, offsets, groups, rows, in_dim, hidden_dim, dtype, h_dtype, layout, activation);
+    if (r != MOE_OK) return r;
+    const bool flux = layout == MOE_LAYOUT_FLUX_OUT_IN;
+    const int wcols = flux ? hidden_dim : in_dim, wrows = flux ? in_dim : hidden_dim;
+    if ((a != nullptr) != (b != nullptr)) return op_fail(fn, "a and b come together");
+    if (ldx < in_dim || ldh < hidden_dim || ldw1 < wcols || ldw3 < wcols || (a && (lda < hidden_dim || ldb < hidden_dim)))
+        return op_fail(fn, "a row stride is smaller than its row");
+    if (groups > 1 && (w1_stride < (wrows - 1) * ldw1 + wcols || w3_stride < (wrows - 1) * ldw3 + wcols))
+        return op_fail(fn, "a weight's stride is smaller than a matrix");
+    if (rows == 0) return MOE_OK;
+    if (!x || !w1 || !w3 || !h) return op_fail(fn, "null buffer");
+    if (op_any_misaligned(dtype, {x, w1, w3, a, b}) || op_misaligned(h, h_dtype))
+        return op_fail(fn, "a buffer is not aligned to its elements");
+    r = op_check_workspace(fn, gated_workspace(OM_GATED, groups, rows, hidden_dim, in_dim, dtype), workspace, workspace_bytes);
+    if (r != MOE_OK) return r;
+    const int64_t es = op_bytes(dtype);
+    r = op_check_results(fn,
+                         {OpRegion(h, hidden_dim, ldh, rows, 0, 1, op_bytes(h_dtype)), OpRegion(a, hidden_dim, lda, rows, 0, 1, es),
+                          OpRegion(b, hidden_dim, ldb, rows, 0, 1, es)},
+                         {OpRegion(x, in_dim, ldx, rows, 0, 1, es), OpRegion(w1, wcols, ldw1, wrows, w1_stride, groups, es),
+                          OpRegion(w3, wcols, ldw3, wrows, w3_stride, groups, es),
+                          OpRegion(offsets, 4 * ((int64_t)groups + 1))});
+    if (r != MOE_OK) return r;
+    OpGemmArgs g{};
+    g.A = x, g.lda = ldx;
+    g.B = w1, g.ldb = ldw1, g.b_stride = groups > 1 ? w1_stride : 0;
+    g.B2 = w3, g.ldb2 = ldw3, g.b2_stride = groups > 1 ? w3_stride : 0;
+    g.C = h, g.ldc = ldh, g.c_f32 = h_dtype == MOE_F32;
+    g.C2 = a, g.ldc2 = lda, g.C3 = b, g.ldc3 = ldb;
+    g.offsets = offsets, g.E = groups, g.rows = rows, g.N = hidden_dim, g.K = in_dim, g.act = activation;
+    const int ot = dtype == MOE_F32 ? OT_F32 : OT_BF16;
+    g.splits = op_gated_splits(OM_GATED, ot, flux, rows, groups, hidden_dim, in_dim, op_cus());
+    g.ws = (float *)workspace;
+    return op_done(fn, launch_op_gated(OM_GATED, ot, flux, g, op_cus(), (hipStream_t)stream));
+}
+
+int moe_gated_matmul_grad_workspace(int32_t groups, int32_t rows, int32_t hidden_dim, int32_t out_dim, int32_t dtype,
+                                    int64_t *bytes) {
+    return gated_workspace_of("moe_gated_matmul_grad_workspace", OM_GATE_GRAD, groups, rows, hidden_dim, out_dim, dtype, bytes);
+}
+
+int moe_gated_matmul_grad_async(const void *dy, int64_t lddy, const void *w2, int64_t ldw2, int64_t w2_stride,
+                                int32_t layout, int32_t activation, const void *a, int64_t lda, const void *b, int64_t ldb,
+                                const int32_t *offsets, int32_t groups, int32_t rows, int32_t hidden_dim, int32_t out_dim,
+                                int32_t dtype, void *da, int64_t ldda, void *db, int64_t lddb, void *h, int64_t ldh,
+                                void *workspace, int64_t workspace_bytes, void *stream) {
+    const char *fn = "moe_gated_matmul_grad_async";
+    int r = op_check_gated(fn, offsets, groups, rows, hidden_dim, out_dim, dtype, dtype, layout, activation);
+    if (r != MOE_OK) return r;
+    const bool flux = layout == MOE_LAYOUT_FLUX_OUT_IN;
+    const int wcols = flux ? out_dim : hidden_dim, wrows = flux ? hidden_dim : out_dim;
+    if (!w2 && out_dim != hidden_dim) return op_fail(fn, "without w2 dy is the gradient of h: out_dim must be hidden_dim");
+    if (lddy < out_dim || (w2 && ldw2 < wcols) || std::min({lda, ldb, ldda, lddb, ldh}) < hidden_dim)
+        return op_fail(fn, "a row stride is smaller than its row");
+    if (w2 && groups > 1 && w2_stride < (wrows - 1) * ldw2 + wcols) return op_fail(fn, "w2_stride is smaller than a matrix");
+    if (rows == 0) return MOE_OK;
+    if (!dy || !a || !b || !da || !db || !h) return op_fail(fn, "null buffer");
+    if (op_any_misaligned(dtype, {dy, w2, a, b, da, db, h})) return op_fail(fn, "a buffer is not aligned to its elements");
+    if (w2) {
+        r = op_check_workspace(fn, gated_workspace(OM_GATE_GRAD, groups, rows, hidden_dim, out_dim, dtype), workspace,
+                               workspace_bytes);
+        if (r != MOE_OK) return r;
+    }
+    const int64_t es = op_bytes(dtype);
+    auto rows_of = [&](const void *p, int64_t cols, int64_t ld) { return OpRegion(p, cols, ld, rows, 0, 1, es); };
+    r = op_check_results(fn, {rows_of(da, hidden_dim, ldda), rows_of(db, hidden_dim, lddb), rows_of(h, hidden_dim, ldh)},
+                         {rows_of(dy, out_dim, lddy), rows_of(a, hidden_dim, lda), rows_of(b, hidden_dim, ldb),
+                          OpRegion(w2, wcols, ldw2, wrows, w2_stride, groups, es),
+                          OpRegion(offsets, 4 * ((int64_t)groups + 1))});
+    if (r != MOE_OK) return r;
+    OpGemmArgs g{};
+    g.A = dy, g.lda = lddy;
+    g.B = w2, g.ldb = ldw2, g.b_stride = groups > 1 ? w2_stride : 0;
+    g.ga = a, g.ldga = lda, g.gb = b, g.ldgb = ldb;
+    g.C = da, g.ldc = ldda, g.C2 = db, g.ldc2 = lddb, g.C3 = h, g.ldc3 = ldh;
+    g.offsets = offsets, g.E = groups, g.rows = rows, g.N = hidden_dim, g.K = out_dim, g.act = activation;
+    g.c_f32 = dtype == MOE_F32, g.splits = 1;
+    const int ot = dtype == MOE_F32 ? OT_F32 : OT_BF16;
+    if (!w2) return op_done(fn, launch_op_gate_rows(ot, g, (hipStream_t)stream));
+    // dh = W2' dy: the weight's k is its out_dim, contiguous in the flux order
+    g.splits = op_gated_splits(OM_GATE_GRAD, ot, !flux, rows, groups, hidden_dim, out_dim, op_cus());
+    g.ws = (float *)workspace;
+    return op_done(fn, launch_op_gated(OM_GATE_GRAD, ot, !flux, g, op_cus(), (hipStream_t)stream));
+}
+
+int moe_gated_matmul_grad_x_workspace(int32_t groups, int32_t rows, int32_t in_dim, int32_t hidden_dim, int32_t dtype,
+                                      int64_t *bytes) {
+    return gated_workspace_of("moe_gated_matmul_grad_x_workspace", OM_TWO, groups, rows, in_dim, hidden_dim, dtype, bytes);
+}
+
+int moe_gated_matmul_grad_x_async(const void *da, int64_t ldda, const void *db, int64_t lddb, const void *w1,
+                                  int64_t ldw1, int64_t w1_stride, const void *w3, int64_t ldw3, int64_t w3_stride,
+                                  int32_t layout, const int32_t *offsets, int32_t groups, int32_t rows, int32_t in_dim,
+                                  int32_t hidden_dim, int32_t dtype, void *dx, int64_t lddx, int32_t dx_dtype,
+                                  void *workspace, int64_t workspace_bytes, void *stream) {
+    const char *fn = "moe_gated_matmul_grad_x_async";
+    int r = op_check_gated(fn, offsets, groups, rows, in_dim, hidden_dim, dtype, dx_dtype, layout, MOE_ACT_IDENTITY);
+    if (r != MOE_OK) return r;
+    const bool flux = layout == MOE_LAYOUT_FLUX_OUT_IN;
+    const int wcols = flux ? hidden_dim : in_dim, wrows = flux ? in_dim : hidden_dim;
+    if (ldda < hidden_dim || lddb < hidden_dim || lddx < in_dim || ldw1 < wcols || ldw3 < wcols)
+        return op_fail(fn, "a row stride is smaller than its row");
+    if (groups > 1 && (w1_stride < (wrows - 1) * ldw1 + wcols || w3_stride < (wrows - 1) * ldw3 + wcols))
+        return op_fail(fn, "a weight's stride is smaller than a matrix");
+    if (rows == 0) return MOE_OK;
+    if (!da || !db || !w1 || !w3 || !dx) return op_fail(fn, "null buffer");
+    if (op_any_misaligned(dtype, {da, db, w1, w3}) || op_misaligned(dx, dx_dtype))
+        return op_fail(fn, "a buffer is not aligned to its elements");
+    r = op_check_workspace(fn, gated_workspace(OM_TWO, groups, rows, in_dim, hidden_dim, dtype), workspace, workspace_bytes);
+    if (r != MOE_OK) return r;
+    const int64_t es = op_bytes(dtype);
+    r = op_check_overlap(fn, OpRegion(dx, in_dim, lddx, rows, 0, 1, op_bytes(dx_dtype)),
+                         {OpRegion(da, hidden_dim, ldda, rows, 0, 1, es), OpRegion(db, hidden_dim, lddb, rows, 0, 1, es),
+                          OpRegion(w1, wcols, ldw1, wrows, w1_stride, groups, es),
+                          OpRegion(w3, wcols, ldw3, wrows, w3_stride, groups, es),
+                          OpRegion(offsets, 4 * ((int64_t)groups + 1))});
+    if (r != MOE_OK) return r;
+    OpGemmArgs g{};
+    g.A = da, g.lda = ldda, g.A2 = db, g.lda2 = lddb;
+    g.B = w1, g.ldb = ldw1, g.b_stride = groups > 1 ? w1_stride : 0;
+    g.B2 = w3, g.ldb2 = ldw3, g.b2_stride = groups > 1 ? w3_stride : 0;
+    g.C = dx, g.ldc = lddx, g.c_f32 = dx_dtype == MOE_F32;
+    g.offsets = offsets, g.E = groups, g.rows = rows, g.N = in_dim, g.K = hidden_dim;
+    const int ot = dtype == MOE_F32 ? OT_F32 : OT_BF16;
+    g.splits = op_gated_splits(OM_TWO, ot, !flux, rows, groups, in_dim, hidden_dim, op_cus());
+    g.ws = (float *)workspace;
+    return op_done(fn, launch_op_gated(OM_TWO, ot, !flux, g, op_cus(), (hipStream_t)stream));
 }
 
 int moe_quantize_int8_async(const void *x, int64_t ldx, int32_t x_dtype, int64_t rows, int32_t cols, void *q,

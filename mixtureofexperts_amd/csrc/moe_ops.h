@@ -34,7 +34,22 @@ struct OpGemmArgs {
     float *ws;                     // partial sums (splits > 1), [range][rows][N] or [group][range][M][N]
     int splits;                    // ranges that k is split into over workgroups (1: none)
     int nt, mt;                    // tiles along N, and (ragged k) along M
+    // Gated blocks (OpMode), operand and result types as above:
+    int act;                       // MOE_ACT_*
+    const void *A2, *B2;           // the second rows, the second weight
+    long long lda2, ldb2, b2_stride;
+    const void *ga, *gb;           // OM_GATE_GRAD: the pre-activations
+    long long ldga, ldgb;
+    void *C2, *C3;                 // OM_GATED: a and b (or null); OM_GATE_GRAD: db and h
+    long long ldc2, ldc3;
 };
+
+// What a product of ragged rows computes:
+//   OM_PLAIN      C = A B'
+//   OM_GATED      a = A B', b = A B2', C = act(a) b
+//   OM_GATE_GRAD  dh = A B', C = dh gb act'(ga), C2 = dh act(ga), C3 = act(ga) gb
+//   OM_TWO        C = A B' + A2 B2'
+enum OpMode { OM_PLAIN = 0, OM_GATED = 1, OM_GATE_GRAD = 2, OM_TWO = 3 };
 
 // The rows of group e, held within [0, rows] whatever the offsets say.
 __device__ __forceinline__ void op_group(const int *offsets, int e, int rows, int &lo, int &hi) {
@@ -118,6 +133,13 @@ inline int op_matrix_splits(int ot, long long rows, long long E, long long M, lo
     return ot == OT_F32 ? op_tile_splits(tiles, rows / E, 800, 4000, ncu) : op_splits(tiles, rows / E, 512, ncu);
 }
 
+// The gated products, by the sizes of the product that they are: 2 hidden columns (two
+// weights), one product of dh, 2 hidden elements of k.  The gradients are never streamed.
+inline int op_gated_splits(OpMode mode, int ot, bool b_col, long long rows, long long E, long long N, long long K, int ncu) {
+    if (mode == OM_GATED && op_streamed(ot, b_col, rows, E, N, K, ncu)) return op_rows_splits(ot, b_col, rows, E, N, K, ncu);
+    return op_rows_splits(ot, true, rows, E, mode == OM_GATED ? 2 * N : N, mode == OM_TWO ? 2 * K : K, ncu);
+}
+
 // What a launcher answers to a call of more workgroups than one launch takes.
 constexpr hipError_t kOpTooLarge = hipErrorNotSupported;
 
@@ -130,6 +152,12 @@ hipError_t launch_op_gemm_i8(OpGemmArgs g, int ncu, hipStream_t s);
 hipError_t launch_op_stream(int ot, const OpGemmArgs &g, hipStream_t s);
 // C of a call whose k was split: its ranges' sums, in range order
 hipError_t launch_op_fold(int ot, bool ragged_k, const OpGemmArgs &g, hipStream_t s);
+
+// OM_GATED, OM_GATE_GRAD and OM_TWO
+hipError_t launch_op_gated(int mode, int ot, bool b_col, OpGemmArgs g, int ncu, hipStream_t s);
+// the results of the first two where k was split; dh given, not a product: g.A its rows
+hipError_t launch_op_gate_fold(int mode, int ot, const OpGemmArgs &g, hipStream_t s);
+hipError_t launch_op_gate_rows(int ot, const OpGemmArgs &g, hipStream_t s);
 
 // q[r][k] = rne(127 x[r][k] / max|x[r]|) as int8, scale[r] = max|x[r]| / 127;
 // columns [cols, ldq) are not written past pad_to (zeros up to it)

@@ -1,0 +1,139 @@
+// moe_ops_gate.h -- the gate of a gated feed-forward block, h = act(a) b, and
+// its gradients: da = dh b act'(a), db = dh act(a).
+//
+//   silu, gelu: act = a s, s = 1 / (1 + e^-z), z = r (a + c a^3); silu: r = 1, c = 0;
+//     gelu: r = 2 sqrt(2 / pi), c = 0.044715 (its tanh form: 0.5 (1 + tanh(z / 2)) = s);
+//     act' = s + a s (1 - s) r (1 + 3 c a^2)
+//   relu, identity: act = a, act' = 1 but where a <= floor: 0; floor = 0 or NaN
+// so that a kernel holds two forms, not four (a four-way choice by the activation
+// around a tile's results was compiled wrong: one register of 16 was left unset for
+// the identity).
+#pragma once
+#include <type_traits>
+
+#include "moe_internal.h"
+#include "moe_ops.h"
+
+namespace moe {
+namespace ops {
+
+// FAST: the hardware's exp and reciprocal, 2^-22 of the result each, where a, b and
+// dh come from bf16 operands; else expf and an IEEE division.
+template <bool FAST>
+__device__ __forceinline__ float gate_sigmoid(float z) {
+    if constexpr (FAST) return __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+    else return 1.0f / (1.0f + expf(-z));
+}
+
+struct GateValue {
+    float f, d;  // act(a), act'(a)
+};
+
+struct Gate {
+    float r, c, floor;
+    bool smooth;
+    __device__ __forceinline__ explicit Gate(int act)
+        : r(act == MOE_ACT_GELU ? 1.5957691216057308f : 1.0f), c(act == MOE_ACT_GELU ? 0.044715f : 0.0f),
+          floor(act == MOE_ACT_RELU ? 0.0f : __builtin_nanf("")), smooth(act == MOE_ACT_SILU || act == MOE_ACT_GELU) {}
+
+    template <bool SMOOTH, bool FAST>
+    __device__ __forceinline__ GateValue value(float a) const {
+        if constexpr (SMOOTH) {
+            // past |a| = 32 gelu's s is 0 or 1 in 32 bits: the powers of a stop there, where
+            // they could overflow (and 0 times infinity would be NaN)
+            const float q = __builtin_amdgcn_fmed3f(a, -32.0f, 32.0f), q2 = q * q;
+            const float s = gate_sigmoid<FAST>(r * (a + c * q2 * q)), f = a * s;
+            return {f, s + fminf(f, 3e38f) * (1.0f - s) * (r * (1.0f + 3.0f * c * q2))};
+        } else {
+            const bool zero = a <= floor;
+            return {zero ? 0.0f : a, zero ? 0.0f : 1.0f};
+        }
+    }
+};
+
+struct GateBack {
+    float da, db, h;
+};
+template <bool SMOOTH, bool FAST>
+__device__ __forceinline__ GateBack gate_back(const Gate &g, float dh, float a, float b) {
+    const GateValue v = g.value<SMOOTH, FAST>(a);
+    return {dh * b * v.d, dh * v.f, v.f * b};
+}
+
+// CE elements of a row from column n on, N its columns: 16 bytes at any alignment,
+// element by element past the end.
+template <bool BF16>
+struct GateChunk {
+    static constexpr int CE = BF16 ? 8 : 4;
+    float v[CE];
+    __device__ __forceinline__ void load(const void *row, int n, int N) {
+        if (n + CE <= N) {
+            if constexpr (BF16) {
+                uint4 u;
+                __builtin_memcpy(&u, (const uint16_t *)row + n, 16);
+                const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    v[2 * q] = __uint_as_float(w[q] << 16);
+                    v[2 * q + 1] = __uint_as_float(w[q] & 0xffff0000u);
+                }
+            } else {
+                __builtin_memcpy(v, (const float *)row + n, 16);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < CE; ++q) {
+                v[q] = 0.0f;
+                if (n + q < N) v[q] = BF16 ? bf16_to_f32(((const uint16_t *)row)[n + q]) : ((const float *)row)[n + q];
+            }
+        }
+    }
+    __device__ __forceinline__ void store(void *row, int n, int N) const {
+        if constexpr (BF16) {
+            typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+            bf16x8 o;
+#pragma unroll
+            for (int q = 0; q < CE; ++q) o[q] = (__bf16)v[q];
+            if (n + CE <= N) {
+                __builtin_memcpy((uint16_t *)row + n, &o, 16);
+            } else {
+#pragma unroll
+                for (int q = 0; q < CE; ++q)
+                    if (n + q < N) ((uint16_t *)row)[n + q] = f32_to_bf16(v[q]);
+            }
+        } else {
+            if (n + CE <= N) {
+                __builtin_memcpy((float *)row + n, v, 16);
+            } else {
+#pragma unroll
+                for (int q = 0; q < CE; ++q)
+                    if (n + q < N) ((float *)row)[n + q] = v[q];
+            }
+        }
+    }
+};
+
+// Row `row`, columns n .. n + CE - 1 of da, db and h from dh there.
+template <bool BF16>
+__device__ __forceinline__ void gate_store(const OpGemmArgs &g, long long row, int n, const GateChunk<BF16> &dh) {
+    constexpr int ES = BF16 ? 2 : 4;
+    GateChunk<BF16> a, b, da, db, h;
+    a.load((const uint8_t *)g.ga + row * g.ldga * ES, n, g.N);
+    b.load((const uint8_t *)g.gb + row * g.ldgb * ES, n, g.N);
+    const Gate gate(g.act);
+    auto all = [&](auto SMOOTH) {
+#pragma unroll
+        for (int q = 0; q < GateChunk<BF16>::CE; ++q) {
+            const GateBack r = gate_back<decltype(SMOOTH)::value, BF16>(gate, dh.v[q], a.v[q], b.v[q]);
+            da.v[q] = r.da, db.v[q] = r.db, h.v[q] = r.h;
+        }
+    };
+    if (gate.smooth) all(std::true_type{});
+    else all(std::false_type{});
+    da.store((uint8_t *)g.C + row * g.ldc * ES, n, g.N);
+    db.store((uint8_t *)g.C2 + row * g.ldc2 * ES, n, g.N);
+    h.store((uint8_t *)g.C3 + row * g.ldc3 * ES, n, g.N);
+}
+
+}  // namespace ops
+}  // namespace moe

@@ -27,6 +27,7 @@
 
 #include "moe_internal.h"
 #include "moe_ops.h"
+#include "moe_ops_gate.h"
 
 namespace moe {
 namespace ops {
@@ -209,6 +210,11 @@ struct Tile {
                 voff[j] = ok ? (unsigned)(row * (int)ldb + elem * ES) : kOutOfRange;
             }
         }
+    }
+    // the same rows, lengths and strides at another address
+    __device__ __forceinline__ void move(unsigned long long b) {
+        base_lo = __builtin_amdgcn_readfirstlane((unsigned)b);
+        base_hi = __builtin_amdgcn_readfirstlane((unsigned)(b >> 32));
     }
     // Stage s straight into the LDS image at byte offset lds (DIRECT).  Inline
     // assembly that the compiler does not see as a memory access: its wait
@@ -642,6 +648,53 @@ __device__ __forceinline__ void store_tile_rows(const OpGemmArgs &g, lds_u8 *rin
     }
 }
 
+// A tile of dh through LDS in fp32, then whole chunks of da, db and h from it and the
+// same chunks of a and b, which are read once, in rows.  LDS as in store_tile_rows.
+template <int OT, int BM, int BN, int WM, int WN, int RING, typename Val>
+__device__ __forceinline__ void gate_tile_rows(const OpGemmArgs &g, lds_u8 *ring, long long row0, int mrows, int n0,
+                                               int wm, int wn, int lane, Val val) {
+    constexpr bool BF16 = OT == OT_BF16;
+    constexpr int NT = WM * WN * 64, NJ = BN / WN / 16;
+    constexpr int CW = BN * 4, CH = CW / 16;
+    constexpr int FIT = RING / CW;
+    constexpr int PR = FIT >= BM ? BM : (FIT >= BM / 2 ? BM / 2 : BM / 4);  // rows per pass
+    constexpr int CE = GateChunk<BF16>::CE, OC = BN / CE;  // results per chunk, chunks per row
+    static_assert(PR % (WM * 16) == 0 && BM % PR == 0 && NT % OC == 0 && PR % (NT / OC) == 0 && PR <= FIT, "passes");
+    constexpr int IP = PR / (WM * 16);
+    typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+    const int r16 = lane & 15, q4 = lane >> 4;
+#pragma unroll
+    for (int p = 0; p < BM / PR; ++p) {
+        if (p * PR >= mrows) break;
+        __syncthreads();  // the ring (the previous pass) is no longer read
+#pragma unroll
+        for (int ii = 0; ii < IP; ++ii) {
+            const int i = p * IP + ii, r = (ii * WM + wm) * 16 + r16;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int c = (wn * NJ + j) * 4 + q4;
+                *(lds_f32x4 *)(ring + r * CW + ((c ^ (r & (CH - 1))) << 4)) =
+                    f32x4{val(i, j, 0), val(i, j, 1), val(i, j, 2), val(i, j, 3)};
+            }
+        }
+        __syncthreads();
+        const int oc = (int)threadIdx.x % OC, n = n0 + oc * CE;
+        const int rows = min(PR, mrows - p * PR);
+        if (n < g.N) {
+            for (int r = (int)threadIdx.x / OC; r < rows; r += NT / OC) {
+                GateChunk<BF16> dh;
+#pragma unroll
+                for (int k = 0; k < CE / 4; ++k) {
+                    const f32x4 t = *(const lds_f32x4 *)(ring + r * CW + (((oc * (CE / 4) + k) ^ (r & (CH - 1))) << 4));
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) dh.v[4 * k + q] = t[q];
+                }
+                gate_store<BF16>(g, row0 + p * PR + r, n, dh);
+            }
+        }
+    }
+}
+
 // ---- the kernel --------------------------------------------------------------------
 // Bound by the matrix units at the clock that their load leaves: 8192 rows, 8
 // bf16 experts of 4096 / 14336 in 835 to 862 us (1140 TFLOP/s, units 56 % busy; one 8192
@@ -662,19 +715,27 @@ __device__ __forceinline__ void store_tile_rows(const OpGemmArgs &g, lds_u8 *rin
 // Loads past the last stage read zeros without touching memory, which keeps
 // the count of loads in flight exact (a stage loaded by dwords counts for more
 // and is waited for earlier).
-template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int KSUB, int NS, int VB>
+//
+// OM_GATED: the two weights' tiles, BN / 2 rows each, lie side by side in the ring,
+// and a wave's two column halves are the same columns of a and of b: the gate is
+// taken in its registers.  OM_TWO: the stages of the first pair of operands, then
+// those of the second, into the same sums.
+template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int KSUB, int NS, int VB,
+          int MODE = OM_PLAIN>
 __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_) {
     constexpr int ES = op_size(OT), NT = WM * WN * 64, KE = KSUB * 64 / ES;
     constexpr int MI = BM / WM / 16, NJ = BN / WN / 16, JH = NJ / 2;
-    constexpr bool DIRECT = VB > 0;
+    constexpr bool DIRECT = VB > 0, GATED = MODE == OM_GATED, TWO = MODE == OM_TWO;
+    static_assert(MODE == OM_PLAIN || (!RAGK && OT != OT_I8), "gated: ragged rows of floats");
+    constexpr int BR = GATED ? BN / 2 : BN;  // rows of a weight in a tile: columns of its results
     using TA = Tile<ES, BM, ACOL, NT, KSUB, VB>;
-    using TB = Tile<ES, BN, BCOL, NT, KSUB, VB>;
+    using TB = Tile<ES, BR, BCOL, NT, KSUB, VB>;
 
     OpJob jb;
     if constexpr (RAGK) {
         if (!matrix_job(g, jb, BM, BN, KE)) return;
     } else {
-        if (!ragged_job<BM>(g, jb, BN)) return;
+        if (!ragged_job<BM>(g, jb, BR)) return;
     }
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -682,7 +743,16 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
 
     TA ta;
     TB tb;
+    std::conditional_t<GATED, TB, int> tb2;
     int klen;
+    // OM_TWO: stages of one pair, this range's first stage and its end, of the stages of both
+    int pair = 0, first = 0, end = 0;
+    constexpr bool MOVE = TWO && BM == 256;  // (registers for one stride only: op_gemm_plan)
+    const uint8_t *A2 = nullptr, *B2 = nullptr;
+    auto second = [&]() __attribute__((always_inline)) {  // the tiles of A2 and B2
+        ta.init(A2, g.lda2 * ES, jb.len - jb.m0, g.K);
+        tb.init(B2, g.ldb2 * ES, g.N - jb.n0, g.K);
+    };
     {
         const uint8_t *A = (const uint8_t *)g.A, *B = (const uint8_t *)g.B;
         if constexpr (RAGK) {
@@ -692,11 +762,27 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
         } else {
             static_assert(!ACOL || RAGK, "ragged rows: A is a row operand");
             int k0;
-            k_range(g, jb.ks, KE, k0, klen);
+            if constexpr (TWO) {
+                k0 = 0;
+                klen = g.K;
+                pair = (g.K + KE - 1) / KE;
+                const int per = (2 * pair + g.splits - 1) / g.splits;
+                first = __builtin_amdgcn_readfirstlane(min(jb.ks * per, 2 * pair));
+                end = __builtin_amdgcn_readfirstlane(min(first + per, 2 * pair));
+            } else {
+                k_range(g, jb.ks, KE, k0, klen);
+            }
             ta.init(A + ((long long)(jb.lo + jb.m0) * g.lda + k0) * ES, g.lda * ES, jb.len - jb.m0, klen);
             B += (long long)jb.e * g.b_stride * ES;
             tb.init(B + (BCOL ? (long long)k0 * g.ldb + jb.n0 : (long long)jb.n0 * g.ldb + k0) * ES, g.ldb * ES,
                     g.N - jb.n0, klen);
+            B2 = (const uint8_t *)g.B2 +
+                 ((long long)jb.e * g.b2_stride + (BCOL ? (long long)k0 * g.ldb2 + jb.n0 : (long long)jb.n0 * g.ldb2 + k0)) * ES;
+            if constexpr (GATED) tb2.init(B2, g.ldb2 * ES, g.N - jb.n0, klen);
+            if constexpr (TWO) {
+                A2 = (const uint8_t *)g.A2 + (long long)(jb.lo + jb.m0) * g.lda2 * ES;
+                if (DIRECT && !MOVE && first > pair) second();
+            }
         }
     }
     // int8: the scales of the tile's rows, the same in every wave, on their way under
@@ -719,16 +805,47 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
     // instruction's 16-bit offset of each other
     auto a_slot = [](auto SLOT) { return decltype(SLOT)::value * TA::BYTES; };
     auto b_slot = [](auto SLOT) { return NS * TA::BYTES + decltype(SLOT)::value * TB::BYTES; };
-    const int S = (klen + KE - 1) / KE;
+    auto b2_slot = [](auto SLOT) { return NS * (TA::BYTES + TB::BYTES) + decltype(SLOT)::value * TB::BYTES; };
+    const int S = TWO ? end - first : (klen + KE - 1) / KE;
     auto read_a = [&](auto SLOT, int i, int ks) { return TA::frag(ring + a_slot(SLOT), i * WM + wm, ks, lane); };
-    auto read_b = [&](auto SLOT, int j, int ks) { return TB::frag(ring + b_slot(SLOT), wn * NJ + j, ks, lane); };
+    auto read_b = [&](auto SLOT, int j, int ks) {
+        if constexpr (GATED) {
+            return j < JH ? TB::frag(ring + b_slot(SLOT), wn * JH + j, ks, lane)
+                          : TB::frag(ring + b2_slot(SLOT), wn * JH + j - JH, ks, lane);
+        } else {
+            return TB::frag(ring + b_slot(SLOT), wn * NJ + j, ks, lane);
+        }
+    };
+    // OM_TWO: stage s of this range as a stage of its pair (one past its last, which reads
+    // as zeros, from the range's end on)
+    auto in_pair = [&](int s) __attribute__((always_inline)) {
+        const int t = first + s;
+        if constexpr (MOVE) {
+            const unsigned long long a1 = (unsigned long long)ta.base, b1 = (unsigned long long)tb.base;
+            ta.move(t < pair ? a1 : (unsigned long long)A2);
+            tb.move(t < pair ? b1 : (unsigned long long)B2);
+        } else if constexpr (!DIRECT) {
+            const bool two = t >= pair;
+            ta.init(two ? A2 : (const uint8_t *)g.A + (long long)(jb.lo + jb.m0) * g.lda * ES, (two ? g.lda2 : g.lda) * ES,
+                    jb.len - jb.m0, g.K);
+            tb.init(two ? B2
+                        : (const uint8_t *)g.B +
+                              ((long long)jb.e * g.b_stride + (BCOL ? (long long)jb.n0 : (long long)jb.n0 * g.ldb)) * ES,
+                    (two ? g.ldb2 : g.ldb) * ES, g.N - jb.n0, g.K);
+        } else if (t == pair && t < end) {
+            second();
+        }
+        return t >= end ? pair : (t < pair ? t : t - pair);
+    };
     if (S > 0) {
         if constexpr (DIRECT) {
-            constexpr int NL = TA::NC + TB::NC;
+            constexpr int NL = TA::NC + (GATED ? 2 : 1) * TB::NC;
             const unsigned l0 = (unsigned)(uintptr_t)ring;
             auto load = [&](auto SLOT, int s) {
+                if constexpr (TWO) s = in_pair(s);
                 ta.load_lds(s, l0 + a_slot(SLOT), w);
                 tb.load_lds(s, l0 + b_slot(SLOT), w);
+                if constexpr (GATED) tb2.load_lds(s, l0 + b2_slot(SLOT), w);
             };
             load(num<0>{}, 0);
             load(num<1>{}, 1);
@@ -801,12 +918,20 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
             }
             wait_loads<0>();  // no load may still be writing LDS when the workgroup ends
         } else {
+            auto load = [&](int s) {
+                if constexpr (TWO) s = in_pair(s);
+                ta.load_regs(s);
+                tb.load_regs(s);
+                if constexpr (GATED) tb2.load_regs(s);
+            };
+            auto keep = [&](auto SLOT) {
+                ta.store_regs(ring + a_slot(SLOT));
+                tb.store_regs(ring + b_slot(SLOT));
+                if constexpr (GATED) tb2.store_regs(ring + b2_slot(SLOT));
+            };
             auto step = [&](auto SLOT, int s) {
                 lds_barrier();
-                if (s + 1 < S) {
-                    ta.load_regs(s + 1);
-                    tb.load_regs(s + 1);
-                }
+                if (s + 1 < S) load(s + 1);
 #pragma unroll
                 for (int ks = 0; ks < KSUB; ++ks) {
                     u32x4 fa[MI], fb[NJ];
@@ -819,16 +944,10 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
 #pragma unroll
                         for (int j = 0; j < NJ; ++j) acc[i][j] = fma16<OT>(fb[j], fa[i], acc[i][j]);
                 }
-                if (s + 1 < S) {
-                    using Other = num<1 - decltype(SLOT)::value>;
-                    ta.store_regs(ring + a_slot(Other{}));
-                    tb.store_regs(ring + b_slot(Other{}));
-                }
+                if (s + 1 < S) keep(num<1 - decltype(SLOT)::value>{});
             };
-            ta.load_regs(0);
-            tb.load_regs(0);
-            ta.store_regs(ring + a_slot(num<0>{}));
-            tb.store_regs(ring + b_slot(num<0>{}));
+            load(0);
+            keep(num<0>{});
             int s = 0;
             for (; s + 2 <= S; s += 2) {
                 step(num<0>{}, s);
@@ -841,16 +960,17 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
     const int r16 = lane & 15, q4 = lane >> 4;
     if constexpr (BM <= 64) {  // (split calls run the smallest tiles)
         if (g.splits > 1) {    // a range's sums, folded by op_fold_kernel
-            const long long first = RAGK ? (long long)(jb.e * g.splits + jb.ks) * g.M + jb.m0
-                                         : (long long)jb.ks * g.rows + jb.lo + jb.m0;
+            // (OM_GATED: [range][a, b][rows][N])
+            const long long row0 = RAGK ? (long long)(jb.e * g.splits + jb.ks) * g.M + jb.m0
+                                        : (long long)jb.ks * (GATED ? 2 : 1) * g.rows + jb.lo + jb.m0;
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
                 const int ml = (i * WM + wm) * 16 + r16;
                 if (ml >= mrows) continue;
-                acc_elem<OT> *ws = (acc_elem<OT> *)g.ws + (first + ml) * g.N;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
-                    const int n = jb.n0 + (wn * NJ + j) * 16 + 4 * q4;
+                    acc_elem<OT> *ws = (acc_elem<OT> *)g.ws + (row0 + (GATED && j >= JH ? g.rows : 0) + ml) * g.N;
+                    const int n = jb.n0 + (GATED ? wn * JH + j % JH : wn * NJ + j) * 16 + 4 * q4;
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
                         if (n + c < g.N) ws[n + c] = acc[i][j][c];
@@ -882,7 +1002,40 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
         for (int i = 0; i < RS; ++i) far |= RowScale(rscale[i]).back != 1.0f;
         far = __any(far);
     }
-    constexpr int RING = NS * (TA::BYTES + TB::BYTES);
+    constexpr int RING = NS * (TA::BYTES + (GATED ? 2 : 1) * TB::BYTES);
+    if constexpr (GATED) {
+        constexpr int EO = ES;  // a and b in the operands' type
+        if (g.C2) {
+            OpGemmArgs t = g;
+            t.C = g.C2, t.ldc = g.ldc2;
+            store_tile_rows<EO, BM, BR, WM, WN, RING, false>(t, ring, (long long)(jb.lo + jb.m0) * g.ldc2, mrows, jb.n0, wm,
+                                                             wn, lane, [&](int i, int j, int c) { return acc[i][j][c]; });
+            t.C = g.C3, t.ldc = g.ldc3;
+            store_tile_rows<EO, BM, BR, WM, WN, RING, false>(t, ring, (long long)(jb.lo + jb.m0) * g.ldc3, mrows, jb.n0, wm,
+                                                             wn, lane, [&](int i, int j, int c) { return acc[i][JH + j][c]; });
+        }
+        const Gate gate(g.act);
+        auto all = [&](auto SMOOTH) {
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < JH; ++j)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        acc[i][j][c] = gate.value<decltype(SMOOTH)::value, OT == OT_BF16>(acc[i][j][c]).f * acc[i][JH + j][c];
+        };
+        if (gate.smooth) all(std::true_type{});
+        else all(std::false_type{});
+        auto val = [&](int i, int j, int c) -> float { return acc[i][j][c]; };
+        if (g.c_f32) store_tile_rows<4, BM, BR, WM, WN, RING, false>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
+        else store_tile_rows<2, BM, BR, WM, WN, RING, false>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
+        return;
+    }
+    if constexpr (MODE == OM_GATE_GRAD) {
+        gate_tile_rows<OT, BM, BN, WM, WN, RING>(g, ring, jb.lo + jb.m0, mrows, jb.n0, wm, wn, lane,
+                                                 [&](int i, int j, int c) -> float { return acc[i][j][c]; });
+        return;
+    }
     auto store = [&](auto val) {
         if (g.c_f32) store_tile_rows<4, BM, BN, WM, WN, RING, RAGK>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
         else store_tile_rows<2, BM, BN, WM, WN, RING, RAGK>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
@@ -924,6 +1077,13 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WP
     op_gemm_tile<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, KSUB, NS, VB>(g, ring);
 }
 
+template <int MODE, int OT, bool BCOL, int BM, int BN, int WM, int WN, int KSUB, int NS, int WPE, int VB>
+__global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void op_gated_kernel(
+    OpGemmArgs g) {
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * (BM + BN) * 64 * KSUB];
+    op_gemm_tile<OT, false, BCOL, false, BM, BN, WM, WN, KSUB, NS, VB, MODE>(g, ring);
+}
+
 // Rows of whole, aligned pieces of `bytes`.
 inline bool whole_pieces(const void *p, long long ld, long long stride, int contiguous, int es, int bytes) {
     return (((uintptr_t)p | (uintptr_t)(ld * es) | (uintptr_t)(stride * es)) & (bytes - 1)) == 0 &&
@@ -932,9 +1092,11 @@ inline bool whole_pieces(const void *p, long long ld, long long stride, int cont
 // A tile's byte offsets (up to 255 rows) within 31 bits.
 inline bool tile_offsets_ok(long long ld, int es) { return ld * es < (1ll << 22); }
 
-template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int KSUB, int NS, int WPE>
+template <int OT, bool ACOL, bool BCOL, bool RAGK, int BM, int BN, int WM, int WN, int KSUB, int NS, int WPE,
+          int MODE = OM_PLAIN>
 hipError_t launch_tiles(OpGemmArgs g, int vb, hipStream_t s) {
-    g.nt = (g.N + BN - 1) / BN;
+    constexpr int BC = MODE == OM_GATED ? BN / 2 : BN;  // result columns of a tile
+    g.nt = (g.N + BC - 1) / BC;
     g.mt = RAGK ? (g.M + BM - 1) / BM : 0;
     // ragged rows: sum of ceil(rows_e / BM) <= rows / BM + the groups that can hold a row
     // ragged k: every XCD's part of every group
@@ -946,7 +1108,11 @@ hipError_t launch_tiles(OpGemmArgs g, int vb, hipStream_t s) {
     // (bf16 pairs by dwords: the registers of three waves per SIMD are too few)
     constexpr int W4 = WPE == 3 && BM == 128 && OT == OT_BF16 ? 2 : WPE;
 #define MOE_OP_TILES(KS_, NS_, VB_)                                                                       \
-    op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, KS_, NS_, VB_ == 4 ? W4 : WPE, VB_><<<(unsigned)grid, b, 0, \
+    if constexpr (MODE != OM_PLAIN)                                                                               \
+        op_gated_kernel<MODE, OT, BCOL, BM, BN, WM, WN, KS_, NS_, VB_ == 4 ? W4 : WPE, VB_>                       \
+            <<<(unsigned)grid, b, 0, s>>>(g);                                                                     \
+    else                                                                                                          \
+        op_gemm_kernel<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, KS_, NS_, VB_ == 4 ? W4 : WPE, VB_><<<(unsigned)grid, b, 0, \
                                                                                               s>>>(g)
     if (vb == 16) {
         MOE_OP_TILES(KSUB, NS, 16);
@@ -956,7 +1122,7 @@ hipError_t launch_tiles(OpGemmArgs g, int vb, hipStream_t s) {
         MOE_OP_TILES(KSUB, NS, 4);
     } else if constexpr (OT == OT_F32) {
         if constexpr (BM == 64) {
-            MOE_OP_TILES(1, 2, 0);  // row strides of 4 MB and more
+            MOE_OP_TILES((MODE == OM_GATED ? 2 : 1), 2, 0);  // row strides of 4 MB and more
         } else {
             return hipErrorInvalidValue;
         }
@@ -965,7 +1131,9 @@ hipError_t launch_tiles(OpGemmArgs g, int vb, hipStream_t s) {
     }
 #undef MOE_OP_TILES
     const hipError_t e = hipGetLastError();
-    return e == hipSuccess && g.splits > 1 ? launch_op_fold(OT, RAGK, g, s) : e;
+    if (e != hipSuccess || g.splits <= 1) return e;
+    if constexpr (MODE == OM_GATED || MODE == OM_GATE_GRAD) return launch_op_gate_fold(MODE, OT, g, s);
+    else return launch_op_fold(OT, RAGK, g, s);
 }
 
 // Tile and load form of a call.  256 x 256 tiles where there are two rounds of
@@ -976,7 +1144,7 @@ hipError_t launch_tiles(OpGemmArgs g, int vb, hipStream_t s) {
 // gradient of 64 Zipf groups of 2048 / 1408, 256 x 256 against 128 x 128 with three
 // workgroups per CU: 411 / 453 us.  Where even 64 x 64 tiles are few, k is split into
 // ranges (op_rows_splits, op_matrix_splits).
-template <int OT, bool ACOL, bool BCOL, bool RAGK>
+template <int OT, bool ACOL, bool BCOL, bool RAGK, int MODE = OM_PLAIN>
 hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
     constexpr int ES = op_size(OT);
     // row operands are loaded in whole 128-byte lines
@@ -985,26 +1153,35 @@ hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
     int vb = 0;
     if (tile_offsets_ok(g.lda, ES) && tile_offsets_ok(g.ldb, ES)) {
         auto pieces = [&](int bytes) {
-            return whole_pieces(g.A, g.lda, 0, ACOL ? g.M : g.K, ES, bytes) &&
-                   whole_pieces(g.B, g.ldb, g.b_stride, BCOL ? g.N : g.K, ES, bytes);
+            bool ok = whole_pieces(g.A, g.lda, 0, ACOL ? g.M : g.K, ES, bytes) &&
+                      whole_pieces(g.B, g.ldb, g.b_stride, BCOL ? g.N : g.K, ES, bytes);
+            if (MODE == OM_TWO) ok = ok && whole_pieces(g.A2, g.lda2, 0, g.K, ES, bytes);
+            if (MODE == OM_TWO || MODE == OM_GATED)
+                ok = ok && whole_pieces(g.B2, g.ldb2, g.b2_stride, BCOL ? g.N : g.K, ES, bytes);
+            return ok;
         };
-        if (pieces(16)) vb = 16;
-        else if (g.lda >= 16 / ES && g.ldb >= 16 / ES && pieces(4)) vb = 4;
+        const bool near2 = (MODE != OM_TWO || tile_offsets_ok(g.lda2, ES)) &&
+                           ((MODE != OM_TWO && MODE != OM_GATED) || tile_offsets_ok(g.ldb2, ES));
+        const bool wide2 = (MODE != OM_TWO || g.lda2 >= 16 / ES) && ((MODE != OM_TWO && MODE != OM_GATED) || g.ldb2 >= 16 / ES);
+        if (near2 && pieces(16)) vb = 16;
+        else if (near2 && wide2 && g.lda >= 16 / ES && g.ldb >= 16 / ES && pieces(4)) vb = 4;
     }
+    const long long NN = MODE == OM_GATED ? 2ll * g.N : g.N;  // columns of products
     auto tiles = [&](int b) -> long long {
-        const long long nt = (g.N + b - 1) / b;
+        const long long nt = (NN + b - 1) / b;
         if (RAGK) return nt * ((g.M + b - 1) / b) * g.E;
         const long long few = (long long)g.rows / b > g.E ? (long long)g.rows / b : (g.E < g.rows ? g.E : g.rows);
         return nt * few;
     };
     const long long avg = RAGK ? g.M : (long long)g.rows / g.E;
-    if (g.splits > 1) return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, KSUB, 4 / KSUB, 3>(g, vb, s);
+    if (g.splits > 1) return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, KSUB, 4 / KSUB, 3, MODE>(g, vb, s);
     if constexpr (OT != OT_F32) {
-        const bool large = RAGK ? tiles(256) >= 2 * ncu : avg >= 192 && g.N >= 192 && tiles(256) >= 2 * ncu;
-        if (vb == 16 && large)
-            return launch_tiles<OT, ACOL, BCOL, RAGK, 256, 256, 4, 2, KSUB, 4 / KSUB, 2>(g, vb, s);
+        const bool large = RAGK ? tiles(256) >= 2 * ncu : avg >= 192 && NN >= 192 && tiles(256) >= 2 * ncu;
+        const bool one_ld = MODE != OM_TWO || (g.lda == g.lda2 && g.ldb == g.ldb2);
+        if (vb == 16 && large && one_ld)
+            return launch_tiles<OT, ACOL, BCOL, RAGK, 256, 256, 4, 2, KSUB, 4 / KSUB, 2, MODE>(g, vb, s);
     }
-    bool medium = avg >= 64 && g.N >= 64 && tiles(128) >= ncu;
+    bool medium = avg >= 64 && NN >= 64 && tiles(128) >= ncu;
     if constexpr (OT == OT_F32) {
         // fp32 is bound by its matrix rate: the CU with the most tiles decides, a 128 x 128
         // tile taking as long as 3.8 of 64 x 64 (weight gradient, whose stores it spares:
@@ -1013,7 +1190,7 @@ hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
         // 545, 44114 rows 2240 / 192 409 / 326; weight gradients of 4096 cubed 957 / 1009, 12 groups
         // of 259 rows 1001 / 2731 164 / 194, 3 of 1325 rows 12810 / 69 176 / 135.
         auto per_cu = [&](int b) -> long long {
-            const long long nt = (g.N + b - 1) / b;
+            const long long nt = (NN + b - 1) / b;
             const long long mt = RAGK ? (g.M + b - 1) / b * (long long)g.E
                                       : (g.E > 1 ? g.rows / b + (g.E < g.rows ? g.E : g.rows) / 2 + 1 : (g.rows + b - 1) / b);
             return (nt * mt + ncu - 1) / ncu;
@@ -1024,8 +1201,8 @@ hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
         else if (!RAGK || g.rows >= 64ll * g.E) medium = (RAGK ? 34 : 38) * per_cu(128) < 10 * per_cu(64);
     }
     if (medium)
-        return launch_tiles<OT, ACOL, BCOL, RAGK, 128, 128, 2, 2, KSUB, RAGK ? 3 : 4 / KSUB, RAGK ? 3 : 2>(g, vb, s);
-    return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, KSUB, 4 / KSUB, 3>(g, vb, s);
+        return launch_tiles<OT, ACOL, BCOL, RAGK, 128, 128, 2, 2, KSUB, RAGK ? 3 : 4 / KSUB, RAGK ? 3 : 2, MODE>(g, vb, s);
+    return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, KSUB, 4 / KSUB, 3, MODE>(g, vb, s);
 }
 
 }  // namespace ops

@@ -110,14 +110,10 @@ __device__ __forceinline__ void stream_rows(const OpGemmArgs &g, int e, int n0, 
     __syncthreads();
 }
 
-template <int OT>
-__global__ __launch_bounds__(kStreamWaves * 64) void op_stream_kernel(OpGemmArgs g) {
-    __shared__ __attribute__((aligned(16))) uint8_t red_[kStreamWaves * 4 * 64 * 16];
-    lds_u8 *red = (lds_u8 *)red_;
-    // workgroup (r, n): the r-th group that holds rows, 16 columns
-    int r = blockIdx.x / g.nt;
-    const int n0 = (blockIdx.x - r * g.nt) * 16, lane = threadIdx.x & 63;
-    int e = -1, lo = 0, hi = 0;
+// The r-th group that holds rows, with them; e < 0: there are fewer.
+__device__ __forceinline__ void held_group(const OpGemmArgs &g, int r, int &e, int &lo, int &hi) {
+    const int lane = threadIdx.x & 63;
+    e = -1, lo = 0, hi = 0;
     for (int base = 0; base < g.E && e < 0; base += 64) {
         int a = 0, b = 0;
         if (base + lane < g.E) op_group(g.offsets, base + lane, g.rows, a, b);
@@ -135,6 +131,16 @@ __global__ __launch_bounds__(kStreamWaves * 64) void op_stream_kernel(OpGemmArgs
     e = __builtin_amdgcn_readfirstlane(e);
     lo = __builtin_amdgcn_readfirstlane(lo);
     hi = __builtin_amdgcn_readfirstlane(hi);
+}
+
+template <int OT>
+__global__ __launch_bounds__(kStreamWaves * 64) void op_stream_kernel(OpGemmArgs g) {
+    __shared__ __attribute__((aligned(16))) uint8_t red_[kStreamWaves * 4 * 64 * 16];
+    lds_u8 *red = (lds_u8 *)red_;
+    // workgroup (r, n): the r-th group that holds rows, 16 columns
+    const int r = blockIdx.x / g.nt, n0 = (blockIdx.x - r * g.nt) * 16;
+    int e, lo, hi;
+    held_group(g, r, e, lo, hi);
     if (e < 0) return;
     while (lo < hi) {
         const int rows = min(hi - lo, 64);

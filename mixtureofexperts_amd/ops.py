@@ -31,6 +31,7 @@ import ctypes
 
 from . import _lib
 from ._lib import MOE_EINVAL, MOE_LAYOUT_FLUX_OUT_IN, MOE_LAYOUT_LLAMA_IN_OUT
+from .activations import activation_code, silu
 
 _torch = _forward_ad = _grad_enabled = _written = None
 _codes = {}
@@ -269,6 +270,146 @@ def grouped_matmul_grad_w(x, dy, offsets=None, *, layout=MOE_LAYOUT_LLAMA_IN_OUT
     _call(L.moe_grouped_matmul_grad_w_async, device, xp, ldx, dp, lddy, layout, _offsets(offsets, E), E, x.shape[0],
           x.shape[1], dy.shape[1], _codes[x.dtype], out.data_ptr(), ldw, stride, _codes[out.dtype], int(accumulate),
           wsp, wsn)
+    if given is not None:
+        _written(out)  # autograd sees the caller's tensor change
+    return out
+
+
+def _results(out, names, shape, dtypes, allowed, like, clear):
+    """The caller's tensors `out` (None: new ones) for the results `names`, checked."""
+    if out is None:
+        return tuple(_result(None, shape, t, a, like, clear) for t, a in zip(dtypes, allowed))
+    if not isinstance(out, (tuple, list)) or len(out) != len(names):
+        _bad(f"out must be ({', '.join(names)})")
+    for t, name, dtype, a in zip(out, names, dtypes, allowed):
+        _tensor(t, name, a, (2,))
+        if t.shape != shape:
+            _bad(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+        if dtype is not None and t.dtype != dtype:
+            _bad("out and out_dtype differ")
+    return tuple(out)
+
+
+def _two_weights(w1, w3, dtype):
+    """w1 and w3 of one shape: (E, a, b), (pointer, row stride, matrix stride) of each."""
+    E, a, b, ld1, s1 = _matrices(w1, "w1", (dtype,))
+    E3, a3, b3, ld3, s3 = _matrices(w3, "w3", (dtype,))
+    if (E3, a3, b3) != (E, a, b):
+        _bad(f"w1 and w3 must have one shape, got {tuple(w1.shape)} and {tuple(w3.shape)}")
+    return E, a, b, (w1.data_ptr(), ld1, s1, w3.data_ptr(), ld3, s3)
+
+
+def gated_matmul(x, w1, w3, offsets=None, *, activation=silu, layout=MOE_LAYOUT_LLAMA_IN_OUT, out=None, out_dtype=None,
+                 save=False):
+    """The two projections of a gated feed-forward block, its activation and the
+    product in one kernel: h[r] = act(a[r]) * b[r], a[r] = W1_e x[r], b[r] = W3_e x[r]
+    for the rows r of expert e.  x (M, in) float32 or bfloat16, w1 and w3 of the
+    same type; activation silu, gelu (tanh form), relu or identity; sums and gate in
+    float32; h in x's type or, for bfloat16, ``out_dtype=torch.float32``.  With
+    ``save`` (h, a, b), a and b in x's type, as gated_matmul_grad takes them; ``out``
+    is then a tuple of the three.  Without ``out`` rows outside every group are
+    zeros."""
+    given = out
+    _plain("x w1 w3 out out out", x, w1, w3, *(out if isinstance(out, (tuple, list)) else (out,)))
+    act = activation_code(activation)
+    xp, ldx = _rows(x, "x", _floats)
+    E, a, b, w = _two_weights(w1, w3, x.dtype)
+    k, n = (a, b) if _layout(layout) else (b, a)
+    if x.shape[1] != k:
+        _bad(f"x has {x.shape[1]} columns, the weights take {k}")
+    M, dt, shape = x.shape[0], _codes[x.dtype], (x.shape[0], n)
+    if out is None and out_dtype is None:
+        out_dtype = x.dtype
+    kept = (x.dtype,)
+    if save:
+        res = _results(out, ("h", "a", "b"), shape, (out_dtype, x.dtype, x.dtype), (_float_types(x.dtype), kept, kept), x,
+                       offsets is not None)
+    else:
+        res = (_result(out, shape, out_dtype, _float_types(x.dtype), x, offsets is not None),)
+    device = _same_device(x, w1, w3, offsets, *res)
+    ws, wsp, wsn = _workspace(_lib.lib().moe_gated_matmul_workspace, device, E, M, k, n, dt)
+    pre = [v for t, name in zip(res[1:], "ab") for v in (t.data_ptr(), _row_stride(t, name))] or [None, 0, None, 0]
+    _call(_lib.lib().moe_gated_matmul_async, device, xp, ldx, *w, layout, act, _offsets(offsets, E), E, M, k, n, dt,
+          res[0].data_ptr(), _row_stride(res[0], "out"), _codes[res[0].dtype], *pre, wsp, wsn)
+    if given is not None:
+        for t in res:
+            _written(t)  # autograd sees the caller's tensors change
+    return res if save else res[0]
+
+
+def gated_matmul_grad(dy, a, b, w2=None, offsets=None, *, activation=silu, layout=MOE_LAYOUT_LLAMA_IN_OUT, out=None):
+    """The gradients of a gated block y[r] = W2_e h[r], h = act(a) * b with respect to
+    a and b, from dy (M, out) and what gated_matmul saved:
+
+        dh = W2' dy,  da = dh * b * act'(a),  db = dh * act(a)
+
+    Returns (da, db, h), all in dy's type: h is formed again for the gradient of W2.
+    dh stays in float32 and is not stored.  w2 (E, out, hidden) in ``layout``; without
+    it dy is dh itself (M, hidden).  The rest of the backward pass: dx is
+    gated_matmul_grad_x(da, db, w1, w3, ...), the gradients of w1, w3 and w2 are
+    grouped_matmul_grad_w of (x, da), (x, db) and (h, dy).  ``out`` is a tuple (da, db,
+    h); without it rows outside every group are zeros."""
+    given = out
+    _plain("dy a b w2 out out out", dy, a, b, w2, *(out if isinstance(out, (tuple, list)) else (out,)))
+    act = activation_code(activation)
+    dp, lddy = _rows(dy, "dy", _floats)
+    kept = (dy.dtype,)
+    ap, lda = _rows(a, "a", kept)
+    bp, ldb = _rows(b, "b", kept)
+    M, n = a.shape
+    if b.shape != a.shape or dy.shape[0] != M:
+        _bad("a and b must have one shape, and dy their rows")
+    if w2 is None:
+        _layout(layout)
+        E = 1 if offsets is None else _tensor(offsets, "offsets", (_torch.int32,), (1,)).shape[0] - 1
+        if E < 1:
+            _bad("offsets must hold at least two row numbers")
+        k, w = n, (None, 0, 0)
+    else:
+        E, p, q, ldw, stride = _matrices(w2, "w2", kept)
+        hidden, k = (p, q) if _layout(layout) else (q, p)
+        if hidden != n:
+            _bad(f"a has {n} columns, w2 takes {hidden}")
+        w = (w2.data_ptr(), ldw, stride)
+    if dy.shape[1] != k:
+        _bad(f"dy has {dy.shape[1]} columns, " + (f"w2 gives {k}" if w2 is not None else f"without w2 it is dh, of {n}"))
+    dt = _codes[dy.dtype]
+    res = _results(out, ("da", "db", "h"), a.shape, (dy.dtype,) * 3, (kept,) * 3, a, offsets is not None)
+    device = _same_device(dy, a, b, w2, offsets, *res)
+    ws, wsp, wsn = None, None, 0
+    if w2 is not None:
+        ws, wsp, wsn = _workspace(_lib.lib().moe_gated_matmul_grad_workspace, device, E, M, n, k, dt)
+    to = [v for t, name in zip(res, ("da", "db", "h")) for v in (t.data_ptr(), _row_stride(t, name))]
+    _call(_lib.lib().moe_gated_matmul_grad_async, device, dp, lddy, *w, layout, act, ap, lda, bp, ldb, _offsets(offsets, E),
+          E, M, n, k, dt, *to, wsp, wsn)
+    if given is not None:
+        for t in res:
+            _written(t)  # autograd sees the caller's tensors change
+    return res
+
+
+def gated_matmul_grad_x(da, db, w1, w3, offsets=None, *, layout=MOE_LAYOUT_LLAMA_IN_OUT, out=None, out_dtype=None):
+    """The gradient of gated_matmul with respect to x, both projections in one sum:
+    dx[r] = W1_e' da[r] + W3_e' db[r]; da and db (M, hidden) of the weights' type, the
+    result as grouped_matmul's."""
+    _plain("da db w1 w3 out", da, db, w1, w3, out)
+    ap, lda = _rows(da, "da", _floats)
+    bp, ldb = _rows(db, "db", (da.dtype,))
+    if db.shape != da.shape:
+        _bad("da and db must have one shape")
+    E, a, b, w = _two_weights(w1, w3, da.dtype)
+    k, n = (a, b) if _layout(layout) else (b, a)
+    if da.shape[1] != n:
+        _bad(f"da has {da.shape[1]} columns, the weights give {n}")
+    M, dt = da.shape[0], _codes[da.dtype]
+    if out is None and out_dtype is None:
+        out_dtype = da.dtype
+    given = out
+    out = _result(out, (M, k), out_dtype, _float_types(da.dtype), da, offsets is not None)
+    device = _same_device(da, db, w1, w3, offsets, out)
+    ws, wsp, wsn = _workspace(_lib.lib().moe_gated_matmul_grad_x_workspace, device, E, M, k, n, dt)
+    _call(_lib.lib().moe_gated_matmul_grad_x_async, device, ap, lda, bp, ldb, *w, layout, _offsets(offsets, E), E, M, k, n, dt,
+          out.data_ptr(), _row_stride(out, "out"), _codes[out.dtype], wsp, wsn)
     if given is not None:
         _written(out)  # autograd sees the caller's tensor change
     return out
