@@ -514,6 +514,35 @@ int moe_int8_matmul_async(const void *x, int64_t ldx, int32_t x_dtype, const flo
                           int32_t rows, int32_t in_dim, int32_t out_dim, void *y, int64_t ldy, int32_t y_dtype,
                           void *workspace, int64_t workspace_bytes, void *stream);
 
+/* 8-bit floating point (e4m3: 3 bits of fraction, 448 at most) with a scale for each
+ * block of block_rows x 128 elements of a matrix (1: each row's; 128; blocks at the end
+ * may be smaller): scale = max|block| / 448, q = 448 x / max|block| rounded to nearest
+ * even, exactly.  A block of zeros has scale 0 and codes 0; one that holds an infinity
+ * or a NaN has scale NaN and codes 0.  x [matrices][rows][cols] MOE_F32 or MOE_BF16, rows
+ * ldx and matrices x_stride elements apart; q likewise; scale
+ * [matrices][ceil(rows / block_rows)][ceil(cols / 128)], dense.  A matrix' blocks of 128 x 128
+ * are those of its transpose. */
+int moe_quantize_fp8_async(const void *x, int64_t ldx, int64_t x_stride, int32_t x_dtype, int64_t matrices, int64_t rows,
+                           int32_t cols, int32_t block_rows, void *q, int64_t ldq, int64_t q_stride, float *scale,
+                           void *stream);
+/* y[r][n] = sum over k of (q[r][k] x_scale[r][k / 128]) (w[e][n][k] w_scale[e][n / 128][k / 128])
+ * for the rows r of group e: the codes' products of a block summed in fp32, times
+ * both scales, the blocks summed in fp32 (few rows, or scales whose products leave
+ * fp32's normal range: in fp64).  x_dtype MOE_FP8_E4M3: x holds the codes and x_scale
+ * [rows][ceil(in_dim / 128)] their scales, dense.  MOE_BF16 or MOE_F32: the rows are
+ * quantised as moe_quantize_fp8_async does with block_rows 1, into the workspace, and
+ * x_scale is not read.  w: codes [groups][out_dim][in_dim], w_scale
+ * [groups][ceil(out_dim / 128)][ceil(in_dim / 128)], dense (block_rows 128); y MOE_F32 or
+ * MOE_BF16.  workspace: 16-byte aligned, the bytes that moe_fp8_matmul_workspace gives
+ * for these sizes.  The gradient with respect to x is the same product of dy with the
+ * transposed codes and scales. */
+int moe_fp8_matmul_workspace(int32_t groups, int32_t rows, int32_t in_dim, int32_t out_dim, int32_t x_dtype,
+                             int64_t *bytes);
+int moe_fp8_matmul_async(const void *x, int64_t ldx, int32_t x_dtype, const float *x_scale, const void *w, int64_t ldw,
+                         int64_t w_stride, const float *w_scale, const int32_t *offsets, int32_t groups, int32_t rows,
+                         int32_t in_dim, int32_t out_dim, void *y, int64_t ldy, int32_t y_dtype, void *workspace,
+                         int64_t workspace_bytes, void *stream);
+
 /* The norms before and after a block, its gate and the residual, in one pass:
  *   z = y .* rstd(y) .* post_weight     (post_weight NULL: z = y)
  *   r = alpha x + beta gate .* z        (gate NULL: 1; y NULL: r = alpha x)

@@ -46,7 +46,8 @@ EXPORTED_SYMBOLS = [
     "moe_grouped_matmul_grad_w_workspace", "moe_gated_matmul_workspace", "moe_gated_matmul_async",
     "moe_gated_matmul_grad_workspace", "moe_gated_matmul_grad_async", "moe_gated_matmul_grad_x_workspace",
     "moe_gated_matmul_grad_x_async", "moe_quantize_int8_async", "moe_int8_matmul_async",
-    "moe_int8_matmul_workspace", "moe_block_norm_async", "moe_block_norm_grad_async", "moe_block_norm_grad_workspace",
+    "moe_int8_matmul_workspace", "moe_quantize_fp8_async", "moe_fp8_matmul_workspace", "moe_fp8_matmul_async",
+    "moe_block_norm_async", "moe_block_norm_grad_async", "moe_block_norm_grad_workspace",
 ]
 
 
@@ -177,6 +178,9 @@ def lib():
     L.moe_int8_matmul_workspace.argtypes = [i32, i32, i32, i32, i32, i64p]
     L.moe_int8_matmul_async.argtypes = [vp, i64, i32, vp, vp, i64, i64, vp, vp, i32, i32, i32, i32, vp, i64, i32, vp,
                                         i64, vp]
+    L.moe_quantize_fp8_async.argtypes = [vp, i64, i64, i32, i64, i64, i32, i32, vp, i64, i64, vp, vp]
+    L.moe_fp8_matmul_workspace.argtypes = L.moe_int8_matmul_workspace.argtypes
+    L.moe_fp8_matmul_async.argtypes = L.moe_int8_matmul_async.argtypes
     L.moe_block_norm_async.argtypes = [vp, i32, vp, i32, vp, vp, i32, vp, i32, i64, f32, f32, f32, i64, i32, vp, vp,
                                        i32, vp, vp]
     L.moe_block_norm_grad_workspace.argtypes = [i64, i32, i64, i64p]

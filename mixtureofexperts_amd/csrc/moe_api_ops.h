@@ -515,6 +515,103 @@ int moe_int8_matmul_async(const void *x, int64_t ldx, int32_t x_dtype, const flo
     return op_done(fn, launch_op_gemm_i8(g, op_cus(), (hipStream_t)stream));
 }
 
+// ---- 8-bit floating point ------------------------------------------------------------
+int moe_quantize_fp8_async(const void *x, int64_t ldx, int64_t x_stride, int32_t x_dtype, int64_t matrices, int64_t rows,
+                           int32_t cols, int32_t block_rows, void *q, int64_t ldq, int64_t q_stride, float *scale,
+                           void *stream) {
+    const char *fn = "moe_quantize_fp8_async";
+    if (x_dtype != MOE_F32 && x_dtype != MOE_BF16) return op_fail(fn, "x_dtype must be MOE_F32 or MOE_BF16");
+    if (block_rows != 1 && block_rows != kF8Block) return op_fail(fn, "block_rows must be 1 or 128");
+    if (matrices < 0 || rows < 0 || cols < 1) return op_fail(fn, "matrices and rows must not be negative and cols positive");
+    if (matrices > kOpMaxSize || rows > kOpMaxSize || cols > kOpMaxSize) return op_fail(fn, "sizes above 2^30");
+    if (ldx < cols || ldq < cols) return op_fail(fn, "a row stride is smaller than its row");
+    if (matrices > 1 && (x_stride < (rows - 1) * ldx + cols || q_stride < (rows - 1) * ldq + cols))
+        return op_fail(fn, "a matrix stride is smaller than a matrix");
+    if (matrices == 0 || rows == 0) return MOE_OK;
+    if (!x || !q || !scale) return op_fail(fn, "null buffer");
+    if (op_misaligned(x, x_dtype) || op_misaligned(scale, MOE_F32))
+        return op_fail(fn, "a buffer is not aligned to its elements");
+    const int64_t scales = matrices * ((rows + block_rows - 1) / block_rows) * ((cols + kF8Block - 1) / kF8Block);
+    const OpRegion from(x, cols, ldx, rows, x_stride, matrices, op_bytes(x_dtype));
+    const int r = op_check_results(fn, {OpRegion(q, cols, ldq, rows, q_stride, matrices, 1), OpRegion(scale, 4 * scales)}, {from});
+    if (r != MOE_OK) return r;
+    const QuantF8Args a{x, ldx, matrices > 1 ? x_stride : 0, x_dtype == MOE_BF16, matrices, rows, cols, block_rows,
+                        (uint8_t *)q, ldq, matrices > 1 ? q_stride : 0, cols, scale};
+    return op_done(fn, launch_quantize_f8(a, (hipStream_t)stream));
+}
+
+// Workspace of the product: partial sums, then the rows' scales and codes (padded to 16
+// bytes) where the call quantises them.
+static int64_t fp8_partial_bytes(int32_t groups, int32_t rows, int32_t in_dim, int32_t out_dim) {
+    const int s = op_rows_splits(OT_F8, false, rows, groups, out_dim, in_dim, op_cus());
+    return s > 1 ? round_up((int64_t)4 * s * rows * out_dim, 16) : 0;
+}
+static int64_t fp8_blocks(int64_t n) { return (n + kF8Block - 1) / kF8Block; }
+
+int moe_fp8_matmul_workspace(int32_t groups, int32_t rows, int32_t in_dim, int32_t out_dim, int32_t x_dtype,
+                             int64_t *bytes) {
+    const char *fn = "moe_fp8_matmul_workspace";
+    if (!bytes) return op_fail(fn, "null bytes");
+    const int r = op_check_groups(fn, (const int32_t *)bytes, groups, rows, in_dim, out_dim);
+    if (r != MOE_OK) return r;
+    *bytes = rows > 0 ? fp8_partial_bytes(groups, rows, in_dim, out_dim) : 0;
+    if (x_dtype != MOE_FP8_E4M3)
+        *bytes += round_up((int64_t)rows * fp8_blocks(in_dim) * 4, 16) + (int64_t)rows * round_up((int64_t)in_dim, 16);
+    return MOE_OK;
+}
+
+int moe_fp8_matmul_async(const void *x, int64_t ldx, int32_t x_dtype, const float *x_scale, const void *w, int64_t ldw,
+                         int64_t w_stride, const float *w_scale, const int32_t *offsets, int32_t groups, int32_t rows,
+                         int32_t in_dim, int32_t out_dim, void *y, int64_t ldy, int32_t y_dtype, void *workspace,
+                         int64_t workspace_bytes, void *stream) {
+    const char *fn = "moe_fp8_matmul_async";
+    int r = op_check_groups(fn, offsets, groups, rows, in_dim, out_dim);
+    if (r != MOE_OK) return r;
+    const bool codes = x_dtype == MOE_FP8_E4M3;
+    if (!codes && x_dtype != MOE_F32 && x_dtype != MOE_BF16)
+        return op_fail(fn, "x_dtype must be MOE_FP8_E4M3, MOE_BF16 or MOE_F32");
+    if (y_dtype != MOE_F32 && y_dtype != MOE_BF16) return op_fail(fn, "the result must be MOE_F32 or MOE_BF16");
+    if (ldx < in_dim || ldy < out_dim || ldw < in_dim) return op_fail(fn, "a row stride is smaller than its row");
+    if (groups > 1 && w_stride < (out_dim - 1) * ldw + in_dim) return op_fail(fn, "w_stride is smaller than a matrix");
+    if (rows == 0) return MOE_OK;
+    if (!x || !w || !w_scale || !y) return op_fail(fn, "null buffer");
+    if (codes && !x_scale) return op_fail(fn, "coded rows need x_scale");
+    if ((!codes && op_misaligned(x, x_dtype)) || op_misaligned(y, y_dtype) || op_misaligned(w_scale, MOE_F32) ||
+        (codes && op_misaligned(x_scale, MOE_F32)))
+        return op_fail(fn, "a buffer is not aligned to its elements");
+    int64_t need = 0;
+    r = moe_fp8_matmul_workspace(groups, rows, in_dim, out_dim, x_dtype, &need);
+    if (r == MOE_OK) r = op_check_workspace(fn, need, workspace, workspace_bytes);
+    if (r != MOE_OK) return r;
+    const int64_t kb = fp8_blocks(in_dim);
+    r = op_check_overlap(fn, OpRegion(y, out_dim, ldy, rows, 0, 1, op_bytes(y_dtype)),
+                         {OpRegion(x, in_dim, ldx, rows, 0, 1, op_bytes(x_dtype)),
+                          OpRegion(w, in_dim, ldw, out_dim, w_stride, groups, 1),
+                          OpRegion(codes ? x_scale : nullptr, 4 * (int64_t)rows * kb),
+                          OpRegion(w_scale, 4 * (int64_t)groups * fp8_blocks(out_dim) * kb),
+                          OpRegion(offsets, 4 * ((int64_t)groups + 1))});
+    if (r != MOE_OK) return r;
+    if (!codes) {
+        float *sx = (float *)((uint8_t *)workspace + fp8_partial_bytes(groups, rows, in_dim, out_dim));
+        uint8_t *q = (uint8_t *)sx + round_up((int64_t)rows * kb * 4, 16);
+        const int64_t ldq = round_up((int64_t)in_dim, 16);
+        const QuantF8Args a{x, ldx, 0, x_dtype == MOE_BF16, 1, rows, in_dim, 1, q, ldq, 0, (int)ldq, sx};
+        r = op_done(fn, launch_quantize_f8(a, (hipStream_t)stream));
+        if (r != MOE_OK) return r;
+        x = q, ldx = ldq, x_scale = sx;
+    }
+    OpGemmArgs g{};
+    g.A = x, g.B = w, g.C = y;
+    g.lda = ldx, g.ldb = ldw, g.ldc = ldy;
+    g.b_stride = groups > 1 ? w_stride : 0;
+    g.offsets = offsets, g.E = groups, g.rows = rows;
+    g.N = out_dim, g.K = in_dim, g.c_f32 = y_dtype == MOE_F32;
+    g.splits = op_rows_splits(OT_F8, false, rows, groups, out_dim, in_dim, op_cus());
+    g.ws = (float *)workspace;
+    g.sa = x_scale, g.sb = w_scale, g.kb = (int)kb;
+    return op_done(fn, launch_op_gemm_f8(g, op_cus(), (hipStream_t)stream));
+}
+
 static int op_check_norm(const char *fn, int64_t T, int32_t D, int32_t x_dtype, int32_t y_dtype, int32_t h_dtype,
                          int32_t w_dtype, int32_t gate_dtype, const void *gate, int64_t gate_rows) {
     for (const int32_t t : {x_dtype, y_dtype, h_dtype, w_dtype, gate_dtype})

@@ -7,7 +7,7 @@
 
 namespace moe {
 
-enum OpType { OT_F32 = 0, OT_BF16 = 1, OT_I8 = 2 };
+enum OpType { OT_F32 = 0, OT_BF16 = 1, OT_I8 = 2, OT_F8 = 3 };  // (OT_F8: e4m3)
 __host__ __device__ constexpr int op_size(int ot) { return ot == OT_F32 ? 4 : (ot == OT_BF16 ? 2 : 1); }
 
 // C[m][n] = sum_k A(m, k) B(n, k) per group.  An operand is held with k
@@ -29,8 +29,9 @@ struct OpGemmArgs {
     int M, N, K;                   // sizes that are not ragged
     int c_f32;                     // C in fp32, else bf16
     int accumulate;                // ragged k: C += (fp32 sums, one rounding)
-    const float *sa;               // int8: scale per row of A
-    const float *sb;               // int8: scale per group and column [E][N]
+    const float *sa;               // int8: scale per row of A; e4m3: [rows][kb]
+    const float *sb;               // int8: scale per group and column [E][N]; e4m3: [E][ceil(N / 128)][kb]
+    int kb;                        // e4m3: blocks of 128 along K
     float *ws;                     // partial sums (splits > 1), [range][rows][N] or [group][range][M][N]
     int splits;                    // ranges that k is split into over workgroups (1: none)
     int nt, mt;                    // tiles along N, and (ragged k) along M
@@ -163,6 +164,23 @@ hipError_t launch_op_gate_rows(int ot, const OpGemmArgs &g, hipStream_t s);
 // columns [cols, ldq) are not written past pad_to (zeros up to it)
 hipError_t launch_quantize_i8(const void *x, long long ldx, int x_bf16, long long rows, int cols, int8_t *q,
                               long long ldq, int pad_to, float *scale, hipStream_t s);
+
+// ---- 8-bit floating point, a scale per block of 128 ---------------------------------
+constexpr int kF8Block = 128;
+// Blocks of block_rows (1 or 128) x 128: scale = max|block| / 448, q = e4m3(448 x / max|block|).
+struct QuantF8Args {
+    const void *x;
+    long long ldx, x_stride;  // elements
+    int x_bf16;
+    long long mats, rows;
+    int cols, block_rows;
+    uint8_t *q;
+    long long ldq, q_stride;
+    int pad_to;               // zeros in columns [cols, pad_to)
+    float *scale;             // [mats][ceil(rows / block_rows)][ceil(cols / 128)]
+};
+hipError_t launch_quantize_f8(const QuantF8Args &a, hipStream_t s);
+hipError_t launch_op_gemm_f8(OpGemmArgs g, int ncu, hipStream_t s);
 
 // ---- norms around a block ----------------------------------------------------------
 // z = y (post: y rstd(y) post), r = alpha x + beta gate z (rounded to x's

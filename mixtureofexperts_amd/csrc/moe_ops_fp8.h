@@ -1,0 +1,724 @@
+// moe_ops_fp8.h -- 8-bit floating point (e4m3) with a scale for each block of 128:
+// codes of rows (1 x 128) and of weights (128 x 128), and the products
+//
+//   y[r][n] = sum over blocks kb of xs[r][kb] ws[n / 128][kb] (sum over k in kb of q[r][k] w[n][k])
+//
+// A stage of k is one block: the matrix unit gives a block's sum of 128 products, the
+// vector unit multiplies it with its two scales and adds it to the fp32 sum.
+//
+// The matrix unit's 8-bit instructions (16x16x128_f8f6f4 and 16x16x32_fp8_fp8 alike) cut
+// each product to a multiple of 2^-13 of the largest of its eight neighbours along k: sums of
+// N(0, 1) codes are off by 1.4e-5 of themselves, of codes of all magnitudes by 5e-5.  That is
+// a hundredth of a bf16 result's rounding, and the instruction is twice as fast (4040
+// TFLOP/s in a loop, 16x16x32_bf16 1960), so tiles with bf16 results take it.  fp32 results,
+// and few rows, where the weights' bytes bind, have the codes widened to bf16, which is
+// exact, and products that are exact and summed in fp32 (1e-8 and 8e-8).
+#pragma once
+#include "moe_ops_gemm.h"
+#include "moe_ops_stream.h"
+
+namespace moe {
+namespace ops {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// ---- codes --------------------------------------------------------------------------
+// 448 x / m rounded to e4m3, to the bit: m a block's largest magnitude.  The product with
+// 448 / m is off by at most 2 steps of fp32; where that could cross a border between two
+// codes, 448 |x| and border * m are compared in fp64, where both are exact (27 and 29
+// bits).  Subnormal and large m are moved by 2^64 first.
+struct F8Code {
+    float adj, m, mul;
+    bool live;  // (false for 0, infinity and NaN: codes 0)
+    __device__ __forceinline__ explicit F8Code(unsigned bits) {
+        const float a = __uint_as_float(bits);
+        live = bits != 0u && bits < 0x7f800000u;
+        adj = a > 0x1p64f ? 0x1p-64f : (a < 0x1p-64f ? 0x1p64f : 1.0f);
+        m = live ? a * adj : 1.0f;
+        mul = 448.0f / m;
+    }
+    static __device__ __forceinline__ float offset(float y) { return fabsf(y) < 0x1p-6f ? 0x1p-6f : 0.0f; }
+    // whether a border may lie within y's roundings: 20 bits below e4m3's three (of y
+    // below 2^-6, whose codes are 2^-9 apart, those of |y| + 2^-6)
+    static __device__ __forceinline__ bool near_border(float y) {
+        const unsigned t = __float_as_uint(fabsf(y) + offset(y)) & 0xfffffu;
+        return t - 0x7fff8u <= 16u;
+    }
+    __device__ __forceinline__ float rough(float x) const { return live ? x * adj * mul : 0.0f; }
+    __device__ __forceinline__ float decided(float x, float y) const {
+        const float off = offset(y), z = fabsf(y) + off;
+        const unsigned mid = (__float_as_uint(z) & 0xfff00000u) | 0x80000u;
+        const double border = ((double)__uint_as_float(mid) - (double)off) * (double)m;
+        const double v = 448.0 * (double)fabsf(x * adj);
+        const unsigned r = v > border ? mid + 64u : (v < border ? mid - 64u : mid);
+        return copysignf(__uint_as_float(r) - off, x);
+    }
+};
+
+// N values' codes, four to a dword.
+template <int N>
+__device__ __forceinline__ void f8_codes(const F8Code &code, const float (&x)[N], unsigned (&out)[N / 4]) {
+    float y[N];
+    bool near = false;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        y[k] = code.rough(x[k]);
+        near |= F8Code::near_border(y[k]);
+    }
+    if (near && code.live) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (F8Code::near_border(y[k])) y[k] = code.decided(x[k], y[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < N / 4; ++k) {
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * k], y[4 * k + 1], 0, false);
+        w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * k + 2], y[4 * k + 3], w, true);
+        out[k] = (unsigned)w;
+    }
+}
+
+// Eight columns from c on of a row (those past cols are 0).
+template <int XB, bool VEC>
+__device__ __forceinline__ void f8_load(const void *row, int c, int cols, float (&v)[8]) {
+    if constexpr (VEC) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+        if (c >= cols) return;
+        if constexpr (XB) {
+            const uint4 u = *(const uint4 *)((const uint16_t *)row + c);
+            const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v[2 * k] = __uint_as_float(w[k] << 16);
+                v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+            }
+        } else {
+            const float4 a = *(const float4 *)((const float *)row + c), b = *(const float4 *)((const float *)row + c + 4);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            v[k] = 0.0f;
+            if (c + k < cols) v[k] = XB ? bf16_to_f32(((const uint16_t *)row)[c + k]) : ((const float *)row)[c + k];
+        }
+    }
+}
+template <bool VEC>
+__device__ __forceinline__ void f8_store(uint8_t *row, int c, int pad_to, const unsigned (&w)[2]) {
+    if constexpr (VEC) {
+        if (c < pad_to) *(uint2 *)(row + c) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (c + k < pad_to) row[c + k] = (uint8_t)(w[k >> 2] >> (8 * (k & 3)));
+    }
+}
+__device__ __forceinline__ unsigned f8_largest(const float (&v)[8]) {
+    unsigned m = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
+    return m;
+}
+// over the 16 lanes of a block's row
+__device__ __forceinline__ unsigned f8_over_row(unsigned m) {
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, d));
+    return m;
+}
+__device__ __forceinline__ float f8_scale(unsigned bits) {
+    return bits < 0x7f800000u ? __uint_as_float(bits) / 448.0f : __builtin_nanf("");
+}
+
+// Blocks of a row: 16 lanes each, 2^lx of a workgroup's 16 along the row.
+template <int XB, bool VEC>
+__global__ __launch_bounds__(256) void quantize_f8_rows_kernel(QuantF8Args a, int lx) {
+    const int group = threadIdx.x >> 4, l = threadIdx.x & 15;
+    const int kbs = (a.cols + 127) >> 7;
+    const long long kb = ((long long)blockIdx.x << lx) + (group & ((1 << lx) - 1));
+    if (kb >= kbs) return;
+    const int c = (int)kb * 128 + l * 8;
+    constexpr int XS = XB ? 2 : 4;
+    for (long long e = blockIdx.z; e < a.mats; e += gridDim.z) {
+        for (long long r = ((long long)blockIdx.y << (4 - lx)) + (group >> lx); r < a.rows; r += (long long)gridDim.y << (4 - lx)) {
+            float v[8];
+            f8_load<XB, VEC>((const uint8_t *)a.x + (e * a.x_stride + r * a.ldx) * XS, c, a.cols, v);
+            const unsigned m = f8_over_row(f8_largest(v));
+            if (l == 0) a.scale[(e * a.rows + r) * kbs + kb] = f8_scale(m);
+            unsigned w[2];
+            f8_codes(F8Code(m), v, w);
+            f8_store<VEC>(a.q + e * a.q_stride + r * a.ldq, c, a.pad_to, w);
+        }
+    }
+}
+
+// Blocks of 128 x 128, one per workgroup: held in registers between the maximum and the
+// codes, read once.
+template <int XB, bool VEC>
+__global__ __launch_bounds__(256) void quantize_f8_tiles_kernel(QuantF8Args a) {
+    __shared__ unsigned part[4];
+    const int kbs = (a.cols + 127) >> 7;
+    const long long rbs = (a.rows + 127) >> 7;
+    const long long tile = op_row_block();
+    if (tile >= a.mats * rbs * kbs) return;
+    const long long e = tile / (rbs * kbs), t = tile - e * (rbs * kbs);
+    const long long rb = t / kbs;
+    const int kb = (int)(t - rb * kbs);
+    constexpr int XS = XB ? 2 : 4;
+    const int c = kb * 128 + ((int)threadIdx.x & 15) * 8;
+    const long long r0 = rb * 128 + (threadIdx.x >> 4);
+    const uint8_t *x = (const uint8_t *)a.x + e * a.x_stride * XS;
+    float v[8][8];
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const long long r = r0 + i * 16;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[i][k] = 0.0f;
+        if (r < a.rows) f8_load<XB, VEC>(x + r * a.ldx * XS, c, a.cols, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, f8_largest(v[i]));
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, d));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = max(max(part[0], part[1]), max(part[2], part[3]));
+    if (threadIdx.x == 0) a.scale[tile] = f8_scale(m);
+    const F8Code code(m);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const long long r = r0 + i * 16;
+        unsigned w[2];
+        f8_codes(code, v[i], w);
+        if (r < a.rows) f8_store<VEC>(a.q + e * a.q_stride + r * a.ldq, c, a.pad_to, w);
+    }
+}
+
+// ---- products -----------------------------------------------------------------------
+struct F8Frag {
+    u32x4 h[2];  // 32 codes of a row
+};
+struct F8Wide {
+    bf16x8_t v[4];  // the same in bf16
+    __device__ __forceinline__ F8Wide() {}
+    __device__ __forceinline__ explicit F8Wide(const F8Frag &f) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = widen_fp8x8(f.h[k / 2][k % 2 * 2], f.h[k / 2][k % 2 * 2 + 1]);
+    }
+};
+// A block's products: rows of `b` become the 16 x 16 block's rows (4 (lane / 16) + c), rows of
+// `a` its columns (lane % 16).  The order of k within a lane's 32 codes is free, as
+// long as both operands have the same.
+__device__ __forceinline__ f32x4 f8_block(const F8Frag &b, const F8Frag &a) {
+    union { u32x4 h[2]; i32x8 v; } fb, fa;
+    fb.h[0] = b.h[0], fb.h[1] = b.h[1], fa.h[0] = a.h[0], fa.h[1] = a.h[1];
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb.v, fa.v, f32x4{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 f8_block(const F8Wide &b, const F8Wide &a) {
+    f32x4 c = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.v[k], a.v[k], c, 0, 0, 0);
+    return c;
+}
+
+// 16 MT rows x 16 columns by a wave, straight from global memory: pieces p, p + step, ...
+// of the range [k0, k0 + klen).  Sums in fp64, which scales of any size cannot leave.
+template <int MT>
+__device__ __forceinline__ void f8_direct(const OpGemmArgs &g, int e, int n0, int lo, int rows, int k0, int klen, int p,
+                                          int step, double (&acc)[MT][4]) {
+    constexpr int U = MT == 1 ? 4 : 2;
+    const int lane = threadIdx.x & 63, r16 = lane & 15, q4 = lane >> 4;
+    // rows past the last one repeat it (their results are not stored)
+    const uint8_t *b = (const uint8_t *)g.B + (long long)e * g.b_stride + (long long)min(n0 + r16, g.N - 1) * g.ldb + k0;
+    const float *sb = g.sb + ((long long)e * ((g.N + 127) >> 7) + (n0 >> 7)) * g.kb + (k0 >> 7);
+    const uint8_t *a[MT];
+    const float *sa[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const long long row = lo + min(m * 16 + r16, rows - 1);
+        a[m] = (const uint8_t *)g.A + row * g.lda + k0;
+        sa[m] = g.sa + row * g.kb + (k0 >> 7);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[m][c] = 0.0;
+    }
+    auto add = [&](int m, const f32x4 &v, float x, float w) {
+        const double f = (double)x * (double)w;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[m][c] += (double)v[c] * f;
+    };
+    const int pieces = (klen + 127) >> 7, whole = klen >> 7;
+    auto some = [&](auto UU_) {
+        constexpr int UU = decltype(UU_)::value;
+        F8Frag fb[UU], fa[MT][UU];
+        float w[UU], x[MT][UU];
+#pragma unroll
+        for (int u = 0; u < UU; ++u) {
+            const int q = p + u * step;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const long long o = (long long)q * 128 + h * 64 + q4 * 16;
+                __builtin_memcpy(&fb[u].h[h], b + o, 16);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) __builtin_memcpy(&fa[m][u].h[h], a[m] + o, 16);
+            }
+            w[u] = sb[q];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) x[m][u] = sa[m][q];
+        }
+#pragma unroll
+        for (int u = 0; u < UU; ++u) {
+            const F8Wide wide(fb[u]);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) add(m, f8_block(wide, F8Wide(fa[m][u])), x[m][u], w[u]);
+        }
+        p += UU * step;
+    };
+    while (p + (U - 1) * step < whole) some(num<U>{});
+    while (p < whole) some(num<1>{});
+    if (p < pieces) {  // the last, part piece
+        F8Frag fb;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = p * 128 + h * 64 + q4 * 16;
+            fb.h[h] = load_chunk<1>(b + k, klen - k);
+        }
+        const F8Wide wide(fb);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            F8Frag fa;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int k = p * 128 + h * 64 + q4 * 16;
+                fa.h[h] = load_chunk<1>(a[m] + k, klen - k);
+            }
+            add(m, f8_block(wide, F8Wide(fa)), sa[m][p], sb[p]);
+        }
+    }
+}
+
+// Results of row lo + ml at columns n .. n + 3, or a range's sums of them.
+__device__ __forceinline__ void f8_put4(const OpGemmArgs &g, long long row, int n, int ks, const float (&v)[4]) {
+    if (g.splits > 1) {
+        float *ws = g.ws + ((long long)ks * g.rows + row) * g.N;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (n + c < g.N) ws[n + c] = v[c];
+    } else {
+        put4(g, row * g.ldc + n, n, v[0], v[1], v[2], v[3], vec_ok(g));
+    }
+}
+
+// As stream_rows.
+template <int MT>
+__device__ __forceinline__ void f8_stream_rows(const OpGemmArgs &g, int e, int n0, int lo, int rows, int ks, double *red) {
+    const int lane = threadIdx.x & 63, r16 = lane & 15, q4 = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int k0, klen;
+    k_range(g, ks, 128, k0, klen);
+    double acc[MT][4];
+    f8_direct<MT>(g, e, n0, lo, rows, k0, klen, w, kStreamWaves, acc);
+    // red: [wave][MT][4][64 lanes]
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) red[((w * MT + m) * 4 + c) * 64 + lane] = acc[m][c];
+    __syncthreads();
+    if (w < MT) {
+        float v[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            double s = red[(w * 4 + c) * 64 + lane];
+            for (int x = 1; x < kStreamWaves; ++x) s += red[((x * MT + w) * 4 + c) * 64 + lane];
+            v[c] = (float)s;
+        }
+        const int ml = w * 16 + r16, n = n0 + 4 * q4;
+        if (ml < rows && n < g.N) f8_put4(g, lo + ml, n, ks, v);
+    }
+    __syncthreads();
+}
+
+__global__ __launch_bounds__(kStreamWaves * 64) void op_f8_stream_kernel(OpGemmArgs g) {
+    __shared__ double red[kStreamWaves * 4 * 4 * 64];
+    const int r = blockIdx.x / g.nt, n0 = (blockIdx.x - r * g.nt) * 16;
+    int e, lo, hi;
+    held_group(g, r, e, lo, hi);
+    if (e < 0) return;
+    while (lo < hi) {
+        const int rows = min(hi - lo, 64);
+        if (rows <= 16) f8_stream_rows<1>(g, e, n0, lo, rows, blockIdx.y, red);
+        else if (rows <= 32) f8_stream_rows<2>(g, e, n0, lo, rows, blockIdx.y, red);
+        else f8_stream_rows<4>(g, e, n0, lo, rows, blockIdx.y, red);
+        lo += rows;
+    }
+}
+
+// The largest and the smallest non-zero magnitude of the scales that a lane multiplies
+// with: products of two of them have to be normal fp32 numbers.
+struct F8Range {
+    unsigned most = 0, least = ~0u;  // bits; bits of twice the magnitude less one (0: ~0)
+    __device__ __forceinline__ void take(float s) {
+        const unsigned u = __float_as_uint(s);
+        most = max(most, u & 0x7fffffffu);
+        least = min(least, (u << 1) - 1u);
+    }
+    // exponents (subnormal: -127)
+    __device__ __forceinline__ int hi() const { return (int)(most >> 23) - 127; }
+    __device__ __forceinline__ int lo() const { return (int)((least + 1u) >> 24) - 127; }
+    static __device__ __forceinline__ bool far(const F8Range &x, const F8Range &w) {
+        if (x.least == ~0u || w.least == ~0u) return false;  // all products are zero
+        return x.hi() + w.hi() > 125 || x.lo() + w.lo() < -125;
+    }
+};
+
+// The tile loop: as op_gemm_tile, a stage one block of k, the wave's columns taken one
+// 16-column block at a time.  Step j of a stage:
+//   MFMAs of column block j: the block's sums, MI x 4 registers
+//   the sums of block j - 1 (of the stage before: its last) times the scales, into acc
+//   reads of column block j + 1; in the last step the wait for stage s + 1, the barrier
+//   and the reads of its scales, first columns and rows, and the loads of stage s + 2
+// so that the vector unit's part runs under the next MFMAs.  The scales of a stage, one
+// for each row and column of the tile, come into the ring with it.
+// WIDE: the codes in bf16.
+template <int BM, int BN, int WM, int WN, int NS, int VB, bool WIDE>
+__device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_) {
+    constexpr int NT = WM * WN * 64, KE = 128;
+    constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;
+    constexpr bool DIRECT = VB > 0;
+    static_assert(NS == 2 && NJ % 2 == 0 && BM + BN <= NT && 128 % (BN / WN) == 0, "slots, scales, one block of columns per wave");
+    using TA = Tile<1, BM, false, NT, 2, VB>;
+    using TB = Tile<1, BN, false, NT, 2, VB>;
+    constexpr int RING = NS * (TA::BYTES + TB::BYTES), SCALES = RING;  // then NS x NT scales
+
+    OpJob jb;
+    if (!ragged_job<BM>(g, jb, BN)) return;
+    const int lane = threadIdx.x & 63, r16 = lane & 15, q4 = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = w % WM, wn = w / WM;
+    const int mrows = jb.len - jb.m0;
+    int k0, klen;
+    k_range(g, jb.ks, KE, k0, klen);
+    TA ta;
+    TB tb;
+    ta.init((const uint8_t *)g.A + (long long)(jb.lo + jb.m0) * g.lda + k0, g.lda, mrows, klen);
+    tb.init((const uint8_t *)g.B + (long long)jb.e * g.b_stride + (long long)jb.n0 * g.ldb + k0, g.ldb, g.N - jb.n0, klen);
+    // this thread's scale: of tile row t (t < BM), of tile column t - BM
+    const float *sbase = w * 64 < BM ? g.sa + (long long)(jb.lo + jb.m0) * g.kb + (k0 >> 7)
+                                     : g.sb + ((long long)jb.e * ((g.N + 127) >> 7) + (jb.n0 >> 7)) * g.kb + (k0 >> 7);
+    const unsigned sb_lo = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long long)sbase);
+    const unsigned sb_hi = __builtin_amdgcn_readfirstlane((unsigned)((unsigned long long)sbase >> 32));
+    unsigned soff = kOutOfRange;
+    if constexpr (DIRECT) {
+        const int t = threadIdx.x;
+        if (t < BM) {
+            if (t < mrows) soff = (unsigned)(t * g.kb * 4);
+        } else if (t < BM + BN) {
+            if (t - BM < g.N - jb.n0) soff = (unsigned)(((t - BM) >> 7) * g.kb * 4);
+        }
+    }
+    const int S = (klen + KE - 1) / KE;
+    lds_u8 *ring = (lds_u8 *)ring_;
+    constexpr int A0 = 0, B0 = NS * TA::BYTES;  // all slots of A, all of B, all scales
+    auto a_slot = [](auto SLOT) { return A0 + decltype(SLOT)::value * TA::BYTES; };
+    auto b_slot = [](auto SLOT) { return B0 + decltype(SLOT)::value * TB::BYTES; };
+    auto s_slot = [](auto SLOT) { return SCALES + decltype(SLOT)::value * NT * 4; };
+    // The lane's places in the images, of the first slot and block: the others are within
+    // a DS instruction's offset of them.  (Opaque: the compiler would otherwise keep an
+    // address for each read, more than there are registers.)
+    auto place = [&](int at) {
+        unsigned v = (unsigned)(uintptr_t)ring + at;
+        asm("" : "+v"(v));
+        return v;
+    };
+    auto chunk = [&](int half) { return ((half * 4 + q4) ^ TA::row_swz(r16)) << 4; };
+    const unsigned a_at[2] = {place(A0 + (wm * 16 + r16) * 128 + chunk(0)), place(A0 + (wm * 16 + r16) * 128 + chunk(1))};
+    const unsigned b_at[2] = {place(B0 + (wn * NJ * 16 + r16) * 128 + chunk(0)), place(B0 + (wn * NJ * 16 + r16) * 128 + chunk(1))};
+    const unsigned x_at = place(SCALES + (wm * 16 + r16) * 4), w_at = place(SCALES + (BM + wn * (BN / WN)) * 4);
+    using FragA = std::conditional_t<WIDE, F8Wide, F8Frag>;
+    auto read_a = [&](auto SLOT, int i) {
+        F8Frag f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            f.h[h] = *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)(a_at[h] + decltype(SLOT)::value * TA::BYTES + i * WM * 2048);
+        return FragA(f);
+    };
+    auto read_b = [&](auto SLOT, int j) {
+        F8Frag f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            f.h[h] = *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)(b_at[h] + decltype(SLOT)::value * TB::BYTES + j * 2048);
+        return f;
+    };
+    typedef __attribute__((address_space(3))) float lds_f32;
+    F8Range rx, rw;
+    auto read_scales = [&](auto SLOT, float (&f)[MI]) {
+        const float sw = *(const lds_f32 *)(uintptr_t)(w_at + decltype(SLOT)::value * NT * 4);
+        rw.take(sw);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const float sx = *(const lds_f32 *)(uintptr_t)(x_at + decltype(SLOT)::value * NT * 4 + i * WM * 64);
+            rx.take(sx);
+            f[i] = sx * sw;
+        }
+    };
+    f32x4 acc[MI][NJ];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    FragA fa[MI];
+    F8Frag fb[2];
+    f32x4 part[2][MI];
+    float f[2][MI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i) part[1][i] = f32x4{0, 0, 0, 0}, f[1][i] = 0.0f;
+    auto scaled = [&](int j, const f32x4 (&p)[MI], const float (&by)[MI]) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[i][j][c] = fmaf(p[i][c], by[i], acc[i][j][c]);
+    };
+    // P: the parity of the stage
+    auto step = [&](auto P, int j) {
+        constexpr int p = decltype(P)::value;
+        const FragA b(fb[j & 1]);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) part[j & 1][i] = f8_block(b, fa[i]);
+        if (j == 0) scaled(NJ - 1, part[1], f[1 - p]);
+        else scaled(j - 1, part[1 - (j & 1)], f[p]);
+    };
+    if (S > 0) {
+        if constexpr (DIRECT) {
+            constexpr int NL = TA::NC + TB::NC + 1;
+            const unsigned l0 = (unsigned)(uintptr_t)ring;
+            auto load = [&](auto SLOT, int s) {
+                ta.load_lds(s, l0 + a_slot(SLOT), w);
+                tb.load_lds(s, l0 + b_slot(SLOT), w);
+                const unsigned long long at = ((unsigned long long)sb_hi << 32 | sb_lo) + 4ull * s;
+                u32x4 rs;
+                rs[0] = __builtin_amdgcn_readfirstlane((unsigned)at);
+                rs[1] = __builtin_amdgcn_readfirstlane((unsigned)(at >> 32) & 0xffffu);
+                rs[2] = 0x7fffffffu;
+                rs[3] = 0x00027000u;
+                const unsigned v = s < S ? soff : kOutOfRange;
+                const unsigned m0 = __builtin_amdgcn_readfirstlane(l0 + s_slot(SLOT) + w * 256);
+                asm volatile("s_nop 4\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(v),
+                             "s"(rs), "s"(m0)
+                             : "m0");
+            };
+            load(num<0>{}, 0);
+            load(num<1>{}, 1);
+            wait_loads<NL>();
+            lds_barrier();
+            read_scales(num<0>{}, f[0]);
+#pragma unroll
+            for (int i = 0; i < MI; ++i) fa[i] = read_a(num<0>{}, i);
+            fb[0] = read_b(num<0>{}, 0);
+            auto stage = [&](auto SLOT, int s) {
+                constexpr int P = decltype(SLOT)::value;
+                using Next = num<1 - P>;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    if (j < NJ - 1) {
+                        fb[1 - (j & 1)] = read_b(SLOT, j + 1);
+                        step(SLOT, j);
+                    } else {
+                        wait_loads<0>();
+                        lds_barrier();
+                        load(SLOT, s + NS);
+                        fb[0] = read_b(Next{}, 0);
+                        step(SLOT, j);
+                        read_scales(Next{}, f[1 - P]);
+#pragma unroll
+                        for (int i = 0; i < MI; ++i) fa[i] = read_a(Next{}, i);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+            int s = 0;
+            for (; s + 2 <= S; s += 2) {
+                stage(num<0>{}, s);
+                stage(num<1>{}, s + 1);
+            }
+            if (s < S) stage(num<0>{}, s);
+            wait_loads<0>();  // no load may still be writing LDS when the workgroup ends
+        } else {
+            float sreg = 0.0f;
+            auto load = [&](int s) {
+                ta.load_regs(s);
+                tb.load_regs(s);
+                const int t = threadIdx.x;  // (rows may be too far apart for 32 bits here)
+                const bool row = t < BM, ok = row ? t < mrows : t < BM + BN && t - BM < g.N - jb.n0;
+                sreg = ok ? sbase[(row ? (long long)t : (long long)((t - BM) >> 7)) * g.kb + s] : 0.0f;
+            };
+            auto keep = [&](auto SLOT) {
+                ta.store_regs(ring + a_slot(SLOT));
+                tb.store_regs(ring + b_slot(SLOT));
+                ((lds_f32 *)(ring + s_slot(SLOT)))[threadIdx.x] = sreg;
+            };
+            auto stage = [&](auto SLOT, int s) {
+                lds_barrier();
+                if (s + 1 < S) load(s + 1);
+                read_scales(SLOT, f[decltype(SLOT)::value]);
+#pragma unroll
+                for (int i = 0; i < MI; ++i) fa[i] = read_a(SLOT, i);
+                fb[0] = read_b(SLOT, 0);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    if (j < NJ - 1) fb[1 - (j & 1)] = read_b(SLOT, j + 1);
+                    step(SLOT, j);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (s + 1 < S) keep(num<1 - decltype(SLOT)::value>{});
+            };
+            load(0);
+            keep(num<0>{});
+            int s = 0;
+            for (; s + 2 <= S; s += 2) {
+                stage(num<0>{}, s);
+                stage(num<1>{}, s + 1);
+            }
+            if (s < S) stage(num<0>{}, s);
+        }
+#pragma unroll
+        for (int i = 0; i < MI; ++i) f[1][i] = (S & 1) ? f[0][i] : f[1][i];
+        scaled(NJ - 1, part[1], f[1]);
+    }
+    typedef __attribute__((address_space(3))) int lds_int;
+    lds_int *flags = (lds_int *)(ring + SCALES + NS * NT * 4);
+    if (lane == 0) flags[w] = 0;
+    if (F8Range::far(rx, rw)) flags[w] = 1;
+    bool split = false;
+    if constexpr (BM <= 64) split = g.splits > 1;  // (split calls run the smallest tiles)
+    if (split) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int ml = (i * WM + wm) * 16 + r16;
+            if (ml >= mrows) continue;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int n = jb.n0 + (wn * NJ + j) * 16 + 4 * q4;
+                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                f8_put4(g, jb.lo + jb.m0 + ml, n, jb.ks, v);
+            }
+        }
+    } else {
+        const long long at0 = (long long)(jb.lo + jb.m0) * g.ldc;
+        auto val = [&](int i, int j, int c) -> float { return acc[i][j][c]; };
+        if (g.c_f32) store_tile_rows<4, BM, BN, WM, WN, RING, false>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
+        else store_tile_rows<2, BM, BN, WM, WN, RING, false>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
+    }
+    // Scales whose products leave fp32's normal range: the tile's results again, in fp64,
+    // over those just stored (every wave's stores are done at the barrier).
+    wait_loads<0>();
+    lds_barrier();
+    int far = 0;
+#pragma unroll
+    for (int i = 0; i < WM * WN; ++i) far |= flags[i];
+    if (__builtin_amdgcn_readfirstlane(far) == 0) return;
+    for (int i = 0; i < MI; ++i) {
+        const int r0 = (i * WM + wm) * 16;
+        if (r0 >= mrows) continue;
+        for (int j = 0; j < NJ; ++j) {
+            const int n0 = jb.n0 + (wn * NJ + j) * 16;
+            if (n0 >= g.N) continue;
+            double d[1][4];
+            f8_direct<1>(g, jb.e, n0, jb.lo + jb.m0 + r0, min(16, mrows - r0), k0, klen, 0, 1, d);
+            const int n = n0 + 4 * q4;
+            if (r0 + r16 < mrows && n < g.N) {
+                const float v[4] = {(float)d[0][0], (float)d[0][1], (float)d[0][2], (float)d[0][3]};
+                f8_put4(g, jb.lo + jb.m0 + r0 + r16, n, jb.ks, v);
+            }
+        }
+    }
+}
+
+template <int BM, int BN, int WM, int WN, int NS, int WPE, int VB, bool WIDE>
+__global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void op_f8_kernel(OpGemmArgs g) {
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * ((BM + BN) * 128 + WM * WN * 64 * 4) + WM * WN * 4];
+    f8_gemm_tile<BM, BN, WM, WN, NS, VB, WIDE>(g, ring);
+}
+
+}  // namespace ops
+
+template <int BM, int BN, int WM, int WN, int WPE, bool WIDE>
+static hipError_t launch_f8_tiles(OpGemmArgs g, int vb, hipStream_t s) {
+    g.nt = (g.N + BN - 1) / BN;
+    const long long mtiles = (long long)(g.rows / BM) + (g.E < g.rows ? g.E : g.rows);
+    const long long grid = (mtiles * g.nt * g.splits + 7) / 8 * 8;
+    if (grid > 0x7fffffffll / (WM * WN * 64)) return kOpTooLarge;
+    const dim3 gr((unsigned)grid), b(WM * WN * 64);
+    if (vb == 16) {
+        ops::op_f8_kernel<BM, BN, WM, WN, 2, WPE, 16, WIDE><<<gr, b, 0, s>>>(g);
+    } else if constexpr (BN != 64) {
+        return hipErrorInvalidValue;  // (the other loads' registers do not fit beside these tiles)
+    } else if (vb == 4) {
+        ops::op_f8_kernel<BM, BN, WM, WN, 2, WPE, 4, WIDE><<<gr, b, 0, s>>>(g);
+    } else {
+        ops::op_f8_kernel<BM, BN, WM, WN, 2, WIDE ? 2 : WPE, 0, WIDE><<<gr, b, 0, s>>>(g);
+    }
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess && g.splits > 1 ? launch_op_fold(OT_BF16, false, g, s) : e;
+}
+
+hipError_t launch_op_gemm_f8(OpGemmArgs g, int ncu, hipStream_t s) {
+    if (op_streamed(OT_F8, false, g.rows, g.E, g.N, g.K, ncu)) {
+        g.nt = (g.N + 15) / 16;
+        const long long grid = (long long)(g.E < g.rows ? g.E : g.rows) * g.nt;
+        if (grid * g.splits > 0x7fffffffll / (ops::kStreamWaves * 64)) return kOpTooLarge;
+        ops::op_f8_stream_kernel<<<dim3((unsigned)grid, g.splits), ops::kStreamWaves * 64, 0, s>>>(g);
+        const hipError_t e = hipGetLastError();
+        return e == hipSuccess && g.splits > 1 ? launch_op_fold(OT_BF16, false, g, s) : e;
+    }
+    int vb = 0;
+    if (ops::tile_offsets_ok(g.lda, 1) && ops::tile_offsets_ok(g.ldb, 1)) {
+        auto pieces = [&](int bytes) {
+            return ops::whole_pieces(g.A, g.lda, 0, g.K, 1, bytes) && ops::whole_pieces(g.B, g.ldb, g.b_stride, g.K, 1, bytes);
+        };
+        if (pieces(16)) vb = 16;
+        else if (g.lda >= 16 && g.ldb >= 16 && pieces(4)) vb = 4;
+    }
+    const long long avg = (long long)g.rows / g.E;
+    auto tiles = [&](int b) -> long long {
+        const long long few = (long long)g.rows / b > g.E ? (long long)g.rows / b : (g.E < g.rows ? g.E : g.rows);
+        return few * ((g.N + b - 1) / b);
+    };
+    if (g.c_f32 || g.splits > 1) {
+        if (g.splits <= 1 && vb == 16 && avg >= 64 && g.N >= 64 && tiles(128) >= ncu)
+            return launch_f8_tiles<128, 128, 2, 2, 2, true>(g, vb, s);
+        return launch_f8_tiles<64, 64, 2, 2, 3, true>(g, vb, s);
+    }
+    if (vb == 16 && avg >= 192 && g.N >= 192 && tiles(256) >= 2 * ncu) return launch_f8_tiles<256, 256, 4, 2, 2, false>(g, vb, s);
+    if (vb == 16 && avg >= 64 && g.N >= 64 && tiles(128) >= ncu) return launch_f8_tiles<128, 128, 2, 2, 2, false>(g, vb, s);
+    return launch_f8_tiles<64, 64, 2, 2, 3, false>(g, vb, s);
+}
+
+template <int XB, bool VEC>
+static void quantize_f8(const QuantF8Args &a, hipStream_t s) {
+    const long long kbs = (a.cols + 127) / 128;
+    if (a.block_rows != 1) {
+        ops::quantize_f8_tiles_kernel<XB, VEC><<<op_row_grid(a.mats * ((a.rows + 127) / 128) * kbs), 256, 0, s>>>(a);
+        return;
+    }
+    int lx = 0;
+    while (lx < 4 && (1 << lx) < kbs) ++lx;
+    const long long gy = (a.rows + (16 >> lx) - 1) >> (4 - lx);
+    const dim3 gr((unsigned)((kbs + (1 << lx) - 1) >> lx), (unsigned)(gy < 16384 ? gy : 16384),
+                  (unsigned)(a.mats < 1024 ? a.mats : 1024));
+    ops::quantize_f8_rows_kernel<XB, VEC><<<gr, 256, 0, s>>>(a, lx);
+}
+
+hipError_t launch_quantize_f8(const QuantF8Args &a, hipStream_t s) {
+    const int es = a.x_bf16 ? 2 : 4;
+    const bool vec = (((uintptr_t)a.x | (uintptr_t)(a.ldx * es) | (uintptr_t)(a.x_stride * es)) & 15) == 0 &&
+                     (((uintptr_t)a.q | (uintptr_t)a.ldq | (uintptr_t)a.q_stride) & 7) == 0 && (a.cols & 7) == 0 &&
+                     (a.pad_to & 7) == 0;
+    if (a.x_bf16 && vec) quantize_f8<1, true>(a, s);
+    else if (a.x_bf16) quantize_f8<1, false>(a, s);
+    else if (vec) quantize_f8<0, true>(a, s);
+    else quantize_f8<0, false>(a, s);
+    return hipGetLastError();
+}
+
+}  // namespace moe

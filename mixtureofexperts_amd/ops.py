@@ -1,6 +1,7 @@
 """Operators on torch tensors in GPU memory: the grouped products of expert
-FFNs with their gradients, int8 products, and the norms, gate and residual
-around a block.  No counterpart in the reference (it has neither gradients nor
+FFNs with their gradients, the gated projections with theirs, int8 products,
+8-bit floating point products with a scale per block of 128, and the norms, gate
+and residual around a block.  No counterpart in the reference (it has neither gradients nor
 integer weights, and its caller does the norms, src/llama2/inference.jl:61).
 
 Every function runs on torch's current stream of the tensors' device, allocates
@@ -48,7 +49,8 @@ def _t():
         _torch, _forward_ad, _grad_enabled = torch, forward_ad, torch.is_grad_enabled
         _written = torch.autograd.graph.increment_version
         _floats.extend((torch.float32, torch.bfloat16))
-        _codes.update({torch.float32: _lib.MOE_F32, torch.bfloat16: _lib.MOE_BF16, torch.int8: _lib.MOE_INT8})
+        _codes.update({torch.float32: _lib.MOE_F32, torch.bfloat16: _lib.MOE_BF16, torch.int8: _lib.MOE_INT8,
+                       torch.float8_e4m3fn: _lib.MOE_FP8_E4M3})
     return _torch
 
 
@@ -467,6 +469,80 @@ def int8_matmul(x, w, w_scale, offsets=None, *, x_scale=None, out=None, out_dtyp
     _call(L.moe_int8_matmul_async, device, xp, ldx, _codes[x.dtype], x_scale.data_ptr() if codes else None,
           w.data_ptr(), ldw, stride, w_scale.data_ptr(), _offsets(offsets, E), E, x.shape[0], k, n, out.data_ptr(),
           _row_stride(out, "out"), _codes[out.dtype], wsp, wsn)
+    if given is not None:
+        _written(out)  # autograd sees the caller's tensor change
+    return out
+
+
+def quantize_fp8(x, *, block_rows=1):
+    """8-bit floating point codes (torch.float8_e4m3fn) with a float32 scale for each
+    block of 128: x (..., cols) float32 or bfloat16 -> (codes of x's shape, scales).
+    block_rows=1: a scale for each 128 elements of a row, (..., ceil(cols / 128)), as
+    fp8_matmul takes rows.  block_rows=128: x (E, rows, cols) or (rows, cols), a scale
+    for each 128 x 128 block, (E, ceil(rows / 128), ceil(cols / 128)), as it takes weights.
+    scale = max|block| / 448, code = 448 x / max|block| rounded to nearest even, exactly; a
+    block of zeros has scale 0, one that holds an infinity or a NaN scale NaN."""
+    torch = _t()
+    _plain("x", x)
+    if block_rows not in (1, 128):
+        _bad("block_rows must be 1 or 128")
+    _tensor(x, "x", _floats, range(1, 9) if block_rows == 1 else (2, 3))
+    cols = x.shape[-1]
+    if not 1 <= cols < 2**31:
+        _bad("x must have 1 to 2^31 - 1 columns")
+    kb = -(-cols // 128)
+    if block_rows == 1:
+        x2 = x.reshape(-1, cols) if x.dim() != 2 else x
+        E, rows, ldx, stride = 1, x2.shape[0], _row_stride(x2, "x"), 0
+        shape = (*x.shape[:-1], kb)
+    else:
+        x2 = x
+        E, rows, _, ldx, stride = _matrices(x, "x")
+        shape = (*x.shape[:-2], -(-rows // 128), kb)
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(shape, dtype=torch.float32, device=x.device)
+    _call(_lib.lib().moe_quantize_fp8_async, x.device, x2.data_ptr(), ldx, stride, _codes[x.dtype], E, rows, cols, block_rows,
+          q.data_ptr(), cols, rows * cols, scale.data_ptr())
+    return q, scale
+
+
+def fp8_matmul(x, w, w_scale, offsets=None, *, x_scale=None, out=None, out_dtype=None):
+    """y[r][n] = sum_k (q[r][k] x_scale[r][k / 128]) (w[e][n][k] w_scale[e][n / 128][k / 128])
+    for the rows r of expert e.  x (M, in): float8_e4m3fn codes with ``x_scale`` (M,
+    ceil(in / 128)), or float32 / bfloat16 rows, which are quantised as quantize_fp8 does;
+    w (E, out, in) float8_e4m3fn and w_scale from quantize_fp8(w, block_rows=128).  A
+    block's products are summed in float32, scaled, and summed in float32.  The result is
+    bfloat16 or, with ``out_dtype``, float32; without ``out`` rows outside every group are
+    zeros.  The gradient with respect to x is the same call on dy with the transposed codes
+    and scales (w.transpose(1, 2).contiguous()): a matrix' 128 x 128 blocks are those of its
+    transpose."""
+    torch = _t()
+    _plain("x w w_scale x_scale out", x, w, w_scale, x_scale, out)
+    L, f8 = _lib.lib(), torch.float8_e4m3fn
+    xp, ldx = _rows(x, "x", (torch.float32, torch.bfloat16, f8))
+    E, n, k, ldw, stride = _matrices(w, "w", (f8,))
+    if x.shape[1] != k:
+        _bad(f"x has {x.shape[1]} columns, the weights take {k}")
+    M, kb = x.shape[0], -(-k // 128)
+    _tensor(w_scale, "w_scale", (torch.float32,), (w.dim(),))
+    if w_scale.shape != (*w.shape[:-2], -(-n // 128), kb) or not w_scale.is_contiguous():
+        _bad(f"w_scale must be contiguous {(*w.shape[:-2], -(-n // 128), kb)}")
+    codes = x.dtype == f8
+    if codes != (x_scale is not None):
+        _bad("x_scale belongs to float8 rows")
+    if codes:
+        _tensor(x_scale, "x_scale", (torch.float32,), (2,))
+        if x_scale.shape != (M, kb) or not x_scale.is_contiguous():
+            _bad(f"x_scale must be contiguous {(M, kb)}")
+    if out is None and out_dtype is None:
+        out_dtype = torch.bfloat16
+    given = out
+    out = _result(out, (M, n), out_dtype, (torch.bfloat16, torch.float32), x, offsets is not None)
+    device = _same_device(x, w, w_scale, x_scale, offsets, out)
+    ws, wsp, wsn = _workspace(L.moe_fp8_matmul_workspace, device, E, M, k, n, _codes[x.dtype])
+    _call(L.moe_fp8_matmul_async, device, xp, ldx, _codes[x.dtype], x_scale.data_ptr() if codes else None, w.data_ptr(), ldw,
+          stride, w_scale.data_ptr(), _offsets(offsets, E), E, M, k, n, out.data_ptr(), _row_stride(out, "out"),
+          _codes[out.dtype], wsp, wsn)
     if given is not None:
         _written(out)  # autograd sees the caller's tensor change
     return out
