@@ -259,6 +259,8 @@ static int64_t gated_workspace(OpMode mode, int32_t groups, int32_t rows, int32_
         const int s = op_gated_splits(mode, dtype == MOE_F32 ? OT_F32 : OT_BF16, col, rows, groups, n, k, op_cus());
         if (s > 1) bytes = std::max(bytes, (int64_t)4 * (mode == OM_GATED ? 2 : 1) * s * rows * n);
     }
+    if (mode == OM_TWO && op_two_tail(dtype == MOE_F32 ? OT_F32 : OT_BF16, rows, groups, n, k, op_cus()))
+        bytes = std::max(bytes, (int64_t)4 * kOpTailTile * 8 * (op_cus() / 8));
     return bytes;
 }
 static int gated_workspace_of(const char *fn, OpMode mode, int32_t groups, int32_t rows, int32_t n, int32_t k,
@@ -423,6 +425,7 @@ int moe_gated_matmul_grad_x_async(const void *da, int64_t ldda, const void *db, 
     g.offsets = offsets, g.E = groups, g.rows = rows, g.N = in_dim, g.K = hidden_dim;
     const int ot = dtype == MOE_F32 ? OT_F32 : OT_BF16;
     g.splits = op_gated_splits(OM_TWO, ot, !flux, rows, groups, in_dim, hidden_dim, op_cus());
+    g.tail = op_two_tail(ot, rows, groups, in_dim, hidden_dim, op_cus()) ? op_cus() / 8 : 0;
     g.ws = (float *)workspace;
     return op_done(fn, launch_op_gated(OM_TWO, ot, !flux, g, op_cus(), (hipStream_t)stream));
 }

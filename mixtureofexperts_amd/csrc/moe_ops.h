@@ -43,6 +43,7 @@ struct OpGemmArgs {
     long long ldga, ldgb;
     void *C2, *C3;                 // OM_GATED: a and b (or null); OM_GATE_GRAD: db and h
     long long ldc2, ldc3;
+    int tail;                      // OM_TWO, 256 x 256 tiles: CUs of an XCD whose last, part round is split (0: none)
 };
 
 // What a product of ragged rows computes:
@@ -139,6 +140,14 @@ inline int op_matrix_splits(int ot, long long rows, long long E, long long M, lo
 inline int op_gated_splits(OpMode mode, int ot, bool b_col, long long rows, long long E, long long N, long long K, int ncu) {
     if (mode == OM_GATED && op_streamed(ot, b_col, rows, E, N, K, ncu)) return op_rows_splits(ot, b_col, rows, E, N, K, ncu);
     return op_rows_splits(ot, true, rows, E, mode == OM_GATED ? 2 * N : N, mode == OM_TWO ? 2 * K : K, ncu);
+}
+
+// bf16 OM_TWO on 256 x 256 tiles: the last round is split where there are few of them and k
+// (of both pairs) is long.
+constexpr int kOpTailTile = 256 * 256;  // sums of a split tile in ws
+inline bool op_two_tail(int ot, long long rows, long long E, long long N, long long K, int ncu) {
+    const long long mt = rows / 256 > E ? rows / 256 : (E < rows ? E : rows), tiles = mt * ((N + 255) / 256);
+    return ot == OT_BF16 && rows >= 192 * E && N >= 192 && tiles >= 2 * ncu && tiles < 8 * ncu && 2 * K >= 8192;
 }
 
 // What a launcher answers to a call of more workgroups than one launch takes.

@@ -453,7 +453,9 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
     typedef __attribute__((address_space(3))) float lds_f32;
     F8Range rx, rw;
     auto read_scales = [&](auto SLOT, float (&f)[MI]) {
-        const float sw = *(const lds_f32 *)(uintptr_t)(w_at + decltype(SLOT)::value * NT * 4);
+        // one for all columns of the wave
+        const float sw = __uint_as_float(__builtin_amdgcn_readfirstlane(
+            *(const __attribute__((address_space(3))) unsigned *)(uintptr_t)(w_at + decltype(SLOT)::value * NT * 4)));
         rw.take(sw);
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
@@ -488,13 +490,22 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
         if (j == 0) scaled(NJ - 1, part[1], f[1 - p]);
         else scaled(j - 1, part[1 - (j & 1)], f[p]);
     };
+    // the order of a step: reads first, then after each MFMA what fits under it
+    auto mixed = [] {
+        if constexpr (!WIDE) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
+            }
+        }
+    };
     if (S > 0) {
         if constexpr (DIRECT) {
             constexpr int NL = TA::NC + TB::NC + 1;
             const unsigned l0 = (unsigned)(uintptr_t)ring;
-            auto load = [&](auto SLOT, int s) {
-                ta.load_lds(s, l0 + a_slot(SLOT), w);
-                tb.load_lds(s, l0 + b_slot(SLOT), w);
+            auto load_scales = [&](auto SLOT, int s) {
                 const unsigned long long at = ((unsigned long long)sb_hi << 32 | sb_lo) + 4ull * s;
                 u32x4 rs;
                 rs[0] = __builtin_amdgcn_readfirstlane((unsigned)at);
@@ -506,6 +517,11 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
                 asm volatile("s_nop 4\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(v),
                              "s"(rs), "s"(m0)
                              : "m0");
+            };
+            auto load = [&](auto SLOT, int s) {
+                ta.load_lds(s, l0 + a_slot(SLOT), w);
+                tb.load_lds(s, l0 + b_slot(SLOT), w);
+                load_scales(SLOT, s);
             };
             load(num<0>{}, 0);
             load(num<1>{}, 1);
@@ -523,15 +539,25 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
                     if (j < NJ - 1) {
                         fb[1 - (j & 1)] = read_b(SLOT, j + 1);
                         step(SLOT, j);
+                        mixed();
                     } else {
                         wait_loads<0>();
                         lds_barrier();
-                        load(SLOT, s + NS);
                         fb[0] = read_b(Next{}, 0);
-                        step(SLOT, j);
-                        read_scales(Next{}, f[1 - P]);
+                        const FragA b(fb[1]);
 #pragma unroll
-                        for (int i = 0; i < MI; ++i) fa[i] = read_a(Next{}, i);
+                        for (int i = 0; i < MI; ++i) {
+                            part[1][i] = f8_block(b, fa[i]);
+                            fa[i] = read_a(Next{}, i);
+#pragma unroll
+                            for (int c = 0; c < 4; ++c)
+                                acc[i][j - 1][c] = fmaf(part[0][i][c], f[P][i], acc[i][j - 1][c]);
+                            if (i == 0) ta.load_lds(s + NS, l0 + a_slot(SLOT), w);
+                            if (i == 1) tb.load_lds(s + NS, l0 + b_slot(SLOT), w);
+                            if (i == MI - 1) load_scales(SLOT, s + NS);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                        read_scales(Next{}, f[1 - P]);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -654,7 +680,7 @@ static hipError_t launch_f8_tiles(OpGemmArgs g, int vb, hipStream_t s) {
     } else if constexpr (BN != 64) {
         return hipErrorInvalidValue;  // (the other loads' registers do not fit beside these tiles)
     } else if (vb == 4) {
-        ops::op_f8_kernel<BM, BN, WM, WN, 2, WPE, 4, WIDE><<<gr, b, 0, s>>>(g);
+        ops::op_f8_kernel<BM, BN, WM, WN, 2, WIDE ? 2 : WPE, 4, WIDE><<<gr, b, 0, s>>>(g);
     } else {
         ops::op_f8_kernel<BM, BN, WM, WN, 2, WIDE ? 2 : WPE, 0, WIDE><<<gr, b, 0, s>>>(g);
     }

@@ -61,30 +61,42 @@ __device__ __forceinline__ GateBack gate_back(const Gate &g, float dh, float a, 
 }
 
 // CE elements of a row from column n on, N its columns: 16 bytes at any alignment,
-// element by element past the end.
+// element by element past the end.  Raw: as they are in memory.
+struct GateRaw {
+    uint4 u;
+};
+template <bool BF16>
+__device__ __forceinline__ GateRaw gate_load(const void *row, int n, int N) {
+    constexpr int CE = BF16 ? 8 : 4, ES = BF16 ? 2 : 4;
+    GateRaw r;
+    if (n + CE <= N) {
+        __builtin_memcpy(&r.u, (const uint8_t *)row + (long long)n * ES, 16);
+    } else {
+        unsigned w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int q = 0; q < CE; ++q) {
+            if (n + q >= N) continue;
+            if constexpr (BF16) w[q / 2] |= (unsigned)((const uint16_t *)row)[n + q] << (16 * (q & 1));
+            else w[q] = ((const unsigned *)row)[n + q];
+        }
+        r.u = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return r;
+}
 template <bool BF16>
 struct GateChunk {
     static constexpr int CE = BF16 ? 8 : 4;
     float v[CE];
-    __device__ __forceinline__ void load(const void *row, int n, int N) {
-        if (n + CE <= N) {
+    __device__ __forceinline__ GateChunk() {}
+    __device__ __forceinline__ explicit GateChunk(const GateRaw &r) {
+        const unsigned w[4] = {r.u.x, r.u.y, r.u.z, r.u.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
             if constexpr (BF16) {
-                uint4 u;
-                __builtin_memcpy(&u, (const uint16_t *)row + n, 16);
-                const unsigned w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    v[2 * q] = __uint_as_float(w[q] << 16);
-                    v[2 * q + 1] = __uint_as_float(w[q] & 0xffff0000u);
-                }
+                v[2 * q] = __uint_as_float(w[q] << 16);
+                v[2 * q + 1] = __uint_as_float(w[q] & 0xffff0000u);
             } else {
-                __builtin_memcpy(v, (const float *)row + n, 16);
-            }
-        } else {
-#pragma unroll
-            for (int q = 0; q < CE; ++q) {
-                v[q] = 0.0f;
-                if (n + q < N) v[q] = BF16 ? bf16_to_f32(((const uint16_t *)row)[n + q]) : ((const float *)row)[n + q];
+                v[q] = __uint_as_float(w[q]);
             }
         }
     }
@@ -113,13 +125,20 @@ struct GateChunk {
     }
 };
 
-// Row `row`, columns n .. n + CE - 1 of da, db and h from dh there.
+// The pre-activations at a chunk of row `row`.
 template <bool BF16>
-__device__ __forceinline__ void gate_store(const OpGemmArgs &g, long long row, int n, const GateChunk<BF16> &dh) {
+__device__ __forceinline__ void gate_load_ab(const OpGemmArgs &g, long long row, int n, GateRaw &a, GateRaw &b) {
     constexpr int ES = BF16 ? 2 : 4;
-    GateChunk<BF16> a, b, da, db, h;
-    a.load((const uint8_t *)g.ga + row * g.ldga * ES, n, g.N);
-    b.load((const uint8_t *)g.gb + row * g.ldgb * ES, n, g.N);
+    a = gate_load<BF16>((const uint8_t *)g.ga + row * g.ldga * ES, n, g.N);
+    b = gate_load<BF16>((const uint8_t *)g.gb + row * g.ldgb * ES, n, g.N);
+}
+// da, db and h there from dh.
+template <bool BF16>
+__device__ __forceinline__ void gate_store(const OpGemmArgs &g, long long row, int n, const GateChunk<BF16> &dh,
+                                           const GateRaw &ra, const GateRaw &rb) {
+    constexpr int ES = BF16 ? 2 : 4;
+    const GateChunk<BF16> a(ra), b(rb);
+    GateChunk<BF16> da, db, h;
     const Gate gate(g.act);
     auto all = [&](auto SMOOTH) {
 #pragma unroll

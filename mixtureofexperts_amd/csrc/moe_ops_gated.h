@@ -182,7 +182,9 @@ __global__ __launch_bounds__(256) void op_gate_fold_kernel(OpGemmArgs g) {
             for (int c = 0; c < CE; ++c)
                 if (n + c < g.N) dh.v[c] += ws[s * all + c];
         }
-        gate_store<BF16>(g, row, n, dh);
+        GateRaw a, b;
+        gate_load_ab<BF16>(g, row, n, a, b);
+        gate_store<BF16>(g, row, n, dh, a, b);
     }
 }
 
@@ -201,9 +203,10 @@ __global__ __launch_bounds__(256) void op_gate_rows_kernel(OpGemmArgs g, int lx)
     if (n >= g.N) return;
     const long long step = (long long)gridDim.y << (8 - lx);
     for (long long r = lo + ((long long)blockIdx.y << (8 - lx)) + (threadIdx.x >> lx); r < hi; r += step) {
-        GateChunk<BF16> dh;
-        dh.load((const uint8_t *)g.A + r * g.lda * ES, (int)n, g.N);
-        gate_store<BF16>(g, r, (int)n, dh);
+        GateRaw a, b;
+        const GateRaw dh = gate_load<BF16>((const uint8_t *)g.A + r * g.lda * ES, (int)n, g.N);
+        gate_load_ab<BF16>(g, r, (int)n, a, b);
+        gate_store<BF16>(g, r, (int)n, GateChunk<BF16>(dh), a, b);
     }
 }
 

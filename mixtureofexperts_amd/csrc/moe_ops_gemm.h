@@ -340,42 +340,43 @@ struct OpJob {
 // tiles re-reads neither its rows for every n tile nor its matrix for every M tile.
 constexpr int kOpMBlock = 8;
 
-// Item `item` of the tiles of all groups, group-major; false past the last.
-// Every wave scans the groups' lengths, 64 groups at a time.
+// Tiles of the group of this lane (groups base to base + 63), summed over the lanes up
+// to it, and its rows.
 template <int BM>
-__device__ __forceinline__ bool ragged_job(const OpGemmArgs &g, OpJob &jb, int BN) {
-    const int lane = threadIdx.x & 63, NT = g.nt;
-    // tiles of the group of this lane, summed over the lanes up to it
-    auto scan = [&](int base, int &lo, int &len) {
-        lo = 0;
-        len = 0;
-        if (base + lane < g.E) {
-            int hi;
-            op_group(g.offsets, base + lane, g.rows, lo, hi);
-            len = hi - lo;
-        }
-        int t = (len + BM - 1) / BM;
+__device__ __forceinline__ int ragged_scan(const OpGemmArgs &g, int base, int &lo, int &len) {
+    const int lane = threadIdx.x & 63;
+    lo = 0;
+    len = 0;
+    if (base + lane < g.E) {
+        int hi;
+        op_group(g.offsets, base + lane, g.rows, lo, hi);
+        len = hi - lo;
+    }
+    int t = (len + BM - 1) / BM;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int u = __shfl_up(t, d);
-            if (lane >= d) t += u;
-        }
-        return t;
-    };
-    int lo, len, W = 0, t = 0;
+    for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(t, d);
+        if (lane >= d) t += u;
+    }
+    return t;
+}
+// Row tiles of all groups; t, lo, len: of the last 64 groups.
+template <int BM>
+__device__ __forceinline__ int ragged_tiles(const OpGemmArgs &g, int &t, int &lo, int &len) {
+    int W = 0;
+    t = 0;
     for (int base = 0; base < g.E; base += 64) {
-        t = scan(base, lo, len);
+        t = ragged_scan<BM>(g, base, lo, len);
         W += __shfl(t, 63);
     }
-    W *= NT * g.splits;
-    // contiguous per-XCD ranges (block L runs on XCD L mod 8)
-    const int per = (W + 7) >> 3, slot = blockIdx.x >> 3;
-    int item = (blockIdx.x & 7) * per + slot;
-    if (slot >= per || item >= W) return false;
-    jb.ks = __builtin_amdgcn_readfirstlane(item % g.splits);
-    item = __builtin_amdgcn_readfirstlane(item / g.splits);
+    return W;
+}
+// Item `item` of the tiles of all groups, group-major; false past the last.
+template <int BM>
+__device__ __forceinline__ bool ragged_item(const OpGemmArgs &g, OpJob &jb, int BN, int item, int t, int lo, int len) {
+    const int NT = g.nt;
     for (int base = 0; base < g.E; base += 64) {
-        if (g.E > 64) t = scan(base, lo, len);
+        if (g.E > 64) t = ragged_scan<BM>(g, base, lo, len);
         const unsigned long long past = __ballot(t * NT > item);
         if (past) {
             const int src = __ffsll((long long)past) - 1;
@@ -406,6 +407,55 @@ __device__ __forceinline__ bool ragged_job(const OpGemmArgs &g, OpJob &jb, int B
         item -= __shfl(t, 63) * NT;
     }
     return false;
+}
+// This workgroup's item.  Every wave scans the groups' lengths, 64 groups at a time.
+template <int BM>
+__device__ __forceinline__ bool ragged_job(const OpGemmArgs &g, OpJob &jb, int BN) {
+    int t, lo, len;
+    const int W = ragged_tiles<BM>(g, t, lo, len) * g.nt * g.splits;
+    // contiguous per-XCD ranges (block L runs on XCD L mod 8)
+    const int per = (W + 7) >> 3, slot = blockIdx.x >> 3;
+    int item = (blockIdx.x & 7) * per + slot;
+    if (slot >= per || item >= W) return false;
+    jb.ks = __builtin_amdgcn_readfirstlane(item % g.splits);
+    item = __builtin_amdgcn_readfirstlane(item / g.splits);
+    return ragged_item<BM>(g, jb, BN, item, t, lo, len);
+}
+
+// The same where the last, part round of an XCD's g.tail CUs is split: each of its tiles
+// runs as `parts` ranges of k, their sums kept in ws for op_tail_fold_kernel.  (Tiles of
+// 28672 products over 2.25 rounds took three.)
+constexpr int kOpTailParts = 8;
+struct OpTail {
+    int first, tiles, parts;  // of an XCD: items before the split tiles, split tiles, ranges of each
+    int per;                  // items of an XCD, at most
+    __device__ __forceinline__ OpTail(int W, int xcd, int cus) {
+        per = (W + 7) >> 3;
+        const int mine = min(per, W - xcd * per);
+        first = mine > 0 ? (cus > 0 ? mine / cus * cus : mine) : 0;
+        tiles = max(mine, 0) - first;
+        parts = tiles > 0 ? min(kOpTailParts, cus / tiles) : 1;
+        if (parts <= 1) first += tiles, tiles = 0, parts = 1;
+    }
+};
+template <int BM>
+__device__ __forceinline__ bool tail_job(const OpGemmArgs &g, OpJob &jb, int BN, int &parts, int &place) {
+    int t, lo, len;
+    const int W = ragged_tiles<BM>(g, t, lo, len) * g.nt;
+    const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
+    const OpTail tail(W, xcd, g.tail);
+    int item = slot;
+    parts = 1;
+    jb.ks = 0;
+    if (slot >= tail.first) {
+        const int u = slot - tail.first;
+        if (u >= tail.tiles * tail.parts) return false;
+        parts = __builtin_amdgcn_readfirstlane(tail.parts);
+        jb.ks = __builtin_amdgcn_readfirstlane(u % parts);
+        item = tail.first + u / parts;
+        place = __builtin_amdgcn_readfirstlane(xcd * g.tail + u);
+    }
+    return ragged_item<BM>(g, jb, BN, __builtin_amdgcn_readfirstlane(xcd * tail.per + item), t, lo, len);
 }
 
 // The group of the r-th longest length (ties by index), with its rows.  Up to
@@ -649,7 +699,9 @@ __device__ __forceinline__ void store_tile_rows(const OpGemmArgs &g, lds_u8 *rin
 }
 
 // A tile of dh through LDS in fp32, then whole chunks of da, db and h from it and the
-// same chunks of a and b, which are read once, in rows.  LDS as in store_tile_rows.
+// same chunks of a and b, which are read once, in rows.  LDS as in store_tile_rows.  A
+// pass's a and b are on their way while its dh is put into LDS: 32 KB a round trip would
+// hold up a workgroup that has the CU to itself.
 template <int OT, int BM, int BN, int WM, int WN, int RING, typename Val>
 __device__ __forceinline__ void gate_tile_rows(const OpGemmArgs &g, lds_u8 *ring, long long row0, int mrows, int n0,
                                                int wm, int wn, int lane, Val val) {
@@ -660,12 +712,17 @@ __device__ __forceinline__ void gate_tile_rows(const OpGemmArgs &g, lds_u8 *ring
     constexpr int PR = FIT >= BM ? BM : (FIT >= BM / 2 ? BM / 2 : BM / 4);  // rows per pass
     constexpr int CE = GateChunk<BF16>::CE, OC = BN / CE;  // results per chunk, chunks per row
     static_assert(PR % (WM * 16) == 0 && BM % PR == 0 && NT % OC == 0 && PR % (NT / OC) == 0 && PR <= FIT, "passes");
-    constexpr int IP = PR / (WM * 16);
+    constexpr int IP = PR / (WM * 16), RT = NT / OC, IT = PR / RT;  // rows at a time, times
     typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
     const int r16 = lane & 15, q4 = lane >> 4;
+    const int oc = (int)threadIdx.x % OC, rt = (int)threadIdx.x / OC;
+    const int n = n0 + oc * CE, nc = min(n, g.N - 1);  // (columns past the last: not stored)
+    auto pass = [&](auto P) {
+        constexpr int p = decltype(P)::value;
+        if (p * PR >= mrows) return;
+        GateRaw a[IT], b[IT];
 #pragma unroll
-    for (int p = 0; p < BM / PR; ++p) {
-        if (p * PR >= mrows) break;
+        for (int t = 0; t < IT; ++t) gate_load_ab<BF16>(g, row0 + min(p * PR + rt + t * RT, mrows - 1), nc, a[t], b[t]);
         __syncthreads();  // the ring (the previous pass) is no longer read
 #pragma unroll
         for (int ii = 0; ii < IP; ++ii) {
@@ -678,21 +735,23 @@ __device__ __forceinline__ void gate_tile_rows(const OpGemmArgs &g, lds_u8 *ring
             }
         }
         __syncthreads();
-        const int oc = (int)threadIdx.x % OC, n = n0 + oc * CE;
-        const int rows = min(PR, mrows - p * PR);
-        if (n < g.N) {
-            for (int r = (int)threadIdx.x / OC; r < rows; r += NT / OC) {
-                GateChunk<BF16> dh;
 #pragma unroll
-                for (int k = 0; k < CE / 4; ++k) {
-                    const f32x4 t = *(const lds_f32x4 *)(ring + r * CW + (((oc * (CE / 4) + k) ^ (r & (CH - 1))) << 4));
+        for (int t = 0; t < IT; ++t) {
+            const int r = rt + t * RT;
+            if (n >= g.N || p * PR + r >= mrows) continue;
+            GateChunk<BF16> dh;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) dh.v[4 * k + q] = t[q];
-                }
-                gate_store<BF16>(g, row0 + p * PR + r, n, dh);
+            for (int k = 0; k < CE / 4; ++k) {
+                const f32x4 v = *(const lds_f32x4 *)(ring + r * CW + (((oc * (CE / 4) + k) ^ (r & (CH - 1))) << 4));
+#pragma unroll
+                for (int q = 0; q < 4; ++q) dh.v[4 * k + q] = v[q];
             }
+            gate_store<BF16>(g, row0 + p * PR + r, n, dh, a[t], b[t]);
         }
-    }
+    };
+    pass(num<0>{});
+    if constexpr (BM / PR > 1) pass(num<1>{});
+    static_assert(BM / PR <= 2, "passes");
 }
 
 // ---- the kernel --------------------------------------------------------------------
@@ -731,11 +790,17 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
     using TA = Tile<ES, BM, ACOL, NT, KSUB, VB>;
     using TB = Tile<ES, BR, BCOL, NT, KSUB, VB>;
 
+    constexpr bool TAIL = TWO && BM == 256;
+    int parts = g.splits, place = 0;  // ranges of k, TAIL: this one's place in ws
     OpJob jb;
     if constexpr (RAGK) {
         if (!matrix_job(g, jb, BM, BN, KE)) return;
     } else {
-        if (!ragged_job<BM>(g, jb, BR)) return;
+        if constexpr (TAIL) {
+            if (!tail_job<BM>(g, jb, BR, parts, place)) return;
+        } else {
+            if (!ragged_job<BM>(g, jb, BR)) return;
+        }
     }
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -766,7 +831,7 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
                 k0 = 0;
                 klen = g.K;
                 pair = (g.K + KE - 1) / KE;
-                const int per = (2 * pair + g.splits - 1) / g.splits;
+                const int per = (2 * pair + parts - 1) / parts;
                 first = __builtin_amdgcn_readfirstlane(min(jb.ks * per, 2 * pair));
                 end = __builtin_amdgcn_readfirstlane(min(first + per, 2 * pair));
             } else {
@@ -979,6 +1044,16 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
             return;
         }
     }
+    if constexpr (TAIL) {
+        if (parts > 1) {
+            f32x4 *ws = (f32x4 *)g.ws + (long long)place * (MI * NJ * NT) + threadIdx.x;
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) ws[(i * NJ + j) * NT] = acc[i][j];
+            return;
+        }
+    }
     const long long at0 = RAGK ? (long long)jb.e * g.c_stride + (long long)jb.m0 * g.ldc
                                : (long long)(jb.lo + jb.m0) * g.ldc;  // the tile's first row in C
     // int8: the lane's scales, of its row blocks and its columns
@@ -1084,6 +1159,32 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WP
     op_gemm_tile<OT, false, BCOL, false, BM, BN, WM, WN, KSUB, NS, VB, MODE>(g, ring);
 }
 
+// Results of the split tiles of a tail, the ranges' sums in range order: workgroup (XCD and
+// tile of it, column block j of every wave).
+template <int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64) void op_tail_fold_kernel(OpGemmArgs g) {
+    constexpr int NT = WM * WN * 64, MI = BM / WM / 16, NJ = BN / WN / 16;
+    const int xcd = blockIdx.x / g.tail, tile = blockIdx.x - xcd * g.tail, j = blockIdx.y;
+    int t, lo, len;
+    const OpTail tail(ragged_tiles<BM>(g, t, lo, len) * g.nt, xcd, g.tail);
+    if (tile >= tail.tiles) return;
+    OpJob jb;
+    if (!ragged_item<BM>(g, jb, BN, xcd * tail.per + tail.first + tile, t, lo, len)) return;
+    const int lane = threadIdx.x & 63, r16 = lane & 15, q4 = lane >> 4;
+    const int w = threadIdx.x >> 6, wm = w % WM, wn = w / WM;
+    const int n = jb.n0 + (wn * NJ + j) * 16 + 4 * q4;
+    if (n >= g.N) return;
+    const f32x4 *ws = (const f32x4 *)g.ws + (long long)(xcd * g.tail + tile * tail.parts) * (MI * NJ * NT) + threadIdx.x;
+    const bool vec = vec_ok(g);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+        f32x4 v = {0, 0, 0, 0};
+        for (int p = 0; p < tail.parts; ++p) v += ws[((long long)p * MI * NJ + i * NJ + j) * NT];
+        const int ml = (i * WM + wm) * 16 + r16;
+        if (ml < jb.len - jb.m0) put4(g, (long long)(jb.lo + jb.m0 + ml) * g.ldc + n, n, v[0], v[1], v[2], v[3], vec);
+    }
+}
+
 // Rows of whole, aligned pieces of `bytes`.
 inline bool whole_pieces(const void *p, long long ld, long long stride, int contiguous, int es, int bytes) {
     return (((uintptr_t)p | (uintptr_t)(ld * es) | (uintptr_t)(stride * es)) & (bytes - 1)) == 0 &&
@@ -1101,8 +1202,10 @@ hipError_t launch_tiles(OpGemmArgs g, int vb, hipStream_t s) {
     // ragged rows: sum of ceil(rows_e / BM) <= rows / BM + the groups that can hold a row
     // ragged k: every XCD's part of every group
     const long long mtiles = (long long)(g.rows / BM) + (g.E < g.rows ? g.E : g.rows);
-    const long long grid =
-        RAGK ? ((long long)g.mt * g.nt * g.splits + 7) / 8 * 8 * g.E : (mtiles * g.nt * g.splits + 7) / 8 * 8;
+    constexpr bool TAIL = MODE == OM_TWO && BM == 256;
+    if (!TAIL) g.tail = 0;
+    const long long grid = RAGK ? ((long long)g.mt * g.nt * g.splits + 7) / 8 * 8 * g.E
+                                : (mtiles * g.nt * g.splits + 7) / 8 * 8 + 8ll * g.tail;
     if (grid > 0x7fffffffll / (WM * WN * 64)) return kOpTooLarge;
     const dim3 b(WM * WN * 64);
     // (bf16 pairs by dwords: the registers of three waves per SIMD are too few)
@@ -1131,6 +1234,11 @@ hipError_t launch_tiles(OpGemmArgs g, int vb, hipStream_t s) {
     }
 #undef MOE_OP_TILES
     const hipError_t e = hipGetLastError();
+    if constexpr (TAIL) {
+        if (e != hipSuccess || g.tail == 0) return e;
+        op_tail_fold_kernel<BM, BN, WM, WN><<<dim3(8 * g.tail, BN / WN / 16), b, 0, s>>>(g);
+        return hipGetLastError();
+    }
     if (e != hipSuccess || g.splits <= 1) return e;
     if constexpr (MODE == OM_GATED || MODE == OM_GATE_GRAD) return launch_op_gate_fold(MODE, OT, g, s);
     else return launch_op_fold(OT, RAGK, g, s);

@@ -219,6 +219,31 @@ def test_large_tiles(moe, layout):
         _check_grad_x(lens, _f64(res[-1]), da, db, v1, v3, layout, Hx, "bf16")
 
 
+@pytest.mark.parametrize("layout", [LLAMA, FLUX])
+@pytest.mark.parametrize("lens", [[1500, 700, 1896], [1025, 1025, 2046], [2048, 0, 2048]])
+def test_split_last_round(moe, lens, layout):
+    # two rounds of 256 x 256 tiles and a part of one, whose tiles are split; or none
+    rng = np.random.default_rng(16)
+    K, H = 8184, 4100 if layout == FLUX else 4104
+    H = H // 8 * 8
+    M, off = sum(lens), _offsets(lens)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    new = lambda *s: torch.randn(*s, generator=g, device="cuda").to(torch.bfloat16)
+    da, db = new(M + 3, H), new(M + 3, H)
+    shape = (3, H, K) if layout == LLAMA else (3, K, H)
+    w1, w3 = new(*shape), new(*shape)
+    for odt in ("bf16", "f32"):
+        whole, view = _empty(M + 3, K, 0, odt)
+        names = kernels_of(lambda: moe.gated_matmul_grad_x(da, db, w1, w3, off, layout=layout, out=view))
+        assert _tile(names, 3) == (256, 16) and "op_tail_fold_kernel" in names
+        for e, s in _groups(lens):  # float64 on the GPU: 5e11 products
+            m1, m3 = ((w[e] if layout == LLAMA else w[e].t()).double() for w in (w1, w3))
+            a, b = da[s].double(), db[s].double()
+            ref, mag = a @ m1 + b @ m3, a.abs() @ m1.abs() + b.abs() @ m3.abs()
+            assert ((view[s].double() - ref).abs() <= 2 * H * 2.0**-23 * mag + ref.abs() * STEP[odt]).all()
+        assert (view[M:] == SENTINEL).all()
+
+
 # few rows and columns of a long sum: k split over workgroups, streamed and tiled
 LONG = [([1], 8192, 16), ([3, 0, 2], 4001, 125), ([3, 0, 2], 16401, 45), ([71], 5440, 64), ([200, 0, 150], 3456, 131),
         ([40, 3], 2999, 64)]

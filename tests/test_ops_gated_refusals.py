@@ -105,7 +105,9 @@ def test_workspaces(moe):
         for ws, size in ((None, n.value), (P + 8, n.value), (P, 16)):
             _refused(fn + "_async", {**args, "workspace": ws, "workspace_bytes": size}, "workspace")
         assert query(8, 0, 64, 32, BF16, ctypes.byref(n)) == 0 and n.value == 0
-        assert query(8, 8192, 4096, 14336, BF16, ctypes.byref(n)) == 0 and n.value == 0
+        # (the row gradient splits the last round of few large tiles)
+        assert query(8, 8192, 4096, 14336, BF16, ctypes.byref(n)) == 0 and (n.value > 0) == (fn == "moe_gated_matmul_grad_x")
+        assert query(8, 8192, 4096, 14336, F32, ctypes.byref(n)) == 0 and n.value == 0
         assert query(1, 3, 8, 8, FP8, ctypes.byref(n)) == _lib.MOE_EINVAL
         assert query(1, 3, 8, 8, BF16, None) == _lib.MOE_EINVAL
         assert query(0, 3, 8, 8, BF16, ctypes.byref(n)) == _lib.MOE_EINVAL
