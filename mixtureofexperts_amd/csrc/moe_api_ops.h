@@ -546,7 +546,7 @@ int moe_quantize_fp8_async(const void *x, int64_t ldx, int64_t x_stride, int32_t
 // Workspace of the product: partial sums, then the rows' scales and codes (padded to 16
 // bytes) where the call quantises them.
 static int64_t fp8_partial_bytes(int32_t groups, int32_t rows, int32_t in_dim, int32_t out_dim) {
-    const int s = op_rows_splits(OT_F8, false, rows, groups, out_dim, in_dim, op_cus());
+    const int s = op_f8_splits(rows, groups, out_dim, in_dim, op_cus());
     return s > 1 ? round_up((int64_t)4 * s * rows * out_dim, 16) : 0;
 }
 static int64_t fp8_blocks(int64_t n) { return (n + kF8Block - 1) / kF8Block; }
@@ -609,7 +609,7 @@ int moe_fp8_matmul_async(const void *x, int64_t ldx, int32_t x_dtype, const floa
     g.b_stride = groups > 1 ? w_stride : 0;
     g.offsets = offsets, g.E = groups, g.rows = rows;
     g.N = out_dim, g.K = in_dim, g.c_f32 = y_dtype == MOE_F32;
-    g.splits = op_rows_splits(OT_F8, false, rows, groups, out_dim, in_dim, op_cus());
+    g.splits = op_f8_splits(rows, groups, out_dim, in_dim, op_cus());
     g.ws = (float *)workspace;
     g.sa = x_scale, g.sb = w_scale, g.kb = (int)kb;
     return op_done(fn, launch_op_gemm_f8(g, op_cus(), (hipStream_t)stream));

@@ -135,19 +135,91 @@ inline int op_matrix_splits(int ot, long long rows, long long E, long long M, lo
     return ot == OT_F32 ? op_tile_splits(tiles, rows / E, 800, 4000, ncu) : op_splits(tiles, rows / E, 512, ncu);
 }
 
+// Few rows per group of a gated forward product: streamed, against tiles, us: 8 bf16 experts of
+// 4096 / 14336, 1 row each 354 / 368, 8 333 / 352, 16 377 / 367; of 2048 / 4096, 2 rows 47 / 54, 4 60 / 52; one
+// of 4096 / 4096, 8 rows 17 / 33, 16 26 / 20; 64 of 1408 / 2048, 1 row 142 / 142, 8 162 / 146; fp32, 8 of 2048 /
+// 4096, 16 rows 112 / 158.
+inline bool op_gated_streamed(int ot, bool b_col, long long rows, long long E, long long N, long long K, int ncu) {
+    if (b_col) return false;
+    if (ot == OT_F32) return rows <= 16 * E;
+    const long long bytes = K * op_size(ot);
+    const bool few = (E < rows ? E : rows) * ((2 * N + 63) / 64) < ncu;
+    if (rows > 8 * E) return false;
+    if (bytes % 4) return few && (bytes < 4096 || rows <= E);  // (as op_streamed)
+    return few || bytes >= 8192 || (bytes >= 4096 && rows <= 2 * E);
+}
 // The gated products, by the sizes of the product that they are: 2 hidden columns (two
 // weights), one product of dh, 2 hidden elements of k.  The gradients are never streamed.
 inline int op_gated_splits(OpMode mode, int ot, bool b_col, long long rows, long long E, long long N, long long K, int ncu) {
-    if (mode == OM_GATED && op_streamed(ot, b_col, rows, E, N, K, ncu)) return op_rows_splits(ot, b_col, rows, E, N, K, ncu);
+    if (mode == OM_GATED && op_gated_streamed(ot, b_col, rows, E, N, K, ncu)) {
+        const long long held = E < rows ? E : rows;
+        return op_splits(held * ((N + 15) / 16), K * op_size(ot), 8192, ncu);
+    }
     return op_rows_splits(ot, true, rows, E, mode == OM_GATED ? 2 * N : N, mode == OM_TWO ? 2 * K : K, ncu);
 }
 
-// bf16 OM_TWO on 256 x 256 tiles: the last round is split where there are few of them and k
-// (of both pairs) is long.
+// Tiles of the gated and 8-bit products: 256 x 256 (one workgroup per CU), 128 x 128 (two) or
+// 64 x 64 (three), by the rounds that each takes and a round's time, the 128 x 128 one's as
+// 100.  N: columns of products.  Measured, us, 256 / 128 / 64 (bf16 gated: a round 165 / 100 / 65):
+// forward of 24576 rows on 64 experts 2048 / 1408 367 / 390 / 646, of 2048 rows on 8 of 4096 / 2048
+// 117 / 140 / 199, of 512 rows on 8 of 4096 / 4096 122 / 105 / 129; through the down product
+// 266 / 247 / 369, 101 / 60 / 75, 101 / 75 / 82; row gradient of 4096 rows on 8 of 2048 / 4096
+// 209 / 247 / 300.  8-bit, bf16 result (170 / 100 / 60): 24576 rows 109 / 119 / 192, 4096 rows on 8 of
+// 2048 / 4096 64 / 54 / 79, 3102 rows on 64 of 1408 / 2048 48 / 39 / 45; fp32 result (- / 100 / 50): 2048
+// rows on 8 of 4096 / 2048 - / 62 / 58, 4096 rows - / 83 / 103.
+struct OpTileCost {
+    int c256, c128, c64;  // 0: none of these
+};
+constexpr OpTileCost kCostGated = {165, 100, 65}, kCostF8 = {170, 100, 60}, kCostF8Wide = {0, 100, 50};
+// tail: the last round of 256 x 256 tiles is split
+inline int op_pick_tile(const OpTileCost &c, long long rows, long long E, long long N, int ncu, bool tail) {
+    const long long held = E < rows ? E : rows;
+    auto tiles = [&](int b) -> long long {  // a group's last tile is half empty on average
+        const long long mt = E > 1 ? rows / b + held / 2 : (rows + b - 1) / b;
+        return (mt > held ? mt : held) * ((N + b - 1) / b);
+    };
+    auto rounds = [&](int b, long long slots) { return (tiles(b) + slots - 1) / slots; };
+    long long best = rounds(64, 3ll * ncu) * c.c64;
+    int pick = 64;
+    // (groups of fewer rows leave most of a tile empty)
+    if (c.c128 && rows >= 40 * E && N >= 64) {
+        const long long t = rounds(128, 2ll * ncu) * c.c128;
+        if (t <= best) best = t, pick = 128;
+    }
+    if (c.c256 && rows >= 96 * E && N >= 192) {
+        long long t = rounds(256, ncu) * c.c256;
+        if (tail) {
+            const long long whole = tiles(256) / ncu, left = tiles(256) - whole * ncu;
+            t = whole * c.c256 + (left ? c.c256 / (ncu / left) + c.c256 / 10 : 0);
+        }
+        if (t <= best) best = t, pick = 256;
+    }
+    return pick;
+}
+// bf16 OM_TWO on 256 x 256 tiles: the last round is split where rounds are few and k (of both
+// pairs) is long.  8192 rows on 8 skewed experts of 4096 / 14336, 2.25 rounds: 2298 us whole, 1775
+// split.
 constexpr int kOpTailTile = 256 * 256;  // sums of a split tile in ws
 inline bool op_two_tail(int ot, long long rows, long long E, long long N, long long K, int ncu) {
-    const long long mt = rows / 256 > E ? rows / 256 : (E < rows ? E : rows), tiles = mt * ((N + 255) / 256);
-    return ot == OT_BF16 && rows >= 192 * E && N >= 192 && tiles >= 2 * ncu && tiles < 8 * ncu && 2 * K >= 8192;
+    if (ot != OT_BF16 || 2 * K < 8192 || ncu < 8) return false;
+    const long long held = E < rows ? E : rows, tiles = (rows / 256 + held / 2) * ((N + 255) / 256);
+    return tiles < 8 * ncu && op_pick_tile(kCostGated, rows, E, N, ncu, true) == 256;
+}
+// 8-bit products of few rows: streamed where 64 x 64 tiles are fewer than CUs, or of long rows.
+// Streamed / tiles, us: 8 experts of 4096 / 14336, a row on two of them 30.5 / 32.7, 1 row each 101 /
+// 109, 4 104 / 110, 8 113 / 110; of 2048 / 4096, 1 row 14.5 / 17.0, 4 15.8 / 16.8, 8 17.6 / 16.9; 64 of
+// 1408 / 2048 48 / 44.
+inline bool op_f8_streamed(long long rows, long long E, long long N, long long K, int ncu) {
+    const long long held = E < rows ? E : rows;
+    const bool few = held * ((N + 63) / 64) < ncu;
+    if (rows > 8 * E) return false;
+    if (K % 4) return few && (K < 4096 || rows <= E);  // (as op_streamed)
+    return few || (K >= 2048 && rows <= 4 * E);
+}
+inline int op_f8_splits(long long rows, long long E, long long N, long long K, int ncu) {
+    if (!op_f8_streamed(rows, E, N, K, ncu)) return op_rows_splits(OT_F8, true, rows, E, N, K, ncu);
+    const long long held = E < rows ? E : rows;
+    return op_splits(held * ((N + 15) / 16), K, 8192, ncu);
 }
 
 // What a launcher answers to a call of more workgroups than one launch takes.

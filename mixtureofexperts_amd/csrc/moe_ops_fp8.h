@@ -24,29 +24,37 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 // ---- codes --------------------------------------------------------------------------
 // 448 x / m rounded to e4m3, to the bit: m a block's largest magnitude.  The product with
-// 448 / m is off by at most 2 steps of fp32; where that could cross a border between two
-// codes, 448 |x| and border * m are compared in fp64, where both are exact (27 and 29
-// bits).  Subnormal and large m are moved by 2^64 first.
+// 448 rcp(m) in fp32 is off by at most 2^-21.6 of itself (the reciprocal 2^-23, three
+// products 2^-24).
+//   bf16: 448 |x| (11 bits) and a border between two codes times m (13 bits) are equal or at
+//     least 2^-13 apart, and a third of all waves hold an equal one: the product, rounded to 15
+//     bits of fraction, is the border where the quotient is, and on its side elsewhere.
+//   fp32: where 2^-21 less and 2^-21 more round to the same code, so does the quotient.
+//     Else 448 |x| and border * m are compared in fp64, where both are exact (27 and 29 bits),
+//     x and m moved by 2^64 where m is small or large.
 struct F8Code {
-    float adj, m, mul;
-    bool live;  // (false for 0, infinity and NaN: codes 0)
+    float a;          // m
+    float mid, low, high;  // 448 / m, less and more
+    bool live;        // (false for 0, infinity and NaN: codes 0)
+    bool plain;       // they are normal numbers
     __device__ __forceinline__ explicit F8Code(unsigned bits) {
-        const float a = __uint_as_float(bits);
+        a = __uint_as_float(bits);
         live = bits != 0u && bits < 0x7f800000u;
-        adj = a > 0x1p64f ? 0x1p-64f : (a < 0x1p-64f ? 0x1p64f : 1.0f);
-        m = live ? a * adj : 1.0f;
-        mul = 448.0f / m;
+        plain = a >= 0x1p-100f && a <= 0x1p100f;
+        mid = 448.0f * __builtin_amdgcn_rcpf(a);
+        low = mid * (1.0f - 0x1p-21f), high = mid * (1.0f + 0x1p-21f);
     }
-    static __device__ __forceinline__ float offset(float y) { return fabsf(y) < 0x1p-6f ? 0x1p-6f : 0.0f; }
-    // whether a border may lie within y's roundings: 20 bits below e4m3's three (of y
-    // below 2^-6, whose codes are 2^-9 apart, those of |y| + 2^-6)
-    static __device__ __forceinline__ bool near_border(float y) {
-        const unsigned t = __float_as_uint(fabsf(y) + offset(y)) & 0xfffffu;
-        return t - 0x7fff8u <= 16u;
+    static __device__ __forceinline__ float snapped(float y) {
+        return __uint_as_float((__float_as_uint(y) + 0x80u) & 0xffffff00u);
     }
-    __device__ __forceinline__ float rough(float x) const { return live ? x * adj * mul : 0.0f; }
-    __device__ __forceinline__ float decided(float x, float y) const {
-        const float off = offset(y), z = fabsf(y) + off;
+    __device__ __forceinline__ float decided(float x) const {
+        const float adj = a > 0x1p64f ? 0x1p-64f : (a < 0x1p-64f ? 0x1p64f : 1.0f), m = a * adj;
+        const float y = x * adj * (448.0f / m);  // off by 2^-22 at most
+        // 20 bits below e4m3's three; of |y| below 2^-6, whose codes are 2^-9 apart, those
+        // of |y| + 2^-6
+        const float off = fabsf(y) < 0x1p-6f ? 0x1p-6f : 0.0f, z = fabsf(y) + off;
+        const unsigned t = __float_as_uint(z) & 0xfffffu;
+        if (t - 0x7fff8u > 16u) return y;  // no border within y's roundings
         const unsigned mid = (__float_as_uint(z) & 0xfff00000u) | 0x80000u;
         const double border = ((double)__uint_as_float(mid) - (double)off) * (double)m;
         const double v = 448.0 * (double)fabsf(x * adj);
@@ -54,107 +62,154 @@ struct F8Code {
         return copysignf(__uint_as_float(r) - off, x);
     }
 };
-
-// N values' codes, four to a dword.
-template <int N>
-__device__ __forceinline__ void f8_codes(const F8Code &code, const float (&x)[N], unsigned (&out)[N / 4]) {
-    float y[N];
-    bool near = false;
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-        y[k] = code.rough(x[k]);
-        near |= F8Code::near_border(y[k]);
-    }
-    if (near && code.live) {
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (F8Code::near_border(y[k])) y[k] = code.decided(x[k], y[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < N / 4; ++k) {
-        int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * k], y[4 * k + 1], 0, false);
-        w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * k + 2], y[4 * k + 3], w, true);
-        out[k] = (unsigned)w;
-    }
+__device__ __forceinline__ unsigned f8_pack(float a, float b, float c, float d) {
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
-// Eight columns from c on of a row (those past cols are 0).
-template <int XB, bool VEC>
-__device__ __forceinline__ void f8_load(const void *row, int c, int cols, float (&v)[8]) {
-    if constexpr (VEC) {
+// Eight columns from c on of a row (those past cols are 0), as they are in memory.
+template <int XB>
+struct F8Raw {
+    unsigned w[XB ? 4 : 8];
+    __device__ __forceinline__ F8Raw() {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-        if (c >= cols) return;
+        for (unsigned &x : w) x = 0u;
+    }
+    __device__ __forceinline__ float at(int k) const {
+        if constexpr (XB) return __uint_as_float(k & 1 ? w[k / 2] & 0xffff0000u : w[k / 2] << 16);
+        else return __uint_as_float(w[k]);
+    }
+    // bits of the largest magnitude (infinities and NaNs above all numbers)
+    __device__ __forceinline__ unsigned largest() const {
         if constexpr (XB) {
-            const uint4 u = *(const uint4 *)((const uint16_t *)row + c);
-            const unsigned w[4] = {u.x, u.y, u.z, u.w};
+            typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+            u16x2 m = __builtin_bit_cast(u16x2, w[0] & 0x7fff7fffu);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                v[2 * k] = __uint_as_float(w[k] << 16);
-                v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-            }
+            for (int k = 1; k < 4; ++k) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[k] & 0x7fff7fffu));
+            return (unsigned)max(m[0], m[1]) << 16;
         } else {
-            const float4 a = *(const float4 *)((const float *)row + c), b = *(const float4 *)((const float *)row + c + 4);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+            unsigned m = 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) m = max(m, w[k] & 0x7fffffffu);
+            return m;
         }
+    }
+};
+template <int XB, bool VEC>
+__device__ __forceinline__ F8Raw<XB> f8_load(const void *row, int c, int cols) {
+    F8Raw<XB> r;
+    if constexpr (VEC) {
+        if (c >= cols) return r;
+        const uint4 *p = (const uint4 *)((const uint8_t *)row + (long long)c * (XB ? 2 : 4));
+#pragma unroll
+        for (int h = 0; h < (XB ? 1 : 2); ++h) {
+            const uint4 u = p[h];
+            r.w[4 * h] = u.x, r.w[4 * h + 1] = u.y, r.w[4 * h + 2] = u.z, r.w[4 * h + 3] = u.w;
+        }
+    } else if (c + 8 <= cols) {  // at any alignment
+        __builtin_memcpy(r.w, (const uint8_t *)row + (long long)c * (XB ? 2 : 4), sizeof(r.w));
     } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            v[k] = 0.0f;
-            if (c + k < cols) v[k] = XB ? bf16_to_f32(((const uint16_t *)row)[c + k]) : ((const float *)row)[c + k];
+            if (c + k >= cols) continue;
+            if constexpr (XB) r.w[k / 2] |= (unsigned)((const uint16_t *)row)[c + k] << (16 * (k & 1));
+            else r.w[k] = ((const unsigned *)row)[c + k];
         }
     }
+    return r;
+}
+template <int XB>
+__device__ __forceinline__ void f8_codes8(const F8Code &code, const F8Raw<XB> &raw, unsigned (&w)[2]) {
+    unsigned lo[2], hi[2];
+    bool sure = code.plain;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float v[4];
+        if constexpr (XB) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = F8Code::snapped(raw.at(4 * h + k) * code.mid);
+            lo[h] = f8_pack(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = raw.at(4 * h + k);
+            lo[h] = f8_pack(v[0] * code.low, v[1] * code.low, v[2] * code.low, v[3] * code.low);
+            hi[h] = f8_pack(v[0] * code.high, v[1] * code.high, v[2] * code.high, v[3] * code.high);
+            sure &= lo[h] == hi[h];
+        }
+    }
+    if (!sure && code.live) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = code.decided(raw.at(4 * h + k));
+            lo[h] = f8_pack(v[0], v[1], v[2], v[3]);
+        }
+    }
+    w[0] = code.live ? lo[0] : 0u;
+    w[1] = code.live ? lo[1] : 0u;
 }
 template <bool VEC>
 __device__ __forceinline__ void f8_store(uint8_t *row, int c, int pad_to, const unsigned (&w)[2]) {
     if constexpr (VEC) {
         if (c < pad_to) *(uint2 *)(row + c) = make_uint2(w[0], w[1]);
+    } else if (c + 8 <= pad_to) {
+        __builtin_memcpy(row + c, w, 8);
     } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
             if (c + k < pad_to) row[c + k] = (uint8_t)(w[k >> 2] >> (8 * (k & 3)));
     }
 }
-__device__ __forceinline__ unsigned f8_largest(const float (&v)[8]) {
-    unsigned m = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
-    return m;
-}
-// over the 16 lanes of a block's row
+// over the 16 lanes of a block's row (a DPP row, rotated)
 __device__ __forceinline__ unsigned f8_over_row(unsigned m) {
-#pragma unroll
-    for (int d = 8; d > 0; d >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, d));
-    return m;
+    m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x128, 0xf, 0xf, false));
+    m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x124, 0xf, 0xf, false));
+    m = max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x122, 0xf, 0xf, false));
+    return max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x121, 0xf, 0xf, false));
 }
+// m / 448, correctly rounded: a product with 1 / 448 and one step on its remainder, which
+// an fma gives exactly (but where the quotient is subnormal, or 448 q overflows).
 __device__ __forceinline__ float f8_scale(unsigned bits) {
-    return bits < 0x7f800000u ? __uint_as_float(bits) / 448.0f : __builtin_nanf("");
+    const float m = __uint_as_float(bits), q = m * (1.0f / 448.0f);
+    float s = fmaf(fmaf(-448.0f, q, m), 1.0f / 448.0f, q);
+    if (!(m > 0x1p-90f && m < 0x1p120f)) s = bits < 0x7f800000u ? m / 448.0f : __builtin_nanf("");
+    return s;
 }
 
-// Blocks of a row: 16 lanes each, 2^lx of a workgroup's 16 along the row.
+// Blocks of a row: 16 lanes each, 2^lx of a workgroup's 16 along the row; R rows of a lane
+// on their way at once.
 template <int XB, bool VEC>
 __global__ __launch_bounds__(256) void quantize_f8_rows_kernel(QuantF8Args a, int lx) {
+    constexpr int R = 4, XS = XB ? 2 : 4;
     const int group = threadIdx.x >> 4, l = threadIdx.x & 15;
     const int kbs = (a.cols + 127) >> 7;
     const long long kb = ((long long)blockIdx.x << lx) + (group & ((1 << lx) - 1));
     if (kb >= kbs) return;
     const int c = (int)kb * 128 + l * 8;
-    constexpr int XS = XB ? 2 : 4;
+    const long long step = (long long)gridDim.y << (4 - lx);
     for (long long e = blockIdx.z; e < a.mats; e += gridDim.z) {
-        for (long long r = ((long long)blockIdx.y << (4 - lx)) + (group >> lx); r < a.rows; r += (long long)gridDim.y << (4 - lx)) {
-            float v[8];
-            f8_load<XB, VEC>((const uint8_t *)a.x + (e * a.x_stride + r * a.ldx) * XS, c, a.cols, v);
-            const unsigned m = f8_over_row(f8_largest(v));
-            if (l == 0) a.scale[(e * a.rows + r) * kbs + kb] = f8_scale(m);
-            unsigned w[2];
-            f8_codes(F8Code(m), v, w);
-            f8_store<VEC>(a.q + e * a.q_stride + r * a.ldq, c, a.pad_to, w);
+        const uint8_t *x = (const uint8_t *)a.x + e * a.x_stride * XS;
+        for (long long r0 = ((long long)blockIdx.y << (4 - lx)) + (group >> lx); r0 < a.rows; r0 += R * step) {
+            F8Raw<XB> v[R];
+#pragma unroll
+            for (int i = 0; i < R; ++i) v[i] = f8_load<XB, VEC>(x + min(r0 + i * step, a.rows - 1) * a.ldx * XS, c, a.cols);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const long long r = r0 + i * step;
+                if (r >= a.rows) continue;  // (the same for a block's 16 lanes)
+                const unsigned m = f8_over_row(v[i].largest());
+                if (l == 0) a.scale[(e * a.rows + r) * kbs + kb] = f8_scale(m);
+                unsigned w[2];
+                f8_codes8(F8Code(m), v[i], w);
+                f8_store<VEC>(a.q + e * a.q_stride + r * a.ldq, c, a.pad_to, w);
+            }
         }
     }
 }
 
 // Blocks of 128 x 128, one per workgroup: held in registers between the maximum and the
-// codes, read once.
+// codes, read once.  64 matrices of 1408 x 2048 bf16: 141 us (3.9 TB/s).
 template <int XB, bool VEC>
 __global__ __launch_bounds__(256) void quantize_f8_tiles_kernel(QuantF8Args a) {
     __shared__ unsigned part[4];
@@ -169,17 +224,15 @@ __global__ __launch_bounds__(256) void quantize_f8_tiles_kernel(QuantF8Args a) {
     const int c = kb * 128 + ((int)threadIdx.x & 15) * 8;
     const long long r0 = rb * 128 + (threadIdx.x >> 4);
     const uint8_t *x = (const uint8_t *)a.x + e * a.x_stride * XS;
-    float v[8][8];
+    F8Raw<XB> v[8];
     unsigned m = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const long long r = r0 + i * 16;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[i][k] = 0.0f;
-        if (r < a.rows) f8_load<XB, VEC>(x + r * a.ldx * XS, c, a.cols, v[i]);
+        if (r < a.rows) v[i] = f8_load<XB, VEC>(x + r * a.ldx * XS, c, a.cols);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, f8_largest(v[i]));
+    for (int i = 0; i < 8; ++i) m = max(m, v[i].largest());
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, d));
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
@@ -190,9 +243,10 @@ __global__ __launch_bounds__(256) void quantize_f8_tiles_kernel(QuantF8Args a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const long long r = r0 + i * 16;
+        if (r >= a.rows) continue;
         unsigned w[2];
-        f8_codes(code, v[i], w);
-        if (r < a.rows) f8_store<VEC>(a.q + e * a.q_stride + r * a.ldq, c, a.pad_to, w);
+        f8_codes8(code, v[i], w);
+        f8_store<VEC>(a.q + e * a.q_stride + r * a.ldq, c, a.pad_to, w);
     }
 }
 
@@ -223,36 +277,32 @@ __device__ __forceinline__ f32x4 f8_block(const F8Wide &b, const F8Wide &a) {
     return c;
 }
 
-// 16 MT rows x 16 columns by a wave, straight from global memory: pieces p, p + step, ...
+// 16 rows x 16 columns by a wave, straight from global memory: pieces p, p + step, ...
 // of the range [k0, k0 + klen).  Sums in fp64, which scales of any size cannot leave.
-template <int MT>
 __device__ __forceinline__ void f8_direct(const OpGemmArgs &g, int e, int n0, int lo, int rows, int k0, int klen, int p,
-                                          int step, double (&acc)[MT][4]) {
-    constexpr int U = MT == 1 ? 4 : 2;
+                                          int step, double (&acc)[4]) {
+    constexpr int U = 2;
     const int lane = threadIdx.x & 63, r16 = lane & 15, q4 = lane >> 4;
     // rows past the last one repeat it (their results are not stored)
+    const long long row = lo + min(r16, rows - 1);
     const uint8_t *b = (const uint8_t *)g.B + (long long)e * g.b_stride + (long long)min(n0 + r16, g.N - 1) * g.ldb + k0;
+    const uint8_t *a = (const uint8_t *)g.A + row * g.lda + k0;
     const float *sb = g.sb + ((long long)e * ((g.N + 127) >> 7) + (n0 >> 7)) * g.kb + (k0 >> 7);
-    const uint8_t *a[MT];
-    const float *sa[MT];
+    const float *sa = g.sa + row * g.kb + (k0 >> 7);
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const long long row = lo + min(m * 16 + r16, rows - 1);
-        a[m] = (const uint8_t *)g.A + row * g.lda + k0;
-        sa[m] = g.sa + row * g.kb + (k0 >> 7);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[m][c] = 0.0;
-    }
-    auto add = [&](int m, const f32x4 &v, float x, float w) {
+    for (int c = 0; c < 4; ++c) acc[c] = 0.0;
+    auto add = [&](const F8Frag &fb, const F8Frag &fa, float x, float w) {
+        const f32x4 v = f8_block(F8Wide(fb), F8Wide(fa));
         const double f = (double)x * (double)w;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[m][c] += (double)v[c] * f;
+        for (int c = 0; c < 4; ++c) acc[c] += (double)v[c] * f;
     };
     const int pieces = (klen + 127) >> 7, whole = klen >> 7;
+    // UU pieces, all loads in flight before the first product
     auto some = [&](auto UU_) {
         constexpr int UU = decltype(UU_)::value;
-        F8Frag fb[UU], fa[MT][UU];
-        float w[UU], x[MT][UU];
+        F8Frag fb[UU], fa[UU];
+        float w[UU], x[UU];
 #pragma unroll
         for (int u = 0; u < UU; ++u) {
             const int q = p + u * step;
@@ -260,41 +310,26 @@ __device__ __forceinline__ void f8_direct(const OpGemmArgs &g, int e, int n0, in
             for (int h = 0; h < 2; ++h) {
                 const long long o = (long long)q * 128 + h * 64 + q4 * 16;
                 __builtin_memcpy(&fb[u].h[h], b + o, 16);
-#pragma unroll
-                for (int m = 0; m < MT; ++m) __builtin_memcpy(&fa[m][u].h[h], a[m] + o, 16);
+                __builtin_memcpy(&fa[u].h[h], a + o, 16);
             }
             w[u] = sb[q];
-#pragma unroll
-            for (int m = 0; m < MT; ++m) x[m][u] = sa[m][q];
+            x[u] = sa[q];
         }
 #pragma unroll
-        for (int u = 0; u < UU; ++u) {
-            const F8Wide wide(fb[u]);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) add(m, f8_block(wide, F8Wide(fa[m][u])), x[m][u], w[u]);
-        }
+        for (int u = 0; u < UU; ++u) add(fb[u], fa[u], x[u], w[u]);
         p += UU * step;
     };
     while (p + (U - 1) * step < whole) some(num<U>{});
     while (p < whole) some(num<1>{});
     if (p < pieces) {  // the last, part piece
-        F8Frag fb;
+        F8Frag fb, fa;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int k = p * 128 + h * 64 + q4 * 16;
             fb.h[h] = load_chunk<1>(b + k, klen - k);
+            fa.h[h] = load_chunk<1>(a + k, klen - k);
         }
-        const F8Wide wide(fb);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            F8Frag fa;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int k = p * 128 + h * 64 + q4 * 16;
-                fa.h[h] = load_chunk<1>(a[m] + k, klen - k);
-            }
-            add(m, f8_block(wide, F8Wide(fa)), sa[m][p], sb[p]);
-        }
+        add(fb, fa, sa[p], sb[p]);
     }
 }
 
@@ -310,47 +345,33 @@ __device__ __forceinline__ void f8_put4(const OpGemmArgs &g, long long row, int 
     }
 }
 
-// As stream_rows.
-template <int MT>
-__device__ __forceinline__ void f8_stream_rows(const OpGemmArgs &g, int e, int n0, int lo, int rows, int ks, double *red) {
-    const int lane = threadIdx.x & 63, r16 = lane & 15, q4 = lane >> 4;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int k0, klen;
-    k_range(g, ks, 128, k0, klen);
-    double acc[MT][4];
-    f8_direct<MT>(g, e, n0, lo, rows, k0, klen, w, kStreamWaves, acc);
-    // red: [wave][MT][4][64 lanes]
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) red[((w * MT + m) * 4 + c) * 64 + lane] = acc[m][c];
-    __syncthreads();
-    if (w < MT) {
-        float v[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            double s = red[(w * 4 + c) * 64 + lane];
-            for (int x = 1; x < kStreamWaves; ++x) s += red[((x * MT + w) * 4 + c) * 64 + lane];
-            v[c] = (float)s;
-        }
-        const int ml = w * 16 + r16, n = n0 + 4 * q4;
-        if (ml < rows && n < g.N) f8_put4(g, lo + ml, n, ks, v);
-    }
-    __syncthreads();
-}
-
+// Few rows: as op_stream_kernel, 16 rows at a time.
 __global__ __launch_bounds__(kStreamWaves * 64) void op_f8_stream_kernel(OpGemmArgs g) {
-    __shared__ double red[kStreamWaves * 4 * 4 * 64];
-    const int r = blockIdx.x / g.nt, n0 = (blockIdx.x - r * g.nt) * 16;
-    int e, lo, hi;
+    __shared__ double red[kStreamWaves][4][64];
+    const int r = blockIdx.x / g.nt, n0 = (blockIdx.x - r * g.nt) * 16, ks = blockIdx.y;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int e, lo, hi, k0, klen;
     held_group(g, r, e, lo, hi);
     if (e < 0) return;
-    while (lo < hi) {
-        const int rows = min(hi - lo, 64);
-        if (rows <= 16) f8_stream_rows<1>(g, e, n0, lo, rows, blockIdx.y, red);
-        else if (rows <= 32) f8_stream_rows<2>(g, e, n0, lo, rows, blockIdx.y, red);
-        else f8_stream_rows<4>(g, e, n0, lo, rows, blockIdx.y, red);
-        lo += rows;
+    k_range(g, ks, 128, k0, klen);
+    for (; lo < hi; lo += 16) {
+        double acc[4];
+        f8_direct(g, e, n0, lo, min(hi - lo, 16), k0, klen, w, kStreamWaves, acc);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) red[w][c][lane] = acc[c];
+        __syncthreads();
+        if (w == 0) {
+            float v[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                double s = red[0][c][lane];
+                for (int x = 1; x < kStreamWaves; ++x) s += red[x][c][lane];
+                v[c] = (float)s;
+            }
+            const int ml = lane & 15, n = n0 + 4 * (lane >> 4);
+            if (ml < hi - lo && n < g.N) f8_put4(g, lo + ml, n, ks, v);
+        }
+        __syncthreads();
     }
 }
 
@@ -649,11 +670,11 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
         for (int j = 0; j < NJ; ++j) {
             const int n0 = jb.n0 + (wn * NJ + j) * 16;
             if (n0 >= g.N) continue;
-            double d[1][4];
-            f8_direct<1>(g, jb.e, n0, jb.lo + jb.m0 + r0, min(16, mrows - r0), k0, klen, 0, 1, d);
+            double d[4];
+            f8_direct(g, jb.e, n0, jb.lo + jb.m0 + r0, min(16, mrows - r0), k0, klen, 0, 1, d);
             const int n = n0 + 4 * q4;
             if (r0 + r16 < mrows && n < g.N) {
-                const float v[4] = {(float)d[0][0], (float)d[0][1], (float)d[0][2], (float)d[0][3]};
+                const float v[4] = {(float)d[0], (float)d[1], (float)d[2], (float)d[3]};
                 f8_put4(g, jb.lo + jb.m0 + r0 + r16, n, jb.ks, v);
             }
         }
@@ -678,7 +699,7 @@ static hipError_t launch_f8_tiles(OpGemmArgs g, int vb, hipStream_t s) {
     if (vb == 16) {
         ops::op_f8_kernel<BM, BN, WM, WN, 2, WPE, 16, WIDE><<<gr, b, 0, s>>>(g);
     } else if constexpr (BN != 64) {
-        return hipErrorInvalidValue;  // (the other loads' registers do not fit beside these tiles)
+        return hipErrorInvalidValue;
     } else if (vb == 4) {
         ops::op_f8_kernel<BM, BN, WM, WN, 2, WIDE ? 2 : WPE, 4, WIDE><<<gr, b, 0, s>>>(g);
     } else {
@@ -689,7 +710,7 @@ static hipError_t launch_f8_tiles(OpGemmArgs g, int vb, hipStream_t s) {
 }
 
 hipError_t launch_op_gemm_f8(OpGemmArgs g, int ncu, hipStream_t s) {
-    if (op_streamed(OT_F8, false, g.rows, g.E, g.N, g.K, ncu)) {
+    if (op_f8_streamed(g.rows, g.E, g.N, g.K, ncu)) {
         g.nt = (g.N + 15) / 16;
         const long long grid = (long long)(g.E < g.rows ? g.E : g.rows) * g.nt;
         if (grid * g.splits > 0x7fffffffll / (ops::kStreamWaves * 64)) return kOpTooLarge;
@@ -705,18 +726,15 @@ hipError_t launch_op_gemm_f8(OpGemmArgs g, int ncu, hipStream_t s) {
         if (pieces(16)) vb = 16;
         else if (g.lda >= 16 && g.ldb >= 16 && pieces(4)) vb = 4;
     }
-    const long long avg = (long long)g.rows / g.E;
-    auto tiles = [&](int b) -> long long {
-        const long long few = (long long)g.rows / b > g.E ? (long long)g.rows / b : (g.E < g.rows ? g.E : g.rows);
-        return few * ((g.N + b - 1) / b);
-    };
-    if (g.c_f32 || g.splits > 1) {
-        if (g.splits <= 1 && vb == 16 && avg >= 64 && g.N >= 64 && tiles(128) >= ncu)
-            return launch_f8_tiles<128, 128, 2, 2, 2, true>(g, vb, s);
-        return launch_f8_tiles<64, 64, 2, 2, 3, true>(g, vb, s);
-    }
-    if (vb == 16 && avg >= 192 && g.N >= 192 && tiles(256) >= 2 * ncu) return launch_f8_tiles<256, 256, 4, 2, 2, false>(g, vb, s);
-    if (vb == 16 && avg >= 64 && g.N >= 64 && tiles(128) >= ncu) return launch_f8_tiles<128, 128, 2, 2, 2, false>(g, vb, s);
+    // fp32 results, and sums that are folded: the codes widened (above)
+    const bool wide = g.c_f32 || g.splits > 1;
+    OpTileCost c = wide ? kCostF8Wide : kCostF8;
+    if (vb != 16) c.c256 = c.c128 = 0;  // (the other loads' registers do not fit beside these tiles)
+    const int t = g.splits > 1 ? 64 : op_pick_tile(c, g.rows, g.E, g.N, ncu, false);
+    if (t == 256) return launch_f8_tiles<256, 256, 4, 2, 2, false>(g, vb, s);
+    if (t == 128 && wide) return launch_f8_tiles<128, 128, 2, 2, 2, true>(g, vb, s);
+    if (t == 128) return launch_f8_tiles<128, 128, 2, 2, 2, false>(g, vb, s);
+    if (wide) return launch_f8_tiles<64, 64, 2, 2, 3, true>(g, vb, s);
     return launch_f8_tiles<64, 64, 2, 2, 3, false>(g, vb, s);
 }
 
@@ -729,7 +747,7 @@ static void quantize_f8(const QuantF8Args &a, hipStream_t s) {
     }
     int lx = 0;
     while (lx < 4 && (1 << lx) < kbs) ++lx;
-    const long long gy = (a.rows + (16 >> lx) - 1) >> (4 - lx);
+    const long long gy = (((a.rows + (16 >> lx) - 1) >> (4 - lx)) + 3) / 4;
     const dim3 gr((unsigned)((kbs + (1 << lx) - 1) >> lx), (unsigned)(gy < 16384 ? gy : 16384),
                   (unsigned)(a.mats < 1024 ? a.mats : 1024));
     ops::quantize_f8_rows_kernel<XB, VEC><<<gr, 256, 0, s>>>(a, lx);

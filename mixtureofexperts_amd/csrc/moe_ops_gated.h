@@ -255,7 +255,7 @@ static hipError_t gated_plan(bool b_col, const OpGemmArgs &g, int ncu, hipStream
 }
 
 hipError_t launch_op_gated(int mode, int ot, bool b_col, OpGemmArgs g, int ncu, hipStream_t s) {
-    if (mode == OM_GATED && op_streamed(ot, b_col, g.rows, g.E, g.N, g.K, ncu)) return launch_gated_stream(ot, g, s);
+    if (mode == OM_GATED && op_gated_streamed(ot, b_col, g.rows, g.E, g.N, g.K, ncu)) return launch_gated_stream(ot, g, s);
     if (ot == OT_F32) {
         if (mode == OM_GATED) return gated_plan<OT_F32, OM_GATED>(b_col, g, ncu, s);
         if (mode == OM_GATE_GRAD) return gated_plan<OT_F32, OM_GATE_GRAD>(b_col, g, ncu, s);

@@ -1283,10 +1283,17 @@ hipError_t op_gemm_plan(OpGemmArgs g, int ncu, hipStream_t s) {
     };
     const long long avg = RAGK ? g.M : (long long)g.rows / g.E;
     if (g.splits > 1) return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, KSUB, 4 / KSUB, 3, MODE>(g, vb, s);
-    if constexpr (OT != OT_F32) {
+    if constexpr (MODE != OM_PLAIN && OT == OT_BF16) {
+        OpTileCost c = kCostGated;
+        if (vb != 16 || (MODE == OM_TWO && (g.lda != g.lda2 || g.ldb != g.ldb2))) c.c256 = 0, g.tail = 0;
+        const int b = op_pick_tile(c, g.rows, g.E, NN, ncu, g.tail > 0);
+        if (b == 256) return launch_tiles<OT, ACOL, BCOL, RAGK, 256, 256, 4, 2, KSUB, 4 / KSUB, 2, MODE>(g, vb, s);
+        if (b == 128) return launch_tiles<OT, ACOL, BCOL, RAGK, 128, 128, 2, 2, KSUB, 4 / KSUB, 2, MODE>(g, vb, s);
+        return launch_tiles<OT, ACOL, BCOL, RAGK, 64, 64, 2, 2, KSUB, 4 / KSUB, 3, MODE>(g, vb, s);
+    }
+    if constexpr (OT != OT_F32 && MODE == OM_PLAIN) {
         const bool large = RAGK ? tiles(256) >= 2 * ncu : avg >= 192 && NN >= 192 && tiles(256) >= 2 * ncu;
-        const bool one_ld = MODE != OM_TWO || (g.lda == g.lda2 && g.ldb == g.ldb2);
-        if (vb == 16 && large && one_ld)
+        if (vb == 16 && large)
             return launch_tiles<OT, ACOL, BCOL, RAGK, 256, 256, 4, 2, KSUB, 4 / KSUB, 2, MODE>(g, vb, s);
     }
     bool medium = avg >= 64 && NN >= 64 && tiles(128) >= ncu;

@@ -295,9 +295,12 @@ def _results(out, names, shape, dtypes, allowed, like, clear):
 def _two_weights(w1, w3, dtype):
     """w1 and w3 of one shape: (E, a, b), (pointer, row stride, matrix stride) of each."""
     E, a, b, ld1, s1 = _matrices(w1, "w1", (dtype,))
-    E3, a3, b3, ld3, s3 = _matrices(w3, "w3", (dtype,))
-    if (E3, a3, b3) != (E, a, b):
-        _bad(f"w1 and w3 must have one shape, got {tuple(w1.shape)} and {tuple(w3.shape)}")
+    ld3, s3 = ld1, s1
+    _tensor(w3, "w3", (dtype,), (2, 3))
+    if w3.shape != w1.shape or w3.stride() != w1.stride():
+        E3, a3, b3, ld3, s3 = _matrices(w3, "w3")
+        if (E3, a3, b3) != (E, a, b):
+            _bad(f"w1 and w3 must have one shape, got {tuple(w1.shape)} and {tuple(w3.shape)}")
     return E, a, b, (w1.data_ptr(), ld1, s1, w3.data_ptr(), ld3, s3)
 
 
@@ -322,21 +325,27 @@ def gated_matmul(x, w1, w3, offsets=None, *, activation=silu, layout=MOE_LAYOUT_
     M, dt, shape = x.shape[0], _codes[x.dtype], (x.shape[0], n)
     if out is None and out_dtype is None:
         out_dtype = x.dtype
-    kept = (x.dtype,)
+    pa = pb = None
+    lda = ldb = 0
     if save:
+        kept = (x.dtype,)
         res = _results(out, ("h", "a", "b"), shape, (out_dtype, x.dtype, x.dtype), (_float_types(x.dtype), kept, kept), x,
                        offsets is not None)
+        h, ta, tb = res
+        device = _same_device(x, w1, w3, offsets, h, ta, tb)
+        pa, lda, pb, ldb = ta.data_ptr(), _row_stride(ta, "a"), tb.data_ptr(), _row_stride(tb, "b")
     else:
-        res = (_result(out, shape, out_dtype, _float_types(x.dtype), x, offsets is not None),)
-    device = _same_device(x, w1, w3, offsets, *res)
-    ws, wsp, wsn = _workspace(_lib.lib().moe_gated_matmul_workspace, device, E, M, k, n, dt)
-    pre = [v for t, name in zip(res[1:], "ab") for v in (t.data_ptr(), _row_stride(t, name))] or [None, 0, None, 0]
-    _call(_lib.lib().moe_gated_matmul_async, device, xp, ldx, *w, layout, act, _offsets(offsets, E), E, M, k, n, dt,
-          res[0].data_ptr(), _row_stride(res[0], "out"), _codes[res[0].dtype], *pre, wsp, wsn)
+        h = _result(out, shape, out_dtype, _float_types(x.dtype), x, offsets is not None)
+        res = (h,)
+        device = _same_device(x, w1, w3, offsets, h)
+    L = _lib.lib()
+    ws, wsp, wsn = _workspace(L.moe_gated_matmul_workspace, device, E, M, k, n, dt)
+    _call(L.moe_gated_matmul_async, device, xp, ldx, *w, layout, act, _offsets(offsets, E), E, M, k, n, dt,
+          h.data_ptr(), _row_stride(h, "out"), _codes[h.dtype], pa, lda, pb, ldb, wsp, wsn)
     if given is not None:
         for t in res:
             _written(t)  # autograd sees the caller's tensors change
-    return res if save else res[0]
+    return res if save else h
 
 
 def gated_matmul_grad(dy, a, b, w2=None, offsets=None, *, activation=silu, layout=MOE_LAYOUT_LLAMA_IN_OUT, out=None):

@@ -221,7 +221,7 @@ def test_fp8_matmul(moe, xt, odt, wpad):
 
 def test_large_tiles(moe):
     rng = np.random.default_rng(5)
-    for lens, K, N in (([3000, 5500], 160, 4112), ([2100, 1, 3000, 3400], 272, 4040)):
+    for lens, K, N in (([3000, 5500], 160, 7168), ([2100, 1, 3000, 3400], 272, 7064)):
         x, xs = _codes(rng, (sum(lens), K)).cuda().view(F8), _scales(rng, (sum(lens), -(-K // 128))).cuda()
         w, ws = _weights(rng, len(lens), N, K, 0)
         off = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
@@ -234,7 +234,7 @@ def test_large_tiles(moe):
 
 
 def test_forms(moe):
-    for lens, K, N, tile, split in (([3000, 5500], 160, 4112, "256", False), ([700, 0, 900, 500], 144, 2048, "128", False),
+    for lens, K, N, tile, split in (([3000, 5500], 160, 7168, "256", False), ([700, 0, 900, 500], 144, 2048, "128", False),
                                     ([33, 130, 5, 0, 300], 208, 136, "64", False), ([40, 30], 20000, 33, "64", True),
                                     ([0, 3, 0], 7, 5, None, False), ([0, 9, 0], 5001, 50, "64", True),
                                     ([0, 0, 2, 0, 1, 0, 0], 20000, 17, None, True)):
