@@ -496,27 +496,28 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
     float f[2][MI];
 #pragma unroll
     for (int i = 0; i < MI; ++i) part[1][i] = f32x4{0, 0, 0, 0}, f[1][i] = 0.0f;
-    auto scaled = [&](int j, const f32x4 (&p)[MI], const float (&by)[MI]) {
+    // NI: the wave's row blocks that hold rows
+    auto scaled = [&](auto NI, int j, const f32x4 (&p)[MI], const float (&by)[MI]) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
+        for (int i = 0; i < decltype(NI)::value; ++i)
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[i][j][c] = fmaf(p[i][c], by[i], acc[i][j][c]);
     };
     // P: the parity of the stage
-    auto step = [&](auto P, int j) {
+    auto step = [&](auto NI, auto P, int j) {
         constexpr int p = decltype(P)::value;
         const FragA b(fb[j & 1]);
 #pragma unroll
-        for (int i = 0; i < MI; ++i) part[j & 1][i] = f8_block(b, fa[i]);
-        if (j == 0) scaled(NJ - 1, part[1], f[1 - p]);
-        else scaled(j - 1, part[1 - (j & 1)], f[p]);
+        for (int i = 0; i < decltype(NI)::value; ++i) part[j & 1][i] = f8_block(b, fa[i]);
+        if (j == 0) scaled(NI, NJ - 1, part[1], f[1 - p]);
+        else scaled(NI, j - 1, part[1 - (j & 1)], f[p]);
     };
     // the order of a step: reads first, then after each MFMA what fits under it
-    auto mixed = [] {
+    auto mixed = [](auto NI) {
         if constexpr (!WIDE) {
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
 #pragma unroll
-            for (int i = 0; i < MI; ++i) {
+            for (int i = 0; i < decltype(NI)::value; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
             }
@@ -549,46 +550,67 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
             wait_loads<NL>();
             lds_barrier();
             read_scales(num<0>{}, f[0]);
+            auto run = [&](auto NI_) {
+                constexpr int NI = decltype(NI_)::value;
 #pragma unroll
-            for (int i = 0; i < MI; ++i) fa[i] = read_a(num<0>{}, i);
-            fb[0] = read_b(num<0>{}, 0);
-            auto stage = [&](auto SLOT, int s) {
-                constexpr int P = decltype(SLOT)::value;
-                using Next = num<1 - P>;
+                for (int i = 0; i < NI; ++i) fa[i] = read_a(num<0>{}, i);
+                if constexpr (NI > 0) fb[0] = read_b(num<0>{}, 0);
+                auto stage = [&](auto SLOT, int s) {
+                    constexpr int P = decltype(SLOT)::value;
+                    using Next = num<1 - P>;
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    if (j < NJ - 1) {
-                        fb[1 - (j & 1)] = read_b(SLOT, j + 1);
-                        step(SLOT, j);
-                        mixed();
-                    } else {
-                        wait_loads<0>();
-                        lds_barrier();
-                        fb[0] = read_b(Next{}, 0);
-                        const FragA b(fb[1]);
+                    for (int j = 0; j < NJ; ++j) {
+                        if (j < NJ - 1) {
+                            if constexpr (NI > 0) {
+                                fb[1 - (j & 1)] = read_b(SLOT, j + 1);
+                                step(NI_, SLOT, j);
+                                mixed(NI_);
+                            }
+                        } else {
+                            wait_loads<0>();
+                            lds_barrier();
+                            const F8Frag last = fb[1];
+                            if constexpr (NI > 0) fb[0] = read_b(Next{}, 0);
+                            const FragA b(last);
 #pragma unroll
-                        for (int i = 0; i < MI; ++i) {
-                            part[1][i] = f8_block(b, fa[i]);
-                            fa[i] = read_a(Next{}, i);
+                            for (int i = 0; i < MI; ++i) {
+                                if (i < NI) {
+                                    part[1][i] = f8_block(b, fa[i]);
+                                    fa[i] = read_a(Next{}, i);
 #pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                acc[i][j - 1][c] = fmaf(part[0][i][c], f[P][i], acc[i][j - 1][c]);
-                            if (i == 0) ta.load_lds(s + NS, l0 + a_slot(SLOT), w);
-                            if (i == 1) tb.load_lds(s + NS, l0 + b_slot(SLOT), w);
-                            if (i == MI - 1) load_scales(SLOT, s + NS);
-                            __builtin_amdgcn_sched_barrier(0);
+                                    for (int c = 0; c < 4; ++c)
+                                        acc[i][j - 1][c] = fmaf(part[0][i][c], f[P][i], acc[i][j - 1][c]);
+                                }
+                                if (i == 0) ta.load_lds(s + NS, l0 + a_slot(SLOT), w);
+                                if (i == 1) tb.load_lds(s + NS, l0 + b_slot(SLOT), w);
+                                if (i == MI - 1) load_scales(SLOT, s + NS);
+                                __builtin_amdgcn_sched_barrier(0);
+                            }
+                            read_scales(Next{}, f[1 - P]);
                         }
-                        read_scales(Next{}, f[1 - P]);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-                    __builtin_amdgcn_sched_barrier(0);
+                };
+                int s = 0;
+                for (; s + 2 <= S; s += 2) {
+                    stage(num<0>{}, s);
+                    stage(num<1>{}, s + 1);
                 }
+                if (s < S) stage(num<0>{}, s);
+#pragma unroll
+                for (int i = 0; i < NI; ++i) f[1][i] = (S & 1) ? f[0][i] : f[1][i];
+                scaled(NI_, NJ - 1, part[1], f[1]);
             };
-            int s = 0;
-            for (; s + 2 <= S; s += 2) {
-                stage(num<0>{}, s);
-                stage(num<1>{}, s + 1);
+            if constexpr (MI < 4) {
+                run(num<MI>{});
+            } else {
+                const int ni = (mrows - wm * 16 + WM * 16 - 1) / (WM * 16);
+                if (ni >= MI) run(num<MI>{});
+                else if (ni == 3) run(num<3>{});
+                else if (ni == 2) run(num<2>{});
+                else if (ni == 1) run(num<1>{});
+                else run(num<0>{});
             }
-            if (s < S) stage(num<0>{}, s);
             wait_loads<0>();  // no load may still be writing LDS when the workgroup ends
         } else {
             float sreg = 0.0f;
@@ -614,7 +636,7 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
                     if (j < NJ - 1) fb[1 - (j & 1)] = read_b(SLOT, j + 1);
-                    step(SLOT, j);
+                    step(num<MI>{}, SLOT, j);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 if (s + 1 < S) keep(num<1 - decltype(SLOT)::value>{});
@@ -627,10 +649,10 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
                 stage(num<1>{}, s + 1);
             }
             if (s < S) stage(num<0>{}, s);
-        }
 #pragma unroll
-        for (int i = 0; i < MI; ++i) f[1][i] = (S & 1) ? f[0][i] : f[1][i];
-        scaled(NJ - 1, part[1], f[1]);
+            for (int i = 0; i < MI; ++i) f[1][i] = (S & 1) ? f[0][i] : f[1][i];
+            scaled(num<MI>{}, NJ - 1, part[1], f[1]);
+        }
     }
     typedef __attribute__((address_space(3))) int lds_int;
     lds_int *flags = (lds_int *)(ring + SCALES + NS * NT * 4);
@@ -664,6 +686,9 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
 #pragma unroll
     for (int i = 0; i < WM * WN; ++i) far |= flags[i];
     if (__builtin_amdgcn_readfirstlane(far) == 0) return;
+    // (opaque: addresses formed from them before the loop would be kept through it)
+    int e = jb.e, row0 = jb.lo + jb.m0;
+    asm("" : "+s"(e), "+s"(row0));
     for (int i = 0; i < MI; ++i) {
         const int r0 = (i * WM + wm) * 16;
         if (r0 >= mrows) continue;
@@ -671,11 +696,11 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
             const int n0 = jb.n0 + (wn * NJ + j) * 16;
             if (n0 >= g.N) continue;
             double d[4];
-            f8_direct(g, jb.e, n0, jb.lo + jb.m0 + r0, min(16, mrows - r0), k0, klen, 0, 1, d);
+            f8_direct(g, e, n0, row0 + r0, min(16, mrows - r0), k0, klen, 0, 1, d);
             const int n = n0 + 4 * q4;
             if (r0 + r16 < mrows && n < g.N) {
                 const float v[4] = {(float)d[0], (float)d[1], (float)d[2], (float)d[3]};
-                f8_put4(g, jb.lo + jb.m0 + r0 + r16, n, jb.ks, v);
+                f8_put4(g, row0 + r0 + r16, n, jb.ks, v);
             }
         }
     }

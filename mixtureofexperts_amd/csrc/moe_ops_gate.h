@@ -100,14 +100,22 @@ struct GateChunk {
             }
         }
     }
+    // PAST: around the caches
+    template <bool PAST>
     __device__ __forceinline__ void store(void *row, int n, int N) const {
+        typedef unsigned u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
+        auto put = [&](auto &whole, void *at) {
+            const u32x4_u t = __builtin_bit_cast(u32x4_u, whole);
+            if constexpr (PAST) __builtin_nontemporal_store(t, (u32x4_u *)at);
+            else *(u32x4_u *)at = t;
+        };
         if constexpr (BF16) {
             typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
             bf16x8 o;
 #pragma unroll
             for (int q = 0; q < CE; ++q) o[q] = (__bf16)v[q];
             if (n + CE <= N) {
-                __builtin_memcpy((uint16_t *)row + n, &o, 16);
+                put(o, (uint16_t *)row + n);
             } else {
 #pragma unroll
                 for (int q = 0; q < CE; ++q)
@@ -115,7 +123,7 @@ struct GateChunk {
             }
         } else {
             if (n + CE <= N) {
-                __builtin_memcpy((float *)row + n, v, 16);
+                put(v, (float *)row + n);
             } else {
 #pragma unroll
                 for (int q = 0; q < CE; ++q)
@@ -133,7 +141,7 @@ __device__ __forceinline__ void gate_load_ab(const OpGemmArgs &g, long long row,
     b = gate_load<BF16>((const uint8_t *)g.gb + row * g.ldgb * ES, n, g.N);
 }
 // da, db and h there from dh.
-template <bool BF16>
+template <bool BF16, bool PAST = false>
 __device__ __forceinline__ void gate_store(const OpGemmArgs &g, long long row, int n, const GateChunk<BF16> &dh,
                                            const GateRaw &ra, const GateRaw &rb) {
     constexpr int ES = BF16 ? 2 : 4;
@@ -149,9 +157,9 @@ __device__ __forceinline__ void gate_store(const OpGemmArgs &g, long long row, i
     };
     if (gate.smooth) all(std::true_type{});
     else all(std::false_type{});
-    da.store((uint8_t *)g.C + row * g.ldc * ES, n, g.N);
-    db.store((uint8_t *)g.C2 + row * g.ldc2 * ES, n, g.N);
-    h.store((uint8_t *)g.C3 + row * g.ldc3 * ES, n, g.N);
+    da.template store<PAST>((uint8_t *)g.C + row * g.ldc * ES, n, g.N);
+    db.template store<PAST>((uint8_t *)g.C2 + row * g.ldc2 * ES, n, g.N);
+    h.template store<PAST>((uint8_t *)g.C3 + row * g.ldc3 * ES, n, g.N);
 }
 
 }  // namespace ops
