@@ -280,6 +280,65 @@ def test_far_scales(moe, lens, K, N):
             assert (np.abs(_f64(y)[r] - ref) <= (K + 4) * 2.0**-23 * mag + np.abs(ref) * 2.0**-24 + 1e-37).all(), scale
 
 
+def test_far_scales_of_bf16_results(moe):
+    # the same from the 8-bit instruction's tiles, 256 x 256, 128 x 128 and 64 x 64
+    rng = np.random.default_rng(17)
+    for lens, K, N in (([70, 30], 300, 40), ([700, 900], 144, 2048), ([3000, 5500], 160, 7168)):
+        M, kb = sum(lens), -(-K // 128)
+        off = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+        x, xs = _codes(rng, (M, K)), _scales(rng, (M, kb))
+        x[1], xs[1] = 0x38, 2.0**-125  # ones
+        w, ws = _weights(rng, len(lens), N, K, 0)
+        ws = ws * 2.0**-10
+        x, xs = x.cuda().view(F8), xs.cuda()
+        y = moe.fp8_matmul(x, w, ws, off, x_scale=xs)
+        want = moe.fp8_matmul(x, w, ws, off, x_scale=xs, out_dtype=torch.float32)
+        assert torch.equal(y[1], want[1].to(torch.bfloat16)) and (want[1] != 0).any()
+        _check_product([2], _f64(y[:2]), x[:2], xs[:2], w[:1], ws[:1], "bf16")
+
+
+def test_codes_that_are_no_numbers(moe):
+    # a NaN code of the rows makes its row NaN, one of the weights its column, no others
+    rng = np.random.default_rng(19)
+    for lens, K, N in (([3], 300, 40), ([70, 30], 300, 40), ([700, 900], 144, 2048)):
+        off = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+        x, xs = _codes(rng, (sum(lens), K)), _scales(rng, (sum(lens), -(-K // 128))).cuda()
+        w, ws = _weights(rng, len(lens), N, K, 0)
+        x[2, K - 1] = 0xFF
+        w.view(torch.uint8)[0, 5, 130 % K] = 0x7F
+        for odt in ("bf16", "f32"):
+            y = moe.fp8_matmul(x.cuda().view(F8), w, ws, off, x_scale=xs, out_dtype=DT[odt])
+            bad = torch.isnan(y).cpu()
+            want = torch.zeros_like(bad)
+            want[2], want[:lens[0], 5] = True, True
+            assert torch.equal(bad, want)
+
+
+def test_many_groups(moe):
+    rng = np.random.default_rng(18)
+    E, K, N = 700, 136, 24
+    lens = [int(v) for v in rng.integers(0, 3, E)]
+    M = sum(lens)
+    off = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+    x, xs = _codes(rng, (M + 9, K)).cuda().view(F8), _scales(rng, (M + 9, 2)).cuda()
+    w, ws = _weights(rng, E, N, K, 0)
+    y = moe.fp8_matmul(x, w, ws, off, x_scale=xs, out_dtype=torch.float32)
+    _check_product(lens, _f64(y), x, xs, w, ws, "f32")
+    assert (y[M:] == 0).all()
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_ties_of_bf16_values(moe, dtype, block_rows):
+    # values with bf16's eight bits meet borders exactly, again and again
+    rng = np.random.default_rng(20)
+    x = torch.from_numpy(rng.standard_normal((3, 256, 512))).to(torch.bfloat16).to(DT[dtype]).cuda()
+    x[1] = (x[1].float() * 2.0**-110).to(DT[dtype])
+    x[2] = (x[2].float() * 2.0**110).to(DT[dtype])
+    q, s = moe.quantize_fp8(x, block_rows=block_rows)
+    _check_codes(_f64(x), q, s, block_rows, "ties")
+
+
 def test_not_finite(moe):
     # a block that holds an infinity or a NaN makes its row NaN and no other; zero blocks
     # and rows of zeros give zeros

@@ -202,13 +202,18 @@ def test_large_tiles(moe, layout):
     res = []
     names = kernels_of(lambda: res.append(moe.gated_matmul(x, w1, w3, off, layout=layout, save=True)))
     assert _tile(names, 1) == (256, 16)
-    h, a, b = res[-1]
-    _check_forward(lens, "silu", [_f64(t) for t in (h, a, b)], x, w1, w3, layout, K, "bf16", "bf16")
+    _check_forward(lens, "silu", [_f64(t) for t in res[-1]], x, w1, w3, layout, K, "bf16", "bf16")
+    for act in ACTS[1:]:
+        h = moe.gated_matmul(x, w1, w3, off, layout=layout, activation=getattr(moe, act), out_dtype=torch.float32)
+        _check_forward(lens, act, [_f64(h)], x, w1, w3, layout, K, "bf16", "f32")
     dy, w2 = _rows(rng, M, K, "bf16", 8), _mats(rng, 4, K, 2 * H, "bf16", layout)
     a, b = _rows(rng, M, 2 * H, "bf16"), _rows(rng, M, 2 * H, "bf16", 8)
     names = kernels_of(lambda: res.append(moe.gated_matmul_grad(dy, a, b, w2, off, layout=layout)))
     assert _tile(names, 2) == (256, 16)
     _check_grad(lens, "silu", [_f64(t) for t in res[-1]], dy, a, b, w2, layout, K, "bf16")
+    for act in ACTS[1:]:
+        grads = moe.gated_matmul_grad(dy, a, b, w2, off, layout=layout, activation=getattr(moe, act))
+        _check_grad(lens, act, [_f64(t) for t in grads], dy, a, b, w2, layout, K, "bf16")
     # the two pairs' strides alike: 256 x 256 tiles; apart: 128 x 128
     for p, q, rows in ((0, 0, 256), (8, 0, 128), (0, 8, 128)):
         Kx, Hx = 4040, 104
@@ -217,6 +222,38 @@ def test_large_tiles(moe, layout):
         names = kernels_of(lambda: res.append(moe.gated_matmul_grad_x(da, db, v1, v3, off, layout=layout)))
         assert _tile(names, 3) == (rows, 16)
         _check_grad_x(lens, _f64(res[-1]), da, db, v1, v3, layout, Hx, "bf16")
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_every_form_of_every_activation(moe, dtype, act):
+    # 64 x 64 and 128 x 128 tiles and the streamed form, each load form, both orders
+    for lens, K, H, layout in (([40, 0, 33], 64, 72, LLAMA), ([40, 0, 33], 66, 74, FLUX), ([40, 0, 33], 65, 73, LLAMA),
+                               ([3, 0, 1], 64, 72, LLAMA), ([700, 0, 900, 500], 72, 1024, LLAMA),
+                               ([700, 0, 900, 500], 74, 1026, FLUX), ([700, 0, 900, 500], 73, 1025, FLUX)):
+        rng = np.random.default_rng([K, H, layout, 4])
+        M, off, fn = sum(lens), _offsets(lens), getattr(moe, act)
+        x, w1, w3 = _rows(rng, M, K, dtype), *(_mats(rng, len(lens), H, K, dtype, layout) for _ in range(2))
+        print(f"gated forms {dtype} {act} lens={lens} K={K} H={H} layout={layout}", flush=True)
+        res = moe.gated_matmul(x, w1, w3, off, activation=fn, layout=layout, save=True)
+        _check_forward(lens, act, [_f64(t) for t in res], x, w1, w3, layout, K, dtype, dtype)
+        w2, dy = _mats(rng, len(lens), K, H, dtype, layout), _rows(rng, M, K, dtype)
+        grads = moe.gated_matmul_grad(dy, res[1], res[2], w2, off, activation=fn, layout=layout)
+        _check_grad(lens, act, [_f64(t) for t in grads], dy, res[1], res[2], w2, layout, K, dtype)
+
+
+def test_many_groups(moe):
+    # more groups than rows, and more than a wave's scan; rows behind the last one
+    rng = np.random.default_rng(18)
+    E, K, H = 700, 32, 24
+    lens = [int(v) for v in rng.integers(0, 3, E)]
+    M, off = sum(lens), _offsets(lens)
+    x, w1, w3 = _rows(rng, M, K, "bf16", 0, 9), *(_mats(rng, E, H, K, "bf16", LLAMA) for _ in range(2))
+    h, a, b = moe.gated_matmul(x, w1, w3, off, save=True)
+    _check_forward(lens, "silu", [_f64(t) for t in (h, a, b)], x, w1, w3, LLAMA, K, "bf16", "bf16")
+    dx = moe.gated_matmul_grad_x(a, b, w1, w3, off)
+    _check_grad_x(lens, _f64(dx), a, b, w1, w3, LLAMA, H, "bf16")
+    assert (h[M:] == 0).all() and (dx[M:] == 0).all()
 
 
 @pytest.mark.parametrize("layout", [LLAMA, FLUX])
