@@ -1179,12 +1179,28 @@ __global__ __launch_bounds__(WM * WN * 64) void op_tail_fold_kernel(OpGemmArgs g
     if (n >= g.N) return;
     const f32x4 *ws = (const f32x4 *)g.ws + (long long)(xcd * g.tail + tile * tail.parts) * (MI * NJ * NT) + threadIdx.x;
     const bool vec = vec_ok(g);
+    f32x4 v[MI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i) v[i] = f32x4{0, 0, 0, 0};
+    for (int p = 0; p < tail.parts; p += 2) {  // two ranges' loads on their way at once
+        const bool two = p + 1 < tail.parts;
+        f32x4 a[MI], b[MI];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            a[i] = ws[((long long)p * MI * NJ + i * NJ + j) * NT];
+            b[i] = ws[((long long)(two ? p + 1 : p) * MI * NJ + i * NJ + j) * NT];
+        }
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            v[i] += a[i];
+            if (two) v[i] += b[i];
+        }
+    }
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-        f32x4 v = {0, 0, 0, 0};
-        for (int p = 0; p < tail.parts; ++p) v += ws[((long long)p * MI * NJ + i * NJ + j) * NT];
         const int ml = (i * WM + wm) * 16 + r16;
-        if (ml < jb.len - jb.m0) put4(g, (long long)(jb.lo + jb.m0 + ml) * g.ldc + n, n, v[0], v[1], v[2], v[3], vec);
+        if (ml < jb.len - jb.m0)
+            put4(g, (long long)(jb.lo + jb.m0 + ml) * g.ldc + n, n, v[i][0], v[i][1], v[i][2], v[i][3], vec);
     }
 }
 
