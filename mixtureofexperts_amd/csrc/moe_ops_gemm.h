@@ -1155,6 +1155,16 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WP
     op_gemm_tile<OT, ACOL, BCOL, RAGK, BM, BN, WM, WN, KSUB, NS, VB>(g, ring);
 }
 
+// The gated blocks, bound as the products that they are; 8192 rows, 8 bf16 experts of 4096 /
+// 14336, skewed groups (36 tiles of 256 rows where even ones have 32):
+//   forward with both pre-activations: 1780 us (1.08 PFLOP/s, units 50 % busy), its 705 MB of
+//     results after each tile's products with one workgroup per CU
+//   through the down product: 1030 us, of which the product alone is 840 (units 41 % busy): the
+//     tile's 1.2 GB of a, b and results are not under another tile's products (the gate as a
+//     launch of its own: 840 + 243)
+//   row gradient: 1770 us (1.09 PFLOP/s, units 50 % busy), 2.25 rounds of tiles; the two products and their sum in
+//     one kernel, where two calls would read and write the 134 MB of fp32 sums in between
+// Wave priorities (s_setprio) and two stages per scheduling region changed none of them.
 template <int MODE, int OT, bool BCOL, int BM, int BN, int WM, int WN, int KSUB, int NS, int WPE, int VB>
 __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void op_gated_kernel(
     OpGemmArgs g) {
@@ -1163,7 +1173,8 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WP
 }
 
 // Results of the split tiles of a tail, the ranges' sums in range order: workgroup (XCD and
-// tile of it, column block j of every wave).
+// tile of it, column block j of every wave).  32 us for 64 tiles in four ranges (67 MB of sums
+// written and read).
 template <int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64) void op_tail_fold_kernel(OpGemmArgs g) {
     constexpr int NT = WM * WN * 64, MI = BM / WM / 16, NJ = BN / WN / 16;
