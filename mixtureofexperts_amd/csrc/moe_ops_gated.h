@@ -125,21 +125,29 @@ __device__ __forceinline__ void stream_gated_rows(const OpGemmArgs &g, int e, in
     __syncthreads();
 }
 
-// Bound by reading both weights: 32 rows on 8 bf16 experts of 4096 / 14336 (1.88 GB) 320 us,
-// 5.8 TB/s.
-template <int OT>
-__global__ __launch_bounds__(kStreamWaves * 64) void op_gated_stream_kernel(OpGemmArgs g) {
-    __shared__ __attribute__((aligned(16))) uint8_t red_[kStreamWaves * 4 * 2 * 64 * 16];
+// MOST rows at a time.  Bound by reading both weights: 32 rows on 8 bf16 experts of 4096 /
+// 14336 (1.88 GB) 281 to 370 us by where the two weights lie (12 placements; at most of them
+// 326 to 343, 5.6 TB/s; each workgroup starting at another k: 358 to 377).  64 rows take the
+// registers of three workgroups per CU.  32 rows leave room for five, which fp32 rows of up to
+// 4 KB gain by, having few loads each: 64 / 32, us, 8 experts of 512 / 2048, 2 rows each 16.0 /
+// 13.2, 16 17.3 / 14.8, 64 rows on one and 9 on the others 17.7 / 19.9; 64 of 512 / 1408 82 / 72; 8 of
+// 1024 / 4096, 8 rows 60.0 / 59.1.  Longer rows lose: 8 of 2048 / 4096, 16 rows 113 / 115, uneven
+// ones 122 / 131; bf16 with four workgroups per CU, 8 of 2048 / 14336, 1 row 186 / 201, 128 of
+// 2048 / 768 161 / 175.
+template <int OT, int MOST>
+__global__ __launch_bounds__(kStreamWaves * 64) __attribute__((amdgpu_waves_per_eu(MOST == 32 ? 5 : 1))) void
+op_gated_stream_kernel(OpGemmArgs g) {
+    __shared__ __attribute__((aligned(16))) uint8_t red_[kStreamWaves * (MOST / 16) * 2 * 64 * 16];
     lds_u8 *red = (lds_u8 *)red_;
     const int r = blockIdx.x / g.nt, n0 = (blockIdx.x - r * g.nt) * 16;
     int e, lo, hi;
     held_group(g, r, e, lo, hi);
     if (e < 0) return;
     while (lo < hi) {
-        const int rows = min(hi - lo, 64);
+        const int rows = min(hi - lo, MOST);
         if (rows <= 16) stream_gated_rows<OT, 1>(g, e, n0, lo, rows, blockIdx.y, red);
         else if (rows <= 32) stream_gated_rows<OT, 2>(g, e, n0, lo, rows, blockIdx.y, red);
-        else stream_gated_rows<OT, 4>(g, e, n0, lo, rows, blockIdx.y, red);
+        else stream_gated_rows<OT, MOST / 16>(g, e, n0, lo, rows, blockIdx.y, red);
         lo += rows;
     }
 }
@@ -245,8 +253,9 @@ static hipError_t launch_gated_stream(int ot, OpGemmArgs g, hipStream_t s) {
     const long long grid = (long long)(g.E < g.rows ? g.E : g.rows) * g.nt;  // the groups that can hold rows
     if (grid * g.splits > 0x7fffffffll / (ops::kStreamWaves * 64)) return kOpTooLarge;
     const dim3 gr((unsigned)grid, g.splits), b(ops::kStreamWaves * 64);
-    if (ot == OT_F32) ops::op_gated_stream_kernel<OT_F32><<<gr, b, 0, s>>>(g);
-    else ops::op_gated_stream_kernel<OT_BF16><<<gr, b, 0, s>>>(g);
+    if (ot != OT_F32) ops::op_gated_stream_kernel<OT_BF16, 64><<<gr, b, 0, s>>>(g);
+    else if (g.K <= 1024) ops::op_gated_stream_kernel<OT_F32, 32><<<gr, b, 0, s>>>(g);
+    else ops::op_gated_stream_kernel<OT_F32, 64><<<gr, b, 0, s>>>(g);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess && g.splits > 1 ? launch_op_gate_fold(OM_GATED, ot, g, s) : e;
 }

@@ -184,6 +184,20 @@ def test_gradients(moe, dtype, layout, pad):
         _untouched([whole], K, M)
 
 
+@pytest.mark.parametrize("dtype,K,most", [("f32", 200, 32), ("f32", 1024, 32), ("f32", 1032, 64), ("bf16", 200, 64)])
+def test_few_rows_in_uneven_groups(moe, dtype, K, most):
+    """Streamed, by the average of rows: the groups of more are taken in parts."""
+    lens, H, tail = [70, 1, 0, 33, 0, 0, 16] + [0] * 9, 72, 3
+    rng = np.random.default_rng(K)
+    x = _rows(rng, sum(lens), K, dtype, 8, tail)
+    w1, w3 = _mats(rng, len(lens), H, K, dtype, LLAMA, 8), _mats(rng, len(lens), H, K, dtype, LLAMA)
+    res, off = [], _offsets(lens)
+    names = kernels_of(lambda: res.append(moe.gated_matmul(x, w1, w3, off, save=True)))
+    assert names["op_gated_stream_kernel"][1] == str(most)
+    _check_forward(lens, "silu", [_f64(t) for t in res[0]], x, w1, w3, LLAMA, K, dtype, dtype)
+    assert not any(t[sum(lens):].any() for t in res[0])
+
+
 def _tile(names, mode):
     """Rows of the tiles and alignment of the loads of the call's gated kernel."""
     a = names["op_gated_kernel"]
