@@ -528,8 +528,9 @@ int moe_quantize_fp8_async(const void *x, int64_t ldx, int64_t x_stride, int32_t
 /* y[r][n] = sum over k of (q[r][k] x_scale[r][k / 128]) (w[e][n][k] w_scale[e][n / 128][k / 128])
  * for the rows r of group e: the codes' products of a block summed in fp32, times
  * both scales, the blocks summed in fp32 (few rows, or scales whose products leave
- * fp32's normal range: in fp64).  On the way to a MOE_BF16 result the matrix unit may
- * cut a product to 2^-13 of the largest of eight along k.  x_dtype MOE_FP8_E4M3: x holds the codes and x_scale
+ * fp32's normal range: in fp64).  On the way to a MOE_BF16 result of more than a few rows
+ * the matrix unit cuts each product to a multiple of 2^-13 of the largest of eight along k: a
+ * sum is off by less than 7 * 2^-13 of its magnitudes.  x_dtype MOE_FP8_E4M3: x holds the codes and x_scale
  * [rows][ceil(in_dim / 128)] their scales, dense.  MOE_BF16 or MOE_F32: the rows are
  * quantised as moe_quantize_fp8_async does with block_rows 1, into the workspace, and
  * x_scale is not read.  w: codes [groups][out_dim][in_dim], w_scale
@@ -543,6 +544,13 @@ int moe_fp8_matmul_async(const void *x, int64_t ldx, int32_t x_dtype, const floa
                          int64_t w_stride, const float *w_scale, const int32_t *offsets, int32_t groups, int32_t rows,
                          int32_t in_dim, int32_t out_dim, void *y, int64_t ldy, int32_t y_dtype, void *workspace,
                          int64_t workspace_bytes, void *stream);
+/* The same with exact products whatever y_dtype and the number of rows: a MOE_BF16 result
+ * is the MOE_F32 one rounded once.  At the bf16 matrix rate, half that of the 8-bit
+ * instructions. */
+int moe_fp8_matmul_exact_async(const void *x, int64_t ldx, int32_t x_dtype, const float *x_scale, const void *w,
+                               int64_t ldw, int64_t w_stride, const float *w_scale, const int32_t *offsets, int32_t groups,
+                               int32_t rows, int32_t in_dim, int32_t out_dim, void *y, int64_t ldy, int32_t y_dtype,
+                               void *workspace, int64_t workspace_bytes, void *stream);
 
 /* The norms before and after a block, its gate and the residual, in one pass:
  *   z = y .* rstd(y) .* post_weight     (post_weight NULL: z = y)

@@ -47,6 +47,7 @@ EXPORTED_SYMBOLS = [
     "moe_gated_matmul_grad_workspace", "moe_gated_matmul_grad_async", "moe_gated_matmul_grad_x_workspace",
     "moe_gated_matmul_grad_x_async", "moe_quantize_int8_async", "moe_int8_matmul_async",
     "moe_int8_matmul_workspace", "moe_quantize_fp8_async", "moe_fp8_matmul_workspace", "moe_fp8_matmul_async",
+    "moe_fp8_matmul_exact_async",
     "moe_block_norm_async", "moe_block_norm_grad_async", "moe_block_norm_grad_workspace",
 ]
 
@@ -181,6 +182,7 @@ def lib():
     L.moe_quantize_fp8_async.argtypes = [vp, i64, i64, i32, i64, i64, i32, i32, vp, i64, i64, vp, vp]
     L.moe_fp8_matmul_workspace.argtypes = L.moe_int8_matmul_workspace.argtypes
     L.moe_fp8_matmul_async.argtypes = L.moe_int8_matmul_async.argtypes
+    L.moe_fp8_matmul_exact_async.argtypes = L.moe_int8_matmul_async.argtypes
     L.moe_block_norm_async.argtypes = [vp, i32, vp, i32, vp, vp, i32, vp, i32, i64, f32, f32, f32, i64, i32, vp, vp,
                                        i32, vp, vp]
     L.moe_block_norm_grad_workspace.argtypes = [i64, i32, i64, i64p]

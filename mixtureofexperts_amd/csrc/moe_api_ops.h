@@ -563,11 +563,10 @@ int moe_fp8_matmul_workspace(int32_t groups, int32_t rows, int32_t in_dim, int32
     return MOE_OK;
 }
 
-int moe_fp8_matmul_async(const void *x, int64_t ldx, int32_t x_dtype, const float *x_scale, const void *w, int64_t ldw,
-                         int64_t w_stride, const float *w_scale, const int32_t *offsets, int32_t groups, int32_t rows,
-                         int32_t in_dim, int32_t out_dim, void *y, int64_t ldy, int32_t y_dtype, void *workspace,
-                         int64_t workspace_bytes, void *stream) {
-    const char *fn = "moe_fp8_matmul_async";
+static int fp8_matmul(const char *fn, bool exact, const void *x, int64_t ldx, int32_t x_dtype, const float *x_scale,
+                      const void *w, int64_t ldw, int64_t w_stride, const float *w_scale, const int32_t *offsets,
+                      int32_t groups, int32_t rows, int32_t in_dim, int32_t out_dim, void *y, int64_t ldy, int32_t y_dtype,
+                      void *workspace, int64_t workspace_bytes, void *stream) {
     int r = op_check_groups(fn, offsets, groups, rows, in_dim, out_dim);
     if (r != MOE_OK) return r;
     const bool codes = x_dtype == MOE_FP8_E4M3;
@@ -611,8 +610,24 @@ int moe_fp8_matmul_async(const void *x, int64_t ldx, int32_t x_dtype, const floa
     g.N = out_dim, g.K = in_dim, g.c_f32 = y_dtype == MOE_F32;
     g.splits = op_f8_splits(rows, groups, out_dim, in_dim, op_cus());
     g.ws = (float *)workspace;
-    g.sa = x_scale, g.sb = w_scale, g.kb = (int)kb;
+    g.sa = x_scale, g.sb = w_scale, g.kb = (int)kb, g.exact = exact;
     return op_done(fn, launch_op_gemm_f8(g, op_cus(), (hipStream_t)stream));
+}
+
+int moe_fp8_matmul_async(const void *x, int64_t ldx, int32_t x_dtype, const float *x_scale, const void *w, int64_t ldw,
+                         int64_t w_stride, const float *w_scale, const int32_t *offsets, int32_t groups, int32_t rows,
+                         int32_t in_dim, int32_t out_dim, void *y, int64_t ldy, int32_t y_dtype, void *workspace,
+                         int64_t workspace_bytes, void *stream) {
+    return fp8_matmul("moe_fp8_matmul_async", false, x, ldx, x_dtype, x_scale, w, ldw, w_stride, w_scale, offsets, groups,
+                      rows, in_dim, out_dim, y, ldy, y_dtype, workspace, workspace_bytes, stream);
+}
+
+int moe_fp8_matmul_exact_async(const void *x, int64_t ldx, int32_t x_dtype, const float *x_scale, const void *w,
+                               int64_t ldw, int64_t w_stride, const float *w_scale, const int32_t *offsets, int32_t groups,
+                               int32_t rows, int32_t in_dim, int32_t out_dim, void *y, int64_t ldy, int32_t y_dtype,
+                               void *workspace, int64_t workspace_bytes, void *stream) {
+    return fp8_matmul("moe_fp8_matmul_exact_async", true, x, ldx, x_dtype, x_scale, w, ldw, w_stride, w_scale, offsets,
+                      groups, rows, in_dim, out_dim, y, ldy, y_dtype, workspace, workspace_bytes, stream);
 }
 
 static int op_check_norm(const char *fn, int64_t T, int32_t D, int32_t x_dtype, int32_t y_dtype, int32_t h_dtype,

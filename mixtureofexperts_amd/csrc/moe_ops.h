@@ -32,6 +32,7 @@ struct OpGemmArgs {
     const float *sa;               // int8: scale per row of A; e4m3: [rows][kb]
     const float *sb;               // int8: scale per group and column [E][N]; e4m3: [E][ceil(N / 128)][kb]
     int kb;                        // e4m3: blocks of 128 along K
+    int exact;                     // e4m3: exact products, whatever the result's type
     float *ws;                     // partial sums (splits > 1), [range][rows][N] or [group][range][M][N]
     int splits;                    // ranges that k is split into over workgroups (1: none)
     int nt, mt;                    // tiles along N, and (ragged k) along M

@@ -515,17 +515,20 @@ def quantize_fp8(x, *, block_rows=1):
     return q, scale
 
 
-def fp8_matmul(x, w, w_scale, offsets=None, *, x_scale=None, out=None, out_dtype=None):
+def fp8_matmul(x, w, w_scale, offsets=None, *, x_scale=None, out=None, out_dtype=None, exact=False):
     """y[r][n] = sum_k (q[r][k] x_scale[r][k / 128]) (w[e][n][k] w_scale[e][n / 128][k / 128])
     for the rows r of expert e.  x (M, in): float8_e4m3fn codes with ``x_scale`` (M,
     ceil(in / 128)), or float32 / bfloat16 rows, which are quantised as quantize_fp8 does;
     w (E, out, in) float8_e4m3fn and w_scale from quantize_fp8(w, block_rows=128).  A
-    block's products are summed in float32, scaled, and summed in float32; on the way to a
-    bfloat16 result the matrix unit may cut a product to 2^-13 of the largest of eight.  The
-    result is bfloat16 or, with ``out_dtype``, float32; without ``out`` rows outside every group are
-    zeros.  The gradient with respect to x is the same call on dy with the transposed codes
-    and scales (w.transpose(1, 2).contiguous()): a matrix' 128 x 128 blocks are those of its
-    transpose."""
+    block's products are summed in float32, scaled, and summed in float32.  The result is
+    bfloat16 or, with ``out_dtype``, float32.  On the way to a bfloat16 result of more than a
+    few rows the matrix unit's 8-bit instruction cuts a product to a multiple of 2^-13 of the
+    largest of eight (a sum of N(0, 1) codes is off by 1.4e-5 of itself, any sum by less than
+    7 * 2^-13 of its magnitudes); with ``exact`` the products are exact whatever the rows, and
+    a bfloat16 result is the float32 one rounded, at half the matrix rate.  Without ``out``
+    rows outside every group are zeros.  The gradient with respect to x is the same call on
+    dy with the transposed codes and scales (w.transpose(1, 2).contiguous()): a matrix' 128 x
+    128 blocks are those of its transpose."""
     torch = _t()
     _plain("x w w_scale x_scale out", x, w, w_scale, x_scale, out)
     L, f8 = _lib.lib(), torch.float8_e4m3fn
@@ -550,7 +553,7 @@ def fp8_matmul(x, w, w_scale, offsets=None, *, x_scale=None, out=None, out_dtype
     out = _result(out, (M, n), out_dtype, (torch.bfloat16, torch.float32), x, offsets is not None)
     device = _same_device(x, w, w_scale, x_scale, offsets, out)
     ws, wsp, wsn = _workspace(L.moe_fp8_matmul_workspace, device, E, M, k, n, _codes[x.dtype])
-    _call(L.moe_fp8_matmul_async, device, xp, ldx, _codes[x.dtype], x_scale.data_ptr() if codes else None, w.data_ptr(), ldw,
+    _call(L.moe_fp8_matmul_exact_async if exact else L.moe_fp8_matmul_async, device, xp, ldx, _codes[x.dtype], x_scale.data_ptr() if codes else None, w.data_ptr(), ldw,
           stride, w_scale.data_ptr(), _offsets(offsets, E), E, M, k, n, out.data_ptr(), _row_stride(out, "out"),
           _codes[out.dtype], wsp, wsn)
     if given is not None:
