@@ -527,8 +527,9 @@ int moe_quantize_fp8_async(const void *x, int64_t ldx, int64_t x_stride, int32_t
                            void *stream);
 /* y[r][n] = sum over k of (q[r][k] x_scale[r][k / 128]) (w[e][n][k] w_scale[e][n / 128][k / 128])
  * for the rows r of group e: the codes' products of a block summed in fp32, times
- * both scales, the blocks summed in fp32 (few rows, or scales whose products leave
- * fp32's normal range: in fp64).  On the way to a MOE_BF16 result of more than a few rows
+ * both scales, the blocks summed in fp32 (few rows, and rows that have a product of two
+ * scales above 2^31 or only ones below 2^-126: in fp64; parts of a split k are added in
+ * fp32).  On the way to a MOE_BF16 result of more than a few rows
  * the matrix unit cuts each product to a multiple of 2^-13 of the largest of eight along k: a
  * sum is off by less than 7 * 2^-13 of its magnitudes.  x_dtype MOE_FP8_E4M3: x holds the codes and x_scale
  * [rows][ceil(in_dim / 128)] their scales, dense.  MOE_BF16 or MOE_F32: the rows are

@@ -381,23 +381,29 @@ __global__ __launch_bounds__(kStreamWaves * 64) void op_f8_stream_kernel(OpGemmA
     }
 }
 
-// The largest and the smallest non-zero magnitude of the scales that a lane multiplies
-// with: products of two of them have to be normal fp32 numbers.
+// Tiles sum in units of 2^-48.  A product of two scales is then a normal number from 2^-174 on,
+// and a smaller one's rounding, 2^-150 in these units, changes a sum of 2^23 blocks (each below
+// 128 * 448^2 < 2^25) by less than 2^-149, fp32's last place.  Up to 2^31 no such sum
+// overflows, so that an infinity in one is the result's own.
+constexpr float kF8Unit = 0x1p48f, kF8Most = 0x1p79f, kF8Normal = 0x1p-78f;  // 2^31, 2^-126 in it
+// The largest and the smallest non-zero product (in magnitude) that a lane multiplies with.
 struct F8Range {
-    unsigned most = 0, least = ~0u;  // bits; bits of twice the magnitude less one (0: ~0)
-    __device__ __forceinline__ void take(float s) {
-        const unsigned u = __float_as_uint(s);
+    unsigned most = 0, least = ~0u;  // bits; twice the bits less one (0: ~0)
+    __device__ __forceinline__ void take(float f) {
+        const unsigned u = __float_as_uint(f);
         most = max(most, u & 0x7fffffffu);
         least = min(least, (u << 1) - 1u);
     }
-    // exponents (subnormal: -127)
-    __device__ __forceinline__ int hi() const { return (int)(most >> 23) - 127; }
-    __device__ __forceinline__ int lo() const { return (int)((least + 1u) >> 24) - 127; }
-    static __device__ __forceinline__ bool far(const F8Range &x, const F8Range &w) {
-        if (x.least == ~0u || w.least == ~0u) return false;  // all products are zero
-        return x.hi() + w.hi() > 125 || x.lo() + w.lo() < -125;
+    // some row may have to be summed in fp64 (far_row)
+    __device__ __forceinline__ bool far() const {
+        return most > __float_as_uint(kF8Most) || least < 2u * __float_as_uint(kF8Normal) - 1u;
     }
 };
+// Rows that are: one product too large (or no number), or all below fp32's normal range, whose
+// results would be rounded twice.  most: the bits of the row's largest.
+__device__ __forceinline__ bool f8_far_row(unsigned most) {
+    return most > __float_as_uint(kF8Most) || (most > 0u && most < __float_as_uint(kF8Normal));
+}
 
 // The tile loop: as op_gemm_tile, a stage one block of k, the wave's columns taken one
 // 16-column block at a time.  Step j of a stage:
@@ -482,17 +488,17 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
         return f;
     };
     typedef __attribute__((address_space(3))) float lds_f32;
-    F8Range rx, rw;
+    F8Range range;
     auto read_scales = [&](auto SLOT, float (&f)[MI]) {
         // one for all columns of the wave
         const float sw = __uint_as_float(__builtin_amdgcn_readfirstlane(
             *(const __attribute__((address_space(3))) unsigned *)(uintptr_t)(w_at + decltype(SLOT)::value * NT * 4)));
-        rw.take(sw);
+        const float unit = sw * kF8Unit;
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
             const float sx = *(const lds_f32 *)(uintptr_t)(x_at + decltype(SLOT)::value * NT * 4 + i * WM * 64);
-            rx.take(sx);
-            f[i] = sx * sw;
+            f[i] = sx * unit;
+            range.take(f[i]);
         }
     };
     f32x4 acc[MI][NJ];
@@ -664,10 +670,11 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
             scaled(num<MI>{}, NJ - 1, part[1], f[1]);
         }
     }
-    typedef __attribute__((address_space(3))) int lds_int;
-    lds_int *flags = (lds_int *)(ring + SCALES + NS * NT * 4);
-    if (lane == 0) flags[w] = 0;
-    if (F8Range::far(rx, rw)) flags[w] = 1;
+    const bool far = __any(range.far());
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] *= 1.0f / kF8Unit;
     bool split = false;
     if constexpr (BM <= 64) split = g.splits > 1;  // (split calls run the smallest tiles)
     if (split) {
@@ -688,27 +695,36 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
         if (g.c_f32) store_tile_rows<4, BM, BN, WM, WN, RING, false>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
         else store_tile_rows<2, BM, BN, WM, WN, RING, false>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
     }
-    // Scales whose products leave fp32's normal range: the tile's results again, in fp64,
-    // over those just stored (every wave's stores are done at the barrier).
+    // Far rows' results again, in fp64, over those just stored (every wave's stores are done
+    // at the barrier).  A row's depend on its own scales alone.  8192 rows of 4096 / 14336 with
+    // one such row 970 us, 620 without; with one block's scale of 1e-36, where the row or the
+    // weight has ordinary ones too and this only looks, 620 and 680.
     wait_loads<0>();
     lds_barrier();
-    int far = 0;
-#pragma unroll
-    for (int i = 0; i < WM * WN; ++i) far |= flags[i];
-    if (__builtin_amdgcn_readfirstlane(far) == 0) return;
+    if (!far) return;
     // (opaque: addresses formed from them before the loop would be kept through it)
     int e = jb.e, row0 = jb.lo + jb.m0;
     asm("" : "+s"(e), "+s"(row0));
+    const int nw = jb.n0 + wn * (BN / WN);
+    if (nw >= g.N) return;
+    const float *sb = g.sb + ((long long)e * ((g.N + 127) >> 7) + (nw >> 7)) * g.kb + (k0 >> 7);
     for (int i = 0; i < MI; ++i) {
         const int r0 = (i * WM + wm) * 16;
         if (r0 >= mrows) continue;
+        const float *sa = g.sa + (long long)(row0 + min(r0 + r16, mrows - 1)) * g.kb + (k0 >> 7);
+        unsigned most = 0;
+        for (int s = q4; s < S; s += 4) most = max(most, __float_as_uint(sa[s] * (sb[s] * kF8Unit)) & 0x7fffffffu);
+        most = max(most, (unsigned)__shfl_xor((int)most, 16));
+        most = max(most, (unsigned)__shfl_xor((int)most, 32));
+        const bool again = f8_far_row(most);
+        if (!__any(again)) continue;
         for (int j = 0; j < NJ; ++j) {
-            const int n0 = jb.n0 + (wn * NJ + j) * 16;
+            const int n0 = nw + j * 16;
             if (n0 >= g.N) continue;
             double d[4];
             f8_direct(g, e, n0, row0 + r0, min(16, mrows - r0), k0, klen, 0, 1, d);
             const int n = n0 + 4 * q4;
-            if (r0 + r16 < mrows && n < g.N) {
+            if (again && r0 + r16 < mrows && n < g.N) {
                 const float v[4] = {(float)d[0], (float)d[1], (float)d[2], (float)d[3]};
                 f8_put4(g, row0 + r0 + r16, n, jb.ks, v);
             }
@@ -718,7 +734,7 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
 
 template <int BM, int BN, int WM, int WN, int NS, int WPE, int VB, bool WIDE>
 __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void op_f8_kernel(OpGemmArgs g) {
-    __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * ((BM + BN) * 128 + WM * WN * 64 * 4) + WM * WN * 4];
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * ((BM + BN) * 128 + WM * WN * 64 * 4)];
     f8_gemm_tile<BM, BN, WM, WN, NS, VB, WIDE>(g, ring);
 }
 
