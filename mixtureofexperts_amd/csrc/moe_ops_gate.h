@@ -43,7 +43,10 @@ struct Gate {
             // they could overflow (and 0 times infinity would be NaN)
             const float q = __builtin_amdgcn_fmed3f(a, -32.0f, 32.0f), q2 = q * q;
             const float s = gate_sigmoid<FAST>(r * (a + c * q2 * q)), f = a * s;
-            return {f, s + fminf(f, 3e38f) * (1.0f - s) * (r * (1.0f + 3.0f * c * q2))};
+            // (an infinite f, where 1 - s is 0, is kept from being NaN; a NaN, at a = -infinity
+            // too, stays one, which fminf would not let it)
+            const float most = f > 3e38f ? 3e38f : f;
+            return {f, s + most * (1.0f - s) * (r * (1.0f + 3.0f * c * q2))};
         } else {
             const bool zero = a <= floor;
             return {zero ? 0.0f : a, zero ? 0.0f : 1.0f};
