@@ -17,8 +17,11 @@
 namespace moe {
 namespace ops {
 
-// FAST: the hardware's exp and reciprocal, 2^-22 of the result each, where a, b and
-// dh come from bf16 operands; else expf and an IEEE division.
+// FAST: the hardware's exp and reciprocal, for results that are rounded to bf16.  e^-z is
+// 2^(-z log2 e) there, whose rounded exponent costs some 2^-24 |z| of it: act is off by up to
+// 57 * 2^-24 of itself for |z| up to 80 (2.6 * 2^-24 otherwise), a 1000th of a bf16 half step.
+// Else expf and an IEEE division: the forward product of 8192 rows, one bf16 expert of 4096 /
+// 14336, fp32 result, 1580 us, 1530 with the hardware's.
 template <bool FAST>
 __device__ __forceinline__ float gate_sigmoid(float z) {
     if constexpr (FAST) return __builtin_amdgcn_rcpf(1.0f + __expf(-z));
@@ -53,6 +56,19 @@ struct Gate {
         }
     }
 };
+
+// f(SMOOTH, FAST) of the gate's form; f32: results that stay in 32 bits.
+template <bool BF16, typename F>
+__device__ __forceinline__ void gate_form(const Gate &gate, bool f32, F f) {
+    if (!gate.smooth) {
+        f(std::false_type{}, std::false_type{});
+    } else if constexpr (BF16) {
+        if (f32) f(std::true_type{}, std::false_type{});
+        else f(std::true_type{}, std::true_type{});
+    } else {
+        f(std::true_type{}, std::false_type{});
+    }
+}
 
 struct GateBack {
     float da, db, h;
@@ -151,15 +167,13 @@ __device__ __forceinline__ void gate_store(const OpGemmArgs &g, long long row, i
     const GateChunk<BF16> a(ra), b(rb);
     GateChunk<BF16> da, db, h;
     const Gate gate(g.act);
-    auto all = [&](auto SMOOTH) {
+    gate_form<BF16>(gate, !BF16, [&](auto SMOOTH, auto FAST) {
 #pragma unroll
         for (int q = 0; q < GateChunk<BF16>::CE; ++q) {
-            const GateBack r = gate_back<decltype(SMOOTH)::value, BF16>(gate, dh.v[q], a.v[q], b.v[q]);
+            const GateBack r = gate_back<decltype(SMOOTH)::value, decltype(FAST)::value>(gate, dh.v[q], a.v[q], b.v[q]);
             da.v[q] = r.da, db.v[q] = r.db, h.v[q] = r.h;
         }
-    };
-    if (gate.smooth) all(std::true_type{});
-    else all(std::false_type{});
+    });
     da.template store<PAST>((uint8_t *)g.C + row * g.ldc * ES, n, g.N);
     db.template store<PAST>((uint8_t *)g.C2 + row * g.ldc2 * ES, n, g.N);
     h.template store<PAST>((uint8_t *)g.C3 + row * g.ldc3 * ES, n, g.N);

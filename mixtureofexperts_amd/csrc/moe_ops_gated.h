@@ -13,12 +13,10 @@ template <bool BF16>
 __device__ __forceinline__ void gated_put4(const OpGemmArgs &g, long long row, int n, const float *a, const float *b) {
     float f[4];
     const Gate gate(g.act);
-    auto all = [&](auto SMOOTH) {
+    gate_form<BF16>(gate, g.c_f32, [&](auto SMOOTH, auto FAST) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) f[c] = gate.value<decltype(SMOOTH)::value, BF16>(a[c]).f * b[c];
-    };
-    if (gate.smooth) all(std::true_type{});
-    else all(std::false_type{});
+        for (int c = 0; c < 4; ++c) f[c] = gate.value<decltype(SMOOTH)::value, decltype(FAST)::value>(a[c]).f * b[c];
+    });
     put4(g, row * g.ldc + n, n, f[0], f[1], f[2], f[3], vec_ok(g));
     if (g.C2) {
         OpGemmArgs t = g;

@@ -1093,17 +1093,15 @@ __device__ __forceinline__ void op_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
                                                              wn, lane, [&](int i, int j, int c) { return acc[i][JH + j][c]; });
         }
         const Gate gate(g.act);
-        auto all = [&](auto SMOOTH) {
+        gate_form<OT == OT_BF16>(gate, g.c_f32, [&](auto SMOOTH, auto FAST) {
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
                 for (int j = 0; j < JH; ++j)
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
-                        acc[i][j][c] = gate.value<decltype(SMOOTH)::value, OT == OT_BF16>(acc[i][j][c]).f * acc[i][JH + j][c];
-        };
-        if (gate.smooth) all(std::true_type{});
-        else all(std::false_type{});
+                        acc[i][j][c] = gate.value<decltype(SMOOTH)::value, decltype(FAST)::value>(acc[i][j][c]).f * acc[i][JH + j][c];
+        });
         auto val = [&](int i, int j, int c) -> float { return acc[i][j][c]; };
         if (g.c_f32) store_tile_rows<4, BM, BR, WM, WN, RING, false>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
         else store_tile_rows<2, BM, BR, WM, WN, RING, false>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
