@@ -676,7 +676,7 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
 #pragma unroll
         for (int j = 0; j < NJ; ++j) acc[i][j] *= 1.0f / kF8Unit;
     bool split = false;
-    if constexpr (BM <= 64) split = g.splits > 1;  // (split calls run the smallest tiles)
+    if constexpr (WIDE && BM <= 64) split = g.splits > 1;  // (split calls run the smallest tiles, widened)
     if (split) {
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
@@ -692,7 +692,9 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
     } else {
         const long long at0 = (long long)(jb.lo + jb.m0) * g.ldc;
         auto val = [&](int i, int j, int c) -> float { return acc[i][j][c]; };
-        if (g.c_f32) store_tile_rows<4, BM, BN, WM, WN, RING, false>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
+        bool f32 = false;
+        if constexpr (WIDE) f32 = g.c_f32;  // (fp32 results are of widened codes)
+        if (f32) store_tile_rows<4, BM, BN, WM, WN, RING, false>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
         else store_tile_rows<2, BM, BN, WM, WN, RING, false>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
     }
     // Far rows' results again, in fp64, over those just stored (every wave's stores are done
