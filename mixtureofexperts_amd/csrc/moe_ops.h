@@ -167,7 +167,10 @@ inline int op_gated_splits(OpMode mode, int ot, bool b_col, long long rows, long
 // 266 / 247 / 369, 101 / 60 / 75, 101 / 75 / 82; row gradient of 4096 rows on 8 of 2048 / 4096
 // 209 / 247 / 300.  8-bit, bf16 result (170 / 100 / 60): 24576 rows 109 / 119 / 192, 4096 rows on 8 of
 // 2048 / 4096 64 / 54 / 79, 3102 rows on 64 of 1408 / 2048 48 / 39 / 45; fp32 result (- / 100 / 50): 2048
-// rows on 8 of 4096 / 2048 - / 62 / 58, 4096 rows - / 83 / 103.
+// rows on 8 of 4096 / 2048 - / 62 / 58, 4096 rows - / 83 / 103.  One cost for a form's three products
+// and whole rounds are coarse: of these it takes the slower tile, by 7 to 9 %, for the 24576 rows
+// through the down product (256) and in 8 bits (128), the 512 rows through it (64), and the 2048
+// rows with an fp32 result (128).
 struct OpTileCost {
     int c256, c128, c64;  // 0: none of these
 };
@@ -209,7 +212,9 @@ inline bool op_two_tail(int ot, long long rows, long long E, long long N, long l
 // 8-bit products of few rows: streamed where 64 x 64 tiles are fewer than CUs, or of long rows.
 // Streamed / tiles, us: 8 experts of 4096 / 14336, a row on two of them 30.5 / 32.7, 1 row each 101 /
 // 109, 4 104 / 110, 8 113 / 110; of 2048 / 4096, 1 row 14.5 / 17.0, 4 15.8 / 16.8, 8 17.6 / 16.9; 64 of
-// 1408 / 2048 48 / 44.
+// 1408 / 2048 48 / 44.  A group's rows are one workgroup's, 16 at a time, and its weights are read
+// again for each 16: 128 experts of 2048 / 2048, 4 rows each 124 us, the same 512 rows by Zipf 107
+// to 117, all on one 95; 64 of 1408 / 2048, 4 rows each 34, 64 rows on one and 3 on the others 34.
 inline bool op_f8_streamed(long long rows, long long E, long long N, long long K, int ncu) {
     const long long held = E < rows ? E : rows;
     const bool few = held * ((N + 63) / 64) < ncu;

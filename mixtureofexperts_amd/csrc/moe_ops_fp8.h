@@ -12,7 +12,7 @@
 // sums of N(0, 1) codes by 1.4e-5 of themselves, of codes of all magnitudes by 5e-5, a
 // hundredth of a bf16 result's rounding.  The instruction is twice as fast (4040 TFLOP/s in a
 // loop, 16x16x32_bf16 1960), so tiles with bf16 results take it unless the caller asks for
-// exact products (8192 rows, 8 even groups of 4096 / 14336, 623 and 1128 us at one clock).
+// exact products (codes of 8192 rows, 8 even groups of 4096 / 14336: 490 and 870 us).
 // Those, fp32 results, split sums, and few rows, where the weights' bytes bind, have the codes
 // widened to bf16, which is exact, and products that are exact and summed in fp32 (1e-8 and
 // 8e-8).
@@ -414,10 +414,12 @@ __device__ __forceinline__ bool f8_far_row(unsigned most) {
 // so that the vector unit's part runs under the next MFMAs.  The scales of a stage, one
 // for each row and column of the tile, come into the ring with it.
 // WIDE: the codes in bf16.
-// Bound by the matrix units at the clock that their load leaves, and by the scaling: 8192 rows,
-// 8 even groups of 4096 / 14336, 256 x 256 tiles, 481 us (2.0 PFLOP/s, units 46 % busy; the
-// scaling after the products instead of under them 553), skewed groups 500 to 518.  fp32 result,
-// 128 x 128 tiles: 900 to 955 us (units 47 % busy).
+// 8192 rows, 8 even groups of 4096 / 14336, codes given, 256 x 256 tiles: 481 to 499 us (2.0
+// PFLOP/s; the scaling after the products instead of under them 553); skewed groups 526 to 550,
+// of whose cycles the matrix units are busy 42 % and other vector instructions, mostly the
+// scaling's four multiply-adds per product instruction, take 34 %: three quarters if neither ran
+// under the other; in 35 % of their time waves wait.  Widened, 128 x 128 tiles: bf16 870 and 930 us,
+// fp32 890 and 960.
 template <int BM, int BN, int WM, int WN, int NS, int VB, bool WIDE>
 __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_) {
     constexpr int NT = WM * WN * 64, KE = 128;
@@ -698,9 +700,10 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
         else store_tile_rows<2, BM, BN, WM, WN, RING, false>(g, ring, at0, mrows, jb.n0, wm, wn, lane, val);
     }
     // Far rows' results again, in fp64, over those just stored (every wave's stores are done
-    // at the barrier).  A row's depend on its own scales alone.  8192 rows of 4096 / 14336 with
-    // one such row 970 us, 620 without; with one block's scale of 1e-36, where the row or the
-    // weight has ordinary ones too and this only looks, 620 and 680.
+    // at the barrier).  A row's depend on its own scales alone.  8192 rows on 8 experts of 4096 /
+    // 14336, even and skewed groups: with one such row 1094 and 708 us, 490 and 545 without; with
+    // one block's scale of 1e-36 in a row or a weight of otherwise ordinary ones, where this only
+    // looks, 500 and 550.
     wait_loads<0>();
     lds_barrier();
     if (!far) return;

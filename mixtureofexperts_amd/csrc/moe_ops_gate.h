@@ -5,9 +5,8 @@
 //     gelu: r = 2 sqrt(2 / pi), c = 0.044715 (its tanh form: 0.5 (1 + tanh(z / 2)) = s);
 //     act' = s + a s (1 - s) r (1 + 3 c a^2)
 //   relu, identity: act = a, act' = 1 but where a <= floor: 0; floor = 0 or NaN
-// so that a kernel holds two forms, not four (a four-way choice by the activation
-// around a tile's results was compiled wrong: one register of 16 was left unset for
-// the identity).
+// so that a kernel holds two forms, not four.  (With a four-way choice by the activation
+// around a tile's results one value of 16 was wrong for the identity; why was not found out.)
 #pragma once
 #include <type_traits>
 

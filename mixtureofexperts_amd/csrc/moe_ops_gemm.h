@@ -1157,9 +1157,9 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WP
 // 14336, skewed groups (36 tiles of 256 rows where even ones have 32):
 //   forward with both pre-activations: 1780 us (1.08 PFLOP/s, units 55 % busy), its 705 MB of
 //     results after each tile's products with one workgroup per CU
-//   through the down product: 1030 us, of which the product alone is 840 (units 44 % busy): the
-//     tile's 1.2 GB of a, b and results are not under another tile's products (the gate as a
-//     launch of its own: 840 + 243)
+//   through the down product: 1025 to 1080 us, the product alone 840, the gate in a launch of its
+//     own 243 (units 43 % busy): one kernel saves the 235 MB of dh and its rounding, not time,
+//     since the tile's 1.2 GB of a, b and results are not under another tile's products
 //   row gradient: 1770 us (1.09 PFLOP/s, units 55 % busy), 2.25 rounds of tiles; the two products and their sum in
 //     one kernel, where two calls would read and write the 134 MB of fp32 sums in between
 // Wave priorities (s_setprio) and two stages per scheduling region changed none of them.
