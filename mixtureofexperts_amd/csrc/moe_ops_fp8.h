@@ -394,15 +394,16 @@ struct F8Range {
         most = max(most, u & 0x7fffffffu);
         least = min(least, (u << 1) - 1u);
     }
-    // some row may have to be summed in fp64 (far_row)
+    // some row may have to be summed in fp64 (f8_far_row)
     __device__ __forceinline__ bool far() const {
         return most > __float_as_uint(kF8Most) || least < 2u * __float_as_uint(kF8Normal) - 1u;
     }
 };
-// Rows that are: one product too large (or no number), or all below fp32's normal range, whose
-// results would be rounded twice.  most: the bits of the row's largest.
+// Rows that are: one product too large, or all below fp32's normal range, whose results would
+// be rounded twice.  (With a NaN among them the row's are NaN already.)  most: the bits of the
+// row's largest.
 __device__ __forceinline__ bool f8_far_row(unsigned most) {
-    return most > __float_as_uint(kF8Most) || (most > 0u && most < __float_as_uint(kF8Normal));
+    return (most > __float_as_uint(kF8Most) && most <= 0x7f800000u) || (most > 0u && most < __float_as_uint(kF8Normal));
 }
 
 // The tile loop: as op_gemm_tile, a stage one block of k, the wave's columns taken one
@@ -701,7 +702,8 @@ __device__ __forceinline__ void f8_gemm_tile(const OpGemmArgs &g, uint8_t *ring_
     }
     // Far rows' results again, in fp64, over those just stored (every wave's stores are done
     // at the barrier).  A row's depend on its own scales alone.  8192 rows on 8 experts of 4096 /
-    // 14336, even and skewed groups: with one such row 1094 and 708 us, 490 and 545 without; with
+    // 14336, even and skewed groups: with one such row 1094 and 708 us, 490 and 545 without (skewed
+    // ones on a slower box: one row 978, 101 rows 2500, all of them 9800, none 640); with
     // one block's scale of 1e-36 in a row or a weight of otherwise ordinary ones, where this only
     // looks, 500 and 550.
     wait_loads<0>();

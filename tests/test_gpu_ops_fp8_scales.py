@@ -117,3 +117,27 @@ def test_split_sums_that_fp32_holds(moe):
         xs, ws = torch.full((M, kb), a, device="cuda"), torch.full((1, 1, kb), b, device="cuda")
         y = _run(moe, x, xs, w, ws, None, "f32")
         assert (y.double() == K * a * b).all(), (a, b)
+
+
+@pytest.mark.parametrize("odt", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,K,N", SHAPES)
+def test_scales_that_are_no_numbers(moe, lens, K, N, odt):
+    # a NaN or an infinity, alone and beside a far one, leaves no finite number in its row and
+    # every other row as it was; one of a weight in its group's columns
+    rng = np.random.default_rng([K, N, 3])
+    x, xs, w, ws, off = _inputs(rng, lens, K, N)
+    x[2] = 0x38  # ones, so that no sum is 0
+    w[0, :, 128:256] = 0x30
+    want, M = _run(moe, x, xs, w, ws, off, odt), sum(lens)
+    others = torch.arange(M, device="cuda") != 2
+    for bad, beside in ((float("nan"), 0.01), (float("inf"), 0.01), (float("nan"), 2.0**90), (float("nan"), 1e-40)):
+        s = xs.clone()
+        s[2, 1], s[2, 0] = bad, beside
+        y = _run(moe, x, s, w, ws, off, odt)
+        assert torch.equal(y[others], want[others]) and not torch.isfinite(y[2]).any(), (bad, beside)
+        assert torch.isnan(y[2]).all() or bad == float("inf")
+    s = ws.clone()
+    s[0, 0, 1] = float("nan")
+    y = _run(moe, x, xs, w, s, off, odt)
+    assert torch.isnan(y[:lens[0], :128]).all()
+    assert torch.equal(y[:, 128:], want[:, 128:]) and torch.equal(y[lens[0]:], want[lens[0]:])
