@@ -553,9 +553,10 @@ def fp8_matmul(x, w, w_scale, offsets=None, *, x_scale=None, out=None, out_dtype
     out = _result(out, (M, n), out_dtype, (torch.bfloat16, torch.float32), x, offsets is not None)
     device = _same_device(x, w, w_scale, x_scale, offsets, out)
     ws, wsp, wsn = _workspace(L.moe_fp8_matmul_workspace, device, E, M, k, n, _codes[x.dtype])
-    _call(L.moe_fp8_matmul_exact_async if exact else L.moe_fp8_matmul_async, device, xp, ldx, _codes[x.dtype], x_scale.data_ptr() if codes else None, w.data_ptr(), ldw,
-          stride, w_scale.data_ptr(), _offsets(offsets, E), E, M, k, n, out.data_ptr(), _row_stride(out, "out"),
-          _codes[out.dtype], wsp, wsn)
+    fn = L.moe_fp8_matmul_exact_async if exact else L.moe_fp8_matmul_async
+    _call(fn, device, xp, ldx, _codes[x.dtype], x_scale.data_ptr() if codes else None, w.data_ptr(), ldw, stride,
+          w_scale.data_ptr(), _offsets(offsets, E), E, M, k, n, out.data_ptr(), _row_stride(out, "out"), _codes[out.dtype],
+          wsp, wsn)
     if given is not None:
         _written(out)  # autograd sees the caller's tensor change
     return out
